@@ -1,6 +1,7 @@
 /*
  * tpo.h -- C ABI of libtpo_hip.so, the MI355X (gfx950) kernels behind the
- * torch_point_ops operators chamfer / knn / fps / gather_points / emd.
+ * torch_point_ops operators chamfer / knn / fps / gather_points / emd and the
+ * transformer operators layer norm / packed attention / gated projection.
  *
  * Conventions for every entry point:
  *   - all pointers are device pointers (hipMalloc / torch CUDA-device tensors)
@@ -334,6 +335,100 @@ int tpo_emd_bwd(int dtype, const void* grad_cost, const void* xyz1,
                 const void* xyz2, const void* match, int64_t B, int64_t n,
                 int64_t m, void* grad_xyz1, void* grad_xyz2,
                 void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
+ * Transformer operators.  No counterpart in the reference: what a model over
+ * point patches runs between the grouping above and a loss on clouds.
+ * F32/F16/BF16; sums are taken in float and outputs rounded once.
+ *
+ * Layer norm over the last axis of x (rows, width):
+ *   y = (x - mean) rstd weight + bias, rstd = 1 / sqrt(var + eps), var the
+ *   mean square about the mean.
+ *   weight, bias (width) of `wdtype` (x's dtype or F32); NULL for 1 and 0.
+ *   mean, rstd (rows) float: what the backward needs; both NULL to leave out.
+ *   1 <= width <= 2^20, rows < 2^31.
+ * tpo_layer_norm_bwd: grad_x (rows, width) of `dtype`, grad_weight and
+ *   grad_bias (width) of `wdtype`; each may be NULL and is then left out.
+ *   The sums over rows run in a fixed order.  The workspace is needed where
+ *   grad_weight or grad_bias is asked for.
+ */
+int tpo_layer_norm_fwd(int dtype, int wdtype, const void* x, const void* weight,
+                       const void* bias, int64_t rows, int64_t width, double eps,
+                       void* y, float* mean, float* rstd, void* stream);
+int64_t tpo_layer_norm_bwd_workspace_size(int64_t rows, int64_t width);
+int tpo_layer_norm_bwd(int dtype, int wdtype, const void* grad_y, const void* x,
+                       const void* weight, const float* mean, const float* rstd,
+                       int64_t rows, int64_t width, double eps, void* grad_x,
+                       void* grad_weight, void* grad_bias, void* workspace,
+                       int64_t workspace_bytes, void* stream);
+
+/*
+ * Softmax attention over packed sequences, with grouped heads.
+ *   q (Tq,Hq,D), k and v (Tk,Hk,D), Hq a multiple of Hk (query head h reads
+ *   key head h / (Hq / Hk)), 1 <= D <= 128.  These three may be strided:
+ *   *_row and *_head are the strides, in elements, of a row and of a head;
+ *   the D values of a head are contiguous.
+ *   offsets_q, offsets_k (B + 1) int64, not decreasing: sequence b has the
+ *   rows offsets[b] .. offsets[b + 1].  lengths_q, lengths_k (B) int64 or
+ *   NULL: how many of these rows, from the first, are in use (the others are
+ *   not read: a cache with room to grow).  Bounds are clamped to the arrays.
+ *   causal: row i of a sequence sees key j where j <= i + (keys - rows): the
+ *   last row sees every key.
+ *   out (Tq,Hq,D) contiguous; rows not in use, and rows that see no key, are 0.
+ *   lse (Hq,Tq) float: log of the sum of exponentials of each row (-inf for
+ *   a row that sees no key), what the backward needs; NULL to leave out.
+ * tpo_attention_bwd: grad_out, out and the gradients are contiguous.  Every
+ *   row of grad_q, grad_k, grad_v is written, rows not in use with 0; sums
+ *   run in a fixed order.
+ * Workspaces are 256-byte aligned; size 0 means none is used.
+ */
+int64_t tpo_attention_fwd_workspace_size(int dtype, int64_t B, int64_t Tq, int64_t Tk,
+                                         int64_t Hq, int64_t Hk, int64_t D);
+int tpo_attention_fwd(int dtype, const void* q, const void* k, const void* v,
+                      const int64_t* offsets_q, const int64_t* offsets_k,
+                      const int64_t* lengths_q, const int64_t* lengths_k, int64_t B,
+                      int64_t Tq, int64_t Tk, int64_t Hq, int64_t Hk, int64_t D,
+                      int64_t q_row, int64_t q_head, int64_t k_row, int64_t k_head,
+                      int64_t v_row, int64_t v_head, int causal, double scale,
+                      void* out, float* lse, void* workspace,
+                      int64_t workspace_bytes, void* stream);
+int64_t tpo_attention_bwd_workspace_size(int dtype, int64_t B, int64_t Tq, int64_t Tk,
+                                         int64_t Hq, int64_t Hk, int64_t D);
+int tpo_attention_bwd(int dtype, const void* grad_out, const void* q, const void* k,
+                      const void* v, const void* out, const float* lse,
+                      const int64_t* offsets_q, const int64_t* offsets_k,
+                      const int64_t* lengths_q, const int64_t* lengths_k, int64_t B,
+                      int64_t Tq, int64_t Tk, int64_t Hq, int64_t Hk, int64_t D,
+                      int64_t q_row, int64_t q_head, int64_t k_row, int64_t k_head,
+                      int64_t v_row, int64_t v_head, int causal, double scale,
+                      void* grad_q, void* grad_k, void* grad_v, void* workspace,
+                      int64_t workspace_bytes, void* stream);
+
+/*
+ * Gated projection: h = act(x w_gate^T) * (x w_up^T).
+ *   x (M,K), w_gate and w_up (F,K), h (M,F); activation is a TPO_ACT_* code
+ *   (GELU is x times the normal distribution function, by erf).
+ * tpo_gated_bwd: grad_h (M,F) -> grad_x (M,K), grad_w_gate and grad_w_up
+ *   (F,K).  The projections are computed again rather than kept, and the
+ *   gradients at them are rounded to `dtype` between the products.  grad_x,
+ *   or the two weights' gradients together, may be NULL and are left out.
+ * Workspaces are 256-byte aligned; size 0 means none is used.
+ */
+enum {
+  TPO_ACT_SILU = 0,
+  TPO_ACT_GELU = 1,
+  TPO_ACT_RELU = 2,
+  TPO_ACT_SIGMOID = 3
+};
+int64_t tpo_gated_fwd_workspace_size(int dtype, int64_t M, int64_t K, int64_t F);
+int tpo_gated_fwd(int dtype, const void* x, const void* w_gate, const void* w_up,
+                  int64_t M, int64_t K, int64_t F, int activation, void* h,
+                  void* workspace, int64_t workspace_bytes, void* stream);
+int64_t tpo_gated_bwd_workspace_size(int dtype, int64_t M, int64_t K, int64_t F);
+int tpo_gated_bwd(int dtype, const void* grad_h, const void* x, const void* w_gate,
+                  const void* w_up, int64_t M, int64_t K, int64_t F, int activation,
+                  void* grad_x, void* grad_w_gate, void* grad_w_up, void* workspace,
+                  int64_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

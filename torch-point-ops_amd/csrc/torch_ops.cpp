@@ -12,47 +12,10 @@
 // allocation (torch caching allocator); the kernels write every output
 // element, so outputs are created with empty().
 #include <Python.h>
-#include <torch/all.h>
-#include <torch/library.h>
-
-#include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
-#include <c10/core/DeviceGuard.h>
-#include <torch/csrc/autograd/custom_function.h>
-
-#include <tuple>
-
-#include "tpo.h"
+#include "shim_common.hpp"
 
 namespace torch_point_ops {
 namespace {
-
-int dtype_code(const at::Tensor& t, const char* op) {
-  switch (t.scalar_type()) {
-    case at::kFloat: return TPO_F32;
-    case at::kDouble: return TPO_F64;
-    case at::kHalf: return TPO_F16;
-    default:
-      TORCH_CHECK(false, op, " not implemented for '", t.scalar_type(), "'");
-  }
-  return -1;
-}
-
-// A tensor whose data starts on a 16-byte boundary (a copy if it does not).
-at::Tensor aligned16(const at::Tensor& t) {
-  return ((uintptr_t)t.data_ptr() & 15) ? t.clone(at::MemoryFormat::Contiguous) : t;
-}
-
-void* stream_of(const at::Tensor& t) {
-  return (void*)c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(t.device().index()).stream();
-}
-
-void check_rc(int rc, const char* op) {
-  TORCH_CHECK(rc == TPO_OK, op, " failed: ", tpo_last_error());
-}
-
-void check_hip(const at::Tensor& t, const char* name) {
-  TORCH_CHECK(t.is_cuda(), name, " must be a GPU tensor");
-}
 
 // ------------------------------------------------------------------ chamfer
 std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> chamfer_forward_hip(
@@ -202,10 +165,6 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> chamfer_loss_forward_autograd(
   auto out = ChamferLossFunction::apply(xyz1, xyz2, mean);
   return {out[0], out[1], out[2]};
 }
-
-// Whether autograd has to follow the call.  Without it the operator runs as it
-// is, also under transforms that a C++ autograd function refuses.
-bool followed(const at::Tensor& a) { return at::GradMode::is_enabled() && a.requires_grad(); }
 
 // chamfer_forward's autograd (chamfer/__init__.py:6-28) in C++: an unused
 // distance output's gradient arrives undefined and counts as zeros.
@@ -512,11 +471,6 @@ std::tuple<at::Tensor, at::Tensor> knn_backward_hip(const at::Tensor& p1_in,
 // not materialised; the index outputs carry none (knn/__init__.py:6-28).
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
-
-template <typename Op>
-auto typed_op(const char* name) {
-  return c10::Dispatcher::singleton().findSchemaOrThrow(name, "").typed<Op>();
-}
 
 template <bool SORTED>
 auto knn_op() {
