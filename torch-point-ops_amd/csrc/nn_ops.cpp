@@ -367,9 +367,9 @@ Gated gated_args(const Tensor& x, const Tensor& wg, const Tensor& wu, const char
   a.K = x.size(-1);
   a.M = x.numel() / a.K;
   a.F = wg.size(0);
-  a.x = x.contiguous();
-  a.wg = wg.contiguous();
-  a.wu = wu.contiguous();
+  a.x = aligned16(x.contiguous());
+  a.wg = aligned16(wg.contiguous());
+  a.wu = aligned16(wu.contiguous());
   return a;
 }
 
