@@ -10,7 +10,28 @@ constexpr float LOG2E = 1.44269504088896341f;
 constexpr float INV_SQRT2 = 0.70710678118654752f;
 constexpr float INV_SQRT_2PI = 0.39894228040143268f;
 
+// The normal distribution function.  For the half types by Abramowitz and
+// Stegun 7.1.26 (1.5e-7 absolute, far below their rounding): erff is several
+// times as long, and a tile's outputs are many instructions with no products to
+// hide behind.  e2: exp(-g^2 / 2).
+template <typename T>
+__device__ __forceinline__ float normal_cdf(float g, float e2) {
+  if constexpr (sizeof(T) == 4) {
+    return 0.5f * (1.f + erff(g * INV_SQRT2));
+  } else {
+    const float x = fabsf(g) * INV_SQRT2;
+    const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.3275911f, x, 1.f));
+    float y = __builtin_fmaf(1.061405429f, t, -1.453152027f);
+    y = __builtin_fmaf(y, t, 1.421413741f);
+    y = __builtin_fmaf(y, t, -0.284496736f);
+    y = __builtin_fmaf(y, t, 0.254829592f);
+    const float tail = 0.5f * y * t * e2;
+    return g > 0.f ? 1.f - tail : tail;
+  }
+}
+
 // The activation a and its derivative d.
+template <typename T>
 __device__ __forceinline__ void gated_act(int act, float g, float& a, float& d) {
   if (act == TPO_ACT_SILU || act == TPO_ACT_SIGMOID) {
     // exp2 of a large gate is inf and its reciprocal 0: both ends are exact
@@ -18,9 +39,10 @@ __device__ __forceinline__ void gated_act(int act, float g, float& a, float& d) 
     a = act == TPO_ACT_SILU ? g * e : e;
     d = act == TPO_ACT_SILU ? e + e * (1.f - e) * g : e * (1.f - e);
   } else if (act == TPO_ACT_GELU) {
-    const float c = 0.5f * (1.f + erff(g * INV_SQRT2));
+    const float e2 = __builtin_amdgcn_exp2f(-0.5f * LOG2E * g * g);
+    const float c = normal_cdf<T>(g, e2);
     a = g * c;
-    d = c + g * (__builtin_amdgcn_exp2f(-0.5f * LOG2E * g * g) * INV_SQRT_2PI);
+    d = c + g * (e2 * INV_SQRT_2PI);
   } else {
     a = g > 0.f ? g : (g != g ? g : 0.f);
     d = g > 0.f ? 1.f : 0.f;
@@ -42,108 +64,139 @@ __device__ __forceinline__ void tile_of(int tiles_m, int tiles_n, int& m, int& n
   n = in / rows;
 }
 
-template <typename T>
-struct alignas(4 * sizeof(T)) Four {
-  T v[4];
-};
-
-// Both projections of a tile of BM rows and BN / 2 features.  The columns of the
-// product are BN / 4 gate and BN / 4 up features for either half of the waves'
-// columns, so that a lane holds both sums of an output.
-// Forward: h.  Backward (gh given): dg and du, which the two products after it
-// read by rows (d, gate features and then up features, each padded with 0 to
-// Fp) and by columns (dt, rows padded with 0 to Mp).
+// Both projections of a tile of BM / 2 features and BN tokens.  The products'
+// rows are the features: BM / 4 of the gate and the same of the up projection
+// for either half of the waves' rows, so that a lane holds both sums of an
+// output, and four neighbouring outputs of one token.
+// Forward: h.  Backward (gh): dg and du into d, a token's 2 Fp values, Fp >= F
+// with 0 past F.
 template <typename T, int BM, int BN, bool BWD>
 __global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void gated_pair_kernel(
-    Rows x, Rows wg, Rows wu, int bytes, int act, const T* __restrict__ gh, int64_t F,
-    T* __restrict__ h, T* __restrict__ d, int64_t Fp, T* __restrict__ dt, int64_t Mp) {
+    Matrix x, Matrix wg, Matrix wu, int act, const T* __restrict__ gh, int64_t F,
+    T* __restrict__ out, int64_t Fp, int whole) {
   __shared__ TileLds<BM, BN> lds;
+  typedef RowLoader<T, BM> LA;
+  typedef RowLoader<T, BN> LB;
   const int64_t M = x.rows;
   int tm, tn;
-  tile_of((int)((M + BM - 1) / BM), (int)((F + BN / 2 - 1) / (BN / 2)), tm, tn);
-  const int64_t m0 = (int64_t)tm * BM, f0 = (int64_t)tn * (BN / 2);
-  const int w = wave_id(), l = lane_id();
-  const Loader<BM> la(x, m0 + w * (BM / 4));
-  const Loader<BN> lb((w & 1) ? wu : wg, f0 + (w >> 1) * (BN / 4));
+  tile_of((int)((M + BN - 1) / BN), (int)((F + BM / 2 - 1) / (BM / 2)), tm, tn);
+  const int w = wave_id();
+  const int64_t t0 = (int64_t)tm * BN, f0 = (int64_t)tn * (BM / 2) + (w >> 1) * (BM / 4);
+  const LA la((w & 1) ? wu : wg, f0);
+  const LB lb(x, t0 + w * (BN / 4));
   f32x16 acc[BM / 64][BN / 64];
-  gemm_tile<T, BM, BN>(lds, la, lb, 0, bytes, acc);
-  constexpr int TF = BN / 128;  // feature tiles of a wave
-  const int64_t row = m0 + (w >> 1) * (BM / 2) + 4 * (l >> 5);
-  const int64_t col = f0 + (w & 1) * (BN / 4) + (l & 31);
+  gemm_tile<T, BM, BN>(lds, la, lb, 0, (int)((x.bytes + SLAB - 1) / SLAB), acc);
+
+  constexpr int TF = BM / 128;  // feature tiles of a wave
+  typedef Rows32<T, BM / 4> R;
+  const R rg{lds.slab[0] + w * 2 * R::BYTES}, ru{rg.lds + R::BYTES};
+  const int h = lane_id() >> 5;
 #pragma unroll
-  for (int i = 0; i < BM / 64; ++i)
+  for (int j = 0; j < BN / 64; ++j) {
+    const int64_t t = t0 + (w & 1) * (BN / 2) + 32 * j;
+    if (BWD) rg.load(gh, F, t, M, f0, F, whole);
 #pragma unroll
-    for (int j = 0; j < TF; ++j) {
-      const int64_t f = col + 32 * j;
+    for (int i = 0; i < TF; ++i)
 #pragma unroll
       for (int b = 0; b < 4; ++b) {
-        const int64_t m = row + 32 * i + 8 * b;
-        Four<T> pg, pu;
+        const int at = 32 * i + 8 * b + 4 * h;
+        Four<T> p, q;
+        if (BWD) p = *(Four<T>*)rg.four(at);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const float g = acc[i][j][4 * b + e], u = acc[i][j + TF][4 * b + e];
-          float a, s;
-          gated_act(act, g, a, s);
-          const bool in = m + e < M && f < F;
-          if (!BWD) {
-            if (in) h[(m + e) * F + f] = (T)(a * u);
+          const float g = acc[i][j][4 * b + e], u = acc[i + TF][j][4 * b + e];
+          float a, d;
+          gated_act<T>(act, g, a, d);
+          if (BWD) {
+            const float y = (float)p.v[e];
+            const bool in = f0 + at + e < F;
+            p.v[e] = in ? (T)(y * u * d) : (T)0.f;
+            q.v[e] = in ? (T)(y * a) : (T)0.f;
           } else {
-            const float t = in ? (float)gh[(m + e) * F + f] : 0.f;
-            pg.v[e] = in ? (T)(t * u * s) : (T)0.f;
-            pu.v[e] = in ? (T)(t * a) : (T)0.f;
-            if (m + e < M && f < Fp) {
-              d[(m + e) * 2 * Fp + f] = pg.v[e];
-              d[(m + e) * 2 * Fp + Fp + f] = pu.v[e];
-            }
+            p.v[e] = (T)(a * u);
           }
         }
-        if (BWD && f < F && m < Mp) {
-          *(Four<T>*)(dt + f * Mp + m) = pg;
-          *(Four<T>*)(dt + (F + f) * Mp + m) = pu;
-        }
+        *(Four<T>*)rg.four(at) = p;
+        if (BWD) *(Four<T>*)ru.four(at) = q;
       }
+    if (BWD) {
+      rg.store(out, 2 * Fp, t, M, f0, Fp, true);
+      ru.store(out + Fp, 2 * Fp, t, M, f0, Fp, true);
+    } else {
+      rg.store(out, F, t, M, f0, F, whole);
     }
+  }
 }
 
-// out = A B^T, or with part the float sums over one of gridDim.z's shares of
-// the summed axis.  blockIdx.y chooses one of two products (A and out a fixed
-// distance on).
+// A tile of sums to out (M rows of N values) or, as floats, to part.
 template <typename T, int BM, int BN>
-__global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void gated_product_kernel(
-    Rows a, Rows b, int bytes, int share, T* __restrict__ out, T* __restrict__ out2,
-    float* __restrict__ part) {
-  __shared__ TileLds<BM, BN> lds;
-  const int64_t M = a.rows, N = b.rows;
-  int tm, tn;
-  tile_of((int)((M + BM - 1) / BM), (int)((N + BN - 1) / BN), tm, tn);
-  const int64_t m0 = (int64_t)tm * BM, n0 = (int64_t)tn * BN;
-  const int w = wave_id(), l = lane_id();
-  if (blockIdx.y) {
-    a.p += M * a.pitch;
-    out = out2;
-  }
-  const Loader<BM> la(a, m0 + w * (BM / 4));
-  const Loader<BN> lb(b, n0 + w * (BN / 4));
-  const int k0 = (int)blockIdx.z * share;
-  f32x16 acc[BM / 64][BN / 64];
-  gemm_tile<T, BM, BN>(lds, la, lb, k0, bytes - k0 < share ? bytes : k0 + share, acc);
-  const int64_t row = m0 + (w >> 1) * (BM / 2) + 4 * (l >> 5);
-  const int64_t col = n0 + (w & 1) * (BN / 2) + (l & 31);
-  if (part) part += ((int64_t)blockIdx.z * gridDim.y + blockIdx.y) * M * N;
+__device__ __forceinline__ void gated_put(TileLds<BM, BN>& lds, const f32x16 (&acc)[BM / 64][BN / 64],
+                                          int64_t n0, int64_t m0, int64_t N, int64_t M,
+                                          T* __restrict__ out, float* __restrict__ part, int whole) {
+  const int w = wave_id(), h = lane_id() >> 5;
+  n0 += (w >> 1) * (BM / 2);
+  m0 += (w & 1) * (BN / 2);
+  auto put = [&](auto t, auto* to) {
+    typedef decltype(t) V;
+    typedef Rows32<V, BM / 2> R;
+    const R r{lds.slab[0] + w * R::BYTES};
 #pragma unroll
-  for (int i = 0; i < BM / 64; ++i)
+    for (int j = 0; j < BN / 64; ++j) {
 #pragma unroll
-    for (int j = 0; j < BN / 64; ++j)
+      for (int i = 0; i < BM / 64; ++i)
 #pragma unroll
-      for (int v = 0; v < 16; ++v) {
-        const int64_t m = row + 32 * i + 8 * (v >> 2) + (v & 3), n = col + 32 * j;
-        if (m < M && n < N) {
-          if (part)
-            part[m * N + n] = acc[i][j][v];
-          else
-            out[m * N + n] = (T)acc[i][j][v];
+        for (int b = 0; b < 4; ++b) {
+          Four<V> p;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) p.v[e] = (V)acc[i][j][4 * b + e];
+          *(Four<V>*)r.four(32 * i + 8 * b + 4 * h) = p;
         }
-      }
+      r.store(to, N, m0 + 32 * j, M, n0, N, whole);
+    }
+  };
+  if (part)
+    put(float(), part);
+  else
+    put(T(), out);
+}
+
+// dx = [dg du] [Wg; Wu], M tokens of K values; blockIdx.y: a share of the sum.
+template <typename T, int BM, int BN>
+__global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void gated_dx_kernel(
+    Matrix d, Matrix wg, const char* wu, int slabs, int share, int64_t K, T* __restrict__ out,
+    float* __restrict__ part, int whole) {
+  __shared__ TileLds<BM, BN> lds;
+  const int64_t M = d.rows;
+  int tm, tn;
+  tile_of((int)((M + BN - 1) / BN), (int)((K + BM - 1) / BM), tm, tn);
+  const int64_t m0 = (int64_t)tm * BN, n0 = (int64_t)tn * BM;
+  const PairLoader<T, BM> la(wg, wu, slabs, n0);
+  const RowLoader<T, BN> lb(d, m0 + wave_id() * (BN / 4));
+  const int s0 = blockIdx.y * share, s1 = s0 + share < 2 * slabs ? s0 + share : 2 * slabs;
+  f32x16 acc[BM / 64][BN / 64];
+  gemm_tile<T, BM, BN>(lds, la, lb, s0, s1, acc);
+  if (part) part += blockIdx.y * M * K;
+  gated_put<T, BM, BN>(lds, acc, n0, m0, K, M, out, part, whole);
+}
+
+// dWg = dg^T x and dWu = du^T x (blockIdx.z), F rows of K values; blockIdx.y: a
+// share of the sum over the tokens.
+template <typename T, int BM, int BN>
+__global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void gated_dw_kernel(
+    Matrix x, Matrix d, int64_t F, int slabs, int share, int64_t K, T* __restrict__ dwg,
+    T* __restrict__ dwu, float* __restrict__ part, int whole) {
+  __shared__ TileLds<BM, BN> lds;
+  int tm, tn;
+  tile_of((int)((F + BN - 1) / BN), (int)((K + BM - 1) / BM), tm, tn);
+  const int64_t m0 = (int64_t)tm * BN, n0 = (int64_t)tn * BM;
+  if (blockIdx.z) d.p += d.bytes;
+  const ColLoader<T, BM> la(x, n0);
+  const ColLoader<T, BN> lb(d, m0);
+  const int s0 = blockIdx.y * share, s1 = s0 + share < slabs ? s0 + share : slabs;
+  f32x16 acc[BM / 64][BN / 64];
+  gemm_tile<T, BM, BN>(lds, la, lb, s0, s1, acc);
+  if (part) part += ((int64_t)blockIdx.y * 2 + blockIdx.z) * F * K;
+  gated_put<T, BM, BN>(lds, acc, n0, m0, K, F, blockIdx.z ? dwu : dwg, part, whole);
 }
 
 // out, out2 (n values each): the shares of a split product added in order
@@ -160,33 +213,23 @@ __global__ __launch_bounds__(256) void gated_join_kernel(const float* __restrict
   }
 }
 
-// Copies of a matrix (R, C) that the products can read: rows padded with 0 to
-// `pitch` values (plain), or its transpose (C rows of `pitch` values, R of them
-// the matrix's, from column `at` on; 0 up to column `at` + pad).
+// Copies of up to three matrices of C columns with rows padded with 0 to `pitch`
+// values (16 bytes).
+struct Copies {
+  const void* in[3];
+  void* out[3];
+  int64_t rows[3];
+};
 template <typename T>
-__global__ __launch_bounds__(256) void gated_pad_kernel(const T* __restrict__ in, int64_t R,
-                                                        int64_t C, T* __restrict__ out,
-                                                        int64_t pitch) {
-  const int64_t n = R * pitch;
+__global__ __launch_bounds__(256) void gated_pad_kernel(Copies m, int64_t C, int64_t pitch) {
+  const int y = blockIdx.y;
+  const T* in = (const T*)m.in[y];
+  T* out = (T*)m.out[y];
+  const int64_t n = m.rows[y] * pitch;
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
     const int64_t r = i / pitch, c = i - r * pitch;
     out[i] = c < C ? in[r * C + c] : (T)0.f;
   }
-}
-template <typename T>
-__global__ __launch_bounds__(256) void gated_turn_kernel(const T* __restrict__ in, int64_t R,
-                                                         int64_t C, T* __restrict__ out,
-                                                         int64_t pitch, int64_t pad) {
-  __shared__ T s[64][65];
-  const int64_t r0 = (int64_t)blockIdx.x * 64, c0 = (int64_t)blockIdx.y * 64;
-  const int x = threadIdx.x & 63, y = threadIdx.x >> 6;
-#pragma unroll
-  for (int i = 0; i < 64; i += 4)
-    s[y + i][x] = r0 + y + i < R && c0 + x < C ? in[(r0 + y + i) * C + c0 + x] : (T)0.f;
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < 64; i += 4)
-    if (c0 + y + i < C && r0 + x < pad) out[(c0 + y + i) * pitch + r0 + x] = s[x][y + i];
 }
 
 // ---------------------------------------------------------------------- host
@@ -212,43 +255,41 @@ int gated_aligned(const char* op, std::initializer_list<const void*> ps) {
 
 inline int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-// How a product of M x N sums over `bytes` of the summed axis is cut: the tile's
-// edge and the number of shares of that axis.
+// How a product of M x N sums is cut: the tile's edge and the number of shares
+// of the summed axis (`slabs` long).
 struct Cut {
   int tile, shares;
 };
-Cut gated_cut(int64_t M, int64_t N, int64_t products, int64_t bytes, bool may_split) {
-  const int64_t large = cdiv(M, 256) * cdiv(N, 256) * products;
-  const int64_t small = cdiv(M, 128) * cdiv(N, 128) * products;
+Cut gated_cut(int64_t M, int64_t N, int64_t products, int64_t slabs) {
+  auto count = [&](int t) { return cdiv(M, t) * cdiv(N, t) * products; };
   Cut c{256, 1};
-  if (large < 192) c.tile = 128;
-  if (may_split) {
-    const int64_t have = c.tile == 256 ? large : cdiv(small, 2);
-    int64_t s = 256 / (have < 1 ? 1 : have);
-    const int64_t most = bytes / (16 * SLAB);  // a share is worth its sums' way through memory
+  if (count(256) < 192) c.tile = 128;
+  if (c.tile == 128 && count(128) < 192) c.tile = 64;
+  if (slabs > 0) {
+    int64_t s = 256 / (count(c.tile) < 1 ? 1 : count(c.tile));
+    const int64_t most = slabs / 16;  // a share is worth its sums' way through memory
     if (s > most) s = most;
     c.shares = s < 1 ? 1 : (int)s;
   }
   return c;
 }
-inline int gated_share(int64_t bytes, int shares) {
-  return (int)(cdiv(cdiv(bytes, SLAB), shares) * SLAB);
-}
 
 // What the calls keep in the workspace, in bytes from its start.
 struct Plan {
-  int64_t Kp, Fp, Mp;               // widths padded to 16 bytes
-  int64_t x, wg, wu;                // padded copies (-1: the inputs do)
-  int64_t d, dt, wt, xt, part;
+  int64_t Kp, Fp;          // K padded to 16 bytes, F to a slab
+  int64_t x, wg, wu;       // padded copies (-1: the inputs do)
+  int64_t d, part;
+  int64_t fslabs, mslabs;  // slabs of F and of M
   Cut dx, dw;
   int64_t bytes;
 };
 Plan gated_plan(int dtype, int64_t M, int64_t K, int64_t F, bool bwd) {
-  const int64_t z = element_bytes(dtype), per = 16 / z;
+  const int64_t z = element_bytes(dtype), per = SLAB / z;
   Plan p = {};
-  p.Kp = round_up(K, per);
+  p.Kp = round_up(K, 16 / z);
   p.Fp = round_up(F, per);
-  p.Mp = round_up(M, per);
+  p.fslabs = p.Fp / per;
+  p.mslabs = cdiv(M, per);
   auto take = [&](int64_t values, int64_t size) {
     const int64_t at = p.bytes;
     p.bytes += round_up(values * size, 256);
@@ -262,11 +303,8 @@ Plan gated_plan(int dtype, int64_t M, int64_t K, int64_t F, bool bwd) {
   }
   if (bwd) {
     p.d = take(M * 2 * p.Fp, z);
-    p.dt = take(2 * F * p.Mp, z);
-    p.wt = take(K * 2 * p.Fp, z);
-    p.xt = take(K * p.Mp, z);
-    p.dx = gated_cut(M, K, 1, 2 * p.Fp * z, true);
-    p.dw = gated_cut(F, K, 2, p.Mp * z, true);
+    p.dx = gated_cut(M, K, 1, 2 * p.fslabs);
+    p.dw = gated_cut(F, K, 2, p.mslabs);
     const int64_t a = p.dx.shares > 1 ? p.dx.shares * M * K : 0;
     const int64_t b = p.dw.shares > 1 ? p.dw.shares * 2 * F * K : 0;
     p.part = take(a > b ? a : b, 4);
@@ -279,46 +317,67 @@ unsigned gated_blocks(int64_t n) { return (unsigned)(cdiv(n, 256) < 4096 ? cdiv(
 // The inputs as the products read them, padded copies made where needed.
 template <typename T>
 void gated_inputs(const Plan& p, const void* x, const void* wg, const void* wu, int64_t M,
-                  int64_t K, int64_t F, char* ws, hipStream_t s, Rows (&r)[3]) {
+                  int64_t K, int64_t F, char* ws, hipStream_t s, Matrix (&r)[3]) {
   const void* in[3] = {x, wg, wu};
-  const int64_t at[3] = {p.x, p.wg, p.wu}, rows[3] = {M, F, F};
+  const int64_t at[3] = {p.x, p.wg, p.wu}, rows[3] = {M, F, F}, pitch = p.Kp * sizeof(T);
+  Copies c;
   for (int i = 0; i < 3; ++i) {
-    if (at[i] >= 0)
-      gated_pad_kernel<T><<<dim3(gated_blocks(rows[i] * p.Kp)), 256, 0, s>>>(
-          (const T*)in[i], rows[i], K, (T*)(ws + at[i]), p.Kp);
-    r[i] = Rows{at[i] >= 0 ? ws + at[i] : (const char*)in[i], p.Kp * (int64_t)sizeof(T), rows[i]};
+    c.in[i] = in[i];
+    c.out[i] = ws + at[i];
+    c.rows[i] = rows[i];
+    r[i] = Matrix{p.Kp != K ? ws + at[i] : (const char*)in[i], pitch, rows[i], pitch};
   }
+  if (p.Kp != K)
+    gated_pad_kernel<T><<<dim3(gated_blocks((M > F ? M : F) * p.Kp), 3), 256, 0, s>>>(c, K, p.Kp);
+}
+
+// Whether rows of n values starting at p can be written 16 bytes at a time.
+template <typename T>
+int whole_rows(const void* p, int64_t n) {
+  return ((uintptr_t)p & 15) == 0 && n * sizeof(T) % 16 == 0;
 }
 
 template <typename T, bool BWD>
-void gated_pair(const Rows (&r)[3], int act, const T* gh, int64_t F, T* h, T* d, int64_t Fp, T* dt,
-                int64_t Mp, hipStream_t s) {
+void gated_pair(const Matrix (&r)[3], int act, const T* gh, int64_t F, T* out, int64_t Fp,
+                hipStream_t s) {
   const int64_t M = r[0].rows;
-  const Cut c = gated_cut(M, 2 * F, 1, r[0].pitch, false);
-  const unsigned grid = (unsigned)(cdiv(M, c.tile) * cdiv(F, c.tile / 2));
-  if (c.tile == 256)
-    gated_pair_kernel<T, 256, 256, BWD><<<dim3(grid), 256, 0, s>>>(
-        r[0], r[1], r[2], (int)r[0].pitch, act, gh, F, h, d, Fp, dt, Mp);
-  else
-    gated_pair_kernel<T, 128, 128, BWD><<<dim3(grid), 256, 0, s>>>(
-        r[0], r[1], r[2], (int)r[0].pitch, act, gh, F, h, d, Fp, dt, Mp);
+  const int whole = whole_rows<T>(BWD ? (const void*)gh : (const void*)out, F);
+  auto run = [&](auto bm, auto bn) {
+    constexpr int BM = decltype(bm)::value, BN = decltype(bn)::value;
+    gated_pair_kernel<T, BM, BN, BWD><<<dim3((unsigned)(cdiv(M, BN) * cdiv(F, BM / 2))), 256, 0, s>>>(
+        r[0], r[1], r[2], act, gh, F, out, Fp, whole);
+  };
+  typedef std::integral_constant<int, 256> I256;
+  typedef std::integral_constant<int, 128> I128;
+  typedef std::integral_constant<int, 64> I64;
+  switch (gated_cut(M, 2 * F, 1, 0).tile) {
+    case 256: run(I256(), I256()); break;
+    case 128: run(I128(), I128()); break;
+    default: run(I128(), I64());
+  }
 }
 
-// out (and out2, the product with the rows of A after its first ones)
-template <typename T>
-void gated_product(const Rows& a, const Rows& b, const Cut& c, T* out, T* out2, float* part,
-                   hipStream_t s) {
-  const int products = out2 ? 2 : 1, share = gated_share(a.pitch, c.shares);
-  const int shares = share > 0 ? (int)cdiv(a.pitch, share) : 1;
-  const dim3 grid((unsigned)(cdiv(a.rows, c.tile) * cdiv(b.rows, c.tile)), products, shares);
-  float* to = shares > 1 ? part : nullptr;
-  if (c.tile == 256)
-    gated_product_kernel<T, 256, 256><<<grid, 256, 0, s>>>(a, b, (int)a.pitch, share, out, out2, to);
-  else
-    gated_product_kernel<T, 128, 128><<<grid, 256, 0, s>>>(a, b, (int)a.pitch, share, out, out2, to);
+template <typename T, int E>
+void gated_dx(const Plan& p, const Matrix& d, const Matrix& wg, const Matrix& wu, int64_t K, T* out,
+              float* part, hipStream_t s) {
+  const int64_t M = d.rows;
+  const int share = (int)cdiv(2 * p.fslabs, p.dx.shares), shares = p.dx.shares;
+  const int whole = shares > 1 ? K % 4 == 0 : whole_rows<T>(out, K);
+  gated_dx_kernel<T, E, E><<<dim3((unsigned)(cdiv(M, E) * cdiv(K, E)), shares), 256, 0, s>>>(
+      d, wg, wu.p, (int)p.fslabs, share, K, out, shares > 1 ? part : nullptr, whole);
   if (shares > 1)
-    gated_join_kernel<T><<<dim3(gated_blocks(a.rows * b.rows), products), 256, 0, s>>>(
-        part, shares, a.rows * b.rows, out, out2);
+    gated_join_kernel<T><<<dim3(gated_blocks(M * K)), 256, 0, s>>>(part, shares, M * K, out, out);
+}
+
+template <typename T, int E>
+void gated_dw(const Plan& p, const Matrix& x, const Matrix& d, int64_t F, int64_t K, T* dwg, T* dwu,
+              float* part, hipStream_t s) {
+  const int share = (int)cdiv(p.mslabs, p.dw.shares), shares = p.dw.shares;
+  const int whole = shares > 1 ? K % 4 == 0 : whole_rows<T>(dwg, K) && whole_rows<T>(dwu, K);
+  gated_dw_kernel<T, E, E><<<dim3((unsigned)(cdiv(F, E) * cdiv(K, E)), shares, 2), 256, 0, s>>>(
+      x, d, F, (int)p.mslabs, share, K, dwg, dwu, shares > 1 ? part : nullptr, whole);
+  if (shares > 1)
+    gated_join_kernel<T><<<dim3(gated_blocks(F * K), 2), 256, 0, s>>>(part, shares, F * K, dwg, dwu);
 }
 
 }  // namespace tpo
@@ -343,9 +402,9 @@ extern "C" int tpo_gated_fwd(int dtype, const void* x, const void* w_gate, const
   hipStream_t s = (hipStream_t)stream;
   with_element(dtype, [&](auto t) {
     typedef decltype(t) T;
-    Rows r[3];
+    Matrix r[3];
     gated_inputs<T>(p, x, w_gate, w_up, M, K, F, (char*)workspace, s, r);
-    gated_pair<T, false>(r, activation, nullptr, F, (T*)h, nullptr, 0, nullptr, 0, s);
+    gated_pair<T, false>(r, activation, nullptr, F, (T*)h, 0, s);
   });
   return check_launch("gated_fwd");
 }
@@ -372,29 +431,29 @@ extern "C" int tpo_gated_bwd(int dtype, const void* grad_h, const void* x, const
   if (M == 0 && F == 0) return TPO_OK;
   with_element(dtype, [&](auto t) {
     typedef decltype(t) T;
-    const int64_t z = sizeof(T);
-    T *d = (T*)(ws + p.d), *dt = (T*)(ws + p.dt), *wt = (T*)(ws + p.wt), *xt = (T*)(ws + p.xt);
+    Matrix r[3];
+    gated_inputs<T>(p, x, w_gate, w_up, M, K, F, ws, s, r);
+    const int64_t row = 2 * p.Fp * sizeof(T);
     float* part = (float*)(ws + p.part);
-    if (M > 0 && F > 0) {
-      Rows r[3];
-      gated_inputs<T>(p, x, w_gate, w_up, M, K, F, ws, s, r);
-      gated_pair<T, true>(r, activation, (const T*)grad_h, F, nullptr, d, p.Fp, dt, p.Mp, s);
-    }
+    if (M > 0 && F > 0)
+      gated_pair<T, true>(r, activation, (const T*)grad_h, F, (T*)(ws + p.d), p.Fp, s);
     if (grad_x && M > 0) {
-      if (F > 0) {
-        const dim3 grid((unsigned)cdiv(p.Fp, 64), (unsigned)cdiv(K, 64));
-        gated_turn_kernel<T><<<grid, 256, 0, s>>>((const T*)w_gate, F, K, wt, 2 * p.Fp, p.Fp);
-        gated_turn_kernel<T><<<grid, 256, 0, s>>>((const T*)w_up, F, K, wt + p.Fp, 2 * p.Fp, p.Fp);
+      const Matrix d{ws + p.d, row, M, row};
+      T* to = (T*)grad_x;
+      switch (p.dx.tile) {
+        case 256: gated_dx<T, 256>(p, d, r[1], r[2], K, to, part, s); break;
+        case 128: gated_dx<T, 128>(p, d, r[1], r[2], K, to, part, s); break;
+        default: gated_dx<T, 64>(p, d, r[1], r[2], K, to, part, s);
       }
-      gated_product<T>(Rows{(const char*)d, 2 * p.Fp * z, M}, Rows{(const char*)wt, 2 * p.Fp * z, K},
-                       p.dx, (T*)grad_x, nullptr, part, s);
     }
     if (grad_w_gate && F > 0) {
-      if (M > 0)
-        gated_turn_kernel<T><<<dim3((unsigned)cdiv(p.Mp, 64), (unsigned)cdiv(K, 64)), 256, 0, s>>>(
-            (const T*)x, M, K, xt, p.Mp, p.Mp);
-      gated_product<T>(Rows{(const char*)dt, p.Mp * z, F}, Rows{(const char*)xt, p.Mp * z, K}, p.dw,
-                       (T*)grad_w_gate, (T*)grad_w_up, part, s);
+      const Matrix d{ws + p.d, row, M, row / 2};
+      T *g = (T*)grad_w_gate, *u = (T*)grad_w_up;
+      switch (p.dw.tile) {
+        case 256: gated_dw<T, 256>(p, r[0], d, F, K, g, u, part, s); break;
+        case 128: gated_dw<T, 128>(p, r[0], d, F, K, g, u, part, s); break;
+        default: gated_dw<T, 64>(p, r[0], d, F, K, g, u, part, s);
+      }
     }
   });
   return check_launch("gated_bwd");
