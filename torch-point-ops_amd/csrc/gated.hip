@@ -49,6 +49,16 @@ __device__ __forceinline__ void gated_act(int act, float g, float& a, float& d) 
   }
 }
 
+// Slabs: 64 bytes three deep for the large tile (256 x 128), whose waves hold so
+// many operands at a time that a slab's loads and reads go between its products;
+// 128 bytes two deep for the others.  Two workgroups or more share a CU, so that
+// one's products run beside the other's epilogue: a tile of 256 x 256, alone on
+// its CU, took 583 us where 256 x 128 takes 559 (8192 x 2048 x 8192, gelu), and
+// 489 where it takes 390 in the backward's first product.
+template <int BM, int BN>
+using GatedLds = TileLds<BM, BN, BM == 256 ? 64 : 128, BM == 256 ? 3 : 2, BM == 256>;
+constexpr int UNIT = 128;  // bytes of the summed axis that widths and shares are rounded to
+
 // Tile (m, n) of a grid of tiles_m x tiles_n: an XCD takes consecutive tiles
 // (workgroups go round-robin over the eight), which run down groups of eight
 // row tiles, so that the tiles that an XCD works on at a time share rows of both
@@ -71,12 +81,13 @@ __device__ __forceinline__ void tile_of(int tiles_m, int tiles_n, int& m, int& n
 // Forward: h.  Backward (gh): dg and du into d, a token's 2 Fp values, Fp >= F
 // with 0 past F.
 template <typename T, int BM, int BN, bool BWD>
-__global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void gated_pair_kernel(
+__global__ __launch_bounds__(256, 2) void gated_pair_kernel(
     Matrix x, Matrix wg, Matrix wu, int act, const T* __restrict__ gh, int64_t F,
     T* __restrict__ out, int64_t Fp, int whole) {
-  __shared__ TileLds<BM, BN> lds;
-  typedef RowLoader<T, BM> LA;
-  typedef RowLoader<T, BN> LB;
+  __shared__ GatedLds<BM, BN> lds;
+  constexpr int SLAB = GatedLds<BM, BN>::SLAB;
+  typedef RowLoader<T, BM, SLAB> LA;
+  typedef RowLoader<T, BN, SLAB> LB;
   const int64_t M = x.rows;
   int tm, tn;
   tile_of((int)((M + BN - 1) / BN), (int)((F + BM / 2 - 1) / (BM / 2)), tm, tn);
@@ -89,7 +100,7 @@ __global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void gated_pair_kernel(
 
   constexpr int TF = BM / 128;  // feature tiles of a wave
   typedef Rows32<T, BM / 4> R;
-  const R rg{lds.slab[0] + w * 2 * R::BYTES}, ru{rg.lds + R::BYTES};
+  const R rg{(char*)&lds + w * 2 * R::BYTES}, ru{rg.lds + R::BYTES};
   const int h = lane_id() >> 5;
 #pragma unroll
   for (int j = 0; j < BN / 64; ++j) {
@@ -129,8 +140,8 @@ __global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void gated_pair_kernel(
 }
 
 // A tile of sums to out (M rows of N values) or, as floats, to part.
-template <typename T, int BM, int BN>
-__device__ __forceinline__ void gated_put(TileLds<BM, BN>& lds, const f32x16 (&acc)[BM / 64][BN / 64],
+template <typename T, int BM, int BN, typename Lds>
+__device__ __forceinline__ void gated_put(Lds& lds, const f32x16 (&acc)[BM / 64][BN / 64],
                                           int64_t n0, int64_t m0, int64_t N, int64_t M,
                                           T* __restrict__ out, float* __restrict__ part, int whole) {
   const int w = wave_id(), h = lane_id() >> 5;
@@ -139,7 +150,7 @@ __device__ __forceinline__ void gated_put(TileLds<BM, BN>& lds, const f32x16 (&a
   auto put = [&](auto t, auto* to) {
     typedef decltype(t) V;
     typedef Rows32<V, BM / 2> R;
-    const R r{lds.slab[0] + w * R::BYTES};
+    const R r{(char*)&lds + w * R::BYTES};
 #pragma unroll
     for (int j = 0; j < BN / 64; ++j) {
 #pragma unroll
@@ -162,19 +173,20 @@ __device__ __forceinline__ void gated_put(TileLds<BM, BN>& lds, const f32x16 (&a
 
 // dx = [dg du] [Wg; Wu], M tokens of K values; blockIdx.y: a share of the sum.
 template <typename T, int BM, int BN>
-__global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void gated_dx_kernel(
-    Matrix d, Matrix wg, const char* wu, int slabs, int share, int64_t K, T* __restrict__ out,
+__global__ __launch_bounds__(256, 2) void gated_dx_kernel(
+    Matrix d, Matrix wg, const char* wu, int units, int share, int64_t K, T* __restrict__ out,
     float* __restrict__ part, int whole) {
-  __shared__ TileLds<BM, BN> lds;
+  __shared__ GatedLds<BM, BN> lds;
+  constexpr int SLAB = GatedLds<BM, BN>::SLAB;
   const int64_t M = d.rows;
   int tm, tn;
   tile_of((int)((M + BN - 1) / BN), (int)((K + BM - 1) / BM), tm, tn);
   const int64_t m0 = (int64_t)tm * BN, n0 = (int64_t)tn * BM;
-  const PairLoader<T, BM> la(wg, wu, slabs, n0);
-  const RowLoader<T, BN> lb(d, m0 + wave_id() * (BN / 4));
-  const int s0 = blockIdx.y * share, s1 = s0 + share < 2 * slabs ? s0 + share : 2 * slabs;
+  const PairLoader<T, BM, SLAB> la(wg, wu, units * (UNIT / SLAB), n0);
+  const RowLoader<T, BN, SLAB> lb(d, m0 + wave_id() * (BN / 4));
+  const int u0 = blockIdx.y * share, u1 = u0 + share < 2 * units ? u0 + share : 2 * units;
   f32x16 acc[BM / 64][BN / 64];
-  gemm_tile<T, BM, BN>(lds, la, lb, s0, s1, acc);
+  gemm_tile<T, BM, BN>(lds, la, lb, u0 * (UNIT / SLAB), u1 * (UNIT / SLAB), acc);
   if (part) part += blockIdx.y * M * K;
   gated_put<T, BM, BN>(lds, acc, n0, m0, K, M, out, part, whole);
 }
@@ -182,19 +194,20 @@ __global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void gated_dx_kernel(
 // dWg = dg^T x and dWu = du^T x (blockIdx.z), F rows of K values; blockIdx.y: a
 // share of the sum over the tokens.
 template <typename T, int BM, int BN>
-__global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void gated_dw_kernel(
-    Matrix x, Matrix d, int64_t F, int slabs, int share, int64_t K, T* __restrict__ dwg,
+__global__ __launch_bounds__(256, 2) void gated_dw_kernel(
+    Matrix x, Matrix d, int64_t F, int units, int share, int64_t K, T* __restrict__ dwg,
     T* __restrict__ dwu, float* __restrict__ part, int whole) {
-  __shared__ TileLds<BM, BN> lds;
+  __shared__ GatedLds<BM, BN> lds;
+  constexpr int SLAB = GatedLds<BM, BN>::SLAB;
   int tm, tn;
   tile_of((int)((F + BN - 1) / BN), (int)((K + BM - 1) / BM), tm, tn);
   const int64_t m0 = (int64_t)tm * BN, n0 = (int64_t)tn * BM;
   if (blockIdx.z) d.p += d.bytes;
-  const ColLoader<T, BM> la(x, n0);
-  const ColLoader<T, BN> lb(d, m0);
-  const int s0 = blockIdx.y * share, s1 = s0 + share < slabs ? s0 + share : slabs;
+  const ColLoader<T, BM, SLAB> la(x, n0);
+  const ColLoader<T, BN, SLAB> lb(d, m0);
+  const int u0 = blockIdx.y * share, u1 = u0 + share < units ? u0 + share : units;
   f32x16 acc[BM / 64][BN / 64];
-  gemm_tile<T, BM, BN>(lds, la, lb, s0, s1, acc);
+  gemm_tile<T, BM, BN>(lds, la, lb, u0 * (UNIT / SLAB), u1 * (UNIT / SLAB), acc);
   if (part) part += ((int64_t)blockIdx.y * 2 + blockIdx.z) * F * K;
   gated_put<T, BM, BN>(lds, acc, n0, m0, K, F, blockIdx.z ? dwu : dwg, part, whole);
 }
@@ -255,19 +268,27 @@ int gated_aligned(const char* op, std::initializer_list<const void*> ps) {
 
 inline int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-// How a product of M x N sums is cut: the tile's edge and the number of shares
-// of the summed axis (`slabs` long).
+// How a product of `rows` x `cols` sums (the rows being what the tile's longer
+// side covers) is cut: the tile and the number of shares of the summed axis,
+// `units` long.  A CU takes two workgroups of the larger tiles at a time, so the
+// largest tile that gives nearly two a CU is taken (half as many would leave
+// half of the matrix cores' time to waiting); where even the smallest tile gives
+// fewer, the summed axis is shared out, if the caller can add the shares up.
+// 1000 x 385 x 1023 in float, training: 115 us with 64-tiles, 233 with 128.
+enum Tile { LARGE, MIDDLE, SMALL };  // 256 x 128, 128 x 128, 64 x 64 (128 x 64 for the pair)
 struct Cut {
-  int tile, shares;
+  Tile tile;
+  int shares;
 };
-Cut gated_cut(int64_t M, int64_t N, int64_t products, int64_t slabs) {
-  auto count = [&](int t) { return cdiv(M, t) * cdiv(N, t) * products; };
-  Cut c{256, 1};
-  if (count(256) < 192) c.tile = 128;
-  if (c.tile == 128 && count(128) < 192) c.tile = 64;
-  if (slabs > 0) {
-    int64_t s = 256 / (count(c.tile) < 1 ? 1 : count(c.tile));
-    const int64_t most = slabs / 16;  // a share is worth its sums' way through memory
+Cut gated_cut(int64_t rows, int64_t cols, int64_t products, int64_t units) {
+  const int64_t middle = cdiv(rows, 128) * cdiv(cols, 128) * products;
+  Cut c{SMALL, 1};
+  if (cdiv(rows, 256) * cdiv(cols, 128) * products >= 448) c.tile = LARGE;
+  else if (middle >= 384) c.tile = MIDDLE;
+  if (c.tile == SMALL && units > 0) {
+    const int64_t blocks = cdiv(rows, 64) * cdiv(cols, 64) * products;
+    int64_t s = 768 / (blocks < 1 ? 1 : blocks);
+    const int64_t most = units / 8;  // a share is worth its sums' way through memory
     if (s > most) s = most;
     c.shares = s < 1 ? 1 : (int)s;
   }
@@ -276,20 +297,20 @@ Cut gated_cut(int64_t M, int64_t N, int64_t products, int64_t slabs) {
 
 // What the calls keep in the workspace, in bytes from its start.
 struct Plan {
-  int64_t Kp, Fp;          // K padded to 16 bytes, F to a slab
+  int64_t Kp, Fp;          // K padded to 16 bytes, F to a unit
   int64_t x, wg, wu;       // padded copies (-1: the inputs do)
   int64_t d, part;
-  int64_t fslabs, mslabs;  // slabs of F and of M
+  int64_t funits, munits;  // units of F and of M
   Cut dx, dw;
   int64_t bytes;
 };
 Plan gated_plan(int dtype, int64_t M, int64_t K, int64_t F, bool bwd) {
-  const int64_t z = element_bytes(dtype), per = SLAB / z;
+  const int64_t z = element_bytes(dtype), per = UNIT / z;
   Plan p = {};
   p.Kp = round_up(K, 16 / z);
   p.Fp = round_up(F, per);
-  p.fslabs = p.Fp / per;
-  p.mslabs = cdiv(M, per);
+  p.funits = p.Fp / per;
+  p.munits = cdiv(M, per);
   auto take = [&](int64_t values, int64_t size) {
     const int64_t at = p.bytes;
     p.bytes += round_up(values * size, 256);
@@ -303,8 +324,8 @@ Plan gated_plan(int dtype, int64_t M, int64_t K, int64_t F, bool bwd) {
   }
   if (bwd) {
     p.d = take(M * 2 * p.Fp, z);
-    p.dx = gated_cut(M, K, 1, 2 * p.fslabs);
-    p.dw = gated_cut(F, K, 2, p.mslabs);
+    p.dx = gated_cut(K, M, 1, 2 * p.funits);
+    p.dw = gated_cut(K, F, 2, p.munits);
     const int64_t a = p.dx.shares > 1 ? p.dx.shares * M * K : 0;
     const int64_t b = p.dw.shares > 1 ? p.dw.shares * 2 * F * K : 0;
     p.part = take(a > b ? a : b, 4);
@@ -350,32 +371,32 @@ void gated_pair(const Matrix (&r)[3], int act, const T* gh, int64_t F, T* out, i
   typedef std::integral_constant<int, 256> I256;
   typedef std::integral_constant<int, 128> I128;
   typedef std::integral_constant<int, 64> I64;
-  switch (gated_cut(M, 2 * F, 1, 0).tile) {
-    case 256: run(I256(), I256()); break;
-    case 128: run(I128(), I128()); break;
-    default: run(I128(), I64());
+  switch (gated_cut(2 * F, M, 1, 0).tile) {
+    case LARGE: run(I256(), I128()); break;
+    case MIDDLE: run(I128(), I128()); break;
+    case SMALL: run(I128(), I64()); break;
   }
 }
 
-template <typename T, int E>
+template <typename T, int BM, int BN>
 void gated_dx(const Plan& p, const Matrix& d, const Matrix& wg, const Matrix& wu, int64_t K, T* out,
               float* part, hipStream_t s) {
   const int64_t M = d.rows;
-  const int share = (int)cdiv(2 * p.fslabs, p.dx.shares), shares = p.dx.shares;
+  const int share = (int)cdiv(2 * p.funits, p.dx.shares), shares = p.dx.shares;
   const int whole = shares > 1 ? K % 4 == 0 : whole_rows<T>(out, K);
-  gated_dx_kernel<T, E, E><<<dim3((unsigned)(cdiv(M, E) * cdiv(K, E)), shares), 256, 0, s>>>(
-      d, wg, wu.p, (int)p.fslabs, share, K, out, shares > 1 ? part : nullptr, whole);
+  gated_dx_kernel<T, BM, BN><<<dim3((unsigned)(cdiv(M, BN) * cdiv(K, BM)), shares), 256, 0, s>>>(
+      d, wg, wu.p, (int)p.funits, share, K, out, shares > 1 ? part : nullptr, whole);
   if (shares > 1)
     gated_join_kernel<T><<<dim3(gated_blocks(M * K)), 256, 0, s>>>(part, shares, M * K, out, out);
 }
 
-template <typename T, int E>
+template <typename T, int BM, int BN>
 void gated_dw(const Plan& p, const Matrix& x, const Matrix& d, int64_t F, int64_t K, T* dwg, T* dwu,
               float* part, hipStream_t s) {
-  const int share = (int)cdiv(p.mslabs, p.dw.shares), shares = p.dw.shares;
+  const int share = (int)cdiv(p.munits, p.dw.shares), shares = p.dw.shares;
   const int whole = shares > 1 ? K % 4 == 0 : whole_rows<T>(dwg, K) && whole_rows<T>(dwu, K);
-  gated_dw_kernel<T, E, E><<<dim3((unsigned)(cdiv(F, E) * cdiv(K, E)), shares, 2), 256, 0, s>>>(
-      x, d, F, (int)p.mslabs, share, K, dwg, dwu, shares > 1 ? part : nullptr, whole);
+  gated_dw_kernel<T, BM, BN><<<dim3((unsigned)(cdiv(F, BN) * cdiv(K, BM)), shares, 2), 256, 0, s>>>(
+      x, d, F, (int)p.munits, share, K, dwg, dwu, shares > 1 ? part : nullptr, whole);
   if (shares > 1)
     gated_join_kernel<T><<<dim3(gated_blocks(F * K), 2), 256, 0, s>>>(part, shares, F * K, dwg, dwu);
 }
@@ -441,18 +462,18 @@ extern "C" int tpo_gated_bwd(int dtype, const void* grad_h, const void* x, const
       const Matrix d{ws + p.d, row, M, row};
       T* to = (T*)grad_x;
       switch (p.dx.tile) {
-        case 256: gated_dx<T, 256>(p, d, r[1], r[2], K, to, part, s); break;
-        case 128: gated_dx<T, 128>(p, d, r[1], r[2], K, to, part, s); break;
-        default: gated_dx<T, 64>(p, d, r[1], r[2], K, to, part, s);
+        case LARGE: gated_dx<T, 256, 128>(p, d, r[1], r[2], K, to, part, s); break;
+        case MIDDLE: gated_dx<T, 128, 128>(p, d, r[1], r[2], K, to, part, s); break;
+        case SMALL: gated_dx<T, 64, 64>(p, d, r[1], r[2], K, to, part, s); break;
       }
     }
     if (grad_w_gate && F > 0) {
       const Matrix d{ws + p.d, row, M, row / 2};
       T *g = (T*)grad_w_gate, *u = (T*)grad_w_up;
       switch (p.dw.tile) {
-        case 256: gated_dw<T, 256>(p, r[0], d, F, K, g, u, part, s); break;
-        case 128: gated_dw<T, 128>(p, r[0], d, F, K, g, u, part, s); break;
-        default: gated_dw<T, 64>(p, r[0], d, F, K, g, u, part, s);
+        case LARGE: gated_dw<T, 256, 128>(p, r[0], d, F, K, g, u, part, s); break;
+        case MIDDLE: gated_dw<T, 128, 128>(p, r[0], d, F, K, g, u, part, s); break;
+        case SMALL: gated_dw<T, 64, 64>(p, r[0], d, F, K, g, u, part, s); break;
       }
     }
   });

@@ -7,20 +7,19 @@
 // is on its way from memory, written into LDS by the loads themselves.  An
 // operand comes in either of two layouts, so that no matrix is ever turned
 // round in memory:
-//   by rows (RowLoader): the summed axis contiguous.  A slab's row is eight
-//     chunks of 16 bytes, chunk c at place c ^ (row % 8): the eight lanes of a
-//     16-byte LDS read that go together (eight rows, one chunk) touch all banks
-//     once.
+//   by rows (RowLoader): the summed axis contiguous.  A slab's row is eight (or
+//     four) chunks of 16 bytes, which change places with the row so that the
+//     sixteen lanes of a 16-byte LDS read that go together (sixteen rows, one
+//     chunk) touch all 64 banks once.
 //   by columns (ColLoader): the other axis contiguous, a slab is 64 (32) rows
 //     of BM values.  Half operands are read with the transposing LDS read (four
 //     summed values of one column a lane), float ones value by value; chunks
 //     change places so that the four (two) rows read together lie in different
 //     banks.
 //
-// Per slab a wave reads (BM + BN) / 2 rows of LDS for BM BN / 4 sums: at 256 x
-// 256 the reads and the slab's own write fill 1536 of the 2048 cycles that its
-// matrix instructions take, at 128 x 128 all of them; so the large tile is used
-// wherever there are enough tiles.
+// Measured (rocprofv3, 8192 x 2048 x 8192 gelu): LDS 25 % busy, no bank
+// conflicts to speak of, the matrix cores 50 - 60 % busy at the 1.8 - 1.9 GHz
+// that the card's power leaves at that load.
 #pragma once
 
 #include <type_traits>
@@ -58,7 +57,6 @@ __device__ __forceinline__ void mma(f32x16& acc, f32x4 a, f32x4 b) {
   for (int j = 0; j < 4; ++j) acc = __builtin_amdgcn_mfma_f32_32x32x2f32(a[j], b[j], acc, 0, 0, 0);
 }
 
-constexpr int SLAB = 128;                 // bytes of the summed axis in a slab
 constexpr int NOWHERE = (int)0x80000000;  // beyond every buffer: such a load gives 0
 
 // The loads of `bytes` bytes from p; anything beyond reads as 0.
@@ -77,13 +75,17 @@ struct Matrix {
   int64_t pitch, rows, bytes;
 };
 
-// An operand by rows: R of the matrix's rows.  Wave w loads R / 4 of them, from
-// its own row0 on.  A load covers 8 rows: a lane's place among them is one
-// offset, the rows' and the slab's are scalar; the buffer's bound, checked
-// against the sum of both, ends the rows.
-template <typename T, int R>
+// An operand by rows: R of the matrix's rows, SLAB bytes of each a slab.  Wave w
+// loads R / 4 of them, from its own row0 on.  A load covers 1024 / SLAB rows: a
+// lane's place among them is one offset, the rows' and the slab's are scalar;
+// the buffer's bound, checked against the sum of both, ends the rows.
+template <typename T, int R, int SLAB>
 struct RowLoader {
-  static constexpr int N = R / 32;  // loads a wave
+  static constexpr int CPR = SLAB / 16, RPL = 64 / CPR, N = R / 4 / RPL;
+  // chunk c of row r is at place c ^ swap(r)
+  static __device__ __forceinline__ constexpr int swap(int r) {
+    return SLAB == 128 ? r >> 1 & 7 : r >> 2 & 3;
+  }
   int off, chunk, step, bytes;
   __amdgpu_buffer_rsrc_t rsrc;
 
@@ -92,31 +94,41 @@ struct RowLoader {
     int64_t n = m.rows - row0;
     n = n < 0 ? 0 : (n > R / 4 ? R / 4 : n);
     rsrc = buffer(m.p + (n > 0 ? row0 * m.pitch : 0), (int)(n * m.pitch));
-    chunk = ((l & 7) ^ (l >> 3)) << 4;
-    off = (l >> 3) * (int)m.pitch + chunk;
-    step = 8 * (int)m.pitch;
+    chunk = ((l % CPR) ^ swap(l / CPR)) << 4;  // of the loads from rows 0, 16, ..
+    off = (l / CPR) * (int)m.pitch;
+    step = RPL * (int)m.pitch;
     bytes = (int)m.bytes;
   }
-  __device__ __forceinline__ void load(char* lds, int slab) const {
-    const int w = wave_id(), k = slab * SLAB;
-    const int at = k + chunk < bytes ? off : NOWHERE;
-#pragma unroll
-    for (int j = 0; j < N; ++j) load_lds(rsrc, lds + (w * N + j) * 1024, at, k + j * step);
+  // a slab's loads, one after another
+  struct Slab {
+    __amdgpu_buffer_rsrc_t rsrc;
+    int at[2], k, step;
+    __device__ __forceinline__ void load(char* lds, int j) const {
+      load_lds(rsrc, lds + (wave_id() * N + j) * 1024, at[SLAB == 128 ? j & 1 : 0], k + j * step);
+    }
+  };
+  __device__ __forceinline__ Slab slab(int n) const {
+    const int k = n * SLAB;
+    // (rows 8, 24, ..: with eight rows a load, bit 2 of the places turns)
+    return Slab{rsrc,
+                {k + chunk < bytes ? off + chunk : NOWHERE,
+                 k + (chunk ^ 64) < bytes ? off + (chunk ^ 64) : NOWHERE},
+                k,
+                step};
   }
   // rows row0 + l % 32, chunk 2 s + l / 32 of a slab
   static __device__ __forceinline__ typename Chunk<T>::V read(const char* lds, int row0, int s) {
     const int l = lane_id(), r = l & 31, h = l >> 5;
-    return *(const typename Chunk<T>::V*)(lds + (((2 * s + h) ^ (r & 7)) << 4) +
-                                          (row0 + r) * SLAB);
+    return *(const typename Chunk<T>::V*)(lds + (((2 * s + h) ^ swap(r)) << 4) + (row0 + r) * SLAB);
   }
 };
 
 // An operand by columns: R columns from col0 (a multiple of R / 2) on, the
 // matrix's rows being the summed axis.
-template <typename T, int R>
+template <typename T, int R, int SLAB>
 struct ColLoader {
   static constexpr int Z = sizeof(T), PITCH = R * Z, K = SLAB / Z;
-  static constexpr int N = R / 32;            // loads a wave, 1 KB each
+  static constexpr int N = R * SLAB / 4096;   // loads a wave, 1 KB each
   static constexpr int RPL = 1024 / PITCH;    // rows a load
   static constexpr int CPR = PITCH / 16;      // chunks a row
   // chunk c of row r is at place c ^ swap(r)
@@ -128,7 +140,8 @@ struct ColLoader {
   int off[2], step;
 
   __device__ __forceinline__ ColLoader(const Matrix& m, int64_t col0) {
-    const int l = lane_id(), r = l / CPR, c = (l % CPR) ^ swap(r);
+    const int l = lane_id(), r = l / CPR;
+    const int c = (l % CPR) ^ swap(r) ^ swap(wave_id() * (K / 4));
     p = m.p + col0 * Z;
     pitch = m.pitch;
     rows = m.rows;
@@ -142,17 +155,19 @@ struct ColLoader {
   static __device__ __forceinline__ constexpr int other() {
     return Z == 4 ? 8 : RPL == 2 ? 8 : 0;
   }
-  __device__ __forceinline__ void load(char* lds, int slab) const {
-    load_from(p, (int64_t)slab * K, lds);
-  }
-  __device__ __forceinline__ void load_from(const char* from, int64_t row, char* lds) const {
-    const int w = wave_id();
+  struct Slab {
+    __amdgpu_buffer_rsrc_t rsrc;
+    int off[2], step;
+    __device__ __forceinline__ void load(char* lds, int j) const {
+      const int i = wave_id() * N + j;
+      load_lds(rsrc, lds + i * 1024, off[swap(j * RPL) != 0], i * step);
+    }
+  };
+  __device__ __forceinline__ Slab slab(int n) const { return slab_of(p, (int64_t)n * K); }
+  __device__ __forceinline__ Slab slab_of(const char* from, int64_t row) const {
     int64_t n = rows - row;
     n = n < 0 ? 0 : (n > K ? K : n);
-    const __amdgpu_buffer_rsrc_t rsrc = buffer(from + (n > 0 ? row * pitch : 0), (int)(n * pitch));
-#pragma unroll
-    for (int j = 0; j < N; ++j)
-      load_lds(rsrc, lds + (w * N + j) * 1024, off[swap(j * RPL) != 0], (w * N + j) * step);
+    return Slab{buffer(from + (n > 0 ? row * pitch : 0), (int)(n * pitch)), {off[0], off[1]}, step};
   }
   static __device__ __forceinline__ typename Chunk<T>::V read(const char* lds, int row0, int s) {
     const int l = lane_id();
@@ -182,104 +197,152 @@ struct ColLoader {
 
 // Two matrices by columns, one below the other: slabs from `slabs` on are the
 // second's.
-template <typename T, int R>
+template <typename T, int R, int SLAB>
 struct PairLoader {
-  typedef ColLoader<T, R> L;
+  typedef ColLoader<T, R, SLAB> L;
   static constexpr int N = L::N;
   L one;
   const char* second;
   int slabs;
   __device__ __forceinline__ PairLoader(const Matrix& m, const char* p2, int slabs, int64_t col0)
       : one(m, col0), second(p2 + col0 * sizeof(T)), slabs(slabs) {}
-  __device__ __forceinline__ void load(char* lds, int slab) const {
-    const bool up = slab >= slabs;
-    one.load_from(up ? second : one.p, (int64_t)(up ? slab - slabs : slab) * L::K, lds);
+  __device__ __forceinline__ typename L::Slab slab(int n) const {
+    const bool up = n >= slabs;
+    return one.slab_of(up ? second : one.p, (int64_t)(up ? n - slabs : n) * L::K);
   }
   static __device__ __forceinline__ typename Chunk<T>::V read(const char* lds, int row0, int s) {
     return L::read(lds, row0, s);
   }
 };
 
-// A wave's operands of two chunks (of a slab's eight) of the summed axis.
+// A wave's operands of two chunks of the summed axis.
 template <typename T, typename LA, typename LB, int TM, int TN>
 struct Operands {
   typename Chunk<T>::V x[TM], y[TN];
 
-  // chunks 2 s and 2 s + 1; row0, col0: the wave's first row and column
-  __device__ __forceinline__ void read(const char* a, const char* b, int row0, int col0, int s) {
-#pragma unroll
-    for (int i = 0; i < TM; ++i) x[i] = LA::read(a, row0 + 32 * i, s);
-#pragma unroll
-    for (int j = 0; j < TN; ++j) y[j] = LB::read(b, col0 + 32 * j, s);
-    __builtin_amdgcn_sched_barrier(0);
-  }
-  __device__ __forceinline__ void multiply(f32x16 (&acc)[TM][TN]) const {
-#pragma unroll
-    for (int i = 0; i < TM; ++i)
-#pragma unroll
-      for (int j = 0; j < TN; ++j) mma(acc[i][j], x[i], y[j]);
-    __builtin_amdgcn_sched_barrier(0);
+  // operand i (the columns' first) of chunks 2 s and 2 s + 1; row0, col0: the
+  // wave's first row and column
+  __device__ __forceinline__ void read(const char* a, const char* b, int row0, int col0, int s,
+                                       int i) {
+    if (i < TN)
+      y[i] = LB::read(b, col0 + 32 * i, s);
+    else
+      x[i - TN] = LA::read(a, row0 + 32 * (i - TN), s);
   }
 };
 
-// A slab's products while slab `next` loads into the other half of LDS.
-// Operands are read one step ahead of the products that take them: u holds the
-// slab before's last ones, and this slab's at the end, so that the matrix cores
-// are busy while the first reads of a slab are under way.  (That the halves are
-// apart is what `restrict` says: a read need not wait for the loads into the
-// other one.)
-template <typename T, int BM, typename LA, typename LB, int TM, int TN>
+// A slab's products while another slab loads into a part of LDS that no wave
+// reads.  Operands are read one step ahead of the products that take them: u
+// holds the slab before's last ones, and this slab's at the end, so that the
+// matrix cores are busy while the first reads of a slab are under way.  SPREAD:
+// reads and loads go between the matrix instructions; a wave issues in order,
+// and a row of loads that waits for its turn at the memory pipe keeps its
+// products waiting as well (where other waves' fill in, the row is quicker: 276
+// against 318 us for a product of 275 GFLOP in 128 x 128 tiles).  (That the two parts of LDS are apart is what
+// `restrict` says: a read need not wait for the loads.)
+template <typename T, int BM, int SLAB, bool SPREAD, typename LA, typename LB, int TM, int TN>
 __device__ __forceinline__ void slab_step(const char* __restrict__ cur, char* __restrict__ nxt,
-                                          const LA& la, const LB& lb, int next, bool more,
-                                          int row0, int col0, Operands<T, LA, LB, TM, TN>& u,
+                                          const LA& la, const LB& lb, int next, int row0, int col0,
+                                          Operands<T, LA, LB, TM, TN>& u,
                                           f32x16 (&acc)[TM][TN]) {
+  constexpr int STEPS = SLAB / 32, Q = TM * TN, READS = TM + TN, LOADS = LA::N + LB::N;
   const char* b = cur + BM * SLAB;
+  const auto sa = la.slab(next);
+  const auto sb = lb.slab(next);
   Operands<T, LA, LB, TM, TN> t;
-  if (more) {
-    la.load(nxt, next);
-    lb.load(nxt + BM * SLAB, next);
+#pragma unroll
+  for (int s = 0; s < STEPS; ++s) {
+    Operands<T, LA, LB, TM, TN>& now = s % 2 ? t : u;
+    Operands<T, LA, LB, TM, TN>& then = s % 2 ? u : t;
+    if (!SPREAD) {
+      if (s == 0) {
+#pragma unroll
+        for (int i = 0; i < LA::N; ++i) sa.load(nxt, i);
+#pragma unroll
+        for (int i = 0; i < LB::N; ++i) sb.load(nxt + BM * SLAB, i);
+      }
+#pragma unroll
+      for (int i = 0; i < READS; ++i) then.read(cur, b, row0, col0, s, i);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+#pragma unroll
+    for (int q = 0; q < Q; ++q) {
+      if (SPREAD) {
+#pragma unroll
+        for (int i = q * READS / Q; i < (q + 1) * READS / Q; ++i)
+          then.read(cur, b, row0, col0, s, i);
+#pragma unroll
+        for (int i = (s * Q + q) * LOADS / (STEPS * Q); i < (s * Q + q + 1) * LOADS / (STEPS * Q);
+             ++i)
+          if (i < LA::N)
+            sa.load(nxt, i);
+          else
+            sb.load(nxt + BM * SLAB, i - LA::N);
+      }
+      mma(acc[q / TN][q % TN], now.x[q / TN], now.y[q % TN]);
+      if (SPREAD) __builtin_amdgcn_sched_barrier(0);
+    }
+    if (!SPREAD) __builtin_amdgcn_sched_barrier(0);
   }
-  t.read(cur, b, row0, col0, 0);
-  u.multiply(acc);
-  u.read(cur, b, row0, col0, 1);
-  t.multiply(acc);
-  t.read(cur, b, row0, col0, 2);
-  u.multiply(acc);
-  u.read(cur, b, row0, col0, 3);
-  t.multiply(acc);
 }
 
-template <int BM, int BN>
+// The LDS of a tile: slabs of SLAB bytes of the summed axis, DEPTH of them.
+template <int BM, int BN, int SLAB_, int DEPTH_, bool SPREAD_>
 struct alignas(1024) TileLds {
-  char slab[2][(BM + BN) * SLAB];
+  static constexpr int SLAB = SLAB_, DEPTH = DEPTH_;
+  static constexpr bool SPREAD = SPREAD_;
+  char slab[DEPTH][(BM + BN) * SLAB];
 };
 
+// Waits until at most n of the wave's loads are under way and its LDS reads have
+// ended, then for the workgroup's other waves.
+template <int n>
+__device__ __forceinline__ void wait_loads_and_meet() {
+  __builtin_amdgcn_sched_barrier(0);
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt((n & 15) | (n >> 4) << 14 | 0x70);
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_sched_barrier(0);
+}
+
 // The sums over slabs s0 .. s1 of the summed axis; wave w's quarter begins at
-// row (w / 2) BM / 2, column (w % 2) BN / 2 of the tile.  LDS is free for other
-// use afterwards.
-template <typename T, int BM, int BN, typename LA, typename LB>
-__device__ __forceinline__ void gemm_tile(TileLds<BM, BN>& s, const LA& la, const LB& lb, int s0,
-                                          int s1, f32x16 (&acc)[BM / 64][BN / 64]) {
+// row (w / 2) BM / 2, column (w % 2) BN / 2 of the tile.  Slabs after the last
+// one that are loaded are not used.  LDS is free for other use afterwards.
+template <typename T, int BM, int BN, typename Lds, typename LA, typename LB>
+__device__ __forceinline__ void gemm_tile(Lds& lds, const LA& la, const LB& lb, int s0, int s1,
+                                          f32x16 (&acc)[BM / 64][BN / 64]) {
+  constexpr int SLAB = Lds::SLAB, DEPTH = Lds::DEPTH;
   const int w = wave_id(), row0 = (w >> 1) * (BM / 2), col0 = (w & 1) * (BN / 2);
 #pragma unroll
   for (int i = 0; i < BM / 64; ++i)
 #pragma unroll
     for (int j = 0; j < BN / 64; ++j) acc[i][j] = f32x16{};
   if (s0 >= s1) return;
-  la.load(s.slab[0], s0);
-  lb.load(s.slab[0] + BM * SLAB, s0);
-  Operands<T, LA, LB, BM / 64, BN / 64> u = {};  // nothing before the first slab
-  int half = 0;
-  for (int k = s0; k < s1; ++k) {
-    // every wave's loads of the slab have landed, and every wave's reads of the
-    // other half have ended
-    __builtin_amdgcn_s_waitcnt(0);
-    __syncthreads();
-    slab_step<T, BM>(s.slab[half], s.slab[half ^ 1], la, lb, k + 1, k + 1 < s1, row0, col0, u, acc);
-    half ^= 1;
+#pragma unroll
+  for (int d = 0; d < DEPTH - 1; ++d) {
+    const auto sa = la.slab(s0 + d);
+    const auto sb = lb.slab(s0 + d);
+#pragma unroll
+    for (int j = 0; j < LA::N; ++j) sa.load(lds.slab[d], j);
+#pragma unroll
+    for (int j = 0; j < LB::N; ++j) sb.load(lds.slab[d] + BM * SLAB, j);
   }
-  u.multiply(acc);
-  __syncthreads();
+  Operands<T, LA, LB, BM / 64, BN / 64> u = {};  // nothing before the first slab
+  int at = 0;
+  for (int k = s0; k < s1; ++k) {
+    // the slab has landed (DEPTH - 2 younger ones may be on their way), and every
+    // wave has read the last of the slab before it, whose place is loaded next
+    wait_loads_and_meet<(DEPTH - 2) * (LA::N + LB::N)>();
+    const int free = at == 0 ? DEPTH - 1 : at - 1;
+    slab_step<T, BM, SLAB, Lds::SPREAD>(lds.slab[at], lds.slab[free], la, lb, k + DEPTH - 1, row0, col0, u, acc);
+    at = at + 1 == DEPTH ? 0 : at + 1;
+  }
+#pragma unroll
+  for (int i = 0; i < BM / 64; ++i)
+#pragma unroll
+    for (int j = 0; j < BN / 64; ++j) mma(acc[i][j], u.x[i], u.y[j]);
+  wait_loads_and_meet<0>();
 }
 
 // A wave's way from its sums to rows in memory.  A 32-column tile of sums lies
