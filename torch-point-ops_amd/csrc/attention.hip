@@ -1,155 +1,361 @@
-// attention.hip -- softmax attention over packed sequences, forward and
-// backward, grouped heads.  Sequence by sequence, head by head:
+// attention.hip -- softmax attention over packed sequences with grouped heads,
+// forward.  Sequence by sequence, head by head:
 //   S = scale q k^T (causal: row i sees key j where j <= i + Lk - Lq)
 //   P = softmax(S), o = P v; a row that sees no key is 0
-//   dV = P^T dO, dP = dO V^T, dS = P (dP - sum_d dO O),
-//   dQ = scale dS K, dK = scale dS^T Q
-#include "nn_common.hpp"
+//
+// One pass over the keys with each row's running maximum m and sum l:
+//   m' = max(m, max S), a = exp(m - m'), l' = a l + sum exp(S - m'),
+//   o' = a o + exp(S - m') v.
+// m follows only when it would grow by more than 2^8 (in the exponentials'
+// measure): until then exponentials of up to 2^8 are summed, which costs floats
+// nothing, and most tiles need no pass over the sums o.
+// Half types: probabilities are rounded to the type for the second product (the
+// same relative rounding as the result's); their sum is taken before that.
+#include "attention.hpp"
 
 namespace tpo {
 
-constexpr int AT_DMAX = 128;
+// Keys a tile: what two slabs of k and of v leave room for, twice over.
+template <typename T> constexpr int KEYS = sizeof(T) == 4 ? 32 : 64;
 
-struct AttnArgs {
-  Sequences sq, sk;
-  int64_t q_row, q_head, k_row, k_head, v_row, v_head;  // strides in elements
-  int Hq, Hk, D, causal;
-  float scale;
+// A wave's rows under way.
+template <typename T, int DP>
+struct RowSums {
+  f32x16 acc[DP / 32];
+  float m, l;  // l: of the lane's own keys, half of the row's
+
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int i = 0; i < DP / 32; ++i) acc[i] = f32x16{};
+    m = NEG_INF;
+    l = 0.f;
+  }
+  // KT keys from j0 on, of which the lane's row sees those below n; c: what a
+  // score counts in the exponent of 2
+  template <int KT>
+  __device__ __forceinline__ void add(const char* k, const char* v, const HeadRows<T, DP>& q,
+                                      int j0, int n, bool masked, float c) {
+    f32x16 s[KT / 32];
+#pragma unroll
+    for (int t = 0; t < KT / 32; ++t) s[t] = scores<T, DP>(k, 32 * t, q);
+    if (masked) {
+      const int first = j0 + 4 * (lane_id() >> 5);
+#pragma unroll
+      for (int t = 0; t < KT / 32; ++t)
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          if (first + 32 * t + 8 * (e >> 2) + (e & 3) >= n) s[t][e] = NEG_INF;
+    }
+    float top = s[0][0];
+#pragma unroll
+    for (int t = 0; t < KT / 32; ++t)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) top = fmaxf(top, s[t][e]);
+    top = fmaxf(top, other_half(top));
+    if (__builtin_amdgcn_ballot_w64((top - m) * c > 8.f)) {
+      const float m2 = fmaxf(m, top);
+      const float a = m2 == NEG_INF ? 1.f : __builtin_amdgcn_exp2f((m - m2) * c);
+      m = m2;
+      l *= a;
+#pragma unroll
+      for (int i = 0; i < DP / 32; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[i][e] *= a;
+    }
+    const float b = m == NEG_INF ? 0.f : -m * c;
+#pragma unroll
+    for (int t = 0; t < KT / 32; ++t)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        s[t][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][e], c, b));
+        l += s[t][e];
+      }
+#pragma unroll
+    for (int t = 0; t < KT / 32; ++t) multiply_rows<T, DP>(acc, v, 32 * t, s[t]);
+  }
 };
 
-// The sequence (1 .. B, or 0 and B + 1) that row t belongs to.
-__device__ __forceinline__ int attn_sequence(const Sequences& s, int64_t t) {
-  int lo = 0, hi = s.B + 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (s.start(mid) <= t)
-      lo = mid;
-    else
-      hi = mid - 1;
+// The keys that row r (of the rows of a sequence and key head) sees.
+__device__ __forceinline__ int attn_keys(const AttnArgs& a, const AttnSpan& p, int r, int G) {
+  const int t = r / G;
+  if (!a.causal) return p.Lk;
+  const int n = t + p.Lk - p.Lq + 1;
+  return n < 0 ? 0 : (n > p.Lk ? p.Lk : n);
+}
+
+template <typename T, int DP>
+struct alignas(1024) PromptLds {
+  static constexpr int TILE = KEYS<T> * HeadLds<T, DP>::PITCH;
+  static constexpr int OUT = 4 * 32 * (DP * sizeof(T) + 16);
+  char b[4 * TILE > OUT ? 4 * TILE : OUT];
+};
+
+// The loads of a tile of keys and one's products, in parts of LDS that are apart.
+template <typename T, int DP>
+__device__ __forceinline__ void prompt_step(const char* __restrict__ cur, char* __restrict__ nxt,
+                                            const T* k, const T* v, const AttnArgs& a, int left,
+                                            const HeadRows<T, DP>& q, RowSums<T, DP>& rows, int j0,
+                                            int n, int least, int most, float c) {
+  constexpr int KT = KEYS<T>, TILE = PromptLds<T, DP>::TILE;
+  typedef HeadLds<T, DP> L;
+  L::template load<KT, 4, true>(nxt, k, (int)(a.k_row * sizeof(T)), left, a.D, wave_id());
+  L::template load<KT, 4, false>(nxt + TILE, v, (int)(a.v_row * sizeof(T)), left, a.D, wave_id());
+  __builtin_amdgcn_sched_barrier(0);
+  if (j0 < most) rows.template add<KT>(cur, cur + TILE, q, j0, n, j0 + KT > least, c);
+}
+
+// Prompts: a workgroup of four waves takes 128 rows, 32 a wave, and all their
+// keys in tiles that it loads once for all four.
+template <typename T, int DP>
+__global__ __launch_bounds__(256, 2) void attn_prompt_kernel(AttnArgs a, const T* __restrict__ q,
+                                                             const T* __restrict__ k,
+                                                             const T* __restrict__ v,
+                                                             T* __restrict__ out,
+                                                             float* __restrict__ lse) {
+  constexpr int KT = KEYS<T>, TILE = PromptLds<T, DP>::TILE;
+  __shared__ PromptLds<T, DP> lds;
+  const int G = a.Hq / a.Hk, hk = blockIdx.x % a.Hk;
+  // late tiles of a sequence see the most keys: they go first
+  const int64_t place = gridDim.x / a.Hk - 1 - blockIdx.x / a.Hk;
+  const int s = attn_sequence(a.sq, place, G, 128);
+  const AttnSpan p = attn_span(a, s);
+  const int64_t local = uniform(place - attn_first(a.sq, s, G, 128));
+  const int all = p.room_q * G;
+  if (local < 0 || local * 128 >= all) return;
+  const int w = wave_id(), l = lane_id(), r0 = (int)local * 128 + 32 * w, r = r0 + (l & 31);
+  const int used = p.Lq * G;
+  // the wave's rows see between `least` and `most` keys, the workgroup's up to `end`
+  auto keys = [&](int row) { return used ? attn_keys(a, p, row < used ? row : used - 1, G) : 0; };
+  const int least = keys(r0), most = r0 < used ? keys(r0 + 31) : 0;
+  const int end = (int)local * 128 < used ? keys((int)local * 128 + 127) : 0;
+  const int n = keys(r);
+  const bool in = r < used;
+  const int head = hk * G + r % G;
+  const int64_t token = p.q0 + r / G;
+  HeadRows<T, DP> x;
+  x.load(q + token * a.q_row + head * a.q_head, in, a.D);
+  const float c = fmaxf(fabsf(a.scale) * LOG2E, 1e-37f);  // (0 x -inf is not a number)
+  if (a.scale < 0.f) x.negate();
+  RowSums<T, DP> rows;
+  rows.clear();
+  const T* kt = k + p.k0 * a.k_row + hk * a.k_head;
+  const T* vt = v + p.k0 * a.v_row + hk * a.v_head;
+  typedef HeadLds<T, DP> L;
+  if (end > 0) {
+    L::template load<KT, 4, true>(lds.b, kt, (int)(a.k_row * sizeof(T)), p.Lk, a.D, w);
+    L::template load<KT, 4, false>(lds.b + TILE, vt, (int)(a.v_row * sizeof(T)), p.Lk, a.D, w);
   }
-  return lo;
-}
-
-template <typename T>
-__device__ __forceinline__ void attn_load(const T* p, int D, float (&x)[2]) {
-  const int l = lane_id();
-  x[0] = l < D ? (float)p[l] : 0.f;
-  x[1] = l + 64 < D ? (float)p[l + 64] : 0.f;
-}
-template <typename T>
-__device__ __forceinline__ void attn_store(T* p, int D, const float (&x)[2]) {
-  const int l = lane_id();
-  if (l < D) p[l] = (T)x[0];
-  if (l + 64 < D) p[l + 64] = (T)x[1];
-}
-__device__ __forceinline__ float attn_dot(const float (&a)[2], const float (&b)[2]) {
-  return wave_sum(a[0] * b[0] + a[1] * b[1]);
-}
-
-// One wave a query row and head.
-template <typename T>
-__global__ __launch_bounds__(256) void attn_fwd_kernel(AttnArgs a, const T* __restrict__ q,
-                                                       const T* __restrict__ k,
-                                                       const T* __restrict__ v, T* __restrict__ o,
-                                                       float* __restrict__ lse) {
-  const int64_t w = (int64_t)blockIdx.x * 4 + wave_id();
-  const int64_t t = w / a.Hq;
-  const int h = (int)(w % a.Hq);
-  if (t >= a.sq.T) return;
-  const int s = attn_sequence(a.sq, t);
-  const int64_t Lq = a.sq.used(s), Lk = a.sk.used(s), i = t - a.sq.start(s), k0 = a.sk.start(s);
-  int64_t n = i < Lq ? Lk : 0;
-  if (a.causal && i + Lk - Lq + 1 < n) n = i + Lk - Lq + 1;
-  const int hk = h / (a.Hq / a.Hk);
-  float x[2], y[2], acc[2] = {0.f, 0.f}, m = -__builtin_inff(), l = 0.f;
-  attn_load(q + t * a.q_row + h * a.q_head, a.D, x);
-  for (int64_t j = 0; j < n; ++j) {
-    attn_load(k + (k0 + j) * a.k_row + hk * a.k_head, a.D, y);
-    const float e = attn_dot(x, y) * a.scale;
-    const float top = fmaxf(m, e);
-    const float c = top == -__builtin_inff() ? 1.f : expf(m - top);
-    const float p = top == -__builtin_inff() ? 0.f : expf(e - top);
-    attn_load(v + (k0 + j) * a.v_row + hk * a.v_head, a.D, y);
-    l = l * c + p;
-    acc[0] = acc[0] * c + p * y[0];
-    acc[1] = acc[1] * c + p * y[1];
-    m = top;
+  int half = 0;
+  for (int j0 = 0; j0 < end; j0 += KT) {
+    wait_loads_and_meet<0>();
+    kt += KT * a.k_row;
+    vt += KT * a.v_row;
+    prompt_step<T, DP>(lds.b + half * 2 * TILE, lds.b + (half ^ 1) * 2 * TILE, kt, vt, a,
+                       j0 + KT < end ? p.Lk - j0 - KT : 0, x, rows, j0, n, least, most, c);
+    half ^= 1;
   }
-  const float r = l == 0.f ? 0.f : 1.f / l;
-  acc[0] *= r;
-  acc[1] *= r;
-  attn_store(o + (t * a.Hq + h) * a.D, a.D, acc);
-  if (lse && lane_id() == 0) lse[h * a.sq.T + t] = l == 0.f ? -__builtin_inff() : m + logf(l);
-}
+  wait_loads_and_meet<0>();
+  if (r0 >= all) return;
 
-// dQ: one wave a query row and head.
-template <typename T>
-__global__ __launch_bounds__(256) void attn_bwd_q_kernel(
-    AttnArgs a, const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ v,
-    const T* __restrict__ o, const T* __restrict__ go, const float* __restrict__ lse,
-    float* __restrict__ delta, T* __restrict__ gq) {
-  const int64_t w = (int64_t)blockIdx.x * 4 + wave_id();
-  const int64_t t = w / a.Hq;
-  const int h = (int)(w % a.Hq);
-  if (t >= a.sq.T) return;
-  const int s = attn_sequence(a.sq, t);
-  const int64_t Lq = a.sq.used(s), Lk = a.sk.used(s), i = t - a.sq.start(s), k0 = a.sk.start(s);
-  int64_t n = i < Lq ? Lk : 0;
-  if (a.causal && i + Lk - Lq + 1 < n) n = i + Lk - Lq + 1;
-  const int hk = h / (a.Hq / a.Hk);
-  const float m = lse[h * a.sq.T + t];
-  if (m == -__builtin_inff()) n = 0;
-  float x[2], y[2], z[2], g[2], acc[2] = {0.f, 0.f};
-  attn_load(o + (t * a.Hq + h) * a.D, a.D, x);
-  attn_load(go + (t * a.Hq + h) * a.D, a.D, g);
-  const float d = n > 0 ? attn_dot(x, g) : 0.f;
-  if (lane_id() == 0) delta[h * a.sq.T + t] = d;
-  attn_load(q + t * a.q_row + h * a.q_head, a.D, x);
-  for (int64_t j = 0; j < n; ++j) {
-    attn_load(k + (k0 + j) * a.k_row + hk * a.k_head, a.D, y);
-    attn_load(v + (k0 + j) * a.v_row + hk * a.v_head, a.D, z);
-    const float p = expf(attn_dot(x, y) * a.scale - m);
-    const float e = p * (attn_dot(g, z) - d) * a.scale;
-    acc[0] += e * y[0];
-    acc[1] += e * y[1];
-  }
-  attn_store(gq + (t * a.Hq + h) * a.D, a.D, acc);
-}
-
-// dK and dV: one wave a key row and key head.
-template <typename T>
-__global__ __launch_bounds__(256) void attn_bwd_kv_kernel(
-    AttnArgs a, const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ v,
-    const T* __restrict__ go, const float* __restrict__ lse, const float* __restrict__ delta,
-    T* __restrict__ gk, T* __restrict__ gv) {
-  const int64_t w = (int64_t)blockIdx.x * 4 + wave_id();
-  const int64_t t = w / a.Hk;
-  const int hk = (int)(w % a.Hk);
-  if (t >= a.sk.T) return;
-  const int s = attn_sequence(a.sk, t);
-  const int64_t Lq = a.sq.used(s), Lk = a.sk.used(s), j = t - a.sk.start(s), q0 = a.sq.start(s);
-  const int64_t n = j < Lk ? Lq : 0;
-  const int64_t first = a.causal && j - (Lk - Lq) > 0 ? j - (Lk - Lq) : 0;
-  const int G = a.Hq / a.Hk;
-  float x[2], y[2], z[2], g[2], ak[2] = {0.f, 0.f}, av[2] = {0.f, 0.f};
-  attn_load(k + t * a.k_row + hk * a.k_head, a.D, y);
-  attn_load(v + t * a.v_row + hk * a.v_head, a.D, z);
-  for (int h = hk * G; h < hk * G + G; ++h)
-    for (int64_t i = first; i < n; ++i) {
-      const int64_t r = q0 + i;
-      const float m = lse[h * a.sq.T + r];
-      if (m == -__builtin_inff()) continue;
-      attn_load(q + r * a.q_row + h * a.q_head, a.D, x);
-      attn_load(go + (r * a.Hq + h) * a.D, a.D, g);
-      const float p = expf(attn_dot(x, y) * a.scale - m);
-      const float e = p * (attn_dot(g, z) - delta[h * a.sq.T + r]) * a.scale;
-      ak[0] += e * x[0];
-      ak[1] += e * x[1];
-      av[0] += p * g[0];
-      av[1] += p * g[1];
+  const float sum = rows.l + other_half(rows.l);
+  const float inv = in && sum != 0.f ? 1.f / sum : 0.f;
+  typedef Rows32<T, DP> R;
+  const R to{lds.b + w * R::BYTES};
+#pragma unroll
+  for (int i = 0; i < DP / 32; ++i)
+#pragma unroll
+    for (int b = 0; b < 4; ++b) {
+      Four<T> f;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) f.v[e] = inv == 0.f ? (T)0.f : (T)(rows.acc[i][4 * b + e] * inv);
+      *(Four<T>*)to.four(32 * i + 8 * b + 4 * (l >> 5)) = f;
     }
-  attn_store(gk + (t * a.Hk + hk) * a.D, a.D, ak);
-  attn_store(gv + (t * a.Hk + hk) * a.D, a.D, av);
+  to.wait();
+#pragma unroll
+  for (int i = 0; i < 32 * R::CHUNKS; i += 64) {
+    const int rr = (i + l) / R::CHUNKS, cc = (i + l) % R::CHUNKS * R::PER, row = r0 + rr;
+    if (row < all && cc < a.D)
+      *(f32x4*)(out + ((p.q0 + row / G) * a.Hq + hk * G + row % G) * a.D + cc) =
+          *(const f32x4*)((const T*)(to.lds + rr * R::PITCH) + cc);
+  }
+  if (lse && l < 32 && r < all)
+    lse[head * a.sq.T + token] =
+        inv == 0.f ? NEG_INF : (rows.m * c + __builtin_amdgcn_logf(sum)) * LN2;
+}
+
+// Few rows over many keys: a workgroup takes 32 rows and one of gridDim.z shares
+// of their keys, its W waves in turn a tile of 32 keys each from LDS of their own,
+// so that no wave waits for another before the end.
+template <typename T, int DP> constexpr int STEP_WAVES = sizeof(T) == 4 && DP > 64 ? 2 : 4;
+template <typename T, int DP>
+struct alignas(1024) StepLds {
+  static constexpr int TILE = 32 * HeadLds<T, DP>::PITCH;
+  static constexpr int SUMS = STEP_WAVES<T, DP> * 32 * (DP + 4) * 4;
+  static constexpr int TILES = STEP_WAVES<T, DP> * 4 * TILE;
+  char b[TILES > SUMS ? TILES : SUMS];
+  float m[STEP_WAVES<T, DP>][32], l[STEP_WAVES<T, DP>][32];
+};
+
+template <typename T, int DP>
+__device__ __forceinline__ void step_load(char* to, const T* k, const T* v, const AttnArgs& a,
+                                          int left) {
+  typedef HeadLds<T, DP> L;
+  L::template load<32, 1, true>(to, k, (int)(a.k_row * sizeof(T)), left, a.D, 0);
+  L::template load<32, 1, false>(to + StepLds<T, DP>::TILE, v, (int)(a.v_row * sizeof(T)), left,
+                                 a.D, 0);
+}
+template <typename T, int DP>
+__device__ __forceinline__ void step_step(const char* __restrict__ cur, char* __restrict__ nxt,
+                                          const T* k, const T* v, const AttnArgs& a, int left,
+                                          const HeadRows<T, DP>& q, RowSums<T, DP>& rows, int j0,
+                                          int n, int least, float c) {
+  constexpr int TILE = StepLds<T, DP>::TILE, N = 2 * TILE / 1024;  // loads a tile
+  step_load<T, DP>(nxt, k, v, a, left);
+  __builtin_amdgcn_sched_barrier(0);
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt((N & 15) | (N >> 4) << 14 | 0xf70);  // the tile itself has landed
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_sched_barrier(0);
+  rows.template add<32>(cur, cur + TILE, q, j0, n, j0 + 32 > least, c);
+}
+
+// part: with shares, each row's sums (D floats, not divided), and in ml their
+// maximum (in the exponent of 2) and sum
+template <typename T, int DP>
+__global__ __launch_bounds__((64 * STEP_WAVES<T, DP>)) void attn_step_kernel(
+    AttnArgs a, const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ v,
+    T* __restrict__ out, float* __restrict__ lse, float* __restrict__ part,
+    float2* __restrict__ ml) {
+  constexpr int W = STEP_WAVES<T, DP>, TILE = StepLds<T, DP>::TILE;
+  __shared__ StepLds<T, DP> lds;
+  const int G = a.Hq / a.Hk, hk = blockIdx.y, shares = gridDim.z;
+  const int64_t place = blockIdx.x;
+  const int s = attn_sequence(a.sq, place, G, 32);
+  const AttnSpan p = attn_span(a, s);
+  const int64_t local = uniform(place - attn_first(a.sq, s, G, 32));
+  const int all = p.room_q * G;
+  if (local < 0 || local * 32 >= all) return;
+  const int w = wave_id(), l = lane_id(), r0 = (int)local * 32, r = r0 + (l & 31);
+  const int used = p.Lq * G;
+  auto keys = [&](int row) { return used ? attn_keys(a, p, row < used ? row : used - 1, G) : 0; };
+  const int least = keys(r0), most = r0 < used ? keys(r0 + 31) : 0;
+  const int n = keys(r);
+  const int tiles = (most + 31) / 32, per = (tiles + shares - 1) / shares;
+  const int t0 = per * blockIdx.z, t1 = t0 + per < tiles ? t0 + per : tiles;
+  const int head = hk * G + r % G;
+  HeadRows<T, DP> x;
+  x.load(q + (p.q0 + r / G) * a.q_row + head * a.q_head, r < used, a.D);
+  const float c = fmaxf(fabsf(a.scale) * LOG2E, 1e-37f);
+  if (a.scale < 0.f) x.negate();
+  RowSums<T, DP> rows;
+  rows.clear();
+  const T* kt = k + p.k0 * a.k_row + hk * a.k_head;
+  const T* vt = v + p.k0 * a.v_row + hk * a.v_head;
+  char* mine = lds.b + w * 4 * TILE;
+  auto load = [&](int t) {
+    step_load<T, DP>(mine, kt + (int64_t)t * 32 * a.k_row, vt + (int64_t)t * 32 * a.v_row, a,
+                     t < t1 ? most - t * 32 : 0);
+  };
+  if (t0 + w < t1) load(t0 + w);
+  int half = 0;
+  for (int t = t0 + w; t < t1; t += W) {
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0xc07f);  // the other tile's reads have ended
+    const int64_t next = t + W;
+    step_step<T, DP>(mine + half * 2 * TILE, mine + (half ^ 1) * 2 * TILE,
+                     kt + next * 32 * a.k_row, vt + next * 32 * a.v_row, a,
+                     next < t1 ? most - (int)next * 32 : 0, x, rows, t * 32, n, least, c);
+    half ^= 1;
+  }
+  wait_loads_and_meet<0>();
+
+  // the waves' sums together
+  const float sum = rows.l + other_half(rows.l);
+  constexpr int P = DP + 4;
+  float* mysums = (float*)lds.b + w * 32 * P;
+#pragma unroll
+  for (int i = 0; i < DP / 32; ++i)
+#pragma unroll
+    for (int b = 0; b < 4; ++b) {
+      Four<float> f;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) f.v[e] = rows.acc[i][4 * b + e];
+      *(Four<float>*)(mysums + (l & 31) * P + 32 * i + 8 * b + 4 * (l >> 5)) = f;
+    }
+  if (l < 32) {
+    lds.m[w][l] = rows.m;
+    lds.l[w][l] = sum;
+  }
+  __syncthreads();
+  constexpr int PER_ROW = 2 * W, D1 = DP / PER_ROW;  // lanes a row, values a lane
+  const int rr = threadIdx.x / PER_ROW, d0 = threadIdx.x % PER_ROW * D1, row = r0 + rr;
+  if (row >= all) return;
+  float m = NEG_INF, total = 0.f, f[W];
+#pragma unroll
+  for (int i = 0; i < W; ++i) m = fmaxf(m, lds.m[i][rr]);
+#pragma unroll
+  for (int i = 0; i < W; ++i) {
+    const float y = lds.l[i][rr];
+    f[i] = y == 0.f ? 0.f : __builtin_amdgcn_exp2f((lds.m[i][rr] - m) * c);
+    total += f[i] * y;
+  }
+  if (row >= used) total = 0.f;
+  const int64_t at = (p.q0 + row / G) * a.Hq + hk * G + row % G;
+  const float inv = shares > 1 ? 1.f : total != 0.f ? 1.f / total : 0.f;
+#pragma unroll
+  for (int d = 0; d < D1; ++d) {
+    float y = 0.f;
+#pragma unroll
+    for (int i = 0; i < W; ++i)
+      if (f[i] != 0.f) y += f[i] * ((float*)lds.b)[(i * 32 + rr) * P + d0 + d];
+    if (d0 + d < a.D) {
+      if (shares > 1) {
+        if (total != 0.f) part[(at * shares + blockIdx.z) * a.D + d0 + d] = y;
+      } else {
+        out[at * a.D + d0 + d] = total == 0.f ? (T)0.f : (T)(y * inv);
+      }
+    }
+  }
+  if (d0 == 0) {
+    if (shares > 1)
+      ml[at * shares + blockIdx.z] = make_float2(m * c, total);
+    else if (lse)
+      lse[(at % a.Hq) * a.sq.T + at / a.Hq] =
+          total == 0.f ? NEG_INF : (m * c + __builtin_amdgcn_logf(total)) * LN2;
+  }
+}
+
+// The shares' sums of each row together: one wave a row.
+template <typename T>
+__global__ __launch_bounds__(256) void attn_join_kernel(const float* __restrict__ part,
+                                                        const float2* __restrict__ ml, int shares,
+                                                        int64_t rows, int Hq, int64_t Tq, int D,
+                                                        T* __restrict__ out,
+                                                        float* __restrict__ lse) {
+  const int64_t at = (int64_t)blockIdx.x * 4 + wave_id();
+  if (at >= rows) return;
+  const int l = lane_id();
+  float m = NEG_INF;
+  for (int i = 0; i < shares; ++i) {
+    const float2 y = ml[at * shares + i];
+    if (y.y != 0.f) m = fmaxf(m, y.x);
+  }
+  float total = 0.f, o[2] = {0.f, 0.f};
+  for (int i = 0; i < shares; ++i) {
+    const float2 y = ml[at * shares + i];
+    if (y.y == 0.f) continue;
+    const float f = __builtin_amdgcn_exp2f(y.x - m);
+    total += f * y.y;
+    const float* p = part + (at * shares + i) * D;
+    if (l < D) o[0] += f * p[l];
+    if (l + 64 < D) o[1] += f * p[l + 64];
+  }
+  const float inv = total != 0.f ? 1.f / total : 0.f;
+  if (l < D) out[at * D + l] = (T)(o[0] * inv);
+  if (l + 64 < D) out[at * D + l + 64] = (T)(o[1] * inv);
+  if (lse && l == 0)
+    lse[(at % Hq) * Tq + at / Hq] = total == 0.f ? NEG_INF : (m + __builtin_amdgcn_logf(total)) * LN2;
 }
 
 int attn_check(const char* op, int dtype, int64_t B, int64_t Tq, int64_t Tk, int64_t Hq,
@@ -158,13 +364,29 @@ int attn_check(const char* op, int dtype, int64_t B, int64_t Tq, int64_t Tk, int
     return set_error(TPO_ERR_DTYPE, "%s: unsupported dtype %d", op, dtype);
   if (B < 0 || B > (1 << 24) || Tq < 0 || Tk < 0 || Tq >= ((int64_t)1 << 31) ||
       Tk >= ((int64_t)1 << 31) || Hq < 1 || Hk < 1 || Hq > 1024 || Hq % Hk != 0 || D < 1 ||
-      D > AT_DMAX)
+      D > AT_DMAX || Tq * Hq >= ((int64_t)1 << 31) || Tk * Hk >= ((int64_t)1 << 31))
     return set_error(TPO_ERR_ARG,
                      "%s: bad sizes B=%lld Tq=%lld Tk=%lld Hq=%lld Hk=%lld D=%lld (Hq a multiple "
                      "of Hk, D at most %d)",
                      op, (long long)B, (long long)Tq, (long long)Tk, (long long)Hq, (long long)Hk,
                      (long long)D, AT_DMAX);
   return TPO_OK;
+}
+
+// Pointers and strides that the kernels can load 16 bytes at a time, 64 rows of
+// an operand spanning less than 2^31 bytes.
+int attn_layout(const char* op, int dtype, int64_t D, std::initializer_list<const void*> ptrs,
+                std::initializer_list<int64_t> strides, std::initializer_list<int64_t> rows) {
+  const int64_t z = element_bytes(dtype);
+  bool ok = D * z % 16 == 0;
+  for (const void* p : ptrs) ok = ok && ((uintptr_t)p & 15) == 0;
+  for (int64_t s : strides) ok = ok && s >= 0 && s * z % 16 == 0;
+  for (int64_t s : rows) ok = ok && s > 0 && s * z < (1 << 25);
+  return ok ? TPO_OK
+            : set_error(TPO_ERR_ARG,
+                        "%s: pointers, heads and strides must be multiples of 16 bytes, rows apart "
+                        "by 16 to 2^25 bytes",
+                        op);
 }
 
 AttnArgs attn_args(const int64_t* oq, const int64_t* ok, const int64_t* lq, const int64_t* lk,
@@ -188,6 +410,29 @@ AttnArgs attn_args(const int64_t* oq, const int64_t* ok, const int64_t* lq, cons
   return a;
 }
 
+
+// Which kernel a call takes, and the shares of the keys.  Up to 64 rows a
+// sequence and key head on average are few: with a workgroup's 128 rows most
+// lanes would idle.  Shares: enough workgroups for two a CU, but 512 keys or more
+// in each (by the room for keys: what is in use is not known here).
+struct Way {
+  bool step;
+  int shares;
+};
+Way attn_way(int64_t B, int64_t Tq, int64_t Tk, int64_t Hq, int64_t Hk) {
+  Way w{false, 1};
+  const int64_t G = Hq / Hk, n = B < 1 ? 1 : B;
+  w.step = Tq * G <= 64 * n;
+  if (w.step) {
+    const int64_t blocks = (Tq * G / 32 > n ? Tq * G / 32 : n) * Hk;
+    int64_t s = (1024 + blocks - 1) / blocks;
+    if (s > Tk / n / 512) s = Tk / n / 512;
+    if (s > 64) s = 64;
+    w.shares = s < 1 ? 1 : (int)s;
+  }
+  return w;
+}
+
 }  // namespace tpo
 
 using namespace tpo;
@@ -195,7 +440,9 @@ using namespace tpo;
 extern "C" int64_t tpo_attention_fwd_workspace_size(int dtype, int64_t B, int64_t Tq, int64_t Tk,
                                                     int64_t Hq, int64_t Hk, int64_t D) {
   if (attn_check("attention_fwd_workspace_size", dtype, B, Tq, Tk, Hq, Hk, D)) return -1;
-  return 0;
+  const Way w = attn_way(B, Tq, Tk, Hq, Hk);
+  if (w.shares == 1) return 0;
+  return round_up(Tq * Hq * w.shares * D * 4, 256) + round_up(Tq * Hq * w.shares * 8, 256);
 }
 
 extern "C" int tpo_attention_fwd(int dtype, const void* q, const void* k, const void* v,
@@ -207,53 +454,38 @@ extern "C" int tpo_attention_fwd(int dtype, const void* q, const void* k, const 
                                  void* out, float* lse, void* workspace, int64_t workspace_bytes,
                                  void* stream) {
   if (int rc = attn_check("attention_fwd", dtype, B, Tq, Tk, Hq, Hk, D)) return rc;
-  (void)workspace;
-  (void)workspace_bytes;
   if (Tq == 0) return TPO_OK;
-  const AttnArgs a = attn_args(offsets_q, offsets_k, lengths_q, lengths_k, B, Tq, Tk, Hq, Hk, D,
-                               q_row, q_head, k_row, k_head, v_row, v_head, causal, scale);
-  with_element(dtype, [&](auto t) {
-    typedef decltype(t) T;
-    attn_fwd_kernel<T><<<dim3((unsigned)((Tq * Hq + 3) / 4)), 256, 0, (hipStream_t)stream>>>(
-        a, (const T*)q, (const T*)k, (const T*)v, (T*)out, lse);
-  });
-  return check_launch("attention_fwd");
-}
-
-extern "C" int64_t tpo_attention_bwd_workspace_size(int dtype, int64_t B, int64_t Tq, int64_t Tk,
-                                                    int64_t Hq, int64_t Hk, int64_t D) {
-  if (attn_check("attention_bwd_workspace_size", dtype, B, Tq, Tk, Hq, Hk, D)) return -1;
-  return round_up(Tq * Hq * 4, 256);
-}
-
-extern "C" int tpo_attention_bwd(int dtype, const void* grad_out, const void* q, const void* k,
-                                 const void* v, const void* out, const float* lse,
-                                 const int64_t* offsets_q, const int64_t* offsets_k,
-                                 const int64_t* lengths_q, const int64_t* lengths_k, int64_t B,
-                                 int64_t Tq, int64_t Tk, int64_t Hq, int64_t Hk, int64_t D,
-                                 int64_t q_row, int64_t q_head, int64_t k_row, int64_t k_head,
-                                 int64_t v_row, int64_t v_head, int causal, double scale,
-                                 void* grad_q, void* grad_k, void* grad_v, void* workspace,
-                                 int64_t workspace_bytes, void* stream) {
-  if (int rc = attn_check("attention_bwd", dtype, B, Tq, Tk, Hq, Hk, D)) return rc;
-  const int64_t need = tpo_attention_bwd_workspace_size(dtype, B, Tq, Tk, Hq, Hk, D);
+  if (int rc = attn_layout("attention_fwd", dtype, D, {q, k, v, out, workspace},
+                           {q_row, q_head, k_row, k_head, v_row, v_head}, {q_row, k_row, v_row}))
+    return rc;
+  const int64_t need = tpo_attention_fwd_workspace_size(dtype, B, Tq, Tk, Hq, Hk, D);
   if (need > 0 && (!workspace || workspace_bytes < need))
-    return set_error(TPO_ERR_WORKSPACE, "attention_bwd: workspace of %lld bytes needed",
+    return set_error(TPO_ERR_WORKSPACE, "attention_fwd: workspace of %lld bytes needed",
                      (long long)need);
   const AttnArgs a = attn_args(offsets_q, offsets_k, lengths_q, lengths_k, B, Tq, Tk, Hq, Hk, D,
                                q_row, q_head, k_row, k_head, v_row, v_head, causal, scale);
-  float* delta = (float*)workspace;
+  const Way w = attn_way(B, Tq, Tk, Hq, Hk);
+  const int64_t G = Hq / Hk, places = attn_places(Tq, G, B, w.step ? 32 : 128);
+  if (places * Hk >= ((int64_t)1 << 31) || Hk > 65535)
+    return set_error(TPO_ERR_ARG, "attention_fwd: too many rows");
   hipStream_t s = (hipStream_t)stream;
+  float* part = (float*)workspace;
+  float2* ml = (float2*)((char*)workspace + round_up(Tq * Hq * w.shares * D * 4, 256));
   with_element(dtype, [&](auto t) {
     typedef decltype(t) T;
-    if (Tq > 0)
-      attn_bwd_q_kernel<T><<<dim3((unsigned)((Tq * Hq + 3) / 4)), 256, 0, s>>>(
-          a, (const T*)q, (const T*)k, (const T*)v, (const T*)out, (const T*)grad_out, lse, delta,
-          (T*)grad_q);
-    if (Tk > 0)
-      attn_bwd_kv_kernel<T><<<dim3((unsigned)((Tk * Hk + 3) / 4)), 256, 0, s>>>(
-          a, (const T*)q, (const T*)k, (const T*)v, (const T*)grad_out, lse, delta, (T*)grad_k,
-          (T*)grad_v);
+    with_head(D, [&](auto dp) {
+      constexpr int DP = decltype(dp)::value;
+      if (!w.step)
+        attn_prompt_kernel<T, DP><<<dim3((unsigned)(places * Hk)), 256, 0, s>>>(
+            a, (const T*)q, (const T*)k, (const T*)v, (T*)out, lse);
+      else
+        attn_step_kernel<T, DP>
+            <<<dim3((unsigned)places, (unsigned)Hk, w.shares), 64 * STEP_WAVES<T, DP>, 0, s>>>(
+                a, (const T*)q, (const T*)k, (const T*)v, (T*)out, lse, part, ml);
+    });
+    if (w.shares > 1)
+      attn_join_kernel<T><<<dim3((unsigned)((Tq * Hq + 3) / 4)), 256, 0, s>>>(
+          part, ml, w.shares, Tq * Hq, (int)Hq, Tq, (int)D, (T*)out, lse);
   });
-  return check_launch("attention_bwd");
+  return check_launch("attention_fwd");
 }

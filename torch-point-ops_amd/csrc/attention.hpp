@@ -1,0 +1,219 @@
+// attention.hpp -- what the attention kernels share: arguments, the way from a
+// workgroup's number to its rows, and the products of one tile of keys.
+//
+// The rows of a sequence and key head are its queries of all G = Hq / Hk heads of
+// the group, row r = token r / G, head r % G, so that the group shares what is
+// read of k and v, also where a sequence has a single query.
+//
+// A wave works on 32 rows.  Scores are computed transposed, S^T = K Q^T: a lane
+// then has one row (column l % 32 of the product), and of every 32 keys the
+// sixteen 8 (v / 4) + 4 (l / 32) + v % 4.  Its row's maximum and sum need one
+// exchange with the lane 32 on, and the probabilities are already what the
+// second product O^T = V^T P^T takes, if v is read in the same order of keys.
+#pragma once
+
+#include "gemm_tile.hpp"
+
+namespace tpo {
+
+constexpr int AT_DMAX = 128;
+constexpr float LOG2E = 1.44269504088896341f;
+constexpr float LN2 = 0.69314718055994531f;
+#define NEG_INF (-__builtin_inff())
+
+struct AttnArgs {
+  Sequences sq, sk;
+  int64_t q_row, q_head, k_row, k_head, v_row, v_head;  // strides in elements
+  int Hq, Hk, D, causal;
+  float scale;
+};
+
+// The rows of a packed batch in tiles of `tile`: sequence s begins at tile
+// start(s) G / tile + s.  That leaves room for each sequence's tiles (the last
+// one of a sequence and the first of the next may meet in one place, hence + s)
+// without a sum over the sequences before it; some places stay empty.
+inline int64_t attn_places(int64_t T, int64_t G, int64_t B, int tile) { return T * G / tile + B + 2; }
+__device__ __forceinline__ int64_t attn_first(const Sequences& s, int i, int G, int tile) {
+  return s.start(i) * G / tile + i;
+}
+// The last sequence that begins at or before a place: 64 guesses a step.
+__device__ __forceinline__ int attn_sequence(const Sequences& s, int64_t place, int G, int tile) {
+  int lo = 0, n = s.B + 2;  // among lo .. lo + n - 1
+  while (n > 1) {
+    const int step = (n + 63) >> 6, i = lo + lane_id() * step;
+    const bool at = i < lo + n && attn_first(s, i, G, tile) <= place;
+    const uint64_t m = __builtin_amdgcn_ballot_w64(at);
+    const int top = m ? 63 - __builtin_clzll(m) : 0;
+    const int rest = n - top * step;
+    lo += top * step;
+    n = rest < step ? rest : step;
+  }
+  return __builtin_amdgcn_readfirstlane(lo);
+}
+
+// 64-bit values that all lanes share
+__device__ __forceinline__ int64_t uniform(int64_t v) {
+  const uint32_t lo = __builtin_amdgcn_readfirstlane((int)(uint32_t)v);
+  const uint32_t hi = __builtin_amdgcn_readfirstlane((int)(uint32_t)((uint64_t)v >> 32));
+  return (int64_t)((uint64_t)hi << 32 | lo);
+}
+
+// A workgroup's sequence: its queries and keys, and where they begin.
+struct AttnSpan {
+  int64_t q0, k0;       // first rows in the packed arrays
+  int room_q, Lq, Lk;   // query rows (with those not in use), queries and keys in use
+  int room_k;
+};
+__device__ __forceinline__ AttnSpan attn_span(const AttnArgs& a, int s) {
+  AttnSpan p;
+  p.q0 = uniform(a.sq.start(s));
+  p.k0 = uniform(a.sk.start(s));
+  p.room_q = (int)uniform(a.sq.room(s));
+  p.room_k = (int)uniform(a.sk.room(s));
+  p.Lq = (int)uniform(a.sq.used(s));
+  p.Lk = (int)uniform(a.sk.used(s));
+  return p;
+}
+
+// The value of lane l ^ 32
+__device__ __forceinline__ float other_half(float v) { return __shfl_xor(v, 32); }
+
+// How rows of up to DP values lie in LDS.
+template <typename T, int DP>
+struct HeadLds {
+  static constexpr int Z = sizeof(T);
+  static constexpr int PITCH = DP * Z <= 64 ? 64 : DP * Z <= 128 ? 128 : DP * Z <= 256 ? 256 : 512;
+  static constexpr int CPR = PITCH / 16, RPL = 1024 / PITCH;
+  // places of the 16-byte chunks: c ^ swap(row).  Rows are read either sixteen
+  // rows, one chunk at a time (BY_ROW: k, by the products that sum over the
+  // head) or four rows, 64 bytes (v, by those that sum over the keys; floats: two
+  // rows four apart, 128 bytes).
+  template <bool BY_ROW>
+  static __device__ __forceinline__ constexpr int swap(int r) {
+    if (BY_ROW) return PITCH == 64 ? r >> 2 & 3 : PITCH == 128 ? r >> 1 & 7 : r & 15;
+    if (Z == 4) return PITCH >= 256 ? (r >> 2 & 1) << 3 : 0;
+    return PITCH == 64 ? 0 : PITCH == 128 ? (r >> 1 & 1) << 2 : (r & 3) << 2;
+  }
+  // Loads `R` rows into lds, by NW waves of which this is w: the first n rows
+  // from p on, row_bytes apart, D values of each; the rest is 0.
+  template <int R, int NW, bool BY_ROW>
+  static __device__ __forceinline__ void load(char* lds, const T* p, int row_bytes, int n, int D,
+                                              int w) {
+    constexpr int N = R / RPL / NW;
+    static_assert(N >= 1 && N * RPL * NW == R, "rows of a tile");
+    n = n < 0 ? 0 : (n > R ? R : n);
+    const __amdgpu_buffer_rsrc_t rsrc = buffer(p, n * row_bytes);
+    const int l = lane_id(), r = l / CPR, bytes = D * Z;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const int row = (w * N + j) * RPL;  // a multiple of RPL: its part of swap() is apart
+      const int c = ((l % CPR) ^ swap<BY_ROW>(r) ^ swap<BY_ROW>(row)) << 4;
+      load_lds(rsrc, lds + (w * N + j) * 1024, c < bytes ? r * row_bytes + c : NOWHERE,
+               row * row_bytes);
+    }
+  }
+  // rows row0 + l % 32, chunk 2 s + l / 32
+  static __device__ __forceinline__ typename Chunk<T>::V by_row(const char* lds, int row0, int s) {
+    const int l = lane_id(), r = l & 31;
+    return *(const typename Chunk<T>::V*)(lds + (row0 + r) * PITCH +
+                                          (((2 * s + (l >> 5)) ^ swap<true>(r)) << 4));
+  }
+  // half types: value 32 i + l % 32 of the rows row0 + 16 s + 4 (l / 32) + 0 .. 3
+  // and + 8 .. 11
+  static __device__ __forceinline__ typename Chunk<T>::V by_col(const char* lds, int row0, int s,
+                                                                int i) {
+    static_assert(Z == 2, "half types");
+    typedef __attribute__((address_space(3))) i16x4 lds_i16x4;
+    const int l = lane_id(), e = l & 15, g = (l >> 4) & 1, h = l >> 5, q = e >> 2;
+    const char* at =
+        lds + ((row0 + 16 * s + 4 * h + q) * PITCH + (swap<false>(q) << 4) + 32 * g + 8 * (e & 3));
+    const int a0 = (int)(uintptr_t)(lds_t*)at ^ (64 * i);
+    const i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(uintptr_t)a0);
+    const i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(uintptr_t)(a0 + 8 * PITCH));
+    return __builtin_bit_cast(typename Chunk<T>::V,
+                              __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+  }
+  // float: value 32 i + l % 32 of row row0 + 8 (v / 4) + 4 (l / 32) + v % 4
+  static __device__ __forceinline__ float by_col1(const char* lds, int row0, int v, int i) {
+    const int l = lane_id(), r = row0 + 8 * (v >> 2) + 4 * (l >> 5) + (v & 3);
+    const int c = (8 * i + ((l & 31) >> 2)) ^ swap<false>(r);
+    return *(const float*)(lds + r * PITCH + (c << 4) + (l & 3) * 4);
+  }
+};
+
+// acc[i] += X^T P^T over 32 rows of X (in LDS by column) from row0 on: sums of
+// value 32 i + .. of X times the lane's sixteen p.  Half types round p to the type.
+template <typename T, int DP>
+__device__ __forceinline__ void multiply_rows(f32x16 (&acc)[DP / 32], const char* lds, int row0,
+                                              const f32x16& p) {
+  typedef HeadLds<T, DP> L;
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int v = 0; v < 16; ++v)
+#pragma unroll
+      for (int i = 0; i < DP / 32; ++i)
+        acc[i] = __builtin_amdgcn_mfma_f32_32x32x2f32(L::by_col1(lds, row0, v, i), p[v], acc[i], 0,
+                                                      0, 0);
+  } else {
+    typedef typename Chunk<T>::V V;
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      V x;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = (T)p[8 * s + e];
+#pragma unroll
+      for (int i = 0; i < DP / 32; ++i) mma(acc[i], L::by_col(lds, row0, s, i), x);
+    }
+  }
+}
+
+// A wave's 32 rows of q (or of another array laid out as it) as the products
+// take them, chunk 2 s + l / 32 of row l % 32; 0 where there is no row.
+template <typename T, int DP>
+struct HeadRows {
+  static constexpr int N = DP * sizeof(T) / 32;
+  typename Chunk<T>::V x[N];
+  __device__ __forceinline__ void load(const T* p, bool in, int D) {
+    constexpr int PER = 16 / sizeof(T);
+    const int h = lane_id() >> 5;
+#pragma unroll
+    for (int s = 0; s < N; ++s) {
+      x[s] = typename Chunk<T>::V{};
+      if (in && (2 * s + h) * PER < D) x[s] = *(const typename Chunk<T>::V*)(p + (2 * s + h) * PER);
+    }
+  }
+  __device__ __forceinline__ void negate() {
+#pragma unroll
+    for (int s = 0; s < N; ++s) x[s] = -x[s];
+  }
+};
+
+// X Y^T of 32 rows of X in LDS and the wave's rows: the transposed scores.
+template <typename T, int DP>
+__device__ __forceinline__ f32x16 scores(const char* lds, int row0, const HeadRows<T, DP>& y) {
+  f32x16 s = {};
+#pragma unroll
+  for (int c = 0; c < HeadRows<T, DP>::N; ++c)
+    mma(s, HeadLds<T, DP>::by_row(lds, row0, c), y.x[c]);
+  return s;
+}
+
+int attn_check(const char* op, int dtype, int64_t B, int64_t Tq, int64_t Tk, int64_t Hq,
+               int64_t Hk, int64_t D);
+int attn_layout(const char* op, int dtype, int64_t D, std::initializer_list<const void*> p,
+                std::initializer_list<int64_t> strides, std::initializer_list<int64_t> rows);
+AttnArgs attn_args(const int64_t* oq, const int64_t* ok, const int64_t* lq, const int64_t* lk,
+                   int64_t B, int64_t Tq, int64_t Tk, int64_t Hq, int64_t Hk, int64_t D,
+                   int64_t q_row, int64_t q_head, int64_t k_row, int64_t k_head, int64_t v_row,
+                   int64_t v_head, int causal, double scale);
+
+// Calls f with the head size rounded up to one that the kernels are built for.
+template <typename F>
+void with_head(int64_t D, F&& f) {
+  if (D <= 32) f(std::integral_constant<int, 32>());
+  else if (D <= 64) f(std::integral_constant<int, 64>());
+  else if (D <= 96) f(std::integral_constant<int, 96>());
+  else f(std::integral_constant<int, 128>());
+}
+
+}  // namespace tpo

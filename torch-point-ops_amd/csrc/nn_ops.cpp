@@ -174,14 +174,23 @@ Tensor layer_norm_autograd(const Tensor& x, const OptTensor& w, const OptTensor&
 // --------------------------------------------------------- packed attention
 struct Packed {  // checked arguments of an attention call
   Tensor q, k, v, oq, ok, lq, lk;
-  int64_t B, Tq, Tk, Hq, Hk, D;
+  int64_t B, Tq, Tk, Hq, Hk, D;  // D padded to 16 bytes
   int dt;
 };
 
-// q, k and v may be slices (of one projection, say): a head's values lie
-// together, rows and heads at any distance.
-Tensor head_rows(const Tensor& t) {
-  return t.size(2) <= 1 || t.stride(2) == 1 ? t : t.contiguous();
+// The distance of rows and of heads, also where there is one of them only.
+int64_t row_stride(const Tensor& t) { return t.size(0) > 1 ? t.stride(0) : t.size(1) * t.size(2); }
+int64_t head_stride(const Tensor& t) { return t.size(1) > 1 ? t.stride(1) : t.size(2); }
+
+// q, k and v may be slices (of one projection, say) or broadcast over heads: a
+// head's values lie together, rows and heads at any distance that keeps 16-byte
+// loads.  Others are copied, heads that are no multiple of 16 bytes padded.
+Tensor head_rows(const Tensor& t, int64_t D) {
+  const int64_t z = t.element_size();
+  if (t.size(2) != D) return at::constant_pad_nd(t, {0, D - t.size(2)}).contiguous();
+  const bool ok = (D == 1 || t.stride(2) == 1) && row_stride(t) > 0 && row_stride(t) * z % 16 == 0 &&
+                  row_stride(t) * z < (1 << 25) && head_stride(t) * z % 16 == 0;
+  return aligned16(ok ? t : t.contiguous());
 }
 
 Packed packed_args(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& oq,
@@ -214,9 +223,12 @@ Packed packed_args(const Tensor& q, const Tensor& k, const Tensor& v, const Tens
     TORCH_CHECK(!t.defined() ||
                     (t.scalar_type() == at::kLong && t.dim() == 1 && t.size(0) == p.B),
                 op, ": lengths must be int64 with one entry a sequence");
-  p.q = head_rows(q);
-  p.k = head_rows(k);
-  p.v = head_rows(v);
+  TORCH_CHECK(q.size(2) > 0, op, ": the heads of q are empty");
+  const int64_t per = 16 / q.element_size();
+  p.D = (q.size(2) + per - 1) / per * per;
+  p.q = head_rows(q, p.D);
+  p.k = head_rows(k, p.D);
+  p.v = head_rows(v, p.D);
   p.oq = oq.contiguous();
   p.ok = ok.contiguous();
   if (p.lq.defined()) p.lq = p.lq.contiguous();
@@ -225,8 +237,12 @@ Packed packed_args(const Tensor& q, const Tensor& k, const Tensor& v, const Tens
   p.Tk = k.size(0);
   p.Hq = q.size(1);
   p.Hk = k.size(1);
-  p.D = q.size(2);
   return p;
+}
+
+// The first D values of each head of a result.
+Tensor cut_heads(const Tensor& t, int64_t D) {
+  return t.size(2) == D ? t : t.narrow(2, 0, D).contiguous();
 }
 
 std::tuple<Tensor, Tensor> packed_attention_hip(const Tensor& q, const Tensor& k, const Tensor& v,
@@ -243,12 +259,12 @@ std::tuple<Tensor, Tensor> packed_attention_hip(const Tensor& q, const Tensor& k
   check_rc(tpo_attention_fwd(p.dt, p.q.data_ptr(), p.k.data_ptr(), p.v.data_ptr(),
                              p.oq.data_ptr<int64_t>(), p.ok.data_ptr<int64_t>(),
                              (const int64_t*)data_or_null(p.lq), (const int64_t*)data_or_null(p.lk),
-                             p.B, p.Tq, p.Tk, p.Hq, p.Hk, p.D, p.q.stride(0), p.q.stride(1),
-                             p.k.stride(0), p.k.stride(1), p.v.stride(0), p.v.stride(1), causal,
-                             scale, out.data_ptr(), (float*)data_or_null(lse), data_or_null(ws),
+                             p.B, p.Tq, p.Tk, p.Hq, p.Hk, p.D, row_stride(p.q), head_stride(p.q),
+                             row_stride(p.k), head_stride(p.k), row_stride(p.v), head_stride(p.v),
+                             causal, scale, out.data_ptr(), (float*)data_or_null(lse), data_or_null(ws),
                              wsb, stream_of(q)),
            op);
-  return {out, lse};
+  return {cut_heads(out, q.size(2)), lse};
 }
 
 Tensor packed_attention_only_hip(const Tensor& q, const Tensor& k, const Tensor& v,
@@ -278,7 +294,8 @@ std::tuple<Tensor, Tensor, Tensor> packed_attention_backward_hip(
               "packed_attention_backward: out and lse must be the forward's");
   for (const Tensor& t : {grad_in, out_in, lse_in})
     TORCH_CHECK(t.device() == q.device(), op, ": all tensors must be on the same device");
-  const Tensor g = grad_in.to(q.scalar_type()).contiguous(), out = out_in.contiguous();
+  const Tensor g = head_rows(grad_in.to(q.scalar_type()).contiguous(), p.D);
+  const Tensor out = head_rows(out_in.contiguous(), p.D);
   const Tensor lse = lse_in.contiguous();
   Tensor gq = at::empty({p.Tq, p.Hq, p.D}, q.options());
   Tensor gk = at::empty({p.Tk, p.Hk, p.D}, q.options());
@@ -289,11 +306,12 @@ std::tuple<Tensor, Tensor, Tensor> packed_attention_backward_hip(
                              out.data_ptr(), lse.data_ptr<float>(), p.oq.data_ptr<int64_t>(),
                              p.ok.data_ptr<int64_t>(), (const int64_t*)data_or_null(p.lq),
                              (const int64_t*)data_or_null(p.lk), p.B, p.Tq, p.Tk, p.Hq, p.Hk, p.D,
-                             p.q.stride(0), p.q.stride(1), p.k.stride(0), p.k.stride(1),
-                             p.v.stride(0), p.v.stride(1), causal, scale, gq.data_ptr(),
+                             row_stride(p.q), head_stride(p.q), row_stride(p.k), head_stride(p.k),
+                             row_stride(p.v), head_stride(p.v), causal, scale, gq.data_ptr(),
                              gk.data_ptr(), gv.data_ptr(), data_or_null(ws), wsb, stream_of(q)),
            op);
-  return {gq, gk, gv};
+  const int64_t D = q.size(2);
+  return {cut_heads(gq, D), cut_heads(gk, D), cut_heads(gv, D)};
 }
 
 auto packed_attention_op() {
