@@ -15,9 +15,6 @@
 
 namespace tpo {
 
-// Keys a tile: what two slabs of k and of v leave room for, twice over.
-template <typename T> constexpr int KEYS = sizeof(T) == 4 ? 32 : 64;
-
 // A wave's rows under way.
 template <typename T, int DP>
 struct RowSums {
@@ -75,21 +72,6 @@ struct RowSums {
   }
 };
 
-// The keys that row r (of the rows of a sequence and key head) sees.
-__device__ __forceinline__ int attn_keys(const AttnArgs& a, const AttnSpan& p, int r, int G) {
-  const int t = r / G;
-  if (!a.causal) return p.Lk;
-  const int n = t + p.Lk - p.Lq + 1;
-  return n < 0 ? 0 : (n > p.Lk ? p.Lk : n);
-}
-
-template <typename T, int DP>
-struct alignas(1024) PromptLds {
-  static constexpr int TILE = KEYS<T> * HeadLds<T, DP>::PITCH;
-  static constexpr int OUT = 4 * 32 * (DP * sizeof(T) + 16);
-  char b[4 * TILE > OUT ? 4 * TILE : OUT];
-};
-
 // The loads of a tile of keys and one's products, in parts of LDS that are apart.
 template <typename T, int DP>
 __device__ __forceinline__ void prompt_step(const char* __restrict__ cur, char* __restrict__ nxt,
@@ -98,8 +80,8 @@ __device__ __forceinline__ void prompt_step(const char* __restrict__ cur, char* 
                                             int n, int least, int most, float c) {
   constexpr int KT = KEYS<T>, TILE = PromptLds<T, DP>::TILE;
   typedef HeadLds<T, DP> L;
-  L::template load<KT, 4, true>(nxt, k, (int)(a.k_row * sizeof(T)), left, a.D, wave_id());
-  L::template load<KT, 4, false>(nxt + TILE, v, (int)(a.v_row * sizeof(T)), left, a.D, wave_id());
+  L::template load<KT, 4>(nxt, k, (int)(a.k_row * sizeof(T)), left, a.D, wave_id());
+  L::template load<KT, 4>(nxt + TILE, v, (int)(a.v_row * sizeof(T)), left, a.D, wave_id());
   __builtin_amdgcn_sched_barrier(0);
   if (j0 < most) rows.template add<KT>(cur, cur + TILE, q, j0, n, j0 + KT > least, c);
 }
@@ -134,7 +116,7 @@ __global__ __launch_bounds__(256, 2) void attn_prompt_kernel(AttnArgs a, const T
   const int64_t token = p.q0 + r / G;
   HeadRows<T, DP> x;
   x.load(q + token * a.q_row + head * a.q_head, in, a.D);
-  const float c = fmaxf(fabsf(a.scale) * LOG2E, 1e-37f);  // (0 x -inf is not a number)
+  const float c = attn_count(a.scale);
   if (a.scale < 0.f) x.negate();
   RowSums<T, DP> rows;
   rows.clear();
@@ -142,8 +124,8 @@ __global__ __launch_bounds__(256, 2) void attn_prompt_kernel(AttnArgs a, const T
   const T* vt = v + p.k0 * a.v_row + hk * a.v_head;
   typedef HeadLds<T, DP> L;
   if (end > 0) {
-    L::template load<KT, 4, true>(lds.b, kt, (int)(a.k_row * sizeof(T)), p.Lk, a.D, w);
-    L::template load<KT, 4, false>(lds.b + TILE, vt, (int)(a.v_row * sizeof(T)), p.Lk, a.D, w);
+    L::template load<KT, 4>(lds.b, kt, (int)(a.k_row * sizeof(T)), p.Lk, a.D, w);
+    L::template load<KT, 4>(lds.b + TILE, vt, (int)(a.v_row * sizeof(T)), p.Lk, a.D, w);
   }
   int half = 0;
   for (int j0 = 0; j0 < end; j0 += KT) {
@@ -159,25 +141,7 @@ __global__ __launch_bounds__(256, 2) void attn_prompt_kernel(AttnArgs a, const T
 
   const float sum = rows.l + other_half(rows.l);
   const float inv = in && sum != 0.f ? 1.f / sum : 0.f;
-  typedef Rows32<T, DP> R;
-  const R to{lds.b + w * R::BYTES};
-#pragma unroll
-  for (int i = 0; i < DP / 32; ++i)
-#pragma unroll
-    for (int b = 0; b < 4; ++b) {
-      Four<T> f;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) f.v[e] = inv == 0.f ? (T)0.f : (T)(rows.acc[i][4 * b + e] * inv);
-      *(Four<T>*)to.four(32 * i + 8 * b + 4 * (l >> 5)) = f;
-    }
-  to.wait();
-#pragma unroll
-  for (int i = 0; i < 32 * R::CHUNKS; i += 64) {
-    const int rr = (i + l) / R::CHUNKS, cc = (i + l) % R::CHUNKS * R::PER, row = r0 + rr;
-    if (row < all && cc < a.D)
-      *(f32x4*)(out + ((p.q0 + row / G) * a.Hq + hk * G + row % G) * a.D + cc) =
-          *(const f32x4*)((const T*)(to.lds + rr * R::PITCH) + cc);
-  }
+  put_rows<T, DP>(lds.b, rows.acc, inv, out, a, p, hk, r0, all);
   if (lse && l < 32 && r < all)
     lse[head * a.sq.T + token] =
         inv == 0.f ? NEG_INF : (rows.m * c + __builtin_amdgcn_logf(sum)) * LN2;
@@ -200,8 +164,8 @@ template <typename T, int DP>
 __device__ __forceinline__ void step_load(char* to, const T* k, const T* v, const AttnArgs& a,
                                           int left) {
   typedef HeadLds<T, DP> L;
-  L::template load<32, 1, true>(to, k, (int)(a.k_row * sizeof(T)), left, a.D, 0);
-  L::template load<32, 1, false>(to + StepLds<T, DP>::TILE, v, (int)(a.v_row * sizeof(T)), left,
+  L::template load<32, 1>(to, k, (int)(a.k_row * sizeof(T)), left, a.D, 0);
+  L::template load<32, 1>(to + StepLds<T, DP>::TILE, v, (int)(a.v_row * sizeof(T)), left,
                                  a.D, 0);
 }
 template <typename T, int DP>
@@ -245,7 +209,7 @@ __global__ __launch_bounds__((64 * STEP_WAVES<T, DP>)) void attn_step_kernel(
   const int head = hk * G + r % G;
   HeadRows<T, DP> x;
   x.load(q + (p.q0 + r / G) * a.q_row + head * a.q_head, r < used, a.D);
-  const float c = fmaxf(fabsf(a.scale) * LOG2E, 1e-37f);
+  const float c = attn_count(a.scale);
   if (a.scale < 0.f) x.negate();
   RowSums<T, DP> rows;
   rows.clear();

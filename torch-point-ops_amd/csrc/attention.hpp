@@ -84,19 +84,18 @@ struct HeadLds {
   static constexpr int Z = sizeof(T);
   static constexpr int PITCH = DP * Z <= 64 ? 64 : DP * Z <= 128 ? 128 : DP * Z <= 256 ? 256 : 512;
   static constexpr int CPR = PITCH / 16, RPL = 1024 / PITCH;
-  // places of the 16-byte chunks: c ^ swap(row).  Rows are read either sixteen
-  // rows, one chunk at a time (BY_ROW: k, by the products that sum over the
-  // head) or four rows, 64 bytes (v, by those that sum over the keys; floats: two
-  // rows four apart, 128 bytes).
-  template <bool BY_ROW>
+  // Chunk c of a row is at place c ^ swap(row), so that both ways of reading touch
+  // different banks: sixteen rows, one chunk (for products that sum over the head),
+  // and four rows, 64 bytes (for those that sum over the rows; floats: two rows
+  // four apart, 128 bytes, but where a row is no longer than that).
   static __device__ __forceinline__ constexpr int swap(int r) {
-    if (BY_ROW) return PITCH == 64 ? r >> 2 & 3 : PITCH == 128 ? r >> 1 & 7 : r & 15;
-    if (Z == 4) return PITCH >= 256 ? (r >> 2 & 1) << 3 : 0;
-    return PITCH == 64 ? 0 : PITCH == 128 ? (r >> 1 & 1) << 2 : (r & 3) << 2;
+    if (PITCH == 64) return r >> 2 & 3;
+    if (Z == 4) return PITCH == 128 ? r >> 1 & 7 : (r >> 2 & 1) << 3 | (r >> 3 & 1) << 2 | (r & 3);
+    return PITCH == 128 ? (r >> 1 & 1) << 2 | (r >> 2 & 3) : (r & 3) << 2 | (r >> 2 & 3);
   }
   // Loads `R` rows into lds, by NW waves of which this is w: the first n rows
   // from p on, row_bytes apart, D values of each; the rest is 0.
-  template <int R, int NW, bool BY_ROW>
+  template <int R, int NW>
   static __device__ __forceinline__ void load(char* lds, const T* p, int row_bytes, int n, int D,
                                               int w) {
     constexpr int N = R / RPL / NW;
@@ -107,7 +106,7 @@ struct HeadLds {
 #pragma unroll
     for (int j = 0; j < N; ++j) {
       const int row = (w * N + j) * RPL;  // a multiple of RPL: its part of swap() is apart
-      const int c = ((l % CPR) ^ swap<BY_ROW>(r) ^ swap<BY_ROW>(row)) << 4;
+      const int c = ((l % CPR) ^ swap(r) ^ swap(row)) << 4;
       load_lds(rsrc, lds + (w * N + j) * 1024, c < bytes ? r * row_bytes + c : NOWHERE,
                row * row_bytes);
     }
@@ -116,7 +115,7 @@ struct HeadLds {
   static __device__ __forceinline__ typename Chunk<T>::V by_row(const char* lds, int row0, int s) {
     const int l = lane_id(), r = l & 31;
     return *(const typename Chunk<T>::V*)(lds + (row0 + r) * PITCH +
-                                          (((2 * s + (l >> 5)) ^ swap<true>(r)) << 4));
+                                          (((2 * s + (l >> 5)) ^ swap(r)) << 4));
   }
   // half types: value 32 i + l % 32 of the rows row0 + 16 s + 4 (l / 32) + 0 .. 3
   // and + 8 .. 11
@@ -125,18 +124,20 @@ struct HeadLds {
     static_assert(Z == 2, "half types");
     typedef __attribute__((address_space(3))) i16x4 lds_i16x4;
     const int l = lane_id(), e = l & 15, g = (l >> 4) & 1, h = l >> 5, q = e >> 2;
-    const char* at =
-        lds + ((row0 + 16 * s + 4 * h + q) * PITCH + (swap<false>(q) << 4) + 32 * g + 8 * (e & 3));
-    const int a0 = (int)(uintptr_t)(lds_t*)at ^ (64 * i);
+    const int r = 4 * h + q, c = 2 * g + (e >> 1 & 1);
+    const char* at = lds + ((row0 + 16 * s + r) * PITCH + 8 * (e & 1));
+    const int base = (int)(uintptr_t)(lds_t*)at;
+    const int a0 = base + (((c ^ swap(r)) << 4) ^ (64 * i));
+    const int a1 = base + 8 * PITCH + (((c ^ swap(r + 8)) << 4) ^ (64 * i));
     const i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(uintptr_t)a0);
-    const i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(uintptr_t)(a0 + 8 * PITCH));
+    const i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(uintptr_t)a1);
     return __builtin_bit_cast(typename Chunk<T>::V,
                               __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
   }
   // float: value 32 i + l % 32 of row row0 + 8 (v / 4) + 4 (l / 32) + v % 4
   static __device__ __forceinline__ float by_col1(const char* lds, int row0, int v, int i) {
     const int l = lane_id(), r = row0 + 8 * (v >> 2) + 4 * (l >> 5) + (v & 3);
-    const int c = (8 * i + ((l & 31) >> 2)) ^ swap<false>(r);
+    const int c = (8 * i + ((l & 31) >> 2)) ^ swap(r);
     return *(const float*)(lds + r * PITCH + (c << 4) + (l & 3) * 4);
   }
 };
@@ -186,6 +187,58 @@ struct HeadRows {
 #pragma unroll
     for (int s = 0; s < N; ++s) x[s] = -x[s];
   }
+};
+
+// A wave's 32 rows of sums, f times each, to the rows r0 .. of a sequence and key
+// head in an array laid out as out (f 0: nothing but zeros), by way of LDS.
+template <typename T, int DP>
+__device__ __forceinline__ void put_rows(char* lds, const f32x16 (&acc)[DP / 32], float f,
+                                         T* __restrict__ out, const AttnArgs& a, const AttnSpan& p,
+                                         int hk, int r0, int all) {
+  typedef Rows32<T, DP> R;
+  const R to{lds + wave_id() * R::BYTES};
+  const int l = lane_id(), G = a.Hq / a.Hk;
+#pragma unroll
+  for (int i = 0; i < DP / 32; ++i)
+#pragma unroll
+    for (int b = 0; b < 4; ++b) {
+      Four<T> y;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) y.v[e] = f == 0.f ? (T)0.f : (T)(acc[i][4 * b + e] * f);
+      *(Four<T>*)to.four(32 * i + 8 * b + 4 * (l >> 5)) = y;
+    }
+  to.wait();
+#pragma unroll
+  for (int i = 0; i < 32 * R::CHUNKS; i += 64) {
+    const int rr = (i + l) / R::CHUNKS, cc = (i + l) % R::CHUNKS * R::PER, row = r0 + rr;
+    if (row < all && cc < a.D)
+      *(f32x4*)(out + ((p.q0 + row / G) * a.Hq + hk * G + row % G) * a.D + cc) =
+          *(const f32x4*)((const T*)(to.lds + rr * R::PITCH) + cc);
+  }
+}
+
+// The keys that row r (of the rows of a sequence and key head) sees.
+__device__ __forceinline__ int attn_keys(const AttnArgs& a, const AttnSpan& p, int r, int G) {
+  const int t = r / G;
+  if (!a.causal) return p.Lk;
+  const int n = t + p.Lk - p.Lq + 1;
+  return n < 0 ? 0 : (n > p.Lk ? p.Lk : n);
+}
+
+// What a score counts in the exponent of 2; never 0, as 0 x -inf is not a number.
+// A negative scale turns the sign of one operand instead.
+__device__ __forceinline__ float attn_count(float scale) {
+  return fmaxf(fabsf(scale) * LOG2E, 1e-37f);
+}
+
+// Keys (or rows) a tile in LDS: what two operands' tiles leave room for, twice over.
+template <typename T> constexpr int KEYS = sizeof(T) == 4 ? 32 : 64;
+
+template <typename T, int DP>
+struct alignas(1024) PromptLds {
+  static constexpr int TILE = KEYS<T> * HeadLds<T, DP>::PITCH;
+  static constexpr int OUT = 4 * Rows32<T, DP>::BYTES;
+  char b[4 * TILE > OUT ? 4 * TILE : OUT];
 };
 
 // X Y^T of 32 rows of X in LDS and the wave's rows: the transposed scores.

@@ -1,107 +1,286 @@
 // attention_bwd.hip -- backward of softmax attention over packed sequences.
 //   dV = P^T dO, dP = dO V^T, dS = P (dP - sum_d dO O),
 //   dQ = scale dS K, dK = scale dS^T Q
+// P comes from the scores again and the forward's logarithms of the rows' sums.
+// Two kernels, so that every sum has one owner and a fixed order: one holds rows
+// and passes over their keys (dQ), one holds keys and passes over the rows that
+// see them (dK, dV).  The scores and dP are computed in both: 7 products where 5
+// with atomic sums for dQ would do, but the results are the same on every run.
+// A row that sees a single key has dS = 0 (its probability is 1 whatever the
+// score): dP and delta, which are sums in different orders, would leave their
+// rounding there, so it is said outright.
+// Half types: P and dS are rounded to the type for the products that take them.
 #include "attention.hpp"
 
 namespace tpo {
 
-// The sequence (1 .. B, or 0 and B + 1) that row t belongs to.
-__device__ __forceinline__ int attn_row_sequence(const Sequences& s, int64_t t) {
-  int lo = 0, hi = s.B + 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (s.start(mid) <= t)
-      lo = mid;
-    else
-      hi = mid - 1;
+// Of each row: what is subtracted in the exponent of 2 (the logarithm of its sum;
+// infinity where the row sees no key, which makes its P 0), and delta =
+// sum_d dO O.  Sixteen lanes a row.
+template <typename T>
+__global__ __launch_bounds__(256) void attn_delta_kernel(const T* __restrict__ o,
+                                                         const T* __restrict__ go,
+                                                         const float* __restrict__ lse,
+                                                         int64_t rows, int Hq, int64_t Tq, int D,
+                                                         float* __restrict__ sub,
+                                                         float* __restrict__ delta) {
+  const int64_t r = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
+  if (r >= rows) return;
+  constexpr int PER = 16 / sizeof(T);
+  typedef typename Chunk<T>::V V;
+  float s = 0.f;
+  for (int c = (threadIdx.x & 15) * PER; c < D; c += 16 * PER) {
+    const V x = *(const V*)(o + r * D + c), y = *(const V*)(go + r * D + c);
+#pragma unroll
+    for (int e = 0; e < PER; ++e) s = __builtin_fmaf((float)x[e], (float)y[e], s);
   }
-  return lo;
-}
-
-template <typename T>
-__device__ __forceinline__ void attn_load(const T* p, int D, float (&x)[2]) {
-  const int l = lane_id();
-  x[0] = l < D ? (float)p[l] : 0.f;
-  x[1] = l + 64 < D ? (float)p[l + 64] : 0.f;
-}
-template <typename T>
-__device__ __forceinline__ void attn_store(T* p, int D, const float (&x)[2]) {
-  const int l = lane_id();
-  if (l < D) p[l] = (T)x[0];
-  if (l + 64 < D) p[l + 64] = (T)x[1];
-}
-__device__ __forceinline__ float attn_dot(const float (&a)[2], const float (&b)[2]) {
-  return wave_sum(a[0] * b[0] + a[1] * b[1]);
-}
-
-// dQ: one wave a query row and head.
-template <typename T>
-__global__ __launch_bounds__(256) void attn_bwd_q_kernel(
-    AttnArgs a, const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ v,
-    const T* __restrict__ o, const T* __restrict__ go, const float* __restrict__ lse,
-    float* __restrict__ delta, T* __restrict__ gq) {
-  const int64_t w = (int64_t)blockIdx.x * 4 + wave_id();
-  const int64_t t = w / a.Hq;
-  const int h = (int)(w % a.Hq);
-  if (t >= a.sq.T) return;
-  const int s = attn_row_sequence(a.sq, t);
-  const int64_t Lq = a.sq.used(s), Lk = a.sk.used(s), i = t - a.sq.start(s), k0 = a.sk.start(s);
-  int64_t n = i < Lq ? Lk : 0;
-  if (a.causal && i + Lk - Lq + 1 < n) n = i + Lk - Lq + 1;
-  const int hk = h / (a.Hq / a.Hk);
-  const float m = lse[h * a.sq.T + t];
-  if (m == -__builtin_inff()) n = 0;
-  float x[2], y[2], z[2], g[2], acc[2] = {0.f, 0.f};
-  attn_load(o + (t * a.Hq + h) * a.D, a.D, x);
-  attn_load(go + (t * a.Hq + h) * a.D, a.D, g);
-  const float d = n > 0 ? attn_dot(x, g) : 0.f;
-  if (lane_id() == 0) delta[h * a.sq.T + t] = d;
-  attn_load(q + t * a.q_row + h * a.q_head, a.D, x);
-  for (int64_t j = 0; j < n; ++j) {
-    attn_load(k + (k0 + j) * a.k_row + hk * a.k_head, a.D, y);
-    attn_load(v + (k0 + j) * a.v_row + hk * a.v_head, a.D, z);
-    const float p = expf(attn_dot(x, y) * a.scale - m);
-    const float e = p * (attn_dot(g, z) - d) * a.scale;
-    acc[0] += e * y[0];
-    acc[1] += e * y[1];
+#pragma unroll
+  for (int d = 8; d > 0; d >>= 1) s += __shfl_xor(s, d);
+  if ((threadIdx.x & 15) == 0) {
+    const int64_t at = r % Hq * Tq + r / Hq;
+    const float m = lse[at];
+    sub[at] = m == NEG_INF ? -NEG_INF : m * LOG2E;
+    delta[at] = m == NEG_INF ? 0.f : s;
   }
-  attn_store(gq + (t * a.Hq + h) * a.D, a.D, acc);
 }
 
-// dK and dV: one wave a key row and key head.
-template <typename T>
-__global__ __launch_bounds__(256) void attn_bwd_kv_kernel(
-    AttnArgs a, const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ v,
-    const T* __restrict__ go, const float* __restrict__ lse, const float* __restrict__ delta,
-    T* __restrict__ gk, T* __restrict__ gv) {
-  const int64_t w = (int64_t)blockIdx.x * 4 + wave_id();
-  const int64_t t = w / a.Hk;
-  const int hk = (int)(w % a.Hk);
-  if (t >= a.sk.T) return;
-  const int s = attn_row_sequence(a.sk, t);
-  const int64_t Lq = a.sq.used(s), Lk = a.sk.used(s), j = t - a.sk.start(s), q0 = a.sq.start(s);
-  const int64_t n = j < Lk ? Lq : 0;
-  const int64_t first = a.causal && j - (Lk - Lq) > 0 ? j - (Lk - Lq) : 0;
-  const int G = a.Hq / a.Hk;
-  float x[2], y[2], z[2], g[2], ak[2] = {0.f, 0.f}, av[2] = {0.f, 0.f};
-  attn_load(k + t * a.k_row + hk * a.k_head, a.D, y);
-  attn_load(v + t * a.v_row + hk * a.v_head, a.D, z);
-  for (int h = hk * G; h < hk * G + G; ++h)
-    for (int64_t i = first; i < n; ++i) {
-      const int64_t r = q0 + i;
-      const float m = lse[h * a.sq.T + r];
-      if (m == -__builtin_inff()) continue;
-      attn_load(q + r * a.q_row + h * a.q_head, a.D, x);
-      attn_load(go + (r * a.Hq + h) * a.D, a.D, g);
-      const float p = expf(attn_dot(x, y) * a.scale - m);
-      const float e = p * (attn_dot(g, z) - delta[h * a.sq.T + r]) * a.scale;
-      ak[0] += e * x[0];
-      ak[1] += e * x[1];
-      av[0] += p * g[0];
-      av[1] += p * g[1];
+template <typename T, int DP>
+__device__ __forceinline__ void bwd_q_step(const char* __restrict__ cur, char* __restrict__ nxt,
+                                           const T* k, const T* v, const AttnArgs& a, int left,
+                                           const HeadRows<T, DP>& q, const HeadRows<T, DP>& go,
+                                           f32x16 (&acc)[DP / 32], int j0, int n, int least,
+                                           int most, float c, float sub, float delta) {
+  constexpr int KT = KEYS<T>, TILE = PromptLds<T, DP>::TILE;
+  typedef HeadLds<T, DP> L;
+  L::template load<KT, 4>(nxt, k, (int)(a.k_row * sizeof(T)), left, a.D, wave_id());
+  L::template load<KT, 4>(nxt + TILE, v, (int)(a.v_row * sizeof(T)), left, a.D, wave_id());
+  __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+  for (int t = 0; t < KT / 32; ++t) {
+    if (j0 + 32 * t >= most) break;
+    f32x16 s = scores<T, DP>(cur, 32 * t, q);
+    const f32x16 d = scores<T, DP>(cur + TILE, 32 * t, go);
+    const bool masked = j0 + 32 * t + 32 > least;
+    const int first = j0 + 32 * t + 4 * (lane_id() >> 5);
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e], c, -sub));
+      s[e] = p * (d[e] - delta);
+      if (masked && first + 8 * (e >> 2) + (e & 3) >= n) s[e] = 0.f;
     }
-  attn_store(gk + (t * a.Hk + hk) * a.D, a.D, ak);
-  attn_store(gv + (t * a.Hk + hk) * a.D, a.D, av);
+    multiply_rows<T, DP>(acc, cur, 32 * t, s);
+  }
+}
+
+// dQ of 128 rows, 32 a wave; the rows, their order and their keys as the forward
+// for prompts has them.
+template <typename T, int DP>
+__global__ __launch_bounds__(256, (DP * sizeof(T) <= 256 ? 2 : 1)) void attn_bwd_q_kernel(
+    AttnArgs a, const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ v,
+    const T* __restrict__ go, const float* __restrict__ sub, const float* __restrict__ delta,
+    T* __restrict__ gq) {
+  constexpr int KT = KEYS<T>, TILE = PromptLds<T, DP>::TILE;
+  __shared__ PromptLds<T, DP> lds;
+  const int G = a.Hq / a.Hk, hk = blockIdx.x % a.Hk;
+  const int64_t place = gridDim.x / a.Hk - 1 - blockIdx.x / a.Hk;
+  const int s = attn_sequence(a.sq, place, G, 128);
+  const AttnSpan p = attn_span(a, s);
+  const int64_t local = uniform(place - attn_first(a.sq, s, G, 128));
+  const int all = p.room_q * G;
+  if (local < 0 || local * 128 >= all) return;
+  const int w = wave_id(), l = lane_id(), r0 = (int)local * 128 + 32 * w, r = r0 + (l & 31);
+  const int used = p.Lq * G;
+  auto keys = [&](int row) { return used ? attn_keys(a, p, row < used ? row : used - 1, G) : 0; };
+  const int least = keys(r0), most = r0 < used ? keys(r0 + 31) : 0;
+  const int end = (int)local * 128 < used ? keys((int)local * 128 + 127) : 0;
+  const int n = keys(r);
+  const bool in = r < used;
+  const int head = hk * G + r % G;
+  const int64_t token = p.q0 + r / G;
+  HeadRows<T, DP> x, y;
+  x.load(q + token * a.q_row + head * a.q_head, in, a.D);
+  y.load(go + (token * a.Hq + head) * a.D, in, a.D);
+  const float row_sub = in ? sub[head * a.sq.T + token] : -NEG_INF;
+  const float row_delta = in ? delta[head * a.sq.T + token] : 0.f;
+  const float c = attn_count(a.scale);
+  if (a.scale < 0.f) x.negate();
+  f32x16 acc[DP / 32];
+#pragma unroll
+  for (int i = 0; i < DP / 32; ++i) acc[i] = f32x16{};
+  const T* kt = k + p.k0 * a.k_row + hk * a.k_head;
+  const T* vt = v + p.k0 * a.v_row + hk * a.v_head;
+  typedef HeadLds<T, DP> L;
+  if (end > 0) {
+    L::template load<KT, 4>(lds.b, kt, (int)(a.k_row * sizeof(T)), p.Lk, a.D, w);
+    L::template load<KT, 4>(lds.b + TILE, vt, (int)(a.v_row * sizeof(T)), p.Lk, a.D, w);
+  }
+  int half = 0;
+  for (int j0 = 0; j0 < end; j0 += KT) {
+    wait_loads_and_meet<0>();
+    kt += KT * a.k_row;
+    vt += KT * a.v_row;
+    bwd_q_step<T, DP>(lds.b + half * 2 * TILE, lds.b + (half ^ 1) * 2 * TILE, kt, vt, a,
+                      j0 + KT < end ? p.Lk - j0 - KT : 0, x, y, acc, j0, n, least, most, c, row_sub,
+                      row_delta);
+    half ^= 1;
+  }
+  wait_loads_and_meet<0>();
+  if (r0 >= all) return;
+  put_rows<T, DP>(lds.b, acc, in && row_sub != -NEG_INF && n > 1 ? a.scale : 0.f, gq, a, p, hk, r0,
+                  all);
+}
+
+// A tile of rows of q and of go, and what is theirs of sub and delta.
+template <typename T, int DP>
+struct alignas(1024) BwdKeysLds {
+  static constexpr int TILE = KEYS<T> * HeadLds<T, DP>::PITCH;
+  static constexpr int STAGE = 2 * TILE + 1024;
+  static constexpr int OUT = 4 * Rows32<T, DP>::BYTES;
+  char b[2 * STAGE > OUT ? 2 * STAGE : OUT];
+};
+
+template <typename T, int DP>
+__device__ __forceinline__ void bwd_keys_load(char* to, const T* q, const T* go, const float* sub,
+                                              const float* delta, const AttnArgs& a, int left) {
+  constexpr int KT = KEYS<T>, TILE = BwdKeysLds<T, DP>::TILE;
+  typedef HeadLds<T, DP> L;
+  const int w = wave_id();
+  L::template load<KT, 4>(to, q, (int)(a.q_row * sizeof(T)), left, a.D, w);
+  L::template load<KT, 4>(to + TILE, go, (int)(a.Hq * a.D * sizeof(T)), left, a.D, w);
+  if (w < 2) {
+    const int n = left < 0 ? 0 : (left > 64 ? 64 : left);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(buffer(w ? delta : sub, n * 4),
+                                             (lds_t*)(to + 2 * TILE + 256 * w), 4, lane_id() * 4, 0,
+                                             0, 0);
+  }
+}
+
+template <typename T, int DP>
+struct KeySums {
+  f32x16 k[DP / 32], v[DP / 32];
+};
+
+// The products of a tile of rows (from row i0 on, `left` of them in use) with the
+// wave's keys, of which the lane's is seen by rows from `lo` on, the wave's by
+// rows between least and most on.  only: the row that sees a single key (every
+// row: ALL_ROWS).
+constexpr int ALL_ROWS = INT32_MIN;
+template <typename T, int DP>
+__device__ __forceinline__ void bwd_keys_step(const char* __restrict__ cur, char* __restrict__ nxt,
+                                              const T* q, const T* go, const float* sub,
+                                              const float* delta, const AttnArgs& a, int next,
+                                              const HeadRows<T, DP>& k, const HeadRows<T, DP>& v,
+                                              KeySums<T, DP>& sums, int i0, int left, int lo,
+                                              int least, int most, int only, float c) {
+  constexpr int KT = KEYS<T>, TILE = BwdKeysLds<T, DP>::TILE;
+  bwd_keys_load<T, DP>(nxt, q, go, sub, delta, a, next);
+  __builtin_amdgcn_sched_barrier(0);
+  const int h = lane_id() >> 5;
+#pragma unroll
+  for (int t = 0; t < KT / 32; ++t) {
+    const int i = i0 + 32 * t;
+    if (i + 32 <= least || 32 * t >= left) continue;
+    f32x16 s = scores<T, DP>(cur, 32 * t, k);
+    f32x16 d = scores<T, DP>(cur + TILE, 32 * t, v);
+    const bool masked = i < most || 32 * t + 32 > left || only == ALL_ROWS;
+    const float* ps = (const float*)(cur + 2 * TILE) + 32 * t + 4 * h;
+#pragma unroll
+    for (int b = 0; b < 4; ++b) {
+      const f32x4 m = *(const f32x4*)(ps + 8 * b), y = *(const f32x4*)(ps + 64 + 8 * b);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int row = 8 * b + 4 * h + e;
+        float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[4 * b + e], c, -m[e]));
+        float g = p * (d[4 * b + e] - y[e]);
+        if (masked) {
+          if (i + row == only || only == ALL_ROWS) g = 0.f;
+          if (i + row < lo || 32 * t + row >= left) p = g = 0.f;
+        }
+        s[4 * b + e] = p;
+        d[4 * b + e] = g;
+      }
+    }
+    multiply_rows<T, DP>(sums.v, cur + TILE, 32 * t, s);
+    multiply_rows<T, DP>(sums.k, cur, 32 * t, d);
+  }
+}
+
+// dK and dV of 128 keys, 32 a wave: for each head of the group, the rows that see
+// them in tiles that all four waves share.
+template <typename T, int DP>
+__global__ __launch_bounds__(256, (DP * sizeof(T) <= 128 ? 2 : 1)) void attn_bwd_keys_kernel(
+    AttnArgs a, const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ v,
+    const T* __restrict__ go, const float* __restrict__ sub, const float* __restrict__ delta,
+    T* __restrict__ gk, T* __restrict__ gv) {
+  constexpr int KT = KEYS<T>, STAGE = BwdKeysLds<T, DP>::STAGE;
+  __shared__ BwdKeysLds<T, DP> lds;
+  const int G = a.Hq / a.Hk, hk = blockIdx.x % a.Hk;
+  const int64_t place = blockIdx.x / a.Hk;  // early keys, which most rows see, go first
+  const int s = attn_sequence(a.sk, place, 1, 128);
+  const AttnSpan p = attn_span(a, s);
+  const int64_t local = uniform(place - attn_first(a.sk, s, 1, 128));
+  if (local < 0 || local * 128 >= p.room_k) return;
+  const int w = wave_id(), l = lane_id(), b0 = (int)local * 128, j0 = b0 + 32 * w, j = j0 + (l & 31);
+  const bool in = j < p.Lk;
+  HeadRows<T, DP> x, y;
+  x.load(k + (p.k0 + j) * a.k_row + hk * a.k_head, in, a.D);
+  y.load(v + (p.k0 + j) * a.v_row + hk * a.v_head, in, a.D);
+  const float c = attn_count(a.scale);
+  if (a.scale < 0.f) x.negate();
+  // the first row that sees a key
+  auto first = [&](int key) {
+    const int i = key - (p.Lk - p.Lq);
+    return a.causal && i > 0 ? i : 0;
+  };
+  const int lo = first(j), least = first(j0), most = first(j0 + 31);
+  // (the row that sees key 0 alone is the first that sees it, among the masked)
+  const int only = p.Lk == 1 ? ALL_ROWS : a.causal ? p.Lq - p.Lk : -1;
+  const int start = first(b0) / KT * KT, end = b0 < p.Lk ? p.Lq : 0;
+  KeySums<T, DP> sums;
+#pragma unroll
+  for (int i = 0; i < DP / 32; ++i) sums.k[i] = sums.v[i] = f32x16{};
+  const int tiles = start < end ? (end - start + KT - 1) / KT : 0;
+  // tile n of all heads' is rows start + n % tiles * KT of head n / tiles
+  auto at = [&](int g, int i, auto&& f) {
+    const int64_t head = hk * G + g, row = p.q0 + i;
+    f(q + row * a.q_row + head * a.q_head, go + (row * a.Hq + head) * a.D, sub + head * a.sq.T + row,
+      delta + head * a.sq.T + row);
+  };
+  if (tiles > 0)
+    at(0, start, [&](const T* q0, const T* g0, const float* s0, const float* d0) {
+      bwd_keys_load<T, DP>(lds.b, q0, g0, s0, d0, a, end - start);
+    });
+  int half = 0;
+  for (int g = 0; g < G; ++g)
+    for (int i = start; i < end; i += KT) {
+      wait_loads_and_meet<0>();
+      const bool wrap = i + KT >= end;
+      const int ng = wrap ? g + 1 : g, ni = wrap ? start : i + KT;
+      const int left = ng < G ? end - ni : 0;
+      at(ng < G ? ng : g, ni, [&](const T* q0, const T* g0, const float* s0, const float* d0) {
+        bwd_keys_step<T, DP>(lds.b + half * STAGE, lds.b + (half ^ 1) * STAGE, q0, g0, s0, d0, a,
+                             left, x, y, sums, i, end - i, lo, least, most, only, c);
+      });
+      half ^= 1;
+    }
+  wait_loads_and_meet<0>();
+  if (j0 >= p.room_k) return;
+  typedef Rows32<T, DP> R;
+  const R to{lds.b + w * R::BYTES};
+  auto put = [&](const f32x16(&acc)[DP / 32], float f, T* out) {
+#pragma unroll
+    for (int i = 0; i < DP / 32; ++i)
+#pragma unroll
+      for (int b = 0; b < 4; ++b) {
+        Four<T> z;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) z.v[e] = in ? (T)(acc[i][4 * b + e] * f) : (T)0.f;
+        *(Four<T>*)to.four(32 * i + 8 * b + 4 * (l >> 5)) = z;
+      }
+    to.store(out + hk * a.D, (int64_t)a.Hk * a.D, p.k0 + j0, p.k0 + p.room_k, 0, a.D, true);
+  };
+  put(sums.k, a.scale, gk);
+  put(sums.v, 1.f, gv);
 }
 
 }  // namespace tpo
@@ -111,7 +290,7 @@ using namespace tpo;
 extern "C" int64_t tpo_attention_bwd_workspace_size(int dtype, int64_t B, int64_t Tq, int64_t Tk,
                                                     int64_t Hq, int64_t Hk, int64_t D) {
   if (attn_check("attention_bwd_workspace_size", dtype, B, Tq, Tk, Hq, Hk, D)) return -1;
-  return round_up(Tq * Hq * 4, 256);
+  return 2 * round_up(Tq * Hq * 4, 256);
 }
 
 extern "C" int tpo_attention_bwd(int dtype, const void* grad_out, const void* q, const void* k,
@@ -128,20 +307,34 @@ extern "C" int tpo_attention_bwd(int dtype, const void* grad_out, const void* q,
   if (need > 0 && (!workspace || workspace_bytes < need))
     return set_error(TPO_ERR_WORKSPACE, "attention_bwd: workspace of %lld bytes needed",
                      (long long)need);
+  if (Tq == 0 && Tk == 0) return TPO_OK;
+  if (int rc = attn_layout("attention_bwd", dtype, D,
+                           {grad_out, q, k, v, out, grad_q, grad_k, grad_v, workspace},
+                           {q_row, q_head, k_row, k_head, v_row, v_head}, {q_row, k_row, v_row}))
+    return rc;
   const AttnArgs a = attn_args(offsets_q, offsets_k, lengths_q, lengths_k, B, Tq, Tk, Hq, Hk, D,
                                q_row, q_head, k_row, k_head, v_row, v_head, causal, scale);
-  float* delta = (float*)workspace;
+  const int64_t rows = Tq * Hq, G = Hq / Hk;
+  const int64_t places_q = attn_places(Tq, G, B, 128), places_k = attn_places(Tk, 1, B, 128);
+  if (places_q * Hk >= ((int64_t)1 << 31) || places_k * Hk >= ((int64_t)1 << 31))
+    return set_error(TPO_ERR_ARG, "attention_bwd: too many rows");
+  float *sub = (float*)workspace, *delta = (float*)((char*)workspace + need / 2);
   hipStream_t s = (hipStream_t)stream;
   with_element(dtype, [&](auto t) {
     typedef decltype(t) T;
+    const T *go = (const T*)grad_out, *qt = (const T*)q, *kt = (const T*)k, *vt = (const T*)v;
     if (Tq > 0)
-      attn_bwd_q_kernel<T><<<dim3((unsigned)((Tq * Hq + 3) / 4)), 256, 0, s>>>(
-          a, (const T*)q, (const T*)k, (const T*)v, (const T*)out, (const T*)grad_out, lse, delta,
-          (T*)grad_q);
-    if (Tk > 0)
-      attn_bwd_kv_kernel<T><<<dim3((unsigned)((Tk * Hk + 3) / 4)), 256, 0, s>>>(
-          a, (const T*)q, (const T*)k, (const T*)v, (const T*)grad_out, lse, delta, (T*)grad_k,
-          (T*)grad_v);
+      attn_delta_kernel<T><<<dim3((unsigned)((rows + 15) / 16)), 256, 0, s>>>(
+          (const T*)out, go, lse, rows, (int)Hq, Tq, (int)D, sub, delta);
+    with_head(D, [&](auto dp) {
+      constexpr int DP = decltype(dp)::value;
+      if (Tq > 0)
+        attn_bwd_q_kernel<T, DP><<<dim3((unsigned)(places_q * Hk)), 256, 0, s>>>(
+            a, qt, kt, vt, go, sub, delta, (T*)grad_q);
+      if (Tk > 0)
+        attn_bwd_keys_kernel<T, DP><<<dim3((unsigned)(places_k * Hk)), 256, 0, s>>>(
+            a, qt, kt, vt, go, sub, delta, (T*)grad_k, (T*)grad_v);
+    });
   });
   return check_launch("attention_bwd");
 }
