@@ -12,8 +12,197 @@ __device__ __forceinline__ float ln_at(const W* w, int64_t c, float none) {
   return w ? (float)w[c] : none;
 }
 
-template <typename T, typename W>
+// A row held in registers by a team of 64 or 256 lanes: N loads a lane of PER
+// values each (16 bytes, or one value where rows are not made of 16-byte pieces).
+// x is read once; the variance is taken about the mean, from the registers.
+// HBM-bound: what is read and written is all that counts, so teams go on to
+// other rows with the weights in registers, and there are enough of them to keep
+// the memory busy.
+template <typename T, int PER>
+struct alignas(PER * sizeof(T)) Piece {
+  T v[PER];
+};
+
+template <int TEAM>
+__device__ __forceinline__ float team_sum(float v, float (&s)[4]) {
+  v = wave_sum(v);
+  if constexpr (TEAM == 64) {
+    return v;
+  } else {
+    __syncthreads();  // the last sum has been read
+    if (lane_id() == 0) s[wave_id()] = v;
+    __syncthreads();
+    return (s[0] + s[1]) + (s[2] + s[3]);
+  }
+}
+
+template <typename T, int PER, int N, int TEAM>
+struct RowHeld {
+  float v[N][PER];
+  static __device__ __forceinline__ int64_t column(int i) {
+    return ((int64_t)i * TEAM + threadIdx.x % TEAM) * PER;
+  }
+  __device__ __forceinline__ void load(const T* p, int64_t width, float none = 0.f) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int64_t c = column(i);
+      if (c < width) {
+        const Piece<T, PER> x = *(const Piece<T, PER>*)(p + c);
+#pragma unroll
+        for (int e = 0; e < PER; ++e) v[i][e] = (float)x.v[e];
+      } else {
+#pragma unroll
+        for (int e = 0; e < PER; ++e) v[i][e] = none;
+      }
+    }
+  }
+  __device__ __forceinline__ void fill(float f) {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+      for (int e = 0; e < PER; ++e) v[i][e] = f;
+  }
+  __device__ __forceinline__ void store(T* p, int64_t width) const {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int64_t c = column(i);
+      if (c < width) {
+        Piece<T, PER> x;
+#pragma unroll
+        for (int e = 0; e < PER; ++e) x.v[e] = (T)v[i][e];
+        *(Piece<T, PER>*)(p + c) = x;
+      }
+    }
+  }
+};
+
+template <typename T, typename W, int PER, int N, int TEAM>
 __global__ __launch_bounds__(256) void layer_norm_fwd_kernel(
+    const T* __restrict__ x, const W* __restrict__ w, const W* __restrict__ b, int64_t rows,
+    int64_t width, float eps, T* __restrict__ y, float* __restrict__ mean,
+    float* __restrict__ rstd) {
+  __shared__ float s[4];
+  constexpr int TEAMS = 256 / TEAM;
+  RowHeld<W, PER, N, TEAM> ws, bs;
+  RowHeld<T, PER, N, TEAM> xs;
+  int64_t r = (int64_t)blockIdx.x * TEAMS + threadIdx.x / TEAM;
+  if (r >= rows) return;  // (with teams of 256 the whole workgroup)
+  xs.load(x + r * width, width);
+  if (w) ws.load(w, width); else ws.fill(1.f);
+  if (b) bs.load(b, width); else bs.fill(0.f);
+  const float per = 1.f / (float)width;
+  for (;;) {
+    float t = 0.f;
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+      for (int e = 0; e < PER; ++e) t += xs.v[i][e];
+    const float m = team_sum<TEAM>(t, s) * per;
+    t = 0.f;
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+      for (int e = 0; e < PER; ++e) {
+        const float d = xs.v[i][e] - m;
+        if (xs.column(i) < width) t = __builtin_fmaf(d, d, t);
+      }
+    const float q = 1.f / sqrtf(team_sum<TEAM>(t, s) * per + eps);
+    RowHeld<T, PER, N, TEAM> ys;
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+      for (int e = 0; e < PER; ++e)
+        ys.v[i][e] = __builtin_fmaf((xs.v[i][e] - m) * q, ws.v[i][e], bs.v[i][e]);
+    const int64_t next = r + (int64_t)gridDim.x * TEAMS;
+    if (next < rows) xs.load(x + next * width, width);
+    ys.store(y + r * width, width);
+    if (mean && threadIdx.x % TEAM == 0) {
+      mean[r] = m;
+      rstd[r] = q;
+    }
+    if (next >= rows) return;
+    r = next;
+  }
+}
+
+// gx of the team's rows, and the sums over them that the weights' gradients
+// need, a workgroup's in part[blockIdx.x] (weight, then bias).  gy and x are read
+// once for all three results.
+template <typename T, typename W, int PER, int N, int TEAM>
+__global__ __launch_bounds__(256) void layer_norm_bwd_kernel(
+    const T* __restrict__ gy, const T* __restrict__ x, const W* __restrict__ w,
+    const float* __restrict__ mean, const float* __restrict__ rstd, int64_t rows, int64_t width,
+    T* __restrict__ gx, float* __restrict__ part) {
+  __shared__ float s[4];
+  __shared__ float sums[TEAM == 64 ? 2 * N * PER * 64 : 1];
+  constexpr int TEAMS = 256 / TEAM;
+  typedef RowHeld<T, PER, N, TEAM> Row;
+  RowHeld<W, PER, N, TEAM> ws;
+  if (w) ws.load(w, width, 1.f); else ws.fill(1.f);
+  Row gs, xs;
+  RowHeld<float, PER, N, TEAM> sw, sb;
+  sw.fill(0.f);
+  sb.fill(0.f);
+  const float per = 1.f / (float)width;
+  for (int64_t r = (int64_t)blockIdx.x * TEAMS + threadIdx.x / TEAM; r < rows;
+       r += (int64_t)gridDim.x * TEAMS) {
+    gs.load(gy + r * width, width);
+    xs.load(x + r * width, width);
+    const float m = mean[r], q = rstd[r];
+    float s1 = 0.f, s2 = 0.f;
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+      for (int e = 0; e < PER; ++e) {
+        const float h = (xs.v[i][e] - m) * q, y = gs.v[i][e], g = y * ws.v[i][e];
+        xs.v[i][e] = h;  // (past the row's end y is 0: nothing is added)
+        sw.v[i][e] = __builtin_fmaf(y, h, sw.v[i][e]);
+        sb.v[i][e] += y;
+        s1 += g;
+        s2 = __builtin_fmaf(g, h, s2);
+      }
+    if (gx) {
+      s1 = team_sum<TEAM>(s1, s) * per;
+      s2 = team_sum<TEAM>(s2, s) * per;
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+#pragma unroll
+        for (int e = 0; e < PER; ++e)
+          xs.v[i][e] = q * (gs.v[i][e] * ws.v[i][e] - s1 - xs.v[i][e] * s2);
+      xs.store(gx + r * width, width);
+    }
+  }
+  if (!part) return;
+  float* p = part + (int64_t)blockIdx.x * 2 * width;
+  if constexpr (TEAM == 64) {  // the four waves' one after another
+    for (int t = 0; t < 4; ++t) {
+      __syncthreads();
+      if (wave_id() == t)
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+#pragma unroll
+          for (int e = 0; e < PER; ++e) {
+            const int at = (i * PER + e) * 64 + lane_id();
+            sums[at] = (t ? sums[at] : 0.f) + sw.v[i][e];
+            sums[at + N * PER * 64] = (t ? sums[at + N * PER * 64] : 0.f) + sb.v[i][e];
+          }
+    }
+    __syncthreads();
+    for (int64_t c = threadIdx.x; c < width; c += 256) {
+      const int64_t i = c / (64 * PER), e = c % PER, l = c / PER % 64;
+      const int at = (int)((i * PER + e) * 64 + l);
+      p[c] = sums[at];
+      p[width + c] = sums[at + N * PER * 64];
+    }
+  } else {
+    sw.store(p, width);
+    sb.store(p + width, width);
+  }
+}
+
+// Rows longer than a team holds: one wave a row, read again for each step.
+template <typename T, typename W>
+__global__ __launch_bounds__(256) void layer_norm_fwd_long_kernel(
     const T* __restrict__ x, const W* __restrict__ w, const W* __restrict__ b, int64_t rows,
     int64_t width, float eps, T* __restrict__ y, float* __restrict__ mean,
     float* __restrict__ rstd) {
@@ -39,7 +228,7 @@ __global__ __launch_bounds__(256) void layer_norm_fwd_kernel(
 }
 
 template <typename T, typename W>
-__global__ __launch_bounds__(256) void layer_norm_bwd_x_kernel(
+__global__ __launch_bounds__(256) void layer_norm_bwd_long_kernel(
     const T* __restrict__ gy, const T* __restrict__ x, const W* __restrict__ w,
     const float* __restrict__ mean, const float* __restrict__ rstd, int64_t rows, int64_t width,
     T* __restrict__ gx) {
@@ -92,8 +281,8 @@ __global__ __launch_bounds__(64) void layer_norm_bwd_narrow_kernel(
   }
 }
 
-// Sums of the weight's and the bias's gradient: a block sums 64 columns over
-// its share of the rows, the second kernel adds the shares in order.
+// Sums of the weight's and the bias's gradient for narrow and for long rows: a
+// block sums 64 columns over its share of the rows.
 template <typename T>
 __global__ __launch_bounds__(256) void layer_norm_bwd_w_kernel(
     const T* __restrict__ gy, const T* __restrict__ x, const float* __restrict__ mean,
@@ -118,24 +307,101 @@ __global__ __launch_bounds__(256) void layer_norm_bwd_w_kernel(
   }
 }
 
+// The shares added up, 64 of the 2 width columns a workgroup: sixteen waves take
+// every sixteenth share each, in a fixed order.
 template <typename W>
-__global__ __launch_bounds__(256) void layer_norm_bwd_sum_kernel(const float* __restrict__ part,
-                                                                 int parts, int64_t width,
-                                                                 W* __restrict__ gw,
-                                                                 W* __restrict__ gb) {
-  const int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (c >= width) return;
-  float a = 0.f, b = 0.f;
-  for (int p = 0; p < parts; ++p) {
-    a += part[(int64_t)p * 2 * width + c];
-    b += part[(int64_t)p * 2 * width + width + c];
+__global__ __launch_bounds__(1024) void layer_norm_bwd_sum_kernel(const float* __restrict__ part,
+                                                                  int parts, int64_t width,
+                                                                  W* __restrict__ gw,
+                                                                  W* __restrict__ gb) {
+  __shared__ float s[16][64];
+  const int lane = lane_id(), wv = wave_id();
+  const int64_t c = (int64_t)blockIdx.x * 64 + lane;
+  float a = 0.f;
+  if (c < 2 * width) {
+    int p = wv;
+    for (; p + 48 < parts; p += 64) {  // four loads under way
+      float y[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) y[i] = part[(int64_t)(p + 16 * i) * 2 * width + c];
+      a += (y[0] + y[1]) + (y[2] + y[3]);
+    }
+    for (; p < parts; p += 16) a += part[(int64_t)p * 2 * width + c];
   }
-  if (gw) gw[c] = (W)a;
-  if (gb) gb[c] = (W)b;
+  s[wv][lane] = a;
+  __syncthreads();
+  if (wv == 0 && c < 2 * width) {
+    a = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) a += s[i][lane];
+    W* to = c < width ? gw : gb;
+    if (to) to[c < width ? c : c - width] = (W)a;
+  }
+}
+
+// The kernels' build for a row: values a load, loads a lane, lanes a row; held
+// false for rows of more than 8192 values.
+struct LnForm {
+  int per, n, team;
+  bool held;
+};
+LnForm ln_form(int64_t width, int64_t size, bool pieces) {
+  const int64_t per = 16 / size;
+  LnForm f{1, 0, 64, true};
+  if (pieces && width % per == 0) {
+    f.per = (int)per;
+    const int64_t loads = (width + per - 1) / per;
+    if (loads <= 64) f.n = 1;
+    else if (loads <= 128) f.n = 2;
+    else if (loads <= 256) f.n = 4;
+    else if (loads <= 512) f.n = 2, f.team = 256;
+    else if (loads <= 1024) f.n = 4, f.team = 256;
+    else f.held = false;
+  } else {
+    if (width <= 256) f.n = 4;
+    else if (width <= 1024) f.n = 16;
+    else if (width <= 2048) f.n = 8, f.team = 256;
+    else if (width <= 8192) f.n = 32, f.team = 256;
+    else f.held = false;
+  }
+  return f;
+}
+// Calls f with the form as types: value counts, loads, team.
+template <typename T, typename F>
+void with_form(const LnForm& f, F&& call) {
+  constexpr int PER = 16 / sizeof(T);
+  auto go = [&](auto per, auto n, auto team) { call(per, n, team); };
+#define LN_FORM(P, N, TEAM)                                                           \
+  if (f.per == P && f.n == N && f.team == TEAM)                                       \
+  return go(std::integral_constant<int, P>(), std::integral_constant<int, N>(),       \
+            std::integral_constant<int, TEAM>())
+  LN_FORM(PER, 1, 64);
+  LN_FORM(PER, 2, 64);
+  LN_FORM(PER, 4, 64);
+  LN_FORM(PER, 2, 256);
+  LN_FORM(PER, 4, 256);
+  LN_FORM(1, 4, 64);
+  LN_FORM(1, 16, 64);
+  LN_FORM(1, 8, 256);
+  LN_FORM(1, 32, 256);
+#undef LN_FORM
 }
 
 constexpr int64_t LN_WIDTH_MAX = 1 << 20;
-inline int ln_parts(int64_t rows) { return (int)(rows < 256 ? (rows + 3) / 4 : 64); }
+// Shares of the rows for the weights' gradients: workgroups that keep the memory
+// busy, but no more than makes their sums' way through memory a twentieth of the
+// rows' (in half types).
+inline int ln_parts(int64_t rows) {
+  const int64_t few = (rows + 3) / 4, most = rows / 16 > 64 ? rows / 16 : 64;
+  const int64_t p = few < most ? few : most;
+  return (int)(p > 1024 ? 1024 : p);
+}
+
+inline bool ln_pieces(std::initializer_list<const void*> ps) {
+  for (const void* p : ps)
+    if ((uintptr_t)p & 15) return false;
+  return true;
+}
 
 // The weights are of the input's type or float.
 template <typename F>
@@ -177,8 +443,21 @@ extern "C" int tpo_layer_norm_fwd(int dtype, int wdtype, const void* x, const vo
       none = true;
       return;
     }
-    layer_norm_fwd_kernel<T, W><<<dim3((unsigned)((rows + 3) / 4)), 256, 0, s>>>(
-        (const T*)x, (const W*)weight, (const W*)bias, rows, width, (float)eps, (T*)y, mean, rstd);
+    const LnForm f = ln_form(width, sizeof(T), ln_pieces({x, weight, bias, y}));
+    if (!f.held) {
+      layer_norm_fwd_long_kernel<T, W><<<dim3((unsigned)((rows + 3) / 4)), 256, 0, s>>>(
+          (const T*)x, (const W*)weight, (const W*)bias, rows, width, (float)eps, (T*)y, mean,
+          rstd);
+      return;
+    }
+    with_form<T>(f, [&](auto per, auto n, auto team) {
+      constexpr int TEAMS = 256 / decltype(team)::value;
+      int64_t blocks = (rows + TEAMS - 1) / TEAMS;
+      if (blocks > 2048) blocks = 2048;  // eight workgroups a CU
+      layer_norm_fwd_kernel<T, W, decltype(per)::value, decltype(n)::value, decltype(team)::value>
+          <<<dim3((unsigned)blocks), 256, 0, s>>>((const T*)x, (const W*)weight, (const W*)bias,
+                                                  rows, width, (float)eps, (T*)y, mean, rstd);
+    });
   });
   return rc || none ? rc : check_launch("layer_norm_fwd");
 }
@@ -203,19 +482,29 @@ extern "C" int tpo_layer_norm_bwd(int dtype, int wdtype, const void* grad_y, con
   const int rc = ln_dispatch("layer_norm_bwd", dtype, wdtype, [&](auto t, auto w) {
     typedef decltype(t) T;
     typedef decltype(w) W;
-    if (grad_x && rows > 0 && width <= LN_NARROW)
-      layer_norm_bwd_narrow_kernel<T, W><<<dim3((unsigned)((rows + 63) / 64)), 64, 0, s>>>(
-          (const T*)grad_y, (const T*)x, (const W*)weight, eps, rows, (int)width, (T*)grad_x);
-    else if (grad_x && rows > 0)
-      layer_norm_bwd_x_kernel<T, W><<<dim3((unsigned)((rows + 3) / 4)), 256, 0, s>>>(
-          (const T*)grad_y, (const T*)x, (const W*)weight, mean, rstd, rows, width, (T*)grad_x);
-    if (!sums) return;
+    const LnForm f = ln_form(width, sizeof(T), ln_pieces({grad_y, x, weight, grad_x}));
     const int parts = ln_parts(rows);
-    if (parts > 0)
-      layer_norm_bwd_w_kernel<T><<<dim3((unsigned)((width + 63) / 64), parts), 256, 0, s>>>(
-          (const T*)grad_y, (const T*)x, mean, rstd, rows, width, (float*)workspace);
-    layer_norm_bwd_sum_kernel<W><<<dim3((unsigned)((width + 255) / 256)), 256, 0, s>>>(
-        (const float*)workspace, parts, width, (W*)grad_weight, (W*)grad_bias);
+    float* part = sums ? (float*)workspace : nullptr;
+    if (rows > 0 && width > LN_NARROW && f.held) {
+      with_form<T>(f, [&](auto per, auto n, auto team) {
+        layer_norm_bwd_kernel<T, W, decltype(per)::value, decltype(n)::value, decltype(team)::value>
+            <<<dim3((unsigned)parts), 256, 0, s>>>((const T*)grad_y, (const T*)x, (const W*)weight,
+                                                   mean, rstd, rows, width, (T*)grad_x, part);
+      });
+    } else if (rows > 0) {
+      if (grad_x && width <= LN_NARROW)
+        layer_norm_bwd_narrow_kernel<T, W><<<dim3((unsigned)((rows + 63) / 64)), 64, 0, s>>>(
+            (const T*)grad_y, (const T*)x, (const W*)weight, eps, rows, (int)width, (T*)grad_x);
+      else if (grad_x)
+        layer_norm_bwd_long_kernel<T, W><<<dim3((unsigned)((rows + 3) / 4)), 256, 0, s>>>(
+            (const T*)grad_y, (const T*)x, (const W*)weight, mean, rstd, rows, width, (T*)grad_x);
+      if (sums)
+        layer_norm_bwd_w_kernel<T><<<dim3((unsigned)((width + 63) / 64), parts), 256, 0, s>>>(
+            (const T*)grad_y, (const T*)x, mean, rstd, rows, width, part);
+    }
+    if (sums)
+      layer_norm_bwd_sum_kernel<W><<<dim3((unsigned)((2 * width + 63) / 64)), 1024, 0, s>>>(
+          part, parts, width, (W*)grad_weight, (W*)grad_bias);
   });
   return rc ? rc : check_launch("layer_norm_bwd");
 }
