@@ -377,7 +377,14 @@ int tpo_layer_norm_bwd(int dtype, int wdtype, const void* grad_y, const void* x,
  *   out (Tq,Hq,D) contiguous; rows not in use, and rows that see no key, are 0.
  *   lse (Hq,Tq) float: log of the sum of exponentials of each row (-inf for
  *   a row that sees no key), what the backward needs; NULL to leave out.
- * tpo_attention_bwd: grad_out, out and the gradients are contiguous.  Every
+ *   rest (as out) or NULL: what rounding to the type took from out, for a
+ *   more exact backward; of no use with F32.
+ *   Pointers, heads (D values) and strides are multiples of 16 bytes, a row's
+ *   stride is 16 to 2^25 bytes.
+ *   A NaN or an infinity in v reaches the rows that see it and, by 0 times it,
+ *   earlier rows of the sequence that share a tile of 64 keys with it; it
+ *   reaches no row of another sequence, and rows not in use are not read.
+ * tpo_attention_bwd: grad_out, out, rest and the gradients are contiguous.  Every
  *   row of grad_q, grad_k, grad_v is written, rows not in use with 0; sums
  *   run in a fixed order.
  * Workspaces are 256-byte aligned; size 0 means none is used.
@@ -390,12 +397,13 @@ int tpo_attention_fwd(int dtype, const void* q, const void* k, const void* v,
                       int64_t Tq, int64_t Tk, int64_t Hq, int64_t Hk, int64_t D,
                       int64_t q_row, int64_t q_head, int64_t k_row, int64_t k_head,
                       int64_t v_row, int64_t v_head, int causal, double scale,
-                      void* out, float* lse, void* workspace,
+                      void* out, float* lse, void* rest, void* workspace,
                       int64_t workspace_bytes, void* stream);
 int64_t tpo_attention_bwd_workspace_size(int dtype, int64_t B, int64_t Tq, int64_t Tk,
                                          int64_t Hq, int64_t Hk, int64_t D);
 int tpo_attention_bwd(int dtype, const void* grad_out, const void* q, const void* k,
-                      const void* v, const void* out, const float* lse,
+                      const void* v, const void* out, const void* rest,
+                      const float* lse,
                       const int64_t* offsets_q, const int64_t* offsets_k,
                       const int64_t* lengths_q, const int64_t* lengths_k, int64_t B,
                       int64_t Tq, int64_t Tk, int64_t Hq, int64_t Hk, int64_t D,

@@ -16,8 +16,8 @@ def lib(tpo):
     L.tpo_last_error.restype = ctypes.c_char_p
     L.tpo_layer_norm_fwd.argtypes = [C, C, P, P, P, I, I, D, P, P, P, P]
     L.tpo_layer_norm_bwd.argtypes = [C, C, P, P, P, P, P, I, I, D, P, P, P, P, I, P]
-    L.tpo_attention_fwd.argtypes = [C] + [P] * 7 + [I] * 12 + [C, D, P, P, P, I, P]
-    L.tpo_attention_bwd.argtypes = [C] + [P] * 10 + [I] * 12 + [C, D, P, P, P, P, I, P]
+    L.tpo_attention_fwd.argtypes = [C] + [P] * 7 + [I] * 12 + [C, D, P, P, P, P, I, P]
+    L.tpo_attention_bwd.argtypes = [C] + [P] * 11 + [I] * 12 + [C, D, P, P, P, P, I, P]
     L.tpo_gated_fwd.argtypes = [C, P, P, P, I, I, I, C, P, P, I, P]
     L.tpo_gated_bwd.argtypes = [C, P, P, P, P, I, I, I, C, P, P, P, P, I, P]
     L.tpo_layer_norm_bwd_workspace_size.argtypes = [I, I]
@@ -44,11 +44,11 @@ def test_fake_shapes(tpo):
         q, k = torch.empty(7, 4, 32), torch.empty(9, 2, 32)
         o = torch.empty(3, dtype=torch.int64)
         assert tpo.packed_attention(q, k, k, o, o).shape == q.shape
-        out, lse = torch.ops.torch_point_ops_attention.packed_attention_forward(
+        out, lse, rest = torch.ops.torch_point_ops_attention.packed_attention_forward(
             q, k, k, o, o, None, None, True, 1.0)
         assert lse.shape == (4, 7)
         g = torch.ops.torch_point_ops_attention.packed_attention_backward(
-            out, q, k, k, out, lse, o, o, None, None, True, 1.0)
+            out, q, k, k, out, lse, rest, o, o, None, None, True, 1.0)
         assert [t.shape for t in g] == [q.shape, k.shape, k.shape]
         x, w = torch.empty(3, 4, 16), torch.empty(24, 16)
         h = tpo.gated_projection(x, w, w)
@@ -107,7 +107,7 @@ def test_layer_norm_entry(lib):
 def _attention(lib, dtype=0, B=1, Tq=4, Tk=4, Hq=2, Hk=2, D=16):
     f = P(4096)
     return lib.tpo_attention_fwd(dtype, f, f, f, f, f, None, None, B, Tq, Tk, Hq, Hk, D,
-                                 *[Hq * D, D] * 3, 1, 1.0, f, None, None, 0, None)
+                                 *[Hq * D, D] * 3, 1, 1.0, f, None, None, None, 0, None)
 
 
 def test_attention_entry(lib):
@@ -118,7 +118,7 @@ def test_attention_entry(lib):
     assert _attention(lib, dtype=1) == -2
     assert _attention(lib, Tq=0) == 0
     f = P(4096)
-    assert lib.tpo_attention_bwd(0, f, f, f, f, f, f, f, f, None, None, 1, 4, 4, 2, 2, 16,
+    assert lib.tpo_attention_bwd(0, f, f, f, f, f, f, f, f, f, None, None, 1, 4, 4, 2, 2, 16,
                                  *[32, 16] * 3, 1, 1.0, f, f, f, None, 0, None) == -4
     assert lib.tpo_attention_fwd_workspace_size(0, 1, 4, 4, 3, 2, 16) == -1
     assert lib.tpo_attention_bwd_workspace_size(3, 1, 4, 4, 2, 2, 200) == -1

@@ -93,7 +93,8 @@ __global__ __launch_bounds__(256, 2) void attn_prompt_kernel(AttnArgs a, const T
                                                              const T* __restrict__ k,
                                                              const T* __restrict__ v,
                                                              T* __restrict__ out,
-                                                             float* __restrict__ lse) {
+                                                             float* __restrict__ lse,
+                                                             T* __restrict__ rest) {
   constexpr int KT = KEYS<T>, TILE = PromptLds<T, DP>::TILE;
   __shared__ PromptLds<T, DP> lds;
   const int G = a.Hq / a.Hk, hk = blockIdx.x % a.Hk;
@@ -142,6 +143,7 @@ __global__ __launch_bounds__(256, 2) void attn_prompt_kernel(AttnArgs a, const T
   const float sum = rows.l + other_half(rows.l);
   const float inv = in && sum != 0.f ? 1.f / sum : 0.f;
   put_rows<T, DP>(lds.b, rows.acc, inv, out, a, p, hk, r0, all);
+  if (rest) put_rows<T, DP, true>(lds.b, rows.acc, inv, rest, a, p, hk, r0, all);
   if (lse && l < 32 && r < all)
     lse[head * a.sq.T + token] =
         inv == 0.f ? NEG_INF : (rows.m * c + __builtin_amdgcn_logf(sum)) * LN2;
@@ -188,8 +190,8 @@ __device__ __forceinline__ void step_step(const char* __restrict__ cur, char* __
 template <typename T, int DP>
 __global__ __launch_bounds__((64 * STEP_WAVES<T, DP>)) void attn_step_kernel(
     AttnArgs a, const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ v,
-    T* __restrict__ out, float* __restrict__ lse, float* __restrict__ part,
-    float2* __restrict__ ml) {
+    T* __restrict__ out, float* __restrict__ lse, T* __restrict__ rest,
+    float* __restrict__ part, float2* __restrict__ ml) {
   constexpr int W = STEP_WAVES<T, DP>, TILE = StepLds<T, DP>::TILE;
   __shared__ StepLds<T, DP> lds;
   const int G = a.Hq / a.Hk, hk = blockIdx.y, shares = gridDim.z;
@@ -277,7 +279,9 @@ __global__ __launch_bounds__((64 * STEP_WAVES<T, DP>)) void attn_step_kernel(
       if (shares > 1) {
         if (total != 0.f) part[(at * shares + blockIdx.z) * a.D + d0 + d] = y;
       } else {
-        out[at * a.D + d0 + d] = total == 0.f ? (T)0.f : (T)(y * inv);
+        const T z = total == 0.f ? (T)0.f : (T)(y * inv);
+        out[at * a.D + d0 + d] = z;
+        if (rest) rest[at * a.D + d0 + d] = total == 0.f ? (T)0.f : (T)(y * inv - (float)z);
       }
     }
   }
@@ -296,7 +300,8 @@ __global__ __launch_bounds__(256) void attn_join_kernel(const float* __restrict_
                                                         const float2* __restrict__ ml, int shares,
                                                         int64_t rows, int Hq, int64_t Tq, int D,
                                                         T* __restrict__ out,
-                                                        float* __restrict__ lse) {
+                                                        float* __restrict__ lse,
+                                                        T* __restrict__ rest) {
   const int64_t at = (int64_t)blockIdx.x * 4 + wave_id();
   if (at >= rows) return;
   const int l = lane_id();
@@ -316,8 +321,13 @@ __global__ __launch_bounds__(256) void attn_join_kernel(const float* __restrict_
     if (l + 64 < D) o[1] += f * p[l + 64];
   }
   const float inv = total != 0.f ? 1.f / total : 0.f;
-  if (l < D) out[at * D + l] = (T)(o[0] * inv);
-  if (l + 64 < D) out[at * D + l + 64] = (T)(o[1] * inv);
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    if (l + 64 * i < D) {
+      const T z = (T)(o[i] * inv);
+      out[at * D + l + 64 * i] = z;
+      if (rest) rest[at * D + l + 64 * i] = (T)(o[i] * inv - (float)z);
+    }
   if (lse && l == 0)
     lse[(at % Hq) * Tq + at / Hq] = total == 0.f ? NEG_INF : (m + __builtin_amdgcn_logf(total)) * LN2;
 }
@@ -415,11 +425,12 @@ extern "C" int tpo_attention_fwd(int dtype, const void* q, const void* k, const 
                                  int64_t Tq, int64_t Tk, int64_t Hq, int64_t Hk, int64_t D,
                                  int64_t q_row, int64_t q_head, int64_t k_row, int64_t k_head,
                                  int64_t v_row, int64_t v_head, int causal, double scale,
-                                 void* out, float* lse, void* workspace, int64_t workspace_bytes,
+                                 void* out, float* lse, void* rest, void* workspace,
+                                 int64_t workspace_bytes,
                                  void* stream) {
   if (int rc = attn_check("attention_fwd", dtype, B, Tq, Tk, Hq, Hk, D)) return rc;
   if (Tq == 0) return TPO_OK;
-  if (int rc = attn_layout("attention_fwd", dtype, D, {q, k, v, out, workspace},
+  if (int rc = attn_layout("attention_fwd", dtype, D, {q, k, v, out, rest, workspace},
                            {q_row, q_head, k_row, k_head, v_row, v_head}, {q_row, k_row, v_row}))
     return rc;
   const int64_t need = tpo_attention_fwd_workspace_size(dtype, B, Tq, Tk, Hq, Hk, D);
@@ -441,15 +452,15 @@ extern "C" int tpo_attention_fwd(int dtype, const void* q, const void* k, const 
       constexpr int DP = decltype(dp)::value;
       if (!w.step)
         attn_prompt_kernel<T, DP><<<dim3((unsigned)(places * Hk)), 256, 0, s>>>(
-            a, (const T*)q, (const T*)k, (const T*)v, (T*)out, lse);
+            a, (const T*)q, (const T*)k, (const T*)v, (T*)out, lse, (T*)rest);
       else
         attn_step_kernel<T, DP>
             <<<dim3((unsigned)places, (unsigned)Hk, w.shares), 64 * STEP_WAVES<T, DP>, 0, s>>>(
-                a, (const T*)q, (const T*)k, (const T*)v, (T*)out, lse, part, ml);
+                a, (const T*)q, (const T*)k, (const T*)v, (T*)out, lse, (T*)rest, part, ml);
     });
     if (w.shares > 1)
       attn_join_kernel<T><<<dim3((unsigned)((Tq * Hq + 3) / 4)), 256, 0, s>>>(
-          part, ml, w.shares, Tq * Hq, (int)Hq, Tq, (int)D, (T*)out, lse);
+          part, ml, w.shares, Tq * Hq, (int)Hq, Tq, (int)D, (T*)out, lse, (T*)rest);
   });
   return check_launch("attention_fwd");
 }

@@ -191,7 +191,8 @@ struct HeadRows {
 
 // A wave's 32 rows of sums, f times each, to the rows r0 .. of a sequence and key
 // head in an array laid out as out (f 0: nothing but zeros), by way of LDS.
-template <typename T, int DP>
+// REST: what rounding takes from them instead.
+template <typename T, int DP, bool REST = false>
 __device__ __forceinline__ void put_rows(char* lds, const f32x16 (&acc)[DP / 32], float f,
                                          T* __restrict__ out, const AttnArgs& a, const AttnSpan& p,
                                          int hk, int r0, int all) {
@@ -204,7 +205,10 @@ __device__ __forceinline__ void put_rows(char* lds, const f32x16 (&acc)[DP / 32]
     for (int b = 0; b < 4; ++b) {
       Four<T> y;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) y.v[e] = f == 0.f ? (T)0.f : (T)(acc[i][4 * b + e] * f);
+      for (int e = 0; e < 4; ++e) {
+        const float z = f == 0.f ? 0.f : acc[i][4 * b + e] * f;
+        y.v[e] = (T)(REST ? z - (float)(T)z : z);
+      }
       *(Four<T>*)to.four(32 * i + 8 * b + 4 * (l >> 5)) = y;
     }
   to.wait();
@@ -215,6 +219,7 @@ __device__ __forceinline__ void put_rows(char* lds, const f32x16 (&acc)[DP / 32]
       *(f32x4*)(out + ((p.q0 + row / G) * a.Hq + hk * G + row % G) * a.D + cc) =
           *(const f32x4*)((const T*)(to.lds + rr * R::PITCH) + cc);
   }
+  to.wait();
 }
 
 // The keys that row r (of the rows of a sequence and key head) sees.

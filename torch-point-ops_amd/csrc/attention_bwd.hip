@@ -16,9 +16,12 @@ namespace tpo {
 
 // Of each row: what is subtracted in the exponent of 2 (the logarithm of its sum;
 // infinity where the row sees no key, which makes its P 0), and delta =
-// sum_d dO O.  Sixteen lanes a row.
+// sum_d dO O.  rest: what rounding took from O.  Without it the rounding of O,
+// which is common to all keys of a row, would add to dQ's error about half of
+// what the rounding of dS does.  Sixteen lanes a row.
 template <typename T>
 __global__ __launch_bounds__(256) void attn_delta_kernel(const T* __restrict__ o,
+                                                         const T* __restrict__ rest,
                                                          const T* __restrict__ go,
                                                          const float* __restrict__ lse,
                                                          int64_t rows, int Hq, int64_t Tq, int D,
@@ -33,6 +36,11 @@ __global__ __launch_bounds__(256) void attn_delta_kernel(const T* __restrict__ o
     const V x = *(const V*)(o + r * D + c), y = *(const V*)(go + r * D + c);
 #pragma unroll
     for (int e = 0; e < PER; ++e) s = __builtin_fmaf((float)x[e], (float)y[e], s);
+    if (rest) {
+      const V z = *(const V*)(rest + r * D + c);
+#pragma unroll
+      for (int e = 0; e < PER; ++e) s = __builtin_fmaf((float)z[e], (float)y[e], s);
+    }
   }
 #pragma unroll
   for (int d = 8; d > 0; d >>= 1) s += __shfl_xor(s, d);
@@ -66,8 +74,11 @@ __device__ __forceinline__ void bwd_q_step(const char* __restrict__ cur, char* _
     for (int e = 0; e < 16; ++e) {
       const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e], c, -sub));
       s[e] = p * (d[e] - delta);
-      if (masked && first + 8 * (e >> 2) + (e & 3) >= n) s[e] = 0.f;
     }
+    if (masked)  // (a pass of its own: a select for each value would be taken everywhere)
+#pragma unroll
+      for (int e = 0; e < 16; ++e)
+        if (first + 8 * (e >> 2) + (e & 3) >= n) s[e] = 0.f;
     multiply_rows<T, DP>(acc, cur, 32 * t, s);
   }
 }
@@ -189,17 +200,17 @@ __device__ __forceinline__ void bwd_keys_step(const char* __restrict__ cur, char
       const f32x4 m = *(const f32x4*)(ps + 8 * b), y = *(const f32x4*)(ps + 64 + 8 * b);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const int row = 8 * b + 4 * h + e;
-        float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[4 * b + e], c, -m[e]));
-        float g = p * (d[4 * b + e] - y[e]);
-        if (masked) {
-          if (i + row == only || only == ALL_ROWS) g = 0.f;
-          if (i + row < lo || 32 * t + row >= left) p = g = 0.f;
-        }
-        s[4 * b + e] = p;
-        d[4 * b + e] = g;
+        s[4 * b + e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[4 * b + e], c, -m[e]));
+        d[4 * b + e] = s[4 * b + e] * (d[4 * b + e] - y[e]);
       }
     }
+    if (masked)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const int row = 32 * t + 8 * (e >> 2) + 4 * h + (e & 3);
+        if (i0 + row == only || only == ALL_ROWS) d[e] = 0.f;
+        if (i0 + row < lo || row >= left) s[e] = d[e] = 0.f;
+      }
     multiply_rows<T, DP>(sums.v, cur + TILE, 32 * t, s);
     multiply_rows<T, DP>(sums.k, cur, 32 * t, d);
   }
@@ -294,7 +305,8 @@ extern "C" int64_t tpo_attention_bwd_workspace_size(int dtype, int64_t B, int64_
 }
 
 extern "C" int tpo_attention_bwd(int dtype, const void* grad_out, const void* q, const void* k,
-                                 const void* v, const void* out, const float* lse,
+                                 const void* v, const void* out, const void* rest,
+                                 const float* lse,
                                  const int64_t* offsets_q, const int64_t* offsets_k,
                                  const int64_t* lengths_q, const int64_t* lengths_k, int64_t B,
                                  int64_t Tq, int64_t Tk, int64_t Hq, int64_t Hk, int64_t D,
@@ -309,7 +321,7 @@ extern "C" int tpo_attention_bwd(int dtype, const void* grad_out, const void* q,
                      (long long)need);
   if (Tq == 0 && Tk == 0) return TPO_OK;
   if (int rc = attn_layout("attention_bwd", dtype, D,
-                           {grad_out, q, k, v, out, grad_q, grad_k, grad_v, workspace},
+                           {grad_out, q, k, v, out, rest, grad_q, grad_k, grad_v, workspace},
                            {q_row, q_head, k_row, k_head, v_row, v_head}, {q_row, k_row, v_row}))
     return rc;
   const AttnArgs a = attn_args(offsets_q, offsets_k, lengths_q, lengths_k, B, Tq, Tk, Hq, Hk, D,
@@ -325,7 +337,7 @@ extern "C" int tpo_attention_bwd(int dtype, const void* grad_out, const void* q,
     const T *go = (const T*)grad_out, *qt = (const T*)q, *kt = (const T*)k, *vt = (const T*)v;
     if (Tq > 0)
       attn_delta_kernel<T><<<dim3((unsigned)((rows + 15) / 16)), 256, 0, s>>>(
-          (const T*)out, go, lse, rows, (int)Hq, Tq, (int)D, sub, delta);
+          (const T*)out, (const T*)rest, go, lse, rows, (int)Hq, Tq, (int)D, sub, delta);
     with_head(D, [&](auto dp) {
       constexpr int DP = decltype(dp)::value;
       if (Tq > 0)

@@ -245,15 +245,16 @@ Tensor cut_heads(const Tensor& t, int64_t D) {
   return t.size(2) == D ? t : t.narrow(2, 0, D).contiguous();
 }
 
-std::tuple<Tensor, Tensor> packed_attention_hip(const Tensor& q, const Tensor& k, const Tensor& v,
+std::tuple<Tensor, Tensor, Tensor> packed_attention_hip(const Tensor& q, const Tensor& k, const Tensor& v,
                                                 const Tensor& oq, const Tensor& ok,
                                                 const OptTensor& lq, const OptTensor& lk,
                                                 bool causal, double scale, bool stats) {
   const char* op = "packed_attention";
   const Packed p = packed_args(q, k, v, oq, ok, lq, lk, op);
   c10::OptionalDeviceGuard guard(q.device());
-  Tensor out = at::empty({p.Tq, p.Hq, p.D}, q.options()), lse;
+  Tensor out = at::empty({p.Tq, p.Hq, p.D}, q.options()), lse, rest;
   if (stats) lse = at::empty({p.Hq, p.Tq}, q.options().dtype(at::kFloat));
+  if (stats) rest = p.dt == TPO_F32 ? nothing(q) : at::empty_like(out);
   const int64_t wsb = tpo_attention_fwd_workspace_size(p.dt, p.B, p.Tq, p.Tk, p.Hq, p.Hk, p.D);
   const Tensor ws = workspace(wsb, q, op);
   check_rc(tpo_attention_fwd(p.dt, p.q.data_ptr(), p.k.data_ptr(), p.v.data_ptr(),
@@ -261,10 +262,11 @@ std::tuple<Tensor, Tensor> packed_attention_hip(const Tensor& q, const Tensor& k
                              (const int64_t*)data_or_null(p.lq), (const int64_t*)data_or_null(p.lk),
                              p.B, p.Tq, p.Tk, p.Hq, p.Hk, p.D, row_stride(p.q), head_stride(p.q),
                              row_stride(p.k), head_stride(p.k), row_stride(p.v), head_stride(p.v),
-                             causal, scale, out.data_ptr(), (float*)data_or_null(lse), data_or_null(ws),
-                             wsb, stream_of(q)),
+                             causal, scale, out.data_ptr(), (float*)data_or_null(lse), data_or_null(rest),
+                             data_or_null(ws), wsb, stream_of(q)),
            op);
-  return {cut_heads(out, q.size(2)), lse};
+  if (stats && rest.dim() == 3) rest = cut_heads(rest, q.size(2));
+  return {cut_heads(out, q.size(2)), lse, rest};
 }
 
 Tensor packed_attention_only_hip(const Tensor& q, const Tensor& k, const Tensor& v,
@@ -272,7 +274,7 @@ Tensor packed_attention_only_hip(const Tensor& q, const Tensor& k, const Tensor&
                                  const OptTensor& lk, bool causal, double scale) {
   return std::get<0>(packed_attention_hip(q, k, v, oq, ok, lq, lk, causal, scale, false));
 }
-std::tuple<Tensor, Tensor> packed_attention_forward_hip(const Tensor& q, const Tensor& k,
+std::tuple<Tensor, Tensor, Tensor> packed_attention_forward_hip(const Tensor& q, const Tensor& k,
                                                         const Tensor& v, const Tensor& oq,
                                                         const Tensor& ok, const OptTensor& lq,
                                                         const OptTensor& lk, bool causal,
@@ -282,8 +284,8 @@ std::tuple<Tensor, Tensor> packed_attention_forward_hip(const Tensor& q, const T
 
 std::tuple<Tensor, Tensor, Tensor> packed_attention_backward_hip(
     const Tensor& grad_in, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& out_in,
-    const Tensor& lse_in, const Tensor& oq, const Tensor& ok, const OptTensor& lq,
-    const OptTensor& lk, bool causal, double scale) {
+    const Tensor& lse_in, const Tensor& rest_in, const Tensor& oq, const Tensor& ok,
+    const OptTensor& lq, const OptTensor& lk, bool causal, double scale) {
   const char* op = "packed_attention_backward";
   const Packed p = packed_args(q, k, v, oq, ok, lq, lk, op);
   c10::OptionalDeviceGuard guard(q.device());
@@ -292,18 +294,23 @@ std::tuple<Tensor, Tensor, Tensor> packed_attention_backward_hip(
   TORCH_CHECK(out_in.scalar_type() == q.scalar_type() && lse_in.scalar_type() == at::kFloat &&
                   lse_in.numel() == p.Tq * p.Hq,
               "packed_attention_backward: out and lse must be the forward's");
-  for (const Tensor& t : {grad_in, out_in, lse_in})
+  TORCH_CHECK(rest_in.numel() == 0 || (rest_in.sizes() == q.sizes() &&
+                                       rest_in.scalar_type() == q.scalar_type()),
+              "packed_attention_backward: rest must be the forward's");
+  for (const Tensor& t : {grad_in, out_in, lse_in, rest_in})
     TORCH_CHECK(t.device() == q.device(), op, ": all tensors must be on the same device");
   const Tensor g = head_rows(grad_in.to(q.scalar_type()).contiguous(), p.D);
   const Tensor out = head_rows(out_in.contiguous(), p.D);
   const Tensor lse = lse_in.contiguous();
+  Tensor rest;
+  if (rest_in.numel() > 0) rest = head_rows(rest_in.contiguous(), p.D);
   Tensor gq = at::empty({p.Tq, p.Hq, p.D}, q.options());
   Tensor gk = at::empty({p.Tk, p.Hk, p.D}, q.options());
   Tensor gv = at::empty({p.Tk, p.Hk, p.D}, q.options());
   const int64_t wsb = tpo_attention_bwd_workspace_size(p.dt, p.B, p.Tq, p.Tk, p.Hq, p.Hk, p.D);
   const Tensor ws = workspace(wsb, q, op);
   check_rc(tpo_attention_bwd(p.dt, g.data_ptr(), p.q.data_ptr(), p.k.data_ptr(), p.v.data_ptr(),
-                             out.data_ptr(), lse.data_ptr<float>(), p.oq.data_ptr<int64_t>(),
+                             out.data_ptr(), data_or_null(rest), lse.data_ptr<float>(), p.oq.data_ptr<int64_t>(),
                              p.ok.data_ptr<int64_t>(), (const int64_t*)data_or_null(p.lq),
                              (const int64_t*)data_or_null(p.lk), p.B, p.Tq, p.Tk, p.Hq, p.Hk, p.D,
                              row_stride(p.q), head_stride(p.q), row_stride(p.k), head_stride(p.k),
@@ -327,13 +334,13 @@ class PackedAttentionFunction : public torch::autograd::Function<PackedAttention
   static Tensor forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v,
                         const Tensor& oq, const Tensor& ok, const OptTensor& lq,
                         const OptTensor& lk, bool causal, double scale) {
-    static auto op = typed_op<std::tuple<Tensor, Tensor>(
+    static auto op = typed_op<std::tuple<Tensor, Tensor, Tensor>(
         const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&,
         const OptTensor&, const OptTensor&, bool, double)>(
         "torch_point_ops_attention::packed_attention_forward");
     at::AutoDispatchBelowADInplaceOrView below;
-    auto [out, lse] = op.call(q, k, v, oq, ok, lq, lk, causal, scale);
-    ctx->save_for_backward({q, k, v, out, lse, oq, ok, get(lq), get(lk)});
+    auto [out, lse, rest] = op.call(q, k, v, oq, ok, lq, lk, causal, scale);
+    ctx->save_for_backward({q, k, v, out, lse, rest, oq, ok, get(lq), get(lk)});
     ctx->saved_data["causal"] = causal;
     ctx->saved_data["scale"] = scale;
     return out;
@@ -341,11 +348,11 @@ class PackedAttentionFunction : public torch::autograd::Function<PackedAttention
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     static auto op = typed_op<std::tuple<Tensor, Tensor, Tensor>(
         const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&,
-        const Tensor&, const Tensor&, const OptTensor&, const OptTensor&, bool, double)>(
-        "torch_point_ops_attention::packed_attention_backward");
+        const Tensor&, const Tensor&, const Tensor&, const OptTensor&, const OptTensor&, bool,
+        double)>("torch_point_ops_attention::packed_attention_backward");
     const auto s = ctx->get_saved_variables();
-    auto [gq, gk, gv] = op.call(grads[0], s[0], s[1], s[2], s[3], s[4], s[5], s[6], opt(s[7]),
-                                opt(s[8]), ctx->saved_data["causal"].toBool(),
+    auto [gq, gk, gv] = op.call(grads[0], s[0], s[1], s[2], s[3], s[4], s[5], s[6], s[7], opt(s[8]),
+                                opt(s[9]), ctx->saved_data["causal"].toBool(),
                                 ctx->saved_data["scale"].toDouble());
     const Tensor none;
     return {gq, gk, gv, none, none, none, none, none, none};
@@ -481,7 +488,7 @@ Tensor packed_attention_cpu(const Tensor&, const Tensor&, const Tensor&, const T
                             const Tensor&, const OptTensor&, const OptTensor&, bool, double) {
   TORCH_CHECK(false, "packed_attention is not implemented for CPU");
 }
-std::tuple<Tensor, Tensor> packed_attention_forward_cpu(const Tensor&, const Tensor&,
+std::tuple<Tensor, Tensor, Tensor> packed_attention_forward_cpu(const Tensor&, const Tensor&,
                                                         const Tensor&, const Tensor&,
                                                         const Tensor&, const OptTensor&,
                                                         const OptTensor&, bool, double) {
@@ -517,12 +524,13 @@ TORCH_LIBRARY_IMPL(torch_point_ops_norm, Autograd, m) {
 TORCH_LIBRARY(torch_point_ops_attention, m) {
   m.def("packed_attention(Tensor q, Tensor k, Tensor v, Tensor offsets_q, Tensor offsets_k, "
         "Tensor? lengths_q, Tensor? lengths_k, bool causal, float scale) -> Tensor");
-  // with the logarithm of each row's sum of exponentials
+  // with the logarithm of each row's sum of exponentials, and what rounding took
+  // from the result (half types)
   m.def("packed_attention_forward(Tensor q, Tensor k, Tensor v, Tensor offsets_q, "
         "Tensor offsets_k, Tensor? lengths_q, Tensor? lengths_k, bool causal, float scale) -> "
-        "(Tensor, Tensor)");
+        "(Tensor, Tensor, Tensor)");
   m.def("packed_attention_backward(Tensor grad, Tensor q, Tensor k, Tensor v, Tensor out, "
-        "Tensor lse, Tensor offsets_q, Tensor offsets_k, Tensor? lengths_q, Tensor? lengths_k, "
+        "Tensor lse, Tensor rest, Tensor offsets_q, Tensor offsets_k, Tensor? lengths_q, Tensor? lengths_k, "
         "bool causal, float scale) -> (Tensor, Tensor, Tensor)");
 }
 TORCH_LIBRARY_IMPL(torch_point_ops_attention, CPU, m) {

@@ -16,13 +16,14 @@ def _packed_attention_fake(q, k, v, offsets_q, offsets_k, lengths_q, lengths_k, 
 @torch.library.register_fake("torch_point_ops_attention::packed_attention_forward")
 def _packed_attention_forward_fake(q, k, v, offsets_q, offsets_k, lengths_q, lengths_k, causal,
                                    scale):
-    return (torch.empty(q.shape, device=q.device, dtype=q.dtype),
-            torch.empty(q.shape[1], q.shape[0], device=q.device, dtype=torch.float32))
+    out = torch.empty(q.shape, device=q.device, dtype=q.dtype)
+    return (out, torch.empty(q.shape[1], q.shape[0], device=q.device, dtype=torch.float32),
+            q.new_empty(0) if q.dtype == torch.float32 else torch.empty_like(out))
 
 
 @torch.library.register_fake("torch_point_ops_attention::packed_attention_backward")
-def _packed_attention_backward_fake(grad, q, k, v, out, lse, offsets_q, offsets_k, lengths_q,
-                                    lengths_k, causal, scale):
+def _packed_attention_backward_fake(grad, q, k, v, out, lse, rest, offsets_q, offsets_k,
+                                    lengths_q, lengths_k, causal, scale):
     return tuple(torch.empty(t.shape, device=t.device, dtype=t.dtype) for t in (q, k, v))
 
 
