@@ -98,19 +98,17 @@ __global__ __launch_bounds__(256, 2) void attn_prompt_kernel(AttnArgs a, const T
   constexpr int KT = KEYS<T>, TILE = PromptLds<T, DP>::TILE;
   __shared__ PromptLds<T, DP> lds;
   const int G = a.Hq / a.Hk, hk = blockIdx.x % a.Hk;
-  // late tiles of a sequence see the most keys: they go first
-  const int64_t place = gridDim.x / a.Hk - 1 - blockIdx.x / a.Hk;
-  const int s = attn_sequence(a.sq, place, G, 128);
+  int local;
+  const int s = attn_tile<true>(a.sq, blockIdx.x / a.Hk, gridDim.x / a.Hk, G, 128, local);
+  if (s < 0) return;
   const AttnSpan p = attn_span(a, s);
-  const int64_t local = uniform(place - attn_first(a.sq, s, G, 128));
   const int all = p.room_q * G;
-  if (local < 0 || local * 128 >= all) return;
-  const int w = wave_id(), l = lane_id(), r0 = (int)local * 128 + 32 * w, r = r0 + (l & 31);
+  const int w = wave_id(), l = lane_id(), r0 = local * 128 + 32 * w, r = r0 + (l & 31);
   const int used = p.Lq * G;
   // the wave's rows see between `least` and `most` keys, the workgroup's up to `end`
   auto keys = [&](int row) { return used ? attn_keys(a, p, row < used ? row : used - 1, G) : 0; };
   const int least = keys(r0), most = r0 < used ? keys(r0 + 31) : 0;
-  const int end = (int)local * 128 < used ? keys((int)local * 128 + 127) : 0;
+  const int end = local * 128 < used ? keys(local * 128 + 127) : 0;
   const int n = keys(r);
   const bool in = r < used;
   const int head = hk * G + r % G;

@@ -58,6 +58,72 @@ __device__ __forceinline__ int64_t uniform(int64_t v) {
   return (int64_t)((uint64_t)hi << 32 | lo);
 }
 
+// Tile number p in the order of falling size: a sequence of c tiles has one of
+// each size 1 .. c (a causal prompt's last tile sees the most keys, its first keys
+// are seen by the most rows).  Where workgroups are few, the long ones have to
+// start first: in the order of places a training step's dK and dV kept the CUs
+// busy for 58 % of its time.  A lane tries one size; sequences, at most 64 of
+// them, are passed round.  Returns the sequence, or -1, and the tile's size.
+__device__ __forceinline__ int attn_by_size(const Sequences& s, int p, int G, int tile, int& size) {
+  const int l = lane_id();
+  const int c = l < s.B + 2 ? (int)((s.room(l) * G + tile - 1) / tile) : 0;
+  int lo = 0, hi = 0;
+  for (int i = 0; i < s.B + 2; ++i) {
+    const int y = __builtin_amdgcn_readlane(c, i);
+    hi = y > hi ? y : hi;
+  }
+  // the smallest u of lo .. hi with n(u) <= p, n(u): tiles larger than u
+  while (hi > lo) {
+    const int step = (hi - lo + 63) >> 6, u = lo + l * step;
+    int n = 0;
+    for (int i = 0; i < s.B + 2; ++i) {
+      const int y = __builtin_amdgcn_readlane(c, i) - u;
+      n += y > 0 ? y : 0;
+    }
+    const uint64_t m = __builtin_amdgcn_ballot_w64(n <= p);
+    const int f = m ? __builtin_ctzll(m) : 64;
+    const int top = lo + f * step;
+    if (top < hi) hi = top;
+    if (f > 0) lo += (f - 1) * step + 1;
+    if (lo > hi) lo = hi;
+  }
+  size = lo;
+  if (lo == 0) return -1;
+  int n = 0;
+  for (int i = 0; i < s.B + 2; ++i) {
+    const int y = __builtin_amdgcn_readlane(c, i) - lo;
+    n += y > 0 ? y : 0;
+  }
+  const uint64_t m = __builtin_amdgcn_ballot_w64(c >= lo);
+  const int rank = __builtin_popcountll(m & ((1ull << l) - 1));
+  const uint64_t at = __builtin_amdgcn_ballot_w64(c >= lo && rank == p - n);
+  return at ? __builtin_ctzll(at) : -1;
+}
+
+// The sequence and tile of workgroup p, the largest first; -1: none.  LATE: a
+// sequence's last tile is its largest.
+template <bool LATE>
+__device__ __forceinline__ int attn_tile(const Sequences& s, int p, int places, int G, int tile,
+                                         int& local) {
+  int i;
+  if (s.B + 2 <= 64) {
+    int size;
+    i = attn_by_size(s, p, G, tile, size);
+    if (i < 0) return -1;
+    i = __builtin_amdgcn_readfirstlane(i);
+    const int c = (int)((uniform(s.room(i)) * G + tile - 1) / tile);
+    local = LATE ? size - 1 : c - size;
+  } else {  // many sequences: many workgroups
+    const int64_t place = LATE ? places - 1 - p : p;
+    i = attn_sequence(s, place, G, tile);
+    const int64_t n = uniform(place - attn_first(s, i, G, tile));
+    if (n < 0 || n * tile >= uniform(s.room(i)) * G) return -1;
+    local = (int)n;
+  }
+  return i;
+}
+
+
 // A workgroup's sequence: its queries and keys, and where they begin.
 struct AttnSpan {
   int64_t q0, k0;       // first rows in the packed arrays

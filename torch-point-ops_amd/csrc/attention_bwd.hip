@@ -93,17 +93,16 @@ __global__ __launch_bounds__(256, (DP * sizeof(T) <= 256 ? 2 : 1)) void attn_bwd
   constexpr int KT = KEYS<T>, TILE = PromptLds<T, DP>::TILE;
   __shared__ PromptLds<T, DP> lds;
   const int G = a.Hq / a.Hk, hk = blockIdx.x % a.Hk;
-  const int64_t place = gridDim.x / a.Hk - 1 - blockIdx.x / a.Hk;
-  const int s = attn_sequence(a.sq, place, G, 128);
+  int local;
+  const int s = attn_tile<true>(a.sq, blockIdx.x / a.Hk, gridDim.x / a.Hk, G, 128, local);
+  if (s < 0) return;
   const AttnSpan p = attn_span(a, s);
-  const int64_t local = uniform(place - attn_first(a.sq, s, G, 128));
   const int all = p.room_q * G;
-  if (local < 0 || local * 128 >= all) return;
-  const int w = wave_id(), l = lane_id(), r0 = (int)local * 128 + 32 * w, r = r0 + (l & 31);
+  const int w = wave_id(), l = lane_id(), r0 = local * 128 + 32 * w, r = r0 + (l & 31);
   const int used = p.Lq * G;
   auto keys = [&](int row) { return used ? attn_keys(a, p, row < used ? row : used - 1, G) : 0; };
   const int least = keys(r0), most = r0 < used ? keys(r0 + 31) : 0;
-  const int end = (int)local * 128 < used ? keys((int)local * 128 + 127) : 0;
+  const int end = local * 128 < used ? keys(local * 128 + 127) : 0;
   const int n = keys(r);
   const bool in = r < used;
   const int head = hk * G + r % G;
@@ -226,12 +225,11 @@ __global__ __launch_bounds__(256, (DP * sizeof(T) <= 128 ? 2 : 1)) void attn_bwd
   constexpr int KT = KEYS<T>, STAGE = BwdKeysLds<T, DP>::STAGE;
   __shared__ BwdKeysLds<T, DP> lds;
   const int G = a.Hq / a.Hk, hk = blockIdx.x % a.Hk;
-  const int64_t place = blockIdx.x / a.Hk;  // early keys, which most rows see, go first
-  const int s = attn_sequence(a.sk, place, 1, 128);
+  int local;
+  const int s = attn_tile<false>(a.sk, blockIdx.x / a.Hk, gridDim.x / a.Hk, 1, 128, local);
+  if (s < 0) return;
   const AttnSpan p = attn_span(a, s);
-  const int64_t local = uniform(place - attn_first(a.sk, s, 1, 128));
-  if (local < 0 || local * 128 >= p.room_k) return;
-  const int w = wave_id(), l = lane_id(), b0 = (int)local * 128, j0 = b0 + 32 * w, j = j0 + (l & 31);
+  const int w = wave_id(), l = lane_id(), b0 = local * 128, j0 = b0 + 32 * w, j = j0 + (l & 31);
   const bool in = j < p.Lk;
   HeadRows<T, DP> x, y;
   x.load(k + (p.k0 + j) * a.k_row + hk * a.k_head, in, a.D);
