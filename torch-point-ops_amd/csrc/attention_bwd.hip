@@ -140,19 +140,22 @@ __global__ __launch_bounds__(256, (DP * sizeof(T) <= 256 ? 2 : 1)) void attn_bwd
                   all);
 }
 
-// A tile of rows of q and of go, and what is theirs of sub and delta.
+// A tile of 64 rows of q and of go, and what is theirs of sub and delta; later
+// the sums that the waves exchange, and the rows on their way out.
+constexpr int BWD_ROWS = 64;
 template <typename T, int DP>
 struct alignas(1024) BwdKeysLds {
-  static constexpr int TILE = KEYS<T> * HeadLds<T, DP>::PITCH;
+  static constexpr int TILE = BWD_ROWS * HeadLds<T, DP>::PITCH;
   static constexpr int STAGE = 2 * TILE + 1024;
-  static constexpr int OUT = 4 * Rows32<T, DP>::BYTES;
-  char b[2 * STAGE > OUT ? 2 * STAGE : OUT];
+  static constexpr int OUT = 4 * Rows32<T, DP>::BYTES, SUMS = 4 * DP * 128;
+  static constexpr int MORE = OUT > SUMS ? OUT : SUMS;
+  char b[2 * STAGE > MORE ? 2 * STAGE : MORE];
 };
 
 template <typename T, int DP>
 __device__ __forceinline__ void bwd_keys_load(char* to, const T* q, const T* go, const float* sub,
                                               const float* delta, const AttnArgs& a, int left) {
-  constexpr int KT = KEYS<T>, TILE = BwdKeysLds<T, DP>::TILE;
+  constexpr int KT = BWD_ROWS, TILE = BwdKeysLds<T, DP>::TILE;
   typedef HeadLds<T, DP> L;
   const int w = wave_id();
   L::template load<KT, 4>(to, q, (int)(a.q_row * sizeof(T)), left, a.D, w);
@@ -170,66 +173,66 @@ struct KeySums {
   f32x16 k[DP / 32], v[DP / 32];
 };
 
-// The products of a tile of rows (from row i0 on, `left` of them in use) with the
-// wave's keys, of which the lane's is seen by rows from `lo` on, the wave's by
-// rows between least and most on.  only: the row that sees a single key (every
-// row: ALL_ROWS).
+// The products of half a tile's rows (half t; the tile from row i0 on, `left` of
+// its rows in use) with the wave's keys, of which the lane's is seen by rows from
+// `lo` on, the wave's by rows between least and most on.  only: the row that sees
+// a single key (every row: ALL_ROWS).
 constexpr int ALL_ROWS = INT32_MIN;
 template <typename T, int DP>
 __device__ __forceinline__ void bwd_keys_step(const char* __restrict__ cur, char* __restrict__ nxt,
                                               const T* q, const T* go, const float* sub,
                                               const float* delta, const AttnArgs& a, int next,
                                               const HeadRows<T, DP>& k, const HeadRows<T, DP>& v,
-                                              KeySums<T, DP>& sums, int i0, int left, int lo,
-                                              int least, int most, int only, float c) {
-  constexpr int KT = KEYS<T>, TILE = BwdKeysLds<T, DP>::TILE;
+                                              KeySums<T, DP>& sums, int t, int i0, int left,
+                                              int lo, int least, int most, int only, float c) {
+  constexpr int TILE = BwdKeysLds<T, DP>::TILE;
   bwd_keys_load<T, DP>(nxt, q, go, sub, delta, a, next);
   __builtin_amdgcn_sched_barrier(0);
   const int h = lane_id() >> 5;
+  const int i = i0 + 32 * t;
+  if (i + 32 <= least || 32 * t >= left) return;
+  f32x16 s = scores<T, DP>(cur, 32 * t, k);
+  f32x16 d = scores<T, DP>(cur + TILE, 32 * t, v);
+  const bool masked = i < most || 32 * t + 32 > left || only == ALL_ROWS;
+  const float* ps = (const float*)(cur + 2 * TILE) + 32 * t + 4 * h;
 #pragma unroll
-  for (int t = 0; t < KT / 32; ++t) {
-    const int i = i0 + 32 * t;
-    if (i + 32 <= least || 32 * t >= left) continue;
-    f32x16 s = scores<T, DP>(cur, 32 * t, k);
-    f32x16 d = scores<T, DP>(cur + TILE, 32 * t, v);
-    const bool masked = i < most || 32 * t + 32 > left || only == ALL_ROWS;
-    const float* ps = (const float*)(cur + 2 * TILE) + 32 * t + 4 * h;
+  for (int b = 0; b < 4; ++b) {
+    const f32x4 m = *(const f32x4*)(ps + 8 * b), y = *(const f32x4*)(ps + 64 + 8 * b);
 #pragma unroll
-    for (int b = 0; b < 4; ++b) {
-      const f32x4 m = *(const f32x4*)(ps + 8 * b), y = *(const f32x4*)(ps + 64 + 8 * b);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        s[4 * b + e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[4 * b + e], c, -m[e]));
-        d[4 * b + e] = s[4 * b + e] * (d[4 * b + e] - y[e]);
-      }
+    for (int e = 0; e < 4; ++e) {
+      s[4 * b + e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[4 * b + e], c, -m[e]));
+      d[4 * b + e] = s[4 * b + e] * (d[4 * b + e] - y[e]);
     }
-    if (masked)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const int row = 32 * t + 8 * (e >> 2) + 4 * h + (e & 3);
-        if (i0 + row == only || only == ALL_ROWS) d[e] = 0.f;
-        if (i0 + row < lo || row >= left) s[e] = d[e] = 0.f;
-      }
-    multiply_rows<T, DP>(sums.v, cur + TILE, 32 * t, s);
-    multiply_rows<T, DP>(sums.k, cur, 32 * t, d);
   }
+  if (masked)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const int row = 32 * t + 8 * (e >> 2) + 4 * h + (e & 3);
+      if (i0 + row == only || only == ALL_ROWS) d[e] = 0.f;
+      if (i0 + row < lo || row >= left) s[e] = d[e] = 0.f;
+    }
+  multiply_rows<T, DP>(sums.v, cur + TILE, 32 * t, s);
+  multiply_rows<T, DP>(sums.k, cur, 32 * t, d);
 }
 
-// dK and dV of 128 keys, 32 a wave: for each head of the group, the rows that see
-// them in tiles that all four waves share.
+// dK and dV of 64 keys: for each head of the group, the rows that see them in
+// tiles that all four waves share.  Wave w has keys 32 (w % 2) .. + 31 and half w /
+// 2 of each tile's rows; at the end two waves add what they have, one stores dK,
+// one dV.  (128 keys with all rows a wave: half as many workgroups of twice the
+// length, 128 us where this takes KEYS_US for 8 x 2048.)
 template <typename T, int DP>
 __global__ __launch_bounds__(256, (DP * sizeof(T) <= 128 ? 2 : 1)) void attn_bwd_keys_kernel(
     AttnArgs a, const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ v,
     const T* __restrict__ go, const float* __restrict__ sub, const float* __restrict__ delta,
     T* __restrict__ gk, T* __restrict__ gv) {
-  constexpr int KT = KEYS<T>, STAGE = BwdKeysLds<T, DP>::STAGE;
+  constexpr int KT = BWD_ROWS, STAGE = BwdKeysLds<T, DP>::STAGE;
   __shared__ BwdKeysLds<T, DP> lds;
   const int G = a.Hq / a.Hk, hk = blockIdx.x % a.Hk;
   int local;
-  const int s = attn_tile<false>(a.sk, blockIdx.x / a.Hk, gridDim.x / a.Hk, 1, 128, local);
+  const int s = attn_tile<false>(a.sk, blockIdx.x / a.Hk, gridDim.x / a.Hk, 1, 64, local);
   if (s < 0) return;
   const AttnSpan p = attn_span(a, s);
-  const int w = wave_id(), l = lane_id(), b0 = local * 128, j0 = b0 + 32 * w, j = j0 + (l & 31);
+  const int w = wave_id(), l = lane_id(), b0 = local * 64, j0 = b0 + 32 * (w & 1), j = j0 + (l & 31);
   const bool in = j < p.Lk;
   HeadRows<T, DP> x, y;
   x.load(k + (p.k0 + j) * a.k_row + hk * a.k_head, in, a.D);
@@ -268,28 +271,49 @@ __global__ __launch_bounds__(256, (DP * sizeof(T) <= 128 ? 2 : 1)) void attn_bwd
       const int left = ng < G ? end - ni : 0;
       at(ng < G ? ng : g, ni, [&](const T* q0, const T* g0, const float* s0, const float* d0) {
         bwd_keys_step<T, DP>(lds.b + half * STAGE, lds.b + (half ^ 1) * STAGE, q0, g0, s0, d0, a,
-                             left, x, y, sums, i, end - i, lo, least, most, only, c);
+                             left, x, y, sums, w >> 1, i, end - i, lo, least, most, only, c);
       });
       half ^= 1;
     }
   wait_loads_and_meet<0>();
-  if (j0 >= p.room_k) return;
-  typedef Rows32<T, DP> R;
-  const R to{lds.b + w * R::BYTES};
-  auto put = [&](const f32x16(&acc)[DP / 32], float f, T* out) {
+  // waves 0 and 1 take dK from waves 2 and 3 and give them their dV
+  f32x16(&own)[DP / 32] = w < 2 ? sums.k : sums.v;
+  {
+    const f32x16(&give)[DP / 32] = w < 2 ? sums.v : sums.k;
+    f32x4* to = (f32x4*)(lds.b + w * DP * 128) + l;
+#pragma unroll
+    for (int i = 0; i < DP / 32; ++i)
+#pragma unroll
+      for (int b = 0; b < 4; ++b)
+        to[(4 * i + b) * 64] = f32x4{give[i][4 * b], give[i][4 * b + 1], give[i][4 * b + 2],
+                                     give[i][4 * b + 3]};
+    __syncthreads();
+    const f32x4* from = (const f32x4*)(lds.b + (w ^ 2) * DP * 128) + l;
 #pragma unroll
     for (int i = 0; i < DP / 32; ++i)
 #pragma unroll
       for (int b = 0; b < 4; ++b) {
-        Four<T> z;
+        const f32x4 y = from[(4 * i + b) * 64];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) z.v[e] = in ? (T)(acc[i][4 * b + e] * f) : (T)0.f;
-        *(Four<T>*)to.four(32 * i + 8 * b + 4 * (l >> 5)) = z;
+        for (int e = 0; e < 4; ++e) own[i][4 * b + e] += y[e];
       }
-    to.store(out + hk * a.D, (int64_t)a.Hk * a.D, p.k0 + j0, p.k0 + p.room_k, 0, a.D, true);
-  };
-  put(sums.k, a.scale, gk);
-  put(sums.v, 1.f, gv);
+    __syncthreads();
+  }
+  if (j0 >= p.room_k) return;
+  typedef Rows32<T, DP> R;
+  const R to{lds.b + w * R::BYTES};
+  const float f = w < 2 ? a.scale : 1.f;
+#pragma unroll
+  for (int i = 0; i < DP / 32; ++i)
+#pragma unroll
+    for (int b = 0; b < 4; ++b) {
+      Four<T> z;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) z.v[e] = in ? (T)(own[i][4 * b + e] * f) : (T)0.f;
+      *(Four<T>*)to.four(32 * i + 8 * b + 4 * (l >> 5)) = z;
+    }
+  to.store((w < 2 ? gk : gv) + hk * a.D, (int64_t)a.Hk * a.D, p.k0 + j0, p.k0 + p.room_k, 0, a.D,
+           true);
 }
 
 }  // namespace tpo
@@ -325,7 +349,7 @@ extern "C" int tpo_attention_bwd(int dtype, const void* grad_out, const void* q,
   const AttnArgs a = attn_args(offsets_q, offsets_k, lengths_q, lengths_k, B, Tq, Tk, Hq, Hk, D,
                                q_row, q_head, k_row, k_head, v_row, v_head, causal, scale);
   const int64_t rows = Tq * Hq, G = Hq / Hk;
-  const int64_t places_q = attn_places(Tq, G, B, 128), places_k = attn_places(Tk, 1, B, 128);
+  const int64_t places_q = attn_places(Tq, G, B, 128), places_k = attn_places(Tk, 1, B, 64);
   if (places_q * Hk >= ((int64_t)1 << 31) || places_k * Hk >= ((int64_t)1 << 31))
     return set_error(TPO_ERR_ARG, "attention_bwd: too many rows");
   float *sub = (float*)workspace, *delta = (float*)((char*)workspace + need / 2);
