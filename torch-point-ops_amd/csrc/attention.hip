@@ -27,14 +27,16 @@ struct RowSums {
     m = NEG_INF;
     l = 0.f;
   }
-  // KT keys from j0 on, of which the lane's row sees those below n; c: what a
-  // score counts in the exponent of 2
+  // KT keys from j0 on (k at lds, v after it), of which the lane's row sees those
+  // below n; c: what a score counts in the exponent of 2
   template <int KT>
-  __device__ __forceinline__ void add(const char* k, const char* v, const HeadRows<T, DP>& q,
-                                      int j0, int n, bool masked, float c) {
+  __device__ __forceinline__ void add(const HeadLanes<T, DP>& lanes, const char* lds,
+                                      const HeadRows<T, DP>& q, int j0, int n, bool masked,
+                                      float c) {
+    constexpr int PITCH = HeadLds<T, DP>::PITCH;
     f32x16 s[KT / 32];
 #pragma unroll
-    for (int t = 0; t < KT / 32; ++t) s[t] = scores<T, DP>(k, 32 * t, q);
+    for (int t = 0; t < KT / 32; ++t) s[t] = scores<T, DP>(lanes, lds + 32 * t * PITCH, q);
     if (masked) {
       const int first = j0 + 4 * (lane_id() >> 5);
 #pragma unroll
@@ -68,14 +70,16 @@ struct RowSums {
         l += s[t][e];
       }
 #pragma unroll
-    for (int t = 0; t < KT / 32; ++t) multiply_rows<T, DP>(acc, v, 32 * t, s[t]);
+    for (int t = 0; t < KT / 32; ++t)
+      multiply_rows<T, DP>(acc, lanes, lds + (KT + 32 * t) * PITCH, s[t]);
   }
 };
 
 // The loads of a tile of keys and one's products, in parts of LDS that are apart.
 template <typename T, int DP>
 __device__ __forceinline__ void prompt_step(const char* __restrict__ cur, char* __restrict__ nxt,
-                                            const T* k, const T* v, const AttnArgs& a, int left,
+                                            const HeadLanes<T, DP>& lanes, const T* k, const T* v,
+                                            const AttnArgs& a, int left,
                                             const HeadRows<T, DP>& q, RowSums<T, DP>& rows, int j0,
                                             int n, int least, int most, float c) {
   constexpr int KT = KEYS<T>, TILE = PromptLds<T, DP>::TILE;
@@ -83,7 +87,7 @@ __device__ __forceinline__ void prompt_step(const char* __restrict__ cur, char* 
   L::template load<KT, 4>(nxt, k, (int)(a.k_row * sizeof(T)), left, a.D, wave_id());
   L::template load<KT, 4>(nxt + TILE, v, (int)(a.v_row * sizeof(T)), left, a.D, wave_id());
   __builtin_amdgcn_sched_barrier(0);
-  if (j0 < most) rows.template add<KT>(cur, cur + TILE, q, j0, n, j0 + KT > least, c);
+  if (j0 < most) rows.template add<KT>(lanes, cur, q, j0, n, j0 + KT > least, c);
 }
 
 // Prompts: a workgroup of four waves takes 128 rows, 32 a wave, and all their
@@ -126,14 +130,18 @@ __global__ __launch_bounds__(256, 2) void attn_prompt_kernel(AttnArgs a, const T
     L::template load<KT, 4>(lds.b, kt, (int)(a.k_row * sizeof(T)), p.Lk, a.D, w);
     L::template load<KT, 4>(lds.b + TILE, vt, (int)(a.v_row * sizeof(T)), p.Lk, a.D, w);
   }
-  int half = 0;
-  for (int j0 = 0; j0 < end; j0 += KT) {
+  const HeadLanes<T, DP> lanes;
+  auto step = [&](auto half, int j0) {  // (the halves by name: LDS addresses are constants)
+    constexpr int H = decltype(half)::value;
     wait_loads_and_meet<0>();
     kt += KT * a.k_row;
     vt += KT * a.v_row;
-    prompt_step<T, DP>(lds.b + half * 2 * TILE, lds.b + (half ^ 1) * 2 * TILE, kt, vt, a,
+    prompt_step<T, DP>(lds.b + H * 2 * TILE, lds.b + (1 - H) * 2 * TILE, lanes, kt, vt, a,
                        j0 + KT < end ? p.Lk - j0 - KT : 0, x, rows, j0, n, least, most, c);
-    half ^= 1;
+  };
+  for (int j0 = 0; j0 < end; j0 += 2 * KT) {
+    step(std::integral_constant<int, 0>(), j0);
+    if (j0 + KT < end) step(std::integral_constant<int, 1>(), j0 + KT);
   }
   wait_loads_and_meet<0>();
   if (r0 >= all) return;
@@ -170,7 +178,7 @@ __device__ __forceinline__ void step_load(char* to, const T* k, const T* v, cons
 }
 template <typename T, int DP>
 __device__ __forceinline__ void step_step(const char* __restrict__ cur, char* __restrict__ nxt,
-                                          const T* k, const T* v, const AttnArgs& a, int left,
+                                          const HeadLanes<T, DP>& lanes, const T* k, const T* v, const AttnArgs& a, int left,
                                           const HeadRows<T, DP>& q, RowSums<T, DP>& rows, int j0,
                                           int n, int least, float c) {
   constexpr int TILE = StepLds<T, DP>::TILE, N = 2 * TILE / 1024;  // loads a tile
@@ -180,7 +188,7 @@ __device__ __forceinline__ void step_step(const char* __restrict__ cur, char* __
   __builtin_amdgcn_s_waitcnt((N & 15) | (N >> 4) << 14 | 0xf70);  // the tile itself has landed
   asm volatile("" ::: "memory");
   __builtin_amdgcn_sched_barrier(0);
-  rows.template add<32>(cur, cur + TILE, q, j0, n, j0 + 32 > least, c);
+  rows.template add<32>(lanes, cur, q, j0, n, j0 + 32 > least, c);
 }
 
 // part: with shares, each row's sums (D floats, not divided), and in ml their
@@ -220,6 +228,7 @@ __global__ __launch_bounds__((64 * STEP_WAVES<T, DP>)) void attn_step_kernel(
     step_load<T, DP>(mine, kt + (int64_t)t * 32 * a.k_row, vt + (int64_t)t * 32 * a.v_row, a,
                      t < t1 ? most - t * 32 : 0);
   };
+  const HeadLanes<T, DP> lanes;
   if (t0 + w < t1) load(t0 + w);
   int half = 0;
   for (int t = t0 + w; t < t1; t += W) {
@@ -227,7 +236,7 @@ __global__ __launch_bounds__((64 * STEP_WAVES<T, DP>)) void attn_step_kernel(
     asm volatile("" ::: "memory");
     __builtin_amdgcn_s_waitcnt(0xc07f);  // the other tile's reads have ended
     const int64_t next = t + W;
-    step_step<T, DP>(mine + half * 2 * TILE, mine + (half ^ 1) * 2 * TILE,
+    step_step<T, DP>(mine + half * 2 * TILE, mine + (half ^ 1) * 2 * TILE, lanes,
                      kt + next * 32 * a.k_row, vt + next * 32 * a.v_row, a,
                      next < t1 ? most - (int)next * 32 : 0, x, rows, t * 32, n, least, c);
     half ^= 1;

@@ -177,59 +177,73 @@ struct HeadLds {
                row * row_bytes);
     }
   }
-  // rows row0 + l % 32, chunk 2 s + l / 32
-  static __device__ __forceinline__ typename Chunk<T>::V by_row(const char* lds, int row0, int s) {
-    const int l = lane_id(), r = l & 31;
-    return *(const typename Chunk<T>::V*)(lds + (row0 + r) * PITCH +
-                                          (((2 * s + (l >> 5)) ^ swap(r)) << 4));
+};
+
+// Where a lane reads, from the start of a tile's rows: as numbers that are made
+// once, so that a read in the loop is one instruction with a constant offset.
+template <typename T, int DP>
+struct HeadLanes {
+  typedef HeadLds<T, DP> L;
+  typedef typename Chunk<T>::V V;
+  static constexpr int N = DP * L::Z / 32, M = DP / 32, PITCH = L::PITCH;
+  int row[N];        // row l % 32, chunk 2 s + l / 32
+  int lo[M], hi[M];  // half types: see by_col; float: lo[0]
+
+  __device__ __forceinline__ HeadLanes() {
+    const int l = lane_id(), h = l >> 5, r = l & 31;
+#pragma unroll
+    for (int s = 0; s < N; ++s) row[s] = r * PITCH + (((2 * s + h) ^ L::swap(r)) << 4);
+    if constexpr (L::Z == 4) {
+      lo[0] = 4 * h * PITCH + ((((l & 31) >> 2) ^ L::swap(4 * h)) << 4) + (l & 3) * 4;
+    } else {
+      const int e = l & 15, g = (l >> 4) & 1, q = 4 * h + (e >> 2), c = 2 * g + (e >> 1 & 1);
+#pragma unroll
+      for (int i = 0; i < M; ++i) {
+        lo[i] = q * PITCH + 8 * (e & 1) + (((c ^ L::swap(q)) << 4) ^ (64 * i));
+        hi[i] = (q + 8) * PITCH + 8 * (e & 1) + (((c ^ L::swap(q + 8)) << 4) ^ (64 * i));
+      }
+    }
   }
-  // half types: value 32 i + l % 32 of the rows row0 + 16 s + 4 (l / 32) + 0 .. 3
-  // and + 8 .. 11
-  static __device__ __forceinline__ typename Chunk<T>::V by_col(const char* lds, int row0, int s,
-                                                                int i) {
-    static_assert(Z == 2, "half types");
+  // chunk 2 s + l / 32 of row l % 32 of the rows at lds
+  __device__ __forceinline__ V by_row(const char* lds, int s) const {
+    return *(const V*)(lds + row[s]);
+  }
+  // half types: value 32 i + l % 32 of the rows 16 s + 4 (l / 32) + 0 .. 3 and + 8 ..
+  // 11: sixteen lanes give the addresses of 4 rows x 16 columns and get a column each
+  __device__ __forceinline__ V by_col(const char* lds, int s, int i) const {
+    static_assert(L::Z == 2, "half types");
     typedef __attribute__((address_space(3))) i16x4 lds_i16x4;
-    const int l = lane_id(), e = l & 15, g = (l >> 4) & 1, h = l >> 5, q = e >> 2;
-    const int r = 4 * h + q, c = 2 * g + (e >> 1 & 1);
-    const char* at = lds + ((row0 + 16 * s + r) * PITCH + 8 * (e & 1));
-    const int base = (int)(uintptr_t)(lds_t*)at;
-    const int a0 = base + (((c ^ swap(r)) << 4) ^ (64 * i));
-    const int a1 = base + 8 * PITCH + (((c ^ swap(r + 8)) << 4) ^ (64 * i));
-    const i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(uintptr_t)a0);
-    const i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(uintptr_t)a1);
-    return __builtin_bit_cast(typename Chunk<T>::V,
-                              __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+    lds += 16 * s * PITCH;
+    const i16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(lds + lo[i]));
+    const i16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(lds + hi[i]));
+    return __builtin_bit_cast(V, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
   }
-  // float: value 32 i + l % 32 of row row0 + 8 (v / 4) + 4 (l / 32) + v % 4
-  static __device__ __forceinline__ float by_col1(const char* lds, int row0, int v, int i) {
-    const int l = lane_id(), r = row0 + 8 * (v >> 2) + 4 * (l >> 5) + (v & 3);
-    const int c = (8 * i + ((l & 31) >> 2)) ^ swap(r);
-    return *(const float*)(lds + r * PITCH + (c << 4) + (l & 3) * 4);
+  // float: value 32 i + l % 32 of row 8 (v / 4) + 4 (l / 32) + v % 4
+  __device__ __forceinline__ float by_col1(const char* lds, int v, int i) const {
+    const int r = 8 * (v >> 2) + (v & 3);
+    return *(const float*)(lds + r * PITCH + (lo[0] ^ (L::swap(r) << 4) ^ (128 * i)));
   }
 };
 
-// acc[i] += X^T P^T over 32 rows of X (in LDS by column) from row0 on: sums of
-// value 32 i + .. of X times the lane's sixteen p.  Half types round p to the type.
+// acc[i] += X^T P^T over the 32 rows of X at lds: sums of value
+// 32 i + .. of X times the lane's sixteen p.  Half types round p to the type.
 template <typename T, int DP>
-__device__ __forceinline__ void multiply_rows(f32x16 (&acc)[DP / 32], const char* lds, int row0,
-                                              const f32x16& p) {
-  typedef HeadLds<T, DP> L;
+__device__ __forceinline__ void multiply_rows(f32x16 (&acc)[DP / 32], const HeadLanes<T, DP>& x,
+                                              const char* lds, const f32x16& p) {
   if constexpr (sizeof(T) == 4) {
 #pragma unroll
     for (int v = 0; v < 16; ++v)
 #pragma unroll
       for (int i = 0; i < DP / 32; ++i)
-        acc[i] = __builtin_amdgcn_mfma_f32_32x32x2f32(L::by_col1(lds, row0, v, i), p[v], acc[i], 0,
-                                                      0, 0);
+        acc[i] = __builtin_amdgcn_mfma_f32_32x32x2f32(x.by_col1(lds, v, i), p[v], acc[i], 0, 0, 0);
   } else {
-    typedef typename Chunk<T>::V V;
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
-      V x;
+      typename Chunk<T>::V y;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] = (T)p[8 * s + e];
+      for (int e = 0; e < 8; ++e) y[e] = (T)p[8 * s + e];
 #pragma unroll
-      for (int i = 0; i < DP / 32; ++i) mma(acc[i], L::by_col(lds, row0, s, i), x);
+      for (int i = 0; i < DP / 32; ++i) mma(acc[i], x.by_col(lds, s, i), y);
     }
   }
 }
@@ -312,13 +326,13 @@ struct alignas(1024) PromptLds {
   char b[4 * TILE > OUT ? 4 * TILE : OUT];
 };
 
-// X Y^T of 32 rows of X in LDS and the wave's rows: the transposed scores.
+// X Y^T of the 32 rows of X at lds and the wave's rows: transposed scores.
 template <typename T, int DP>
-__device__ __forceinline__ f32x16 scores(const char* lds, int row0, const HeadRows<T, DP>& y) {
+__device__ __forceinline__ f32x16 scores(const HeadLanes<T, DP>& x, const char* lds,
+                                         const HeadRows<T, DP>& y) {
   f32x16 s = {};
 #pragma unroll
-  for (int c = 0; c < HeadRows<T, DP>::N; ++c)
-    mma(s, HeadLds<T, DP>::by_row(lds, row0, c), y.x[c]);
+  for (int c = 0; c < HeadRows<T, DP>::N; ++c) mma(s, x.by_row(lds, c), y.x[c]);
   return s;
 }
 

@@ -54,11 +54,11 @@ __global__ __launch_bounds__(256) void attn_delta_kernel(const T* __restrict__ o
 
 template <typename T, int DP>
 __device__ __forceinline__ void bwd_q_step(const char* __restrict__ cur, char* __restrict__ nxt,
-                                           const T* k, const T* v, const AttnArgs& a, int left,
+                                           const HeadLanes<T, DP>& lanes, const T* k, const T* v, const AttnArgs& a, int left,
                                            const HeadRows<T, DP>& q, const HeadRows<T, DP>& go,
                                            f32x16 (&acc)[DP / 32], int j0, int n, int least,
                                            int most, float c, float sub, float delta) {
-  constexpr int KT = KEYS<T>, TILE = PromptLds<T, DP>::TILE;
+  constexpr int KT = KEYS<T>, TILE = PromptLds<T, DP>::TILE, PITCH = HeadLds<T, DP>::PITCH;
   typedef HeadLds<T, DP> L;
   L::template load<KT, 4>(nxt, k, (int)(a.k_row * sizeof(T)), left, a.D, wave_id());
   L::template load<KT, 4>(nxt + TILE, v, (int)(a.v_row * sizeof(T)), left, a.D, wave_id());
@@ -66,8 +66,8 @@ __device__ __forceinline__ void bwd_q_step(const char* __restrict__ cur, char* _
 #pragma unroll
   for (int t = 0; t < KT / 32; ++t) {
     if (j0 + 32 * t >= most) break;
-    f32x16 s = scores<T, DP>(cur, 32 * t, q);
-    const f32x16 d = scores<T, DP>(cur + TILE, 32 * t, go);
+    f32x16 s = scores<T, DP>(lanes, cur + 32 * t * PITCH, q);
+    const f32x16 d = scores<T, DP>(lanes, cur + TILE + 32 * t * PITCH, go);
     const bool masked = j0 + 32 * t + 32 > least;
     const int first = j0 + 32 * t + 4 * (lane_id() >> 5);
 #pragma unroll
@@ -79,7 +79,7 @@ __device__ __forceinline__ void bwd_q_step(const char* __restrict__ cur, char* _
 #pragma unroll
       for (int e = 0; e < 16; ++e)
         if (first + 8 * (e >> 2) + (e & 3) >= n) s[e] = 0.f;
-    multiply_rows<T, DP>(acc, cur, 32 * t, s);
+    multiply_rows<T, DP>(acc, lanes, cur + 32 * t * PITCH, s);
   }
 }
 
@@ -124,15 +124,19 @@ __global__ __launch_bounds__(256, (DP * sizeof(T) <= 256 ? 2 : 1)) void attn_bwd
     L::template load<KT, 4>(lds.b, kt, (int)(a.k_row * sizeof(T)), p.Lk, a.D, w);
     L::template load<KT, 4>(lds.b + TILE, vt, (int)(a.v_row * sizeof(T)), p.Lk, a.D, w);
   }
-  int half = 0;
-  for (int j0 = 0; j0 < end; j0 += KT) {
+  const HeadLanes<T, DP> lanes;
+  auto step = [&](auto half, int j0) {
+    constexpr int H = decltype(half)::value;
     wait_loads_and_meet<0>();
     kt += KT * a.k_row;
     vt += KT * a.v_row;
-    bwd_q_step<T, DP>(lds.b + half * 2 * TILE, lds.b + (half ^ 1) * 2 * TILE, kt, vt, a,
+    bwd_q_step<T, DP>(lds.b + H * 2 * TILE, lds.b + (1 - H) * 2 * TILE, lanes, kt, vt, a,
                       j0 + KT < end ? p.Lk - j0 - KT : 0, x, y, acc, j0, n, least, most, c, row_sub,
                       row_delta);
-    half ^= 1;
+  };
+  for (int j0 = 0; j0 < end; j0 += 2 * KT) {
+    step(std::integral_constant<int, 0>(), j0);
+    if (j0 + KT < end) step(std::integral_constant<int, 1>(), j0 + KT);
   }
   wait_loads_and_meet<0>();
   if (r0 >= all) return;
@@ -180,19 +184,20 @@ struct KeySums {
 constexpr int ALL_ROWS = INT32_MIN;
 template <typename T, int DP>
 __device__ __forceinline__ void bwd_keys_step(const char* __restrict__ cur, char* __restrict__ nxt,
-                                              const T* q, const T* go, const float* sub,
+                                              const HeadLanes<T, DP>& lanes, const T* q, const T* go, const float* sub,
                                               const float* delta, const AttnArgs& a, int next,
                                               const HeadRows<T, DP>& k, const HeadRows<T, DP>& v,
                                               KeySums<T, DP>& sums, int t, int i0, int left,
                                               int lo, int least, int most, int only, float c) {
-  constexpr int TILE = BwdKeysLds<T, DP>::TILE;
+  constexpr int TILE = BwdKeysLds<T, DP>::TILE, PITCH = HeadLds<T, DP>::PITCH;
   bwd_keys_load<T, DP>(nxt, q, go, sub, delta, a, next);
   __builtin_amdgcn_sched_barrier(0);
   const int h = lane_id() >> 5;
   const int i = i0 + 32 * t;
   if (i + 32 <= least || 32 * t >= left) return;
-  f32x16 s = scores<T, DP>(cur, 32 * t, k);
-  f32x16 d = scores<T, DP>(cur + TILE, 32 * t, v);
+  const char* at = cur + 32 * t * PITCH;
+  f32x16 s = scores<T, DP>(lanes, at, k);
+  f32x16 d = scores<T, DP>(lanes, at + TILE, v);
   const bool masked = i < most || 32 * t + 32 > left || only == ALL_ROWS;
   const float* ps = (const float*)(cur + 2 * TILE) + 32 * t + 4 * h;
 #pragma unroll
@@ -211,8 +216,8 @@ __device__ __forceinline__ void bwd_keys_step(const char* __restrict__ cur, char
       if (i0 + row == only || only == ALL_ROWS) d[e] = 0.f;
       if (i0 + row < lo || row >= left) s[e] = d[e] = 0.f;
     }
-  multiply_rows<T, DP>(sums.v, cur + TILE, 32 * t, s);
-  multiply_rows<T, DP>(sums.k, cur, 32 * t, d);
+  multiply_rows<T, DP>(sums.v, lanes, at + TILE, s);
+  multiply_rows<T, DP>(sums.k, lanes, at, d);
 }
 
 // dK and dV of 64 keys: for each head of the group, the rows that see them in
@@ -252,29 +257,50 @@ __global__ __launch_bounds__(256, (DP * sizeof(T) <= 128 ? 2 : 1)) void attn_bwd
 #pragma unroll
   for (int i = 0; i < DP / 32; ++i) sums.k[i] = sums.v[i] = f32x16{};
   const int tiles = start < end ? (end - start + KT - 1) / KT : 0;
-  // tile n of all heads' is rows start + n % tiles * KT of head n / tiles
-  auto at = [&](int g, int i, auto&& f) {
-    const int64_t head = hk * G + g, row = p.q0 + i;
-    f(q + row * a.q_row + head * a.q_head, go + (row * a.Hq + head) * a.D, sub + head * a.sq.T + row,
-      delta + head * a.sq.T + row);
+  // tiles of rows, head after head; the next one to load is head ng's from row ni on
+  const T *qt, *gt;
+  const float *st, *dt;
+  int ng = 0, ni = start;
+  auto head_at = [&]() {
+    const int64_t head = hk * G + ng, row = p.q0 + start;
+    qt = q + row * a.q_row + head * a.q_head;
+    gt = go + (row * a.Hq + head) * a.D;
+    st = sub + head * a.sq.T + row;
+    dt = delta + head * a.sq.T + row;
   };
-  if (tiles > 0)
-    at(0, start, [&](const T* q0, const T* g0, const float* s0, const float* d0) {
-      bwd_keys_load<T, DP>(lds.b, q0, g0, s0, d0, a, end - start);
-    });
-  int half = 0;
-  for (int g = 0; g < G; ++g)
-    for (int i = start; i < end; i += KT) {
-      wait_loads_and_meet<0>();
-      const bool wrap = i + KT >= end;
-      const int ng = wrap ? g + 1 : g, ni = wrap ? start : i + KT;
-      const int left = ng < G ? end - ni : 0;
-      at(ng < G ? ng : g, ni, [&](const T* q0, const T* g0, const float* s0, const float* d0) {
-        bwd_keys_step<T, DP>(lds.b + half * STAGE, lds.b + (half ^ 1) * STAGE, q0, g0, s0, d0, a,
-                             left, x, y, sums, w >> 1, i, end - i, lo, least, most, only, c);
-      });
-      half ^= 1;
+  auto advance = [&]() {
+    ni += KT;
+    qt += KT * a.q_row;
+    gt += (int64_t)KT * a.Hq * a.D;
+    st += KT;
+    dt += KT;
+    if (ni >= end) {
+      ni = start;
+      if (++ng < G) head_at();
     }
+  };
+  const HeadLanes<T, DP> lanes;
+  auto step = [&](auto half, int i) {
+    constexpr int H = decltype(half)::value;
+    wait_loads_and_meet<0>();
+    bwd_keys_step<T, DP>(lds.b + H * STAGE, lds.b + (1 - H) * STAGE, lanes, qt, gt, st, dt, a,
+                         ng < G ? end - ni : 0, x, y, sums, w >> 1, i, end - i, lo, least, most,
+                         only, c);
+    advance();
+  };
+  if (tiles > 0) {
+    head_at();
+    bwd_keys_load<T, DP>(lds.b, qt, gt, st, dt, a, end - start);
+    advance();
+    int i = start;
+    const int all = tiles * G;
+    for (int n = 0; n < all; n += 2) {
+      step(std::integral_constant<int, 0>(), i);
+      i = i + KT >= end ? start : i + KT;
+      if (n + 1 < all) step(std::integral_constant<int, 1>(), i);
+      i = i + KT >= end ? start : i + KT;
+    }
+  }
   wait_loads_and_meet<0>();
   // waves 0 and 1 take dK from waves 2 and 3 and give them their dV
   f32x16(&own)[DP / 32] = w < 2 ? sums.k : sums.v;
