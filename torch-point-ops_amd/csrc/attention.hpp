@@ -166,7 +166,8 @@ struct HeadLds {
                                               int w) {
     constexpr int N = R / RPL / NW;
     static_assert(N >= 1 && N * RPL * NW == R, "rows of a tile");
-    n = n < 0 ? 0 : (n > R ? R : n);
+    // (clamped by vector instructions: said to be uniform, or each load becomes a loop)
+    n = __builtin_amdgcn_readfirstlane(n < 0 ? 0 : (n > R ? R : n));
     const __amdgpu_buffer_rsrc_t rsrc = buffer(p, n * row_bytes);
     const int l = lane_id(), r = l / CPR, bytes = D * Z;
 #pragma unroll

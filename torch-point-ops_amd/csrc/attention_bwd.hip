@@ -165,7 +165,7 @@ __device__ __forceinline__ void bwd_keys_load(char* to, const T* q, const T* go,
   L::template load<KT, 4>(to, q, (int)(a.q_row * sizeof(T)), left, a.D, w);
   L::template load<KT, 4>(to + TILE, go, (int)(a.Hq * a.D * sizeof(T)), left, a.D, w);
   if (w < 2) {
-    const int n = left < 0 ? 0 : (left > 64 ? 64 : left);
+    const int n = __builtin_amdgcn_readfirstlane(left < 0 ? 0 : (left > 64 ? 64 : left));
     __builtin_amdgcn_raw_ptr_buffer_load_lds(buffer(w ? delta : sub, n * 4),
                                              (lds_t*)(to + 2 * TILE + 256 * w), 4, lane_id() * 4, 0,
                                              0, 0);
