@@ -394,7 +394,8 @@ AttnArgs attn_args(const int64_t* oq, const int64_t* ok, const int64_t* lq, cons
 
 // Which kernel a call takes, and the shares of the keys.  Up to 64 rows a
 // sequence and key head on average are few: with a workgroup's 128 rows most
-// lanes would idle.  Shares: enough workgroups for two a CU, but 512 keys or more
+// lanes would idle.  So are fewer rows than 128 for each CU: 32 a workgroup, the
+// keys shared by its waves, fill four times as many (WAY_US).  Shares: enough workgroups for two a CU, but 512 keys or more
 // in each (by the room for keys: what is in use is not known here).
 struct Way {
   bool step;
@@ -403,7 +404,7 @@ struct Way {
 Way attn_way(int64_t B, int64_t Tq, int64_t Tk, int64_t Hq, int64_t Hk) {
   Way w{false, 1};
   const int64_t G = Hq / Hk, n = B < 1 ? 1 : B;
-  w.step = Tq * G <= 64 * n;
+  w.step = Tq * G <= 64 * n || Tq * Hq < 128 * 256;
   if (w.step) {
     const int64_t blocks = (Tq * G / 32 > n ? Tq * G / 32 : n) * Hk;
     int64_t s = (1024 + blocks - 1) / blocks;

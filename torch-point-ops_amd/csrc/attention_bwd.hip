@@ -52,57 +52,72 @@ __global__ __launch_bounds__(256) void attn_delta_kernel(const T* __restrict__ o
   }
 }
 
+// Two tiles of 64 rows, twice over; later what waves exchange, and the rows on
+// their way out.
+constexpr int BWD_ROWS = 64;
 template <typename T, int DP>
-__device__ __forceinline__ void bwd_q_step(const char* __restrict__ cur, char* __restrict__ nxt,
-                                           const HeadLanes<T, DP>& lanes, const T* k, const T* v, const AttnArgs& a, int left,
-                                           const HeadRows<T, DP>& q, const HeadRows<T, DP>& go,
-                                           f32x16 (&acc)[DP / 32], int j0, int n, int least,
-                                           int most, float c, float sub, float delta) {
-  constexpr int KT = KEYS<T>, TILE = PromptLds<T, DP>::TILE, PITCH = HeadLds<T, DP>::PITCH;
+struct alignas(1024) BwdRowsLds {
+  static constexpr int TILE = BWD_ROWS * HeadLds<T, DP>::PITCH;
+  static constexpr int OUT = 4 * Rows32<T, DP>::BYTES;
+  char b[4 * TILE > OUT ? 4 * TILE : OUT];
+};
+
+template <typename T, int DP>
+__device__ __forceinline__ void bwd_q_load(char* to, const T* k, const T* v, const AttnArgs& a,
+                                           int left) {
   typedef HeadLds<T, DP> L;
-  L::template load<KT, 4>(nxt, k, (int)(a.k_row * sizeof(T)), left, a.D, wave_id());
-  L::template load<KT, 4>(nxt + TILE, v, (int)(a.v_row * sizeof(T)), left, a.D, wave_id());
-  __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-  for (int t = 0; t < KT / 32; ++t) {
-    if (j0 + 32 * t >= most) break;
-    f32x16 s = scores<T, DP>(lanes, cur + 32 * t * PITCH, q);
-    const f32x16 d = scores<T, DP>(lanes, cur + TILE + 32 * t * PITCH, go);
-    const bool masked = j0 + 32 * t + 32 > least;
-    const int first = j0 + 32 * t + 4 * (lane_id() >> 5);
-#pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e], c, -sub));
-      s[e] = p * (d[e] - delta);
-    }
-    if (masked)  // (a pass of its own: a select for each value would be taken everywhere)
-#pragma unroll
-      for (int e = 0; e < 16; ++e)
-        if (first + 8 * (e >> 2) + (e & 3) >= n) s[e] = 0.f;
-    multiply_rows<T, DP>(acc, lanes, cur + 32 * t * PITCH, s);
-  }
+  const int w = wave_id();
+  L::template load<BWD_ROWS, 4>(to, k, (int)(a.k_row * sizeof(T)), left, a.D, w);
+  L::template load<BWD_ROWS, 4>(to + BwdRowsLds<T, DP>::TILE, v, (int)(a.v_row * sizeof(T)), left,
+                                a.D, w);
 }
 
-// dQ of 128 rows, 32 a wave; the rows, their order and their keys as the forward
-// for prompts has them.
+// The products of the wave's rows with 32 keys from j0 on, `half` of a tile.
+template <typename T, int DP>
+__device__ __forceinline__ void bwd_q_step(const char* __restrict__ cur, char* __restrict__ nxt,
+                                           const HeadLanes<T, DP>& lanes, const T* k, const T* v,
+                                           const AttnArgs& a, int left, const HeadRows<T, DP>& q,
+                                           const HeadRows<T, DP>& go, f32x16 (&acc)[DP / 32],
+                                           int half, int j0, int n, int least, int most, float c,
+                                           float sub, float delta) {
+  bwd_q_load<T, DP>(nxt, k, v, a, left);
+  __builtin_amdgcn_sched_barrier(0);
+  if (j0 >= most) return;
+  const char* at = cur + half * 32 * HeadLds<T, DP>::PITCH;
+  f32x16 s = scores<T, DP>(lanes, at, q);
+  const f32x16 d = scores<T, DP>(lanes, at + BwdRowsLds<T, DP>::TILE, go);
+  const int first = j0 + 4 * (lane_id() >> 5);
+#pragma unroll
+  for (int e = 0; e < 16; ++e)
+    s[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e], c, -sub)) * (d[e] - delta);
+  if (j0 + 32 > least)  // (a pass of its own: a select for each value would be taken everywhere)
+#pragma unroll
+    for (int e = 0; e < 16; ++e)
+      if (first + 8 * (e >> 2) + (e & 3) >= n) s[e] = 0.f;
+  multiply_rows<T, DP>(acc, lanes, at, s);
+}
+
+// dQ of 64 rows; the rows and their keys as the forward for prompts has them.
+// Wave w has rows 32 (w % 2) .. + 31 and half w / 2 of each tile of keys; at the
+// end two waves' sums are added.
 template <typename T, int DP>
 __global__ __launch_bounds__(256, (DP * sizeof(T) <= 256 ? 2 : 1)) void attn_bwd_q_kernel(
     AttnArgs a, const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ v,
     const T* __restrict__ go, const float* __restrict__ sub, const float* __restrict__ delta,
     T* __restrict__ gq) {
-  constexpr int KT = KEYS<T>, TILE = PromptLds<T, DP>::TILE;
-  __shared__ PromptLds<T, DP> lds;
+  constexpr int KT = BWD_ROWS, TILE = BwdRowsLds<T, DP>::TILE;
+  __shared__ BwdRowsLds<T, DP> lds;
   const int G = a.Hq / a.Hk, hk = blockIdx.x % a.Hk;
   int local;
-  const int s = attn_tile<true>(a.sq, blockIdx.x / a.Hk, gridDim.x / a.Hk, G, 128, local);
+  const int s = attn_tile<true>(a.sq, blockIdx.x / a.Hk, gridDim.x / a.Hk, G, 64, local);
   if (s < 0) return;
   const AttnSpan p = attn_span(a, s);
   const int all = p.room_q * G;
-  const int w = wave_id(), l = lane_id(), r0 = local * 128 + 32 * w, r = r0 + (l & 31);
+  const int w = wave_id(), l = lane_id(), r0 = local * 64 + 32 * (w & 1), r = r0 + (l & 31);
   const int used = p.Lq * G;
   auto keys = [&](int row) { return used ? attn_keys(a, p, row < used ? row : used - 1, G) : 0; };
   const int least = keys(r0), most = r0 < used ? keys(r0 + 31) : 0;
-  const int end = local * 128 < used ? keys(local * 128 + 127) : 0;
+  const int end = local * 64 < used ? keys(local * 64 + 63) : 0;
   const int n = keys(r);
   const bool in = r < used;
   const int head = hk * G + r % G;
@@ -119,11 +134,7 @@ __global__ __launch_bounds__(256, (DP * sizeof(T) <= 256 ? 2 : 1)) void attn_bwd
   for (int i = 0; i < DP / 32; ++i) acc[i] = f32x16{};
   const T* kt = k + p.k0 * a.k_row + hk * a.k_head;
   const T* vt = v + p.k0 * a.v_row + hk * a.v_head;
-  typedef HeadLds<T, DP> L;
-  if (end > 0) {
-    L::template load<KT, 4>(lds.b, kt, (int)(a.k_row * sizeof(T)), p.Lk, a.D, w);
-    L::template load<KT, 4>(lds.b + TILE, vt, (int)(a.v_row * sizeof(T)), p.Lk, a.D, w);
-  }
+  if (end > 0) bwd_q_load<T, DP>(lds.b, kt, vt, a, p.Lk);
   const HeadLanes<T, DP> lanes;
   auto step = [&](auto half, int j0) {
     constexpr int H = decltype(half)::value;
@@ -131,22 +142,42 @@ __global__ __launch_bounds__(256, (DP * sizeof(T) <= 256 ? 2 : 1)) void attn_bwd
     kt += KT * a.k_row;
     vt += KT * a.v_row;
     bwd_q_step<T, DP>(lds.b + H * 2 * TILE, lds.b + (1 - H) * 2 * TILE, lanes, kt, vt, a,
-                      j0 + KT < end ? p.Lk - j0 - KT : 0, x, y, acc, j0, n, least, most, c, row_sub,
-                      row_delta);
+                      j0 + KT < end ? p.Lk - j0 - KT : 0, x, y, acc, w >> 1, j0 + 32 * (w >> 1), n,
+                      least, most, c, row_sub, row_delta);
   };
   for (int j0 = 0; j0 < end; j0 += 2 * KT) {
     step(std::integral_constant<int, 0>(), j0);
     if (j0 + KT < end) step(std::integral_constant<int, 1>(), j0 + KT);
   }
   wait_loads_and_meet<0>();
-  if (r0 >= all) return;
+  f32x4* sums = (f32x4*)(lds.b + (w & 1) * DP * 128) + l;
+  if (w >= 2) {
+#pragma unroll
+    for (int i = 0; i < DP / 32; ++i)
+#pragma unroll
+      for (int b = 0; b < 4; ++b)
+        sums[(4 * i + b) * 64] =
+            f32x4{acc[i][4 * b], acc[i][4 * b + 1], acc[i][4 * b + 2], acc[i][4 * b + 3]};
+  }
+  __syncthreads();
+  if (w < 2) {
+#pragma unroll
+    for (int i = 0; i < DP / 32; ++i)
+#pragma unroll
+      for (int b = 0; b < 4; ++b) {
+        const f32x4 z = sums[(4 * i + b) * 64];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[i][4 * b + e] += z[e];
+      }
+  }
+  __syncthreads();
+  if (w >= 2 || r0 >= all) return;
   put_rows<T, DP>(lds.b, acc, in && row_sub != -NEG_INF && n > 1 ? a.scale : 0.f, gq, a, p, hk, r0,
                   all);
 }
 
 // A tile of 64 rows of q and of go, and what is theirs of sub and delta; later
 // the sums that the waves exchange, and the rows on their way out.
-constexpr int BWD_ROWS = 64;
 template <typename T, int DP>
 struct alignas(1024) BwdKeysLds {
   static constexpr int TILE = BWD_ROWS * HeadLds<T, DP>::PITCH;
@@ -375,7 +406,7 @@ extern "C" int tpo_attention_bwd(int dtype, const void* grad_out, const void* q,
   const AttnArgs a = attn_args(offsets_q, offsets_k, lengths_q, lengths_k, B, Tq, Tk, Hq, Hk, D,
                                q_row, q_head, k_row, k_head, v_row, v_head, causal, scale);
   const int64_t rows = Tq * Hq, G = Hq / Hk;
-  const int64_t places_q = attn_places(Tq, G, B, 128), places_k = attn_places(Tk, 1, B, 64);
+  const int64_t places_q = attn_places(Tq, G, B, 64), places_k = attn_places(Tk, 1, B, 64);
   if (places_q * Hk >= ((int64_t)1 << 31) || places_k * Hk >= ((int64_t)1 << 31))
     return set_error(TPO_ERR_ARG, "attention_bwd: too many rows");
   float *sub = (float*)workspace, *delta = (float*)((char*)workspace + need / 2);

@@ -165,9 +165,10 @@ struct ColLoader {
   };
   __device__ __forceinline__ Slab slab(int n) const { return slab_of(p, (int64_t)n * K); }
   __device__ __forceinline__ Slab slab_of(const char* from, int64_t row) const {
-    int64_t n = rows - row;
-    n = n < 0 ? 0 : (n > K ? K : n);
-    return Slab{buffer(from + (n > 0 ? row * pitch : 0), (int)(n * pitch)), {off[0], off[1]}, step};
+    const int64_t left = rows - row;
+    // (said to be uniform: what a vector instruction clamps would make each load a loop)
+    const int n = __builtin_amdgcn_readfirstlane(left < 0 ? 0 : (left > K ? K : (int)left));
+    return Slab{buffer(from + (n > 0 ? row * pitch : 0), n * (int)pitch), {off[0], off[1]}, step};
   }
   static __device__ __forceinline__ typename Chunk<T>::V read(const char* lds, int row0, int s) {
     const int l = lane_id();
