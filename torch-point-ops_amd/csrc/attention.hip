@@ -31,12 +31,12 @@ struct RowSums {
   // below n; c: what a score counts in the exponent of 2
   template <int KT>
   __device__ __forceinline__ void add(const HeadLanes<T, DP>& lanes, const char* lds,
-                                      const HeadRows<T, DP>& q, int j0, int n, bool masked,
-                                      float c) {
+                                      const HeadRows<T, DP>& q, int D, int j0, int n,
+                                      bool masked, float c) {
     constexpr int PITCH = HeadLds<T, DP>::PITCH;
     f32x16 s[KT / 32];
 #pragma unroll
-    for (int t = 0; t < KT / 32; ++t) s[t] = scores<T, DP>(lanes, lds + 32 * t * PITCH, q);
+    for (int t = 0; t < KT / 32; ++t) s[t] = scores<T, DP>(lanes, lds + 32 * t * PITCH, q, D);
     if (masked) {
       const int first = j0 + 4 * (lane_id() >> 5);
 #pragma unroll
@@ -87,7 +87,7 @@ __device__ __forceinline__ void prompt_step(const char* __restrict__ cur, char* 
   L::template load<KT, 4>(nxt, k, (int)(a.k_row * sizeof(T)), left, a.D, wave_id());
   L::template load<KT, 4>(nxt + TILE, v, (int)(a.v_row * sizeof(T)), left, a.D, wave_id());
   __builtin_amdgcn_sched_barrier(0);
-  if (j0 < most) rows.template add<KT>(lanes, cur, q, j0, n, j0 + KT > least, c);
+  if (j0 < most) rows.template add<KT>(lanes, cur, q, a.D, j0, n, j0 + KT > least, c);
 }
 
 // Prompts: a workgroup of four waves takes 128 rows, 32 a wave, and all their
@@ -188,7 +188,7 @@ __device__ __forceinline__ void step_step(const char* __restrict__ cur, char* __
   __builtin_amdgcn_s_waitcnt((N & 15) | (N >> 4) << 14 | 0xf70);  // the tile itself has landed
   asm volatile("" ::: "memory");
   __builtin_amdgcn_sched_barrier(0);
-  rows.template add<32>(lanes, cur, q, j0, n, j0 + 32 > least, c);
+  rows.template add<32>(lanes, cur, q, a.D, j0, n, j0 + 32 > least, c);
 }
 
 // part: with shares, each row's sums (D floats, not divided), and in ml their
@@ -301,41 +301,56 @@ __global__ __launch_bounds__((64 * STEP_WAVES<T, DP>)) void attn_step_kernel(
   }
 }
 
-// The shares' sums of each row together: one wave a row.
+// The shares' sums of each row together: a workgroup a row.  A lane weighs a share
+// (there are at most 64), the waves add every fourth one's values, four loads
+// under way at a time.
 template <typename T>
 __global__ __launch_bounds__(256) void attn_join_kernel(const float* __restrict__ part,
                                                         const float2* __restrict__ ml, int shares,
-                                                        int64_t rows, int Hq, int64_t Tq, int D,
+                                                        int Hq, int64_t Tq, int D,
                                                         T* __restrict__ out,
                                                         float* __restrict__ lse,
                                                         T* __restrict__ rest) {
-  const int64_t at = (int64_t)blockIdx.x * 4 + wave_id();
-  if (at >= rows) return;
-  const int l = lane_id();
-  float m = NEG_INF;
-  for (int i = 0; i < shares; ++i) {
-    const float2 y = ml[at * shares + i];
-    if (y.y != 0.f) m = fmaxf(m, y.x);
-  }
-  float total = 0.f, o[2] = {0.f, 0.f};
-  for (int i = 0; i < shares; ++i) {
-    const float2 y = ml[at * shares + i];
-    if (y.y == 0.f) continue;
-    const float f = __builtin_amdgcn_exp2f(y.x - m);
-    total += f * y.y;
-    const float* p = part + (at * shares + i) * D;
-    if (l < D) o[0] += f * p[l];
-    if (l + 64 < D) o[1] += f * p[l + 64];
-  }
-  const float inv = total != 0.f ? 1.f / total : 0.f;
+  __shared__ float s[4][AT_DMAX];
+  const int64_t at = blockIdx.x;
+  const int l = lane_id(), w = wave_id();
+  const float2 mine = l < shares ? ml[at * shares + l] : make_float2(0.f, 0.f);
+  const bool has = mine.y != 0.f;  // a share without keys has written no values
+  const float m = wave_max(has ? mine.x : NEG_INF);
+  const float f = has ? __builtin_amdgcn_exp2f(mine.x - m) : 0.f;
+  const float total = wave_sum(f * mine.y);
+  const uint64_t there = __builtin_amdgcn_ballot_w64(has);
+  const float* p = part + at * shares * D;
+  const int d1 = l + 64;
+  float o[2] = {0.f, 0.f};
+  for (int i = w; i < shares; i += 16) {
+    float x[4][2];
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
-    if (l + 64 * i < D) {
-      const T z = (T)(o[i] * inv);
-      out[at * D + l + 64 * i] = z;
-      if (rest) rest[at * D + l + 64 * i] = (T)(o[i] * inv - (float)z);
+    for (int j = 0; j < 4; ++j) {
+      const int k = i + 4 * j;
+      const bool in = k < shares && (there >> k & 1);
+      x[j][0] = in && l < D ? p[(int64_t)k * D + l] : 0.f;
+      x[j][1] = in && d1 < D ? p[(int64_t)k * D + d1] : 0.f;
     }
-  if (lse && l == 0)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float g = __shfl(f, (i + 4 * j) & 63);
+      const bool in = i + 4 * j < shares && (there >> (i + 4 * j) & 1);
+      if (in) o[0] = __builtin_fmaf(g, x[j][0], o[0]);
+      if (in) o[1] = __builtin_fmaf(g, x[j][1], o[1]);
+    }
+  }
+  s[w][l] = o[0];
+  s[w][l + 64] = o[1];
+  __syncthreads();
+  const int d = threadIdx.x;
+  if (d < D) {
+    const float y = ((s[0][d] + s[1][d]) + (s[2][d] + s[3][d])) * (total != 0.f ? 1.f / total : 0.f);
+    const T z = (T)y;
+    out[at * D + d] = z;
+    if (rest) rest[at * D + d] = (T)(y - (float)z);
+  }
+  if (lse && d == 0)
     lse[(at % Hq) * Tq + at / Hq] = total == 0.f ? NEG_INF : (m + __builtin_amdgcn_logf(total)) * LN2;
 }
 
@@ -395,8 +410,10 @@ AttnArgs attn_args(const int64_t* oq, const int64_t* ok, const int64_t* lq, cons
 // Which kernel a call takes, and the shares of the keys.  Up to 64 rows a
 // sequence and key head on average are few: with a workgroup's 128 rows most
 // lanes would idle.  So are fewer rows than 128 for each CU: 32 a workgroup, the
-// keys shared by its waves, fill four times as many (WAY_US).  Shares: enough workgroups for two a CU, but 512 keys or more
-// in each (by the room for keys: what is in use is not known here).
+// keys shared by its waves, fill four times as many (float 5 x 600: 42 us where
+// prompts' tiles take 52).  Shares: for four workgroups a CU, of 256 keys or more
+// each (by the room for keys: what is in use is not known here), and none up to
+// 1024 keys, where adding them up takes as long as it saves.
 struct Way {
   bool step;
   int shares;
@@ -408,7 +425,8 @@ Way attn_way(int64_t B, int64_t Tq, int64_t Tk, int64_t Hq, int64_t Hk) {
   if (w.step) {
     const int64_t blocks = (Tq * G / 32 > n ? Tq * G / 32 : n) * Hk;
     int64_t s = (1024 + blocks - 1) / blocks;
-    if (s > Tk / n / 512) s = Tk / n / 512;
+    if (s > Tk / n / 256) s = Tk / n / 256;
+    if (Tk / n < 1024) s = 1;
     if (s > 64) s = 64;
     w.shares = s < 1 ? 1 : (int)s;
   }
@@ -467,8 +485,8 @@ extern "C" int tpo_attention_fwd(int dtype, const void* q, const void* k, const 
                 a, (const T*)q, (const T*)k, (const T*)v, (T*)out, lse, (T*)rest, part, ml);
     });
     if (w.shares > 1)
-      attn_join_kernel<T><<<dim3((unsigned)((Tq * Hq + 3) / 4)), 256, 0, s>>>(
-          part, ml, w.shares, Tq * Hq, (int)Hq, Tq, (int)D, (T*)out, lse, (T*)rest);
+      attn_join_kernel<T><<<dim3((unsigned)(Tq * Hq)), 256, 0, s>>>(
+          part, ml, w.shares, (int)Hq, Tq, (int)D, (T*)out, lse, (T*)rest);
   });
   return check_launch("attention_fwd");
 }

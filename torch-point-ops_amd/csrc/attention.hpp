@@ -328,12 +328,16 @@ struct alignas(1024) PromptLds {
 };
 
 // X Y^T of the 32 rows of X at lds and the wave's rows: transposed scores.
+// Float chunks past D (of 8 values, four slow matrix instructions) are left out.
 template <typename T, int DP>
 __device__ __forceinline__ f32x16 scores(const HeadLanes<T, DP>& x, const char* lds,
-                                         const HeadRows<T, DP>& y) {
+                                         const HeadRows<T, DP>& y, int D) {
   f32x16 s = {};
 #pragma unroll
-  for (int c = 0; c < HeadRows<T, DP>::N; ++c) mma(s, x.by_row(lds, c), y.x[c]);
+  for (int c = 0; c < HeadRows<T, DP>::N; ++c) {
+    if (sizeof(T) == 4 && 8 * c >= D) break;
+    mma(s, x.by_row(lds, c), y.x[c]);
+  }
   return s;
 }
 

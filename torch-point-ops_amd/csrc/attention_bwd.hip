@@ -84,8 +84,8 @@ __device__ __forceinline__ void bwd_q_step(const char* __restrict__ cur, char* _
   __builtin_amdgcn_sched_barrier(0);
   if (j0 >= most) return;
   const char* at = cur + half * 32 * HeadLds<T, DP>::PITCH;
-  f32x16 s = scores<T, DP>(lanes, at, q);
-  const f32x16 d = scores<T, DP>(lanes, at + BwdRowsLds<T, DP>::TILE, go);
+  f32x16 s = scores<T, DP>(lanes, at, q, a.D);
+  const f32x16 d = scores<T, DP>(lanes, at + BwdRowsLds<T, DP>::TILE, go, a.D);
   const int first = j0 + 4 * (lane_id() >> 5);
 #pragma unroll
   for (int e = 0; e < 16; ++e)
@@ -227,8 +227,8 @@ __device__ __forceinline__ void bwd_keys_step(const char* __restrict__ cur, char
   const int i = i0 + 32 * t;
   if (i + 32 <= least || 32 * t >= left) return;
   const char* at = cur + 32 * t * PITCH;
-  f32x16 s = scores<T, DP>(lanes, at, k);
-  f32x16 d = scores<T, DP>(lanes, at + TILE, v);
+  f32x16 s = scores<T, DP>(lanes, at, k, a.D);
+  f32x16 d = scores<T, DP>(lanes, at + TILE, v, a.D);
   const bool masked = i < most || 32 * t + 32 > left || only == ALL_ROWS;
   const float* ps = (const float*)(cur + 2 * TILE) + 32 * t + 4 * h;
 #pragma unroll

@@ -13,13 +13,15 @@ __device__ __forceinline__ float ln_at(const W* w, int64_t c, float none) {
 }
 
 // A row held in registers by a team of 64 or 256 lanes: N loads a lane of PER
-// values each (16 bytes, or one value where rows are not made of 16-byte pieces).
-// x is read once; the variance is taken about the mean, from the registers.
-// HBM-bound: what is read and written is all that counts, so teams go on to
-// other rows with the weights in registers, and there are enough of them to keep
-// the memory busy.
+// values (16 bytes) each.  Rows of other widths begin anywhere: the memory takes
+// 16-byte accesses at any element (at 32768 x 1023 in bfloat16 one value a load
+// took 188 us where this takes LN_ODD), and only a row's last piece goes value by
+// value.  x is read once; the variance is taken about the mean, from the
+// registers.  HBM-bound: what is read and written is all that counts, so teams go
+// on to other rows with the weights in registers, and there are enough of them to
+// keep the memory busy.
 template <typename T, int PER>
-struct alignas(PER * sizeof(T)) Piece {
+struct __attribute__((packed, aligned(sizeof(T)))) Piece {
   T v[PER];
 };
 
@@ -46,14 +48,15 @@ struct RowHeld {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const int64_t c = column(i);
-      if (c < width) {
-        const Piece<T, PER> x = *(const Piece<T, PER>*)(p + c);
-#pragma unroll
-        for (int e = 0; e < PER; ++e) v[i][e] = (float)x.v[e];
+      Piece<T, PER> x;
+      if (c + PER <= width) {
+        x = *(const Piece<T, PER>*)(p + c);
       } else {
 #pragma unroll
-        for (int e = 0; e < PER; ++e) v[i][e] = none;
+        for (int e = 0; e < PER; ++e) x.v[e] = c + e < width ? p[c + e] : (T)none;
       }
+#pragma unroll
+      for (int e = 0; e < PER; ++e) v[i][e] = (float)x.v[e];
     }
   }
   __device__ __forceinline__ void fill(float f) {
@@ -66,11 +69,15 @@ struct RowHeld {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const int64_t c = column(i);
-      if (c < width) {
-        Piece<T, PER> x;
+      Piece<T, PER> x;
 #pragma unroll
-        for (int e = 0; e < PER; ++e) x.v[e] = (T)v[i][e];
+      for (int e = 0; e < PER; ++e) x.v[e] = (T)v[i][e];
+      if (c + PER <= width) {
         *(Piece<T, PER>*)(p + c) = x;
+      } else {
+#pragma unroll
+        for (int e = 0; e < PER; ++e)
+          if (c + e < width) p[c + e] = x.v[e];
       }
     }
   }
@@ -104,7 +111,7 @@ __global__ __launch_bounds__(256) void layer_norm_fwd_kernel(
 #pragma unroll
       for (int e = 0; e < PER; ++e) {
         const float d = xs.v[i][e] - m;
-        if (xs.column(i) < width) t = __builtin_fmaf(d, d, t);
+        if (xs.column(i) + e < width) t = __builtin_fmaf(d, d, t);
       }
     const float q = 1.f / sqrtf(team_sum<TEAM>(t, s) * per + eps);
     RowHeld<T, PER, N, TEAM> ys;
@@ -339,51 +346,36 @@ __global__ __launch_bounds__(1024) void layer_norm_bwd_sum_kernel(const float* _
   }
 }
 
-// The kernels' build for a row: values a load, loads a lane, lanes a row; held
-// false for rows of more than 8192 values.
+// The kernels' build for a row: loads a lane, lanes a row; held false for rows
+// longer than 256 lanes hold.
 struct LnForm {
-  int per, n, team;
+  int n, team;
   bool held;
 };
-LnForm ln_form(int64_t width, int64_t size, bool pieces) {
-  const int64_t per = 16 / size;
-  LnForm f{1, 0, 64, true};
-  if (pieces && width % per == 0) {
-    f.per = (int)per;
-    const int64_t loads = (width + per - 1) / per;
-    if (loads <= 64) f.n = 1;
-    else if (loads <= 128) f.n = 2;
-    else if (loads <= 256) f.n = 4;
-    else if (loads <= 512) f.n = 2, f.team = 256;
-    else if (loads <= 1024) f.n = 4, f.team = 256;
-    else f.held = false;
-  } else {
-    if (width <= 256) f.n = 4;
-    else if (width <= 1024) f.n = 16;
-    else if (width <= 2048) f.n = 8, f.team = 256;
-    else if (width <= 8192) f.n = 32, f.team = 256;
-    else f.held = false;
-  }
-  return f;
+LnForm ln_form(int64_t width, int64_t size) {
+  const int64_t loads = (width * size + 15) / 16;
+  if (loads <= 64) return {1, 64, true};
+  if (loads <= 128) return {2, 64, true};
+  if (loads <= 256) return {4, 64, true};
+  if (loads <= 512) return {2, 256, true};
+  if (loads <= 1024) return {4, 256, true};
+  if (loads <= 2048) return {8, 256, true};
+  return {0, 0, false};
 }
-// Calls f with the form as types: value counts, loads, team.
+// Calls f with the form as types: values a load, loads, team.
 template <typename T, typename F>
 void with_form(const LnForm& f, F&& call) {
   constexpr int PER = 16 / sizeof(T);
-  auto go = [&](auto per, auto n, auto team) { call(per, n, team); };
-#define LN_FORM(P, N, TEAM)                                                           \
-  if (f.per == P && f.n == N && f.team == TEAM)                                       \
-  return go(std::integral_constant<int, P>(), std::integral_constant<int, N>(),       \
-            std::integral_constant<int, TEAM>())
-  LN_FORM(PER, 1, 64);
-  LN_FORM(PER, 2, 64);
-  LN_FORM(PER, 4, 64);
-  LN_FORM(PER, 2, 256);
-  LN_FORM(PER, 4, 256);
-  LN_FORM(1, 4, 64);
-  LN_FORM(1, 16, 64);
-  LN_FORM(1, 8, 256);
-  LN_FORM(1, 32, 256);
+#define LN_FORM(N, TEAM)                                                              \
+  if (f.n == N && f.team == TEAM)                                                     \
+  return call(std::integral_constant<int, PER>(), std::integral_constant<int, N>(),   \
+              std::integral_constant<int, TEAM>())
+  LN_FORM(1, 64);
+  LN_FORM(2, 64);
+  LN_FORM(4, 64);
+  LN_FORM(2, 256);
+  LN_FORM(4, 256);
+  LN_FORM(8, 256);
 #undef LN_FORM
 }
 
@@ -395,12 +387,6 @@ inline int ln_parts(int64_t rows) {
   const int64_t few = (rows + 3) / 4, most = rows / 16 > 64 ? rows / 16 : 64;
   const int64_t p = few < most ? few : most;
   return (int)(p > 1024 ? 1024 : p);
-}
-
-inline bool ln_pieces(std::initializer_list<const void*> ps) {
-  for (const void* p : ps)
-    if ((uintptr_t)p & 15) return false;
-  return true;
 }
 
 // The weights are of the input's type or float.
@@ -443,7 +429,7 @@ extern "C" int tpo_layer_norm_fwd(int dtype, int wdtype, const void* x, const vo
       none = true;
       return;
     }
-    const LnForm f = ln_form(width, sizeof(T), ln_pieces({x, weight, bias, y}));
+    const LnForm f = ln_form(width, sizeof(T));
     if (!f.held) {
       layer_norm_fwd_long_kernel<T, W><<<dim3((unsigned)((rows + 3) / 4)), 256, 0, s>>>(
           (const T*)x, (const W*)weight, (const W*)bias, rows, width, (float)eps, (T*)y, mean,
@@ -482,7 +468,7 @@ extern "C" int tpo_layer_norm_bwd(int dtype, int wdtype, const void* grad_y, con
   const int rc = ln_dispatch("layer_norm_bwd", dtype, wdtype, [&](auto t, auto w) {
     typedef decltype(t) T;
     typedef decltype(w) W;
-    const LnForm f = ln_form(width, sizeof(T), ln_pieces({grad_y, x, weight, grad_x}));
+    const LnForm f = ln_form(width, sizeof(T));
     const int parts = ln_parts(rows);
     float* part = sums ? (float*)workspace : nullptr;
     if (rows > 0 && width > LN_NARROW && f.held) {
