@@ -155,17 +155,17 @@ __global__ __launch_bounds__(256, 2) void attn_prompt_kernel(AttnArgs a, const T
         inv == 0.f ? NEG_INF : (rows.m * c + __builtin_amdgcn_logf(sum)) * LN2;
 }
 
-// Few rows over many keys: a workgroup takes 32 rows and one of gridDim.z shares
+// Few rows over many keys: a workgroup takes 32 NR rows and one of gridDim.z shares
 // of their keys, its W waves in turn a tile of 32 keys each from LDS of their own,
 // so that no wave waits for another before the end.
 template <typename T, int DP> constexpr int STEP_WAVES = sizeof(T) == 4 && DP > 64 ? 2 : 4;
-template <typename T, int DP>
+template <typename T, int DP, int NR = 1>
 struct alignas(1024) StepLds {
   static constexpr int TILE = 32 * HeadLds<T, DP>::PITCH;
-  static constexpr int SUMS = STEP_WAVES<T, DP> * 32 * (DP + 4) * 4;
+  static constexpr int SUMS = STEP_WAVES<T, DP> * 32 * NR * (DP + 4) * 4;
   static constexpr int TILES = STEP_WAVES<T, DP> * 4 * TILE;
   char b[TILES > SUMS ? TILES : SUMS];
-  float m[STEP_WAVES<T, DP>][32], l[STEP_WAVES<T, DP>][32];
+  float m[STEP_WAVES<T, DP>][32 * NR], l[STEP_WAVES<T, DP>][32 * NR];
 };
 
 template <typename T, int DP>
@@ -176,11 +176,18 @@ __device__ __forceinline__ void step_load(char* to, const T* k, const T* v, cons
   L::template load<32, 1>(to + StepLds<T, DP>::TILE, v, (int)(a.v_row * sizeof(T)), left,
                                  a.D, 0);
 }
-template <typename T, int DP>
+// What a lane's row sees: n keys, the rows of its 32 between least and most.
+struct StepRows {
+  int n, least, most;
+};
+
+template <typename T, int DP, int NR>
 __device__ __forceinline__ void step_step(const char* __restrict__ cur, char* __restrict__ nxt,
-                                          const HeadLanes<T, DP>& lanes, const T* k, const T* v, const AttnArgs& a, int left,
-                                          const HeadRows<T, DP>& q, RowSums<T, DP>& rows, int j0,
-                                          int n, int least, float c) {
+                                          const HeadLanes<T, DP>& lanes, const T* k, const T* v,
+                                          const AttnArgs& a, int left,
+                                          const HeadRows<T, DP> (&q)[NR],
+                                          RowSums<T, DP> (&rows)[NR], const StepRows (&sees)[NR],
+                                          int j0, float c) {
   constexpr int TILE = StepLds<T, DP>::TILE, N = 2 * TILE / 1024;  // loads a tile
   step_load<T, DP>(nxt, k, v, a, left);
   __builtin_amdgcn_sched_barrier(0);
@@ -188,47 +195,54 @@ __device__ __forceinline__ void step_step(const char* __restrict__ cur, char* __
   __builtin_amdgcn_s_waitcnt((N & 15) | (N >> 4) << 14 | 0xf70);  // the tile itself has landed
   asm volatile("" ::: "memory");
   __builtin_amdgcn_sched_barrier(0);
-  rows.template add<32>(lanes, cur, q, a.D, j0, n, j0 + 32 > least, c);
+#pragma unroll
+  for (int i = 0; i < NR; ++i)
+    if (j0 < sees[i].most)
+      rows[i].template add<32>(lanes, cur, q[i], a.D, j0, sees[i].n, j0 + 32 > sees[i].least, c);
 }
 
 // part: with shares, each row's sums (D floats, not divided), and in ml their
 // maximum (in the exponent of 2) and sum
-template <typename T, int DP>
+template <typename T, int DP, int NR>
 __global__ __launch_bounds__((64 * STEP_WAVES<T, DP>)) void attn_step_kernel(
     AttnArgs a, const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ v,
     T* __restrict__ out, float* __restrict__ lse, T* __restrict__ rest,
     float* __restrict__ part, float2* __restrict__ ml) {
-  constexpr int W = STEP_WAVES<T, DP>, TILE = StepLds<T, DP>::TILE;
-  __shared__ StepLds<T, DP> lds;
+  constexpr int W = STEP_WAVES<T, DP>, TILE = StepLds<T, DP>::TILE, R = 32 * NR;
+  __shared__ StepLds<T, DP, NR> lds;
   const int G = a.Hq / a.Hk, hk = blockIdx.y, shares = gridDim.z;
   const int64_t place = blockIdx.x;
-  const int s = attn_sequence(a.sq, place, G, 32);
+  const int s = attn_sequence(a.sq, place, G, R);
   const AttnSpan p = attn_span(a, s);
-  const int64_t local = uniform(place - attn_first(a.sq, s, G, 32));
+  const int64_t local = uniform(place - attn_first(a.sq, s, G, R));
   const int all = p.room_q * G;
-  if (local < 0 || local * 32 >= all) return;
-  const int w = wave_id(), l = lane_id(), r0 = (int)local * 32, r = r0 + (l & 31);
+  if (local < 0 || local * R >= all) return;
+  const int w = wave_id(), l = lane_id(), r0 = (int)local * R;
   const int used = p.Lq * G;
   auto keys = [&](int row) { return used ? attn_keys(a, p, row < used ? row : used - 1, G) : 0; };
-  const int least = keys(r0), most = r0 < used ? keys(r0 + 31) : 0;
-  const int n = keys(r);
+  StepRows sees[NR];
+  HeadRows<T, DP> x[NR];
+  RowSums<T, DP> rows[NR];
+#pragma unroll
+  for (int i = 0; i < NR; ++i) {
+    const int first = r0 + 32 * i, r = first + (l & 31);
+    sees[i] = StepRows{keys(r), keys(first), first < used ? keys(first + 31) : 0};
+    x[i].load(q + (p.q0 + r / G) * a.q_row + (hk * G + r % G) * a.q_head, r < used, a.D);
+    if (a.scale < 0.f) x[i].negate();
+    rows[i].clear();
+  }
+  const int most = r0 < used ? keys(r0 + R - 1) : 0;
   const int tiles = (most + 31) / 32, per = (tiles + shares - 1) / shares;
   const int t0 = per * blockIdx.z, t1 = t0 + per < tiles ? t0 + per : tiles;
-  const int head = hk * G + r % G;
-  HeadRows<T, DP> x;
-  x.load(q + (p.q0 + r / G) * a.q_row + head * a.q_head, r < used, a.D);
   const float c = attn_count(a.scale);
-  if (a.scale < 0.f) x.negate();
-  RowSums<T, DP> rows;
-  rows.clear();
   const T* kt = k + p.k0 * a.k_row + hk * a.k_head;
   const T* vt = v + p.k0 * a.v_row + hk * a.v_head;
   char* mine = lds.b + w * 4 * TILE;
+  const HeadLanes<T, DP> lanes;
   auto load = [&](int t) {
     step_load<T, DP>(mine, kt + (int64_t)t * 32 * a.k_row, vt + (int64_t)t * 32 * a.v_row, a,
                      t < t1 ? most - t * 32 : 0);
   };
-  const HeadLanes<T, DP> lanes;
   if (t0 + w < t1) load(t0 + w);
   int half = 0;
   for (int t = t0 + w; t < t1; t += W) {
@@ -236,68 +250,74 @@ __global__ __launch_bounds__((64 * STEP_WAVES<T, DP>)) void attn_step_kernel(
     asm volatile("" ::: "memory");
     __builtin_amdgcn_s_waitcnt(0xc07f);  // the other tile's reads have ended
     const int64_t next = t + W;
-    step_step<T, DP>(mine + half * 2 * TILE, mine + (half ^ 1) * 2 * TILE, lanes,
-                     kt + next * 32 * a.k_row, vt + next * 32 * a.v_row, a,
-                     next < t1 ? most - (int)next * 32 : 0, x, rows, t * 32, n, least, c);
+    step_step<T, DP, NR>(mine + half * 2 * TILE, mine + (half ^ 1) * 2 * TILE, lanes,
+                         kt + next * 32 * a.k_row, vt + next * 32 * a.v_row, a,
+                         next < t1 ? most - (int)next * 32 : 0, x, rows, sees, t * 32, c);
     half ^= 1;
   }
   wait_loads_and_meet<0>();
 
   // the waves' sums together
-  const float sum = rows.l + other_half(rows.l);
   constexpr int P = DP + 4;
-  float* mysums = (float*)lds.b + w * 32 * P;
 #pragma unroll
-  for (int i = 0; i < DP / 32; ++i)
+  for (int j = 0; j < NR; ++j) {
+    const float sum = rows[j].l + other_half(rows[j].l);
+    float* mysums = (float*)lds.b + (w * R + 32 * j) * P;
 #pragma unroll
-    for (int b = 0; b < 4; ++b) {
-      Four<float> f;
+    for (int i = 0; i < DP / 32; ++i)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) f.v[e] = rows.acc[i][4 * b + e];
-      *(Four<float>*)(mysums + (l & 31) * P + 32 * i + 8 * b + 4 * (l >> 5)) = f;
+      for (int b = 0; b < 4; ++b) {
+        Four<float> f;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) f.v[e] = rows[j].acc[i][4 * b + e];
+        *(Four<float>*)(mysums + (l & 31) * P + 32 * i + 8 * b + 4 * (l >> 5)) = f;
+      }
+    if (l < 32) {
+      lds.m[w][32 * j + l] = rows[j].m;
+      lds.l[w][32 * j + l] = sum;
     }
-  if (l < 32) {
-    lds.m[w][l] = rows.m;
-    lds.l[w][l] = sum;
   }
   __syncthreads();
   constexpr int PER_ROW = 2 * W, D1 = DP / PER_ROW;  // lanes a row, values a lane
-  const int rr = threadIdx.x / PER_ROW, d0 = threadIdx.x % PER_ROW * D1, row = r0 + rr;
-  if (row >= all) return;
-  float m = NEG_INF, total = 0.f, f[W];
 #pragma unroll
-  for (int i = 0; i < W; ++i) m = fmaxf(m, lds.m[i][rr]);
+  for (int j = 0; j < NR; ++j) {
+    const int rr = 32 * j + threadIdx.x / PER_ROW, d0 = threadIdx.x % PER_ROW * D1, row = r0 + rr;
+    if (row >= all) return;
+    float m = NEG_INF, total = 0.f, f[W];
 #pragma unroll
-  for (int i = 0; i < W; ++i) {
-    const float y = lds.l[i][rr];
-    f[i] = y == 0.f ? 0.f : __builtin_amdgcn_exp2f((lds.m[i][rr] - m) * c);
-    total += f[i] * y;
-  }
-  if (row >= used) total = 0.f;
-  const int64_t at = (p.q0 + row / G) * a.Hq + hk * G + row % G;
-  const float inv = shares > 1 ? 1.f : total != 0.f ? 1.f / total : 0.f;
+    for (int i = 0; i < W; ++i) m = fmaxf(m, lds.m[i][rr]);
 #pragma unroll
-  for (int d = 0; d < D1; ++d) {
-    float y = 0.f;
+    for (int i = 0; i < W; ++i) {
+      const float y = lds.l[i][rr];
+      f[i] = y == 0.f ? 0.f : __builtin_amdgcn_exp2f((lds.m[i][rr] - m) * c);
+      total += f[i] * y;
+    }
+    if (row >= used) total = 0.f;
+    const int64_t at = (p.q0 + row / G) * a.Hq + hk * G + row % G;
+    const float inv = shares > 1 ? 1.f : total != 0.f ? 1.f / total : 0.f;
 #pragma unroll
-    for (int i = 0; i < W; ++i)
-      if (f[i] != 0.f) y += f[i] * ((float*)lds.b)[(i * 32 + rr) * P + d0 + d];
-    if (d0 + d < a.D) {
-      if (shares > 1) {
-        if (total != 0.f) part[(at * shares + blockIdx.z) * a.D + d0 + d] = y;
-      } else {
-        const T z = total == 0.f ? (T)0.f : (T)(y * inv);
-        out[at * a.D + d0 + d] = z;
-        if (rest) rest[at * a.D + d0 + d] = total == 0.f ? (T)0.f : (T)(y * inv - (float)z);
+    for (int d = 0; d < D1; ++d) {
+      float y = 0.f;
+#pragma unroll
+      for (int i = 0; i < W; ++i)
+        if (f[i] != 0.f) y += f[i] * ((float*)lds.b)[(i * R + rr) * P + d0 + d];
+      if (d0 + d < a.D) {
+        if (shares > 1) {
+          if (total != 0.f) part[(at * shares + blockIdx.z) * a.D + d0 + d] = y;
+        } else {
+          const T z = total == 0.f ? (T)0.f : (T)(y * inv);
+          out[at * a.D + d0 + d] = z;
+          if (rest) rest[at * a.D + d0 + d] = total == 0.f ? (T)0.f : (T)(y * inv - (float)z);
+        }
       }
     }
-  }
-  if (d0 == 0) {
-    if (shares > 1)
-      ml[at * shares + blockIdx.z] = make_float2(m * c, total);
-    else if (lse)
-      lse[(at % a.Hq) * a.sq.T + at / a.Hq] =
-          total == 0.f ? NEG_INF : (m * c + __builtin_amdgcn_logf(total)) * LN2;
+    if (d0 == 0) {
+      if (shares > 1)
+        ml[at * shares + blockIdx.z] = make_float2(m * c, total);
+      else if (lse)
+        lse[(at % a.Hq) * a.sq.T + at / a.Hq] =
+            total == 0.f ? NEG_INF : (m * c + __builtin_amdgcn_logf(total)) * LN2;
+    }
   }
 }
 
@@ -411,25 +431,31 @@ AttnArgs attn_args(const int64_t* oq, const int64_t* ok, const int64_t* lq, cons
 // sequence and key head on average are few: with a workgroup's 128 rows most
 // lanes would idle.  So are fewer rows than 128 for each CU: 32 a workgroup, the
 // keys shared by its waves, fill four times as many (float 5 x 600: 42 us where
-// prompts' tiles take 52).  Shares: for four workgroups a CU, of 256 keys or more
-// each (by the room for keys: what is in use is not known here), and none up to
-// 1024 keys, where adding them up takes as long as it saves.
+// prompts' tiles take 52).  Shares (by the room for keys: what is in use is not
+// known here): as many as give every place on the CUs a workgroup, with keys enough
+// in each that starting and adding up are worth it (fewer in float, whose products
+// take longer); for long keys four times as many, so that sequences of different
+// lengths even out.
 struct Way {
-  bool step;
+  int rows;  // a workgroup's: 32 or 64 (few rows), 128 (prompts)
   int shares;
 };
-Way attn_way(int64_t B, int64_t Tq, int64_t Tk, int64_t Hq, int64_t Hk) {
-  Way w{false, 1};
-  const int64_t G = Hq / Hk, n = B < 1 ? 1 : B;
-  w.step = Tq * G <= 64 * n || Tq * Hq < 128 * 256;
-  if (w.step) {
-    const int64_t blocks = (Tq * G / 32 > n ? Tq * G / 32 : n) * Hk;
-    int64_t s = (1024 + blocks - 1) / blocks;
-    if (s > Tk / n / 256) s = Tk / n / 256;
-    if (Tk / n < 1024) s = 1;
-    if (s > 64) s = 64;
-    w.shares = s < 1 ? 1 : (int)s;
-  }
+Way attn_way(int dtype, int64_t B, int64_t Tq, int64_t Tk, int64_t Hq, int64_t Hk, int64_t D) {
+  Way w{128, 1};
+  const int64_t G = Hq / Hk, n = B < 1 ? 1 : B, keys = Tk / n;
+  const int64_t each = Tq < 1 ? 1 : (Tq * G + n - 1) / n;
+  if (each > 64 && Tq * Hq >= 128 * 256) return w;
+  // 33 to 64 rows: both halves at once, k and v read once for them
+  w.rows = each > 32 && each <= 64 ? 64 : 32;
+  const int64_t blocks = (each + w.rows - 1) / w.rows * n * Hk;
+  const int64_t resident = D <= 32 ? 4 : D <= 64 && dtype != TPO_F32 ? 2 : 1;  // workgroups a CU
+  const int64_t least = dtype == TPO_F32 ? 64 : 256;
+  int64_t s = (256 * resident + blocks - 1) / blocks, t = 1024 / blocks;
+  if (s > keys / least) s = keys / least;
+  if (t > keys / 1024) t = keys / 1024;
+  if (s < t) s = t;
+  if (keys < 4 * least) s = 1;
+  w.shares = s < 1 ? 1 : s > 64 ? 64 : (int)s;
   return w;
 }
 
@@ -440,7 +466,7 @@ using namespace tpo;
 extern "C" int64_t tpo_attention_fwd_workspace_size(int dtype, int64_t B, int64_t Tq, int64_t Tk,
                                                     int64_t Hq, int64_t Hk, int64_t D) {
   if (attn_check("attention_fwd_workspace_size", dtype, B, Tq, Tk, Hq, Hk, D)) return -1;
-  const Way w = attn_way(B, Tq, Tk, Hq, Hk);
+  const Way w = attn_way(dtype, B, Tq, Tk, Hq, Hk, D);
   if (w.shares == 1) return 0;
   return round_up(Tq * Hq * w.shares * D * 4, 256) + round_up(Tq * Hq * w.shares * 8, 256);
 }
@@ -465,8 +491,8 @@ extern "C" int tpo_attention_fwd(int dtype, const void* q, const void* k, const 
                      (long long)need);
   const AttnArgs a = attn_args(offsets_q, offsets_k, lengths_q, lengths_k, B, Tq, Tk, Hq, Hk, D,
                                q_row, q_head, k_row, k_head, v_row, v_head, causal, scale);
-  const Way w = attn_way(B, Tq, Tk, Hq, Hk);
-  const int64_t G = Hq / Hk, places = attn_places(Tq, G, B, w.step ? 32 : 128);
+  const Way w = attn_way(dtype, B, Tq, Tk, Hq, Hk, D);
+  const int64_t G = Hq / Hk, places = attn_places(Tq, G, B, w.rows);
   if (places * Hk >= ((int64_t)1 << 31) || Hk > 65535)
     return set_error(TPO_ERR_ARG, "attention_fwd: too many rows");
   hipStream_t s = (hipStream_t)stream;
@@ -476,13 +502,18 @@ extern "C" int tpo_attention_fwd(int dtype, const void* q, const void* k, const 
     typedef decltype(t) T;
     with_head(D, [&](auto dp) {
       constexpr int DP = decltype(dp)::value;
-      if (!w.step)
-        attn_prompt_kernel<T, DP><<<dim3((unsigned)(places * Hk)), 256, 0, s>>>(
-            a, (const T*)q, (const T*)k, (const T*)v, (T*)out, lse, (T*)rest);
-      else
-        attn_step_kernel<T, DP>
+      auto step = [&](auto nr) {
+        attn_step_kernel<T, DP, decltype(nr)::value>
             <<<dim3((unsigned)places, (unsigned)Hk, w.shares), 64 * STEP_WAVES<T, DP>, 0, s>>>(
                 a, (const T*)q, (const T*)k, (const T*)v, (T*)out, lse, (T*)rest, part, ml);
+      };
+      if (w.rows == 128)
+        attn_prompt_kernel<T, DP><<<dim3((unsigned)(places * Hk)), 256, 0, s>>>(
+            a, (const T*)q, (const T*)k, (const T*)v, (T*)out, lse, (T*)rest);
+      else if (w.rows == 64)
+        step(std::integral_constant<int, 2>());
+      else
+        step(std::integral_constant<int, 1>());
     });
     if (w.shares > 1)
       attn_join_kernel<T><<<dim3((unsigned)(Tq * Hq)), 256, 0, s>>>(

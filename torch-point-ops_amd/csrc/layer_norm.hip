@@ -15,7 +15,7 @@ __device__ __forceinline__ float ln_at(const W* w, int64_t c, float none) {
 // A row held in registers by a team of 64 or 256 lanes: N loads a lane of PER
 // values (16 bytes) each.  Rows of other widths begin anywhere: the memory takes
 // 16-byte accesses at any element (at 32768 x 1023 in bfloat16 one value a load
-// took 188 us where this takes LN_ODD), and only a row's last piece goes value by
+// took 188 us where this takes 77), and only a row's last piece goes value by
 // value.  x is read once; the variance is taken about the mean, from the
 // registers.  HBM-bound: what is read and written is all that counts, so teams go
 // on to other rows with the weights in registers, and there are enough of them to
@@ -359,7 +359,7 @@ LnForm ln_form(int64_t width, int64_t size) {
   if (loads <= 256) return {4, 64, true};
   if (loads <= 512) return {2, 256, true};
   if (loads <= 1024) return {4, 256, true};
-  if (loads <= 2048) return {8, 256, true};
+  if (loads <= 2048 && size == 4) return {8, 256, true};  // (16384 half values spill)
   return {0, 0, false};
 }
 // Calls f with the form as types: values a load, loads, team.
@@ -375,18 +375,21 @@ void with_form(const LnForm& f, F&& call) {
   LN_FORM(4, 64);
   LN_FORM(2, 256);
   LN_FORM(4, 256);
-  LN_FORM(8, 256);
+  if constexpr (sizeof(T) == 4) LN_FORM(8, 256);
 #undef LN_FORM
 }
 
 constexpr int64_t LN_WIDTH_MAX = 1 << 20;
 // Shares of the rows for the weights' gradients: workgroups that keep the memory
-// busy, but no more than makes their sums' way through memory a twentieth of the
-// rows' (in half types).
-inline int ln_parts(int64_t rows) {
-  const int64_t few = (rows + 3) / 4, most = rows / 16 > 64 ? rows / 16 : 64;
+// busy, but no more than keeps their sums' way through memory short beside the
+// rows' (16 rows a share, and 8 where a workgroup has one row at a time).  Loading
+// the next row ahead of the sums instead was slower (32768 x 1024: 103 us for 80):
+// it costs the registers of other workgroups.
+inline int ln_parts(int64_t rows, int64_t width) {
+  const int64_t each = width > 2048 ? 8 : 16, top = width > 2048 ? 512 : 1024;
+  const int64_t few = (rows + 3) / 4, most = rows / each > 64 ? rows / each : 64;
   const int64_t p = few < most ? few : most;
-  return (int)(p > 1024 ? 1024 : p);
+  return (int)(p > top ? top : p);
 }
 
 // The weights are of the input's type or float.
@@ -450,7 +453,7 @@ extern "C" int tpo_layer_norm_fwd(int dtype, int wdtype, const void* x, const vo
 
 extern "C" int64_t tpo_layer_norm_bwd_workspace_size(int64_t rows, int64_t width) {
   if (ln_check("layer_norm_bwd_workspace_size", rows, width)) return -1;
-  return round_up((int64_t)ln_parts(rows) * 2 * width * 4, 256);
+  return round_up((int64_t)ln_parts(rows, width) * 2 * width * 4, 256);
 }
 
 extern "C" int tpo_layer_norm_bwd(int dtype, int wdtype, const void* grad_y, const void* x,
@@ -469,7 +472,7 @@ extern "C" int tpo_layer_norm_bwd(int dtype, int wdtype, const void* grad_y, con
     typedef decltype(t) T;
     typedef decltype(w) W;
     const LnForm f = ln_form(width, sizeof(T));
-    const int parts = ln_parts(rows);
+    const int parts = ln_parts(rows, width);
     float* part = sums ? (float*)workspace : nullptr;
     if (rows > 0 && width > LN_NARROW && f.held) {
       with_form<T>(f, [&](auto per, auto n, auto team) {
