@@ -27,14 +27,14 @@ struct RowSums {
     m = NEG_INF;
     l = 0.f;
   }
-  // KT keys from j0 on (k at lds, v after it), of which the lane's row sees those
-  // below n; c: what a score counts in the exponent of 2
+  // The exponentials of KT keys from j0 on (k at lds), of which the lane's row sees
+  // those below n, with the sums brought to their maximum; c: what a score counts in
+  // the exponent of 2.
   template <int KT>
-  __device__ __forceinline__ void add(const HeadLanes<T, DP>& lanes, const char* lds,
-                                      const HeadRows<T, DP>& q, int D, int j0, int n,
-                                      bool masked, float c) {
+  __device__ __forceinline__ void weigh(f32x16 (&s)[KT / 32], const HeadLanes<T, DP>& lanes,
+                                        const char* lds, const HeadRows<T, DP>& q, int D, int j0,
+                                        int n, bool masked, float c) {
     constexpr int PITCH = HeadLds<T, DP>::PITCH;
-    f32x16 s[KT / 32];
 #pragma unroll
     for (int t = 0; t < KT / 32; ++t) s[t] = scores<T, DP>(lanes, lds + 32 * t * PITCH, q, D);
     if (masked) {
@@ -69,9 +69,14 @@ struct RowSums {
         s[t][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][e], c, b));
         l += s[t][e];
       }
+  }
+  // Their part of the sums (v at lds).
+  template <int KT>
+  __device__ __forceinline__ void gather(const f32x16 (&s)[KT / 32], const HeadLanes<T, DP>& lanes,
+                                         const char* lds) {
 #pragma unroll
     for (int t = 0; t < KT / 32; ++t)
-      multiply_rows<T, DP>(acc, lanes, lds + (KT + 32 * t) * PITCH, s[t]);
+      multiply_rows<T, DP>(acc, lanes, lds + 32 * t * HeadLds<T, DP>::PITCH, s[t]);
   }
 };
 
@@ -87,7 +92,11 @@ __device__ __forceinline__ void prompt_step(const char* __restrict__ cur, char* 
   L::template load<KT, 4>(nxt, k, (int)(a.k_row * sizeof(T)), left, a.D, wave_id());
   L::template load<KT, 4>(nxt + TILE, v, (int)(a.v_row * sizeof(T)), left, a.D, wave_id());
   __builtin_amdgcn_sched_barrier(0);
-  if (j0 < most) rows.template add<KT>(lanes, cur, q, a.D, j0, n, j0 + KT > least, c);
+  if (j0 < most) {
+    f32x16 s[KT / 32];
+    rows.template weigh<KT>(s, lanes, cur, q, a.D, j0, n, j0 + KT > least, c);
+    rows.template gather<KT>(s, lanes, cur + TILE);
+  }
 }
 
 // Prompts: a workgroup of four waves takes 128 rows, 32 a wave, and all their
@@ -156,59 +165,80 @@ __global__ __launch_bounds__(256, 2) void attn_prompt_kernel(AttnArgs a, const T
 }
 
 // Few rows over many keys: a workgroup takes 32 NR rows and one of gridDim.z shares
-// of their keys, its W waves in turn a tile of 32 keys each from LDS of their own,
-// so that no wave waits for another before the end.
-template <typename T, int DP> constexpr int STEP_WAVES = sizeof(T) == 4 && DP > 64 ? 2 : 4;
+// of their keys, its four waves in turn a tile of 32 keys each from LDS of their
+// own, so that no wave waits for another before the end.  A wave has room for one
+// tile of k and one of v: v is on its way while the scores are computed, the next
+// k while they are multiplied with v.
+constexpr int STEP_WAVES = 4;
 template <typename T, int DP, int NR = 1>
 struct alignas(1024) StepLds {
   static constexpr int TILE = 32 * HeadLds<T, DP>::PITCH;
-  static constexpr int SUMS = STEP_WAVES<T, DP> * 32 * NR * (DP + 4) * 4;
-  static constexpr int TILES = STEP_WAVES<T, DP> * 4 * TILE;
+  static constexpr int SUMS = STEP_WAVES * 32 * NR * (DP + 4) * 4;
+  static constexpr int TILES = STEP_WAVES * 2 * TILE;
   char b[TILES > SUMS ? TILES : SUMS];
-  float m[STEP_WAVES<T, DP>][32 * NR], l[STEP_WAVES<T, DP>][32 * NR];
+  float m[STEP_WAVES][32 * NR], l[STEP_WAVES][32 * NR];
 };
 
+// 32 rows of k or of v from p on, `left` of them, to a wave's own LDS.
 template <typename T, int DP>
-__device__ __forceinline__ void step_load(char* to, const T* k, const T* v, const AttnArgs& a,
+__device__ __forceinline__ void step_load(char* to, const T* p, int64_t row, const AttnArgs& a,
                                           int left) {
-  typedef HeadLds<T, DP> L;
-  L::template load<32, 1>(to, k, (int)(a.k_row * sizeof(T)), left, a.D, 0);
-  L::template load<32, 1>(to + StepLds<T, DP>::TILE, v, (int)(a.v_row * sizeof(T)), left,
-                                 a.D, 0);
+  HeadLds<T, DP>::template load<32, 1>(to, p, (int)(row * sizeof(T)), left, a.D, 0);
 }
+// Waits until of a wave's loads only the youngest tile's are under way and its LDS
+// reads have ended.
+template <int LOADS>
+__device__ __forceinline__ void step_wait() {
+  __builtin_amdgcn_sched_barrier(0);
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt((LOADS & 15) | (LOADS >> 4) << 14 | 0x70);
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_sched_barrier(0);
+}
+
 // What a lane's row sees: n keys, the rows of its 32 between least and most.
 struct StepRows {
   int n, least, most;
 };
 
+// The two halves of a tile's work; k and v are apart in LDS.
 template <typename T, int DP, int NR>
-__device__ __forceinline__ void step_step(const char* __restrict__ cur, char* __restrict__ nxt,
-                                          const HeadLanes<T, DP>& lanes, const T* k, const T* v,
-                                          const AttnArgs& a, int left,
-                                          const HeadRows<T, DP> (&q)[NR],
-                                          RowSums<T, DP> (&rows)[NR], const StepRows (&sees)[NR],
-                                          int j0, float c) {
-  constexpr int TILE = StepLds<T, DP>::TILE, N = 2 * TILE / 1024;  // loads a tile
-  step_load<T, DP>(nxt, k, v, a, left);
-  __builtin_amdgcn_sched_barrier(0);
-  asm volatile("" ::: "memory");
-  __builtin_amdgcn_s_waitcnt((N & 15) | (N >> 4) << 14 | 0xf70);  // the tile itself has landed
-  asm volatile("" ::: "memory");
-  __builtin_amdgcn_sched_barrier(0);
+__device__ __forceinline__ void step_weigh(const char* __restrict__ kl, char* __restrict__ vl,
+                                           const HeadLanes<T, DP>& lanes, const T* v,
+                                           const AttnArgs& a, int left,
+                                           const HeadRows<T, DP> (&q)[NR],
+                                           RowSums<T, DP> (&rows)[NR], const StepRows (&sees)[NR],
+                                           f32x16 (&s)[NR][1], int j0, float c) {
+  step_load<T, DP>(vl, v, a.v_row, a, left);
+  step_wait<StepLds<T, DP>::TILE / 1024>();  // k has landed
 #pragma unroll
   for (int i = 0; i < NR; ++i)
     if (j0 < sees[i].most)
-      rows[i].template add<32>(lanes, cur, q[i], a.D, j0, sees[i].n, j0 + 32 > sees[i].least, c);
+      rows[i].template weigh<32>(s[i], lanes, kl, q[i], a.D, j0, sees[i].n, j0 + 32 > sees[i].least,
+                                 c);
+}
+template <typename T, int DP, int NR>
+__device__ __forceinline__ void step_gather(char* __restrict__ kl, const char* __restrict__ vl,
+                                            const HeadLanes<T, DP>& lanes, const T* k,
+                                            const AttnArgs& a, int left,
+                                            RowSums<T, DP> (&rows)[NR], const StepRows (&sees)[NR],
+                                            const f32x16 (&s)[NR][1], int j0) {
+  step_load<T, DP>(kl, k, a.k_row, a, left);
+  step_wait<StepLds<T, DP>::TILE / 1024>();  // v has landed
+#pragma unroll
+  for (int i = 0; i < NR; ++i)
+    if (j0 < sees[i].most) rows[i].template gather<32>(s[i], lanes, vl);
 }
 
 // part: with shares, each row's sums (D floats, not divided), and in ml their
 // maximum (in the exponent of 2) and sum
 template <typename T, int DP, int NR>
-__global__ __launch_bounds__((64 * STEP_WAVES<T, DP>)) void attn_step_kernel(
+__global__ __launch_bounds__(64 * STEP_WAVES, (NR == 1 && DP * sizeof(T) <= 256 ? 2 : 1)) void
+attn_step_kernel(
     AttnArgs a, const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ v,
     T* __restrict__ out, float* __restrict__ lse, T* __restrict__ rest,
     float* __restrict__ part, float2* __restrict__ ml) {
-  constexpr int W = STEP_WAVES<T, DP>, TILE = StepLds<T, DP>::TILE, R = 32 * NR;
+  constexpr int W = STEP_WAVES, TILE = StepLds<T, DP>::TILE, R = 32 * NR;
   __shared__ StepLds<T, DP, NR> lds;
   const int G = a.Hq / a.Hk, hk = blockIdx.y, shares = gridDim.z;
   const int64_t place = blockIdx.x;
@@ -237,23 +267,19 @@ __global__ __launch_bounds__((64 * STEP_WAVES<T, DP>)) void attn_step_kernel(
   const float c = attn_count(a.scale);
   const T* kt = k + p.k0 * a.k_row + hk * a.k_head;
   const T* vt = v + p.k0 * a.v_row + hk * a.v_head;
-  char* mine = lds.b + w * 4 * TILE;
+  char *kl = lds.b + w * 2 * TILE, *vl = kl + TILE;
   const HeadLanes<T, DP> lanes;
-  auto load = [&](int t) {
-    step_load<T, DP>(mine, kt + (int64_t)t * 32 * a.k_row, vt + (int64_t)t * 32 * a.v_row, a,
-                     t < t1 ? most - t * 32 : 0);
-  };
-  if (t0 + w < t1) load(t0 + w);
-  int half = 0;
+  if (t0 + w < t1)
+    step_load<T, DP>(kl, kt + (int64_t)(t0 + w) * 32 * a.k_row, a.k_row, a, most - (t0 + w) * 32);
   for (int t = t0 + w; t < t1; t += W) {
-    __builtin_amdgcn_sched_barrier(0);
-    asm volatile("" ::: "memory");
-    __builtin_amdgcn_s_waitcnt(0xc07f);  // the other tile's reads have ended
-    const int64_t next = t + W;
-    step_step<T, DP, NR>(mine + half * 2 * TILE, mine + (half ^ 1) * 2 * TILE, lanes,
-                         kt + next * 32 * a.k_row, vt + next * 32 * a.v_row, a,
-                         next < t1 ? most - (int)next * 32 : 0, x, rows, sees, t * 32, c);
-    half ^= 1;
+    const int64_t j0 = (int64_t)t * 32, next = j0 + 32 * W;
+    f32x16 sc[NR][1];
+    step_wait<TILE / 1024>();  // (the reads of v's place have ended)
+    step_weigh<T, DP, NR>(kl, vl, lanes, vt + j0 * a.v_row, a, most - (int)j0, x, rows, sees, sc,
+                          (int)j0, c);
+    step_wait<TILE / 1024>();  // (and those of k's)
+    step_gather<T, DP, NR>(kl, vl, lanes, kt + next * a.k_row, a,
+                           t + W < t1 ? most - (int)next : 0, rows, sees, sc, (int)j0);
   }
   wait_loads_and_meet<0>();
 
@@ -445,10 +471,11 @@ Way attn_way(int dtype, int64_t B, int64_t Tq, int64_t Tk, int64_t Hq, int64_t H
   const int64_t G = Hq / Hk, n = B < 1 ? 1 : B, keys = Tk / n;
   const int64_t each = Tq < 1 ? 1 : (Tq * G + n - 1) / n;
   if (each > 64 && Tq * Hq >= 128 * 256) return w;
-  // 33 to 64 rows: both halves at once, k and v read once for them
-  w.rows = each > 32 && each <= 64 ? 64 : 32;
+  // 33 to 64 rows: both halves at once, k and v read once for them (long float heads
+  // leave no registers for that)
+  w.rows = each > 32 && each <= 64 && !(dtype == TPO_F32 && D > 96) ? 64 : 32;
   const int64_t blocks = (each + w.rows - 1) / w.rows * n * Hk;
-  const int64_t resident = D <= 32 ? 4 : D <= 64 && dtype != TPO_F32 ? 2 : 1;  // workgroups a CU
+  const int64_t resident = w.rows == 32 && D * element_bytes(dtype) <= 256 ? 2 : 1;  // on a CU
   const int64_t least = dtype == TPO_F32 ? 64 : 256;
   int64_t s = (256 * resident + blocks - 1) / blocks, t = 1024 / blocks;
   if (s > keys / least) s = keys / least;
@@ -504,16 +531,16 @@ extern "C" int tpo_attention_fwd(int dtype, const void* q, const void* k, const 
       constexpr int DP = decltype(dp)::value;
       auto step = [&](auto nr) {
         attn_step_kernel<T, DP, decltype(nr)::value>
-            <<<dim3((unsigned)places, (unsigned)Hk, w.shares), 64 * STEP_WAVES<T, DP>, 0, s>>>(
+            <<<dim3((unsigned)places, (unsigned)Hk, w.shares), 64 * STEP_WAVES, 0, s>>>(
                 a, (const T*)q, (const T*)k, (const T*)v, (T*)out, lse, (T*)rest, part, ml);
       };
       if (w.rows == 128)
         attn_prompt_kernel<T, DP><<<dim3((unsigned)(places * Hk)), 256, 0, s>>>(
             a, (const T*)q, (const T*)k, (const T*)v, (T*)out, lse, (T*)rest);
-      else if (w.rows == 64)
-        step(std::integral_constant<int, 2>());
-      else
+      else if (w.rows == 32)
         step(std::integral_constant<int, 1>());
+      else if constexpr (DP * sizeof(T) < 512)
+        step(std::integral_constant<int, 2>());
     });
     if (w.shares > 1)
       attn_join_kernel<T><<<dim3((unsigned)(Tq * Hq)), 256, 0, s>>>(

@@ -334,10 +334,8 @@ __device__ __forceinline__ f32x16 scores(const HeadLanes<T, DP>& x, const char* 
                                          const HeadRows<T, DP>& y, int D) {
   f32x16 s = {};
 #pragma unroll
-  for (int c = 0; c < HeadRows<T, DP>::N; ++c) {
-    if (sizeof(T) == 4 && 8 * c >= D) break;
-    mma(s, x.by_row(lds, c), y.x[c]);
-  }
+  for (int c = 0; c < HeadRows<T, DP>::N; ++c)
+    if (sizeof(T) == 2 || 8 * c < D) mma(s, x.by_row(lds, c), y.x[c]);
   return s;
 }
 
