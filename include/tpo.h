@@ -417,9 +417,14 @@ int tpo_attention_bwd(int dtype, const void* grad_out, const void* q, const void
  *   x (M,K), w_gate and w_up (F,K), h (M,F); activation is a TPO_ACT_* code
  *   (GELU is x times the normal distribution function, by erf).
  * tpo_gated_bwd: grad_h (M,F) -> grad_x (M,K), grad_w_gate and grad_w_up
- *   (F,K).  The projections are computed again rather than kept, and the
- *   gradients at them are rounded to `dtype` between the products.  grad_x,
- *   or the two weights' gradients together, may be NULL and are left out.
+ *   (F,K).  The gradients at the projections are rounded to `dtype` between
+ *   the products.  grad_x, or the two weights' gradients together, may be NULL
+ *   and are left out.
+ *   keep (M,2F), F32 only, or NULL: the forward's projections, which the
+ *   backward then takes as kept; with NULL it computes them again (as it
+ *   always does for the half types, whose products take less time than
+ *   unrounded projections take through memory).
+ * x, the weights and the workspace are 16-byte aligned.
  * Workspaces are 256-byte aligned; size 0 means none is used.
  */
 enum {
@@ -431,11 +436,11 @@ enum {
 int64_t tpo_gated_fwd_workspace_size(int dtype, int64_t M, int64_t K, int64_t F);
 int tpo_gated_fwd(int dtype, const void* x, const void* w_gate, const void* w_up,
                   int64_t M, int64_t K, int64_t F, int activation, void* h,
-                  void* workspace, int64_t workspace_bytes, void* stream);
+                  void* keep, void* workspace, int64_t workspace_bytes, void* stream);
 int64_t tpo_gated_bwd_workspace_size(int dtype, int64_t M, int64_t K, int64_t F);
 int tpo_gated_bwd(int dtype, const void* grad_h, const void* x, const void* w_gate,
-                  const void* w_up, int64_t M, int64_t K, int64_t F, int activation,
-                  void* grad_x, void* grad_w_gate, void* grad_w_up, void* workspace,
+                  const void* w_up, const void* kept, int64_t M, int64_t K, int64_t F,
+                  int activation, void* grad_x, void* grad_w_gate, void* grad_w_up, void* workspace,
                   int64_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus

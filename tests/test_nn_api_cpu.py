@@ -18,8 +18,8 @@ def lib(tpo):
     L.tpo_layer_norm_bwd.argtypes = [C, C, P, P, P, P, P, I, I, D, P, P, P, P, I, P]
     L.tpo_attention_fwd.argtypes = [C] + [P] * 7 + [I] * 12 + [C, D, P, P, P, P, I, P]
     L.tpo_attention_bwd.argtypes = [C] + [P] * 11 + [I] * 12 + [C, D, P, P, P, P, I, P]
-    L.tpo_gated_fwd.argtypes = [C, P, P, P, I, I, I, C, P, P, I, P]
-    L.tpo_gated_bwd.argtypes = [C, P, P, P, P, I, I, I, C, P, P, P, P, I, P]
+    L.tpo_gated_fwd.argtypes = [C, P, P, P, I, I, I, C, P, P, P, I, P]
+    L.tpo_gated_bwd.argtypes = [C, P, P, P, P, P, I, I, I, C, P, P, P, P, I, P]
     L.tpo_layer_norm_bwd_workspace_size.argtypes = [I, I]
     for n in ("attention_fwd", "attention_bwd"):
         getattr(L, f"tpo_{n}_workspace_size").argtypes = [C] + [I] * 6
@@ -53,7 +53,8 @@ def test_fake_shapes(tpo):
         x, w = torch.empty(3, 4, 16), torch.empty(24, 16)
         h = tpo.gated_projection(x, w, w)
         assert h.shape == (3, 4, 24)
-        g = torch.ops.torch_point_ops_gated.gated_projection_backward(h, x, w, w, 0, [True, False])
+        g = torch.ops.torch_point_ops_gated.gated_projection_backward(
+            h, x, w, w, torch.empty(0), 0, [True, False])
         assert [t.shape for t in g] == [x.shape, (0,), (0,)]
 
 
@@ -127,10 +128,12 @@ def test_attention_entry(lib):
 def test_gated_entry(lib):
     f = P(4096)
     for M, K, F in ((-1, 8, 8), (4, 0, 8), (4, 8, -1), (1 << 40, 8, 8)):
-        assert lib.tpo_gated_fwd(0, f, f, f, M, K, F, 0, f, None, 0, None) == -1
-    assert lib.tpo_gated_fwd(0, f, f, f, 4, 8, 8, 4, f, None, 0, None) == -1
+        assert lib.tpo_gated_fwd(0, f, f, f, M, K, F, 0, f, None, None, 0, None) == -1
+    assert lib.tpo_gated_fwd(0, f, f, f, 4, 8, 8, 4, f, None, None, 0, None) == -1
     assert b"activation" in lib.tpo_last_error()
-    assert lib.tpo_gated_fwd(1, f, f, f, 4, 8, 8, 0, f, None, 0, None) == -2
-    assert lib.tpo_gated_fwd(3, f, f, f, 0, 8, 8, 0, f, None, 0, None) == 0
-    assert lib.tpo_gated_bwd(3, f, f, f, f, 4, 8, 8, 0, f, f, f, None, 0, None) == -4
+    assert lib.tpo_gated_fwd(1, f, f, f, 4, 8, 8, 0, f, None, None, 0, None) == -2
+    assert lib.tpo_gated_fwd(3, f, f, f, 0, 8, 8, 0, f, None, None, 0, None) == 0
+    assert lib.tpo_gated_bwd(3, f, f, f, f, None, 4, 8, 8, 0, f, f, f, None, 0, None) == -4
+    assert lib.tpo_gated_fwd(3, f, f, f, 4, 8, 8, 0, f, f, None, 0, None) == -1  # halves: not kept
+    assert lib.tpo_gated_bwd(3, f, f, f, f, f, 4, 8, 8, 0, f, f, f, f, 1 << 20, None) == -1
     assert lib.tpo_gated_bwd_workspace_size(3, -1, 8, 8) == -1

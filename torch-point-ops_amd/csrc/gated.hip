@@ -78,12 +78,12 @@ __device__ __forceinline__ void tile_of(int tiles_m, int tiles_n, int& m, int& n
 // rows are the features: BM / 4 of the gate and the same of the up projection
 // for either half of the waves' rows, so that a lane holds both sums of an
 // output, and four neighbouring outputs of one token.
-// Forward: h.  Backward (gh): dg and du into d, a token's 2 Fp values, Fp >= F
-// with 0 past F.
+// Forward: h, and with keep g and u themselves, a token's 2 F values.  Backward
+// (gh): dg and du into d, a token's 2 Fp values, Fp >= F with 0 past F.
 template <typename T, int BM, int BN, bool BWD>
 __global__ __launch_bounds__(256, 2) void gated_pair_kernel(
     Matrix x, Matrix wg, Matrix wu, int act, const T* __restrict__ gh, int64_t F,
-    T* __restrict__ out, int64_t Fp, int whole) {
+    T* __restrict__ out, T* __restrict__ keep, int64_t Fp, int whole) {
   __shared__ GatedLds<BM, BN> lds;
   constexpr int SLAB = GatedLds<BM, BN>::SLAB;
   typedef RowLoader<T, BM, SLAB> LA;
@@ -130,12 +130,48 @@ __global__ __launch_bounds__(256, 2) void gated_pair_kernel(
         *(Four<T>*)rg.four(at) = p;
         if (BWD) *(Four<T>*)ru.four(at) = q;
       }
-    if (BWD) {
+    if (!BWD && sizeof(T) == 4 && keep) {
+      rg.store(out, F, t, M, f0, F, whole);
+      for (int y = 0; y < 2; ++y) {
+#pragma unroll
+        for (int i = 0; i < TF; ++i)
+#pragma unroll
+          for (int b = 0; b < 4; ++b) {
+            Four<T> p;
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              p.v[e] = (T)(y ? acc[i + TF][j][4 * b + e] : acc[i][j][4 * b + e]);
+            *(Four<T>*)rg.four(32 * i + 8 * b + 4 * h) = p;
+          }
+        rg.store(keep + y * F, 2 * F, t, M, f0, F, whole);
+      }
+    } else if (BWD) {
       rg.store(out, 2 * Fp, t, M, f0, Fp, true);
       ru.store(out + Fp, 2 * Fp, t, M, f0, Fp, true);
     } else {
       rg.store(out, F, t, M, f0, F, whole);
     }
+  }
+}
+
+// dg and du into d from the g and u that the forward kept.
+__global__ __launch_bounds__(256) void gated_kept_kernel(const float* __restrict__ keep,
+                                                         const float* __restrict__ gh, int64_t M,
+                                                         int64_t F, int64_t Fp, int act,
+                                                         float* __restrict__ d) {
+  const int64_t f = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (f >= Fp) return;
+  for (int64_t m = blockIdx.y; m < M; m += gridDim.y) {
+    float dg = 0.f, du = 0.f;
+    if (f < F) {
+      const float g = keep[m * 2 * F + f], u = keep[m * 2 * F + F + f], y = gh[m * F + f];
+      float a, s;
+      gated_act<float>(act, g, a, s);
+      dg = y * u * s;
+      du = y * a;
+    }
+    d[m * 2 * Fp + f] = dg;
+    d[m * 2 * Fp + Fp + f] = du;
   }
 }
 
@@ -287,7 +323,7 @@ Cut gated_cut(int64_t rows, int64_t cols, int64_t products, int64_t units) {
   else if (middle >= 384) c.tile = MIDDLE;
   if (c.tile == SMALL && units > 0) {
     const int64_t blocks = cdiv(rows, 64) * cdiv(cols, 64) * products;
-    int64_t s = 768 / (blocks < 1 ? 1 : blocks);
+    int64_t s = 1024 / (blocks < 1 ? 1 : blocks);
     const int64_t most = units / 8;  // a share is worth its sums' way through memory
     if (s > most) s = most;
     c.shares = s < 1 ? 1 : (int)s;
@@ -359,14 +395,14 @@ int whole_rows(const void* p, int64_t n) {
 }
 
 template <typename T, bool BWD>
-void gated_pair(const Matrix (&r)[3], int act, const T* gh, int64_t F, T* out, int64_t Fp,
+void gated_pair(const Matrix (&r)[3], int act, const T* gh, int64_t F, T* out, T* keep, int64_t Fp,
                 hipStream_t s) {
   const int64_t M = r[0].rows;
-  const int whole = whole_rows<T>(BWD ? (const void*)gh : (const void*)out, F);
+  const int whole = whole_rows<T>(BWD ? (const void*)gh : (const void*)out, F) && ((uintptr_t)keep & 15) == 0;
   auto run = [&](auto bm, auto bn) {
     constexpr int BM = decltype(bm)::value, BN = decltype(bn)::value;
     gated_pair_kernel<T, BM, BN, BWD><<<dim3((unsigned)(cdiv(M, BN) * cdiv(F, BM / 2))), 256, 0, s>>>(
-        r[0], r[1], r[2], act, gh, F, out, Fp, whole);
+        r[0], r[1], r[2], act, gh, F, out, keep, Fp, whole);
   };
   typedef std::integral_constant<int, 256> I256;
   typedef std::integral_constant<int, 128> I128;
@@ -412,10 +448,12 @@ extern "C" int64_t tpo_gated_fwd_workspace_size(int dtype, int64_t M, int64_t K,
 
 extern "C" int tpo_gated_fwd(int dtype, const void* x, const void* w_gate, const void* w_up,
                              int64_t M, int64_t K, int64_t F, int activation, void* h,
-                             void* workspace, int64_t workspace_bytes, void* stream) {
+                             void* keep, void* workspace, int64_t workspace_bytes, void* stream) {
   if (int rc = gated_check("gated_fwd", dtype, M, K, F, activation)) return rc;
   if (M == 0 || F == 0) return TPO_OK;
   if (int rc = gated_aligned("gated_fwd", {x, w_gate, w_up, workspace})) return rc;
+  if (keep && dtype != TPO_F32)
+    return set_error(TPO_ERR_ARG, "gated_fwd: only float projections are kept");
   const Plan p = gated_plan(dtype, M, K, F, false);
   if (p.bytes > 0 && (!workspace || workspace_bytes < p.bytes))
     return set_error(TPO_ERR_WORKSPACE, "gated_fwd: workspace of %lld bytes needed",
@@ -425,7 +463,7 @@ extern "C" int tpo_gated_fwd(int dtype, const void* x, const void* w_gate, const
     typedef decltype(t) T;
     Matrix r[3];
     gated_inputs<T>(p, x, w_gate, w_up, M, K, F, (char*)workspace, s, r);
-    gated_pair<T, false>(r, activation, nullptr, F, (T*)h, 0, s);
+    gated_pair<T, false>(r, activation, nullptr, F, (T*)h, (T*)keep, 0, s);
   });
   return check_launch("gated_fwd");
 }
@@ -436,7 +474,7 @@ extern "C" int64_t tpo_gated_bwd_workspace_size(int dtype, int64_t M, int64_t K,
 }
 
 extern "C" int tpo_gated_bwd(int dtype, const void* grad_h, const void* x, const void* w_gate,
-                             const void* w_up, int64_t M, int64_t K, int64_t F, int activation,
+                             const void* w_up, const void* kept, int64_t M, int64_t K, int64_t F, int activation,
                              void* grad_x, void* grad_w_gate, void* grad_w_up, void* workspace,
                              int64_t workspace_bytes, void* stream) {
   if (int rc = gated_check("gated_bwd", dtype, M, K, F, activation)) return rc;
@@ -450,14 +488,20 @@ extern "C" int tpo_gated_bwd(int dtype, const void* grad_h, const void* x, const
   hipStream_t s = (hipStream_t)stream;
   char* ws = (char*)workspace;
   if (M == 0 && F == 0) return TPO_OK;
+  if (kept && dtype != TPO_F32)
+    return set_error(TPO_ERR_ARG, "gated_bwd: only float projections are kept");
   with_element(dtype, [&](auto t) {
     typedef decltype(t) T;
     Matrix r[3];
     gated_inputs<T>(p, x, w_gate, w_up, M, K, F, ws, s, r);
     const int64_t row = 2 * p.Fp * sizeof(T);
     float* part = (float*)(ws + p.part);
-    if (M > 0 && F > 0)
-      gated_pair<T, true>(r, activation, (const T*)grad_h, F, (T*)(ws + p.d), p.Fp, s);
+    if (M > 0 && F > 0 && kept)
+      gated_kept_kernel<<<dim3((unsigned)cdiv(p.Fp, 256), (unsigned)(M < 16384 ? M : 16384)), 256, 0,
+                          s>>>((const float*)kept, (const float*)grad_h, M, F, p.Fp, activation,
+                               (float*)(ws + p.d));
+    else if (M > 0 && F > 0)
+      gated_pair<T, true>(r, activation, (const T*)grad_h, F, (T*)(ws + p.d), nullptr, p.Fp, s);
     if (grad_x && M > 0) {
       const Matrix d{ws + p.d, row, M, row};
       T* to = (T*)grad_x;

@@ -398,24 +398,36 @@ Gated gated_args(const Tensor& x, const Tensor& wg, const Tensor& wu, const char
   return a;
 }
 
-Tensor gated_projection_hip(const Tensor& x, const Tensor& wg, const Tensor& wu, int64_t act) {
+std::tuple<Tensor, Tensor> gated_projection_both(const Tensor& x, const Tensor& wg,
+                                                 const Tensor& wu, int64_t act, bool keep) {
   const char* op = "gated_projection";
   const Gated a = gated_args(x, wg, wu, op);
   c10::OptionalDeviceGuard guard(x.device());
   std::vector<int64_t> shape = x.sizes().vec();
   shape.back() = a.F;
-  Tensor h = at::empty(shape, x.options());
+  Tensor h = at::empty(shape, x.options()), kept;
+  if (keep) kept = a.dt == TPO_F32 ? at::empty({a.M, 2 * a.F}, x.options()) : nothing(x);
   const int64_t wsb = tpo_gated_fwd_workspace_size(a.dt, a.M, a.K, a.F);
   const Tensor ws = workspace(wsb, x, op);
   check_rc(tpo_gated_fwd(a.dt, a.x.data_ptr(), a.wg.data_ptr(), a.wu.data_ptr(), a.M, a.K, a.F,
-                         (int)act, h.data_ptr(), data_or_null(ws), wsb, stream_of(x)),
+                         (int)act, h.data_ptr(), data_or_null(kept), data_or_null(ws), wsb,
+                         stream_of(x)),
            op);
-  return h;
+  return {h, kept};
+}
+
+Tensor gated_projection_hip(const Tensor& x, const Tensor& wg, const Tensor& wu, int64_t act) {
+  return std::get<0>(gated_projection_both(x, wg, wu, act, false));
+}
+std::tuple<Tensor, Tensor> gated_projection_forward_hip(const Tensor& x, const Tensor& wg,
+                                                        const Tensor& wu, int64_t act) {
+  return gated_projection_both(x, wg, wu, act, true);
 }
 
 std::tuple<Tensor, Tensor, Tensor> gated_projection_backward_hip(const Tensor& grad_in,
                                                                  const Tensor& x, const Tensor& wg,
-                                                                 const Tensor& wu, int64_t act,
+                                                                 const Tensor& wu,
+                                                                 const Tensor& kept_in, int64_t act,
                                                                  std::array<bool, 2> mask) {
   const char* op = "gated_projection_backward";
   const Gated a = gated_args(x, wg, wu, op);
@@ -423,6 +435,12 @@ std::tuple<Tensor, Tensor, Tensor> gated_projection_backward_hip(const Tensor& g
   TORCH_CHECK(grad_in.dim() == x.dim() && grad_in.size(-1) == a.F &&
                   grad_in.numel() == a.M * a.F && grad_in.device() == x.device(),
               "gated_projection_backward: the gradient must have the output's shape and device");
+  TORCH_CHECK(kept_in.numel() == 0 ||
+                  (kept_in.scalar_type() == at::kFloat && x.scalar_type() == at::kFloat &&
+                   kept_in.numel() == 2 * a.M * a.F && kept_in.device() == x.device()),
+              "gated_projection_backward: kept must be the forward's");
+  Tensor kept;
+  if (kept_in.numel() > 0) kept = kept_in.contiguous();
   const Tensor g = grad_in.to(x.scalar_type()).contiguous();
   Tensor gx, gg, gu;
   if (mask[0]) gx = at::empty(x.sizes(), x.options());
@@ -432,8 +450,8 @@ std::tuple<Tensor, Tensor, Tensor> gated_projection_backward_hip(const Tensor& g
   }
   const int64_t wsb = tpo_gated_bwd_workspace_size(a.dt, a.M, a.K, a.F);
   const Tensor ws = workspace(wsb, x, op);
-  check_rc(tpo_gated_bwd(a.dt, g.data_ptr(), a.x.data_ptr(), a.wg.data_ptr(), a.wu.data_ptr(), a.M,
-                         a.K, a.F, (int)act, data_or_null(gx), data_or_null(gg), data_or_null(gu),
+  check_rc(tpo_gated_bwd(a.dt, g.data_ptr(), a.x.data_ptr(), a.wg.data_ptr(), a.wu.data_ptr(),
+                         data_or_null(kept), a.M, a.K, a.F, (int)act, data_or_null(gx), data_or_null(gg), data_or_null(gu),
                          data_or_null(ws), wsb, stream_of(x)),
            op);
   if (!gx.defined()) gx = nothing(x);
@@ -451,19 +469,24 @@ class GatedProjectionFunction : public torch::autograd::Function<GatedProjection
  public:
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& wg, const Tensor& wu,
                         int64_t act) {
-    ctx->save_for_backward({x, wg, wu});
-    ctx->saved_data["act"] = act;
+    static auto op =
+        typed_op<std::tuple<Tensor, Tensor>(const Tensor&, const Tensor&, const Tensor&, int64_t)>(
+            "torch_point_ops_gated::gated_projection_forward");
     at::AutoDispatchBelowADInplaceOrView below;
-    return gated_projection_op().call(x, wg, wu, act);
+    auto [h, kept] = op.call(x, wg, wu, act);
+    ctx->save_for_backward({x, wg, wu, kept});
+    ctx->saved_data["act"] = act;
+    return h;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     static auto op = typed_op<std::tuple<Tensor, Tensor, Tensor>(
-        const Tensor&, const Tensor&, const Tensor&, const Tensor&, int64_t, std::array<bool, 2>)>(
-        "torch_point_ops_gated::gated_projection_backward");
+        const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&, int64_t,
+        std::array<bool, 2>)>("torch_point_ops_gated::gated_projection_backward");
     const auto s = ctx->get_saved_variables();
     const bool gate = ctx->needs_input_grad(1), up = ctx->needs_input_grad(2);
     const std::array<bool, 2> mask = {ctx->needs_input_grad(0), gate || up};
-    auto [gx, gg, gu] = op.call(grads[0], s[0], s[1], s[2], ctx->saved_data["act"].toInt(), mask);
+    auto [gx, gg, gu] =
+        op.call(grads[0], s[0], s[1], s[2], s[3], ctx->saved_data["act"].toInt(), mask);
     return {mask[0] ? gx : Tensor(), gate ? gg : Tensor(), up ? gu : Tensor(), Tensor()};
   }
 };
@@ -493,6 +516,10 @@ std::tuple<Tensor, Tensor, Tensor> packed_attention_forward_cpu(const Tensor&, c
                                                         const Tensor&, const OptTensor&,
                                                         const OptTensor&, bool, double) {
   TORCH_CHECK(false, "packed_attention is not implemented for CPU");
+}
+std::tuple<Tensor, Tensor> gated_projection_forward_cpu(const Tensor&, const Tensor&,
+                                                        const Tensor&, int64_t) {
+  TORCH_CHECK(false, "gated_projection is not implemented for CPU");
 }
 Tensor gated_projection_cpu(const Tensor&, const Tensor&, const Tensor&, int64_t) {
   TORCH_CHECK(false, "gated_projection is not implemented for CPU");
@@ -548,14 +575,19 @@ TORCH_LIBRARY_IMPL(torch_point_ops_attention, Autograd, m) {
 
 TORCH_LIBRARY(torch_point_ops_gated, m) {
   m.def("gated_projection(Tensor x, Tensor w_gate, Tensor w_up, int activation) -> Tensor");
+  // with the projections themselves (float; empty for the half types)
+  m.def("gated_projection_forward(Tensor x, Tensor w_gate, Tensor w_up, int activation) -> "
+        "(Tensor, Tensor)");
   m.def("gated_projection_backward(Tensor grad, Tensor x, Tensor w_gate, Tensor w_up, "
-        "int activation, bool[2] mask) -> (Tensor, Tensor, Tensor)");
+        "Tensor kept, int activation, bool[2] mask) -> (Tensor, Tensor, Tensor)");
 }
 TORCH_LIBRARY_IMPL(torch_point_ops_gated, CPU, m) {
   m.impl("gated_projection", &gated_projection_cpu);
+  m.impl("gated_projection_forward", &gated_projection_forward_cpu);
 }
 TORCH_LIBRARY_IMPL(torch_point_ops_gated, CUDA, m) {
   m.impl("gated_projection", &gated_projection_hip);
+  m.impl("gated_projection_forward", &gated_projection_forward_hip);
   m.impl("gated_projection_backward", &gated_projection_backward_hip);
 }
 TORCH_LIBRARY_IMPL(torch_point_ops_gated, Autograd, m) {

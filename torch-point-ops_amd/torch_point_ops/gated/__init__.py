@@ -16,8 +16,16 @@ def _gated_projection_fake(x, w_gate, w_up, activation):
     return torch.empty(*x.shape[:-1], w_gate.shape[0], device=x.device, dtype=x.dtype)
 
 
+@torch.library.register_fake("torch_point_ops_gated::gated_projection_forward")
+def _gated_projection_forward_fake(x, w_gate, w_up, activation):
+    rows = x.numel() // x.shape[-1]
+    return (torch.empty(*x.shape[:-1], w_gate.shape[0], device=x.device, dtype=x.dtype),
+            x.new_empty(rows, 2 * w_gate.shape[0]) if x.dtype == torch.float32
+            else x.new_empty(0))
+
+
 @torch.library.register_fake("torch_point_ops_gated::gated_projection_backward")
-def _gated_projection_backward_fake(grad, x, w_gate, w_up, activation, mask):
+def _gated_projection_backward_fake(grad, x, w_gate, w_up, kept, activation, mask):
     gx = torch.empty(x.shape if mask[0] else (0,), device=x.device, dtype=x.dtype)
     gg, gu = (torch.empty(w_gate.shape if mask[1] else (0,), device=x.device, dtype=x.dtype)
               for _ in range(2))
@@ -29,9 +37,10 @@ def gated_projection(x, w_gate, w_up, activation="silu"):
 
     Args: x (..., K), w_gate and w_up (F, K), float32, float16 or bfloat16; activation
     "silu", "gelu" (x times the normal distribution function), "relu" or "sigmoid".
-    Differentiable in x and the weights; the backward computes the projections again
-    instead of keeping them, and rounds the gradients at them to x's type between the
-    products.  All sums are float32.  Returns (..., F).
+    Differentiable in x and the weights.  A float32 forward keeps the two projections for
+    the backward; for the half types the backward computes them again, which takes less
+    time than unrounded ones take through memory, and rounds the gradients at them to x's
+    type between the products.  All sums are float32.  Returns (..., F).
     """
     code = _ACTIVATIONS.get(activation)
     if code is None:
