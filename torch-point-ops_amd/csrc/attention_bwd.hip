@@ -255,7 +255,7 @@ __device__ __forceinline__ void bwd_keys_step(const char* __restrict__ cur, char
 // tiles that all four waves share.  Wave w has keys 32 (w % 2) .. + 31 and half w /
 // 2 of each tile's rows; at the end two waves add what they have, one stores dK,
 // one dV.  (128 keys with all rows a wave: half as many workgroups of twice the
-// length, 128 us where this takes KEYS_US for 8 x 2048.)
+// length, 128 us where this takes 123 for 8 x 2048.)
 template <typename T, int DP>
 __global__ __launch_bounds__(256, (DP * sizeof(T) <= 128 ? 2 : 1)) void attn_bwd_keys_kernel(
     AttnArgs a, const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ v,

@@ -154,6 +154,138 @@ __global__ __launch_bounds__(256, 2) void gated_pair_kernel(
   }
 }
 
+// Few tokens (up to 32 TN): the weights' way from memory is all that counts.  A
+// workgroup takes 32 features and all tokens; its four waves take every fourth slab
+// of the summed axis each, through LDS of their own and without waiting for each
+// other, and add up their sums at the end.  Results as gated_pair_kernel's.
+template <typename T, int TN>
+struct alignas(1024) FewLds {
+  static constexpr int SLAB = 128, DEPTH = TN == 1 ? 3 : 2, STAGE = (64 + 32 * TN) * SLAB;
+  char b[4][DEPTH][STAGE];
+};
+
+// A wave's loads of a slab: 32 rows of the gate's weights, of the up projection's,
+// of 32 TN tokens.
+template <typename T, int TN>
+struct FewLoader {
+  typedef RowLoader<T, 128, 128> L;  // 32 rows: a quarter of 128
+  static constexpr int LOADS = (2 + TN) * L::N;
+  L g, u, x0, x1;  // (x1: the second 32 tokens)
+  __device__ __forceinline__ FewLoader(const Matrix& wg, const Matrix& wu, const Matrix& xs,
+                                       int64_t f0)
+      : g(wg, f0), u(wu, f0), x0(xs, 0), x1(xs, 32) {}
+  __device__ __forceinline__ void load(char* lds, int slab) const {
+    lds -= wave_id() * L::N * 1024;  // (where the loader puts wave 0's rows)
+    const auto sg = g.slab(slab), su = u.slab(slab);
+#pragma unroll
+    for (int j = 0; j < L::N; ++j) sg.load(lds, j);
+#pragma unroll
+    for (int j = 0; j < L::N; ++j) su.load(lds + 32 * 128, j);
+#pragma unroll
+    for (int i = 0; i < TN; ++i) {
+      const auto sx = (i ? x1 : x0).slab(slab);
+#pragma unroll
+      for (int j = 0; j < L::N; ++j) sx.load(lds + (64 + 32 * i) * 128, j);
+    }
+  }
+};
+
+template <typename T, int TN>
+__device__ __forceinline__ void few_step(const char* __restrict__ cur, char* __restrict__ nxt,
+                                         const FewLoader<T, TN>& load, int next,
+                                         f32x16 (&acc)[2][TN]) {
+  typedef RowLoader<T, 128, 128> L;
+  load.load(nxt, next);
+  __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+  for (int s = 0; s < 4; ++s) {
+    const auto g = L::read(cur, 0, s), u = L::read(cur, 32, s);
+#pragma unroll
+    for (int i = 0; i < TN; ++i) {
+      const auto x = L::read(cur, 64 + 32 * i, s);
+      mma(acc[0][i], g, x);
+      mma(acc[1][i], u, x);
+    }
+  }
+}
+
+template <typename T, int TN, bool BWD>
+__global__ __launch_bounds__(256) void gated_few_kernel(Matrix x, Matrix wg, Matrix wu, int act,
+                                                        const T* __restrict__ gh, int64_t F,
+                                                        T* __restrict__ out, T* __restrict__ keep,
+                                                        int64_t Fp) {
+  typedef FewLds<T, TN> Lds;
+  __shared__ Lds lds;
+  const int w = wave_id(), l = lane_id();
+  const int64_t f0 = (int64_t)blockIdx.x * 32;
+  const FewLoader<T, TN> load(wg, wu, x, f0);
+  const int slabs = (int)((x.bytes + 127) / 128);
+  f32x16 acc[2][TN];
+#pragma unroll
+  for (int i = 0; i < TN; ++i) acc[0][i] = acc[1][i] = f32x16{};
+#pragma unroll
+  for (int d = 0; d < Lds::DEPTH - 1; ++d) load.load(lds.b[w][d], w + 4 * d);
+  int at = 0;
+  for (int k = w; k < slabs; k += 4) {
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("" ::: "memory");
+    constexpr int n = (Lds::DEPTH - 2) * FewLoader<T, TN>::LOADS;
+    __builtin_amdgcn_s_waitcnt((n & 15) | (n >> 4) << 14 | 0x70);  // the slab has landed
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+    const int free = at == 0 ? Lds::DEPTH - 1 : at - 1;
+    few_step<T, TN>(lds.b[w][at], lds.b[w][free], load, k + 4 * (Lds::DEPTH - 1), acc);
+    at = at + 1 == Lds::DEPTH ? 0 : at + 1;
+  }
+  wait_loads_and_meet<0>();
+  f32x4* sums = (f32x4*)&lds;  // [wave][gate, up][tokens][b][lane]
+#pragma unroll
+  for (int y = 0; y < 2; ++y)
+#pragma unroll
+    for (int i = 0; i < TN; ++i)
+#pragma unroll
+      for (int b = 0; b < 4; ++b)
+        sums[(((w * 2 + y) * TN + i) * 4 + b) * 64 + l] =
+            f32x4{acc[y][i][4 * b], acc[y][i][4 * b + 1], acc[y][i][4 * b + 2], acc[y][i][4 * b + 3]};
+  __syncthreads();
+  // wave w finishes values b = w of the lanes' columns
+#pragma unroll
+  for (int i = 0; i < TN; ++i) {
+    f32x4 g = {}, u = {};
+#pragma unroll
+    for (int v = 0; v < 4; ++v) {
+      const f32x4 y = sums[(((v * 2 + 0) * TN + i) * 4 + w) * 64 + l];
+      const f32x4 z = sums[(((v * 2 + 1) * TN + i) * 4 + w) * 64 + l];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        g[e] += y[e];
+        u[e] += z[e];
+      }
+    }
+    const int64_t m = 32 * i + (l & 31), f = f0 + 8 * w + 4 * (l >> 5);
+    if (m >= x.rows) continue;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      float a, d;
+      gated_act<T>(act, g[e], a, d);
+      if (BWD) {
+        const bool in = f + e < F;
+        const float y = in ? (float)gh[m * F + f + e] : 0.f;
+        if (f + e < Fp) {
+          out[m * 2 * Fp + f + e] = in ? (T)(y * u[e] * d) : (T)0.f;
+          out[m * 2 * Fp + Fp + f + e] = in ? (T)(y * a) : (T)0.f;
+        }
+      } else if (f + e < F) {
+        out[m * F + f + e] = (T)(a * u[e]);
+        if (keep) {
+          keep[m * 2 * F + f + e] = (T)g[e];
+          keep[m * 2 * F + F + f + e] = (T)u[e];
+        }
+      }
+    }
+  }
+}
+
 // dg and du into d from the g and u that the forward kept.
 __global__ __launch_bounds__(256) void gated_kept_kernel(const float* __restrict__ keep,
                                                          const float* __restrict__ gh, int64_t M,
@@ -404,6 +536,14 @@ void gated_pair(const Matrix (&r)[3], int act, const T* gh, int64_t F, T* out, T
     gated_pair_kernel<T, BM, BN, BWD><<<dim3((unsigned)(cdiv(M, BN) * cdiv(F, BM / 2))), 256, 0, s>>>(
         r[0], r[1], r[2], act, gh, F, out, keep, Fp, whole);
   };
+  if (M <= 64) {  // (16 x 2048 x 8192: 12.8 where the smallest tile takes 22.6)
+    const dim3 grid((unsigned)cdiv(BWD ? Fp : F, 32));
+    if (M <= 32)
+      gated_few_kernel<T, 1, BWD><<<grid, 256, 0, s>>>(r[0], r[1], r[2], act, gh, F, out, keep, Fp);
+    else
+      gated_few_kernel<T, 2, BWD><<<grid, 256, 0, s>>>(r[0], r[1], r[2], act, gh, F, out, keep, Fp);
+    return;
+  }
   typedef std::integral_constant<int, 256> I256;
   typedef std::integral_constant<int, 128> I128;
   typedef std::integral_constant<int, 64> I64;
