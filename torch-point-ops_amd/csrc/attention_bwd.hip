@@ -254,13 +254,14 @@ __device__ __forceinline__ void bwd_keys_step(const char* __restrict__ cur, char
 // dK and dV of 64 keys: for each head of the group, the rows that see them in
 // tiles that all four waves share.  Wave w has keys 32 (w % 2) .. + 31 and half w /
 // 2 of each tile's rows; at the end two waves add what they have, one stores dK,
-// one dV.  (128 keys with all rows a wave: half as many workgroups of twice the
+// one dV.  blockIdx.y: a share of the group's heads, `heads` of them; with more than
+// one its sums go to part as floats (dK, then dV).  (128 keys with all rows a wave: half as many workgroups of twice the
 // length, 128 us where this takes 123 for 8 x 2048.)
 template <typename T, int DP>
-__global__ __launch_bounds__(256, (DP * sizeof(T) <= 128 ? 2 : 1)) void attn_bwd_keys_kernel(
+__global__ __launch_bounds__(256, (DP * sizeof(T) <= 192 ? 2 : 1)) void attn_bwd_keys_kernel(
     AttnArgs a, const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ v,
     const T* __restrict__ go, const float* __restrict__ sub, const float* __restrict__ delta,
-    T* __restrict__ gk, T* __restrict__ gv) {
+    T* __restrict__ gk, T* __restrict__ gv, int heads, float* __restrict__ part) {
   constexpr int KT = BWD_ROWS, STAGE = BwdKeysLds<T, DP>::STAGE;
   __shared__ BwdKeysLds<T, DP> lds;
   const int G = a.Hq / a.Hk, hk = blockIdx.x % a.Hk;
@@ -291,7 +292,8 @@ __global__ __launch_bounds__(256, (DP * sizeof(T) <= 128 ? 2 : 1)) void attn_bwd
   // tiles of rows, head after head; the next one to load is head ng's from row ni on
   const T *qt, *gt;
   const float *st, *dt;
-  int ng = 0, ni = start;
+  const int g0 = blockIdx.y * heads, g1 = g0 + heads < G ? g0 + heads : G;
+  int ng = g0, ni = start;
   auto head_at = [&]() {
     const int64_t head = hk * G + ng, row = p.q0 + start;
     qt = q + row * a.q_row + head * a.q_head;
@@ -307,7 +309,7 @@ __global__ __launch_bounds__(256, (DP * sizeof(T) <= 128 ? 2 : 1)) void attn_bwd
     dt += KT;
     if (ni >= end) {
       ni = start;
-      if (++ng < G) head_at();
+      if (++ng < g1) head_at();
     }
   };
   const HeadLanes<T, DP> lanes;
@@ -315,7 +317,7 @@ __global__ __launch_bounds__(256, (DP * sizeof(T) <= 128 ? 2 : 1)) void attn_bwd
     constexpr int H = decltype(half)::value;
     wait_loads_and_meet<0>();
     bwd_keys_step<T, DP>(lds.b + H * STAGE, lds.b + (1 - H) * STAGE, lanes, qt, gt, st, dt, a,
-                         ng < G ? end - ni : 0, x, y, sums, w >> 1, i, end - i, lo, least, most,
+                         ng < g1 ? end - ni : 0, x, y, sums, w >> 1, i, end - i, lo, least, most,
                          only, c);
     advance();
   };
@@ -324,7 +326,7 @@ __global__ __launch_bounds__(256, (DP * sizeof(T) <= 128 ? 2 : 1)) void attn_bwd
     bwd_keys_load<T, DP>(lds.b, qt, gt, st, dt, a, end - start);
     advance();
     int i = start;
-    const int all = tiles * G;
+    const int all = tiles * (g1 - g0);
     for (int n = 0; n < all; n += 2) {
       step(std::integral_constant<int, 0>(), i);
       i = i + KT >= end ? start : i + KT;
@@ -357,9 +359,26 @@ __global__ __launch_bounds__(256, (DP * sizeof(T) <= 128 ? 2 : 1)) void attn_bwd
     __syncthreads();
   }
   if (j0 >= p.room_k) return;
+  const float f = w < 2 ? a.scale : 1.f;
+  if (part) {  // a lane's values one after another: few bytes beside the products
+    if (j < p.room_k) {
+      float* to = part + (((int64_t)blockIdx.y * 2 + (w >> 1)) * a.sk.T + p.k0 + j) * a.Hk * a.D +
+                  hk * a.D + 4 * (l >> 5);
+#pragma unroll
+      for (int i = 0; i < DP / 32; ++i)
+#pragma unroll
+        for (int b = 0; b < 4; ++b)
+          if (32 * i + 8 * b + 4 * (l >> 5) < a.D) {
+            f32x4 z;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) z[e] = in ? own[i][4 * b + e] * f : 0.f;
+            *(f32x4*)(to + 32 * i + 8 * b) = z;
+          }
+    }
+    return;
+  }
   typedef Rows32<T, DP> R;
   const R to{lds.b + w * R::BYTES};
-  const float f = w < 2 ? a.scale : 1.f;
 #pragma unroll
   for (int i = 0; i < DP / 32; ++i)
 #pragma unroll
@@ -373,6 +392,38 @@ __global__ __launch_bounds__(256, (DP * sizeof(T) <= 128 ? 2 : 1)) void attn_bwd
            true);
 }
 
+// The shares of the group's heads added up: n values of dK, then n of dV.
+template <typename T>
+__global__ __launch_bounds__(256) void attn_bwd_join_kernel(const float* __restrict__ part,
+                                                            int shares, int64_t n,
+                                                            T* __restrict__ gk,
+                                                            T* __restrict__ gv) {
+  T* to = blockIdx.y ? gv : gk;
+  for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4; i < n;
+       i += (int64_t)gridDim.x * 1024) {
+    f32x4 s = {};
+    for (int p = 0; p < shares; ++p) {
+      const f32x4 x = *(const f32x4*)(part + ((int64_t)p * 2 + blockIdx.y) * n + i);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[e] += x[e];
+    }
+    Four<T> z;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) z.v[e] = (T)s[e];
+    *(Four<T>*)(to + i) = z;
+  }
+}
+
+// How many shares of a group's heads dK and dV take: enough to give every CU four
+// workgroups, where keys alone do not (2000 keys of two heads, eight query heads
+// each: 270 us for all heads in one, 157 and 11 for the sums by three shares).
+int attn_bwd_shares(int64_t B, int64_t Tk, int64_t Hq, int64_t Hk) {
+  const int64_t G = Hq / Hk, blocks = (Tk / 64 + B / 2 + 1) * Hk;
+  int64_t s = 1024 / blocks;
+  if (s > G) s = G;
+  return s < 2 ? 1 : (int)s;
+}
+
 }  // namespace tpo
 
 using namespace tpo;
@@ -380,7 +431,9 @@ using namespace tpo;
 extern "C" int64_t tpo_attention_bwd_workspace_size(int dtype, int64_t B, int64_t Tq, int64_t Tk,
                                                     int64_t Hq, int64_t Hk, int64_t D) {
   if (attn_check("attention_bwd_workspace_size", dtype, B, Tq, Tk, Hq, Hk, D)) return -1;
-  return 2 * round_up(Tq * Hq * 4, 256);
+  const int64_t shares = attn_bwd_shares(B, Tk, Hq, Hk);
+  return 2 * round_up(Tq * Hq * 4, 256) +
+         (shares > 1 ? round_up(shares * 2 * Tk * Hk * D * 4, 256) : 0);
 }
 
 extern "C" int tpo_attention_bwd(int dtype, const void* grad_out, const void* q, const void* k,
@@ -409,7 +462,11 @@ extern "C" int tpo_attention_bwd(int dtype, const void* grad_out, const void* q,
   const int64_t places_q = attn_places(Tq, G, B, 64), places_k = attn_places(Tk, 1, B, 64);
   if (places_q * Hk >= ((int64_t)1 << 31) || places_k * Hk >= ((int64_t)1 << 31))
     return set_error(TPO_ERR_ARG, "attention_bwd: too many rows");
-  float *sub = (float*)workspace, *delta = (float*)((char*)workspace + need / 2);
+  const int64_t stats = round_up(Tq * Hq * 4, 256);
+  float *sub = (float*)workspace, *delta = (float*)((char*)workspace + stats);
+  const int shares = attn_bwd_shares(B, Tk, Hq, Hk), heads = (int)((G + shares - 1) / shares);
+  const int used = (int)((G + heads - 1) / heads);  // shares that have a head
+  float* part = used > 1 ? (float*)((char*)workspace + 2 * stats) : nullptr;
   hipStream_t s = (hipStream_t)stream;
   with_element(dtype, [&](auto t) {
     typedef decltype(t) T;
@@ -423,9 +480,14 @@ extern "C" int tpo_attention_bwd(int dtype, const void* grad_out, const void* q,
         attn_bwd_q_kernel<T, DP><<<dim3((unsigned)(places_q * Hk)), 256, 0, s>>>(
             a, qt, kt, vt, go, sub, delta, (T*)grad_q);
       if (Tk > 0)
-        attn_bwd_keys_kernel<T, DP><<<dim3((unsigned)(places_k * Hk)), 256, 0, s>>>(
-            a, qt, kt, vt, go, sub, delta, (T*)grad_k, (T*)grad_v);
+        attn_bwd_keys_kernel<T, DP><<<dim3((unsigned)(places_k * Hk), used), 256, 0, s>>>(
+            a, qt, kt, vt, go, sub, delta, (T*)grad_k, (T*)grad_v, heads, part);
     });
+    if (Tk > 0 && part) {
+      const int64_t n = Tk * Hk * D, blocks = (n + 1023) / 1024;
+      attn_bwd_join_kernel<T><<<dim3((unsigned)(blocks < 2048 ? blocks : 2048), 2), 256, 0, s>>>(
+          part, used, n, (T*)grad_k, (T*)grad_v);
+    }
   });
   return check_launch("attention_bwd");
 }

@@ -438,29 +438,42 @@ inline int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // How a product of `rows` x `cols` sums (the rows being what the tile's longer
 // side covers) is cut: the tile and the number of shares of the summed axis,
-// `units` long.  A CU takes two workgroups of the larger tiles at a time, so the
-// largest tile that gives nearly two a CU is taken (half as many would leave
-// half of the matrix cores' time to waiting); where even the smallest tile gives
-// fewer, the summed axis is shared out, if the caller can add the shares up.
-// 1000 x 385 x 1023 in float, training: 115 us with 64-tiles, 233 with 128.
+// `units` long (0: not to be shared).  By estimated time: a tile's products at the
+// rate that the tile reached with every place on the CUs taken (PFLOP/s of half
+// types, of float at about a seventh: 256 x 128 1.05, 128 x 128 0.9, 64 x 64
+// 0.56), in as many rounds as there are places; shares' sums at 4 TB/s through
+// memory, and a launch that adds them.  dX of 4096 x 1024 x 4096: 117 us in
+// 64-tiles, 97 as it is cut; float 1000 x 385 x 1023 training: 115 us with
+// 64-tiles, 233 with 128.
 enum Tile { LARGE, MIDDLE, SMALL };  // 256 x 128, 128 x 128, 64 x 64 (128 x 64 for the pair)
 struct Cut {
   Tile tile;
   int shares;
 };
-Cut gated_cut(int64_t rows, int64_t cols, int64_t products, int64_t units) {
-  const int64_t middle = cdiv(rows, 128) * cdiv(cols, 128) * products;
-  Cut c{SMALL, 1};
-  if (cdiv(rows, 256) * cdiv(cols, 128) * products >= 448) c.tile = LARGE;
-  else if (middle >= 384) c.tile = MIDDLE;
-  if (c.tile == SMALL && units > 0) {
-    const int64_t blocks = cdiv(rows, 64) * cdiv(cols, 64) * products;
-    int64_t s = 1024 / (blocks < 1 ? 1 : blocks);
-    const int64_t most = units / 8;  // a share is worth its sums' way through memory
-    if (s > most) s = most;
-    c.shares = s < 1 ? 1 : (int)s;
+Cut gated_cut(int dtype, int64_t rows, int64_t cols, int64_t products, int64_t units,
+              int64_t summed) {
+  static const int64_t R[] = {256, 128, 64}, C[] = {128, 128, 64}, PLACES[] = {512, 512, 1024};
+  static const double RATE[] = {1.05e15, 0.9e15, 0.56e15}, FLOAT_RATE[] = {0.13e15, 0.13e15, 0.1e15};
+  Cut best{SMALL, 1};
+  double least = 1e30;
+  for (int t = 0; t < 3; ++t) {
+    const double rate = dtype == TPO_F32 ? FLOAT_RATE[t] : RATE[t];
+    const int64_t blocks = cdiv(rows, R[t]) * cdiv(cols, C[t]) * products;
+    for (int64_t s = 1; s <= 64; s *= 2) {
+      if (s > 1 && s > units / 8) break;
+      // rounds by halves: places that are half taken work faster, though not twice
+      const double filled = (double)(blocks * s) / PLACES[t];
+      const double rounds = filled <= 0.5 ? 0.62 : filled <= 1 ? 1 : 0.5 * (double)(int64_t)(2 * filled + 0.99);
+      const double tile = 2.0 * R[t] * C[t] * ((double)summed / s);
+      double time = rounds * tile * PLACES[t] / rate;
+      if (s > 1) time += 8.0 * s * rows * cols * products / 4e12 + 5e-6;
+      if (time < least) {
+        least = time;
+        best = Cut{(Tile)t, (int)s};
+      }
+    }
   }
-  return c;
+  return best;
 }
 
 // What the calls keep in the workspace, in bytes from its start.
@@ -492,8 +505,8 @@ Plan gated_plan(int dtype, int64_t M, int64_t K, int64_t F, bool bwd) {
   }
   if (bwd) {
     p.d = take(M * 2 * p.Fp, z);
-    p.dx = gated_cut(K, M, 1, 2 * p.funits);
-    p.dw = gated_cut(K, F, 2, p.munits);
+    p.dx = gated_cut(dtype, K, M, 1, 2 * p.funits, 2 * p.Fp);
+    p.dw = gated_cut(dtype, K, F, 2, p.munits, M);
     const int64_t a = p.dx.shares > 1 ? p.dx.shares * M * K : 0;
     const int64_t b = p.dw.shares > 1 ? p.dw.shares * 2 * F * K : 0;
     p.part = take(a > b ? a : b, 4);
@@ -547,7 +560,7 @@ void gated_pair(const Matrix (&r)[3], int act, const T* gh, int64_t F, T* out, T
   typedef std::integral_constant<int, 256> I256;
   typedef std::integral_constant<int, 128> I128;
   typedef std::integral_constant<int, 64> I64;
-  switch (gated_cut(2 * F, M, 1, 0).tile) {
+  switch (gated_cut(sizeof(T) == 4 ? TPO_F32 : TPO_BF16, 2 * F, M, 1, 0, r[0].bytes / sizeof(T)).tile) {
     case LARGE: run(I256(), I128()); break;
     case MIDDLE: run(I128(), I128()); break;
     case SMALL: run(I128(), I64()); break;
