@@ -78,6 +78,43 @@ def test_grouped_heads(tpo, dev, Hq, Hk, causal):
     _check(tpo, dev, [50, 3, 90], [50, 3, 90], Hq, Hk, 32, torch.bfloat16, causal, seed=Hq)
 
 
+# rows enough to fill the chip without sharing keys: tiles of 128 rows
+@pytest.mark.parametrize("D", [8, 33, 40, 64, 96, 128])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("causal", [True, False])
+def test_many_rows(tpo, dev, D, dtype, causal):
+    lens = [600, 1, 0, 437, 130, 64, 65]
+    _check(tpo, dev, lens, lens, 32, 8, D, dtype, causal, seed=D, grad=D == 64)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("causal", [True, False])
+def test_many_rows_of_rooms_in_part_used(tpo, dev, dtype, causal):
+    lens_q, lens_k = [300, 200, 0, 140, 500], [500, 20, 40, 140, 130]
+    _check(tpo, dev, lens_q, lens_k, 32, 16, 32, dtype, causal, lq=[290, 129, 0, 0, 499],
+           lk=[333, 20, 1, 140, 127], before=(3, 5), after=(7, 2), seed=33, grad=False)
+
+
+# 33 to 64 rows a key head on average, of queries or of the heads that share keys,
+# over few keys and over many (in shares)
+@pytest.mark.parametrize("lens_q,lens_k,Hq", [
+    ([40, 64, 33], [40, 64, 33], 1), ([40, 65, 3], [2500, 1100, 3000], 1), ([5, 7, 8], [2500, 0, 3000], 8),
+    ([1, 1], [5000, 1025], 40), ([3, 4], [5, 2], 16),
+])
+@pytest.mark.parametrize("D", [40, 64, 128])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("causal", [True, False])
+def test_pairs_of_tiles(tpo, dev, lens_q, lens_k, Hq, D, dtype, causal):
+    _check(tpo, dev, lens_q, lens_k, Hq, 1, D, dtype, causal, seed=D + Hq, grad=D == 64)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_shares_of_rooms_in_part_used(tpo, dev, dtype):
+    """Keys are shared by their room; of some sequences whole shares are unused."""
+    _check(tpo, dev, [1, 2, 1, 1], [4000, 3000, 2000, 5000], 8, 2, 64, dtype, True,
+           lk=[4000, 17, 0, 2049], seed=8)
+
+
 # rows and keys of different numbers: causal rows that see no key, a few rows
 # over many keys, many rows over few, no keys at all
 @pytest.mark.parametrize("lens_q,lens_k", [
@@ -282,6 +319,31 @@ def test_step_by_step_over_a_cache(tpo, dev):
         step = tpo.packed_attention(Q.view(B, P, Hq, D)[:, t], ck.view(-1, Hk, D),
                                     cv.view(-1, Hk, D), one, o, lengths_k=used)
         nn64.near(step, whole[:, t].cpu().double())
+
+
+@pytest.mark.parametrize("causal", [True, False])
+def test_many_sequences(tpo, dev, causal):
+    """More sequences than a wave has lanes, of more than one tile each."""
+    lens = [150 + b for b in range(70)]
+    _check(tpo, dev, lens, lens, 2, 1, 32, torch.bfloat16, causal, seed=70)
+
+
+def test_cache_beyond_32_bits(tpo, dev):
+    """Sequences that begin more than 2^32 bytes into the arrays of keys and values."""
+    H, D, n = 8, 128, 300
+    T = (1 << 32) // (H * D * 2) + 2 * n
+    q, k, v, go = _qkv(2 * n, 2 * n, H, H, D, torch.bfloat16, 12)
+    K, V = (torch.empty(T, H, D, dtype=torch.bfloat16, device=dev) for _ in range(2))
+    for big, small in ((K, k), (V, v)):
+        big[:n], big[-n:] = small[:n], small[-n:]
+    oq, ok = [0, n, 2 * n], [0, T - n, T]
+    want = nn64.attention(q, k, v, oq, oq, None, None, True, D ** -0.5)
+    lk = [n, n]
+    got = tpo.packed_attention(q.to(dev), K, V, *_dev(dev, oq, ok, None, lk))
+    nn64.near(got, want, roundings=2)
+    last = torch.tensor([0, n - 1, n, 2 * n - 1])  # one row a sequence: every key, by shares
+    step = tpo.packed_attention(q.to(dev)[last[1::2]], K, V, *_dev(dev, [0, 1, 2], ok, None, lk))
+    nn64.near(step, want[last[1::2]], roundings=2)
 
 
 def test_empty_calls(tpo, dev):

@@ -43,6 +43,17 @@ def test_values_and_gradients(tpo, dev, M, K, F, dtype):
     _check(tpo, dev, M, K, F, dtype, "silu", seed=M + K + F)
 
 
+# enough of two of the axes for the largest tiles in one product each (the
+# projections; x's gradient; the weights'), and for the middle ones in all, with
+# sums that are shared and ends inside tiles
+@pytest.mark.parametrize("M,K,F", [
+    (5000, 99, 2203), (8180, 2041, 66), (131, 2041, 4090), (1999, 2050, 1027), (4097, 100, 2050),
+])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_large_tiles(tpo, dev, M, K, F, dtype):
+    _check(tpo, dev, M, K, F, dtype, "gelu", seed=M + K + F)
+
+
 @pytest.mark.parametrize("name", ACTS)
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_activations(tpo, dev, name, dtype):
@@ -112,6 +123,17 @@ def test_layouts_and_shapes(tpo, dev, dtype):
     nn64.near(tpo.gated_projection(wide[:, 1:73], G, U), want, **f)
     flat = torch.cat([torch.zeros(1, dtype=dtype, device=dev), G.flatten()])
     nn64.near(tpo.gated_projection(X, flat[1:].view(40, 72), U), want, **f)  # off the 16-byte grid
+
+
+def test_more_than_32_bits_of_values(tpo, dev):
+    """Outputs beyond 2^31 values; one weight's rows and the last tokens are checked."""
+    M, F = (1 << 31) // 8192 + 100, 8192
+    x, wg, wu, _ = _inputs(200, 64, F, torch.bfloat16, 13)
+    X = torch.zeros(M, 64, dtype=torch.bfloat16, device=dev)
+    X[-200:] = x.to(dev)
+    h = tpo.gated_projection(X, wg.to(dev), wu.to(dev))
+    nn64.near(h[-200:], nn64.gated(x, wg, wu, "silu"), floats=4e-6)
+    assert (h[:3] == 0).all()
 
 
 def test_nonfinite_rows_stay_apart(tpo, dev):

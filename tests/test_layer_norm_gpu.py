@@ -125,6 +125,18 @@ def test_layouts_streams_and_empty(tpo, dev):
     assert y.shape == ge.shape == (0, 48) and (gw == 0).all()
 
 
+def test_more_than_32_bits_of_values(tpo, dev):
+    rows, width = (1 << 31) // 4096 + 5, 4096
+    x = torch.empty(rows, width, dtype=torch.bfloat16, device=dev)
+    g = torch.Generator().manual_seed(3)
+    tail = torch.randn(7, width, generator=g).to(torch.bfloat16)
+    x.zero_()
+    x[-7:] = tail
+    y = tpo.layer_norm(x)
+    nn64.near(y[-7:], nn64.layer_norm(tail, None, None, 1e-5))
+    assert (y[:3] == 0).all()
+
+
 def test_gradient_sums_repeat(tpo, dev):
     x, w, b, gy = _inputs((9000, 130), torch.float32, "same", 8)
     X, W, B = _on(dev, x, w, b)
