@@ -268,6 +268,16 @@ struct HeadRows {
 #pragma unroll
     for (int s = 0; s < N; ++s) x[s] = -x[s];
   }
+  // The lane's part of the sum of products with another array's row.
+  __device__ __forceinline__ float dot(const HeadRows& y) const {
+    float sum = 0.f;
+#pragma unroll
+    for (int s = 0; s < N; ++s)
+#pragma unroll
+      for (int e = 0; e < (int)(16 / sizeof(T)); ++e)
+        sum = __builtin_fmaf((float)x[s][e], (float)y.x[s][e], sum);
+    return sum;
+  }
 };
 
 // A wave's 32 rows of sums, f times each, to the rows r0 .. of a sequence and key

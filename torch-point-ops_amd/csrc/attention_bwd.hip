@@ -10,47 +10,12 @@
 // score): dP and delta, which are sums in different orders, would leave their
 // rounding there, so it is said outright.
 // Half types: P and dS are rounded to the type for the products that take them.
+// The first kernel also makes, of each row, what is subtracted in the exponent of 2
+// (the logarithm of its sum; infinity where the row sees no key, which makes its P
+// 0) and delta = sum_d dO O, and leaves them to the second one.
 #include "attention.hpp"
 
 namespace tpo {
-
-// Of each row: what is subtracted in the exponent of 2 (the logarithm of its sum;
-// infinity where the row sees no key, which makes its P 0), and delta =
-// sum_d dO O.  rest: what rounding took from O.  Without it the rounding of O,
-// which is common to all keys of a row, would add to dQ's error about half of
-// what the rounding of dS does.  Sixteen lanes a row.
-template <typename T>
-__global__ __launch_bounds__(256) void attn_delta_kernel(const T* __restrict__ o,
-                                                         const T* __restrict__ rest,
-                                                         const T* __restrict__ go,
-                                                         const float* __restrict__ lse,
-                                                         int64_t rows, int Hq, int64_t Tq, int D,
-                                                         float* __restrict__ sub,
-                                                         float* __restrict__ delta) {
-  const int64_t r = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
-  if (r >= rows) return;
-  constexpr int PER = 16 / sizeof(T);
-  typedef typename Chunk<T>::V V;
-  float s = 0.f;
-  for (int c = (threadIdx.x & 15) * PER; c < D; c += 16 * PER) {
-    const V x = *(const V*)(o + r * D + c), y = *(const V*)(go + r * D + c);
-#pragma unroll
-    for (int e = 0; e < PER; ++e) s = __builtin_fmaf((float)x[e], (float)y[e], s);
-    if (rest) {
-      const V z = *(const V*)(rest + r * D + c);
-#pragma unroll
-      for (int e = 0; e < PER; ++e) s = __builtin_fmaf((float)z[e], (float)y[e], s);
-    }
-  }
-#pragma unroll
-  for (int d = 8; d > 0; d >>= 1) s += __shfl_xor(s, d);
-  if ((threadIdx.x & 15) == 0) {
-    const int64_t at = r % Hq * Tq + r / Hq;
-    const float m = lse[at];
-    sub[at] = m == NEG_INF ? -NEG_INF : m * LOG2E;
-    delta[at] = m == NEG_INF ? 0.f : s;
-  }
-}
 
 // Two tiles of 64 rows, twice over; later what waves exchange, and the rows on
 // their way out.
@@ -99,11 +64,15 @@ __device__ __forceinline__ void bwd_q_step(const char* __restrict__ cur, char* _
 
 // dQ of 64 rows; the rows and their keys as the forward for prompts has them.
 // Wave w has rows 32 (w % 2) .. + 31 and half w / 2 of each tile of keys; at the
-// end two waves' sums are added.
+// end two waves' sums are added.  rest: what rounding took from O.  Without it the
+// rounding of O, which is common to all keys of a row, would add to dQ's error about
+// half of what the rounding of dS does.  (delta by a kernel of its own, which reads dO
+// once more, took 18 us of 234 for 8 x 2048; so they are 226.)
 template <typename T, int DP>
 __global__ __launch_bounds__(256, (DP * sizeof(T) <= 256 ? 2 : 1)) void attn_bwd_q_kernel(
     AttnArgs a, const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ v,
-    const T* __restrict__ go, const float* __restrict__ sub, const float* __restrict__ delta,
+    const T* __restrict__ go, const T* __restrict__ o, const T* __restrict__ rest,
+    const float* __restrict__ lse, float* __restrict__ sub, float* __restrict__ delta,
     T* __restrict__ gq) {
   constexpr int KT = BWD_ROWS, TILE = BwdRowsLds<T, DP>::TILE;
   __shared__ BwdRowsLds<T, DP> lds;
@@ -125,8 +94,25 @@ __global__ __launch_bounds__(256, (DP * sizeof(T) <= 256 ? 2 : 1)) void attn_bwd
   HeadRows<T, DP> x, y;
   x.load(q + token * a.q_row + head * a.q_head, in, a.D);
   y.load(go + (token * a.Hq + head) * a.D, in, a.D);
-  const float row_sub = in ? sub[head * a.sq.T + token] : -NEG_INF;
-  const float row_delta = in ? delta[head * a.sq.T + token] : 0.f;
+  const int64_t at = head * a.sq.T + token;
+  const float m = in ? lse[at] : NEG_INF;
+  const float row_sub = m == NEG_INF ? -NEG_INF : m * LOG2E;
+  float row_delta = 0.f;
+  {
+    HeadRows<T, DP> z;
+    z.load(o + (token * a.Hq + head) * a.D, in, a.D);
+    row_delta += y.dot(z);
+    if (rest) {
+      z.load(rest + (token * a.Hq + head) * a.D, in, a.D);
+      row_delta += y.dot(z);
+    }
+    row_delta += other_half(row_delta);
+    if (m == NEG_INF) row_delta = 0.f;
+  }
+  if (in && w < 2 && l < 32) {
+    sub[at] = row_sub;
+    delta[at] = row_delta;
+  }
   const float c = attn_count(a.scale);
   if (a.scale < 0.f) x.negate();
   f32x16 acc[DP / 32];
@@ -458,7 +444,7 @@ extern "C" int tpo_attention_bwd(int dtype, const void* grad_out, const void* q,
     return rc;
   const AttnArgs a = attn_args(offsets_q, offsets_k, lengths_q, lengths_k, B, Tq, Tk, Hq, Hk, D,
                                q_row, q_head, k_row, k_head, v_row, v_head, causal, scale);
-  const int64_t rows = Tq * Hq, G = Hq / Hk;
+  const int64_t G = Hq / Hk;
   const int64_t places_q = attn_places(Tq, G, B, 64), places_k = attn_places(Tk, 1, B, 64);
   if (places_q * Hk >= ((int64_t)1 << 31) || places_k * Hk >= ((int64_t)1 << 31))
     return set_error(TPO_ERR_ARG, "attention_bwd: too many rows");
@@ -471,14 +457,11 @@ extern "C" int tpo_attention_bwd(int dtype, const void* grad_out, const void* q,
   with_element(dtype, [&](auto t) {
     typedef decltype(t) T;
     const T *go = (const T*)grad_out, *qt = (const T*)q, *kt = (const T*)k, *vt = (const T*)v;
-    if (Tq > 0)
-      attn_delta_kernel<T><<<dim3((unsigned)((rows + 15) / 16)), 256, 0, s>>>(
-          (const T*)out, (const T*)rest, go, lse, rows, (int)Hq, Tq, (int)D, sub, delta);
     with_head(D, [&](auto dp) {
       constexpr int DP = decltype(dp)::value;
       if (Tq > 0)
         attn_bwd_q_kernel<T, DP><<<dim3((unsigned)(places_q * Hk)), 256, 0, s>>>(
-            a, qt, kt, vt, go, sub, delta, (T*)grad_q);
+            a, qt, kt, vt, go, (const T*)out, (const T*)rest, lse, sub, delta, (T*)grad_q);
       if (Tk > 0)
         attn_bwd_keys_kernel<T, DP><<<dim3((unsigned)(places_k * Hk), used), 256, 0, s>>>(
             a, qt, kt, vt, go, sub, delta, (T*)grad_k, (T*)grad_v, heads, part);
