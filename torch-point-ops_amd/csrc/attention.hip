@@ -112,9 +112,8 @@ __global__ __launch_bounds__(256, 2) void attn_prompt_kernel(AttnArgs a, const T
   __shared__ PromptLds<T, DP> lds;
   const int G = a.Hq / a.Hk, hk = blockIdx.x % a.Hk;
   int local;
-  const int s = attn_tile<true>(a.sq, blockIdx.x / a.Hk, gridDim.x / a.Hk, G, 128, local);
-  if (s < 0) return;
-  const AttnSpan p = attn_span(a, s);
+  AttnSpan p;
+  if (!attn_tile<false>(a, blockIdx.x / a.Hk, gridDim.x / a.Hk, G, 128, p, local)) return;
   const int all = p.room_q * G;
   const int w = wave_id(), l = lane_id(), r0 = local * 128 + 32 * w, r = r0 + (l & 31);
   const int used = p.Lq * G;
@@ -126,12 +125,6 @@ __global__ __launch_bounds__(256, 2) void attn_prompt_kernel(AttnArgs a, const T
   const bool in = r < used;
   const int head = hk * G + r % G;
   const int64_t token = p.q0 + r / G;
-  HeadRows<T, DP> x;
-  x.load(q + token * a.q_row + head * a.q_head, in, a.D);
-  const float c = attn_count(a.scale);
-  if (a.scale < 0.f) x.negate();
-  RowSums<T, DP> rows;
-  rows.clear();
   const T* kt = k + p.k0 * a.k_row + hk * a.k_head;
   const T* vt = v + p.k0 * a.v_row + hk * a.v_head;
   typedef HeadLds<T, DP> L;
@@ -139,6 +132,12 @@ __global__ __launch_bounds__(256, 2) void attn_prompt_kernel(AttnArgs a, const T
     L::template load<KT, 4>(lds.b, kt, (int)(a.k_row * sizeof(T)), p.Lk, a.D, w);
     L::template load<KT, 4>(lds.b + TILE, vt, (int)(a.v_row * sizeof(T)), p.Lk, a.D, w);
   }
+  HeadRows<T, DP> x;
+  x.load(q + token * a.q_row + head * a.q_head, in, a.D);
+  const float c = attn_count(a.scale);
+  if (a.scale < 0.f) x.negate();
+  RowSums<T, DP> rows;
+  rows.clear();
   const HeadLanes<T, DP> lanes;
   auto step = [&](auto half, int j0) {  // (the halves by name: LDS addresses are constants)
     constexpr int H = decltype(half)::value;
@@ -241,13 +240,11 @@ attn_step_kernel(
   constexpr int W = STEP_WAVES, TILE = StepLds<T, DP>::TILE, R = 32 * NR;
   __shared__ StepLds<T, DP, NR> lds;
   const int G = a.Hq / a.Hk, hk = blockIdx.y, shares = gridDim.z;
-  const int64_t place = blockIdx.x;
-  const int s = attn_sequence(a.sq, place, G, R);
-  const AttnSpan p = attn_span(a, s);
-  const int64_t local = uniform(place - attn_first(a.sq, s, G, R));
+  int local;
+  AttnSpan p;
+  if (!attn_place(a, blockIdx.x, G, R, p, local)) return;
   const int all = p.room_q * G;
-  if (local < 0 || local * R >= all) return;
-  const int w = wave_id(), l = lane_id(), r0 = (int)local * R;
+  const int w = wave_id(), l = lane_id(), r0 = local * R;
   const int used = p.Lq * G;
   auto keys = [&](int row) { return used ? attn_keys(a, p, row < used ? row : used - 1, G) : 0; };
   StepRows sees[NR];

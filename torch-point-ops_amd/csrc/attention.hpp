@@ -62,13 +62,13 @@ __device__ __forceinline__ int64_t uniform(int64_t v) {
 // each size 1 .. c (a causal prompt's last tile sees the most keys, its first keys
 // are seen by the most rows).  Where workgroups are few, the long ones have to
 // start first: in the order of places a training step's dK and dV kept the CUs
-// busy for 58 % of its time.  A lane tries one size; sequences, at most 64 of
-// them, are passed round.  Returns the sequence, or -1, and the tile's size.
-__device__ __forceinline__ int attn_by_size(const Sequences& s, int p, int G, int tile, int& size) {
+// busy for 58 % of its time.  A lane tries one size; sequences, n of them with c
+// tiles in lane c's place, are passed round.  Returns the sequence, or -1, and the
+// tile's size.
+__device__ __forceinline__ int attn_by_size(int c, int seqs, int p, int& size) {
   const int l = lane_id();
-  const int c = l < s.B + 2 ? (int)((s.room(l) * G + tile - 1) / tile) : 0;
   int lo = 0, hi = 0;
-  for (int i = 0; i < s.B + 2; ++i) {
+  for (int i = 0; i < seqs; ++i) {
     const int y = __builtin_amdgcn_readlane(c, i);
     hi = y > hi ? y : hi;
   }
@@ -76,7 +76,7 @@ __device__ __forceinline__ int attn_by_size(const Sequences& s, int p, int G, in
   while (hi > lo) {
     const int step = (hi - lo + 63) >> 6, u = lo + l * step;
     int n = 0;
-    for (int i = 0; i < s.B + 2; ++i) {
+    for (int i = 0; i < seqs; ++i) {
       const int y = __builtin_amdgcn_readlane(c, i) - u;
       n += y > 0 ? y : 0;
     }
@@ -90,7 +90,7 @@ __device__ __forceinline__ int attn_by_size(const Sequences& s, int p, int G, in
   size = lo;
   if (lo == 0) return -1;
   int n = 0;
-  for (int i = 0; i < s.B + 2; ++i) {
+  for (int i = 0; i < seqs; ++i) {
     const int y = __builtin_amdgcn_readlane(c, i) - lo;
     n += y > 0 ? y : 0;
   }
@@ -99,30 +99,6 @@ __device__ __forceinline__ int attn_by_size(const Sequences& s, int p, int G, in
   const uint64_t at = __builtin_amdgcn_ballot_w64(c >= lo && rank == p - n);
   return at ? __builtin_ctzll(at) : -1;
 }
-
-// The sequence and tile of workgroup p, the largest first; -1: none.  LATE: a
-// sequence's last tile is its largest.
-template <bool LATE>
-__device__ __forceinline__ int attn_tile(const Sequences& s, int p, int places, int G, int tile,
-                                         int& local) {
-  int i;
-  if (s.B + 2 <= 64) {
-    int size;
-    i = attn_by_size(s, p, G, tile, size);
-    if (i < 0) return -1;
-    i = __builtin_amdgcn_readfirstlane(i);
-    const int c = (int)((uniform(s.room(i)) * G + tile - 1) / tile);
-    local = LATE ? size - 1 : c - size;
-  } else {  // many sequences: many workgroups
-    const int64_t place = LATE ? places - 1 - p : p;
-    i = attn_sequence(s, place, G, tile);
-    const int64_t n = uniform(place - attn_first(s, i, G, tile));
-    if (n < 0 || n * tile >= uniform(s.room(i)) * G) return -1;
-    local = (int)n;
-  }
-  return i;
-}
-
 
 // A workgroup's sequence: its queries and keys, and where they begin.
 struct AttnSpan {
@@ -139,6 +115,96 @@ __device__ __forceinline__ AttnSpan attn_span(const AttnArgs& a, int s) {
   p.Lq = (int)uniform(a.sq.used(s));
   p.Lk = (int)uniform(a.sk.used(s));
   return p;
+}
+
+// Up to 62 sequences: each lane has one of them (with the rows before the first and
+// after the last), so that one trip to memory brings what decides and all that is
+// needed of the sequence then.  (In two or three trips a workgroup's beginning took
+// 5 us of its 40 for 8 x 2048.)
+constexpr int ATTN_LANES = 62;
+struct AttnLanes {
+  int start[2], room[2], used[2];  // of queries, of keys
+  __device__ __forceinline__ explicit AttnLanes(const AttnArgs& a) {
+    const int l = lane_id(), B = a.sq.B;
+    const int i = l < 1 ? 0 : (l - 1 < B ? l - 1 : B), j = l < B ? l : B;
+    int64_t o[2], p[2], n[2];
+#pragma unroll
+    for (int y = 0; y < 2; ++y) {
+      const Sequences& s = y ? a.sk : a.sq;
+      o[y] = s.offsets[i];
+      p[y] = s.offsets[j];
+      n[y] = s.T;
+      if (s.lengths && l >= 1 && l <= B) n[y] = s.lengths[l - 1];
+    }
+#pragma unroll
+    for (int y = 0; y < 2; ++y) {
+      const int T = (int)(y ? a.sk.T : a.sq.T);
+      auto inside = [](int64_t v, int most) { return v < 0 ? 0 : (v > most ? most : (int)v); };
+      start[y] = l < 1 ? 0 : (l > B + 1 ? T : inside(o[y], T));
+      const int next = l > B ? T : inside(p[y], T);
+      room[y] = next > start[y] ? next - start[y] : 0;
+      used[y] = l < 1 || l > B ? 0 : inside(n[y], room[y]);
+    }
+  }
+  __device__ __forceinline__ AttnSpan span(int s) const {
+    AttnSpan p;
+    p.q0 = __builtin_amdgcn_readlane(start[0], s);
+    p.k0 = __builtin_amdgcn_readlane(start[1], s);
+    p.room_q = __builtin_amdgcn_readlane(room[0], s);
+    p.room_k = __builtin_amdgcn_readlane(room[1], s);
+    p.Lq = __builtin_amdgcn_readlane(used[0], s);
+    p.Lk = __builtin_amdgcn_readlane(used[1], s);
+    return p;
+  }
+};
+
+// The sequence and tile (of queries, or with KEYS_ of keys) of workgroup p of
+// `places`, the largest first; false: none.  A sequence's last tile of queries is its
+// largest, its first tile of keys.
+template <bool KEYS_>
+__device__ __forceinline__ bool attn_tile(const AttnArgs& a, int p, int places, int G, int tile,
+                                          AttnSpan& span, int& local) {
+  if (a.sq.B <= ATTN_LANES) {
+    const AttnLanes lanes(a);
+    const int c = (int)(((int64_t)lanes.room[KEYS_] * G + tile - 1) / tile);
+    int size;
+    int i = attn_by_size(c, a.sq.B + 2, p, size);
+    if (i < 0) return false;
+    i = __builtin_amdgcn_readfirstlane(i);
+    local = KEYS_ ? __builtin_amdgcn_readlane(c, i) - size : size - 1;
+    span = lanes.span(i);
+    return true;
+  }
+  // many sequences: many workgroups
+  const Sequences& s = KEYS_ ? a.sk : a.sq;
+  const int64_t place = KEYS_ ? p : places - 1 - p;
+  const int i = attn_sequence(s, place, G, tile);
+  const int64_t n = uniform(place - attn_first(s, i, G, tile));
+  if (n < 0 || n * tile >= uniform(s.room(i)) * G) return false;
+  local = (int)n;
+  span = attn_span(a, i);
+  return true;
+}
+
+// As much for the rows at a place, in the order of places.
+__device__ __forceinline__ bool attn_place(const AttnArgs& a, int64_t place, int G, int tile,
+                                           AttnSpan& span, int& local) {
+  int64_t first;
+  if (a.sq.B <= ATTN_LANES) {
+    const AttnLanes lanes(a);
+    const int64_t at = (int64_t)lanes.start[0] * G / tile + lane_id();
+    const uint64_t m = __builtin_amdgcn_ballot_w64(lane_id() < a.sq.B + 2 && at <= place);
+    const int i = m ? 63 - __builtin_clzll(m) : 0;
+    span = lanes.span(i);
+    first = span.q0 * G / tile + i;
+  } else {
+    const int i = attn_sequence(a.sq, place, G, tile);
+    span = attn_span(a, i);
+    first = span.q0 * G / tile + i;
+  }
+  const int64_t n = place - first;
+  local = (int)n;
+  return n >= 0 && n * tile < (int64_t)span.room_q * G;
 }
 
 // The value of lane l ^ 32

@@ -78,9 +78,8 @@ __global__ __launch_bounds__(256, (DP * sizeof(T) <= 256 ? 2 : 1)) void attn_bwd
   __shared__ BwdRowsLds<T, DP> lds;
   const int G = a.Hq / a.Hk, hk = blockIdx.x % a.Hk;
   int local;
-  const int s = attn_tile<true>(a.sq, blockIdx.x / a.Hk, gridDim.x / a.Hk, G, 64, local);
-  if (s < 0) return;
-  const AttnSpan p = attn_span(a, s);
+  AttnSpan p;
+  if (!attn_tile<false>(a, blockIdx.x / a.Hk, gridDim.x / a.Hk, G, 64, p, local)) return;
   const int all = p.room_q * G;
   const int w = wave_id(), l = lane_id(), r0 = local * 64 + 32 * (w & 1), r = r0 + (l & 31);
   const int used = p.Lq * G;
@@ -91,6 +90,9 @@ __global__ __launch_bounds__(256, (DP * sizeof(T) <= 256 ? 2 : 1)) void attn_bwd
   const bool in = r < used;
   const int head = hk * G + r % G;
   const int64_t token = p.q0 + r / G;
+  const T* kt = k + p.k0 * a.k_row + hk * a.k_head;
+  const T* vt = v + p.k0 * a.v_row + hk * a.v_head;
+  if (end > 0) bwd_q_load<T, DP>(lds.b, kt, vt, a, p.Lk);
   HeadRows<T, DP> x, y;
   x.load(q + token * a.q_row + head * a.q_head, in, a.D);
   y.load(go + (token * a.Hq + head) * a.D, in, a.D);
@@ -118,9 +120,6 @@ __global__ __launch_bounds__(256, (DP * sizeof(T) <= 256 ? 2 : 1)) void attn_bwd
   f32x16 acc[DP / 32];
 #pragma unroll
   for (int i = 0; i < DP / 32; ++i) acc[i] = f32x16{};
-  const T* kt = k + p.k0 * a.k_row + hk * a.k_head;
-  const T* vt = v + p.k0 * a.v_row + hk * a.v_head;
-  if (end > 0) bwd_q_load<T, DP>(lds.b, kt, vt, a, p.Lk);
   const HeadLanes<T, DP> lanes;
   auto step = [&](auto half, int j0) {
     constexpr int H = decltype(half)::value;
@@ -252,9 +251,8 @@ __global__ __launch_bounds__(256, (DP * sizeof(T) <= 192 ? 2 : 1)) void attn_bwd
   __shared__ BwdKeysLds<T, DP> lds;
   const int G = a.Hq / a.Hk, hk = blockIdx.x % a.Hk;
   int local;
-  const int s = attn_tile<false>(a.sk, blockIdx.x / a.Hk, gridDim.x / a.Hk, 1, 64, local);
-  if (s < 0) return;
-  const AttnSpan p = attn_span(a, s);
+  AttnSpan p;
+  if (!attn_tile<true>(a, blockIdx.x / a.Hk, gridDim.x / a.Hk, 1, 64, p, local)) return;
   const int w = wave_id(), l = lane_id(), b0 = local * 64, j0 = b0 + 32 * (w & 1), j = j0 + (l & 31);
   const bool in = j < p.Lk;
   HeadRows<T, DP> x, y;
