@@ -95,6 +95,32 @@ def test_many_rows_of_rooms_in_part_used(tpo, dev, dtype, causal):
            lk=[333, 20, 1, 140, 127], before=(3, 5), after=(7, 2), seed=33, grad=False)
 
 
+# as many workgroups by heads of their own; and by sequences of a few rows each
+@pytest.mark.parametrize("D", [8, 33, 64, 96, 128])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("causal", [True, False])
+def test_many_heads(tpo, dev, D, dtype, causal):
+    lens = [600, 1, 0, 437, 130, 64, 65]
+    _check(tpo, dev, lens, lens, 32, 32, D, dtype, causal, seed=D + 1, grad=D == 64)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("causal", [True, False])
+def test_many_heads_of_rooms_in_part_used(tpo, dev, dtype, causal):
+    lens_q, lens_k = [300, 200, 0, 140, 500], [500, 20, 40, 140, 130]
+    _check(tpo, dev, lens_q, lens_k, 64, 64, 32, dtype, causal, lq=[290, 129, 0, 0, 499],
+           lk=[333, 20, 1, 140, 127], before=(3, 5), after=(7, 2), seed=34, grad=False)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("causal", [True, False])
+def test_many_short_sequences(tpo, dev, D, dtype, causal):
+    lens_q, lens_k = [b % 5 for b in range(70)], [7 * b % 200 for b in range(70)]
+    _check(tpo, dev, lens_q, lens_k, 16, 8, D, dtype, causal, lk=[7 * b % 200 * (b % 3) // 2 for b in range(70)],
+           seed=D + 2, grad=False)
+
+
 # 33 to 64 rows a key head on average, of queries or of the heads that share keys,
 # over few keys and over many (in shares)
 @pytest.mark.parametrize("lens_q,lens_k,Hq", [

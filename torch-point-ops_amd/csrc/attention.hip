@@ -163,19 +163,19 @@ __global__ __launch_bounds__(256, 2) void attn_prompt_kernel(AttnArgs a, const T
         inv == 0.f ? NEG_INF : (rows.m * c + __builtin_amdgcn_logf(sum)) * LN2;
 }
 
-// Few rows over many keys: a workgroup takes 32 NR rows and one of gridDim.z shares
+// Few rows over many keys: a workgroup takes 32 rows and one of gridDim.z shares
 // of their keys, its four waves in turn a tile of 32 keys each from LDS of their
 // own, so that no wave waits for another before the end.  A wave has room for one
 // tile of k and one of v: v is on its way while the scores are computed, the next
 // k while they are multiplied with v.
 constexpr int STEP_WAVES = 4;
-template <typename T, int DP, int NR = 1>
+template <typename T, int DP>
 struct alignas(1024) StepLds {
   static constexpr int TILE = 32 * HeadLds<T, DP>::PITCH;
-  static constexpr int SUMS = STEP_WAVES * 32 * NR * (DP + 4) * 4;
+  static constexpr int SUMS = STEP_WAVES * 32 * (DP + 4) * 4;
   static constexpr int TILES = STEP_WAVES * 2 * TILE;
   char b[TILES > SUMS ? TILES : SUMS];
-  float m[STEP_WAVES][32 * NR], l[STEP_WAVES][32 * NR];
+  float m[STEP_WAVES][32], l[STEP_WAVES][32];
 };
 
 // 32 rows of k or of v from p on, `left` of them, to a wave's own LDS.
@@ -201,64 +201,52 @@ struct StepRows {
 };
 
 // The two halves of a tile's work; k and v are apart in LDS.
-template <typename T, int DP, int NR>
+template <typename T, int DP>
 __device__ __forceinline__ void step_weigh(const char* __restrict__ kl, char* __restrict__ vl,
                                            const HeadLanes<T, DP>& lanes, const T* v,
                                            const AttnArgs& a, int left,
-                                           const HeadRows<T, DP> (&q)[NR],
-                                           RowSums<T, DP> (&rows)[NR], const StepRows (&sees)[NR],
-                                           f32x16 (&s)[NR][1], int j0, float c) {
+                                           const HeadRows<T, DP>& q, RowSums<T, DP>& rows,
+                                           const StepRows& sees, f32x16 (&s)[1], int j0, float c) {
   step_load<T, DP>(vl, v, a.v_row, a, left);
   step_wait<StepLds<T, DP>::TILE / 1024>();  // k has landed
-#pragma unroll
-  for (int i = 0; i < NR; ++i)
-    if (j0 < sees[i].most)
-      rows[i].template weigh<32>(s[i], lanes, kl, q[i], a.D, j0, sees[i].n, j0 + 32 > sees[i].least,
-                                 c);
+  if (j0 < sees.most)
+    rows.template weigh<32>(s, lanes, kl, q, a.D, j0, sees.n, j0 + 32 > sees.least, c);
 }
-template <typename T, int DP, int NR>
+template <typename T, int DP>
 __device__ __forceinline__ void step_gather(char* __restrict__ kl, const char* __restrict__ vl,
                                             const HeadLanes<T, DP>& lanes, const T* k,
                                             const AttnArgs& a, int left,
-                                            RowSums<T, DP> (&rows)[NR], const StepRows (&sees)[NR],
-                                            const f32x16 (&s)[NR][1], int j0) {
+                                            RowSums<T, DP>& rows, const StepRows& sees,
+                                            const f32x16 (&s)[1], int j0) {
   step_load<T, DP>(kl, k, a.k_row, a, left);
   step_wait<StepLds<T, DP>::TILE / 1024>();  // v has landed
-#pragma unroll
-  for (int i = 0; i < NR; ++i)
-    if (j0 < sees[i].most) rows[i].template gather<32>(s[i], lanes, vl);
+  if (j0 < sees.most) rows.template gather<32>(s, lanes, vl);
 }
 
 // part: with shares, each row's sums (D floats, not divided), and in ml their
 // maximum (in the exponent of 2) and sum
-template <typename T, int DP, int NR>
-__global__ __launch_bounds__(64 * STEP_WAVES, (NR == 1 && DP * sizeof(T) <= 256 ? 2 : 1)) void
-attn_step_kernel(
+template <typename T, int DP>
+__global__ __launch_bounds__(64 * STEP_WAVES, (DP * sizeof(T) <= 256 ? 2 : 1)) void attn_step_kernel(
     AttnArgs a, const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ v,
     T* __restrict__ out, float* __restrict__ lse, T* __restrict__ rest,
     float* __restrict__ part, float2* __restrict__ ml) {
-  constexpr int W = STEP_WAVES, TILE = StepLds<T, DP>::TILE, R = 32 * NR;
-  __shared__ StepLds<T, DP, NR> lds;
+  constexpr int W = STEP_WAVES, TILE = StepLds<T, DP>::TILE;
+  __shared__ StepLds<T, DP> lds;
   const int G = a.Hq / a.Hk, hk = blockIdx.y, shares = gridDim.z;
   int local;
   AttnSpan p;
-  if (!attn_place(a, blockIdx.x, G, R, p, local)) return;
+  if (!attn_place(a, blockIdx.x, G, 32, p, local)) return;
   const int all = p.room_q * G;
-  const int w = wave_id(), l = lane_id(), r0 = local * R;
+  const int w = wave_id(), l = lane_id(), r0 = local * 32;
   const int used = p.Lq * G;
   auto keys = [&](int row) { return used ? attn_keys(a, p, row < used ? row : used - 1, G) : 0; };
-  StepRows sees[NR];
-  HeadRows<T, DP> x[NR];
-  RowSums<T, DP> rows[NR];
-#pragma unroll
-  for (int i = 0; i < NR; ++i) {
-    const int first = r0 + 32 * i, r = first + (l & 31);
-    sees[i] = StepRows{keys(r), keys(first), first < used ? keys(first + 31) : 0};
-    x[i].load(q + (p.q0 + r / G) * a.q_row + (hk * G + r % G) * a.q_head, r < used, a.D);
-    if (a.scale < 0.f) x[i].negate();
-    rows[i].clear();
-  }
-  const int most = r0 < used ? keys(r0 + R - 1) : 0;
+  const int r = r0 + (l & 31), most = r0 < used ? keys(r0 + 31) : 0;
+  const StepRows sees{keys(r), keys(r0), most};
+  HeadRows<T, DP> x;
+  x.load(q + (p.q0 + r / G) * a.q_row + (hk * G + r % G) * a.q_head, r < used, a.D);
+  if (a.scale < 0.f) x.negate();
+  RowSums<T, DP> rows;
+  rows.clear();
   const int tiles = (most + 31) / 32, per = (tiles + shares - 1) / shares;
   const int t0 = per * blockIdx.z, t1 = t0 + per < tiles ? t0 + per : tiles;
   const float c = attn_count(a.scale);
@@ -270,77 +258,71 @@ attn_step_kernel(
     step_load<T, DP>(kl, kt + (int64_t)(t0 + w) * 32 * a.k_row, a.k_row, a, most - (t0 + w) * 32);
   for (int t = t0 + w; t < t1; t += W) {
     const int64_t j0 = (int64_t)t * 32, next = j0 + 32 * W;
-    f32x16 sc[NR][1];
+    f32x16 sc[1];
     step_wait<TILE / 1024>();  // (the reads of v's place have ended)
-    step_weigh<T, DP, NR>(kl, vl, lanes, vt + j0 * a.v_row, a, most - (int)j0, x, rows, sees, sc,
-                          (int)j0, c);
+    step_weigh<T, DP>(kl, vl, lanes, vt + j0 * a.v_row, a, most - (int)j0, x, rows, sees, sc,
+                      (int)j0, c);
     step_wait<TILE / 1024>();  // (and those of k's)
-    step_gather<T, DP, NR>(kl, vl, lanes, kt + next * a.k_row, a,
-                           t + W < t1 ? most - (int)next : 0, rows, sees, sc, (int)j0);
+    step_gather<T, DP>(kl, vl, lanes, kt + next * a.k_row, a, t + W < t1 ? most - (int)next : 0,
+                       rows, sees, sc, (int)j0);
   }
   wait_loads_and_meet<0>();
 
   // the waves' sums together
   constexpr int P = DP + 4;
+  const float sum = rows.l + other_half(rows.l);
+  float* mysums = (float*)lds.b + w * 32 * P;
 #pragma unroll
-  for (int j = 0; j < NR; ++j) {
-    const float sum = rows[j].l + other_half(rows[j].l);
-    float* mysums = (float*)lds.b + (w * R + 32 * j) * P;
+  for (int i = 0; i < DP / 32; ++i)
 #pragma unroll
-    for (int i = 0; i < DP / 32; ++i)
+    for (int b = 0; b < 4; ++b) {
+      Four<float> f;
 #pragma unroll
-      for (int b = 0; b < 4; ++b) {
-        Four<float> f;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) f.v[e] = rows[j].acc[i][4 * b + e];
-        *(Four<float>*)(mysums + (l & 31) * P + 32 * i + 8 * b + 4 * (l >> 5)) = f;
-      }
-    if (l < 32) {
-      lds.m[w][32 * j + l] = rows[j].m;
-      lds.l[w][32 * j + l] = sum;
+      for (int e = 0; e < 4; ++e) f.v[e] = rows.acc[i][4 * b + e];
+      *(Four<float>*)(mysums + (l & 31) * P + 32 * i + 8 * b + 4 * (l >> 5)) = f;
     }
+  if (l < 32) {
+    lds.m[w][l] = rows.m;
+    lds.l[w][l] = sum;
   }
   __syncthreads();
   constexpr int PER_ROW = 2 * W, D1 = DP / PER_ROW;  // lanes a row, values a lane
+  const int rr = threadIdx.x / PER_ROW, d0 = threadIdx.x % PER_ROW * D1, row = r0 + rr;
+  if (row >= all) return;
+  float m = NEG_INF, total = 0.f, f[W];
 #pragma unroll
-  for (int j = 0; j < NR; ++j) {
-    const int rr = 32 * j + threadIdx.x / PER_ROW, d0 = threadIdx.x % PER_ROW * D1, row = r0 + rr;
-    if (row >= all) return;
-    float m = NEG_INF, total = 0.f, f[W];
+  for (int i = 0; i < W; ++i) m = fmaxf(m, lds.m[i][rr]);
 #pragma unroll
-    for (int i = 0; i < W; ++i) m = fmaxf(m, lds.m[i][rr]);
+  for (int i = 0; i < W; ++i) {
+    const float y = lds.l[i][rr];
+    f[i] = y == 0.f ? 0.f : __builtin_amdgcn_exp2f((lds.m[i][rr] - m) * c);
+    total += f[i] * y;
+  }
+  if (row >= used) total = 0.f;
+  const int64_t at = (p.q0 + row / G) * a.Hq + hk * G + row % G;
+  const float inv = shares > 1 ? 1.f : total != 0.f ? 1.f / total : 0.f;
 #pragma unroll
-    for (int i = 0; i < W; ++i) {
-      const float y = lds.l[i][rr];
-      f[i] = y == 0.f ? 0.f : __builtin_amdgcn_exp2f((lds.m[i][rr] - m) * c);
-      total += f[i] * y;
-    }
-    if (row >= used) total = 0.f;
-    const int64_t at = (p.q0 + row / G) * a.Hq + hk * G + row % G;
-    const float inv = shares > 1 ? 1.f : total != 0.f ? 1.f / total : 0.f;
+  for (int d = 0; d < D1; ++d) {
+    float y = 0.f;
 #pragma unroll
-    for (int d = 0; d < D1; ++d) {
-      float y = 0.f;
-#pragma unroll
-      for (int i = 0; i < W; ++i)
-        if (f[i] != 0.f) y += f[i] * ((float*)lds.b)[(i * R + rr) * P + d0 + d];
-      if (d0 + d < a.D) {
-        if (shares > 1) {
-          if (total != 0.f) part[(at * shares + blockIdx.z) * a.D + d0 + d] = y;
-        } else {
-          const T z = total == 0.f ? (T)0.f : (T)(y * inv);
-          out[at * a.D + d0 + d] = z;
-          if (rest) rest[at * a.D + d0 + d] = total == 0.f ? (T)0.f : (T)(y * inv - (float)z);
-        }
+    for (int i = 0; i < W; ++i)
+      if (f[i] != 0.f) y += f[i] * ((float*)lds.b)[(i * 32 + rr) * P + d0 + d];
+    if (d0 + d < a.D) {
+      if (shares > 1) {
+        if (total != 0.f) part[(at * shares + blockIdx.z) * a.D + d0 + d] = y;
+      } else {
+        const T z = total == 0.f ? (T)0.f : (T)(y * inv);
+        out[at * a.D + d0 + d] = z;
+        if (rest) rest[at * a.D + d0 + d] = total == 0.f ? (T)0.f : (T)(y * inv - (float)z);
       }
     }
-    if (d0 == 0) {
-      if (shares > 1)
-        ml[at * shares + blockIdx.z] = make_float2(m * c, total);
-      else if (lse)
-        lse[(at % a.Hq) * a.sq.T + at / a.Hq] =
-            total == 0.f ? NEG_INF : (m * c + __builtin_amdgcn_logf(total)) * LN2;
-    }
+  }
+  if (d0 == 0) {
+    if (shares > 1)
+      ml[at * shares + blockIdx.z] = make_float2(m * c, total);
+    else if (lse)
+      lse[(at % a.Hq) * a.sq.T + at / a.Hq] =
+          total == 0.f ? NEG_INF : (m * c + __builtin_amdgcn_logf(total)) * LN2;
   }
 }
 
@@ -450,37 +432,43 @@ AttnArgs attn_args(const int64_t* oq, const int64_t* ok, const int64_t* lq, cons
 }
 
 
-// Which kernel a call takes, and the shares of the keys.  Up to 64 rows a
-// sequence and key head on average are few: with a workgroup's 128 rows most
-// lanes would idle.  So are fewer rows than 128 for each CU: 32 a workgroup, the
-// keys shared by its waves, fill four times as many (float 5 x 600: 42 us where
-// prompts' tiles take 52).  Shares (by the room for keys: what is in use is not
-// known here): as many as give every place on the CUs a workgroup, with keys enough
-// in each that starting and adding up are worth it (fewer in float, whose products
-// take longer); for long keys four times as many, so that sequences of different
-// lengths even out.
+// Which kernel a call takes, and the shares of the keys.
+// Prompts' workgroups of 128 rows load each key once for all of them; the others'
+// of 32 rows share the keys among their waves, and fill the CUs where there are few
+// rows.  So it goes by the number of workgroups of 128 rows, with each sequence and
+// key head's last one not full: half types, heads of 64 and less (four such
+// workgroups on a CU) from 352 on (384 of 4096 keys, causal: 66 us, by 32 rows 69;
+// 256: 62, 50), longer heads from 144 on (128 of 1024: 25, 22; 144 of 1536: 34, 36;
+// 192 of 3000: 59, 65), float, whose products take longer, from 448 on (350 of 1000
+// keys: 80, 69; 512 of 4096, heads of 128: 735, 911).  Where there are at most 32 rows
+// to a sequence, three of four waves only help to load: that pays for 512 and more of
+// them with keys few enough to be no more than a wave's share (64 x 8 heads, 512
+// keys: 21, 24; 256 x 8, 2048 keys: 256, 237), not in float.
+// Shares (by the room for keys: what is in use is not known here): for 128
+// workgroups in all where that leaves a share 256 keys (64 in float); starting and
+// adding up cost more than the other CUs would give (16384 keys, 8 workgroups: 16
+// shares 21.5 us, 32 23.9, 64 26.2).  For long keys up to 1024 workgroups, so that
+// sequences of different lengths even out (64 x 16384 keys: one share each 162 us, 4
+// 99, 16 76).
 struct Way {
-  int rows;  // a workgroup's: 32 or 64 (few rows), 128 (prompts)
+  int rows;  // a workgroup's: 32 (few rows) or 128 (prompts)
   int shares;
 };
 Way attn_way(int dtype, int64_t B, int64_t Tq, int64_t Tk, int64_t Hq, int64_t Hk, int64_t D) {
-  Way w{128, 1};
   const int64_t G = Hq / Hk, n = B < 1 ? 1 : B, keys = Tk / n;
   const int64_t each = Tq < 1 ? 1 : (Tq * G + n - 1) / n;
-  if (each > 64 && Tq * Hq >= 128 * 256) return w;
-  // 33 to 64 rows: both halves at once, k and v read once for them (long float heads
-  // leave no registers for that)
-  w.rows = each > 32 && each <= 64 && !(dtype == TPO_F32 && D > 96) ? 64 : 32;
-  const int64_t blocks = (each + w.rows - 1) / w.rows * n * Hk;
-  const int64_t resident = w.rows == 32 && D * element_bytes(dtype) <= 256 ? 2 : 1;  // on a CU
-  const int64_t least = dtype == TPO_F32 ? 64 : 256;
-  int64_t s = (256 * resident + blocks - 1) / blocks, t = 1024 / blocks;
+  const bool single = dtype == TPO_F32;
+  const int64_t prompts = (each + 127) / 128 * n * Hk, blocks = (each + 31) / 32 * n * Hk;
+  if (each > 32 ? prompts >= (single ? 448 : D > 64 ? 144 : 352)
+                : prompts >= 512 && keys <= 1024 && !single)
+    return Way{128, 1};
+  const int64_t least = single ? 64 : 256, more = single ? 512 : 1024;
+  int64_t s = (128 + blocks - 1) / blocks, t = 1024 / blocks;
   if (s > keys / least) s = keys / least;
-  if (t > keys / 1024) t = keys / 1024;
+  if (t > keys / more) t = keys / more;
   if (s < t) s = t;
-  if (keys < 4 * least) s = 1;
-  w.shares = s < 1 ? 1 : s > 64 ? 64 : (int)s;
-  return w;
+  if (keys < 4 * least || s < 1) s = 1;
+  return Way{32, s > 64 ? 64 : (int)s};
 }
 
 }  // namespace tpo
@@ -526,18 +514,13 @@ extern "C" int tpo_attention_fwd(int dtype, const void* q, const void* k, const 
     typedef decltype(t) T;
     with_head(D, [&](auto dp) {
       constexpr int DP = decltype(dp)::value;
-      auto step = [&](auto nr) {
-        attn_step_kernel<T, DP, decltype(nr)::value>
-            <<<dim3((unsigned)places, (unsigned)Hk, w.shares), 64 * STEP_WAVES, 0, s>>>(
-                a, (const T*)q, (const T*)k, (const T*)v, (T*)out, lse, (T*)rest, part, ml);
-      };
       if (w.rows == 128)
         attn_prompt_kernel<T, DP><<<dim3((unsigned)(places * Hk)), 256, 0, s>>>(
             a, (const T*)q, (const T*)k, (const T*)v, (T*)out, lse, (T*)rest);
-      else if (w.rows == 32)
-        step(std::integral_constant<int, 1>());
-      else if constexpr (DP * sizeof(T) < 512)
-        step(std::integral_constant<int, 2>());
+      else
+        attn_step_kernel<T, DP>
+            <<<dim3((unsigned)places, (unsigned)Hk, w.shares), 64 * STEP_WAVES, 0, s>>>(
+                a, (const T*)q, (const T*)k, (const T*)v, (T*)out, lse, (T*)rest, part, ml);
     });
     if (w.shares > 1)
       attn_join_kernel<T><<<dim3((unsigned)(Tq * Hq)), 256, 0, s>>>(
