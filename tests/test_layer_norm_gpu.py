@@ -51,6 +51,22 @@ def test_values_and_gradients(tpo, dev, shape, dtype, weights):
         nn64.near(a, e, floats=2e-6 + 1e-7 * x.numel() ** 0.5 / max(1.0, e.norm().item()))
 
 
+# rows that several waves hold, the last of them in part, and more rows than workgroups
+@pytest.mark.parametrize("shape", [(600, 1030), (700, 1500), (300, 2048), (600, 2049), (300, 2500),
+                                   (600, 4097), (600, 5000), (300, 9000), (300, 16384), (70, 16390),
+                                   (70, 32769)])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_wide_rows(tpo, dev, shape, dtype):
+    x, w, b, gy = _inputs(shape, dtype, "same", sum(shape))
+    want, gwant = nn64.grads(lambda x, w, b: nn64.layer_norm(x, w, b, 1e-5), (x, w, b), gy)
+    X, W, B = _on(dev, x, w, b)
+    y = tpo.layer_norm(X, W, B)
+    nn64.near(y, want)
+    for a, e in zip(torch.autograd.grad(y, (X, W, B), gy.to(dev)), gwant):
+        # sums over the rows of terms of either sign
+        nn64.near(a, e, floats=2e-6 + 1e-7 * x.numel() ** 0.5 / max(1.0, e.norm().item()))
+
+
 def test_each_gradient_alone(tpo, dev):
     x, w, b, gy = _inputs((37, 200), torch.bfloat16, "same", 5)
     X, W, B = _on(dev, x, w, b)

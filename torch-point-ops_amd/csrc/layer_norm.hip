@@ -12,7 +12,7 @@ __device__ __forceinline__ float ln_at(const W* w, int64_t c, float none) {
   return w ? (float)w[c] : none;
 }
 
-// A row held in registers by a team of 64 or 256 lanes: N loads a lane of PER
+// A row held in registers by a team of 64 to 1024 lanes: N loads a lane of PER
 // values (16 bytes) each.  Rows of other widths begin anywhere: the memory takes
 // 16-byte accesses at any element (at 32768 x 1023 in bfloat16 one value a load
 // took 188 us where this takes 77), and only a row's last piece goes value by
@@ -25,18 +25,37 @@ struct __attribute__((packed, aligned(sizeof(T)))) Piece {
   T v[PER];
 };
 
+// Sums over a team, two at a time.  The waves' sums go to one of two places in
+// turn, so that a place is written again only after a barrier that follows its
+// reads.
 template <int TEAM>
-__device__ __forceinline__ float team_sum(float v, float (&s)[4]) {
-  v = wave_sum(v);
-  if constexpr (TEAM == 64) {
-    return v;
-  } else {
-    __syncthreads();  // the last sum has been read
-    if (lane_id() == 0) s[wave_id()] = v;
+struct TeamSums {
+  float2 s[2][TEAM / 64];
+};
+template <int TEAM>
+__device__ __forceinline__ void team_sum(float& a, float& b, TeamSums<TEAM>& lds, int& turn) {
+  a = wave_sum(a);
+  b = wave_sum(b);
+  if constexpr (TEAM > 64) {
+    float2* s = lds.s[turn];
+    turn ^= 1;
+    if (lane_id() == 0) s[wave_id()] = make_float2(a, b);
     __syncthreads();
-    return (s[0] + s[1]) + (s[2] + s[3]);
+    a = b = 0.f;
+#pragma unroll
+    for (int i = 0; i < TEAM / 64; ++i) {
+      a += s[i].x;
+      b += s[i].y;
+    }
   }
 }
+template <int TEAM>
+__device__ __forceinline__ float team_sum(float a, TeamSums<TEAM>& lds, int& turn) {
+  float none = 0.f;
+  team_sum<TEAM>(a, none, lds, turn);
+  return a;
+}
+constexpr int ln_threads(int team) { return team == 64 ? 256 : team; }
 
 template <typename T, int PER, int N, int TEAM>
 struct RowHeld {
@@ -84,16 +103,17 @@ struct RowHeld {
 };
 
 template <typename T, typename W, int PER, int N, int TEAM>
-__global__ __launch_bounds__(256) void layer_norm_fwd_kernel(
+__global__ __launch_bounds__(ln_threads(TEAM)) void layer_norm_fwd_kernel(
     const T* __restrict__ x, const W* __restrict__ w, const W* __restrict__ b, int64_t rows,
     int64_t width, float eps, T* __restrict__ y, float* __restrict__ mean,
     float* __restrict__ rstd) {
-  __shared__ float s[4];
-  constexpr int TEAMS = 256 / TEAM;
+  __shared__ TeamSums<TEAM> s;
+  int turn = 0;
+  constexpr int TEAMS = ln_threads(TEAM) / TEAM;
   RowHeld<W, PER, N, TEAM> ws, bs;
   RowHeld<T, PER, N, TEAM> xs;
   int64_t r = (int64_t)blockIdx.x * TEAMS + threadIdx.x / TEAM;
-  if (r >= rows) return;  // (with teams of 256 the whole workgroup)
+  if (r >= rows) return;  // (with teams of several waves the whole workgroup)
   xs.load(x + r * width, width);
   if (w) ws.load(w, width); else ws.fill(1.f);
   if (b) bs.load(b, width); else bs.fill(0.f);
@@ -104,7 +124,7 @@ __global__ __launch_bounds__(256) void layer_norm_fwd_kernel(
     for (int i = 0; i < N; ++i)
 #pragma unroll
       for (int e = 0; e < PER; ++e) t += xs.v[i][e];
-    const float m = team_sum<TEAM>(t, s) * per;
+    const float m = team_sum<TEAM>(t, s, turn) * per;
     t = 0.f;
 #pragma unroll
     for (int i = 0; i < N; ++i)
@@ -113,7 +133,7 @@ __global__ __launch_bounds__(256) void layer_norm_fwd_kernel(
         const float d = xs.v[i][e] - m;
         if (xs.column(i) + e < width) t = __builtin_fmaf(d, d, t);
       }
-    const float q = 1.f / sqrtf(team_sum<TEAM>(t, s) * per + eps);
+    const float q = 1.f / sqrtf(team_sum<TEAM>(t, s, turn) * per + eps);
     RowHeld<T, PER, N, TEAM> ys;
 #pragma unroll
     for (int i = 0; i < N; ++i)
@@ -136,13 +156,14 @@ __global__ __launch_bounds__(256) void layer_norm_fwd_kernel(
 // need, a workgroup's in part[blockIdx.x] (weight, then bias).  gy and x are read
 // once for all three results.
 template <typename T, typename W, int PER, int N, int TEAM>
-__global__ __launch_bounds__(256) void layer_norm_bwd_kernel(
+__global__ __launch_bounds__(ln_threads(TEAM)) void layer_norm_bwd_kernel(
     const T* __restrict__ gy, const T* __restrict__ x, const W* __restrict__ w,
     const float* __restrict__ mean, const float* __restrict__ rstd, int64_t rows, int64_t width,
     T* __restrict__ gx, float* __restrict__ part) {
-  __shared__ float s[4];
+  __shared__ TeamSums<TEAM> s;
+  int turn = 0;
   __shared__ float sums[TEAM == 64 ? 2 * N * PER * 64 : 1];
-  constexpr int TEAMS = 256 / TEAM;
+  constexpr int TEAMS = ln_threads(TEAM) / TEAM;
   typedef RowHeld<T, PER, N, TEAM> Row;
   RowHeld<W, PER, N, TEAM> ws;
   if (w) ws.load(w, width, 1.f); else ws.fill(1.f);
@@ -169,8 +190,9 @@ __global__ __launch_bounds__(256) void layer_norm_bwd_kernel(
         s2 = __builtin_fmaf(g, h, s2);
       }
     if (gx) {
-      s1 = team_sum<TEAM>(s1, s) * per;
-      s2 = team_sum<TEAM>(s2, s) * per;
+      team_sum<TEAM>(s1, s2, s, turn);
+      s1 *= per;
+      s2 *= per;
 #pragma unroll
       for (int i = 0; i < N; ++i)
 #pragma unroll
@@ -347,19 +369,25 @@ __global__ __launch_bounds__(1024) void layer_norm_bwd_sum_kernel(const float* _
 }
 
 // The kernels' build for a row: loads a lane, lanes a row; held false for rows
-// longer than 256 lanes hold.
+// longer than 1024 lanes hold.  A wave a row as long as the backward, which holds
+// five arrays, leaves room for other waves; then more waves a row rather than
+// more loads a lane (half types, training: 16000 x 2048 98 us with a wave a row, 74
+// with four; 4000 x 8192 135 with four, 79 with sixteen), in float with two loads, so
+// as many values, a lane (8000 x 3000: 99, with one 109).
 struct LnForm {
   int n, team;
   bool held;
 };
 LnForm ln_form(int64_t width, int64_t size) {
   const int64_t loads = (width * size + 15) / 16;
+  const bool single = size == 4;
   if (loads <= 64) return {1, 64, true};
   if (loads <= 128) return {2, 64, true};
-  if (loads <= 256) return {4, 64, true};
-  if (loads <= 512) return {2, 256, true};
-  if (loads <= 1024) return {4, 256, true};
-  if (loads <= 2048 && size == 4) return {8, 256, true};  // (16384 half values spill)
+  if (loads <= 256) return single ? LnForm{4, 64, true} : LnForm{1, 256, true};
+  if (loads <= 512) return single ? LnForm{2, 256, true} : LnForm{1, 512, true};
+  if (loads <= 1024) return single ? LnForm{2, 512, true} : LnForm{1, 1024, true};
+  if (loads <= 2048) return {2, 1024, true};
+  if (loads <= 4096 && single) return {4, 1024, true};  // (32768 half values spill)
   return {0, 0, false};
 }
 // Calls f with the form as types: values a load, loads, team.
@@ -372,10 +400,17 @@ void with_form(const LnForm& f, F&& call) {
               std::integral_constant<int, TEAM>())
   LN_FORM(1, 64);
   LN_FORM(2, 64);
-  LN_FORM(4, 64);
-  LN_FORM(2, 256);
-  LN_FORM(4, 256);
-  if constexpr (sizeof(T) == 4) LN_FORM(8, 256);
+  LN_FORM(2, 1024);
+  if constexpr (sizeof(T) == 4) {
+    LN_FORM(4, 64);
+    LN_FORM(2, 256);
+    LN_FORM(2, 512);
+    LN_FORM(4, 1024);
+  } else {
+    LN_FORM(1, 256);
+    LN_FORM(1, 512);
+    LN_FORM(1, 1024);
+  }
 #undef LN_FORM
 }
 
@@ -440,11 +475,12 @@ extern "C" int tpo_layer_norm_fwd(int dtype, int wdtype, const void* x, const vo
       return;
     }
     with_form<T>(f, [&](auto per, auto n, auto team) {
-      constexpr int TEAMS = 256 / decltype(team)::value;
+      constexpr int TEAM = decltype(team)::value, THREADS = ln_threads(TEAM);
+      constexpr int TEAMS = THREADS / TEAM;
       int64_t blocks = (rows + TEAMS - 1) / TEAMS;
       if (blocks > 2048) blocks = 2048;  // eight workgroups a CU
-      layer_norm_fwd_kernel<T, W, decltype(per)::value, decltype(n)::value, decltype(team)::value>
-          <<<dim3((unsigned)blocks), 256, 0, s>>>((const T*)x, (const W*)weight, (const W*)bias,
+      layer_norm_fwd_kernel<T, W, decltype(per)::value, decltype(n)::value, TEAM>
+          <<<dim3((unsigned)blocks), THREADS, 0, s>>>((const T*)x, (const W*)weight, (const W*)bias,
                                                   rows, width, (float)eps, (T*)y, mean, rstd);
     });
   });
@@ -459,8 +495,8 @@ extern "C" int64_t tpo_layer_norm_bwd_workspace_size(int64_t rows, int64_t width
 extern "C" int tpo_layer_norm_bwd(int dtype, int wdtype, const void* grad_y, const void* x,
                                   const void* weight, const float* mean, const float* rstd,
                                   int64_t rows, int64_t width, double eps, void* grad_x,
-                                  void* grad_weight, void* grad_bias, void* workspace, int64_t workspace_bytes,
-                                  void* stream) {
+                                  void* grad_weight, void* grad_bias, void* workspace,
+                                  int64_t workspace_bytes, void* stream) {
   if (int rc = ln_check("layer_norm_bwd", rows, width)) return rc;
   const bool sums = grad_weight || grad_bias;
   if (sums && (workspace_bytes < tpo_layer_norm_bwd_workspace_size(rows, width) ||
@@ -476,9 +512,11 @@ extern "C" int tpo_layer_norm_bwd(int dtype, int wdtype, const void* grad_y, con
     float* part = sums ? (float*)workspace : nullptr;
     if (rows > 0 && width > LN_NARROW && f.held) {
       with_form<T>(f, [&](auto per, auto n, auto team) {
-        layer_norm_bwd_kernel<T, W, decltype(per)::value, decltype(n)::value, decltype(team)::value>
-            <<<dim3((unsigned)parts), 256, 0, s>>>((const T*)grad_y, (const T*)x, (const W*)weight,
-                                                   mean, rstd, rows, width, (T*)grad_x, part);
+        constexpr int TEAM = decltype(team)::value;
+        layer_norm_bwd_kernel<T, W, decltype(per)::value, decltype(n)::value, TEAM>
+            <<<dim3((unsigned)parts), ln_threads(TEAM), 0, s>>>(
+                (const T*)grad_y, (const T*)x, (const W*)weight, mean, rstd, rows, width, (T*)grad_x,
+                part);
       });
     } else if (rows > 0) {
       if (grad_x && width <= LN_NARROW)
