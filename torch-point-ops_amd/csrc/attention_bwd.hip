@@ -372,8 +372,7 @@ __global__ __launch_bounds__(256, (DP * sizeof(T) <= 192 ? 2 : 1)) void attn_bwd
       for (int e = 0; e < 4; ++e) z.v[e] = in ? (T)(own[i][4 * b + e] * f) : (T)0.f;
       *(Four<T>*)to.four(32 * i + 8 * b + 4 * (l >> 5)) = z;
     }
-  to.store((w < 2 ? gk : gv) + hk * a.D, (int64_t)a.Hk * a.D, p.k0 + j0, p.k0 + p.room_k, 0, a.D,
-           true);
+  to.store((w < 2 ? gk : gv) + hk * a.D, (int64_t)a.Hk * a.D, p.k0 + j0, p.k0 + p.room_k, 0, a.D);
 }
 
 // The shares of the group's heads added up: n values of dK, then n of dV.

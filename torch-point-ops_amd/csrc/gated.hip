@@ -96,7 +96,7 @@ __device__ __forceinline__ void tile_of(int tiles_m, int tiles_n, int& m, int& n
 template <typename T, int BM, int BN, bool BWD>
 __global__ __launch_bounds__(256, 2) void gated_pair_kernel(
     Matrix x, Matrix wg, Matrix wu, int act, const T* __restrict__ gh, int64_t F,
-    T* __restrict__ out, T* __restrict__ keep, int64_t Fp, int whole) {
+    T* __restrict__ out, T* __restrict__ keep, int64_t Fp) {
   __shared__ GatedLds<BM, BN> lds;
   constexpr int SLAB = GatedLds<BM, BN>::SLAB;
   typedef RowLoader<T, BM, SLAB> LA;
@@ -118,7 +118,7 @@ __global__ __launch_bounds__(256, 2) void gated_pair_kernel(
 #pragma unroll
   for (int j = 0; j < BN / 64; ++j) {
     const int64_t t = t0 + (w & 1) * (BN / 2) + 32 * j;
-    if (BWD) rg.load(gh, F, t, M, f0, F, whole);
+    if (BWD) rg.load(gh, F, t, M, f0, F);
     with_act(act, [&](auto name) {
 #pragma unroll
       for (int i = 0; i < TF; ++i)
@@ -146,7 +146,7 @@ __global__ __launch_bounds__(256, 2) void gated_pair_kernel(
         }
     });
     if (!BWD && sizeof(T) == 4 && keep) {
-      rg.store(out, F, t, M, f0, F, whole);
+      rg.store(out, F, t, M, f0, F);
       for (int y = 0; y < 2; ++y) {
 #pragma unroll
         for (int i = 0; i < TF; ++i)
@@ -158,13 +158,13 @@ __global__ __launch_bounds__(256, 2) void gated_pair_kernel(
               p.v[e] = (T)(y ? acc[i + TF][j][4 * b + e] : acc[i][j][4 * b + e]);
             *(Four<T>*)rg.four(32 * i + 8 * b + 4 * h) = p;
           }
-        rg.store(keep + y * F, 2 * F, t, M, f0, F, whole);
+        rg.store(keep + y * F, 2 * F, t, M, f0, F);
       }
     } else if (BWD) {
-      rg.store(out, 2 * Fp, t, M, f0, Fp, true);
-      ru.store(out + Fp, 2 * Fp, t, M, f0, Fp, true);
+      rg.store(out, 2 * Fp, t, M, f0, Fp);
+      ru.store(out + Fp, 2 * Fp, t, M, f0, Fp);
     } else {
-      rg.store(out, F, t, M, f0, F, whole);
+      rg.store(out, F, t, M, f0, F);
     }
   }
 }
@@ -326,7 +326,7 @@ __global__ __launch_bounds__(256) void gated_kept_kernel(const float* __restrict
 template <typename T, int BM, int BN, typename Lds>
 __device__ __forceinline__ void gated_put(Lds& lds, const f32x16 (&acc)[BM / 64][BN / 64],
                                           int64_t n0, int64_t m0, int64_t N, int64_t M,
-                                          T* __restrict__ out, float* __restrict__ part, int whole) {
+                                          T* __restrict__ out, float* __restrict__ part) {
   const int w = wave_id(), h = lane_id() >> 5;
   n0 += (w >> 1) * (BM / 2);
   m0 += (w & 1) * (BN / 2);
@@ -345,7 +345,7 @@ __device__ __forceinline__ void gated_put(Lds& lds, const f32x16 (&acc)[BM / 64]
           for (int e = 0; e < 4; ++e) p.v[e] = (V)acc[i][j][4 * b + e];
           *(Four<V>*)r.four(32 * i + 8 * b + 4 * h) = p;
         }
-      r.store(to, N, m0 + 32 * j, M, n0, N, whole);
+      r.store(to, N, m0 + 32 * j, M, n0, N);
     }
   };
   if (part)
@@ -358,7 +358,7 @@ __device__ __forceinline__ void gated_put(Lds& lds, const f32x16 (&acc)[BM / 64]
 template <typename T, int BM, int BN>
 __global__ __launch_bounds__(256, 2) void gated_dx_kernel(
     Matrix d, Matrix wg, const char* wu, int units, int share, int64_t K, T* __restrict__ out,
-    float* __restrict__ part, int whole) {
+    float* __restrict__ part) {
   __shared__ GatedLds<BM, BN> lds;
   constexpr int SLAB = GatedLds<BM, BN>::SLAB;
   const int64_t M = d.rows;
@@ -371,7 +371,7 @@ __global__ __launch_bounds__(256, 2) void gated_dx_kernel(
   f32x16 acc[BM / 64][BN / 64];
   gemm_tile<T, BM, BN>(lds, la, lb, u0 * (UNIT / SLAB), u1 * (UNIT / SLAB), acc);
   if (part) part += blockIdx.y * M * K;
-  gated_put<T, BM, BN>(lds, acc, n0, m0, K, M, out, part, whole);
+  gated_put<T, BM, BN>(lds, acc, n0, m0, K, M, out, part);
 }
 
 // dWg = dg^T x and dWu = du^T x (blockIdx.z), F rows of K values; blockIdx.y: a
@@ -379,7 +379,7 @@ __global__ __launch_bounds__(256, 2) void gated_dx_kernel(
 template <typename T, int BM, int BN>
 __global__ __launch_bounds__(256, 2) void gated_dw_kernel(
     Matrix x, Matrix d, int64_t F, int units, int share, int64_t K, T* __restrict__ dwg,
-    T* __restrict__ dwu, float* __restrict__ part, int whole) {
+    T* __restrict__ dwu, float* __restrict__ part) {
   __shared__ GatedLds<BM, BN> lds;
   constexpr int SLAB = GatedLds<BM, BN>::SLAB;
   int tm, tn;
@@ -392,7 +392,7 @@ __global__ __launch_bounds__(256, 2) void gated_dw_kernel(
   f32x16 acc[BM / 64][BN / 64];
   gemm_tile<T, BM, BN>(lds, la, lb, u0 * (UNIT / SLAB), u1 * (UNIT / SLAB), acc);
   if (part) part += ((int64_t)blockIdx.y * 2 + blockIdx.z) * F * K;
-  gated_put<T, BM, BN>(lds, acc, n0, m0, K, F, blockIdx.z ? dwu : dwg, part, whole);
+  gated_put<T, BM, BN>(lds, acc, n0, m0, K, F, blockIdx.z ? dwu : dwg, part);
 }
 
 // out, out2 (n values each): the shares of a split product added in order
@@ -417,14 +417,22 @@ struct Copies {
   int64_t rows[3];
 };
 template <typename T>
-__global__ __launch_bounds__(256) void gated_pad_kernel(Copies m, int64_t C, int64_t pitch) {
-  const int y = blockIdx.y;
+__global__ __launch_bounds__(256) void gated_pad_kernel(Copies m, int C, int pitch) {
+  constexpr int PER = 16 / sizeof(T);
+  const int y = blockIdx.z;
   const T* in = (const T*)m.in[y];
   T* out = (T*)m.out[y];
-  const int64_t n = m.rows[y] * pitch;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
-    const int64_t r = i / pitch, c = i - r * pitch;
-    out[i] = c < C ? in[r * C + c] : (T)0.f;
+  const int c = (blockIdx.x * 64 + threadIdx.x % 64) * PER;
+  if (c >= pitch) return;
+  for (int64_t r = blockIdx.y * 4 + threadIdx.x / 64; r < m.rows[y]; r += gridDim.y * 4) {
+    Piece<T, PER> v = {};
+    if (c + PER <= C)
+      v = *(const Piece<T, PER>*)(in + r * C + c);
+    else
+#pragma unroll
+      for (int e = 0; e < PER; ++e)
+        if (c + e < C) v.v[e] = in[r * C + c + e];
+    *(f32x4*)(out + r * pitch + c) = __builtin_bit_cast(f32x4, v);
   }
 }
 
@@ -544,25 +552,22 @@ void gated_inputs(const Plan& p, const void* x, const void* wg, const void* wu, 
     c.rows[i] = rows[i];
     r[i] = Matrix{p.Kp != K ? ws + at[i] : (const char*)in[i], pitch, rows[i], pitch};
   }
-  if (p.Kp != K)
-    gated_pad_kernel<T><<<dim3(gated_blocks((M > F ? M : F) * p.Kp), 3), 256, 0, s>>>(c, K, p.Kp);
-}
-
-// Whether rows of n values starting at p can be written 16 bytes at a time.
-template <typename T>
-int whole_rows(const void* p, int64_t n) {
-  return ((uintptr_t)p & 15) == 0 && n * sizeof(T) % 16 == 0;
+  if (p.Kp != K) {
+    const int64_t rows4 = cdiv(M > F ? M : F, 4);
+    gated_pad_kernel<T><<<dim3((unsigned)cdiv(p.Kp * sizeof(T), 1024),
+                               (unsigned)(rows4 < 2048 ? rows4 : 2048), 3),
+                          256, 0, s>>>(c, (int)K, (int)p.Kp);
+  }
 }
 
 template <typename T, bool BWD>
 void gated_pair(const Matrix (&r)[3], int act, const T* gh, int64_t F, T* out, T* keep, int64_t Fp,
                 hipStream_t s) {
   const int64_t M = r[0].rows;
-  const int whole = whole_rows<T>(BWD ? (const void*)gh : (const void*)out, F) && ((uintptr_t)keep & 15) == 0;
   auto run = [&](auto bm, auto bn) {
     constexpr int BM = decltype(bm)::value, BN = decltype(bn)::value;
     gated_pair_kernel<T, BM, BN, BWD><<<dim3((unsigned)(cdiv(M, BN) * cdiv(F, BM / 2))), 256, 0, s>>>(
-        r[0], r[1], r[2], act, gh, F, out, keep, Fp, whole);
+        r[0], r[1], r[2], act, gh, F, out, keep, Fp);
   };
   if (M <= 64) {  // (16 x 2048 x 8192: 12.8 where the smallest tile takes 22.6)
     const dim3 grid((unsigned)cdiv(BWD ? Fp : F, 32));
@@ -587,9 +592,8 @@ void gated_dx(const Plan& p, const Matrix& d, const Matrix& wg, const Matrix& wu
               float* part, hipStream_t s) {
   const int64_t M = d.rows;
   const int share = (int)cdiv(2 * p.funits, p.dx.shares), shares = p.dx.shares;
-  const int whole = shares > 1 ? K % 4 == 0 : whole_rows<T>(out, K);
   gated_dx_kernel<T, BM, BN><<<dim3((unsigned)(cdiv(M, BN) * cdiv(K, BM)), shares), 256, 0, s>>>(
-      d, wg, wu.p, (int)p.funits, share, K, out, shares > 1 ? part : nullptr, whole);
+      d, wg, wu.p, (int)p.funits, share, K, out, shares > 1 ? part : nullptr);
   if (shares > 1)
     gated_join_kernel<T><<<dim3(gated_blocks(M * K)), 256, 0, s>>>(part, shares, M * K, out, out);
 }
@@ -598,9 +602,8 @@ template <typename T, int BM, int BN>
 void gated_dw(const Plan& p, const Matrix& x, const Matrix& d, int64_t F, int64_t K, T* dwg, T* dwu,
               float* part, hipStream_t s) {
   const int share = (int)cdiv(p.munits, p.dw.shares), shares = p.dw.shares;
-  const int whole = shares > 1 ? K % 4 == 0 : whole_rows<T>(dwg, K) && whole_rows<T>(dwu, K);
   gated_dw_kernel<T, BM, BN><<<dim3((unsigned)(cdiv(F, BN) * cdiv(K, BM)), shares, 2), 256, 0, s>>>(
-      x, d, F, (int)p.munits, share, K, dwg, dwu, shares > 1 ? part : nullptr, whole);
+      x, d, F, (int)p.munits, share, K, dwg, dwu, shares > 1 ? part : nullptr);
   if (shares > 1)
     gated_join_kernel<T><<<dim3(gated_blocks(F * K), 2), 256, 0, s>>>(part, shares, F * K, dwg, dwu);
 }

@@ -12,19 +12,6 @@ __device__ __forceinline__ float ln_at(const W* w, int64_t c, float none) {
   return w ? (float)w[c] : none;
 }
 
-// A row held in registers by a team of 64 to 1024 lanes: N loads a lane of PER
-// values (16 bytes) each.  Rows of other widths begin anywhere: the memory takes
-// 16-byte accesses at any element (at 32768 x 1023 in bfloat16 one value a load
-// took 188 us where this takes 77), and only a row's last piece goes value by
-// value.  x is read once; the variance is taken about the mean, from the
-// registers.  HBM-bound: what is read and written is all that counts, so teams go
-// on to other rows with the weights in registers, and there are enough of them to
-// keep the memory busy.
-template <typename T, int PER>
-struct __attribute__((packed, aligned(sizeof(T)))) Piece {
-  T v[PER];
-};
-
 // Sums over a team, two at a time.  The waves' sums go to one of two places in
 // turn, so that a place is written again only after a barrier that follows its
 // reads.
@@ -57,6 +44,14 @@ __device__ __forceinline__ float team_sum(float a, TeamSums<TEAM>& lds, int& tur
 }
 constexpr int ln_threads(int team) { return team == 64 ? 256 : team; }
 
+// A row held in registers by a team of 64 to 1024 lanes: N loads a lane of PER
+// values (16 bytes) each.  Rows of other widths begin anywhere: the memory takes
+// 16-byte accesses at any element (at 32768 x 1023 in bfloat16 one value a load
+// took 188 us where this takes 77), and only a row's last piece goes value by
+// value.  x is read once; the variance is taken about the mean, from the
+// registers.  HBM-bound: what is read and written is all that counts, so teams go
+// on to other rows with the weights in registers, and there are enough of them to
+// keep the memory busy.
 template <typename T, int PER, int N, int TEAM>
 struct RowHeld {
   float v[N][PER];

@@ -23,6 +23,13 @@ __device__ __forceinline__ float wave_max(float v) {
   return v;
 }
 
+// Values that are loaded and stored at once and begin at any element: the memory
+// takes 16-byte accesses there too.
+template <typename T, int PER>
+struct __attribute__((packed, aligned(sizeof(T)))) Piece {
+  T v[PER];
+};
+
 // Calls f with a value of the element type of `dtype`; false for another code.
 template <typename F>
 inline bool with_element(int dtype, F&& f) {
