@@ -54,6 +54,13 @@ def test_large_tiles(tpo, dev, M, K, F, dtype):
     _check(tpo, dev, M, K, F, dtype, "gelu", seed=M + K + F)
 
 
+# more workgroups of few tokens than CUs, but few tiles: the smallest ones
+@pytest.mark.parametrize("M,K,F", [(600, 72, 1100), (900, 131, 701), (1025, 520, 640)])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_small_tiles(tpo, dev, M, K, F, dtype):
+    _check(tpo, dev, M, K, F, dtype, "relu", seed=M + K + F)
+
+
 @pytest.mark.parametrize("name", ACTS)
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_activations(tpo, dev, name, dtype):

@@ -169,8 +169,8 @@ __global__ __launch_bounds__(256, 2) void gated_pair_kernel(
   }
 }
 
-// Few tokens (up to 32 TN): the weights' way from memory is all that counts.  A
-// workgroup takes 32 features and all tokens; its four waves take every fourth slab
+// Few tokens, where the weights' way from memory is all that counts, and few tiles: a
+// workgroup takes 32 features and 32 TN tokens; its four waves take every fourth slab
 // of the summed axis each, through LDS of their own and without waiting for each
 // other, and add up their sums at the end.  Results as gated_pair_kernel's.
 template <typename T, int TN>
@@ -187,8 +187,8 @@ struct FewLoader {
   static constexpr int LOADS = (2 + TN) * L::N;
   L g, u, x0, x1;  // (x1: the second 32 tokens)
   __device__ __forceinline__ FewLoader(const Matrix& wg, const Matrix& wu, const Matrix& xs,
-                                       int64_t f0)
-      : g(wg, f0), u(wu, f0), x0(xs, 0), x1(xs, 32) {}
+                                       int64_t f0, int64_t m0)
+      : g(wg, f0), u(wu, f0), x0(xs, m0), x1(xs, m0 + 32) {}
   __device__ __forceinline__ void load(char* lds, int slab) const {
     lds -= wave_id() * L::N * 1024;  // (where the loader puts wave 0's rows)
     const auto sg = g.slab(slab), su = u.slab(slab);
@@ -232,8 +232,8 @@ __global__ __launch_bounds__(256) void gated_few_kernel(Matrix x, Matrix wg, Mat
   typedef FewLds<T, TN> Lds;
   __shared__ Lds lds;
   const int w = wave_id(), l = lane_id();
-  const int64_t f0 = (int64_t)blockIdx.x * 32;
-  const FewLoader<T, TN> load(wg, wu, x, f0);
+  const int64_t f0 = (int64_t)blockIdx.x * 32, m0 = (int64_t)blockIdx.y * 32 * TN;
+  const FewLoader<T, TN> load(wg, wu, x, f0, m0);
   const int slabs = (int)((x.bytes + 127) / 128);
   f32x16 acc[2][TN];
 #pragma unroll
@@ -277,7 +277,7 @@ __global__ __launch_bounds__(256) void gated_few_kernel(Matrix x, Matrix wg, Mat
         u[e] += z[e];
       }
     }
-    const int64_t m = 32 * i + (l & 31), f = f0 + 8 * w + 4 * (l >> 5);
+    const int64_t m = m0 + 32 * i + (l & 31), f = f0 + 8 * w + 4 * (l >> 5);
     if (m >= x.rows) continue;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
@@ -569,14 +569,20 @@ void gated_pair(const Matrix (&r)[3], int act, const T* gh, int64_t F, T* out, T
     gated_pair_kernel<T, BM, BN, BWD><<<dim3((unsigned)(cdiv(M, BN) * cdiv(F, BM / 2))), 256, 0, s>>>(
         r[0], r[1], r[2], act, gh, F, out, keep, Fp);
   };
-  if (M <= 64) {  // (16 x 2048 x 8192: 12.8 where the smallest tile takes 22.6)
-    const dim3 grid((unsigned)cdiv(BWD ? Fp : F, 32));
-    if (M <= 32)
-      gated_few_kernel<T, 1, BWD><<<grid, 256, 0, s>>>(r[0], r[1], r[2], act, gh, F, out, keep, Fp);
-    else
-      gated_few_kernel<T, 2, BWD><<<grid, 256, 0, s>>>(r[0], r[1], r[2], act, gh, F, out, keep, Fp);
-    return;
-  }
+  // In one round of a workgroup a CU the shared sums beat the tiles' (float 185 x 384
+  // -> 315: 9 us where the smallest tile takes 17; bfloat16 128 x 4096 -> 1024: 11,
+  // 26), by 32 tokens if that is one round, by 64 if not (float 200 x 512 -> 2048: 13,
+  // by 32 15, tiles 21); in two rounds they do not (500 x 512 -> 2048: 25, 22), but
+  // where there are no more tokens and all else waits for the weights (16 x 2048 ->
+  // 8192: 13, 22).
+  const int64_t fs = cdiv(BWD ? Fp : F, 32);
+  auto few = [&](auto n) {
+    constexpr int TN = decltype(n)::value;
+    gated_few_kernel<T, TN, BWD><<<dim3((unsigned)fs, (unsigned)cdiv(M, 32 * TN)), 256, 0, s>>>(
+        r[0], r[1], r[2], act, gh, F, out, keep, Fp);
+  };
+  if (M <= 32 || fs * cdiv(M, 32) <= 256) return few(std::integral_constant<int, 1>());
+  if (M <= 64 || fs * cdiv(M, 64) <= 256) return few(std::integral_constant<int, 2>());
   typedef std::integral_constant<int, 256> I256;
   typedef std::integral_constant<int, 128> I128;
   typedef std::integral_constant<int, 64> I64;
