@@ -75,7 +75,8 @@ constexpr int UNIT = 128;  // bytes of the summed axis that widths and shares ar
 // Tile (m, n) of a grid of tiles_m x tiles_n: an XCD takes consecutive tiles
 // (workgroups go round-robin over the eight), which run down groups of eight
 // row tiles, so that the tiles that an XCD works on at a time share rows of both
-// operands in its L2.
+// operands in its L2.  A group begins at a column as far on as it is down, so that the
+// XCDs' stores, a row's length apart each, go to different places in the rows.
 __device__ __forceinline__ void tile_of(int tiles_m, int tiles_n, int& m, int& n) {
   const int grid = tiles_m * tiles_n, p = blockIdx.x;
   const int q = grid >> 3, r = grid & 7, x = p & 7;
@@ -84,7 +85,16 @@ __device__ __forceinline__ void tile_of(int tiles_m, int tiles_n, int& m, int& n
   const int rows = tiles_m - first < 8 ? tiles_m - first : 8;
   const int in = t - group * 8 * tiles_n;
   m = first + in % rows;
-  n = in / rows;
+  n = in / rows + (int)((int64_t)group * tiles_n / ((tiles_m + 7) / 8));
+  n -= n >= tiles_n ? tiles_n : 0;
+}
+
+// The values from one row of d to the next: dg, du, and 256 bytes more, so that rows of
+// a power of two of bytes begin in different channels of the memory (8192 x 512 x 2048
+// in bfloat16, training: 203 us without them, 195).
+template <typename T>
+__host__ __device__ constexpr int64_t d_pitch(int64_t Fp) {
+  return 2 * Fp + 256 / (int64_t)sizeof(T);
 }
 
 // Both projections of a tile of BM / 2 features and BN tokens.  The products'
@@ -92,7 +102,7 @@ __device__ __forceinline__ void tile_of(int tiles_m, int tiles_n, int& m, int& n
 // for either half of the waves' rows, so that a lane holds both sums of an
 // output, and four neighbouring outputs of one token.
 // Forward: h, and with keep g and u themselves, a token's 2 F values.  Backward
-// (gh): dg and du into d, a token's 2 Fp values, Fp >= F with 0 past F.
+// (gh): dg and du into d, a token's 2 Fp values, Fp >= F with 0 past F, d_pitch apart.
 template <typename T, int BM, int BN, bool BWD>
 __global__ __launch_bounds__(256, 2) void gated_pair_kernel(
     Matrix x, Matrix wg, Matrix wu, int act, const T* __restrict__ gh, int64_t F,
@@ -161,8 +171,8 @@ __global__ __launch_bounds__(256, 2) void gated_pair_kernel(
         rg.store(keep + y * F, 2 * F, t, M, f0, F);
       }
     } else if (BWD) {
-      rg.store(out, 2 * Fp, t, M, f0, Fp);
-      ru.store(out + Fp, 2 * Fp, t, M, f0, Fp);
+      rg.store(out, d_pitch<T>(Fp), t, M, f0, Fp);
+      ru.store(out + Fp, d_pitch<T>(Fp), t, M, f0, Fp);
     } else {
       rg.store(out, F, t, M, f0, F);
     }
@@ -287,8 +297,8 @@ __global__ __launch_bounds__(256) void gated_few_kernel(Matrix x, Matrix wg, Mat
         const bool in = f + e < F;
         const float y = in ? (float)gh[m * F + f + e] : 0.f;
         if (f + e < Fp) {
-          out[m * 2 * Fp + f + e] = in ? (T)(y * u[e] * d) : (T)0.f;
-          out[m * 2 * Fp + Fp + f + e] = in ? (T)(y * a) : (T)0.f;
+          out[m * d_pitch<T>(Fp) + f + e] = in ? (T)(y * u[e] * d) : (T)0.f;
+          out[m * d_pitch<T>(Fp) + Fp + f + e] = in ? (T)(y * a) : (T)0.f;
         }
       } else if (f + e < F) {
         out[m * F + f + e] = (T)(a * u[e]);
@@ -317,8 +327,8 @@ __global__ __launch_bounds__(256) void gated_kept_kernel(const float* __restrict
       dg = y * u * s;
       du = y * a;
     }
-    d[m * 2 * Fp + f] = dg;
-    d[m * 2 * Fp + Fp + f] = du;
+    d[m * d_pitch<float>(Fp) + f] = dg;
+    d[m * d_pitch<float>(Fp) + Fp + f] = du;
   }
 }
 
@@ -527,7 +537,7 @@ Plan gated_plan(int dtype, int64_t M, int64_t K, int64_t F, bool bwd) {
     p.wu = take(F * p.Kp, z);
   }
   if (bwd) {
-    p.d = take(M * 2 * p.Fp, z);
+    p.d = take(M * (2 * p.Fp + 256 / z), z);  // d_pitch
     p.dx = gated_cut(dtype, K, M, 1, 2 * p.funits, 2 * p.Fp);
     p.dw = gated_cut(dtype, K, F, 2, p.munits, M);
     const int64_t a = p.dx.shares > 1 ? p.dx.shares * M * K : 0;
@@ -671,7 +681,7 @@ extern "C" int tpo_gated_bwd(int dtype, const void* grad_h, const void* x, const
     typedef decltype(t) T;
     Matrix r[3];
     gated_inputs<T>(p, x, w_gate, w_up, M, K, F, ws, s, r);
-    const int64_t row = 2 * p.Fp * sizeof(T);
+    const int64_t row = 2 * p.Fp * sizeof(T), pitch = d_pitch<T>(p.Fp) * sizeof(T);
     float* part = (float*)(ws + p.part);
     if (M > 0 && F > 0 && kept)
       gated_kept_kernel<<<dim3((unsigned)cdiv(p.Fp, 256), (unsigned)(M < 16384 ? M : 16384)), 256, 0,
@@ -680,7 +690,7 @@ extern "C" int tpo_gated_bwd(int dtype, const void* grad_h, const void* x, const
     else if (M > 0 && F > 0)
       gated_pair<T, true>(r, activation, (const T*)grad_h, F, (T*)(ws + p.d), nullptr, p.Fp, s);
     if (grad_x && M > 0) {
-      const Matrix d{ws + p.d, row, M, row};
+      const Matrix d{ws + p.d, pitch, M, row};
       T* to = (T*)grad_x;
       switch (p.dx.tile) {
         case LARGE: gated_dx<T, 256, 128>(p, d, r[1], r[2], K, to, part, s); break;
@@ -689,7 +699,7 @@ extern "C" int tpo_gated_bwd(int dtype, const void* grad_h, const void* x, const
       }
     }
     if (grad_w_gate && F > 0) {
-      const Matrix d{ws + p.d, row, M, row / 2};
+      const Matrix d{ws + p.d, pitch, M, row / 2};
       T *g = (T*)grad_w_gate, *u = (T*)grad_w_up;
       switch (p.dw.tile) {
         case LARGE: gated_dw<T, 256, 128>(p, r[0], d, F, K, g, u, part, s); break;
