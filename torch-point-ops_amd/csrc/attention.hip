@@ -226,7 +226,8 @@ __device__ __forceinline__ void step_gather(char* __restrict__ kl, const char* _
 // part: with shares, each row's sums (D floats, not divided), and in ml their
 // maximum (in the exponent of 2) and sum
 template <typename T, int DP>
-__global__ __launch_bounds__(64 * STEP_WAVES, (DP * sizeof(T) <= 256 ? 2 : 1)) void attn_step_kernel(
+__global__ __launch_bounds__(64 * STEP_WAVES,
+                             (DP * sizeof(T) <= 256 ? 2 : 1)) void attn_step_kernel(
     AttnArgs a, const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ v,
     T* __restrict__ out, float* __restrict__ lse, T* __restrict__ rest,
     float* __restrict__ part, float2* __restrict__ ml) {
@@ -370,13 +371,15 @@ __global__ __launch_bounds__(256) void attn_join_kernel(const float* __restrict_
   __syncthreads();
   const int d = threadIdx.x;
   if (d < D) {
-    const float y = ((s[0][d] + s[1][d]) + (s[2][d] + s[3][d])) * (total != 0.f ? 1.f / total : 0.f);
+    const float inv = total != 0.f ? 1.f / total : 0.f;
+    const float y = ((s[0][d] + s[1][d]) + (s[2][d] + s[3][d])) * inv;
     const T z = (T)y;
     out[at * D + d] = z;
     if (rest) rest[at * D + d] = (T)(y - (float)z);
   }
   if (lse && d == 0)
-    lse[(at % Hq) * Tq + at / Hq] = total == 0.f ? NEG_INF : (m + __builtin_amdgcn_logf(total)) * LN2;
+    lse[(at % Hq) * Tq + at / Hq] =
+        total == 0.f ? NEG_INF : (m + __builtin_amdgcn_logf(total)) * LN2;
 }
 
 int attn_check(const char* op, int dtype, int64_t B, int64_t Tq, int64_t Tk, int64_t Hq,

@@ -32,7 +32,9 @@ struct AttnArgs {
 // start(s) G / tile + s.  That leaves room for each sequence's tiles (the last
 // one of a sequence and the first of the next may meet in one place, hence + s)
 // without a sum over the sequences before it; some places stay empty.
-inline int64_t attn_places(int64_t T, int64_t G, int64_t B, int tile) { return T * G / tile + B + 2; }
+inline int64_t attn_places(int64_t T, int64_t G, int64_t B, int tile) {
+  return T * G / tile + B + 2;
+}
 __device__ __forceinline__ int64_t attn_first(const Sequences& s, int i, int G, int tile) {
   return s.start(i) * G / tile + i;
 }

@@ -200,7 +200,8 @@ struct KeySums {
 constexpr int ALL_ROWS = INT32_MIN;
 template <typename T, int DP>
 __device__ __forceinline__ void bwd_keys_step(const char* __restrict__ cur, char* __restrict__ nxt,
-                                              const HeadLanes<T, DP>& lanes, const T* q, const T* go, const float* sub,
+                                              const HeadLanes<T, DP>& lanes, const T* q,
+                                              const T* go, const float* sub,
                                               const float* delta, const AttnArgs& a, int next,
                                               const HeadRows<T, DP>& k, const HeadRows<T, DP>& v,
                                               KeySums<T, DP>& sums, int t, int i0, int left,
@@ -240,8 +241,9 @@ __device__ __forceinline__ void bwd_keys_step(const char* __restrict__ cur, char
 // tiles that all four waves share.  Wave w has keys 32 (w % 2) .. + 31 and half w /
 // 2 of each tile's rows; at the end two waves add what they have, one stores dK,
 // one dV.  blockIdx.y: a share of the group's heads, `heads` of them; with more than
-// one its sums go to part as floats (dK, then dV).  (128 keys with all rows a wave: half as many workgroups of twice the
-// length, 128 us where this takes 123 for 8 x 2048.)
+// one its sums go to part as floats (dK, then dV).  (128 keys with all rows a wave:
+// half as many workgroups of twice the length, 128 us where this takes 123 for 8 x
+// 2048.)
 template <typename T, int DP>
 __global__ __launch_bounds__(256, (DP * sizeof(T) <= 192 ? 2 : 1)) void attn_bwd_keys_kernel(
     AttnArgs a, const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ v,
@@ -253,7 +255,8 @@ __global__ __launch_bounds__(256, (DP * sizeof(T) <= 192 ? 2 : 1)) void attn_bwd
   int local;
   AttnSpan p;
   if (!attn_tile<true>(a, blockIdx.x / a.Hk, gridDim.x / a.Hk, 1, 64, p, local)) return;
-  const int w = wave_id(), l = lane_id(), b0 = local * 64, j0 = b0 + 32 * (w & 1), j = j0 + (l & 31);
+  const int w = wave_id(), l = lane_id(), b0 = local * 64;
+  const int j0 = b0 + 32 * (w & 1), j = j0 + (l & 31);
   const bool in = j < p.Lk;
   HeadRows<T, DP> x, y;
   x.load(k + (p.k0 + j) * a.k_row + hk * a.k_head, in, a.D);

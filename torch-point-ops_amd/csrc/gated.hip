@@ -271,7 +271,8 @@ __global__ __launch_bounds__(256) void gated_few_kernel(Matrix x, Matrix wg, Mat
 #pragma unroll
       for (int b = 0; b < 4; ++b)
         sums[(((w * 2 + y) * TN + i) * 4 + b) * 64 + l] =
-            f32x4{acc[y][i][4 * b], acc[y][i][4 * b + 1], acc[y][i][4 * b + 2], acc[y][i][4 * b + 3]};
+            f32x4{acc[y][i][4 * b], acc[y][i][4 * b + 1], acc[y][i][4 * b + 2],
+                  acc[y][i][4 * b + 3]};
   __syncthreads();
   // wave w finishes values b = w of the lanes' columns
 #pragma unroll
@@ -486,7 +487,8 @@ struct Cut {
 Cut gated_cut(int dtype, int64_t rows, int64_t cols, int64_t products, int64_t units,
               int64_t summed) {
   static const int64_t R[] = {256, 128, 64}, C[] = {128, 128, 64}, PLACES[] = {512, 512, 1024};
-  static const double RATE[] = {1.05e15, 0.9e15, 0.56e15}, FLOAT_RATE[] = {0.13e15, 0.13e15, 0.1e15};
+  static const double RATE[] = {1.05e15, 0.9e15, 0.56e15};
+  static const double FLOAT_RATE[] = {0.13e15, 0.13e15, 0.1e15};
   Cut best{SMALL, 1};
   double least = 1e30;
   for (int t = 0; t < 3; ++t) {
@@ -496,7 +498,8 @@ Cut gated_cut(int dtype, int64_t rows, int64_t cols, int64_t products, int64_t u
       if (s > 1 && s > units / 8) break;
       // rounds by halves: places that are half taken work faster, though not twice
       const double filled = (double)(blocks * s) / PLACES[t];
-      const double rounds = filled <= 0.5 ? 0.62 : filled <= 1 ? 1 : 0.5 * (double)(int64_t)(2 * filled + 0.99);
+      const double halves = (double)(int64_t)(2 * filled + 0.99);
+      const double rounds = filled <= 0.5 ? 0.62 : filled <= 1 ? 1 : 0.5 * halves;
       const double tile = 2.0 * R[t] * C[t] * ((double)summed / s);
       double time = rounds * tile * PLACES[t] / rate;
       if (s > 1) time += 8.0 * s * rows * cols * products / 4e12 + 5e-6;
@@ -576,7 +579,8 @@ void gated_pair(const Matrix (&r)[3], int act, const T* gh, int64_t F, T* out, T
   const int64_t M = r[0].rows;
   auto run = [&](auto bm, auto bn) {
     constexpr int BM = decltype(bm)::value, BN = decltype(bn)::value;
-    gated_pair_kernel<T, BM, BN, BWD><<<dim3((unsigned)(cdiv(M, BN) * cdiv(F, BM / 2))), 256, 0, s>>>(
+    const int64_t tiles = cdiv(M, BN) * cdiv(F, BM / 2);
+    gated_pair_kernel<T, BM, BN, BWD><<<dim3((unsigned)tiles), 256, 0, s>>>(
         r[0], r[1], r[2], act, gh, F, out, keep, Fp);
   };
   // In one round of a workgroup a CU the shared sums beat the tiles' (float 185 x 384
@@ -596,7 +600,8 @@ void gated_pair(const Matrix (&r)[3], int act, const T* gh, int64_t F, T* out, T
   typedef std::integral_constant<int, 256> I256;
   typedef std::integral_constant<int, 128> I128;
   typedef std::integral_constant<int, 64> I64;
-  switch (gated_cut(sizeof(T) == 4 ? TPO_F32 : TPO_BF16, 2 * F, M, 1, 0, r[0].bytes / sizeof(T)).tile) {
+  const int type = sizeof(T) == 4 ? TPO_F32 : TPO_BF16;
+  switch (gated_cut(type, 2 * F, M, 1, 0, r[0].bytes / sizeof(T)).tile) {
     case LARGE: run(I256(), I128()); break;
     case MIDDLE: run(I128(), I128()); break;
     case SMALL: run(I128(), I64()); break;
@@ -621,7 +626,8 @@ void gated_dw(const Plan& p, const Matrix& x, const Matrix& d, int64_t F, int64_
   gated_dw_kernel<T, BM, BN><<<dim3((unsigned)(cdiv(F, BN) * cdiv(K, BM)), shares, 2), 256, 0, s>>>(
       x, d, F, (int)p.munits, share, K, dwg, dwu, shares > 1 ? part : nullptr);
   if (shares > 1)
-    gated_join_kernel<T><<<dim3(gated_blocks(F * K), 2), 256, 0, s>>>(part, shares, F * K, dwg, dwu);
+    gated_join_kernel<T><<<dim3(gated_blocks(F * K), 2), 256, 0, s>>>(part, shares, F * K, dwg,
+                                                                      dwu);
 }
 
 }  // namespace tpo
@@ -661,7 +667,8 @@ extern "C" int64_t tpo_gated_bwd_workspace_size(int dtype, int64_t M, int64_t K,
 }
 
 extern "C" int tpo_gated_bwd(int dtype, const void* grad_h, const void* x, const void* w_gate,
-                             const void* w_up, const void* kept, int64_t M, int64_t K, int64_t F, int activation,
+                             const void* w_up, const void* kept, int64_t M, int64_t K, int64_t F,
+                             int activation,
                              void* grad_x, void* grad_w_gate, void* grad_w_up, void* workspace,
                              int64_t workspace_bytes, void* stream) {
   if (int rc = gated_check("gated_bwd", dtype, M, K, F, activation)) return rc;
@@ -684,8 +691,8 @@ extern "C" int tpo_gated_bwd(int dtype, const void* grad_h, const void* x, const
     const int64_t row = 2 * p.Fp * sizeof(T), pitch = d_pitch<T>(p.Fp) * sizeof(T);
     float* part = (float*)(ws + p.part);
     if (M > 0 && F > 0 && kept)
-      gated_kept_kernel<<<dim3((unsigned)cdiv(p.Fp, 256), (unsigned)(M < 16384 ? M : 16384)), 256, 0,
-                          s>>>((const float*)kept, (const float*)grad_h, M, F, p.Fp, activation,
+      gated_kept_kernel<<<dim3((unsigned)cdiv(p.Fp, 256), (unsigned)(M < 16384 ? M : 16384)), 256,
+                          0, s>>>((const float*)kept, (const float*)grad_h, M, F, p.Fp, activation,
                                (float*)(ws + p.d));
     else if (M > 0 && F > 0)
       gated_pair<T, true>(r, activation, (const T*)grad_h, F, (T*)(ws + p.d), nullptr, p.Fp, s);

@@ -239,8 +239,8 @@ struct Operands {
 // reads and loads go between the matrix instructions; a wave issues in order,
 // and a row of loads that waits for its turn at the memory pipe keeps its
 // products waiting as well (where other waves' fill in, the row is quicker: 276
-// against 318 us for a product of 275 GFLOP in 128 x 128 tiles).  (That the two parts of LDS are apart is what
-// `restrict` says: a read need not wait for the loads.)
+// against 318 us for a product of 275 GFLOP in 128 x 128 tiles).  That the two parts of
+// LDS are apart is what `restrict` says: a read need not wait for the loads.
 template <typename T, int BM, int SLAB, bool SPREAD, typename LA, typename LB, int TM, int TN>
 __device__ __forceinline__ void slab_step(const char* __restrict__ cur, char* __restrict__ nxt,
                                           const LA& la, const LB& lb, int next, int row0, int col0,
@@ -336,7 +336,8 @@ __device__ __forceinline__ void gemm_tile(Lds& lds, const LA& la, const LB& lb, 
     // wave has read the last of the slab before it, whose place is loaded next
     wait_loads_and_meet<(DEPTH - 2) * (LA::N + LB::N)>();
     const int free = at == 0 ? DEPTH - 1 : at - 1;
-    slab_step<T, BM, SLAB, Lds::SPREAD>(lds.slab[at], lds.slab[free], la, lb, k + DEPTH - 1, row0, col0, u, acc);
+    slab_step<T, BM, SLAB, Lds::SPREAD>(lds.slab[at], lds.slab[free], la, lb, k + DEPTH - 1, row0,
+                                        col0, u, acc);
     at = at + 1 == DEPTH ? 0 : at + 1;
   }
 #pragma unroll

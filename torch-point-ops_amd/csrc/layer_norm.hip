@@ -518,8 +518,8 @@ extern "C" int tpo_layer_norm_bwd(int dtype, int wdtype, const void* grad_y, con
         constexpr int TEAM = decltype(team)::value;
         layer_norm_bwd_kernel<T, W, decltype(per)::value, decltype(n)::value, TEAM>
             <<<dim3((unsigned)parts), ln_threads(TEAM), 0, s>>>(
-                (const T*)grad_y, (const T*)x, (const W*)weight, mean, rstd, rows, width, (T*)grad_x,
-                part);
+                (const T*)grad_y, (const T*)x, (const W*)weight, mean, rstd, rows, width,
+                (T*)grad_x, part);
       });
     } else if (rows > 0) {
       if (grad_x && width <= LN_NARROW)
