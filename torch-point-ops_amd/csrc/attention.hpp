@@ -64,9 +64,9 @@ __device__ __forceinline__ int64_t uniform(int64_t v) {
 // each size 1 .. c (a causal prompt's last tile sees the most keys, its first keys
 // are seen by the most rows).  Where workgroups are few, the long ones have to
 // start first: in the order of places a training step's dK and dV kept the CUs
-// busy for 58 % of its time.  A lane tries one size; sequences, n of them with c
-// tiles in lane c's place, are passed round.  Returns the sequence, or -1, and the
-// tile's size.
+// busy for 58 % of its time.  A lane tries one size; the sequences, `seqs` of them, each
+// with the c tiles of its lane, are passed round.  Returns the sequence, or -1, and
+// the tile's size.
 __device__ __forceinline__ int attn_by_size(int c, int seqs, int p, int& size) {
   const int l = lane_id();
   int lo = 0, hi = 0;
