@@ -6,6 +6,7 @@
 #include <torch/library.h>
 
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
 #include <torch/csrc/autograd/custom_function.h>
 
@@ -45,9 +46,12 @@ namespace {
 }
 
 // Whether autograd has to follow the call.  Without it the operator runs as it
-// is, also under transforms that a C++ autograd function refuses.
+// is, also under transforms that a C++ autograd function refuses.  A tangent
+// counts as well: forward mode has no formula here, and the function says so where
+// the operator alone would return a result without one.
 [[maybe_unused]] bool followed(const at::Tensor& a) {
-  return at::GradMode::is_enabled() && a.requires_grad();
+  return (at::GradMode::is_enabled() && a.requires_grad()) ||
+         (c10::AutogradState::get_tls_state().get_fw_grad_mode() && a._fw_grad(0).defined());
 }
 
 template <typename Op>
