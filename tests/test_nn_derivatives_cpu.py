@@ -50,3 +50,39 @@ def test_tangents_are_refused(tpo, name):
         with pytest.raises(RuntimeError, match="functorch transforms"):
             torch.func.jvp(lambda t: f(*inputs[:at], t, *inputs[at + 1:]), (x,),
                            (torch.empty_like(x),))
+
+
+NN = NAMES[:3]
+
+
+@pytest.mark.parametrize("name", NN)
+def test_gradients_of_gradients_are_refused(tpo, name):
+    f, inputs = _calls(tpo)[name]
+    inputs = [t.requires_grad_(True) for t in inputs]
+    y = f(*inputs)
+    once = torch.autograd.grad(y.sum(), inputs, create_graph=True)
+    assert [g.shape for g in once] == [t.shape for t in inputs]
+    for g in once:
+        # also where the loss has another way to the inputs
+        for loss in (g.sum(), g.sum() + y.sum()):
+            with pytest.raises(RuntimeError, match="_backward is not implemented"):
+                torch.autograd.grad(loss, inputs, retain_graph=True, allow_unused=True)
+    # a result that was only asked to keep its graph has its first derivative
+    again = torch.autograd.grad(y.sum(), inputs, create_graph=True)
+    assert [g.shape for g in again] == [t.shape for t in inputs]
+
+
+@pytest.mark.parametrize("name", NN)
+def test_inner_operators_have_no_derivative(tpo, name):
+    """The operators that the autograd functions call, called alone."""
+    f, inputs = _calls(tpo)[name]
+    o = torch.empty(3, dtype=torch.int64, device="meta")
+    more = {"layer_norm": (1e-5,), "packed_attention": (o, o, None, None, True, 1.0),
+            "gated_projection": (0,)}[name]
+    ns = {"layer_norm": "norm", "packed_attention": "attention", "gated_projection": "gated"}[name]
+    op = getattr(getattr(torch.ops, f"torch_point_ops_{ns}"), f"{name}_forward")
+    inputs = [t.requires_grad_(True) for t in inputs]
+    with pytest.raises(RuntimeError, match="_forward is not implemented"):
+        op(*inputs, *more)[0].sum().backward()
+    with fw.dual_level(), pytest.raises(RuntimeError, match="forward AD"):
+        op(*[fw.make_dual(t.detach(), torch.empty_like(t)) for t in inputs], *more)

@@ -4,6 +4,8 @@
 // torch_ops.cpp does them; the kernels are libtpo_hip.so's.
 #include "shim_common.hpp"
 
+#include <torch/csrc/autograd/autograd_not_implemented_fallback.h>
+
 namespace torch_point_ops {
 namespace {
 
@@ -499,6 +501,10 @@ Tensor gated_projection_autograd(const Tensor& x, const Tensor& wg, const Tensor
   return GatedProjectionFunction::apply(x, wg, wu, act);
 }
 
+// The operators that the functions above call have no formula of their own: a
+// gradient of a gradient, or a tangent, is refused instead of left out.
+torch::CppFunction no_formula() { return torch::autograd::autogradNotImplementedFallback(); }
+
 // There are no CPU kernels: as Chamfer and EMD, a call says so.
 Tensor layer_norm_cpu(const Tensor&, const OptTensor&, const OptTensor&, double) {
   TORCH_CHECK(false, "layer_norm is not implemented for CPU");
@@ -546,6 +552,8 @@ TORCH_LIBRARY_IMPL(torch_point_ops_norm, CUDA, m) {
 }
 TORCH_LIBRARY_IMPL(torch_point_ops_norm, Autograd, m) {
   m.impl("layer_norm", &layer_norm_autograd);
+  m.impl("layer_norm_forward", no_formula());
+  m.impl("layer_norm_backward", no_formula());
 }
 
 TORCH_LIBRARY(torch_point_ops_attention, m) {
@@ -571,6 +579,8 @@ TORCH_LIBRARY_IMPL(torch_point_ops_attention, CUDA, m) {
 }
 TORCH_LIBRARY_IMPL(torch_point_ops_attention, Autograd, m) {
   m.impl("packed_attention", &packed_attention_autograd);
+  m.impl("packed_attention_forward", no_formula());
+  m.impl("packed_attention_backward", no_formula());
 }
 
 TORCH_LIBRARY(torch_point_ops_gated, m) {
@@ -592,6 +602,8 @@ TORCH_LIBRARY_IMPL(torch_point_ops_gated, CUDA, m) {
 }
 TORCH_LIBRARY_IMPL(torch_point_ops_gated, Autograd, m) {
   m.impl("gated_projection", &gated_projection_autograd);
+  m.impl("gated_projection_forward", no_formula());
+  m.impl("gated_projection_backward", no_formula());
 }
 
 }  // namespace torch_point_ops
