@@ -79,6 +79,16 @@ struct RowHeld {
 #pragma unroll
       for (int e = 0; e < PER; ++e) v[i][e] = f;
   }
+  // f in the places past the row's end
+  __device__ __forceinline__ void past(int64_t width, float f) {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (column(i) + PER > width) {
+#pragma unroll
+        for (int e = 0; e < PER; ++e)
+          if (column(i) + e >= width) v[i][e] = f;
+      }
+  }
   __device__ __forceinline__ void store(T* p, int64_t width) const {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
@@ -172,13 +182,14 @@ __global__ __launch_bounds__(ln_threads(TEAM)) void layer_norm_bwd_kernel(
     gs.load(gy + r * width, width);
     xs.load(x + r * width, width);
     const float m = mean[r], q = rstd[r];
+    xs.past(width, m);  // h = 0: (0 - m) q can be infinite, and 0 times it no number
     float s1 = 0.f, s2 = 0.f;
 #pragma unroll
     for (int i = 0; i < N; ++i)
 #pragma unroll
       for (int e = 0; e < PER; ++e) {
         const float h = (xs.v[i][e] - m) * q, y = gs.v[i][e], g = y * ws.v[i][e];
-        xs.v[i][e] = h;  // (past the row's end y is 0: nothing is added)
+        xs.v[i][e] = h;  // (past the row's end y and h are 0: nothing is added)
         sw.v[i][e] = __builtin_fmaf(y, h, sw.v[i][e]);
         sb.v[i][e] += y;
         s1 += g;
