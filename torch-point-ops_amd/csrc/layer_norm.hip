@@ -429,18 +429,30 @@ void with_form(const LnForm& f, F&& call) {
 
 constexpr int64_t LN_WIDTH_MAX = 1 << 20;
 inline dim3 ln_long_grid(int64_t rows) { return dim3((unsigned)(rows < 65536 ? rows : 65536)); }
-// Shares of the rows for the weights' gradients: workgroups that keep the memory
-// busy, but no more than keeps their sums' way through memory short beside the
-// rows' (16 rows a share, and 8 where a workgroup has one row at a time).  Loading
-// the next row ahead of the sums instead was slower (32768 x 1024: 103 us for 80):
-// it costs the registers of other workgroups.
-inline int ln_parts(int64_t rows, int64_t width) {
-  const int64_t each = width > 2048 ? 8 : 16, top = width > 2048 ? 512 : 1024;
-  const int64_t few = (rows + 3) / 4, most = rows / each > 64 ? rows / each : 64;
-  const int64_t p = few < most ? few : most;
-  return (int)(p > top ? top : p);
+// Workgroups where nothing is summed over the rows: up to eight a CU.
+inline unsigned ln_blocks(int64_t rows, int64_t teams) {
+  const int64_t n = (rows + teams - 1) / teams;
+  return (unsigned)(n < 2048 ? n : 2048);
 }
-
+// Workgroups of the backward, which are the shares of the rows for the weights'
+// gradients: as many as have a row for each of their teams, up to two a CU (one where a
+// row takes sixteen waves); where a workgroup is one team, two rows each from half of
+// that on; and one for every 8 rows beyond, as the shares' sums go through memory twice.
+// (16 x 8192 in bfloat16: 11.6 us by 4 workgroups, 6.8 by 16; 256 x 8192: 16.3 by 256,
+// 14.0 by 128; 500 x 16384: 41.5 by 64, 26.8 by 250; 1000 x 1500: 30.3 by 64, 13.8 by
+// 500; 1000 x 700, four teams each: 16.0 by 64, 10.3 by 250.)  Loading the next row ahead
+// of the sums instead was slower (32768 x 1024: 103 us for 80): it costs the registers
+// of other workgroups.
+int ln_parts(int64_t rows, int64_t width, int64_t size) {
+  const LnForm f = ln_form(width, size);
+  const int64_t teams = f.held ? ln_threads(f.team) / f.team : 4;
+  int64_t few = (rows + teams - 1) / teams, most = !f.held ? 64 : f.team <= 512 ? 512 : 256;
+  if (teams == 1 && few > most / 2) few = rows > most ? rows / 2 : most / 2;
+  if (most < rows / 8) most = rows / 8;
+  const int64_t top = width > 2048 ? 512 : 1024;
+  if (most > top) most = top;
+  return (int)(few < most ? few : most);
+}
 // The weights are of the input's type or float.
 template <typename F>
 int ln_dispatch(const char* op, int dtype, int wdtype, F&& f) {
@@ -490,12 +502,10 @@ extern "C" int tpo_layer_norm_fwd(int dtype, int wdtype, const void* x, const vo
     }
     with_form<T>(f, [&](auto per, auto n, auto team) {
       constexpr int TEAM = decltype(team)::value, THREADS = ln_threads(TEAM);
-      constexpr int TEAMS = THREADS / TEAM;
-      int64_t blocks = (rows + TEAMS - 1) / TEAMS;
-      if (blocks > 2048) blocks = 2048;  // eight workgroups a CU
       layer_norm_fwd_kernel<T, W, decltype(per)::value, decltype(n)::value, TEAM>
-          <<<dim3((unsigned)blocks), THREADS, 0, s>>>((const T*)x, (const W*)weight, (const W*)bias,
-                                                  rows, width, (float)eps, (T*)y, mean, rstd);
+          <<<dim3(ln_blocks(rows, THREADS / TEAM)), THREADS, 0, s>>>(
+              (const T*)x, (const W*)weight, (const W*)bias, rows, width, (float)eps, (T*)y, mean,
+              rstd);
     });
   });
   return rc || none ? rc : check_launch("layer_norm_fwd");
@@ -503,7 +513,8 @@ extern "C" int tpo_layer_norm_fwd(int dtype, int wdtype, const void* x, const vo
 
 extern "C" int64_t tpo_layer_norm_bwd_workspace_size(int64_t rows, int64_t width) {
   if (ln_check("layer_norm_bwd_workspace_size", rows, width)) return -1;
-  return round_up((int64_t)ln_parts(rows, width) * 2 * width * 4, 256);
+  const int a = ln_parts(rows, width, 2), b = ln_parts(rows, width, 4);
+  return round_up((int64_t)(a > b ? a : b) * 2 * width * 4, 256);
 }
 
 extern "C" int tpo_layer_norm_bwd(int dtype, int wdtype, const void* grad_y, const void* x,
@@ -522,13 +533,14 @@ extern "C" int tpo_layer_norm_bwd(int dtype, int wdtype, const void* grad_y, con
     typedef decltype(t) T;
     typedef decltype(w) W;
     const LnForm f = ln_form(width, sizeof(T));
-    const int parts = ln_parts(rows, width);
+    const int parts = ln_parts(rows, width, sizeof(T));
     float* part = sums ? (float*)workspace : nullptr;
     if (rows > 0 && width > LN_NARROW && f.held) {
       with_form<T>(f, [&](auto per, auto n, auto team) {
-        constexpr int TEAM = decltype(team)::value;
+        constexpr int TEAM = decltype(team)::value, THREADS = ln_threads(TEAM);
+        const unsigned blocks = sums ? (unsigned)parts : ln_blocks(rows, THREADS / TEAM);
         layer_norm_bwd_kernel<T, W, decltype(per)::value, decltype(n)::value, TEAM>
-            <<<dim3((unsigned)parts), ln_threads(TEAM), 0, s>>>(
+            <<<dim3(blocks), THREADS, 0, s>>>(
                 (const T*)grad_y, (const T*)x, (const W*)weight, mean, rstd, rows, width,
                 (T*)grad_x, part);
       });
