@@ -4,6 +4,7 @@
 // torch_ops.cpp does them; the kernels are libtpo_hip.so's.
 #include "shim_common.hpp"
 
+#include <ATen/autocast_mode.h>
 #include <torch/csrc/autograd/autograd_not_implemented_fallback.h>
 
 namespace torch_point_ops {
@@ -501,6 +502,24 @@ Tensor gated_projection_autograd(const Tensor& x, const Tensor& wg, const Tensor
   return GatedProjectionFunction::apply(x, wg, wu, act);
 }
 
+// Under autocast the two operators that are products take its type, as torch's own
+// products do; layer norm takes x and weights of different types as they are.
+Tensor autocast(const Tensor& t) {
+  return at::autocast::cached_cast(at::autocast::get_autocast_dtype(at::kCUDA), t, at::kCUDA);
+}
+Tensor packed_attention_autocast(const Tensor& q, const Tensor& k, const Tensor& v,
+                                 const Tensor& oq, const Tensor& ok, const OptTensor& lq,
+                                 const OptTensor& lk, bool causal, double scale) {
+  c10::impl::ExcludeDispatchKeyGuard below(c10::DispatchKey::AutocastCUDA);
+  return packed_attention_op().call(autocast(q), autocast(k), autocast(v), oq, ok, lq, lk, causal,
+                                    scale);
+}
+Tensor gated_projection_autocast(const Tensor& x, const Tensor& wg, const Tensor& wu,
+                                 int64_t act) {
+  c10::impl::ExcludeDispatchKeyGuard below(c10::DispatchKey::AutocastCUDA);
+  return gated_projection_op().call(autocast(x), autocast(wg), autocast(wu), act);
+}
+
 // The operators that the functions above call have no formula of their own: a
 // gradient of a gradient, or a tangent, is refused instead of left out.
 torch::CppFunction no_formula() { return torch::autograd::autogradNotImplementedFallback(); }
@@ -577,6 +596,9 @@ TORCH_LIBRARY_IMPL(torch_point_ops_attention, CUDA, m) {
   m.impl("packed_attention_forward", &packed_attention_forward_hip);
   m.impl("packed_attention_backward", &packed_attention_backward_hip);
 }
+TORCH_LIBRARY_IMPL(torch_point_ops_attention, AutocastCUDA, m) {
+  m.impl("packed_attention", &packed_attention_autocast);
+}
 TORCH_LIBRARY_IMPL(torch_point_ops_attention, Autograd, m) {
   m.impl("packed_attention", &packed_attention_autograd);
   m.impl("packed_attention_forward", no_formula());
@@ -599,6 +621,9 @@ TORCH_LIBRARY_IMPL(torch_point_ops_gated, CUDA, m) {
   m.impl("gated_projection", &gated_projection_hip);
   m.impl("gated_projection_forward", &gated_projection_forward_hip);
   m.impl("gated_projection_backward", &gated_projection_backward_hip);
+}
+TORCH_LIBRARY_IMPL(torch_point_ops_gated, AutocastCUDA, m) {
+  m.impl("gated_projection", &gated_projection_autocast);
 }
 TORCH_LIBRARY_IMPL(torch_point_ops_gated, Autograd, m) {
   m.impl("gated_projection", &gated_projection_autograd);

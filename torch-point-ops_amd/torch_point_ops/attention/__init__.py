@@ -47,7 +47,8 @@ def packed_attention(q, k, v, offsets_q, offsets_k=None, lengths_q=None, lengths
     Returns (Tq, Hq, D) of q's type; rows that are not in use or see no key are 0.
     Differentiable in q, k and v, with sums in a fixed order.  Scores, their statistics and
     all sums are float32; half and bfloat16 probabilities (and the scores' gradients) are
-    rounded to the type for the products.
+    rounded to the type for the products.  Under torch.autocast q, k and v are taken in its
+    type.
     """
     if offsets_k is None:
         if lengths_k is not None:

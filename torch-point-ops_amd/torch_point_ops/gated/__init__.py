@@ -40,7 +40,8 @@ def gated_projection(x, w_gate, w_up, activation="silu"):
     Differentiable in x and the weights.  A float32 forward keeps the two projections for
     the backward; for the half types the backward computes them again, which takes less
     time than unrounded ones take through memory, and rounds the gradients at them to x's
-    type between the products.  All sums are float32.  Returns (..., F).
+    type between the products.  All sums are float32.  Under torch.autocast the inputs
+    are taken in its type, as a linear layer's are.  Returns (..., F).
     """
     code = _ACTIVATIONS.get(activation)
     if code is None:
