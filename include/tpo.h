@@ -386,7 +386,8 @@ int tpo_layer_norm_bwd(int dtype, int wdtype, const void* grad_y, const void* x,
  *   reaches no row of another sequence, and rows not in use are not read.
  * tpo_attention_bwd: grad_out, out, rest and the gradients are contiguous.  Every
  *   row of grad_q, grad_k, grad_v is written, rows not in use with 0; sums
- *   run in a fixed order.
+ *   run in a fixed order.  grad_q, or grad_k and grad_v together, may be NULL and
+ *   are left out; without grad_k and grad_v no workspace is needed.
  * Workspaces are 256-byte aligned; size 0 means none is used.
  */
 int64_t tpo_attention_fwd_workspace_size(int dtype, int64_t B, int64_t Tq, int64_t Tk,

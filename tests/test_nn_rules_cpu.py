@@ -39,3 +39,32 @@ def test_narrow_rows_have_a_wave_each(lib, width):
 def test_shares_stay_small_beside_many_rows(lib, width):
     for rows in (8192, 32768, 1 << 20, (1 << 31) - 1):
         assert 1 <= _shares(lib, rows, width) <= min(1024, rows // 8)
+
+
+def test_attention_backward_of_some(tpo, lib):
+    """dK and dV go together and alone take the workspace; each operator result can be left out."""
+    import torch
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    P, C, D = ctypes.c_void_p, ctypes.c_int, ctypes.c_double
+    lib.tpo_last_error.restype = ctypes.c_char_p
+    lib.tpo_attention_bwd.argtypes = [C] + [P] * 11 + [I] * 12 + [C, D, P, P, P, P, I, P]
+    f = P(4096)  # never dereferenced
+
+    def call(gq, gk, gv, rows=4, ws=None):
+        return lib.tpo_attention_bwd(0, f, f, f, f, f, f, f, f, f, None, None, 1, rows, rows, 2, 2,
+                                     16, *[32, 16] * 3, 1, 1.0, gq, gk, gv, ws, 0, None)
+
+    for gk, gv in ((f, None), (None, f)):
+        assert call(f, gk, gv) == -1 and b"go together" in lib.tpo_last_error()
+    assert call(None, f, f) == -4
+    assert call(None, None, None) == 0
+    assert call(f, None, None, rows=0) == 0
+    with FakeTensorMode():
+        q, k, o = torch.empty(7, 4, 32), torch.empty(9, 2, 32), torch.empty(3, dtype=torch.int64)
+        lse = torch.empty(4, 7)
+        for mask in ([True, False, False], [False, True, False], [False, False, True]):
+            g = torch.ops.torch_point_ops_attention.packed_attention_backward(
+                q, q, k, k, q, lse, torch.empty(0), o, o, None, None, True, 1.0, mask)
+            assert [t.shape for t in g] == [t.shape if on else (0,)
+                                            for t, on in zip((q, k, k), mask)]

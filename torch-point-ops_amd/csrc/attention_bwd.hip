@@ -67,7 +67,8 @@ __device__ __forceinline__ void bwd_q_step(const char* __restrict__ cur, char* _
 // end two waves' sums are added.  rest: what rounding took from O.  Without it the
 // rounding of O, which is common to all keys of a row, would add to dQ's error about
 // half of what the rounding of dS does.  (delta by a kernel of its own, which reads dO
-// once more, took 18 us of 234 for 8 x 2048; so they are 226.)
+// once more, took 18 us of 234 for 8 x 2048; so they are 226.)  gq null: only what dK
+// and dV need of the rows, sub and delta; sub null: only dQ.
 template <typename T, int DP>
 __global__ __launch_bounds__(256, (DP * sizeof(T) <= 256 ? 2 : 1)) void attn_bwd_q_kernel(
     AttnArgs a, const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ v,
@@ -92,7 +93,7 @@ __global__ __launch_bounds__(256, (DP * sizeof(T) <= 256 ? 2 : 1)) void attn_bwd
   const int64_t token = p.q0 + r / G;
   const T* kt = k + p.k0 * a.k_row + hk * a.k_head;
   const T* vt = v + p.k0 * a.v_row + hk * a.v_head;
-  if (end > 0) bwd_q_load<T, DP>(lds.b, kt, vt, a, p.Lk);
+  if (end > 0 && gq) bwd_q_load<T, DP>(lds.b, kt, vt, a, p.Lk);
   HeadRows<T, DP> x, y;
   x.load(q + token * a.q_row + head * a.q_head, in, a.D);
   y.load(go + (token * a.Hq + head) * a.D, in, a.D);
@@ -111,10 +112,11 @@ __global__ __launch_bounds__(256, (DP * sizeof(T) <= 256 ? 2 : 1)) void attn_bwd
     row_delta += other_half(row_delta);
     if (m == NEG_INF) row_delta = 0.f;
   }
-  if (in && w < 2 && l < 32) {
+  if (sub && in && w < 2 && l < 32) {
     sub[at] = row_sub;
     delta[at] = row_delta;
   }
+  if (!gq) return;
   const float c = attn_count(a.scale);
   if (a.scale < 0.f) x.negate();
   f32x16 acc[DP / 32];
@@ -433,11 +435,15 @@ extern "C" int tpo_attention_bwd(int dtype, const void* grad_out, const void* q,
                                  void* grad_q, void* grad_k, void* grad_v, void* workspace,
                                  int64_t workspace_bytes, void* stream) {
   if (int rc = attn_check("attention_bwd", dtype, B, Tq, Tk, Hq, Hk, D)) return rc;
-  const int64_t need = tpo_attention_bwd_workspace_size(dtype, B, Tq, Tk, Hq, Hk, D);
+  if ((grad_k == nullptr) != (grad_v == nullptr))
+    return set_error(TPO_ERR_ARG, "attention_bwd: grad_k and grad_v go together");
+  // (dQ alone needs nothing beside its rows)
+  const int64_t need =
+      grad_k ? tpo_attention_bwd_workspace_size(dtype, B, Tq, Tk, Hq, Hk, D) : 0;
   if (need > 0 && (!workspace || workspace_bytes < need))
     return set_error(TPO_ERR_WORKSPACE, "attention_bwd: workspace of %lld bytes needed",
                      (long long)need);
-  if (Tq == 0 && Tk == 0) return TPO_OK;
+  if ((Tq == 0 && Tk == 0) || (!grad_q && !grad_k)) return TPO_OK;
   if (int rc = attn_layout("attention_bwd", dtype, D,
                            {grad_out, q, k, v, out, rest, grad_q, grad_k, grad_v, workspace},
                            {q_row, q_head, k_row, k_head, v_row, v_head}, {q_row, k_row, v_row}))
@@ -449,10 +455,11 @@ extern "C" int tpo_attention_bwd(int dtype, const void* grad_out, const void* q,
   if (places_q * Hk >= ((int64_t)1 << 31) || places_k * Hk >= ((int64_t)1 << 31))
     return set_error(TPO_ERR_ARG, "attention_bwd: too many rows");
   const int64_t stats = round_up(Tq * Hq * 4, 256);
-  float *sub = (float*)workspace, *delta = (float*)((char*)workspace + stats);
+  float* sub = grad_k ? (float*)workspace : nullptr;
+  float* delta = grad_k ? (float*)((char*)workspace + stats) : nullptr;
   const int shares = attn_bwd_shares(B, Tk, Hq, Hk), heads = (int)((G + shares - 1) / shares);
   const int used = (int)((G + heads - 1) / heads);  // shares that have a head
-  float* part = used > 1 ? (float*)((char*)workspace + 2 * stats) : nullptr;
+  float* part = grad_k && used > 1 ? (float*)((char*)workspace + 2 * stats) : nullptr;
   hipStream_t s = (hipStream_t)stream;
   with_element(dtype, [&](auto t) {
     typedef decltype(t) T;
@@ -462,11 +469,11 @@ extern "C" int tpo_attention_bwd(int dtype, const void* grad_out, const void* q,
       if (Tq > 0)
         attn_bwd_q_kernel<T, DP><<<dim3((unsigned)(places_q * Hk)), 256, 0, s>>>(
             a, qt, kt, vt, go, (const T*)out, (const T*)rest, lse, sub, delta, (T*)grad_q);
-      if (Tk > 0)
+      if (Tk > 0 && grad_k)
         attn_bwd_keys_kernel<T, DP><<<dim3((unsigned)(places_k * Hk), used), 256, 0, s>>>(
             a, qt, kt, vt, go, sub, delta, (T*)grad_k, (T*)grad_v, heads, part);
     });
-    if (Tk > 0 && part) {
+    if (part && Tk > 0) {
       const int64_t n = Tk * Hk * D, blocks = (n + 1023) / 1024;
       attn_bwd_join_kernel<T><<<dim3((unsigned)(blocks < 2048 ? blocks : 2048), 2), 256, 0, s>>>(
           part, used, n, (T*)grad_k, (T*)grad_v);

@@ -288,7 +288,8 @@ std::tuple<Tensor, Tensor, Tensor> packed_attention_forward_hip(const Tensor& q,
 std::tuple<Tensor, Tensor, Tensor> packed_attention_backward_hip(
     const Tensor& grad_in, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& out_in,
     const Tensor& lse_in, const Tensor& rest_in, const Tensor& oq, const Tensor& ok,
-    const OptTensor& lq, const OptTensor& lk, bool causal, double scale) {
+    const OptTensor& lq, const OptTensor& lk, bool causal, double scale,
+    std::array<bool, 3> mask) {
   const char* op = "packed_attention_backward";
   const Packed p = packed_args(q, k, v, oq, ok, lq, lk, op);
   c10::OptionalDeviceGuard guard(q.device());
@@ -307,21 +308,29 @@ std::tuple<Tensor, Tensor, Tensor> packed_attention_backward_hip(
   const Tensor lse = lse_in.contiguous();
   Tensor rest;
   if (rest_in.numel() > 0) rest = head_rows(rest_in.contiguous(), p.D);
-  Tensor gq = at::empty({p.Tq, p.Hq, p.D}, q.options());
-  Tensor gk = at::empty({p.Tk, p.Hk, p.D}, q.options());
-  Tensor gv = at::empty({p.Tk, p.Hk, p.D}, q.options());
-  const int64_t wsb = tpo_attention_bwd_workspace_size(p.dt, p.B, p.Tq, p.Tk, p.Hq, p.Hk, p.D);
-  const Tensor ws = workspace(wsb, q, op);
+  // dK and dV come from one kernel
+  const bool keys = mask[1] || mask[2];
+  Tensor gq, gk, gv, ws;
+  int64_t wsb = 0;
+  if (mask[0]) gq = at::empty({p.Tq, p.Hq, p.D}, q.options());
+  if (keys) {
+    gk = at::empty({p.Tk, p.Hk, p.D}, q.options());
+    gv = at::empty({p.Tk, p.Hk, p.D}, q.options());
+    wsb = tpo_attention_bwd_workspace_size(p.dt, p.B, p.Tq, p.Tk, p.Hq, p.Hk, p.D);
+    ws = workspace(wsb, q, op);
+  }
   check_rc(tpo_attention_bwd(p.dt, g.data_ptr(), p.q.data_ptr(), p.k.data_ptr(), p.v.data_ptr(),
-                             out.data_ptr(), data_or_null(rest), lse.data_ptr<float>(), p.oq.data_ptr<int64_t>(),
-                             p.ok.data_ptr<int64_t>(), (const int64_t*)data_or_null(p.lq),
-                             (const int64_t*)data_or_null(p.lk), p.B, p.Tq, p.Tk, p.Hq, p.Hk, p.D,
-                             row_stride(p.q), head_stride(p.q), row_stride(p.k), head_stride(p.k),
-                             row_stride(p.v), head_stride(p.v), causal, scale, gq.data_ptr(),
-                             gk.data_ptr(), gv.data_ptr(), data_or_null(ws), wsb, stream_of(q)),
+                             out.data_ptr(), data_or_null(rest), lse.data_ptr<float>(),
+                             p.oq.data_ptr<int64_t>(), p.ok.data_ptr<int64_t>(),
+                             (const int64_t*)data_or_null(p.lq), (const int64_t*)data_or_null(p.lk),
+                             p.B, p.Tq, p.Tk, p.Hq, p.Hk, p.D, row_stride(p.q), head_stride(p.q),
+                             row_stride(p.k), head_stride(p.k), row_stride(p.v), head_stride(p.v),
+                             causal, scale, data_or_null(gq), data_or_null(gk), data_or_null(gv),
+                             data_or_null(ws), wsb, stream_of(q)),
            op);
   const int64_t D = q.size(2);
-  return {cut_heads(gq, D), cut_heads(gk, D), cut_heads(gv, D)};
+  return {mask[0] ? cut_heads(gq, D) : nothing(q), mask[1] ? cut_heads(gk, D) : nothing(q),
+          mask[2] ? cut_heads(gv, D) : nothing(q)};
 }
 
 auto packed_attention_op() {
@@ -352,13 +361,16 @@ class PackedAttentionFunction : public torch::autograd::Function<PackedAttention
     static auto op = typed_op<std::tuple<Tensor, Tensor, Tensor>(
         const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&,
         const Tensor&, const Tensor&, const Tensor&, const OptTensor&, const OptTensor&, bool,
-        double)>("torch_point_ops_attention::packed_attention_backward");
+        double, std::array<bool, 3>)>("torch_point_ops_attention::packed_attention_backward");
     const auto s = ctx->get_saved_variables();
+    const std::array<bool, 3> mask = {ctx->needs_input_grad(0), ctx->needs_input_grad(1),
+                                      ctx->needs_input_grad(2)};
     auto [gq, gk, gv] = op.call(grads[0], s[0], s[1], s[2], s[3], s[4], s[5], s[6], s[7], opt(s[8]),
                                 opt(s[9]), ctx->saved_data["causal"].toBool(),
-                                ctx->saved_data["scale"].toDouble());
+                                ctx->saved_data["scale"].toDouble(), mask);
     const Tensor none;
-    return {gq, gk, gv, none, none, none, none, none, none};
+    return {mask[0] ? gq : none, mask[1] ? gk : none, mask[2] ? gv : none,
+            none, none, none, none, none, none};
   }
 };
 
@@ -584,8 +596,9 @@ TORCH_LIBRARY(torch_point_ops_attention, m) {
         "Tensor offsets_k, Tensor? lengths_q, Tensor? lengths_k, bool causal, float scale) -> "
         "(Tensor, Tensor, Tensor)");
   m.def("packed_attention_backward(Tensor grad, Tensor q, Tensor k, Tensor v, Tensor out, "
-        "Tensor lse, Tensor rest, Tensor offsets_q, Tensor offsets_k, Tensor? lengths_q, Tensor? lengths_k, "
-        "bool causal, float scale) -> (Tensor, Tensor, Tensor)");
+        "Tensor lse, Tensor rest, Tensor offsets_q, Tensor offsets_k, Tensor? lengths_q, "
+        "Tensor? lengths_k, bool causal, float scale, bool[3] mask=[True, True, True]) -> "
+        "(Tensor, Tensor, Tensor)");
 }
 TORCH_LIBRARY_IMPL(torch_point_ops_attention, CPU, m) {
   m.impl("packed_attention", &packed_attention_cpu);

@@ -23,8 +23,10 @@ def _packed_attention_forward_fake(q, k, v, offsets_q, offsets_k, lengths_q, len
 
 @torch.library.register_fake("torch_point_ops_attention::packed_attention_backward")
 def _packed_attention_backward_fake(grad, q, k, v, out, lse, rest, offsets_q, offsets_k,
-                                    lengths_q, lengths_k, causal, scale):
-    return tuple(torch.empty(t.shape, device=t.device, dtype=t.dtype) for t in (q, k, v))
+                                    lengths_q, lengths_k, causal, scale,
+                                    mask=(True, True, True)):
+    return tuple(torch.empty(t.shape if on else (0,), device=t.device, dtype=t.dtype)
+                 for t, on in zip((q, k, v), mask))
 
 
 def packed_attention(q, k, v, offsets_q, offsets_k=None, lengths_q=None, lengths_k=None,
