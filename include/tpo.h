@@ -389,7 +389,12 @@ int tpo_layer_norm_bwd(int dtype, int wdtype, const void* grad_y, const void* x,
  *   run in a fixed order.  grad_q, or grad_k and grad_v together, may be NULL and
  *   are left out; without grad_k and grad_v no workspace is needed.
  * Workspaces are 256-byte aligned; size 0 means none is used.
+ * tpo_attention_fwd_rows is a diagnostic: the query rows (tokens times the heads
+ *   of a group) that a workgroup of the forward takes for these sizes, 128 where
+ *   it loads its keys once for all of them, 32 where waves share the keys.
  */
+int tpo_attention_fwd_rows(int dtype, int64_t B, int64_t Tq, int64_t Tk, int64_t Hq,
+                           int64_t Hk, int64_t D);
 int64_t tpo_attention_fwd_workspace_size(int dtype, int64_t B, int64_t Tq, int64_t Tk,
                                          int64_t Hq, int64_t Hk, int64_t D);
 int tpo_attention_fwd(int dtype, const void* q, const void* k, const void* v,

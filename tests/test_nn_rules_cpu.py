@@ -68,3 +68,28 @@ def test_attention_backward_of_some(tpo, lib):
                 q, q, k, k, q, lse, torch.empty(0), o, o, None, None, True, 1.0, mask)
             assert [t.shape for t in g] == [t.shape if on else (0,)
                                             for t, on in zip((q, k, k), mask)]
+
+
+def test_attention_kernels_of_the_gpu_tests(tpo, lib):
+    """Which kernel the sizes of tests/test_attention_more_gpu.py take, so that no change of
+    the rule leaves one of them without its tests."""
+    from tests import test_attention_more_gpu as t
+
+    lib.tpo_attention_fwd_rows.argtypes = [ctypes.c_int] + [I] * 6
+
+    def rows(dtype, lens_q, lens_k, Hq, Hk, D, more=(0, 0)):
+        return lib.tpo_attention_fwd_rows(dtype, len(lens_q), sum(lens_q) + more[0],
+                                          sum(lens_k) + more[1], Hq, Hk, D)
+
+    for dtype in (0, 2, 3):
+        for Hq, Hk in t.PROMPT_HEADS:
+            for D in (40, 64, 128):
+                assert rows(dtype, t.PROMPT, t.PROMPT, Hq, Hk, D) == 128
+            assert rows(dtype, t.ROOMS_Q, t.ROOMS_K, Hq, Hk, 32, (10, 7)) == 128
+        assert [rows(dtype, lens, lens, Hq, Hk, D) for lens, Hq, Hk, D in t.SCALED] == [32, 32, 128]
+        for B in (61, 62, 63, 64, 65):
+            for lens in (t._mixed(B, 40), t._mixed(B, 150)):
+                many = lens == t._mixed(B, 150)
+                assert rows(dtype, lens, lens, *((16, 8) if many else (4, 2)), 32,
+                            (3, 3)) == (128 if many else 32)
+    assert rows(0, [4], [4], 3, 2, 16) == -1 and rows(1, [4], [4], 2, 2, 16) == -2

@@ -486,6 +486,12 @@ extern "C" int64_t tpo_attention_fwd_workspace_size(int dtype, int64_t B, int64_
   return round_up(Tq * Hq * w.shares * D * 4, 256) + round_up(Tq * Hq * w.shares * 8, 256);
 }
 
+extern "C" int tpo_attention_fwd_rows(int dtype, int64_t B, int64_t Tq, int64_t Tk, int64_t Hq,
+                                      int64_t Hk, int64_t D) {
+  if (int rc = attn_check("attention_fwd_rows", dtype, B, Tq, Tk, Hq, Hk, D)) return rc;
+  return attn_way(dtype, B, Tq, Tk, Hq, Hk, D).rows;
+}
+
 extern "C" int tpo_attention_fwd(int dtype, const void* q, const void* k, const void* v,
                                  const int64_t* offsets_q, const int64_t* offsets_k,
                                  const int64_t* lengths_q, const int64_t* lengths_k, int64_t B,
