@@ -381,9 +381,12 @@ int tpo_layer_norm_bwd(int dtype, int wdtype, const void* grad_y, const void* x,
  *   more exact backward; of no use with F32.
  *   Pointers, heads (D values) and strides are multiples of 16 bytes, a row's
  *   stride is 16 to 2^25 bytes.
+ *   B <= 2^24, Hq <= 1024, Tq Hq and Tk Hk < 2^31.
  *   A NaN or an infinity in v reaches the rows that see it and, by 0 times it,
  *   earlier rows of the sequence that share a tile of 64 keys with it; it
- *   reaches no row of another sequence, and rows not in use are not read.
+ *   reaches no row of another sequence, and rows not in use are not read.  In
+ *   the backward one in q, k or grad_out likewise reaches gradients of keys and
+ *   rows of its tile that do not see each other.
  * tpo_attention_bwd: grad_out, out, rest and the gradients are contiguous.  Every
  *   row of grad_q, grad_k, grad_v is written, rows not in use with 0; sums
  *   run in a fixed order.  grad_q, or grad_k and grad_v together, may be NULL and
@@ -420,8 +423,9 @@ int tpo_attention_bwd(int dtype, const void* grad_out, const void* q, const void
 
 /*
  * Gated projection: h = act(x w_gate^T) * (x w_up^T).
- *   x (M,K), w_gate and w_up (F,K), h (M,F); activation is a TPO_ACT_* code
- *   (GELU is x times the normal distribution function, by erf).
+ *   x (M,K), w_gate and w_up (F,K), h (M,F), M <= 2^22, 1 <= K <= 2^20,
+ *   F <= 2^20; activation is a TPO_ACT_* code (GELU is x times the normal
+ *   distribution function, by erf).
  * tpo_gated_bwd: grad_h (M,F) -> grad_x (M,K), grad_w_gate and grad_w_up
  *   (F,K).  The gradients at the projections are rounded to `dtype` between
  *   the products.  grad_x, or the two weights' gradients together, may be NULL

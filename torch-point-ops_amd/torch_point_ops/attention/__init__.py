@@ -47,9 +47,11 @@ def packed_attention(q, k, v, offsets_q, offsets_k=None, lengths_q=None, lengths
       scale: None for D ** -0.5.
 
     Returns (Tq, Hq, D) of q's type; rows that are not in use or see no key are 0.
-    Differentiable in q, k and v, with sums in a fixed order.  Scores, their statistics and
-    all sums are float32; half and bfloat16 probabilities (and the scores' gradients) are
-    rounded to the type for the products.  Under torch.autocast q, k and v are taken in its
+    Differentiable once, in reverse mode, in q, k and v, with sums in a fixed order; only the
+    gradients that are asked for are computed (k's and v's by one kernel).  Scores, their
+    statistics and all sums are float32; half and bfloat16 probabilities (and the scores'
+    gradients, which float16 holds from 6e-8 on: scale the loss) are rounded to the type for
+    the products.  Under torch.autocast q, k and v are taken in its
     type.
     """
     if offsets_k is None:

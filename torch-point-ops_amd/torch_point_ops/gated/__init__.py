@@ -37,7 +37,7 @@ def gated_projection(x, w_gate, w_up, activation="silu"):
 
     Args: x (..., K), w_gate and w_up (F, K), float32, float16 or bfloat16; activation
     "silu", "gelu" (x times the normal distribution function), "relu" or "sigmoid".
-    Differentiable in x and the weights.  A float32 forward keeps the two projections for
+    Differentiable once, in reverse mode, in x and the weights.  A float32 forward keeps the two projections for
     the backward; for the half types the backward computes them again, which takes less
     time than unrounded ones take through memory, and rounds the gradients at them to x's
     type between the products.  All sums are float32.  Under torch.autocast the inputs

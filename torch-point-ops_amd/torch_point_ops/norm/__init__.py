@@ -34,8 +34,8 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
 
     Args: x (..., C) float32, float16 or bfloat16; weight, bias (C) of x's type
     or float32, or None; eps >= 0.  Sums are taken in float32 whatever x's type.
-    Differentiable in x, weight and bias; the weights' gradients are summed in a
-    fixed order.  Returns a tensor of x's shape and type.
+    Differentiable once, in reverse mode, in x, weight and bias; the weights' gradients
+    are summed in a fixed order.  C is at most 2^20.  Returns a tensor of x's shape and type.
     """
     return torch.ops.torch_point_ops_norm.layer_norm(x, weight, bias, eps)
 
