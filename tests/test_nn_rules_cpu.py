@@ -93,3 +93,36 @@ def test_attention_kernels_of_the_gpu_tests(tpo, lib):
                 assert rows(dtype, lens, lens, *((16, 8) if many else (4, 2)), 32,
                             (3, 3)) == (128 if many else 32)
     assert rows(0, [4], [4], 3, 2, 16) == -1 and rows(1, [4], [4], 2, 2, 16) == -2
+
+
+def test_missing_arrays_are_refused(lib):
+    """A NULL for an array that a call would read or write is an error of the call."""
+    P, C, D = ctypes.c_void_p, ctypes.c_int, ctypes.c_double
+    lib.tpo_last_error.restype = ctypes.c_char_p
+    lib.tpo_layer_norm_fwd.argtypes = [C, C, P, P, P, I, I, D, P, P, P, P]
+    lib.tpo_layer_norm_bwd.argtypes = [C, C, P, P, P, P, P, I, I, D, P, P, P, P, I, P]
+    lib.tpo_attention_fwd.argtypes = [C] + [P] * 7 + [I] * 12 + [C, D, P, P, P, P, I, P]
+    lib.tpo_attention_bwd.argtypes = [C] + [P] * 11 + [I] * 12 + [C, D, P, P, P, P, I, P]
+    lib.tpo_gated_fwd.argtypes = [C, P, P, P, I, I, I, C, P, P, P, I, P]
+    lib.tpo_gated_bwd.argtypes = [C, P, P, P, P, P, I, I, I, C, P, P, P, P, I, P]
+    f = P(4096)  # never dereferenced
+    sizes = [1, 4, 4, 2, 2, 16, *[32, 16] * 3, 1, 1.0]
+
+    def refused(entry, args, needed):
+        for at in needed:
+            a = list(args)
+            a[at] = None
+            assert entry(*a) == -1, at
+            assert b"NULL" in lib.tpo_last_error()
+
+    refused(lib.tpo_layer_norm_fwd, [0, 0, f, f, f, 4, 8, 1e-5, f, None, None, None], (2, 8))
+    refused(lib.tpo_layer_norm_bwd,
+            [0, 0, f, f, f, f, f, 4, 8, 1e-5, f, None, None, None, 0, None], (2, 3, 5, 6))
+    refused(lib.tpo_attention_fwd,
+            [0, f, f, f, f, f, None, None, *sizes, f, None, None, None, 0, None], (1, 2, 3, 4, 5, 22))
+    refused(lib.tpo_attention_bwd,
+            [0, f, f, f, f, f, f, f, f, f, None, None, *sizes, f, None, None, None, 0, None],
+            (1, 2, 3, 4, 5, 7, 8, 9))
+    refused(lib.tpo_gated_fwd, [0, f, f, f, 4, 8, 8, 0, f, None, None, 0, None], (1, 2, 3, 8))
+    refused(lib.tpo_gated_bwd, [0, f, f, f, f, None, 4, 8, 8, 0, f, f, f, f, 1 << 30, None],
+            (1, 2, 3, 4))

@@ -503,6 +503,9 @@ extern "C" int tpo_attention_fwd(int dtype, const void* q, const void* k, const 
                                  void* stream) {
   if (int rc = attn_check("attention_fwd", dtype, B, Tq, Tk, Hq, Hk, D)) return rc;
   if (Tq == 0) return TPO_OK;
+  if (int rc = all_there("attention_fwd", {q, offsets_q, offsets_k, out})) return rc;
+  if (Tk > 0)
+    if (int rc = all_there("attention_fwd", {k, v})) return rc;
   if (int rc = attn_layout("attention_fwd", dtype, D, {q, k, v, out, rest, workspace},
                            {q_row, q_head, k_row, k_head, v_row, v_head}, {q_row, k_row, v_row}))
     return rc;

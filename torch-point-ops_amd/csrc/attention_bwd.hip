@@ -444,6 +444,11 @@ extern "C" int tpo_attention_bwd(int dtype, const void* grad_out, const void* q,
     return set_error(TPO_ERR_WORKSPACE, "attention_bwd: workspace of %lld bytes needed",
                      (long long)need);
   if ((Tq == 0 && Tk == 0) || (!grad_q && !grad_k)) return TPO_OK;
+  if (int rc = all_there("attention_bwd", {offsets_q, offsets_k})) return rc;
+  if (Tq > 0)
+    if (int rc = all_there("attention_bwd", {grad_out, q, out, lse})) return rc;
+  if (Tk > 0)
+    if (int rc = all_there("attention_bwd", {k, v})) return rc;
   if (int rc = attn_layout("attention_bwd", dtype, D,
                            {grad_out, q, k, v, out, rest, grad_q, grad_k, grad_v, workspace},
                            {q_row, q_head, k_row, k_head, v_row, v_head}, {q_row, k_row, v_row}))

@@ -644,6 +644,7 @@ extern "C" int tpo_gated_fwd(int dtype, const void* x, const void* w_gate, const
                              void* keep, void* workspace, int64_t workspace_bytes, void* stream) {
   if (int rc = gated_check("gated_fwd", dtype, M, K, F, activation)) return rc;
   if (M == 0 || F == 0) return TPO_OK;
+  if (int rc = all_there("gated_fwd", {x, w_gate, w_up, h})) return rc;
   if (int rc = gated_aligned("gated_fwd", {x, w_gate, w_up, workspace})) return rc;
   if (keep && dtype != TPO_F32)
     return set_error(TPO_ERR_ARG, "gated_fwd: only float projections are kept");
@@ -682,6 +683,8 @@ extern "C" int tpo_gated_bwd(int dtype, const void* grad_h, const void* x, const
   hipStream_t s = (hipStream_t)stream;
   char* ws = (char*)workspace;
   if (M == 0 && F == 0) return TPO_OK;
+  if (M > 0 && F > 0)
+    if (int rc = all_there("gated_bwd", {grad_h, x, w_gate, w_up})) return rc;
   if (kept && dtype != TPO_F32)
     return set_error(TPO_ERR_ARG, "gated_bwd: only float projections are kept");
   with_element(dtype, [&](auto t) {

@@ -484,6 +484,8 @@ extern "C" int tpo_layer_norm_fwd(int dtype, int wdtype, const void* x, const vo
   if (int rc = ln_check("layer_norm_fwd", rows, width)) return rc;
   if ((mean == nullptr) != (rstd == nullptr))
     return set_error(TPO_ERR_ARG, "layer_norm_fwd: mean and rstd go together");
+  if (rows > 0)
+    if (int rc = all_there("layer_norm_fwd", {x, y})) return rc;
   hipStream_t s = (hipStream_t)stream;
   bool none = false;
   const int rc = ln_dispatch("layer_norm_fwd", dtype, wdtype, [&](auto t, auto w) {
@@ -528,6 +530,8 @@ extern "C" int tpo_layer_norm_bwd(int dtype, int wdtype, const void* grad_y, con
                (!workspace && rows > 0)))
     return set_error(TPO_ERR_WORKSPACE, "layer_norm_bwd: workspace of %lld bytes needed",
                      (long long)tpo_layer_norm_bwd_workspace_size(rows, width));
+  if (rows > 0)
+    if (int rc = all_there("layer_norm_bwd", {grad_y, x, mean, rstd})) return rc;
   hipStream_t s = (hipStream_t)stream;
   const int rc = ln_dispatch("layer_norm_bwd", dtype, wdtype, [&](auto t, auto w) {
     typedef decltype(t) T;

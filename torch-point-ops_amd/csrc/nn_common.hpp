@@ -6,6 +6,8 @@
 // an output is rounded to its type once.
 #pragma once
 
+#include <initializer_list>
+
 #include "tpo_common.hpp"
 
 namespace tpo {
@@ -39,6 +41,12 @@ inline bool with_element(int dtype, F&& f) {
     case TPO_BF16: f(bf16_t()); return true;
     default: return false;
   }
+}
+// An error where one of the arrays that a call reads or writes is missing.
+inline int all_there(const char* op, std::initializer_list<const void*> arrays) {
+  for (const void* p : arrays)
+    if (!p) return set_error(TPO_ERR_ARG, "%s: an array is NULL", op);
+  return TPO_OK;
 }
 inline int64_t element_bytes(int dtype) { return dtype == TPO_F32 ? 4 : 2; }
 inline int64_t round_up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
