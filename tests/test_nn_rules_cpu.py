@@ -95,6 +95,24 @@ def test_attention_kernels_of_the_gpu_tests(tpo, lib):
     assert rows(0, [4], [4], 3, 2, 16) == -1 and rows(1, [4], [4], 2, 2, 16) == -2
 
 
+def test_launches_stay_below_their_threads(lib):
+    """A launch has fewer than 2^32 threads along an axis: more rows are an error of the call."""
+    P, C, D = ctypes.c_void_p, ctypes.c_int, ctypes.c_double
+    lib.tpo_last_error.restype = ctypes.c_char_p
+    lib.tpo_attention_fwd.argtypes = [C] + [P] * 7 + [I] * 12 + [C, D, P, P, P, P, I, P]
+    lib.tpo_attention_bwd.argtypes = [C] + [P] * 11 + [I] * 12 + [C, D, P, P, P, P, I, P]
+    f = P(4096)  # never dereferenced
+    B, T, H = 1 << 20, 1 << 20, 16
+    assert lib.tpo_attention_fwd_rows(2, B, T, T, H, H, 16) == 128
+    assert lib.tpo_attention_fwd(2, f, f, f, f, f, None, None, B, T, T, H, H, 16, *[256, 16] * 3, 1,
+                                 1.0, f, None, None, None, 0, None) == -1
+    assert b"too many rows" in lib.tpo_last_error()
+    T = 1 << 26
+    assert lib.tpo_attention_bwd(2, f, f, f, f, f, None, f, f, f, None, None, 1, T, 64, H, H, 16,
+                                 *[256, 16] * 3, 1, 1.0, f, None, None, None, 0, None) == -1
+    assert b"too many rows" in lib.tpo_last_error()
+
+
 def test_missing_arrays_are_refused(lib):
     """A NULL for an array that a call would read or write is an error of the call."""
     P, C, D = ctypes.c_void_p, ctypes.c_int, ctypes.c_double

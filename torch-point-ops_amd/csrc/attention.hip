@@ -517,7 +517,7 @@ extern "C" int tpo_attention_fwd(int dtype, const void* q, const void* k, const 
                                q_row, q_head, k_row, k_head, v_row, v_head, causal, scale);
   const Way w = attn_way(dtype, B, Tq, Tk, Hq, Hk, D);
   const int64_t G = Hq / Hk, places = attn_places(Tq, G, B, w.rows);
-  if (places * Hk >= ((int64_t)1 << 31) || Hk > 65535)
+  if ((w.rows == 128 ? places * Hk : places) >= AT_GRID)
     return set_error(TPO_ERR_ARG, "attention_fwd: too many rows");
   hipStream_t s = (hipStream_t)stream;
   float* part = (float*)workspace;

@@ -28,6 +28,9 @@ struct AttnArgs {
   float scale;
 };
 
+// Workgroups of 256 along one axis of a launch: it takes fewer than 2^32 threads there.
+constexpr int64_t AT_GRID = (int64_t)1 << 24;
+
 // The rows of a packed batch in tiles of `tile`: sequence s begins at tile
 // start(s) G / tile + s.  That leaves room for each sequence's tiles (the last
 // one of a sequence and the first of the next may meet in one place, hence + s)

@@ -457,7 +457,7 @@ extern "C" int tpo_attention_bwd(int dtype, const void* grad_out, const void* q,
                                q_row, q_head, k_row, k_head, v_row, v_head, causal, scale);
   const int64_t G = Hq / Hk;
   const int64_t places_q = attn_places(Tq, G, B, 64), places_k = attn_places(Tk, 1, B, 64);
-  if (places_q * Hk >= ((int64_t)1 << 31) || places_k * Hk >= ((int64_t)1 << 31))
+  if (places_q * Hk >= AT_GRID || (grad_k && places_k * Hk >= AT_GRID))
     return set_error(TPO_ERR_ARG, "attention_bwd: too many rows");
   const int64_t stats = round_up(Tq * Hq * 4, 256);
   float* sub = grad_k ? (float*)workspace : nullptr;
