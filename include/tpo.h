@@ -1,7 +1,8 @@
 /*
  * tpo.h -- C ABI of libtpo_hip.so, the MI355X (gfx950) kernels behind the
  * torch_point_ops operators chamfer / knn / fps / gather_points / emd and the
- * transformer operators layer norm / packed attention / gated projection.
+ * transformer operators layer norm / packed attention / gated projection /
+ * rotary positions / 8-bit cache.
  *
  * Conventions for every entry point:
  *   - all pointers are device pointers (hipMalloc / torch CUDA-device tensors)
@@ -32,7 +33,8 @@ enum {
   TPO_F32 = 0,
   TPO_F64 = 1,
   TPO_F16 = 2,
-  TPO_BF16 = 3
+  TPO_BF16 = 3,
+  TPO_I64 = 4 /* of places (tpo_rotary, tpo_cache_append) only */
 };
 
 enum {
@@ -452,6 +454,80 @@ int tpo_gated_bwd(int dtype, const void* grad_h, const void* x, const void* w_ga
                   const void* w_up, const void* kept, int64_t M, int64_t K, int64_t F,
                   int activation, void* grad_x, void* grad_w_gate, void* grad_w_up, void* workspace,
                   int64_t workspace_bytes, void* stream);
+
+/*
+ * Rotary positions: pairs of a head's values turned by angles that grow with a
+ * token's place.
+ *   y1 = m (x1 cos a - x2 sin a), y2 = m (x2 cos a + x1 sin a), a = place f_j,
+ *   pair j being values j and j + pairs of a head (interleaved: 2 j and
+ *   2 j + 1), m the amplitude; the D - 2 pairs values behind stay as they are.
+ *   x (tokens,heads,D) strided: x_row and x_head are the strides, in elements,
+ *   of a token and of a head; the D values of a head are contiguous.  y
+ *   contiguous, not x.  Any alignment.  1 <= D <= 512, heads <= 2^16.
+ *   places (tokens,axes) of places_dtype (I64 or F32), frequencies (pairs)
+ *   double: pair j goes by axis j / (pairs / axes).  Angles are taken in 64 bits;
+ *   those beyond 2^45 give NaN.
+ *   back: the angles' signs turned, which makes it the gradient.
+ */
+int tpo_rotary(int dtype, const void* x, int64_t tokens, int64_t heads, int64_t D,
+               int64_t x_row, int64_t x_head, const void* places, int places_dtype,
+               int64_t axes, const double* frequencies, int64_t pairs, int interleaved,
+               double amplitude, int back, void* y, void* stream);
+
+/*
+ * A cache of keys and values in pages of 8-bit codes (e4m3: 448 the largest, no
+ * infinities), Dr being D rounded up to 16:
+ *   keys (pages,Hk,page/32,Dr/16,32,16), values (pages,Hk,page/32,Dr,32),
+ *   key_scales and value_scales (pages,Hk) float, positive: a value is its code
+ *   times the scale of its page and head; 16-byte aligned.
+ *   table (B,M) int32: the pages of each sequence in order.  An entry outside of
+ *   [0, pages) is a page that is not there: nothing is written to it, and its
+ *   places are not seen.  lengths (B) int64: the tokens of each sequence, those
+ *   that a call brings included, clamped to M page.
+ *   page is 32 to 256 in steps of 32, 1 <= D <= 128, M page < 2^31.
+ * The rows of a call (T) belong to the sequences as those of the packed
+ * attention do: offsets (B + 1) int64, lengths_new or lengths_q (B) int64 or
+ * NULL.  The n rows of a sequence that are in use are its last n tokens.
+ *
+ * tpo_cache_append puts k and v (T,Hk,D) into the pages, k turned by its places
+ *   as tpo_rotary turns (pairs = 0: as it is) in 64 bits and rounded once.  places
+ *   (T,axes) or NULL for the tokens' own places in their sequences.  Scales are
+ *   powers of two, 2^-40 to 2^40, the smallest with every value of the page at
+ *   most 448 times it: a page whose first token is new gets its own, one that
+ *   holds older tokens keeps its scale or, where a new token needs it, grows, and
+ *   its older codes are rounded to the new one.  What is not finite becomes the
+ *   code for NaN, what is beyond 448 2^40 that value.  No two sequences of a call
+ *   may write to one page.  Nothing but the new tokens' codes, the codes before
+ *   them in a page whose scale grows, and the scales of these pages is written.
+ *   q (T,Hq,D) or NULL: turned likewise into q_out (T,Hq,D) contiguous, of
+ *   k's type; rows not in use are 0.
+ * tpo_cache_attention: softmax(scale q k^T) v over the cache, into out (T,Hq,D)
+ *   contiguous.  Causal: row i of a sequence's n sees place j where
+ *   j <= i + length - n.  Rows not in use, and rows that see no key, are 0.
+ *   What lies behind a sequence's last token is read but never counts, whatever
+ *   it holds.  q as the packed attention takes it.
+ * Workspaces are 256-byte aligned; size 0 means none is used.
+ */
+int tpo_cache_append(int dtype, const void* k, const void* v, const void* q,
+                     const int64_t* offsets, const int64_t* lengths_new, int64_t B,
+                     int64_t T, int64_t Hq, int64_t D, int64_t k_row, int64_t k_head,
+                     int64_t v_row, int64_t v_head, int64_t q_row, int64_t q_head,
+                     const void* places, int places_dtype, int64_t axes,
+                     const double* frequencies, int64_t pairs, int interleaved,
+                     double amplitude, void* keys, void* values, float* key_scales,
+                     float* value_scales, const int32_t* table, const int64_t* lengths,
+                     int64_t pages, int64_t Hk, int64_t page, int64_t Dr, int64_t M,
+                     void* q_out, void* stream);
+int64_t tpo_cache_attention_workspace_size(int dtype, int64_t B, int64_t T, int64_t Hq,
+                                           int64_t Hk, int64_t D, int64_t page, int64_t M);
+int tpo_cache_attention(int dtype, const void* q, const int64_t* offsets,
+                        const int64_t* lengths_q, int64_t B, int64_t T, int64_t Hq,
+                        int64_t D, int64_t q_row, int64_t q_head, const void* keys,
+                        const void* values, const float* key_scales,
+                        const float* value_scales, const int32_t* table,
+                        const int64_t* lengths, int64_t pages, int64_t Hk, int64_t page,
+                        int64_t Dr, int64_t M, int causal, double scale, void* out,
+                        void* workspace, int64_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -26,7 +26,7 @@ INCLUDE = os.path.join(REPO, "include")
 ROCM = os.environ.get("ROCM_PATH", "/opt/rocm")
 ARCH = "gfx950"
 
-HIP_SOURCES = ["capi.hip", "chamfer.hip", "chamfer_grid.hip", "knn.hip", "knn_hd.hip", "knn_bwd.hip", "knn_grid.hip", "knn_near.hip", "knn_feat.hip", "knn_redo.hip", "knn_bf16.hip", "fps.hip", "gather.hip", "emd.hip", "layer_norm.hip", "attention.hip", "attention_bwd.hip", "gated.hip"]
+HIP_SOURCES = ["capi.hip", "chamfer.hip", "chamfer_grid.hip", "knn.hip", "knn_hd.hip", "knn_bwd.hip", "knn_grid.hip", "knn_near.hip", "knn_feat.hip", "knn_redo.hip", "knn_bf16.hip", "fps.hip", "gather.hip", "emd.hip", "layer_norm.hip", "attention.hip", "attention_bwd.hip", "gated.hip", "rotary.hip", "cache_append.hip", "cache_attention.hip"]
 
 HIPCC_FLAGS = [
     f"--offload-arch={ARCH}",
@@ -84,7 +84,7 @@ def build_hip_lib(jobs: int = 8, verbose: bool = False) -> str:
     return out
 
 
-SHIM_SOURCES = ["torch_ops.cpp", "nn_ops.cpp", "cpu_ops.cpp"]
+SHIM_SOURCES = ["torch_ops.cpp", "nn_ops.cpp", "cache_ops.cpp", "cpu_ops.cpp"]
 
 
 def build_torch_shim(jobs: int = 8, verbose: bool = False) -> str:

@@ -420,6 +420,61 @@ __device__ __forceinline__ f32x16 scores(const HeadLanes<T, DP>& x, const char* 
   return s;
 }
 
+// The shares' sums of each row together: a workgroup a row.  A lane weighs a share
+// (there are at most 64), the waves add every fourth one's values, four loads
+// under way at a time.
+template <typename T>
+__global__ __launch_bounds__(256) void attn_join_kernel(const float* __restrict__ part,
+                                                        const float2* __restrict__ ml, int shares,
+                                                        int Hq, int64_t Tq, int D,
+                                                        T* __restrict__ out,
+                                                        float* __restrict__ lse,
+                                                        T* __restrict__ rest) {
+  __shared__ float s[4][AT_DMAX];
+  const int64_t at = blockIdx.x;
+  const int l = lane_id(), w = wave_id();
+  const float2 mine = l < shares ? ml[at * shares + l] : make_float2(0.f, 0.f);
+  const bool has = mine.y != 0.f;  // a share without keys has written no values
+  const float m = wave_max(has ? mine.x : NEG_INF);
+  const float f = has ? __builtin_amdgcn_exp2f(mine.x - m) : 0.f;
+  const float total = wave_sum(f * mine.y);
+  const uint64_t there = __builtin_amdgcn_ballot_w64(has);
+  const float* p = part + at * shares * D;
+  const int d1 = l + 64;
+  float o[2] = {0.f, 0.f};
+  for (int i = w; i < shares; i += 16) {
+    float x[4][2];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int k = i + 4 * j;
+      const bool in = k < shares && (there >> k & 1);
+      x[j][0] = in && l < D ? p[(int64_t)k * D + l] : 0.f;
+      x[j][1] = in && d1 < D ? p[(int64_t)k * D + d1] : 0.f;
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float g = __shfl(f, (i + 4 * j) & 63);
+      const bool in = i + 4 * j < shares && (there >> (i + 4 * j) & 1);
+      if (in) o[0] = __builtin_fmaf(g, x[j][0], o[0]);
+      if (in) o[1] = __builtin_fmaf(g, x[j][1], o[1]);
+    }
+  }
+  s[w][l] = o[0];
+  s[w][l + 64] = o[1];
+  __syncthreads();
+  const int d = threadIdx.x;
+  if (d < D) {
+    const float inv = total != 0.f ? 1.f / total : 0.f;
+    const float y = ((s[0][d] + s[1][d]) + (s[2][d] + s[3][d])) * inv;
+    const T z = (T)y;
+    out[at * D + d] = z;
+    if (rest) rest[at * D + d] = (T)(y - (float)z);
+  }
+  if (lse && d == 0)
+    lse[(at % Hq) * Tq + at / Hq] =
+        total == 0.f ? NEG_INF : (m + __builtin_amdgcn_logf(total)) * LN2;
+}
+
 int attn_check(const char* op, int dtype, int64_t B, int64_t Tq, int64_t Tk, int64_t Hq,
                int64_t Hk, int64_t D);
 int attn_layout(const char* op, int dtype, int64_t D, std::initializer_list<const void*> p,

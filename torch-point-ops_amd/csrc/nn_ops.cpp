@@ -2,39 +2,10 @@
 // (torch_point_ops_norm, torch_point_ops_attention, torch_point_ops_gated),
 // which the reference does not have.  Validation, allocation and autograd as
 // torch_ops.cpp does them; the kernels are libtpo_hip.so's.
-#include "shim_common.hpp"
-
-#include <ATen/autocast_mode.h>
-#include <torch/csrc/autograd/autograd_not_implemented_fallback.h>
+#include "nn_shim.hpp"
 
 namespace torch_point_ops {
 namespace {
-
-using at::Tensor;
-using torch::autograd::AutogradContext;
-using torch::autograd::variable_list;
-typedef std::optional<Tensor> OptTensor;
-
-int nn_dtype(const Tensor& t, const char* op) {
-  switch (t.scalar_type()) {
-    case at::kFloat: return TPO_F32;
-    case at::kHalf: return TPO_F16;
-    case at::kBFloat16: return TPO_BF16;
-    default:
-      TORCH_CHECK(false, op, " not implemented for '", t.scalar_type(), "'");
-  }
-  return -1;
-}
-
-Tensor workspace(int64_t bytes, const Tensor& like, const char* op) {
-  TORCH_CHECK(bytes >= 0, op, ": ", tpo_last_error());
-  return bytes > 0 ? at::empty({bytes}, like.options().dtype(at::kByte)) : Tensor();
-}
-void* data_or_null(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
-Tensor get(const OptTensor& t) { return t.has_value() ? *t : Tensor(); }
-OptTensor opt(const Tensor& t) { return t.defined() ? OptTensor(t) : std::nullopt; }
-// the place of a result that was not asked for
-Tensor nothing(const Tensor& like) { return at::empty({0}, like.options()); }
 
 // --------------------------------------------------------------- layer norm
 int ln_weight_dtype(const Tensor& x, const Tensor& w, const char* name, const char* op) {
@@ -181,21 +152,6 @@ struct Packed {  // checked arguments of an attention call
   int dt;
 };
 
-// The distance of rows and of heads, also where there is one of them only.
-int64_t row_stride(const Tensor& t) { return t.size(0) > 1 ? t.stride(0) : t.size(1) * t.size(2); }
-int64_t head_stride(const Tensor& t) { return t.size(1) > 1 ? t.stride(1) : t.size(2); }
-
-// q, k and v may be slices (of one projection, say) or broadcast over heads: a
-// head's values lie together, rows and heads at any distance that keeps 16-byte
-// loads.  Others are copied, heads that are no multiple of 16 bytes padded.
-Tensor head_rows(const Tensor& t, int64_t D) {
-  const int64_t z = t.element_size();
-  if (t.size(2) != D) return at::constant_pad_nd(t, {0, D - t.size(2)}).contiguous();
-  const bool ok = (D == 1 || t.stride(2) == 1) && row_stride(t) > 0 && row_stride(t) * z % 16 == 0 &&
-                  row_stride(t) * z < (1 << 25) && head_stride(t) * z % 16 == 0;
-  return aligned16(ok ? t : t.contiguous());
-}
-
 Packed packed_args(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& oq,
                    const Tensor& ok, const OptTensor& lq, const OptTensor& lk, const char* op) {
   check_hip(q, "q");
@@ -241,11 +197,6 @@ Packed packed_args(const Tensor& q, const Tensor& k, const Tensor& v, const Tens
   p.Hq = q.size(1);
   p.Hk = k.size(1);
   return p;
-}
-
-// The first D values of each head of a result.
-Tensor cut_heads(const Tensor& t, int64_t D) {
-  return t.size(2) == D ? t : t.narrow(2, 0, D).contiguous();
 }
 
 std::tuple<Tensor, Tensor, Tensor> packed_attention_hip(const Tensor& q, const Tensor& k, const Tensor& v,
@@ -516,9 +467,6 @@ Tensor gated_projection_autograd(const Tensor& x, const Tensor& wg, const Tensor
 
 // Under autocast the two operators that are products take its type, as torch's own
 // products do; layer norm takes x and weights of different types as they are.
-Tensor autocast(const Tensor& t) {
-  return at::autocast::cached_cast(at::autocast::get_autocast_dtype(at::kCUDA), t, at::kCUDA);
-}
 Tensor packed_attention_autocast(const Tensor& q, const Tensor& k, const Tensor& v,
                                  const Tensor& oq, const Tensor& ok, const OptTensor& lq,
                                  const OptTensor& lk, bool causal, double scale) {
@@ -531,10 +479,6 @@ Tensor gated_projection_autocast(const Tensor& x, const Tensor& wg, const Tensor
   c10::impl::ExcludeDispatchKeyGuard below(c10::DispatchKey::AutocastCUDA);
   return gated_projection_op().call(autocast(x), autocast(wg), autocast(wu), act);
 }
-
-// The operators that the functions above call have no formula of their own: a
-// gradient of a gradient, or a tangent, is refused instead of left out.
-torch::CppFunction no_formula() { return torch::autograd::autogradNotImplementedFallback(); }
 
 // There are no CPU kernels: as Chamfer and EMD, a call says so.
 Tensor layer_norm_cpu(const Tensor&, const OptTensor&, const OptTensor&, double) {

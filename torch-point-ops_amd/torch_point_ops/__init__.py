@@ -4,7 +4,8 @@ Drop-in for the reference package's nearest-neighbour path: the same module
 layout, functions, nn.Modules and torch.ops registrations
 (torch_point_ops/__init__.py:1-30 of the reference), backed by the HIP
 kernels of libtpo_hip.so; beyond the reference, the operators of a transformer
-over point patches (norm, attention, gated).  Importing fails loudly when the native extension
+over point patches (norm, attention, gated,
+rotary, cache).  Importing fails loudly when the native extension
 (_C.so / libtpo_hip.so) is missing; there is no fallback path.
 """
 import torch  # noqa: F401  (loads libc10 / libtorch before the extension)
@@ -26,6 +27,8 @@ from .fps import (
 from .norm import LayerNorm, layer_norm
 from .attention import PackedAttention, packed_attention
 from .gated import GatedFeedForward, gated_projection
+from .rotary import RotaryPositions, rotary_frequencies, rotary_positions
+from .cache import PagedCache, cache_append, cached_attention
 
 __all__ = [
     "ChamferDistance",
@@ -50,4 +53,10 @@ __all__ = [
     "packed_attention",
     "GatedFeedForward",
     "gated_projection",
+    "RotaryPositions",
+    "rotary_frequencies",
+    "rotary_positions",
+    "PagedCache",
+    "cache_append",
+    "cached_attention",
 ]
