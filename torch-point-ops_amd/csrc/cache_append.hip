@@ -7,6 +7,8 @@
 // value is exact in every type, and older codes of a page whose scale grows stay as they are but
 // for those that become subnormal.  Values that are not finite become the code for NaN and do
 // not count for the scale.
+#include <type_traits>
+
 #include "cache.hpp"
 #include "rotary.hpp"
 
@@ -55,8 +57,11 @@ __device__ __forceinline__ uint32_t codes4(float a, float b, float c, float d) {
   int r = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
   return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, r, true);
 }
-__device__ __forceinline__ uint32_t codes4(const float* v, float f) {
-  return codes4(for_code(v[0], f), for_code(v[1], f), for_code(v[2], f), for_code(v[3], f));
+// rare: values that are not finite, or a scale that is as large as it gets
+__device__ __forceinline__ uint32_t codes4(const float* v, float f, bool rare) {
+  if (rare)
+    return codes4(for_code(v[0], f), for_code(v[1], f), for_code(v[2], f), for_code(v[3], f));
+  return codes4(v[0] * f, v[1] * f, v[2] * f, v[3] * f);
 }
 // Four codes brought to another scale.
 __device__ __forceinline__ uint32_t codes_times(uint32_t x, float f) {
@@ -74,79 +79,133 @@ struct AppendRows {
   int Hq, D, places;  // places: the turn's places are given, not the tokens' own
 };
 
-// Sixteen values from p on, n of them there.
+// A lane's part of a token's key or value: two pieces of eight values, from pa and from pb on.
+// Keys that are turned: eight pairs (halves: the pieces lie n apart; interleaved: side by side);
+// the others sixteen values side by side.  load: how many are there, store: how many the cache
+// has (those behind D are 0).
+struct Part {
+  int pa, pb, load_a, load_b, store_a, store_b, pair;  // pair: the first, -1: not turned
+
+  static __device__ __forceinline__ int upto8(int n) { return n < 0 ? 0 : (n > 8 ? 8 : n); }
+  __device__ __forceinline__ void plain(int from, int D, int Dr) {
+    pa = from;
+    pb = from + 8;
+    load_a = upto8(D - pa);
+    load_b = upto8(D - pb);
+    store_a = upto8(Dr - pa);
+    store_b = upto8(Dr - pb);
+    pair = -1;
+  }
+  __device__ __forceinline__ void key(int i, const Turn& t, int D, int Dr) {
+    const int turned = (t.pairs + 7) / 8;
+    if (i >= turned) {
+      plain(2 * t.pairs + 16 * (i - turned), D, Dr);
+      return;
+    }
+    pair = 8 * i;
+    pa = t.interleaved ? 16 * i : 8 * i;
+    pb = t.interleaved ? 16 * i + 8 : t.pairs + 8 * i;
+    const int n = t.pairs - pair;
+    load_a = store_a = upto8(t.interleaved ? 2 * n : n);
+    load_b = store_b = upto8(t.interleaved ? 2 * n - 8 : n);
+  }
+  // What follows from these is worked out where it is used: kept for all heads it would take
+  // 100 registers more.
+  __device__ __forceinline__ void fresh() {
+    asm volatile("" : "+v"(pa), "+v"(pb), "+v"(load_a), "+v"(load_b), "+v"(store_a), "+v"(store_b));
+  }
+  // parts of a token: of its key, and of its value
+  static __host__ __device__ __forceinline__ int of_key(int pairs, int Dr) {
+    return (pairs + 7) / 8 + (Dr - 2 * pairs + 15) / 16;
+  }
+};
+
 template <typename T>
-__device__ __forceinline__ void load16(const T* p, int n, float (&x)[16]) {
-  constexpr int PER = 16 / sizeof(T);
+struct PartValues {
+  Piece<T, 8> a, b;
+  __device__ __forceinline__ void load(const T* row, const Part& p) {
+    a = some<T, 8>(row + p.pa, p.load_a);
+    b = some<T, 8>(row + p.pb, p.load_b);
+  }
+  // sixteen values side by side to the first and the second of each pair
+  __device__ __forceinline__ void apart() {
+    PartValues o = *this;
 #pragma unroll
-  for (int i = 0; i < 16; i += PER) {
-    const Piece<T, PER> u = n - i > 0 ? some<T, PER>(p + i, n - i) : Piece<T, PER>{};
+    for (int e = 0; e < 8; ++e) {
+      a.v[e] = e < 4 ? o.a.v[2 * e & 7] : o.b.v[2 * e & 7];
+      b.v[e] = e < 4 ? o.a.v[(2 * e + 1) & 7] : o.b.v[(2 * e + 1) & 7];
+    }
+  }
+  // what was worked out of these is not kept
+  __device__ __forceinline__ void fresh() {
+    constexpr int N = sizeof(T) * 2;
+    struct Words { uint32_t w[N]; };
+    Words p = __builtin_bit_cast(Words, a), q = __builtin_bit_cast(Words, b);
 #pragma unroll
-    for (int e = 0; e < PER; ++e) x[i + e] = (float)u.v[e];
+    for (int i = 0; i < N; ++i) asm volatile("" : "+v"(p.w[i]), "+v"(q.w[i]));
+    a = __builtin_bit_cast(Piece<T, 8>, p);
+    b = __builtin_bit_cast(Piece<T, 8>, q);
+  }
+};
+
+// Eight pairs turned, x[e] and x[8 + e] being pair e.  ODD: rounded to odd; else to the nearest
+// float, which has the same code but where it lies half-way between two of them, its last 19
+// bits 0 (e4m3 keeps 3 of 23): true where one may.
+template <bool ODD, typename T>
+__device__ __forceinline__ bool turn_pairs(const PartValues<T>& u, const double2 (&cs)[8],
+                                           float (&x)[16]) {
+  uint32_t least = ~0u;
+  auto rounded = [&](double d) {
+    const float f = ODD ? to_odd(d) : (float)d;
+    const uint32_t low = __builtin_bit_cast(uint32_t, f) & 0x7ffff;
+    least = low < least ? low : least;
+    return f;
+  };
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const double v0 = (float)u.a.v[e], v1 = (float)u.b.v[e];
+    x[e] = rounded(__builtin_fma(-v1, cs[e].y, v0 * cs[e].x));
+    x[8 + e] = rounded(__builtin_fma(v0, cs[e].y, v1 * cs[e].x));
+    if (e % 2) __builtin_amdgcn_sched_barrier(0);
+  }
+  return least == 0;
+}
+template <typename T>
+__device__ __forceinline__ void turn_part(PartValues<T> u, bool interleaved,
+                                          const double2 (&cs)[8], float (&x)[16]) {
+  if (interleaved) u.apart();
+  if (turn_pairs<false>(u, cs, x)) {
+    u.fresh();
+    turn_pairs<true>(u, cs, x);
   }
 }
 
-// Values d0 .. d0 + 15 of a head turned: row, the head's D values; cs, the token's cosines and
-// sines.
-template <typename T>
-__device__ __forceinline__ void turn16(const T* row, int d0, int D, const Turn& t,
-                                       const double2* cs, float (&x)[16]) {
-  const int n = t.pairs;
-  if (d0 >= 2 * n) return;
-  if (t.interleaved) {
+// Eight codes to a key's place in a block: values d .. d + n - 1 of a token.
+__device__ __forceinline__ void store_part(uint8_t* block, int token, int d, int n, uint32_t lo,
+                                           uint32_t hi) {
+  uint8_t* to = block + token * 16;
+  if (n == 8 && d % 8 == 0) {
+    *(uint2*)(to + d / 16 * 512 + d % 16) = make_uint2(lo, hi);
+  } else {
 #pragma unroll
-    for (int e = 0; e < 16; e += 2) {
-      const int j = (d0 + e) / 2;
-      if (j < n) {
-        const double2 w = cs[j];
-        const double a = x[e], b = x[e + 1];
-        x[e] = to_odd(__builtin_fma(-b, w.y, a * w.x));
-        x[e + 1] = to_odd(__builtin_fma(a, w.y, b * w.x));
-      }
-    }
-    return;
+    for (int e = 0; e < 8; ++e)
+      if (e < n) to[(d + e) / 16 * 512 + (d + e) % 16] = (uint8_t)((e < 4 ? lo : hi) >> 8 * (e % 4));
   }
-  constexpr int PER = 16 / sizeof(T);
-#pragma unroll
-  for (int i = 0; i < 16; i += PER) {
-    const int d = d0 + i;
-    if (d >= 2 * n) break;
-    Piece<T, PER> u;
-    if (d + PER <= n)  // a piece in one half: its partners lie together
-      u = *(const Piece<T, PER>*)(row + d + n);
-    else if (d >= n && d + PER <= 2 * n)
-      u = *(const Piece<T, PER>*)(row + d - n);
-    else
-#pragma unroll
-      for (int e = 0; e < PER; ++e)
-        u.v[e] = d + e < n ? row[d + e + n] : (d + e < 2 * n ? row[d + e - n] : (T)0.f);
-#pragma unroll
-    for (int e = 0; e < PER; ++e) {
-      const int j = d + e < n ? d + e : d + e - n;
-      if (j < n) {
-        const double2 w = cs[j];
-        const double s = d + e < n ? -w.y : w.y;
-        x[i + e] = to_odd(__builtin_fma((double)(float)u.v[e], s, (double)x[i + e] * w.x));
-      }
-    }
-  }
-}
-
-__device__ __forceinline__ float top16(const float (&x)[16], float top) {
-#pragma unroll
-  for (int e = 0; e < 16; ++e) top = fmaxf(top, finite(x[e]) ? fabsf(x[e]) : 0.f);
-  return top;
 }
 
 // The queries' part: `block` tokens of a workgroup turned by their places.
-template <typename T>
+template <typename T, bool STREAM>
 __device__ __forceinline__ void append_queries(const Cache& c, const Sequences& sq,
                                                const Turn& turn, const AppendRows<T>& r,
                                                int64_t t0, int block, char* lds) {
   const int n = (int)(sq.T - t0 < block ? sq.T - t0 : block);
+  const TurnAngles<T> angles(turn.pairs, turn.interleaved);
   float2* cs = (float2*)lds;
-  int* at = (int*)(cs + block * turn.pairs);
+  int* at = (int*)(cs + block * angles.pitch);
   int* live = at + block;
+  TurnRows<T, APPEND_THREADS, STREAM> rows(r.q, r.q_row, r.q_head, r.q_out, r.Hq, r.D, t0, n,
+                                           turn.pairs, turn.interleaved);
+  rows.load();
   for (int t = wave_id(); t < n; t += APPEND_THREADS / 64) {
     const CacheRows s =
         cache_rows(sq, c, t0 + t, [](int64_t start, int) { return start; });
@@ -157,38 +216,91 @@ __device__ __forceinline__ void append_queries(const Cache& c, const Sequences& 
     }
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < n * turn.pairs; i += APPEND_THREADS) {
-    const int t = i / turn.pairs, j = i % turn.pairs;
+  for (int i = threadIdx.x; i < n * angles.pitch; i += APPEND_THREADS) {
+    const int t = i / angles.pitch, j = angles.pair(i % angles.pitch);
+    if (j >= turn.pairs) continue;
     const double p = r.places ? turn.place(t0 + t, j) : (double)at[t];
     double s, co;
     sine_cosine(p * turn.f[j], s, co);
     cs[i] = make_float2((float)(co * turn.m), (float)(s * turn.m));
   }
   __syncthreads();
-  turn_rows<T, APPEND_THREADS>(r.q, r.q_row, r.q_head, r.q_out, r.Hq, r.D, t0, n, turn.pairs,
-                               turn.interleaved, cs, live);
+  rows.run(cs, live);
 }
 
-// Workgroups 0 .. places * groups take a sequence's page and `heads` of its heads each, one team
-// of TEAM lanes a head: a wave where a page gets a few tokens, the workgroup where it gets
-// many.  A lane has sixteen values of a token's key and of its value at a time (CH times), which
-// are what it stores of a key and, a token's part of sixteen rows, of a value; `round` tokens go
-// through at a time.  Where a page is one round (any but a large page of wide heads), what was
-// loaded stays in registers between the largest value and the codes; else it is loaded again.
-// The workgroups behind them turn `block` tokens' queries each.
-template <typename T, int TEAM, int CH>
-__global__ __launch_bounds__(APPEND_THREADS) void cache_append_kernel(Cache c, Sequences sq,
-                                                                      Turn turn, AppendRows<T> r,
-                                                                      int groups, int heads,
-                                                                      int round, int kv, int block) {
+// Queries of a call whose kernel for keys and values would leave them too few places on a CU.
+template <typename T, bool STREAM>
+__global__ __launch_bounds__(APPEND_THREADS) void cache_queries_kernel(Cache c, Sequences sq,
+                                                                       Turn turn, AppendRows<T> r,
+                                                                       int block) {
   extern __shared__ double2 lds[];
-  if ((int)blockIdx.x >= kv) {
-    append_queries<T>(c, sq, turn, r, (int64_t)((int)blockIdx.x - kv) * block, block, (char*)lds);
-    return;
+  append_queries<T, STREAM>(c, sq, turn, r, (int64_t)blockIdx.x * block, block, (char*)lds);
+}
+
+// The page's older codes (slots below a) at a new scale, sixteen bytes at a time, four pieces of a
+// lane under way: of keys sixteen values of a token, of values sixteen tokens.  A piece that
+// ends with new tokens gets its older bytes one by one, so that no byte is written twice and
+// the new ones need not wait.
+template <int TEAM>
+__device__ __forceinline__ void scale_older(const Cache& c, uint8_t* codes, int64_t number, int h,
+                                            bool key, int a, float f, int lane) {
+  const int rows = 16 * c.chunks, all = key ? a * c.chunks : (a + 15) / 16 * rows;
+#pragma unroll 1
+  for (int i0 = lane; i0 < all; i0 += 4 * TEAM) {
+    uint4 x[4];
+    uint8_t* p[4];
+    int left[4];
+#pragma unroll
+    for (int y = 0; y < 4; ++y) {
+      const int i = i0 + y * TEAM;
+      left[y] = 0;
+      if (i >= all) continue;
+      const int t = key ? i / c.chunks : i / rows * 16, d = key ? i % c.chunks : i % rows;
+      p[y] = codes + c.block(number, h, t / 32) +
+             (key ? d * 512 + t % 32 * 16 : d * 32 + t % 32);
+      left[y] = key ? 16 : a - t;
+      x[y] = *(const uint4*)p[y];
+    }
+#pragma unroll
+    for (int y = 0; y < 4; ++y) {
+      if (left[y] == 0) continue;
+      const uint4 w = make_uint4(codes_times(x[y].x, f), codes_times(x[y].y, f),
+                                 codes_times(x[y].z, f), codes_times(x[y].w, f));
+      if (left[y] >= 16) {
+        *(uint4*)p[y] = w;
+      } else {
+#pragma unroll 1
+        for (int e = 0; e < left[y]; ++e) {
+          const uint32_t v = e < 8 ? (e < 4 ? w.x : w.y) : (e < 12 ? w.z : w.w);
+          p[y][e] = (uint8_t)(v >> 8 * (e % 4));
+        }
+      }
+    }
   }
-  constexpr int TEAMS = APPEND_THREADS / TEAM;
+}
+
+// Workgroups 0 .. kv - 1 take a sequence's page and `heads` of its heads each, one team of TEAM
+// lanes a head: a wave where a page gets a few tokens, the workgroup where it gets many.  A lane
+// has one part of a token's key, whose angles it works out once for all heads, and one of its
+// value, whose sixteen rows of a block it has a byte of each.  The next key and value are on
+// their way while one is rounded.  `round` tokens go through at a time; where a page is more
+// (MANY: large pages of wide heads), it is loaded twice: for the largest value, then for the
+// codes.
+// Workgroups behind them turn `block` tokens' queries each.
+template <typename T, int THREADS, int TEAM, bool MANY>
+__global__ __launch_bounds__(THREADS, MANY ? 2 : 4) void cache_append_kernel(
+    Cache c, Sequences sq, Turn turn, AppendRows<T> r, int groups, int heads, int round, int kv,
+    int block) {
+  extern __shared__ double2 lds[];
+  if constexpr (TEAM < THREADS)
+    if ((int)blockIdx.x >= kv) {
+      append_queries<T, false>(c, sq, turn, r, (int64_t)((int)blockIdx.x - kv) * block, block,
+                               (char*)lds);
+      return;
+    }
+  constexpr int TEAMS = THREADS / TEAM;
   const int64_t place = blockIdx.x / groups;
-  const int page = c.page, NC = c.chunks;
+  const int page = c.page, NC = c.chunks, Dr = 16 * NC;
   const CacheRows s = cache_rows(sq, c, place, [page](int64_t start, int i) {
     return start / page + 2 * (int64_t)i;
   });
@@ -206,174 +318,183 @@ __global__ __launch_bounds__(APPEND_THREADS) void cache_append_kernel(Cache c, S
   const int z = s.length - base < page ? s.length - base : page;
   const int64_t row0 = s.first + base - before;                         // slot 0's row
 
-  double2* cs = lds;
-  char* tile = (char*)(cs + round * turn.pairs);
+  char* tile = (char*)lds;
   const int tile_pitch = round + 4;
-  float* tops = (float*)(tile + (TEAMS == 1 ? tile_pitch * 16 * NC : 0));
+  float* tops = (float*)(tile + (TEAMS == 1 ? tile_pitch * Dr : 0));
   const int team = threadIdx.x / TEAM, lane = threadIdx.x % TEAM;
-  int tok[CH], chunk[CH];
-#pragma unroll
-  for (int i = 0; i < CH; ++i) {
-    tok[i] = (lane + i * TEAM) / NC;
-    chunk[i] = (lane + i * TEAM) % NC;
-  }
+  const int key_parts = Part::of_key(turn.pairs, Dr), parts = key_parts > NC ? key_parts : NC;
+  const int tok = lane / parts, part = lane % parts;
   // rounds begin at multiples of their length where the values' tile is turned over, so that a
   // round holds whole blocks
   const int r0 = TEAMS == 1 ? a / round * round : a;
   const int rounds = (z - r0 + round - 1) / round;
-  float k[CH][16], v[CH][16];
-
+  auto in = [&](int t0) { return tok < round && t0 + tok >= a && t0 + tok < z; };
+  Part pk, pv;
+  pk.key(part < key_parts ? part : 0, turn, r.D, Dr);
+  pv.plain(16 * (part < NC ? part : 0), r.D, Dr);
+  const bool has_k = part < key_parts, has_v = part < NC;
+  double2 cs[8];
   auto angles = [&](int t0) {
-    const int n = z - t0 < round ? z - t0 : round;
-    for (int i = threadIdx.x; i < n * turn.pairs; i += APPEND_THREADS) {
-      const int t = t0 + i / turn.pairs, j = i % turn.pairs;
-      if (t < a) continue;
-      const double p = r.places ? turn.place(row0 + t, j) : (double)(base + t);
-      double sn, co;
-      sine_cosine(p * turn.f[j], sn, co);
-      cs[i] = make_double2(co * turn.m, sn * turn.m);
-    }
-  };
-  auto in = [&](int t0, int i) {
-    const int t = t0 + tok[i];
-    return tok[i] < round && t >= a && t < z;
-  };
-  auto load = [&](int t0, int h) {
+    if (pk.pair < 0 || !in(t0)) return;
+    const int64_t row = row0 + t0 + tok;
 #pragma unroll
-    for (int i = 0; i < CH; ++i) {
-      if (!in(t0, i)) continue;
-      const int64_t row = row0 + t0 + tok[i];
-      const int d0 = 16 * chunk[i];
-      const T* kr = r.k + row * r.k_row + h * r.k_head;
-      load16<T>(kr + d0, r.D - d0, k[i]);
-      load16<T>(r.v + row * r.v_row + h * r.v_head + d0, r.D - d0, v[i]);
-      turn16<T>(kr, d0, r.D, turn, cs + tok[i] * turn.pairs, k[i]);
+    for (int e = 0; e < 8; ++e) {
+      const int j = pk.pair + e < turn.pairs ? pk.pair + e : pk.pair;
+      cs[e].x = (r.places ? turn.place(row, j) : (double)(base + t0 + tok)) * turn.f[j];
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      double sn, co;
+      sine_cosine(cs[e].x, sn, co);
+      cs[e] = make_double2(co * turn.m, sn * turn.m);
+      if (e % 2) __builtin_amdgcn_sched_barrier(0);  // (eight at once: 200 registers)
     }
   };
 
   const int h0 = (blockIdx.x % groups) * heads;
   const int h1 = h0 + heads < c.Hk ? h0 + heads : c.Hk;
-  for (int hh = h0; hh < h1; hh += TEAMS) {
-    const bool mine = hh + team < h1;
-    const int h = mine ? hh + team : h1 - 1;
-    const int64_t scale_at = (int64_t)number * c.Hk + h;
-    const float old_k = a > 0 ? c.key_scales[scale_at] : 0.f;
-    const float old_v = a > 0 ? c.value_scales[scale_at] : 0.f;
-    float top_k = 0.f, top_v = 0.f;
-    for (int y = 0; y < rounds; ++y) {
-      if (rounds > 1 || hh == h0) {
-        __syncthreads();
-        angles(r0 + y * round);
-        __syncthreads();
-      }
-      load(r0 + y * round, h);
+  // job 2 i: keys of the team's head i of these, job 2 i + 1: its values
+  PartValues<T> u;
+  auto load = [&](int job, int t0) {
+    const int h = h0 + (job >> 1) * TEAMS + team;
+    if (!in(t0) || h >= h1) return;
+    const int64_t row = row0 + t0 + tok;
+    if (job & 1) {
+      if (has_v) u.load(r.v + row * r.v_row + h * r.v_head, pv);
+    } else if (has_k) {
+      u.load(r.k + row * r.k_row + h * r.k_head, pk);
+    }
+  };
+  auto old_scale = [&](int job) {
+    const int h = h0 + (job >> 1) * TEAMS + team;
+    return a > 0 && h < h1 ? (job & 1 ? c.value_scales : c.key_scales)[(int64_t)number * c.Hk + h]
+                           : 0.f;
+  };
+  const int jobs = 2 * ((h1 - h0 + TEAMS - 1) / TEAMS);
+  load(0, r0);
+  float next_old = old_scale(0);
+  if (!MANY || rounds == 1) angles(r0);
+#pragma unroll 1
+  for (int job = 0; job < jobs; ++job) {
+    pk.fresh();
+    pv.fresh();
+    const bool key = !(job & 1);
+    const int h = h0 + (job >> 1) * TEAMS + team;
+    const bool mine = h < h1, has = mine && (key ? has_k : has_v);
+    const int64_t scale_at = (int64_t)number * c.Hk + (mine ? h : h1 - 1);
+    float* scale_p = (key ? c.key_scales : c.value_scales) + scale_at;
+    uint8_t* codes = key ? c.keys : c.values;
+    const float old = next_old;
+    if (job + 1 < jobs) next_old = old_scale(job + 1);
+    float top = 0.f, f = 0.f;
+    float x[16];
+    bool rare = false;
+    auto take = [&](int t0) {  // what was loaded as the cache takes it
 #pragma unroll
-      for (int i = 0; i < CH; ++i)
-        if (in(r0 + y * round, i)) {
-          top_k = top16(k[i], top_k);
-          top_v = top16(v[i], top_v);
-        }
-    }
-    top_k = wave_max(top_k);
-    top_v = wave_max(top_v);
-    if (TEAMS == 1) {
-      __syncthreads();
-      if (lane_id() == 0) {
-        tops[wave_id()] = top_k;
-        tops[4 + wave_id()] = top_v;
+      for (int e = 0; e < 8; ++e) {
+        x[e] = (float)u.a.v[e];
+        x[8 + e] = (float)u.b.v[e];
       }
-      __syncthreads();
-      top_k = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
-      top_v = fmaxf(fmaxf(tops[4], tops[5]), fmaxf(tops[6], tops[7]));
-    }
-    int ek = exponent_for(top_k), ev = exponent_for(top_v);
-    if (a > 0) {
-      const int ok = exponent_of(old_k), ov = exponent_of(old_v);
-      ek = ok > ek ? ok : ek;
-      ev = ov > ev ? ov : ev;
-    }
-    const float fk = power(-ek), fv = power(-ev);
-
-    // older codes of the page at a new scale
-    if (a > 0 && mine && (old_k != power(ek) || old_v != power(ev))) {
-      if (old_k != power(ek))
-        for (int i = lane; i < a * NC; i += TEAM) {
-          const int t = i / NC;
-          uint4* p = (uint4*)(c.keys + c.block(number, h, t / 32) + (i % NC) * 512 + t % 32 * 16);
-          uint4 x = *p;
-          x.x = codes_times(x.x, old_k * fk);
-          x.y = codes_times(x.y, old_k * fk);
-          x.z = codes_times(x.z, old_k * fk);
-          x.w = codes_times(x.w, old_k * fk);
-          *p = x;
-        }
-      if (old_v != power(ev)) {
-        const int rows = 16 * NC;
-        // four tokens of a value at a time, those of new tokens and behind left as they are
-        for (int i = lane; i < (a + 3) / 4 * rows; i += TEAM) {
-          const int t = i / rows * 4, d = i % rows;
-          uint32_t* p = (uint32_t*)(c.values + c.block(number, h, t / 32) + d * 32 + t % 32);
-          const uint32_t x = *p, keep = a - t >= 4 ? ~0u : (1u << 8 * (a - t)) - 1;
-          *p = (codes_times(x, old_v * fv) & keep) | (x & ~keep);
-        }
-      }
-      __threadfence();  // (a new token's codes may share a word with older ones)
-    }
-    if (TEAMS == 1 && a > 0) __syncthreads();
-    if (mine && lane == 0) {
-      c.key_scales[scale_at] = power(ek);
-      c.value_scales[scale_at] = power(ev);
-    }
-
-    for (int y = 0; y < rounds; ++y) {
-      const int t0 = r0 + y * round;
-      if (rounds > 1) {
-        __syncthreads();
-        angles(t0);
-        __syncthreads();
-        load(t0, h);
-      }
+      if (key && pk.pair >= 0) turn_part<T>(u, turn.interleaved, cs, x);
+    };
+    auto measure = [&](int t0) {  // the largest of what is finite
+      if (!has || !in(t0)) return;
+      uint32_t most = 0;
 #pragma unroll
-      for (int i = 0; i < CH; ++i) {
-        if (!in(t0, i) || !mine) continue;
-        const int t = t0 + tok[i];
-        const int64_t block_at = c.block(number, h, t / 32);
-        uint4 x;
-        x.x = codes4(k[i], fk);
-        x.y = codes4(k[i] + 4, fk);
-        x.z = codes4(k[i] + 8, fk);
-        x.w = codes4(k[i] + 12, fk);
-        *(uint4*)(c.keys + block_at + chunk[i] * 512 + t % 32 * 16) = x;
+      for (int e = 0; e < 16; ++e) {
+        const uint32_t b = __builtin_bit_cast(uint32_t, x[e]) & 0x7fffffff;
+        most = b > most ? b : most;
+      }
+      rare = most >= 0x7f800000;
+      if (rare) {
+        most = 0;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const uint32_t b = __builtin_bit_cast(uint32_t, x[e]) & 0x7fffffff;
+          most = b > most && b < 0x7f800000 ? b : most;
+        }
+      }
+      top = fmaxf(top, __builtin_bit_cast(float, most));
+    };
+    auto settle = [&] {  // the page's scale; older codes brought to it
+      top = wave_max(top);
+      if (TEAMS == 1) {
+        __syncthreads();
+        if (lane_id() == 0) tops[wave_id()] = top;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < THREADS / 64; ++i) top = fmaxf(top, tops[i]);
+      }
+      int e = exponent_for(top);
+      if (a > 0) {
+        const int o = exponent_of(old);
+        e = o > e ? o : e;
+      }
+      f = power(-e);
+      if (a > 0 && mine && old != power(e))
+        scale_older<TEAM>(c, codes, number, h, key, a, old * f, lane);
+      if (mine && lane == 0) *scale_p = power(e);
+    };
+    auto store = [&](int t0) {
+      if (has && in(t0)) {
+        const int t = t0 + tok;
+        uint8_t* to = codes + c.block(number, h, t / 32);
         uint32_t w[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) w[e] = codes4(v[i] + 4 * e, fv);
-        if (TEAMS == 1) {
-          char* to = tile + chunk[i] * 16 * tile_pitch + tok[i];
+        for (int e = 0; e < 4; ++e) w[e] = codes4(x + 4 * e, f, rare || f == power(-E_MOST));
+        if (key && pk.pair >= 0 && turn.interleaved) {  // pairs side by side again
+          const uint32_t p[4] = {w[0], w[1], w[2], w[3]};
+          w[0] = __builtin_amdgcn_perm(p[2], p[0], 0x05010400);
+          w[1] = __builtin_amdgcn_perm(p[2], p[0], 0x07030602);
+          w[2] = __builtin_amdgcn_perm(p[3], p[1], 0x05010400);
+          w[3] = __builtin_amdgcn_perm(p[3], p[1], 0x07030602);
+        }
+        if (key) {
+          store_part(to, t % 32, pk.pa, pk.store_a, w[0], w[1]);
+          store_part(to, t % 32, pk.pb, pk.store_b, w[2], w[3]);
+        } else if (TEAMS == 1) {
+          char* at = tile + part * 16 * tile_pitch + tok;
 #pragma unroll
-          for (int e = 0; e < 16; ++e) to[e * tile_pitch] = (char)(w[e / 4] >> 8 * (e % 4));
+          for (int e = 0; e < 16; ++e) at[e * tile_pitch] = (char)(w[e / 4] >> 8 * (e % 4));
         } else {
-          uint8_t* to = c.values + block_at + chunk[i] * 512 + t % 32;
+          to += part * 512 + t % 32;
 #pragma unroll
           for (int e = 0; e < 16; ++e) to[e * 32] = (uint8_t)(w[e / 4] >> 8 * (e % 4));
         }
       }
-      if (TEAMS == 1) {
+      if (TEAMS == 1 && !key) {
         __syncthreads();
-        const int rows = 16 * NC;
-        for (int i = threadIdx.x; i < round / 16 * rows; i += APPEND_THREADS) {
-          const int half = i & 1, d = (i >> 1) % rows, blk = (i >> 1) / rows;
+        for (int i = threadIdx.x; i < round / 16 * Dr; i += THREADS) {
+          const int half = i & 1, d = (i >> 1) % Dr, blk = (i >> 1) / Dr;
           const int lt = 32 * blk + 16 * half, t = t0 + lt;
           if (t + 16 <= a || t >= z) continue;
-          uint8_t* to = c.values + c.block(number, h, t / 32) + d * 32 + t % 32;
+          uint8_t* to = codes + c.block(number, h, t / 32) + d * 32 + t % 32;
           const uint32_t* at = (const uint32_t*)(tile + d * tile_pitch + lt);
-          const uint4 x = make_uint4(at[0], at[1], at[2], at[3]);
           if (t >= a && t + 16 <= z)
-            *(uint4*)to = x;
+            *(uint4*)to = make_uint4(at[0], at[1], at[2], at[3]);
           else
             for (int e = 0; e < 16; ++e)
               if (t + e >= a && t + e < z) to[e] = ((const uint8_t*)at)[e];
         }
         __syncthreads();
+      }
+    };
+    if (!MANY || rounds == 1) {
+      take(r0);
+      if (job + 1 < jobs) load(job + 1, r0);
+      measure(r0);
+      settle();
+      store(r0);
+    } else {
+#pragma unroll 1
+      for (int y = 0; y < 2 * rounds; ++y) {
+        const int t0 = r0 + (y < rounds ? y : y - rounds) * round;
+        load(job, t0);
+        if (key) angles(t0);
+        take(t0);
+        measure(t0);
+        if (y == rounds - 1) settle();
+        if (y >= rounds) store(t0);
       }
     }
   }
@@ -412,21 +533,11 @@ Cache cache_args(const void* keys, const void* values, const float* key_scales,
   return c;
 }
 
-template <typename T, int TEAM, int CH>
-void append_launch(const Cache& c, const Sequences& sq, const Turn& t, const AppendRows<T>& r,
-                   int64_t places, int groups, int heads, int64_t q_blocks, int block,
-                   hipStream_t s) {
-  // tokens of a round: what the team's lanes hold, whole blocks for a workgroup
-  int round = TEAM * CH / c.chunks;
-  if (TEAM == APPEND_THREADS) round = round >= c.page ? c.page : round / 32 * 32;
-  const int64_t angles = (int64_t)round * t.pairs * sizeof(double2);
-  const int64_t kv_lds =
-      angles + (TEAM == APPEND_THREADS ? (int64_t)(round + 4) * 16 * c.chunks : 0) + 64;
-  const int64_t q_lds = (int64_t)block * t.pairs * sizeof(float2) + block * 2 * sizeof(int);
-  cache_append_kernel<T, TEAM, CH>
-      <<<dim3((unsigned)(places * groups + q_blocks)), APPEND_THREADS,
-         (size_t)(kv_lds > q_lds ? kv_lds : q_lds), s>>>(c, sq, t, r, groups, heads, round,
-                                                         (int)(places * groups), block);
+// Tokens that a team of `lanes` takes at a time; whole blocks for a workgroup's.
+int append_round(const Cache& c, const Turn& t, int lanes, bool whole) {
+  const int key_parts = Part::of_key(t.pairs, 16 * c.chunks);
+  const int round = lanes / (key_parts > c.chunks ? key_parts : c.chunks);
+  return round >= c.page ? c.page : (whole ? round / 32 * 32 : round);
 }
 
 }  // namespace tpo
@@ -475,25 +586,55 @@ extern "C" int tpo_cache_append(int dtype, const void* k, const void* v, const v
   // a place for each page that a sequence's new tokens may lie in, see the kernel
   const int64_t slots = T / page + 2 * (B + 2);
   const bool few = T <= 8 * B;
-  int64_t heads = few ? (Hk < 4 ? Hk : 4) : 1;
-  if (!few)
-    while (heads < Hk && (T / page + B) * ((Hk + heads) / (heads + 1)) >= 1024) ++heads;
-  const int64_t groups = (Hk + heads - 1) / heads;
-  int64_t block = few ? 1 : T / 4096;
+  const int64_t about = T / page + B + 1;  // pages
+  int64_t groups = few ? (Hk + 3) / 4 : (512 + about - 1) / about;
+  if (groups > Hk) groups = Hk;
+  const int64_t heads = (Hk + groups - 1) / groups;
+  groups = (Hk + heads - 1) / heads;
+  // tokens' queries of a workgroup: as tpo_rotary's
+  int64_t block = few || !q ? 1 : 16384 / (Hq * D * element_bytes(dtype));
+  if (block > T / 2048) block = T / 2048;
   block = block > 16 ? 16 : (block < 1 ? 1 : block);
   const int64_t q_blocks = q ? (T + block - 1) / block : 0;
-  if (slots * groups + q_blocks >= ((int64_t)1 << 24))
+  if (slots * groups + q_blocks >= ((int64_t)1 << 23))
     return set_error(TPO_ERR_ARG, "%s: too many tokens", op);
+  const int64_t q_pitch = dtype == TPO_F32 ? TurnAngles<float>(t.pairs, t.interleaved).pitch
+                                           : TurnAngles<half_t>(t.pairs, t.interleaved).pitch;
+  const int64_t q_lds = block * (q_pitch * sizeof(float2) + 2 * sizeof(int));
+  const int kv = (int)(slots * groups);
+  hipStream_t s = (hipStream_t)stream;
   with_element(dtype, [&](auto e) {
     typedef decltype(e) E;
     const AppendRows<E> r{(const E*)k, (const E*)v, (const E*)q, (E*)q_out, k_row, k_head, v_row,
                           v_head, q_row, q_head, (int)Hq, (int)D, places ? 1 : 0};
-    if (few)
-      append_launch<E, 64, 1>(c, sq, t, r, slots, (int)groups, (int)heads, q_blocks, (int)block,
-                              (hipStream_t)stream);
+    if (few) {
+      cache_append_kernel<E, APPEND_THREADS, 64, true>
+          <<<dim3((unsigned)(kv + q_blocks)), APPEND_THREADS, (size_t)q_lds, s>>>(
+              c, sq, t, r, (int)groups, (int)heads, append_round(c, t, 64, false), kv, (int)block);
+      return;
+    }
+    auto launch = [&](auto threads, auto many) {
+      constexpr int N = decltype(threads)::value;
+      const int round = append_round(c, t, N, true);
+      cache_append_kernel<E, N, N, decltype(many)::value>
+          <<<dim3((unsigned)kv), N, (size_t)((round + 4) * Dr + 64), s>>>(
+              c, sq, t, r, (int)groups, (int)heads, round, kv, 0);
+    };
+    if (append_round(c, t, 256, true) >= page)
+      launch(std::integral_constant<int, 256>(), std::false_type());
+    else if (append_round(c, t, 512, true) >= page)
+      launch(std::integral_constant<int, 512>(), std::false_type());
     else
-      append_launch<E, APPEND_THREADS, 2>(c, sq, t, r, slots, (int)groups, (int)heads, q_blocks,
-                                          (int)block, (hipStream_t)stream);
+      launch(std::integral_constant<int, 512>(), std::true_type());
+    if (!q) return;
+    auto turn_queries = [&](auto streaming) {
+      cache_queries_kernel<E, decltype(streaming)::value>
+          <<<dim3((unsigned)q_blocks), APPEND_THREADS, (size_t)q_lds, s>>>(c, sq, t, r, (int)block);
+    };
+    if (T * Hq * D * element_bytes(dtype) > TURN_STREAM)
+      turn_queries(std::true_type());
+    else
+      turn_queries(std::false_type());
   });
   return check_launch(op);
 }

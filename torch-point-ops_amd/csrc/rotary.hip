@@ -1,5 +1,7 @@
 // rotary.hip -- rotary positions of queries and keys, and their gradient (the same with the
 // angles' sign turned).
+#include <type_traits>
+
 #include "rotary.hpp"
 
 namespace tpo {
@@ -8,22 +10,27 @@ constexpr int TURN_THREADS = 256;
 constexpr int TURN_ANGLES = 4096;  // cosines and sines in LDS
 
 // A workgroup takes `block` tokens: first their angles, one a thread, then all heads' rows.
-template <typename T>
+template <typename T, bool STREAM>
 __global__ __launch_bounds__(TURN_THREADS) void rotary_kernel(
     const T* __restrict__ x, int64_t x_row, int64_t x_head, T* __restrict__ y, int64_t tokens,
     int H, int D, Turn turn, int back, int block) {
-  extern __shared__ float2 cs[];
+  extern __shared__ float4 lds[];
+  float2* cs = (float2*)lds;
   const int64_t t0 = (int64_t)blockIdx.x * block;
   const int n = (int)(tokens - t0 < block ? tokens - t0 : block);
-  for (int i = threadIdx.x; i < n * turn.pairs; i += TURN_THREADS) {
-    const int t = i / turn.pairs, j = i % turn.pairs;
+  const TurnAngles<T> angles(turn.pairs, turn.interleaved);
+  TurnRows<T, TURN_THREADS, STREAM> rows(x, x_row, x_head, y, H, D, t0, n, turn.pairs,
+                                         turn.interleaved);
+  rows.load();
+  for (int i = threadIdx.x; i < n * angles.pitch; i += TURN_THREADS) {
+    const int t = i / angles.pitch, j = angles.pair(i % angles.pitch);
+    if (j >= turn.pairs) continue;  // (its products go nowhere)
     double s, c;
     sine_cosine(turn.place(t0 + t, j) * turn.f[j], s, c);
     cs[i] = make_float2((float)(c * turn.m), (float)(back ? -s * turn.m : s * turn.m));
   }
   __syncthreads();
-  turn_rows<T, TURN_THREADS>(x, x_row, x_head, y, H, D, t0, n, turn.pairs, turn.interleaved, cs,
-                             nullptr);
+  rows.run(cs, nullptr);
 }
 
 int turn_args(const char* op, const double* f, const void* at, int64_t pairs, int64_t axes,
@@ -68,20 +75,31 @@ extern "C" int tpo_rotary(int dtype, const void* x, int64_t tokens, int64_t head
   if (int rc = all_there("rotary", {x, y})) return rc;
   if (pairs > 0)
     if (int rc = all_there("rotary", {places, frequencies})) return rc;
-  // tokens of a workgroup: enough workgroups for every CU's places (8 of 256 threads), then
-  // as many as share the launch of one
-  int64_t block = tokens / 4096;
-  if (block > 16) block = 16;
-  if (pairs > 0 && block > TURN_ANGLES / pairs) block = TURN_ANGLES / pairs;
+  // tokens of a workgroup: about 16 KB of them (32768 x 20 x 128 bfloat16: 2 to 4 tokens 81 us,
+  // 8 tokens 87, 32 91: a workgroup's angles come before its first store), and 2048 workgroups
+  const int64_t pitch = dtype == TPO_F32 ? TurnAngles<float>(t.pairs, t.interleaved).pitch
+                                         : TurnAngles<half_t>(t.pairs, t.interleaved).pitch;
+  int64_t block = 16384 / (heads * D * element_bytes(dtype));
+  if (block > tokens / 2048) block = tokens / 2048;
+  if (pitch > 0 && block > TURN_ANGLES / pitch) block = TURN_ANGLES / pitch;
   if (block < 1) block = 1;
   while ((tokens + block - 1) / block >= ((int64_t)1 << 24)) block *= 2;
-  if (block * pairs > 2 * TURN_ANGLES)
+  if (block * pitch > 2 * TURN_ANGLES)
     return set_error(TPO_ERR_ARG, "rotary: too many tokens");
+  const bool stream_out = tokens * heads * D * element_bytes(dtype) > TURN_STREAM;
+  const unsigned blocks = (unsigned)((tokens + block - 1) / block);
+  const size_t lds = (size_t)(block * pitch * sizeof(float2));
   with_element(dtype, [&](auto e) {
     typedef decltype(e) T;
-    rotary_kernel<T><<<dim3((unsigned)((tokens + block - 1) / block)), TURN_THREADS,
-                       (size_t)(block * pairs * sizeof(float2)), (hipStream_t)stream>>>(
-        (const T*)x, x_row, x_head, (T*)y, tokens, (int)heads, (int)D, t, back, (int)block);
+    auto launch = [&](auto streaming) {
+      rotary_kernel<T, decltype(streaming)::value>
+          <<<dim3(blocks), TURN_THREADS, lds, (hipStream_t)stream>>>(
+              (const T*)x, x_row, x_head, (T*)y, tokens, (int)heads, (int)D, t, back, (int)block);
+    };
+    if (stream_out)
+      launch(std::true_type());
+    else
+      launch(std::false_type());
   });
   return check_launch("rotary");
 }
