@@ -50,33 +50,47 @@ struct CacheRows {
   int64_t place;           // of its first in the order asked for
 };
 // The last sequence whose first place is at or before `place`; first(start, s): the first place
-// of sequence s (0 and B + 1 being the rows before and behind), not decreasing.  Up to 62
-// sequences: each lane has one of them, and one trip to memory brings all that is needed.
+// of sequence s (0 and B + 1 being the rows before and behind), not decreasing.  Up to 126
+// sequences: each lane has one or two of them, and one trip to memory brings all that is needed
+// (in four trips, a workgroup's beginning took 2 us of the 12 of 64 sequences' new tokens).
 template <typename F>
 __device__ __forceinline__ CacheRows cache_rows(const Sequences& sq, const Cache& c, int64_t place,
                                                 const F& first) {
   const int l = lane_id(), B = sq.B;
   CacheRows r;
-  if (B <= 62) {
-    const int i = l < 1 ? 0 : (l - 1 < B ? l - 1 : B), j = l < B ? l : B;
-    const bool own = l >= 1 && l <= B;
-    const int64_t o = sq.offsets[i], p = sq.offsets[j];
-    const int64_t n = own ? (sq.lengths ? sq.lengths[l - 1] : sq.T) : 0;
-    const int64_t kept = own ? c.lengths[l - 1] : 0;
+  if (B <= 126) {
+    int64_t o[2], p[2], n[2], kept[2];
+    auto load = [&](int y) {
+      const int k = l + 64 * y;  // sequence k of B + 2
+      const int i = k < 1 ? 0 : (k - 1 < B ? k - 1 : B), j = k < B ? k : B;
+      const bool own = k >= 1 && k <= B;
+      o[y] = sq.offsets[i];
+      p[y] = sq.offsets[j];
+      n[y] = own ? (sq.lengths ? sq.lengths[k - 1] : sq.T) : 0;
+      kept[y] = own ? c.lengths[k - 1] : 0;
+    };
+    load(0);
+    if (B > 62) load(1);
     const int T = (int)sq.T;
     auto inside = [](int64_t v, int most) { return v < 0 ? 0 : (v > most ? most : (int)v); };
-    const int start = l < 1 ? 0 : (l > B + 1 ? T : inside(o, T));
-    const int next = l > B ? T : inside(p, T);
-    const int room = next > start ? next - start : 0;
-    const int used = inside(n, room), length = c.length(kept);
-    const uint64_t m = __builtin_amdgcn_ballot_w64(l < B + 2 && first(start, l) <= place);
-    const int s = m ? 63 - __builtin_clzll(m) : 0;
-    r.first = __builtin_amdgcn_readlane(start, s);
-    r.room = __builtin_amdgcn_readlane(room, s);
-    r.used = __builtin_amdgcn_readlane(used, s);
-    r.length = __builtin_amdgcn_readlane(length, s);
-    r.b = s >= 1 && s <= B ? s - 1 : -1;
-    r.place = first(r.first, s);
+    auto pick = [&](int y) {
+      const int k = l + 64 * y;
+      const int start = k < 1 ? 0 : (k > B + 1 ? T : inside(o[y], T));
+      const int next = k > B ? T : inside(p[y], T);
+      const int room = next > start ? next - start : 0;
+      const int used = inside(n[y], room), length = c.length(kept[y]);
+      const uint64_t m = __builtin_amdgcn_ballot_w64(k < B + 2 && first(start, k) <= place);
+      if (y > 0 && m == 0) return;
+      const int at = m ? 63 - __builtin_clzll(m) : 0, s = at + 64 * y;
+      r.first = __builtin_amdgcn_readlane(start, at);
+      r.room = __builtin_amdgcn_readlane(room, at);
+      r.used = __builtin_amdgcn_readlane(used, at);
+      r.length = __builtin_amdgcn_readlane(length, at);
+      r.b = s >= 1 && s <= B ? s - 1 : -1;
+      r.place = first(r.first, s);
+    };
+    pick(0);
+    if (B > 62) pick(1);
     return r;
   }
   int lo = 0, n = B + 2;  // among lo .. lo + n - 1: 64 guesses a step

@@ -14,7 +14,6 @@
 
 namespace tpo {
 
-constexpr int APPEND_THREADS = 256;
 constexpr int E_LEAST = -40, E_MOST = 40;
 constexpr float CODE_MOST = 448.f;
 
@@ -194,7 +193,7 @@ __device__ __forceinline__ void store_part(uint8_t* block, int token, int d, int
 }
 
 // The queries' part: `block` tokens of a workgroup turned by their places.
-template <typename T, bool STREAM>
+template <typename T, int THREADS, bool STREAM>
 __device__ __forceinline__ void append_queries(const Cache& c, const Sequences& sq,
                                                const Turn& turn, const AppendRows<T>& r,
                                                int64_t t0, int block, char* lds) {
@@ -203,10 +202,10 @@ __device__ __forceinline__ void append_queries(const Cache& c, const Sequences& 
   float2* cs = (float2*)lds;
   int* at = (int*)(cs + block * angles.pitch);
   int* live = at + block;
-  TurnRows<T, APPEND_THREADS, STREAM> rows(r.q, r.q_row, r.q_head, r.q_out, r.Hq, r.D, t0, n,
+  TurnRows<T, THREADS, STREAM> rows(r.q, r.q_row, r.q_head, r.q_out, r.Hq, r.D, t0, n,
                                            turn.pairs, turn.interleaved);
   rows.load();
-  for (int t = wave_id(); t < n; t += APPEND_THREADS / 64) {
+  for (int t = wave_id(); t < n; t += THREADS / 64) {
     const CacheRows s =
         cache_rows(sq, c, t0 + t, [](int64_t start, int) { return start; });
     const int i = (int)(t0 + t - s.first), p = s.length - s.used + i;
@@ -216,7 +215,7 @@ __device__ __forceinline__ void append_queries(const Cache& c, const Sequences& 
     }
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < n * angles.pitch; i += APPEND_THREADS) {
+  for (int i = threadIdx.x; i < n * angles.pitch; i += THREADS) {
     const int t = i / angles.pitch, j = angles.pair(i % angles.pitch);
     if (j >= turn.pairs) continue;
     const double p = r.places ? turn.place(t0 + t, j) : (double)at[t];
@@ -228,30 +227,32 @@ __device__ __forceinline__ void append_queries(const Cache& c, const Sequences& 
   rows.run(cs, live);
 }
 
-// Queries of a call whose kernel for keys and values would leave them too few places on a CU.
-template <typename T, bool STREAM>
-__global__ __launch_bounds__(APPEND_THREADS) void cache_queries_kernel(Cache c, Sequences sq,
-                                                                       Turn turn, AppendRows<T> r,
-                                                                       int block) {
+// The same in a launch of its own, 8 waves a SIMD, for more queries than the caches hold: their way
+// to and from memory is all that counts (20 thousand tokens, 16 heads of 128 in bfloat16: 33 us,
+// 5.2 TB/s; behind the pages' workgroups in one launch, 16 waves a CU, both take 83, apart 47 + 33).
+template <typename T>
+__global__ __launch_bounds__(256) void cache_queries_kernel(Cache c, Sequences sq, Turn turn,
+                                                            AppendRows<T> r, int block) {
   extern __shared__ double2 lds[];
-  append_queries<T, STREAM>(c, sq, turn, r, (int64_t)blockIdx.x * block, block, (char*)lds);
+  append_queries<T, 256, true>(c, sq, turn, r, (int64_t)blockIdx.x * block, block, (char*)lds);
 }
 
-// The page's older codes (slots below a) at a new scale, sixteen bytes at a time, four pieces of a
-// lane under way: of keys sixteen values of a token, of values sixteen tokens.  A piece that
+// The page's older codes (slots below a) at a new scale, sixteen bytes at a time (a wave's lanes
+// with four of them under way): of keys sixteen values of a token, of values sixteen tokens.  A piece that
 // ends with new tokens gets its older bytes one by one, so that no byte is written twice and
 // the new ones need not wait.
 template <int TEAM>
 __device__ __forceinline__ void scale_older(const Cache& c, uint8_t* codes, int64_t number, int h,
                                             bool key, int a, float f, int lane) {
+  constexpr int N = TEAM == 64 ? 4 : 1;
   const int rows = 16 * c.chunks, all = key ? a * c.chunks : (a + 15) / 16 * rows;
 #pragma unroll 1
-  for (int i0 = lane; i0 < all; i0 += 4 * TEAM) {
-    uint4 x[4];
-    uint8_t* p[4];
-    int left[4];
+  for (int i0 = lane; i0 < all; i0 += N * TEAM) {
+    uint4 x[N];
+    uint8_t* p[N];
+    int left[N];
 #pragma unroll
-    for (int y = 0; y < 4; ++y) {
+    for (int y = 0; y < N; ++y) {
       const int i = i0 + y * TEAM;
       left[y] = 0;
       if (i >= all) continue;
@@ -262,7 +263,7 @@ __device__ __forceinline__ void scale_older(const Cache& c, uint8_t* codes, int6
       x[y] = *(const uint4*)p[y];
     }
 #pragma unroll
-    for (int y = 0; y < 4; ++y) {
+    for (int y = 0; y < N; ++y) {
       if (left[y] == 0) continue;
       const uint4 w = make_uint4(codes_times(x[y].x, f), codes_times(x[y].y, f),
                                  codes_times(x[y].z, f), codes_times(x[y].w, f));
@@ -279,115 +280,365 @@ __device__ __forceinline__ void scale_older(const Cache& c, uint8_t* codes, int6
   }
 }
 
-// Workgroups 0 .. kv - 1 take a sequence's page and `heads` of its heads each, one team of TEAM
-// lanes a head: a wave where a page gets a few tokens, the workgroup where it gets many.  A lane
-// has one part of a token's key, whose angles it works out once for all heads, and one of its
-// value, whose sixteen rows of a block it has a byte of each.  The next key and value are on
-// their way while one is rounded.  `round` tokens go through at a time; where a page is more
-// (MANY: large pages of wide heads), it is loaded twice: for the largest value, then for the
-// codes.
-// Workgroups behind them turn `block` tokens' queries each.
-template <typename T, int THREADS, int TEAM, bool MANY>
-__global__ __launch_bounds__(THREADS, MANY ? 2 : 4) void cache_append_kernel(
-    Cache c, Sequences sq, Turn turn, AppendRows<T> r, int groups, int heads, int round, int kv,
-    int block) {
-  extern __shared__ double2 lds[];
-  if constexpr (TEAM < THREADS)
-    if ((int)blockIdx.x >= kv) {
-      append_queries<T, false>(c, sq, turn, r, (int64_t)((int)blockIdx.x - kv) * block, block,
-                               (char*)lds);
-      return;
-    }
-  constexpr int TEAMS = THREADS / TEAM;
-  const int64_t place = blockIdx.x / groups;
-  const int page = c.page, NC = c.chunks, Dr = 16 * NC;
-  const CacheRows s = cache_rows(sq, c, place, [page](int64_t start, int i) {
-    return start / page + 2 * (int64_t)i;
-  });
-  if (s.b < 0) return;
-  const int before = s.length - s.used;  // the place of the first new token
-  const int from = before < 0 ? 0 : before;
-  if (from >= s.length) return;
-  const int64_t past = place - s.place;
-  if (past > (s.length - 1) / page - from / page) return;
-  const int pi = from / page + (int)past;
-  const int number = __builtin_amdgcn_readfirstlane(c.page_of(s.b, pi));
-  if (number < 0) return;
-  const int base = pi * page;
-  const int a = from > base ? from - base : 0;                          // slots a .. z - 1 are new
-  const int z = s.length - base < page ? s.length - base : page;
-  const int64_t row0 = s.first + base - before;                         // slot 0's row
+// A workgroup's page: which tokens of which sequence are new in it.
+struct AppendPage {
+  int found;      // what the table says of the page
+  int number;     // the page, -1: none
+  int base;       // the place of its first slot
+  int a, z;       // slots a .. z - 1 are new
+  int64_t row0;   // slot 0's row
 
+  __device__ __forceinline__ AppendPage(const Cache& c, const Sequences& sq, int64_t place) {
+    const int page = c.page;
+    const CacheRows s = cache_rows(sq, c, place, [page](int64_t start, int i) {
+      return start / page + 2 * (int64_t)i;
+    });
+    a = z = 0;
+    if (s.b < 0) return;
+    const int before = s.length - s.used;  // the place of the first new token
+    const int from = before < 0 ? 0 : before;
+    if (from >= s.length) return;
+    const int64_t past = place - s.place;
+    if (past > (s.length - 1) / page - from / page) return;
+    const int pi = from / page + (int)past;
+    found = c.page_of(s.b, pi);
+    base = pi * page;
+    a = from > base ? from - base : 0;
+    z = s.length - base < page ? s.length - base : page;
+    row0 = s.first + base - before;
+  }
+  // no new tokens here
+  __device__ __forceinline__ bool none() const { return z == 0; }
+  // Whether there is a page; asked for once the rows' loads are on their way.
+  __device__ __forceinline__ bool there() {
+    number = __builtin_amdgcn_readfirstlane(found);
+    return number >= 0;
+  }
+};
+
+// The angles of a part's pairs, of the token in slot t.
+template <typename T>
+__device__ __forceinline__ void part_angles(const Part& p, const Turn& turn,
+                                            const AppendRows<T>& r, const AppendPage& g, int t,
+                                            double2 (&cs)[8]) {
+  double f[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) f[e] = turn.f[p.pair + e < turn.pairs ? p.pair + e : p.pair];
+  if (r.places) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      cs[e].x = turn.place(g.row0 + t, p.pair + e < turn.pairs ? p.pair + e : p.pair) * f[e];
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) cs[e].x = (double)(g.base + t) * f[e];
+  }
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    double s, c;
+    sine_cosine(cs[e].x, s, c);
+    cs[e] = make_double2(c * turn.m, s * turn.m);
+    if (e % 2) __builtin_amdgcn_sched_barrier(0);  // (eight at once: 200 registers)
+  }
+}
+
+// The largest of what is finite among sixteen values, as bits; rare: some are not.
+__device__ __forceinline__ uint32_t top16(const float (&x)[16], bool& rare) {
+  uint32_t top = 0;
+#pragma unroll
+  for (int e = 0; e < 16; ++e) {
+    const uint32_t b = __builtin_bit_cast(uint32_t, x[e]) & 0x7fffffff;
+    top = b > top ? b : top;
+  }
+  rare = top >= 0x7f800000;
+  if (rare) {
+    top = 0;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const uint32_t b = __builtin_bit_cast(uint32_t, x[e]) & 0x7fffffff;
+      top = b > top && b < 0x7f800000 ? b : top;
+    }
+  }
+  return top;
+}
+
+// The largest of a wave's numbers, the same in all lanes: within sixteen lanes by moves between
+// lanes, then over the four of them.
+__device__ __forceinline__ uint32_t wave_top(uint32_t v) {
+  auto with = [&](auto move) {
+    const uint32_t o = (uint32_t)__builtin_amdgcn_mov_dpp((int)v, decltype(move)::value, 15, 15, true);
+    v = o > v ? o : v;
+  };
+  with(std::integral_constant<int, 0xb1>());   // the neighbour
+  with(std::integral_constant<int, 0x4e>());   // two on
+  with(std::integral_constant<int, 0x141>());  // the other four of eight
+  with(std::integral_constant<int, 0x140>());  // the other eight of sixteen
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < 64; i += 16) {
+    const uint32_t o = __builtin_amdgcn_readlane((int)v, i);
+    top = o > top ? o : top;
+  }
+  return top;
+}
+
+// The exponent of a page's scale: of its new values (the largest's bits), and not below the old
+// scale's where the page holds older codes.
+__device__ __forceinline__ int page_exponent(uint32_t top, bool older, float old) {
+  const int e = exponent_for(__builtin_bit_cast(float, top));
+  if (!older) return e;
+  const int o = exponent_of(old);
+  return o > e ? o : e;
+}
+
+// Sixteen values' codes, of a key's part or a value's.
+__device__ __forceinline__ void codes16(const float (&x)[16], float f, bool rare, bool together,
+                                        uint32_t (&w)[4]) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) w[e] = codes4(x + 4 * e, f, rare || f == power(-E_MOST));
+  if (together) {  // the first and second of pairs side by side again
+    const uint32_t p[4] = {w[0], w[1], w[2], w[3]};
+    w[0] = __builtin_amdgcn_perm(p[2], p[0], 0x05010400);
+    w[1] = __builtin_amdgcn_perm(p[2], p[0], 0x07030602);
+    w[2] = __builtin_amdgcn_perm(p[3], p[1], 0x05010400);
+    w[3] = __builtin_amdgcn_perm(p[3], p[1], 0x07030602);
+  }
+}
+
+// A round's values, turned over in LDS (a value's tokens side by side, `pitch` bytes from one
+// value to the next), to a page's blocks: slots t0 .. t0 + round - 1, those of a .. z - 1.
+template <int THREADS>
+__device__ __forceinline__ void store_tile(const Cache& c, const char* tile, int pitch,
+                                           const AppendPage& g, int h, int t0, int round) {
+  const int Dr = 16 * c.chunks;
+  for (int i = threadIdx.x; i < round / 16 * Dr; i += THREADS) {
+    const int half = i & 1, d = (i >> 1) % Dr, blk = (i >> 1) / Dr;
+    const int lt = 32 * blk + 16 * half, t = t0 + lt;
+    if (t + 16 <= g.a || t >= g.z) continue;
+    uint8_t* to = c.values + c.block(g.number, h, t / 32) + d * 32 + t % 32;
+    const uint32_t* at = (const uint32_t*)(tile + d * pitch + lt);
+    if (t >= g.a && t + 16 <= g.z)
+      *(uint4*)to = make_uint4(at[0], at[1], at[2], at[3]);
+    else
+      for (int e = 0; e < 16; ++e)
+        if (t + e >= g.a && t + e < g.z) to[e] = ((const uint8_t*)at)[e];
+  }
+}
+
+// Many tokens: a workgroup takes a sequence's page and `heads` of its heads, one after the
+// other.  A lane has one part of one token's key, whose angles it works out once for all
+// heads, and one of its value; both stay in registers between the largest value and the codes,
+// and the next head's are on their way meanwhile.  Two meetings a head: for the largest values,
+// and where the values have been turned over.
+// Bound by latency: 16 waves a CU, whose 128 registers angles and values take; 8 x 4096 tokens,
+// 4 heads of 128 in bfloat16: PAGEFIG.
+// Workgroups from kv on turn `block` tokens' queries each.
+template <typename T, int THREADS>
+__global__ __launch_bounds__(THREADS, 4) void cache_page_kernel(Cache c, Sequences sq, Turn turn,
+                                                                AppendRows<T> r, int groups,
+                                                                int heads, int kv, int block) {
+  extern __shared__ double2 lds[];
+  if ((int)blockIdx.x >= kv) {
+    append_queries<T, THREADS, false>(c, sq, turn, r, (int64_t)((int)blockIdx.x - kv) * block,
+                                      block, (char*)lds);
+    return;
+  }
+  constexpr int WAVES = THREADS / 64;
+  AppendPage g(c, sq, blockIdx.x / groups);
+  if (g.none()) return;
+  const int NC = c.chunks, Dr = 16 * NC, pitch = c.page + 4;
   char* tile = (char*)lds;
-  const int tile_pitch = round + 4;
-  float* tops = (float*)(tile + (TEAMS == 1 ? tile_pitch * Dr : 0));
+  uint32_t* tops = (uint32_t*)(tile + pitch * Dr);
+  const int key_parts = Part::of_key(turn.pairs, Dr), parts = key_parts > NC ? key_parts : NC;
+  const int t = threadIdx.x / parts, part = threadIdx.x % parts;
+  const bool in = t >= g.a && t < g.z, has_k = in && part < key_parts, has_v = in && part < NC;
+  Part pk, pv;
+  pk.key(part < key_parts ? part : 0, turn, r.D, Dr);
+  pv.plain(16 * (part < NC ? part : 0), r.D, Dr);
+  const int64_t row = g.row0 + t;
+  const T *kr = r.k + row * r.k_row, *vr = r.v + row * r.v_row;
+  PartValues<T> uk = {}, uv = {};
+  const int h0 = (blockIdx.x % groups) * heads;
+  const int h1 = h0 + heads < c.Hk ? h0 + heads : c.Hk;
+  if (has_k) uk.load(kr + h0 * r.k_head, pk);
+  if (has_v) uv.load(vr + h0 * r.v_head, pv);
+  if (!g.there()) return;
+  double2 cs[8];
+  if (has_k && pk.pair >= 0) part_angles(pk, turn, r, g, t, cs);
+#pragma unroll 1
+  for (int h = h0; h < h1; ++h) {
+    pk.fresh();
+    pv.fresh();
+    const int64_t scale_at = (int64_t)g.number * c.Hk + h;
+    const bool older = g.a > 0;
+    const float old_k = older ? c.key_scales[scale_at] : 0.f;
+    const float old_v = older ? c.value_scales[scale_at] : 0.f;
+    float x[16];
+    bool rare_k = false, rare_v = false;
+    uint32_t top_k = 0, top_v = 0;
+    if (has_v) {
+      float y[16];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        y[e] = (float)uv.a.v[e];
+        y[8 + e] = (float)uv.b.v[e];
+      }
+      top_v = top16(y, rare_v);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    if (has_k) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        x[e] = (float)uk.a.v[e];
+        x[8 + e] = (float)uk.b.v[e];
+      }
+      if (pk.pair >= 0) turn_part<T>(uk, turn.interleaved, cs, x);
+      top_k = top16(x, rare_k);
+      if (h + 1 < h1) uk.load(kr + (h + 1) * r.k_head, pk);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    top_k = wave_top(top_k);
+    top_v = wave_top(top_v);
+    if (lane_id() == 0) {
+      tops[wave_id()] = top_k;
+      tops[WAVES + wave_id()] = top_v;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < WAVES; ++i) {
+      top_k = tops[i] > top_k ? tops[i] : top_k;
+      top_v = tops[WAVES + i] > top_v ? tops[WAVES + i] : top_v;
+    }
+    const int ek = page_exponent(top_k, older, old_k), ev = page_exponent(top_v, older, old_v);
+    const float fk = power(-ek), fv = power(-ev);
+    if (older && old_k != power(ek))
+      scale_older<THREADS>(c, c.keys, g.number, h, true, g.a, old_k * fk, threadIdx.x);
+    if (older && old_v != power(ev))
+      scale_older<THREADS>(c, c.values, g.number, h, false, g.a, old_v * fv, threadIdx.x);
+    uint32_t w[4];
+    if (has_k) {
+      codes16(x, fk, rare_k, pk.pair >= 0 && turn.interleaved, w);
+      uint8_t* to = c.keys + c.block(g.number, h, t / 32);
+      store_part(to, t % 32, pk.pa, pk.store_a, w[0], w[1]);
+      store_part(to, t % 32, pk.pb, pk.store_b, w[2], w[3]);
+    }
+    if (has_v) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        x[e] = (float)uv.a.v[e];
+        x[8 + e] = (float)uv.b.v[e];
+      }
+      codes16(x, fv, rare_v, false, w);
+      if (h + 1 < h1) uv.load(vr + (h + 1) * r.v_head, pv);
+      char* at = tile + part * 16 * pitch + t;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) at[e * pitch] = (char)(w[e / 4] >> 8 * (e % 4));
+    }
+    __syncthreads();
+    store_tile<THREADS>(c, tile, pitch, g, h, 0, c.page);
+    if (threadIdx.x == 0) {  // (after both meetings: every wave has read the old ones)
+      c.key_scales[scale_at] = power(ek);
+      c.value_scales[scale_at] = power(ev);
+    }
+  }
+}
+
+// Few tokens a page, or pages that are more than a workgroup's lanes: workgroups 0 .. kv - 1 take a
+// sequence's page and `heads` of its heads each, one team of TEAM lanes (a wave, or the
+// workgroup) a head; keys, then values.  `round` tokens go through at a time; where a page is
+// more than one round, it is loaded twice: for the largest value, then for the codes.  A wave
+// writes a value's sixteen rows of a block itself, a byte each.
+// Workgroups behind them turn `block` tokens' queries each.
+template <typename T, int THREADS, int TEAM>
+__global__ __launch_bounds__(THREADS, 2) void cache_append_kernel(Cache c, Sequences sq, Turn turn,
+                                                                  AppendRows<T> r, int groups,
+                                                                  int heads, int round, int kv,
+                                                                  int block) {
+  extern __shared__ double2 lds[];
+  if ((int)blockIdx.x >= kv) {
+    append_queries<T, THREADS, false>(c, sq, turn, r, (int64_t)((int)blockIdx.x - kv) * block,
+                                      block, (char*)lds);
+    return;
+  }
+  constexpr int TEAMS = THREADS / TEAM, WAVES = THREADS / 64;
+  AppendPage g(c, sq, blockIdx.x / groups);
+  if (g.none()) return;
+  const int NC = c.chunks, Dr = 16 * NC, pitch = round + 4;
+  char* tile = (char*)lds;
+  uint32_t* tops = (uint32_t*)(tile + (TEAMS == 1 ? pitch * Dr : 0));
   const int team = threadIdx.x / TEAM, lane = threadIdx.x % TEAM;
   const int key_parts = Part::of_key(turn.pairs, Dr), parts = key_parts > NC ? key_parts : NC;
   const int tok = lane / parts, part = lane % parts;
   // rounds begin at multiples of their length where the values' tile is turned over, so that a
   // round holds whole blocks
-  const int r0 = TEAMS == 1 ? a / round * round : a;
-  const int rounds = (z - r0 + round - 1) / round;
-  auto in = [&](int t0) { return tok < round && t0 + tok >= a && t0 + tok < z; };
+  const int r0 = TEAMS == 1 ? g.a / round * round : g.a;
+  const int rounds = (g.z - r0 + round - 1) / round;
+  auto in = [&](int t0) { return tok < round && t0 + tok >= g.a && t0 + tok < g.z; };
   Part pk, pv;
   pk.key(part < key_parts ? part : 0, turn, r.D, Dr);
   pv.plain(16 * (part < NC ? part : 0), r.D, Dr);
-  const bool has_k = part < key_parts, has_v = part < NC;
   double2 cs[8];
+  // A round's angles.  Teams of a workgroup have the same tokens: each lane works out one angle
+  // at a time for all of them, in LDS (a lane's eight one after the other are as much code to
+  // fetch and as long a wait for the only tokens there are).
   auto angles = [&](int t0) {
-    if (pk.pair < 0 || !in(t0)) return;
-    const int64_t row = row0 + t0 + tok;
+    const bool turned = part < key_parts && pk.pair >= 0 && in(t0);
+    if constexpr (TEAMS == 1) {
+      if (turned) part_angles(pk, turn, r, g, t0 + tok, cs);
+    } else {
+      const int n = g.z - t0 < round ? g.z - t0 : round;
+      __syncthreads();
+#pragma unroll 1
+      for (int i = threadIdx.x; i < n * turn.pairs; i += THREADS) {
+        const int t = t0 + i / turn.pairs, j = i % turn.pairs;
+        double sn, co;
+        sine_cosine((r.places ? turn.place(g.row0 + t, j) : (double)(g.base + t)) * turn.f[j], sn, co);
+        lds[i] = make_double2(co * turn.m, sn * turn.m);
+      }
+      __syncthreads();
+      if (turned)
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const int j = pk.pair + e < turn.pairs ? pk.pair + e : pk.pair;
-      cs[e].x = (r.places ? turn.place(row, j) : (double)(base + t0 + tok)) * turn.f[j];
-    }
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      double sn, co;
-      sine_cosine(cs[e].x, sn, co);
-      cs[e] = make_double2(co * turn.m, sn * turn.m);
-      if (e % 2) __builtin_amdgcn_sched_barrier(0);  // (eight at once: 200 registers)
+        for (int e = 0; e < 8; ++e)
+          cs[e] = lds[tok * turn.pairs + (pk.pair + e < turn.pairs ? pk.pair + e : pk.pair)];
     }
   };
 
   const int h0 = (blockIdx.x % groups) * heads;
   const int h1 = h0 + heads < c.Hk ? h0 + heads : c.Hk;
   // job 2 i: keys of the team's head i of these, job 2 i + 1: its values
-  PartValues<T> u;
+  const int jobs = 2 * ((h1 - h0 + TEAMS - 1) / TEAMS);
+  PartValues<T> u = {};
   auto load = [&](int job, int t0) {
     const int h = h0 + (job >> 1) * TEAMS + team;
     if (!in(t0) || h >= h1) return;
-    const int64_t row = row0 + t0 + tok;
+    const int64_t row = g.row0 + t0 + tok;
     if (job & 1) {
-      if (has_v) u.load(r.v + row * r.v_row + h * r.v_head, pv);
-    } else if (has_k) {
+      if (part < NC) u.load(r.v + row * r.v_row + h * r.v_head, pv);
+    } else if (part < key_parts) {
       u.load(r.k + row * r.k_row + h * r.k_head, pk);
     }
   };
   auto old_scale = [&](int job) {
     const int h = h0 + (job >> 1) * TEAMS + team;
-    return a > 0 && h < h1 ? (job & 1 ? c.value_scales : c.key_scales)[(int64_t)number * c.Hk + h]
-                           : 0.f;
+    return g.a > 0 && h < h1
+               ? (job & 1 ? c.value_scales : c.key_scales)[(int64_t)g.number * c.Hk + h]
+               : 0.f;
   };
-  const int jobs = 2 * ((h1 - h0 + TEAMS - 1) / TEAMS);
   load(0, r0);
+  if (!g.there()) return;
   float next_old = old_scale(0);
-  if (!MANY || rounds == 1) angles(r0);
+  if (rounds == 1) angles(r0);
 #pragma unroll 1
   for (int job = 0; job < jobs; ++job) {
     pk.fresh();
     pv.fresh();
     const bool key = !(job & 1);
     const int h = h0 + (job >> 1) * TEAMS + team;
-    const bool mine = h < h1, has = mine && (key ? has_k : has_v);
-    const int64_t scale_at = (int64_t)number * c.Hk + (mine ? h : h1 - 1);
-    float* scale_p = (key ? c.key_scales : c.value_scales) + scale_at;
+    const bool mine = h < h1, has = mine && part < (key ? key_parts : NC);
     uint8_t* codes = key ? c.keys : c.values;
     const float old = next_old;
     if (job + 1 < jobs) next_old = old_scale(job + 1);
-    float top = 0.f, f = 0.f;
-    float x[16];
+    uint32_t top = 0;
+    float x[16], f = 0.f;
     bool rare = false;
     auto take = [&](int t0) {  // what was loaded as the cache takes it
 #pragma unroll
@@ -395,67 +646,42 @@ __global__ __launch_bounds__(THREADS, MANY ? 2 : 4) void cache_append_kernel(
         x[e] = (float)u.a.v[e];
         x[8 + e] = (float)u.b.v[e];
       }
-      if (key && pk.pair >= 0) turn_part<T>(u, turn.interleaved, cs, x);
+      if (has && in(t0) && key && pk.pair >= 0) turn_part<T>(u, turn.interleaved, cs, x);
     };
-    auto measure = [&](int t0) {  // the largest of what is finite
+    auto measure = [&](int t0) {
       if (!has || !in(t0)) return;
-      uint32_t most = 0;
-#pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const uint32_t b = __builtin_bit_cast(uint32_t, x[e]) & 0x7fffffff;
-        most = b > most ? b : most;
-      }
-      rare = most >= 0x7f800000;
-      if (rare) {
-        most = 0;
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const uint32_t b = __builtin_bit_cast(uint32_t, x[e]) & 0x7fffffff;
-          most = b > most && b < 0x7f800000 ? b : most;
-        }
-      }
-      top = fmaxf(top, __builtin_bit_cast(float, most));
+      const uint32_t y = top16(x, rare);
+      top = y > top ? y : top;
     };
     auto settle = [&] {  // the page's scale; older codes brought to it
-      top = wave_max(top);
+      top = wave_top(top);
       if (TEAMS == 1) {
         __syncthreads();
         if (lane_id() == 0) tops[wave_id()] = top;
         __syncthreads();
 #pragma unroll
-        for (int i = 0; i < THREADS / 64; ++i) top = fmaxf(top, tops[i]);
+        for (int i = 0; i < WAVES; ++i) top = tops[i] > top ? tops[i] : top;
       }
-      int e = exponent_for(top);
-      if (a > 0) {
-        const int o = exponent_of(old);
-        e = o > e ? o : e;
-      }
+      const int e = page_exponent(top, g.a > 0, old);
       f = power(-e);
-      if (a > 0 && mine && old != power(e))
-        scale_older<TEAM>(c, codes, number, h, key, a, old * f, lane);
-      if (mine && lane == 0) *scale_p = power(e);
+      if (g.a > 0 && mine && old != power(e))
+        scale_older<TEAM>(c, codes, g.number, h, key, g.a, old * f, lane);
+      if (mine && lane == 0)
+        (key ? c.key_scales : c.value_scales)[(int64_t)g.number * c.Hk + h] = power(e);
     };
     auto store = [&](int t0) {
       if (has && in(t0)) {
         const int t = t0 + tok;
-        uint8_t* to = codes + c.block(number, h, t / 32);
         uint32_t w[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) w[e] = codes4(x + 4 * e, f, rare || f == power(-E_MOST));
-        if (key && pk.pair >= 0 && turn.interleaved) {  // pairs side by side again
-          const uint32_t p[4] = {w[0], w[1], w[2], w[3]};
-          w[0] = __builtin_amdgcn_perm(p[2], p[0], 0x05010400);
-          w[1] = __builtin_amdgcn_perm(p[2], p[0], 0x07030602);
-          w[2] = __builtin_amdgcn_perm(p[3], p[1], 0x05010400);
-          w[3] = __builtin_amdgcn_perm(p[3], p[1], 0x07030602);
-        }
+        codes16(x, f, rare, key && pk.pair >= 0 && turn.interleaved, w);
+        uint8_t* to = codes + c.block(g.number, h, t / 32);
         if (key) {
           store_part(to, t % 32, pk.pa, pk.store_a, w[0], w[1]);
           store_part(to, t % 32, pk.pb, pk.store_b, w[2], w[3]);
         } else if (TEAMS == 1) {
-          char* at = tile + part * 16 * tile_pitch + tok;
+          char* at = tile + part * 16 * pitch + tok;
 #pragma unroll
-          for (int e = 0; e < 16; ++e) at[e * tile_pitch] = (char)(w[e / 4] >> 8 * (e % 4));
+          for (int e = 0; e < 16; ++e) at[e * pitch] = (char)(w[e / 4] >> 8 * (e % 4));
         } else {
           to += part * 512 + t % 32;
 #pragma unroll
@@ -464,25 +690,14 @@ __global__ __launch_bounds__(THREADS, MANY ? 2 : 4) void cache_append_kernel(
       }
       if (TEAMS == 1 && !key) {
         __syncthreads();
-        for (int i = threadIdx.x; i < round / 16 * Dr; i += THREADS) {
-          const int half = i & 1, d = (i >> 1) % Dr, blk = (i >> 1) / Dr;
-          const int lt = 32 * blk + 16 * half, t = t0 + lt;
-          if (t + 16 <= a || t >= z) continue;
-          uint8_t* to = codes + c.block(number, h, t / 32) + d * 32 + t % 32;
-          const uint32_t* at = (const uint32_t*)(tile + d * tile_pitch + lt);
-          if (t >= a && t + 16 <= z)
-            *(uint4*)to = make_uint4(at[0], at[1], at[2], at[3]);
-          else
-            for (int e = 0; e < 16; ++e)
-              if (t + e >= a && t + e < z) to[e] = ((const uint8_t*)at)[e];
-        }
+        store_tile<THREADS>(c, tile, pitch, g, h, t0, round);
         __syncthreads();
       }
     };
-    if (!MANY || rounds == 1) {
+    if (rounds == 1) {
       take(r0);
-      if (job + 1 < jobs) load(job + 1, r0);
       measure(r0);
+      if (job + 1 < jobs) load(job + 1, r0);
       settle();
       store(r0);
     } else {
@@ -607,34 +822,31 @@ extern "C" int tpo_cache_append(int dtype, const void* k, const void* v, const v
     typedef decltype(e) E;
     const AppendRows<E> r{(const E*)k, (const E*)v, (const E*)q, (E*)q_out, k_row, k_head, v_row,
                           v_head, q_row, q_head, (int)Hq, (int)D, places ? 1 : 0};
-    if (few) {
-      cache_append_kernel<E, APPEND_THREADS, 64, true>
-          <<<dim3((unsigned)(kv + q_blocks)), APPEND_THREADS, (size_t)q_lds, s>>>(
-              c, sq, t, r, (int)groups, (int)heads, append_round(c, t, 64, false), kv, (int)block);
-      return;
-    }
-    auto launch = [&](auto threads, auto many) {
+    const bool apart = !few && T * Hq * D * element_bytes(dtype) > TURN_STREAM;
+    const unsigned blocks = (unsigned)(kv + (apart ? 0 : q_blocks));
+    auto bytes = [&](int64_t n) { return (size_t)(n > q_lds ? n : q_lds); };
+    auto pages_of = [&](auto threads) {
       constexpr int N = decltype(threads)::value;
-      const int round = append_round(c, t, N, true);
-      cache_append_kernel<E, N, N, decltype(many)::value>
-          <<<dim3((unsigned)kv), N, (size_t)((round + 4) * Dr + 64), s>>>(
-              c, sq, t, r, (int)groups, (int)heads, round, kv, 0);
+      cache_page_kernel<E, N><<<blocks, N, bytes((page + 4) * Dr + 64), s>>>(
+          c, sq, t, r, (int)groups, (int)heads, kv, (int)block);
     };
-    if (append_round(c, t, 256, true) >= page)
-      launch(std::integral_constant<int, 256>(), std::false_type());
-    else if (append_round(c, t, 512, true) >= page)
-      launch(std::integral_constant<int, 512>(), std::false_type());
-    else
-      launch(std::integral_constant<int, 512>(), std::true_type());
-    if (!q) return;
-    auto turn_queries = [&](auto streaming) {
-      cache_queries_kernel<E, decltype(streaming)::value>
-          <<<dim3((unsigned)q_blocks), APPEND_THREADS, (size_t)q_lds, s>>>(c, sq, t, r, (int)block);
-    };
-    if (T * Hq * D * element_bytes(dtype) > TURN_STREAM)
-      turn_queries(std::true_type());
-    else
-      turn_queries(std::false_type());
+    if (few) {
+      const int round = append_round(c, t, 64, false);
+      cache_append_kernel<E, 256, 64>
+          <<<blocks, 256, bytes((int64_t)round * pairs * sizeof(double2)), s>>>(
+              c, sq, t, r, (int)groups, (int)heads, round, kv, (int)block);
+    } else if (append_round(c, t, 256, true) >= page) {
+      pages_of(std::integral_constant<int, 256>());
+    } else if (append_round(c, t, 512, true) >= page) {
+      pages_of(std::integral_constant<int, 512>());
+    } else {
+      const int round = append_round(c, t, 512, true);
+      cache_append_kernel<E, 512, 512><<<blocks, 512, bytes((round + 4) * Dr + 64), s>>>(
+          c, sq, t, r, (int)groups, (int)heads, round, kv, (int)block);
+    }
+    if (apart && q)
+      cache_queries_kernel<E><<<dim3((unsigned)q_blocks), 256, (size_t)q_lds, s>>>(c, sq, t, r,
+                                                                                   (int)block);
   });
   return check_launch(op);
 }
