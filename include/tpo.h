@@ -507,6 +507,8 @@ int tpo_rotary(int dtype, const void* x, int64_t tokens, int64_t heads, int64_t 
  *   What lies behind a sequence's last token is read but never counts, whatever
  *   it holds.  q as the packed attention takes it.
  * Workspaces are 256-byte aligned; size 0 means none is used.
+ * tpo_cache_attention_rows is a diagnostic, as tpo_attention_fwd_rows: 128 where a
+ *   workgroup converts its codes once for as many rows, else 32.
  */
 int tpo_cache_append(int dtype, const void* k, const void* v, const void* q,
                      const int64_t* offsets, const int64_t* lengths_new, int64_t B,
@@ -520,6 +522,8 @@ int tpo_cache_append(int dtype, const void* k, const void* v, const void* q,
                      void* q_out, void* stream);
 int64_t tpo_cache_attention_workspace_size(int dtype, int64_t B, int64_t T, int64_t Hq,
                                            int64_t Hk, int64_t D, int64_t page, int64_t M);
+int tpo_cache_attention_rows(int dtype, int64_t B, int64_t T, int64_t Hq, int64_t Hk,
+                             int64_t D, int64_t page, int64_t M);
 int tpo_cache_attention(int dtype, const void* q, const int64_t* offsets,
                         const int64_t* lengths_q, int64_t B, int64_t T, int64_t Hq,
                         int64_t D, int64_t q_row, int64_t q_head, const void* keys,

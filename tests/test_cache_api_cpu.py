@@ -256,3 +256,23 @@ def test_attention_entry(lib):
     assert call(_4=1, _5=1, _20=256) == -4 and b"workspace" in lib.tpo_last_error()
     assert size(0, 1, 1, 3, 2, 32, 64, 4) == -1 and size(1, 1, 1, 4, 2, 32, 64, 4) == -1
     assert call(_4=1 << 24, _5=(1 << 29) - 1) == -1 and b"too many rows" in lib.tpo_last_error()
+
+
+def test_attention_kernels_of_the_gpu_tests(lib):
+    """Which kernel the sizes of tests/test_cached_attention_gpu.py take, so that no change of the
+    rule leaves one of them without its tests."""
+    from tests import test_cached_attention_gpu as t
+
+    lib.tpo_cache_attention_rows.argtypes = [C] + [I] * 7
+
+    def rows(dtype, new, lengths, Hq, Hk, size, page=64, more=0):
+        return lib.tpo_cache_attention_rows(dtype, len(new), sum(new) + more, Hq, Hk, size, page,
+                                            max(1, -(-max(lengths) // page)))
+
+    for dtype in (0, 2, 3):
+        for new, lengths, Hk in t.PROMPTS:
+            assert rows(dtype, new, lengths, 2 * Hk, Hk, 64, more=7) == 128
+        assert rows(dtype, [40] * 10, [400], 16, 16, 40) == 128
+        for new, lengths in t.CASES:
+            assert rows(dtype, new, lengths, 4, 2, 64) == 32
+    assert rows(0, [4], [4], 3, 2, 16) == -1 and rows(1, [4], [4], 2, 2, 16) == -2

@@ -220,6 +220,71 @@ def test_strides(tpo, dev, dtype):
                   roundings=2)
 
 
+# What takes the kernel of 128 rows a workgroup (tests/test_cache_api_cpu.py looks the rule up):
+# sequences' new tokens and tokens, heads of the cache.
+PROMPTS = [([40] * 20, [40 + 7 * b for b in range(20)], 8),
+           ([129, 1, 0, 200, 64, 63], [129, 70, 5, 260, 64, 200], 16),
+           ([33] * 70, [33 + 3 * b for b in range(70)], 4),
+           ([300, 212], [700, 3000], 20)]
+
+
+@pytest.mark.parametrize("which", range(4))
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("causal", [True, False])
+def test_prompts(tpo, dev, which, dtype, causal):
+    new, lengths, Hk = PROMPTS[which]
+    _check(tpo, dev, new, lengths, 2 * Hk, Hk, 64, dtype, causal=causal, seed=which, before=3,
+           after=4)
+
+
+@pytest.mark.parametrize("D", [1, 16, 20, 32, 40, 63, 72, 80, 96, 100, 127, 128])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_prompts_head_sizes(tpo, dev, D, dtype):
+    _check(tpo, dev, [40] * 10, [40 + 9 * b for b in range(10)], 16, 16, D, dtype, seed=D,
+           page=32 if D % 3 else 96)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_prompts_levels_scales_and_rows(tpo, dev, dtype):
+    new, lengths = [40] * 10, [40 + 30 * b for b in range(10)]
+    for scale in (-0.2, 0.0, 0.5):
+        _check(tpo, dev, new, lengths, 32, 16, 32, dtype, seed=3, spread=3.0, scale=scale)
+    _check(tpo, dev, new, lengths, 32, 16, 32, dtype, lq=[3 * b for b in range(10)], seed=4)
+    _check(tpo, dev, new, [4 * b for b in range(10)], 32, 16, 32, dtype, seed=5)
+    cache = cache64.paged(tpo, dev, lengths, 16, 32, 32, seed=6)
+    cache.table[3, 1], cache.table[5, 0], cache.table[8] = -1, 10 ** 6, -5
+    cache.lengths[9] = 10 ** 12
+    _check(tpo, dev, new, None, 32, 16, 32, dtype, cache=cache, seed=6)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_prompts_nan(tpo, dev, dtype):
+    """As test_nan_reaches_those_that_see_it and test_what_lies_behind_counts_for_nothing, by the
+    other kernel."""
+    new, lengths = [40] * 10, [100] * 10
+    for which in ("keys", "values"):
+        for place in (70, 95, 99):
+            cache = cache64.paged(tpo, dev, lengths, 16, 32, 64, seed=16)
+            q = _q(400, 16, 32, dtype, 16).to(dev)
+            o = torch.tensor(_offsets(new), device=dev)
+            clean = tpo.cached_attention(q, cache, o)
+            p, s = int(cache.table[4, place // 64]), place % 64
+            if which == "keys":
+                cache.keys.view(torch.uint8)[p, 3, s // 32, 0, s % 32, 5] = 0x7f
+            else:
+                cache.values.view(torch.uint8)[p, 3, s // 32, 5, s % 32] = 0xff
+            p = int(cache.table[4, 1])  # behind the sequence's last place
+            cache.keys.view(torch.uint8)[p, :, 1, :, 4:] = 0x7f
+            cache.values.view(torch.uint8)[p, :, 1, :, 4:] = 0x7f
+            got = tpo.cached_attention(q, cache, o)
+            first = 160 + place - 60  # the row whose own token it is
+            bad = got[first:200, 3].isnan()
+            assert bad[..., 5].all()
+            assert bad.all() if which == "keys" else not bad[..., torch.arange(32) != 5].any()
+            got[first:200, 3] = clean[first:200, 3]
+            assert torch.equal(got, clean)
+
+
 def test_past_32_bits(tpo, dev):
     """Pages beyond 2^31 and 2^32 bytes of the pool, written and read."""
     P, Hk, D, page = 140000, 1, 128, 256  # 32 KB a page and head: 4.6 GB of keys

@@ -53,9 +53,9 @@ __device__ __forceinline__ uint32_t nan_codes(uint32_t x) {
   return ((x & 0x7f7f7f7f) + 0x01010101) & 0x80808080;
 }
 
-// A wave's 32 rows of q as the products take them: of values 32 s + 16 (l / 32) + 8 e .. + 7
-// (e = 0, 1), in PARTS parts.
-template <typename T, int DP>
+// A wave's 32 rows of q as the products take them, in PARTS parts: of values 32 s + 16 (l / 32) +
+// 8 e .. + 7 (e = 0, 1; codes straight from memory), or ROWS: 16 s + 8 (l / 32) .. + 7 (from LDS).
+template <typename T, int DP, bool ROWS = false>
 struct CodeRows {
   typedef typename CodeType<T>::E E;
   typedef typename Chunk<E>::V V;
@@ -65,7 +65,7 @@ struct CodeRows {
     const int h = lane_id() >> 5;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const int d = 32 * (i / 2) + 16 * h + 8 * (i % 2);
+      const int d = ROWS ? 16 * i + 8 * h : 32 * (i / 2) + 16 * h + 8 * (i % 2);
       float y[8];
 #pragma unroll
       for (int e = 0; e < 8; e += 16 / sizeof(T)) {
@@ -167,7 +167,22 @@ struct CodeSums {
 #pragma unroll
     for (int e = 1; e < 16; ++e) top = fmaxf(top, s[e]);
     top = __builtin_fmaf(top, f, lv);
-    top = fmaxf(top, other_half(top));
+    follow(fmaxf(top, other_half(top)));
+    weigh(s, f, lv);
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      typename Chunk<E>::V p[PARTS];
+      parts(s, e, p);
+#pragma unroll
+      for (int i = 0; i < DP / 32; ++i) {
+        const auto x = from_codes<E>(t.v[i][2 * e], t.v[i][2 * e + 1]);
+#pragma unroll
+        for (int part = 0; part < PARTS; ++part) mma(acc[i], x, p[part]);
+      }
+    }
+  }
+  // The maximum follows where it grows by more than 2^8.
+  __device__ __forceinline__ void follow(float top) {
     if (__builtin_amdgcn_ballot_w64(top - m > 8.f)) {
       const float m2 = fmaxf(m, top);
       const float a = m2 == NEG_INF ? 1.f : __builtin_amdgcn_exp2f(m - m2);
@@ -178,6 +193,9 @@ struct CodeSums {
 #pragma unroll
         for (int e = 0; e < 16; ++e) acc[i][e] *= a;
     }
+  }
+  // Scores to weights, and their part of the row's sum.
+  __device__ __forceinline__ void weigh(f32x16& s, float f, float lv) {
     const float b = m == NEG_INF ? 0.f : lv - m;
     float sum = 0.f;
 #pragma unroll
@@ -186,24 +204,18 @@ struct CodeSums {
       sum += s[e];
     }
     l = __builtin_fmaf(sum, lv == NEG_INF ? 0.f : __builtin_amdgcn_exp2f(-lv), l);
+  }
+  // Weights 8 e .. + 7 in the products' type.
+  static __device__ __forceinline__ void parts(const f32x16& s, int e,
+                                               typename Chunk<E>::V (&p)[PARTS]) {
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      typename Chunk<E>::V p[PARTS];
+    for (int y = 0; y < 8; ++y) {
+      float r = s[8 * e + y];
 #pragma unroll
-      for (int y = 0; y < 8; ++y) {
-        float r = s[8 * e + y];
-#pragma unroll
-        for (int part = 0; part < PARTS; ++part) {
-          const E z = (E)r;
-          p[part][y] = z;
-          r -= (float)z;
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < DP / 32; ++i) {
-        const auto x = from_codes<E>(t.v[i][2 * e], t.v[i][2 * e + 1]);
-#pragma unroll
-        for (int part = 0; part < PARTS; ++part) mma(acc[i], x, p[part]);
+      for (int part = 0; part < PARTS; ++part) {
+        const E z = (E)r;
+        p[part][y] = z;
+        r -= (float)z;
       }
     }
   }
@@ -259,18 +271,54 @@ __device__ __forceinline__ int cache_keys(int r, int G, int n, int length, int c
   return k < 0 ? 0 : (k > length ? length : k);
 }
 
+// A wave's sums as another wave takes them, lane by lane: both have the same rows and columns.
+template <typename T, int DP>
+struct WaveSums {
+  float4 acc[DP / 8][64];
+  float m[64], l[64];
+
+  __device__ __forceinline__ void put(const CodeSums<T, DP>& s) {
+    const int l = lane_id();
+#pragma unroll
+    for (int i = 0; i < DP / 8; ++i)
+      acc[i][l] = make_float4(s.acc[i / 4][4 * (i % 4)], s.acc[i / 4][4 * (i % 4) + 1],
+                              s.acc[i / 4][4 * (i % 4) + 2], s.acc[i / 4][4 * (i % 4) + 3]);
+    m[l] = s.m;
+    this->l[l] = s.l;
+  }
+  // Adds them to s.  Rows that have seen nothing have m = -inf and sums of 0.
+  __device__ __forceinline__ void add_to(CodeSums<T, DP>& s) const {
+    const int l = lane_id();
+    const float mo = m[l], top = fmaxf(s.m, mo);
+    const float f = s.m == NEG_INF ? 0.f : __builtin_amdgcn_exp2f(s.m - top);
+    const float g = mo == NEG_INF ? 0.f : __builtin_amdgcn_exp2f(mo - top);
+    s.m = top;
+    s.l = __builtin_fmaf(s.l, f, this->l[l] * g);
+#pragma unroll
+    for (int i = 0; i < DP / 8; ++i) {
+      const float4 o = acc[i][l];
+      const float y[4] = {o.x, o.y, o.z, o.w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int at = 4 * (i % 4) + e;
+        s.acc[i / 4][at] = __builtin_fmaf(s.acc[i / 4][at], f, y[e] * g);
+      }
+    }
+  }
+};
+
 // A workgroup takes 32 rows (tokens times the heads of a group, as the packed attention's) and
 // one of gridDim.z shares of their keys, its four waves in turn a tile of 32 keys each.  A tile
 // goes from memory to registers, the next one is on its way while one is multiplied; LDS is
-// used at the end only, where the waves' sums come together.
-// part, ml: see attn_step_kernel; m is in the exponent of 2, the values' scales with it.
+// used at the end only, where the waves' sums come together, two and two.
+// part, ml: see attn_join_kernel; m is in the exponent of 2, the values' scales with it.
 constexpr int CODE_WAVES = 4;
 template <typename T, int DP>
 __global__ __launch_bounds__(64 * CODE_WAVES, (DP * sizeof(T) <= 256 ? 2 : 1)) void
 cache_step_kernel(CacheAttnArgs a, const T* __restrict__ q, T* __restrict__ out,
                   float* __restrict__ part, float2* __restrict__ ml) {
-  constexpr int W = CODE_WAVES, P = DP + 4;
-  __shared__ float sums[W * 32 * P], ms[W][32], ls[W][32];
+  constexpr int W = CODE_WAVES;
+  __shared__ WaveSums<T, DP> lds[2];
   const int G = a.Hq / a.c.Hk, hk = blockIdx.y, shares = gridDim.z;
   const CacheRows p = cache_rows(a.sq, a.c, blockIdx.x, [G](int64_t start, int s) {
     return start * G / 32 + s;
@@ -323,66 +371,330 @@ cache_step_kernel(CacheAttnArgs a, const T* __restrict__ q, T* __restrict__ out,
     }
   }
 
-  // the waves' sums together
-  const float sum = rows.l + other_half(rows.l);
-  float* mysums = sums + w * 32 * P;
-#pragma unroll
-  for (int i = 0; i < DP / 32; ++i)
-#pragma unroll
-    for (int b = 0; b < 4; ++b) {
-      Four<float> f;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) f.v[e] = rows.acc[i][4 * b + e];
-      *(Four<float>*)(mysums + (l & 31) * P + 32 * i + 8 * b + 4 * (l >> 5)) = f;
-    }
-  if (l < 32) {
-    ms[w][l] = rows.m;
-    ls[w][l] = sum;
-  }
+  if (w >= 2) lds[w - 2].put(rows);
   __syncthreads();
-  constexpr int PER_ROW = 2 * W, D1 = DP / PER_ROW;  // lanes a row, values a lane
-  const int rr = threadIdx.x / PER_ROW, d0 = threadIdx.x % PER_ROW * D1, row = r0 + rr;
-  if (row >= all) return;
-  float m = NEG_INF, total = 0.f, f[W];
+  if (w < 2) lds[w].add_to(rows);
+  __syncthreads();
+  if (w == 1) lds[0].put(rows);
+  __syncthreads();
+  if (w != 0 || r >= all) return;
+  lds[0].add_to(rows);
+  float total = rows.l + other_half(rows.l);
+  if (r >= used) total = 0.f;
+  const int64_t at = (p.first + r / G) * a.Hq + hk * G + r % G;
+  const int64_t to = shares > 1 ? at * shares + blockIdx.z : at;
+  const float inv = total == 0.f ? 0.f : shares > 1 ? 1.f : 1.f / total;
+  if (shares == 1 || total != 0.f)
 #pragma unroll
-  for (int i = 0; i < W; ++i) m = fmaxf(m, ms[i][rr]);
+    for (int i = 0; i < DP / 8; ++i) {
+      const int d = 32 * (i / 4) + 8 * (i % 4) + 4 * (l >> 5);
+      float y[4];
 #pragma unroll
-  for (int i = 0; i < W; ++i) {
-    const float y = ls[i][rr];
-    f[i] = y == 0.f ? 0.f : __builtin_amdgcn_exp2f(ms[i][rr] - m);
-    total += f[i] * y;
-  }
-  if (row >= used) total = 0.f;
-  const int64_t at = (p.first + row / G) * a.Hq + hk * G + row % G;
-  const float inv = shares > 1 ? 1.f : total != 0.f ? 1.f / total : 0.f;
-#pragma unroll
-  for (int d = 0; d < D1; ++d) {
-    float y = 0.f;
-#pragma unroll
-    for (int i = 0; i < W; ++i)
-      if (f[i] != 0.f) y += f[i] * sums[(i * 32 + rr) * P + d0 + d];
-    if (d0 + d < a.D) {
+      for (int e = 0; e < 4; ++e)
+        y[e] = inv == 0.f ? 0.f : rows.acc[i / 4][4 * (i % 4) + e] * inv;
+      if (d >= a.D) continue;  // (D is a multiple of four)
       if (shares > 1) {
-        if (total != 0.f) part[(at * shares + blockIdx.z) * a.D + d0 + d] = y;
+        *(float4*)(part + to * a.D + d) = make_float4(y[0], y[1], y[2], y[3]);
       } else {
-        out[at * a.D + d0 + d] = total == 0.f ? (T)0.f : (T)(y * inv);
+        Four<T> f;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) f.v[e] = (T)y[e];
+        *(Four<T>*)(out + to * a.D + d) = f;
       }
     }
-  }
-  if (d0 == 0 && shares > 1) ml[at * shares + blockIdx.z] = make_float2(m, total);
+  if (shares > 1 && l < 32) ml[to] = make_float2(rows.m, total);
 }
 
-// How many workgroups share the keys of 32 rows.
-int cache_shares(int64_t B, int64_t T, int64_t room, int64_t Hq, int64_t Hk) {
+// Prompts over a cache: a workgroup of four waves takes 128 rows, 32 a wave, and their keys in
+// tiles of 64, which its waves load (a quarter each, two tiles ahead), turn into the products'
+// type and put into LDS for all four: a code is converted once for 128 rows, where the kernel
+// above does it for 32 (8 sequences of up to 8192, 1024 new tokens, 16 heads on 4, D = 128 in
+// bfloat16: PROMPTFIG).  Keys lie in LDS in the order of the product's rows in which a lane
+// receives the scores of sixteen tokens in a row; values by value, 64 tokens each, so that
+// sixteen bytes are what a product sums over.  Chunks of 16 bytes change places with the row, as
+// in HeadLds, so that a read touches all banks.
+template <typename T, int DP>
+struct alignas(1024) CodeLds {
+  typedef typename CodeType<T>::E E;
+  static constexpr int PITCH = HeadLds<E, DP>::PITCH, KEYS_AT = 64 * PITCH;
+  static constexpr int TILE = KEYS_AT + DP * 128, OUT = 4 * Rows32<T, DP>::BYTES;
+  char b[2 * TILE > OUT ? 2 * TILE : OUT];
+};
+
+// A wave's quarter of a tile on its way: every other KB of one of its two blocks.
+template <typename T, int DP>
+struct CodeLoads {
+  typedef typename CodeType<T>::E E;
+  typedef CodeLds<T, DP> L;
+  static constexpr int ALL = DP / 32, N = (ALL + 1) / 2;
+  u32x4 k[N], v[N];
+
+  __device__ __forceinline__ void load(const Cache& c, int64_t at, bool there, int u) {
+    const int bytes = there ? 512 * c.chunks : 0;
+    const auto kr = buffer(c.keys + at, bytes), vr = buffer(c.values + at, bytes);
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+      if (2 * j + u < ALL) {
+        k[j] = __builtin_amdgcn_raw_buffer_load_b128(kr, lane_id() * 16, (2 * j + u) * 1024, 0);
+        v[j] = __builtin_amdgcn_raw_buffer_load_b128(vr, lane_id() * 16, (2 * j + u) * 1024, 0);
+      }
+  }
+  // To the tile at lds, of which it is block `block`; `left` places of that are the sequence's.
+  __device__ __forceinline__ void put(char* lds, int block, int u, int left) {
+    typedef typename Chunk<E>::V V;
+    const int l = lane_id();
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const int i = 2 * j + u;
+      if (i >= ALL) continue;
+      const int token = l & 31, c = 2 * i + (l >> 5);  // chunk c of a key
+      const int row = 32 * block + 8 * (token >> 2 & 3) + 4 * (token >> 4) + (token & 3);
+      const int swap = HeadLds<E, DP>::swap(row);
+      char* to = lds + row * L::PITCH;
+      *(V*)(to + ((2 * c ^ swap) << 4)) = from_codes<E>(k[j][0], k[j][1]);
+      *(V*)(to + (((2 * c + 1) ^ swap) << 4)) = from_codes<E>(k[j][2], k[j][3]);
+      const int d = 32 * i + (l >> 1), half = l & 1;  // sixteen tokens of a value
+      if (left < 32) {
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          const int n = left - 16 * half - 4 * w;
+          v[j][w] &= n >= 4 ? ~0u : (n <= 0 ? 0u : (1u << 8 * n) - 1);
+        }
+      }
+      const int at = 4 * block + 2 * half, turn = d >> 1 & 7;
+      to = lds + L::KEYS_AT + d * 128;
+      *(V*)(to + ((at ^ turn) << 4)) = from_codes<E>(v[j][0], v[j][1]);
+      *(V*)(to + (((at + 1) ^ turn) << 4)) = from_codes<E>(v[j][2], v[j][3]);
+    }
+  }
+};
+
+// Values of a chunk that are NaN taken out; their places as ones.
+template <typename V>
+__device__ __forceinline__ V nan_places(V& x) {
+  V at = {};
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const bool bad = x[e] != x[e];
+    at[e] = bad ? 1.f : 0.f;
+    if (bad) x[e] = 0.f;
+  }
+  return at;
+}
+
+// The tiles' work of a wave.
+template <typename T, int DP>
+struct CodePrompt {
+  typedef typename CodeType<T>::E E;
+  typedef typename Chunk<E>::V V;
+  typedef CodeLds<T, DP> L;
+  static constexpr int PARTS = CodeType<T>::PARTS;
+  CodeSums<T, DP> sums;
+  HeadLanes<E, DP> lanes;
+
+  // values 32 i + l % 32, tokens 32 t + 16 (l / 32) + 8 e .. + 7 of the tile
+  __device__ __forceinline__ V value(const char* lds, int t, int e, int i) const {
+    const int l = lane_id(), r = l & 31;
+    return *(const V*)(lds + L::KEYS_AT + (32 * i + r) * 128 +
+                       (((4 * t + 2 * (l >> 5) + e) ^ (r >> 1 & 7)) << 4));
+  }
+  // The keys j0 .. j0 + 63 at lds, of which the lane's row sees those below n.  f, lv: of the
+  // two blocks, see CodeSums.
+  __device__ __forceinline__ void add(const char* lds, const CodeRows<T, DP, true>& q, int j0,
+                                      int n, bool masked, const float (&f)[2],
+                                      const float (&lv)[2]) {
+    f32x16 s[2] = {};
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int c = 0; c < DP / 16; ++c) {
+        const V x = lanes.by_row(lds + 32 * t * L::PITCH, c);
+#pragma unroll
+        for (int p = 0; p < PARTS; ++p) mma(s[t], x, q.x[p][c]);
+      }
+    const int first = j0 + 16 * (lane_id() >> 5);
+    if (masked)
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          if (first + 32 * t + e >= n) s[t][e] = NEG_INF;
+    float top = NEG_INF;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      float y = s[t][0];
+#pragma unroll
+      for (int e = 1; e < 16; ++e) y = fmaxf(y, s[t][e]);
+      top = fmaxf(top, __builtin_fmaf(y, f[t], lv[t]));
+    }
+    sums.follow(fmaxf(top, other_half(top)));
+#pragma unroll
+    for (int t = 0; t < 2; ++t) sums.weigh(s[t], f[t], lv[t]);
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        V p[PARTS];
+        sums.parts(s[t], e, p);
+        V sees;
+        if (masked)
+#pragma unroll
+          for (int y = 0; y < 8; ++y) sees[y] = (E)(first + 32 * t + 8 * e + y < n ? 1.f : 0.f);
+#pragma unroll
+        for (int i = 0; i < DP / 32; ++i) {
+          V x = value(lds, t, e, i);
+          if (masked) {  // a NaN goes to the rows that see it alone, see CodeSums
+            bool any = false;
+#pragma unroll
+            for (int y = 0; y < 8; ++y) any = any || x[y] != x[y];
+            if (__builtin_amdgcn_ballot_w64(any)) {
+              const V at = nan_places(x);
+              f32x16 count = {};
+              mma(count, at, sees);
+#pragma unroll
+              for (int y = 0; y < 16; ++y)
+                if (count[y] > 0.f) sums.acc[i][y] = __builtin_nanf("");
+            }
+          }
+#pragma unroll
+          for (int part = 0; part < PARTS; ++part) mma(sums.acc[i], x, p[part]);
+        }
+      }
+  }
+};
+
+// Places in the order of falling lengths (up to 62 sequences: the long ones start first), 128 rows
+// each; false: none.
+__device__ __forceinline__ bool cache_prompt_rows(const CacheAttnArgs& a, int64_t place, int G,
+                                                  CacheRows& p, int64_t& past) {
+  const int B = a.sq.B;
+  auto first = [G](int64_t start, int s) { return start * G / 128 + s; };
+  if (B <= 62) {
+    const int l = lane_id();
+    const int i = l < 1 ? 0 : (l - 1 < B ? l - 1 : B), j = l < B ? l : B;
+    const bool own = l >= 1 && l <= B;
+    const int64_t o0 = a.sq.offsets[i], o1 = a.sq.offsets[j];
+    const int64_t nn = own ? (a.sq.lengths ? a.sq.lengths[l - 1] : a.sq.T) : 0;
+    const int64_t kept = own ? a.c.lengths[l - 1] : 0;
+    const int T = (int)a.sq.T;
+    auto inside = [](int64_t v, int most) { return v < 0 ? 0 : (v > most ? most : (int)v); };
+    const int start = l < 1 ? 0 : (l > B + 1 ? T : inside(o0, T));
+    const int next = l > B ? T : inside(o1, T);
+    const int room = l < B + 2 && next > start ? next - start : 0;
+    const int used = inside(nn, room), length = a.c.length(kept);
+    const int c = (int)(((int64_t)room * G + 127) / 128);
+    int before = 0;  // places of longer sequences
+    for (int k = 0; k < B + 2; ++k) {
+      const int n = __builtin_amdgcn_readlane(length, k), ck = __builtin_amdgcn_readlane(c, k);
+      before += n > length || (n == length && k < l) ? ck : 0;
+    }
+    const uint64_t m = __builtin_amdgcn_ballot_w64(c > 0 && before <= place && place < before + c);
+    if (!m) return false;
+    const int s = __builtin_ctzll(m);
+    p.first = __builtin_amdgcn_readlane(start, s);
+    p.room = __builtin_amdgcn_readlane(room, s);
+    p.used = __builtin_amdgcn_readlane(used, s);
+    p.length = __builtin_amdgcn_readlane(length, s);
+    p.b = s >= 1 && s <= B ? s - 1 : -1;
+    past = place - __builtin_amdgcn_readlane(before, s);
+    return true;
+  }
+  p = cache_rows(a.sq, a.c, place, first);
+  past = place - p.place;
+  return past * 128 < (int64_t)p.room * G;
+}
+
+template <typename T, int DP>
+__global__ __launch_bounds__(256, (DP * sizeof(T) <= 256 ? 2 : 1)) void cache_prompt_kernel(
+    CacheAttnArgs a, const T* __restrict__ q, T* __restrict__ out) {
+  typedef CodeLds<T, DP> L;
+  __shared__ L lds;
+  const int G = a.Hq / a.c.Hk, hk = blockIdx.x % a.c.Hk;
+  CacheRows p;
+  int64_t past;
+  if (!cache_prompt_rows(a, blockIdx.x / a.c.Hk, G, p, past)) return;
+  const int w = wave_id(), l = lane_id(), b0 = (int)past * 128, r0 = b0 + 32 * w;
+  const int r = r0 + (l & 31), block = w >> 1, u = w & 1;
+  const int all = p.room * G, used = p.b < 0 ? 0 : p.used * G, length = p.b < 0 ? 0 : p.length;
+  auto keys = [&](int row) {
+    return used ? cache_keys(row < used ? row : used - 1, G, p.used, length, a.causal) : 0;
+  };
+  const int n = keys(r), least = keys(r0), most = r0 < used ? keys(r0 + 31) : 0;
+  const int end = b0 < used ? keys(b0 + 127) : 0, tiles = (end + 63) / 64;
+  // 64 blocks' pages at a time: of the tiles that are loaded, and of those that are multiplied
+  TilePages ahead, now;
+  if (tiles > 0) ahead.load(a.c, p.b, hk, 0, 1, 2 * tiles);
+  CodeRows<T, DP, true> x;
+  x.load(q + (p.first + r / G) * a.q_row + (hk * G + r % G) * a.q_head, r < used, a.D,
+         a.scale < 0.f);
+  const float c = attn_count(a.scale);
+  CodePrompt<T, DP> rows;
+  rows.sums.clear();
+  CodeLoads<T, DP> raw;
+  auto load = [&](int t) {
+    const int i = 2 * t + block;
+    const int page = __builtin_amdgcn_readlane(ahead.page, i & 63);
+    const int64_t at = page < 0 ? 0 : a.c.block(page, hk, i % (a.c.page / CACHE_BLOCK));
+    raw.load(a.c, uniform(at), page >= 0, u);
+  };
+  auto put = [&](int t) { raw.put(lds.b + (t & 1) * L::TILE, block, u, length - 64 * t - 32 * block); };
+  if (tiles > 0) {
+    load(0);
+    put(0);
+    if (tiles > 1) load(1);
+  }
+  for (int t = 0; t < tiles; ++t) {
+    __syncthreads();  // tile t is there; the other half of LDS is free
+    if ((t & 31) == 0) now = ahead;
+    if (t + 1 < tiles) {
+      put(t + 1);
+      if (t + 2 < tiles) {
+        if (((t + 2) & 31) == 0) ahead.load(a.c, p.b, hk, 2 * (t + 2), 1, 2 * tiles);
+        load(t + 2);
+      }
+    }
+    if (64 * t < most) {
+      float f[2], lv[2];
+#pragma unroll
+      for (int y = 0; y < 2; ++y) {
+        const int i = (2 * t + y) & 63;
+        f[y] = c * __builtin_bit_cast(
+                       float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, now.ks), i));
+        lv[y] = __builtin_bit_cast(
+            float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, now.lv), i));
+      }
+      rows.add(lds.b + (t & 1) * L::TILE, x, 64 * t, n, 64 * t + 64 > least, f, lv);
+    }
+  }
+  __syncthreads();
+  if (r0 >= all) return;
+  const float total = rows.sums.l + other_half(rows.sums.l);
+  const float inv = r < used && total != 0.f ? 1.f / total : 0.f;
+  AttnArgs at;
+  at.Hq = a.Hq;
+  at.Hk = a.c.Hk;
+  at.D = a.D;
+  AttnSpan span;
+  span.q0 = p.first;
+  put_rows<T, DP>(lds.b, rows.sums.acc, inv, out, at, span, hk, r0, all);
+}
+
+// Which kernel a call takes, and how many workgroups share the keys of 32 rows.
+struct CacheWay {
+  bool prompt;
+  int shares;
+};
+CacheWay cache_way(int64_t B, int64_t T, int64_t room, int64_t Hq, int64_t Hk) {
   const int64_t G = Hq / Hk, n = B < 1 ? 1 : B;
   const int64_t each = T < 1 ? 1 : (T * G + n - 1) / n;
+  if (each > 32 && (each + 127) / 128 * n * Hk >= 144) return CacheWay{true, 1};
   const int64_t blocks = (each + 31) / 32 * n * Hk;
   int64_t s = (128 + blocks - 1) / blocks, t = 1024 / blocks;
   if (s > room / 256) s = room / 256;
   if (t > room / 1024) t = room / 1024;
   if (s < t) s = t;
   if (room < 1024 || s < 1) s = 1;
-  return s > 64 ? 64 : (int)s;
+  return CacheWay{false, s > 64 ? 64 : (int)s};
 }
 
 int cache_attn_check(const char* op, int dtype, int64_t B, int64_t T, int64_t Hq, int64_t Hk,
@@ -407,9 +719,17 @@ extern "C" int64_t tpo_cache_attention_workspace_size(int dtype, int64_t B, int6
   const int64_t Dr = round_up(D, 16);
   if (cache_attn_check("cache_attention_workspace_size", dtype, B, T, Hq, Hk, D, 0, page, Dr, M))
     return -1;
-  const int64_t s = cache_shares(B, T, M * page, Hq, Hk);
+  const int64_t s = cache_way(B, T, M * page, Hq, Hk).shares;
   if (s == 1) return 0;
   return round_up(T * Hq * s * D * 4, 256) + round_up(T * Hq * s * 8, 256);
+}
+
+extern "C" int tpo_cache_attention_rows(int dtype, int64_t B, int64_t T, int64_t Hq, int64_t Hk,
+                                        int64_t D, int64_t page, int64_t M) {
+  if (int rc = cache_attn_check("cache_attention_rows", dtype, B, T, Hq, Hk, D, 0, page,
+                                round_up(D, 16), M))
+    return rc;
+  return cache_way(B, T, M * page, Hq, Hk).prompt ? 128 : 32;
 }
 
 extern "C" int tpo_cache_attention(int dtype, const void* q, const int64_t* offsets,
@@ -445,9 +765,11 @@ extern "C" int tpo_cache_attention(int dtype, const void* q, const int64_t* offs
   a.D = (int)D;
   a.causal = causal ? 1 : 0;
   a.scale = (float)scale;
-  const int64_t G = Hq / Hk, places = attn_places(T, G, B, 32);
-  if (places >= AT_GRID) return set_error(TPO_ERR_ARG, "%s: too many rows", op);
-  const int shares = cache_shares(B, T, M * page, Hq, Hk);
+  const CacheWay way = cache_way(B, T, M * page, Hq, Hk);
+  const int shares = way.shares;
+  const int64_t G = Hq / Hk, places = attn_places(T, G, B, way.prompt ? 128 : 32);
+  if ((way.prompt ? places * Hk : places) >= AT_GRID)
+    return set_error(TPO_ERR_ARG, "%s: too many rows", op);
   hipStream_t s = (hipStream_t)stream;
   float* part = (float*)workspace;
   float2* ml = (float2*)((char*)workspace + round_up(T * Hq * shares * D * 4, 256));
@@ -455,9 +777,13 @@ extern "C" int tpo_cache_attention(int dtype, const void* q, const int64_t* offs
     typedef decltype(t) E;
     with_head(D, [&](auto dp) {
       constexpr int DP = decltype(dp)::value;
-      cache_step_kernel<E, DP>
-          <<<dim3((unsigned)places, (unsigned)Hk, shares), 64 * CODE_WAVES, 0, s>>>(
-              a, (const E*)q, (E*)out, part, ml);
+      if (way.prompt)
+        cache_prompt_kernel<E, DP>
+            <<<dim3((unsigned)(places * Hk)), 256, 0, s>>>(a, (const E*)q, (E*)out);
+      else
+        cache_step_kernel<E, DP>
+            <<<dim3((unsigned)places, (unsigned)Hk, shares), 64 * CODE_WAVES, 0, s>>>(
+                a, (const E*)q, (E*)out, part, ml);
     });
     if (shares > 1)
       attn_join_kernel<E><<<dim3((unsigned)(T * Hq)), 256, 0, s>>>(
