@@ -93,29 +93,37 @@ struct CodeRows {
 template <int DP>
 struct CodeTile {
   u32x4 k[DP / 32], v[DP / 32];
-  __device__ __forceinline__ void load(const Cache& c, int64_t at, bool there) {
+  // at: see BlockPlaces; STREAM: past the caches
+  template <bool STREAM = false>
+  __device__ __forceinline__ void load(const Cache& c, int64_t at) {
+    constexpr int HOW = STREAM ? 2 : 0;
     const int l = lane_id(), r = l & 31, h = l >> 5;
-    const int bytes = there ? 512 * c.chunks : 0;
-    const auto kr = buffer(c.keys + at, bytes), vr = buffer(c.values + at, bytes);
+    const int bytes = at < 0 ? 0 : 512 * c.chunks;
+    const auto kr = buffer(c.keys + (at < 0 ? 0 : at), bytes);
+    const auto vr = buffer(c.values + (at < 0 ? 0 : at), bytes);
     const int key = 16 * (r >> 2 & 1) + 4 * (r >> 3) + (r & 3);
 #pragma unroll
     for (int i = 0; i < DP / 32; ++i)
-      k[i] = __builtin_amdgcn_raw_buffer_load_b128(kr, (2 * i + h) * 512 + key * 16, 0, 0);
+      k[i] = __builtin_amdgcn_raw_buffer_load_b128(kr, (2 * i + h) * 512 + key * 16, 0, HOW);
 #pragma unroll
     for (int i = 0; i < DP / 32; ++i)
-      v[i] = __builtin_amdgcn_raw_buffer_load_b128(vr, 1024 * i + 32 * r + 16 * h, 0, 0);
+      v[i] = __builtin_amdgcn_raw_buffer_load_b128(vr, 1024 * i + 32 * r + 16 * h, 0, HOW);
   }
 };
 
-// The pages of a wave's next 64 tiles, a lane each.
-struct TilePages {
-  int page;      // -1: none
+// Where a wave's next 64 blocks are, a lane each: what follows from a block's number is worked
+// out once for all of them.
+struct BlockPlaces {
+  int lo, hi;    // bytes from the first block; hi < 0: the page is not there
   float ks, lv;  // the key's scale, log2 of the value's
-  // tiles first, first + step, .. below end of sequence b
+  // blocks first, first + step, .. below end of sequence b
   __device__ __forceinline__ void load(const Cache& c, int b, int hk, int first, int step,
                                        int end) {
-    const int t = first + lane_id() * step;
-    page = t < end ? c.page_of(b, t * CACHE_BLOCK / c.page) : -1;
+    const int t = first + lane_id() * step, per = c.page / CACHE_BLOCK;
+    const int page = t < end ? c.page_of(b, t / per) : -1;
+    const int64_t at = page < 0 ? -1 : c.block(page, hk, t % per);
+    lo = (int)(uint32_t)at;
+    hi = (int)(at >> 32);
     float vs = 0.f;
     ks = 1.f;
     if (page >= 0) {
@@ -126,6 +134,17 @@ struct TilePages {
     // (what a page that is not there holds weighs nothing; scales are positive numbers)
     lv = page < 0 ? NEG_INF : __builtin_amdgcn_logf(fminf(fmaxf(vs, 0x1p-100f), 0x1p100f));
   }
+  // of block i, the same in all lanes
+  __device__ __forceinline__ int64_t place(int i) const {
+    const uint32_t l = (uint32_t)__builtin_amdgcn_readlane(lo, i & 63);
+    return (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane(hi, i & 63) << 32 | l);
+  }
+  static __device__ __forceinline__ float lane(float v, int i) {
+    return __builtin_bit_cast(
+        float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), i & 63));
+  }
+  __device__ __forceinline__ float key_scale(int i) const { return lane(ks, i); }
+  __device__ __forceinline__ float value_log(int i) const { return lane(lv, i); }
 };
 
 // A wave's rows under way.
@@ -156,12 +175,13 @@ struct CodeSums {
 #pragma unroll
         for (int p = 0; p < PARTS; ++p) mma(s, x, q.x[p][2 * i + e]);
       }
-    const int first = j0 + 16 * (lane_id() >> 5);
-    if (masked) {
+    if (__builtin_expect(masked, 0)) {
+      const int first = j0 + 16 * (lane_id() >> 5);
 #pragma unroll
       for (int e = 0; e < 16; ++e)
         if (first + e >= n) s[e] = NEG_INF;
       mask_values(t, first, n, length);
+      asm volatile("");  // (a branch: for every tile the masks' 70 instructions were a third)
     }
     float top = s[0];
 #pragma unroll
@@ -313,7 +333,7 @@ struct WaveSums {
 // used at the end only, where the waves' sums come together, two and two.
 // part, ml: see attn_join_kernel; m is in the exponent of 2, the values' scales with it.
 constexpr int CODE_WAVES = 4;
-template <typename T, int DP>
+template <typename T, int DP, bool STREAM>
 __global__ __launch_bounds__(64 * CODE_WAVES, (DP * sizeof(T) <= 256 ? 2 : 1)) void
 cache_step_kernel(CacheAttnArgs a, const T* __restrict__ q, T* __restrict__ out,
                   float* __restrict__ part, float2* __restrict__ ml) {
@@ -338,23 +358,17 @@ cache_step_kernel(CacheAttnArgs a, const T* __restrict__ q, T* __restrict__ out,
   rows.clear();
   const float c = attn_count(a.scale);
   CodeRows<T, DP> x;
-  TilePages pages;
+  BlockPlaces pages;
   if (t0 < t1) pages.load(a.c, p.b, hk, t0, W, t1);
   x.load(q + (p.first + r / G) * a.q_row + (hk * G + r % G) * a.q_head, r < used, a.D,
          a.scale < 0.f);
   auto load = [&](CodeTile<DP>& tile, int i) {  // the wave's tile i of those that `pages` has
-    const int t = t0 + i * W, page = __builtin_amdgcn_readlane(pages.page, i & 63);
-    const int64_t at =
-        page < 0 ? 0 : a.c.block(page, hk, t % (a.c.page / CACHE_BLOCK));
-    tile.load(a.c, uniform(at), page >= 0);
+    tile.template load<STREAM>(a.c, pages.place(i));
   };
   auto add = [&](CodeTile<DP>& tile, int i) {
     const int j0 = (t0 + i * W) * CACHE_BLOCK;
-    const float ks = __builtin_bit_cast(
-        float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, pages.ks), i & 63));
-    const float lv = __builtin_bit_cast(
-        float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, pages.lv), i & 63));
-    rows.add(tile, x, j0, n, j0 + 32 > least, length, c * ks, lv);
+    rows.add(tile, x, j0, n, j0 + 32 > least, length, c * pages.key_scale(i),
+             pages.value_log(i));
   };
   const int mine = t0 < t1 ? (t1 - t0 + W - 1) / W : 0;  // the wave's tiles
   CodeTile<DP> one, two;
@@ -428,59 +442,67 @@ struct CodeLoads {
   typedef CodeLds<T, DP> L;
   static constexpr int ALL = DP / 32, N = (ALL + 1) / 2;
   u32x4 k[N], v[N];
+  int u, block;      // of the tile's blocks, every other KB from KB u on
+  int kat[N][2];     // where a lane's two chunks of a key go, and of its value
+  int vat[2], half;  // (half: which sixteen tokens of the value's)
 
-  __device__ __forceinline__ void load(const Cache& c, int64_t at, bool there, int u) {
-    const int bytes = there ? 512 * c.chunks : 0;
-    const auto kr = buffer(c.keys + at, bytes), vr = buffer(c.values + at, bytes);
+  __device__ __forceinline__ explicit CodeLoads(int w) : u(w & 1), block(w >> 1) {
+    const int l = lane_id(), token = l & 31;
+    const int row = 32 * block + 8 * (token >> 2 & 3) + 4 * (token >> 4) + (token & 3);
+    const int swap = HeadLds<E, DP>::swap(row), d = 32 * u + (l & 31), turn = d >> 1 & 7;
+    half = l >> 5;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+#pragma unroll
+      for (int j = 0; j < N; ++j)
+        kat[j][e] = row * L::PITCH + (((2 * (2 * (2 * j + u) + (l >> 5)) + e) ^ swap) << 4);
+      vat[e] = L::KEYS_AT + d * 128 + (((4 * block + 2 * half + e) ^ turn) << 4);
+    }
+  }
+  __device__ __forceinline__ void load(const Cache& c, int64_t at) {
+    const int bytes = at < 0 ? 0 : 512 * c.chunks;
+    const auto kr = buffer(c.keys + (at < 0 ? 0 : at), bytes);
+    const auto vr = buffer(c.values + (at < 0 ? 0 : at), bytes);
 #pragma unroll
     for (int j = 0; j < N; ++j)
       if (2 * j + u < ALL) {
         k[j] = __builtin_amdgcn_raw_buffer_load_b128(kr, lane_id() * 16, (2 * j + u) * 1024, 0);
-        v[j] = __builtin_amdgcn_raw_buffer_load_b128(vr, lane_id() * 16, (2 * j + u) * 1024, 0);
+        v[j] = __builtin_amdgcn_raw_buffer_load_b128(
+            vr, 32 * (lane_id() & 31) + 16 * (lane_id() >> 5), (2 * j + u) * 1024, 0);
       }
   }
-  // To the tile at lds, of which it is block `block`; `left` places of that are the sequence's.
-  __device__ __forceinline__ void put(char* lds, int block, int u, int left) {
+  // To the tile at lds; `left` places from its first are the sequence's.  masked: not all of
+  // the workgroup's rows see all of the tile: values that are NaN become 0, and the result says
+  // that there were some.
+  __device__ __forceinline__ bool put(char* lds, int left, bool masked) {
     typedef typename Chunk<E>::V V;
-    const int l = lane_id();
+    bool bad = false;
+    if (__builtin_expect(masked, 0)) {
+      uint32_t any = 0;
 #pragma unroll
-    for (int j = 0; j < N; ++j) {
-      const int i = 2 * j + u;
-      if (i >= ALL) continue;
-      const int token = l & 31, c = 2 * i + (l >> 5);  // chunk c of a key
-      const int row = 32 * block + 8 * (token >> 2 & 3) + 4 * (token >> 4) + (token & 3);
-      const int swap = HeadLds<E, DP>::swap(row);
-      char* to = lds + row * L::PITCH;
-      *(V*)(to + ((2 * c ^ swap) << 4)) = from_codes<E>(k[j][0], k[j][1]);
-      *(V*)(to + (((2 * c + 1) ^ swap) << 4)) = from_codes<E>(k[j][2], k[j][3]);
-      const int d = 32 * i + (l >> 1), half = l & 1;  // sixteen tokens of a value
-      if (left < 32) {
+      for (int j = 0; j < N; ++j)
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
-          const int n = left - 16 * half - 4 * w;
-          v[j][w] &= n >= 4 ? ~0u : (n <= 0 ? 0u : (1u << 8 * n) - 1);
+          const int n = left - 32 * block - 16 * half - 4 * w;
+          const uint32_t x = v[j][w] & (n >= 4 ? ~0u : (n <= 0 ? 0u : (1u << 8 * n) - 1));
+          const uint32_t nans = nan_codes(x);
+          v[j][w] = x & ~((nans >> 7) * 255u);
+          any |= 2 * j + u < ALL ? nans : 0;
         }
-      }
-      const int at = 4 * block + 2 * half, turn = d >> 1 & 7;
-      to = lds + L::KEYS_AT + d * 128;
-      *(V*)(to + ((at ^ turn) << 4)) = from_codes<E>(v[j][0], v[j][1]);
-      *(V*)(to + (((at + 1) ^ turn) << 4)) = from_codes<E>(v[j][2], v[j][3]);
+      bad = __builtin_amdgcn_ballot_w64(any != 0) != 0;
+      asm volatile("");  // (a branch: worked out for every tile it took as long as the codes)
     }
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      if (2 * j + u >= ALL) continue;
+      *(V*)(lds + kat[j][0]) = from_codes<E>(k[j][0], k[j][1]);
+      *(V*)(lds + kat[j][1]) = from_codes<E>(k[j][2], k[j][3]);
+      *(V*)(lds + vat[0] + j * 64 * 128) = from_codes<E>(v[j][0], v[j][1]);
+      *(V*)(lds + vat[1] + j * 64 * 128) = from_codes<E>(v[j][2], v[j][3]);
+    }
+    return bad;
   }
 };
-
-// Values of a chunk that are NaN taken out; their places as ones.
-template <typename V>
-__device__ __forceinline__ V nan_places(V& x) {
-  V at = {};
-#pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const bool bad = x[e] != x[e];
-    at[e] = bad ? 1.f : 0.f;
-    if (bad) x[e] = 0.f;
-  }
-  return at;
-}
 
 // The tiles' work of a wave.
 template <typename T, int DP>
@@ -491,34 +513,42 @@ struct CodePrompt {
   static constexpr int PARTS = CodeType<T>::PARTS;
   CodeSums<T, DP> sums;
   HeadLanes<E, DP> lanes;
+  int at[4];  // of values l % 32, tokens 8 y + 16 (l / 32) - 8 (y % 2) ..: chunk y of a lane's four
 
-  // values 32 i + l % 32, tokens 32 t + 16 (l / 32) + 8 e .. + 7 of the tile
-  __device__ __forceinline__ V value(const char* lds, int t, int e, int i) const {
+  __device__ __forceinline__ CodePrompt() {
     const int l = lane_id(), r = l & 31;
-    return *(const V*)(lds + L::KEYS_AT + (32 * i + r) * 128 +
-                       (((4 * t + 2 * (l >> 5) + e) ^ (r >> 1 & 7)) << 4));
-  }
-  // The keys j0 .. j0 + 63 at lds, of which the lane's row sees those below n.  f, lv: of the
-  // two blocks, see CodeSums.
-  __device__ __forceinline__ void add(const char* lds, const CodeRows<T, DP, true>& q, int j0,
-                                      int n, bool masked, const float (&f)[2],
-                                      const float (&lv)[2]) {
-    f32x16 s[2] = {};
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
+    for (int y = 0; y < 4; ++y)
+      at[y] = L::KEYS_AT + r * 128 + (((4 * (y / 2) + 2 * (l >> 5) + y % 2) ^ (r >> 1 & 7)) << 4);
+  }
+  // values 32 i + l % 32, tokens 32 t + 16 (l / 32) + 8 e .. + 7 of the tile, y = 2 t + e
+  __device__ __forceinline__ V value(const char* lds, int y, int i) const {
+    return *(const V*)(lds + at[y] + 32 * 128 * i);
+  }
+  // Weights of the keys j0 .. j0 + 63 at lds, of which the lane's row sees those below n.  f, lv:
+  // of the two blocks, see CodeSums.
+  __device__ __forceinline__ void weigh(f32x16 (&s)[2], const char* lds,
+                                        const CodeRows<T, DP, true>& q, int j0, int n, bool masked,
+                                        const float (&f)[2], const float (&lv)[2]) {
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      s[t] = f32x16{};
 #pragma unroll
       for (int c = 0; c < DP / 16; ++c) {
         const V x = lanes.by_row(lds + 32 * t * L::PITCH, c);
 #pragma unroll
         for (int p = 0; p < PARTS; ++p) mma(s[t], x, q.x[p][c]);
       }
-    const int first = j0 + 16 * (lane_id() >> 5);
-    if (masked)
+    }
+    if (__builtin_expect(masked, 0)) {
+      const int first = j0 + 16 * (lane_id() >> 5);
 #pragma unroll
       for (int t = 0; t < 2; ++t)
 #pragma unroll
         for (int e = 0; e < 16; ++e)
           if (first + 32 * t + e >= n) s[t][e] = NEG_INF;
+      asm volatile("");
+    }
     float top = NEG_INF;
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
@@ -530,36 +560,19 @@ struct CodePrompt {
     sums.follow(fmaxf(top, other_half(top)));
 #pragma unroll
     for (int t = 0; t < 2; ++t) sums.weigh(s[t], f[t], lv[t]);
+  }
+  __device__ __forceinline__ void gather(const f32x16 (&s)[2], const char* lds) {
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
+    for (int y = 0; y < 4; ++y) {
+      V p[PARTS];
+      sums.parts(s[y / 2], y % 2, p);
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        V p[PARTS];
-        sums.parts(s[t], e, p);
-        V sees;
-        if (masked)
+      for (int i = 0; i < DP / 32; ++i) {
+        const V x = value(lds, y, i);
 #pragma unroll
-          for (int y = 0; y < 8; ++y) sees[y] = (E)(first + 32 * t + 8 * e + y < n ? 1.f : 0.f);
-#pragma unroll
-        for (int i = 0; i < DP / 32; ++i) {
-          V x = value(lds, t, e, i);
-          if (masked) {  // a NaN goes to the rows that see it alone, see CodeSums
-            bool any = false;
-#pragma unroll
-            for (int y = 0; y < 8; ++y) any = any || x[y] != x[y];
-            if (__builtin_amdgcn_ballot_w64(any)) {
-              const V at = nan_places(x);
-              f32x16 count = {};
-              mma(count, at, sees);
-#pragma unroll
-              for (int y = 0; y < 16; ++y)
-                if (count[y] > 0.f) sums.acc[i][y] = __builtin_nanf("");
-            }
-          }
-#pragma unroll
-          for (int part = 0; part < PARTS; ++part) mma(sums.acc[i], x, p[part]);
-        }
+        for (int part = 0; part < PARTS; ++part) mma(sums.acc[i], x, p[part]);
       }
+    }
   }
 };
 
@@ -604,25 +617,44 @@ __device__ __forceinline__ bool cache_prompt_rows(const CacheAttnArgs& a, int64_
   return past * 128 < (int64_t)p.room * G;
 }
 
+// The codes of the next tile into a half of LDS, and this one's products from the other.
+template <typename T, int DP>
+__device__ __forceinline__ bool code_step(const char* __restrict__ cur, char* __restrict__ nxt,
+                                          CodeLoads<T, DP>& raw, bool more, int left,
+                                          bool next_masked, CodePrompt<T, DP>& rows,
+                                          const CodeRows<T, DP, true>& q, bool any, int j0, int n,
+                                          bool masked, const float (&f)[2],
+                                          const float (&lv)[2]) {
+  const bool bad = more && raw.put(nxt, left, next_masked);
+  if (any) {
+    f32x16 s[2];
+    rows.weigh(s, cur, q, j0, n, masked, f, lv);
+    rows.gather(s, cur);
+  }
+  return bad;
+}
+
 template <typename T, int DP>
 __global__ __launch_bounds__(256, (DP * sizeof(T) <= 256 ? 2 : 1)) void cache_prompt_kernel(
     CacheAttnArgs a, const T* __restrict__ q, T* __restrict__ out) {
   typedef CodeLds<T, DP> L;
   __shared__ L lds;
+  __shared__ int taken_out;  // whether a value that some rows do not see was NaN
+  if (threadIdx.x == 0) taken_out = 0;
   const int G = a.Hq / a.c.Hk, hk = blockIdx.x % a.c.Hk;
   CacheRows p;
   int64_t past;
   if (!cache_prompt_rows(a, blockIdx.x / a.c.Hk, G, p, past)) return;
   const int w = wave_id(), l = lane_id(), b0 = (int)past * 128, r0 = b0 + 32 * w;
-  const int r = r0 + (l & 31), block = w >> 1, u = w & 1;
+  const int r = r0 + (l & 31);
   const int all = p.room * G, used = p.b < 0 ? 0 : p.used * G, length = p.b < 0 ? 0 : p.length;
   auto keys = [&](int row) {
     return used ? cache_keys(row < used ? row : used - 1, G, p.used, length, a.causal) : 0;
   };
   const int n = keys(r), least = keys(r0), most = r0 < used ? keys(r0 + 31) : 0;
-  const int end = b0 < used ? keys(b0 + 127) : 0, tiles = (end + 63) / 64;
+  const int all_see = keys(b0), end = b0 < used ? keys(b0 + 127) : 0, tiles = (end + 63) / 64;
   // 64 blocks' pages at a time: of the tiles that are loaded, and of those that are multiplied
-  TilePages ahead, now;
+  BlockPlaces ahead, now;
   if (tiles > 0) ahead.load(a.c, p.b, hk, 0, 1, 2 * tiles);
   CodeRows<T, DP, true> x;
   x.load(q + (p.first + r / G) * a.q_row + (hk * G + r % G) * a.q_head, r < used, a.D,
@@ -630,44 +662,50 @@ __global__ __launch_bounds__(256, (DP * sizeof(T) <= 256 ? 2 : 1)) void cache_pr
   const float c = attn_count(a.scale);
   CodePrompt<T, DP> rows;
   rows.sums.clear();
-  CodeLoads<T, DP> raw;
-  auto load = [&](int t) {
-    const int i = 2 * t + block;
-    const int page = __builtin_amdgcn_readlane(ahead.page, i & 63);
-    const int64_t at = page < 0 ? 0 : a.c.block(page, hk, i % (a.c.page / CACHE_BLOCK));
-    raw.load(a.c, uniform(at), page >= 0, u);
-  };
-  auto put = [&](int t) { raw.put(lds.b + (t & 1) * L::TILE, block, u, length - 64 * t - 32 * block); };
+  CodeLoads<T, DP> raw(w);
+  auto load = [&](int t) { raw.load(a.c, ahead.place(2 * t + raw.block)); };
+  bool bad = false;
   if (tiles > 0) {
     load(0);
-    put(0);
+    bad = raw.put(lds.b, length, 64 > all_see);
     if (tiles > 1) load(1);
   }
-  for (int t = 0; t < tiles; ++t) {
+  auto step = [&](auto half, int t) {  // (the halves by name: LDS addresses are constants)
+    constexpr int H = decltype(half)::value;
     __syncthreads();  // tile t is there; the other half of LDS is free
     if ((t & 31) == 0) now = ahead;
-    if (t + 1 < tiles) {
-      put(t + 1);
-      if (t + 2 < tiles) {
-        if (((t + 2) & 31) == 0) ahead.load(a.c, p.b, hk, 2 * (t + 2), 1, 2 * tiles);
-        load(t + 2);
-      }
-    }
-    if (64 * t < most) {
-      float f[2], lv[2];
+    float f[2], lv[2];
 #pragma unroll
-      for (int y = 0; y < 2; ++y) {
-        const int i = (2 * t + y) & 63;
-        f[y] = c * __builtin_bit_cast(
-                       float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, now.ks), i));
-        lv[y] = __builtin_bit_cast(
-            float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, now.lv), i));
-      }
-      rows.add(lds.b + (t & 1) * L::TILE, x, 64 * t, n, 64 * t + 64 > least, f, lv);
+    for (int y = 0; y < 2; ++y) {
+      f[y] = c * now.key_scale(2 * t + y);
+      lv[y] = now.value_log(2 * t + y);
     }
+    bad |= code_step<T, DP>(lds.b + H * L::TILE, lds.b + (1 - H) * L::TILE, raw, t + 1 < tiles,
+                            length - 64 * (t + 1), 64 * t + 128 > all_see,
+                            rows, x, 64 * t < most, 64 * t, n, 64 * t + 64 > least, f, lv);
+    if (t + 2 < tiles) {
+      if (((t + 2) & 31) == 0) ahead.load(a.c, p.b, hk, 2 * (t + 2), 1, 2 * tiles);
+      load(t + 2);
+    }
+  };
+  for (int t = 0; t < tiles; t += 2) {
+    step(std::integral_constant<int, 0>(), t);
+    if (t + 1 < tiles) step(std::integral_constant<int, 1>(), t + 1);
   }
+  if (bad) taken_out = 1;
   __syncthreads();
   if (r0 >= all) return;
+  if (taken_out) {  // rare: the rows that see it get it, see CodeSums
+    const int first = all_see / CACHE_BLOCK, last = (end + 31) / CACHE_BLOCK;
+    for (int i = first; i < last; ++i) {
+      const int per = a.c.page / CACHE_BLOCK;
+      const int page = __builtin_amdgcn_readfirstlane(a.c.page_of(p.b, i / per));
+      if (page < 0) continue;
+      CodeTile<DP> tile;
+      tile.load(a.c, uniform(a.c.block(page, hk, i % per)));
+      rows.sums.mask_values(tile, 32 * i + 16 * (l >> 5), n, length);
+    }
+  }
   const float total = rows.sums.l + other_half(rows.sums.l);
   const float inv = r < used && total != 0.f ? 1.f / total : 0.f;
   AttnArgs at;
@@ -679,22 +717,36 @@ __global__ __launch_bounds__(256, (DP * sizeof(T) <= 256 ? 2 : 1)) void cache_pr
   put_rows<T, DP>(lds.b, rows.sums.acc, inv, out, at, span, hk, r0, all);
 }
 
-// Which kernel a call takes, and how many workgroups share the keys of 32 rows.
+// Which kernel a call takes, how many workgroups share the keys of 32 rows, and whether the
+// codes go past the caches.
+// Prompts by 128 rows convert a code once for all of them, which pays where heads are wide and
+// two workgroups are there for every CU (half types, D = 128, 8 sequences of up to 8192 tokens:
+// 1024 such workgroups 386 us, by 32 rows 425; 512: 212, 236; 256: 55, 47; 256 of 16384 keys: 376,
+// 308).  Heads of 64 gain nothing by it (246, 248), float, whose products take three times as
+// long, loses (205, 181).
+// Shares: for 128 workgroups in all where that leaves a share 256 keys; for long caches up to
+// 1024 workgroups, so that sequences of different lengths even out (64 x 16384 tokens, 4 heads:
+// one share each 185 us, 2 160, 4 141).
+// Past the caches: where a row tile is all that reads them in a call, and the next call finds
+// nothing left of a pool that is more than the 256 MB behind the L2s (the same case 141 us, past
+// them 129; 3 x 1500 tokens read by seven row tiles each 17.4, past them 19.1).
 struct CacheWay {
-  bool prompt;
+  bool prompt, stream;
   int shares;
 };
-CacheWay cache_way(int64_t B, int64_t T, int64_t room, int64_t Hq, int64_t Hk) {
+CacheWay cache_way(int dtype, int64_t B, int64_t T, int64_t room, int64_t Hq, int64_t Hk,
+                   int64_t D, int64_t bytes) {
   const int64_t G = Hq / Hk, n = B < 1 ? 1 : B;
   const int64_t each = T < 1 ? 1 : (T * G + n - 1) / n;
-  if (each > 32 && (each + 127) / 128 * n * Hk >= 144) return CacheWay{true, 1};
+  if (dtype != TPO_F32 && D > 64 && each > 32 && (each + 127) / 128 * n * Hk >= 512)
+    return CacheWay{true, false, 1};
   const int64_t blocks = (each + 31) / 32 * n * Hk;
   int64_t s = (128 + blocks - 1) / blocks, t = 1024 / blocks;
   if (s > room / 256) s = room / 256;
   if (t > room / 1024) t = room / 1024;
   if (s < t) s = t;
   if (room < 1024 || s < 1) s = 1;
-  return CacheWay{false, s > 64 ? 64 : (int)s};
+  return CacheWay{false, each <= 32 && bytes > (int64_t)256 << 20, s > 64 ? 64 : (int)s};
 }
 
 int cache_attn_check(const char* op, int dtype, int64_t B, int64_t T, int64_t Hq, int64_t Hk,
@@ -719,7 +771,7 @@ extern "C" int64_t tpo_cache_attention_workspace_size(int dtype, int64_t B, int6
   const int64_t Dr = round_up(D, 16);
   if (cache_attn_check("cache_attention_workspace_size", dtype, B, T, Hq, Hk, D, 0, page, Dr, M))
     return -1;
-  const int64_t s = cache_way(B, T, M * page, Hq, Hk).shares;
+  const int64_t s = cache_way(dtype, B, T, M * page, Hq, Hk, D, 0).shares;
   if (s == 1) return 0;
   return round_up(T * Hq * s * D * 4, 256) + round_up(T * Hq * s * 8, 256);
 }
@@ -729,7 +781,7 @@ extern "C" int tpo_cache_attention_rows(int dtype, int64_t B, int64_t T, int64_t
   if (int rc = cache_attn_check("cache_attention_rows", dtype, B, T, Hq, Hk, D, 0, page,
                                 round_up(D, 16), M))
     return rc;
-  return cache_way(B, T, M * page, Hq, Hk).prompt ? 128 : 32;
+  return cache_way(dtype, B, T, M * page, Hq, Hk, D, 0).prompt ? 128 : 32;
 }
 
 extern "C" int tpo_cache_attention(int dtype, const void* q, const int64_t* offsets,
@@ -765,7 +817,7 @@ extern "C" int tpo_cache_attention(int dtype, const void* q, const int64_t* offs
   a.D = (int)D;
   a.causal = causal ? 1 : 0;
   a.scale = (float)scale;
-  const CacheWay way = cache_way(B, T, M * page, Hq, Hk);
+  const CacheWay way = cache_way(dtype, B, T, M * page, Hq, Hk, D, 2 * pages * Hk * page * Dr);
   const int shares = way.shares;
   const int64_t G = Hq / Hk, places = attn_places(T, G, B, way.prompt ? 128 : 32);
   if ((way.prompt ? places * Hk : places) >= AT_GRID)
@@ -777,13 +829,21 @@ extern "C" int tpo_cache_attention(int dtype, const void* q, const int64_t* offs
     typedef decltype(t) E;
     with_head(D, [&](auto dp) {
       constexpr int DP = decltype(dp)::value;
-      if (way.prompt)
-        cache_prompt_kernel<E, DP>
-            <<<dim3((unsigned)(places * Hk)), 256, 0, s>>>(a, (const E*)q, (E*)out);
-      else
-        cache_step_kernel<E, DP>
+      if constexpr (sizeof(E) == 2 && DP > 64)
+        if (way.prompt) {
+          cache_prompt_kernel<E, DP>
+              <<<dim3((unsigned)(places * Hk)), 256, 0, s>>>(a, (const E*)q, (E*)out);
+          return;
+        }
+      auto step = [&](auto stream) {
+        cache_step_kernel<E, DP, decltype(stream)::value>
             <<<dim3((unsigned)places, (unsigned)Hk, shares), 64 * CODE_WAVES, 0, s>>>(
                 a, (const E*)q, (E*)out, part, ml);
+      };
+      if (way.stream)
+        step(std::true_type());
+      else
+        step(std::false_type());
     });
     if (shares > 1)
       attn_join_kernel<E><<<dim3((unsigned)(T * Hq)), 256, 0, s>>>(
