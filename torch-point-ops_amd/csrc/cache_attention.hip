@@ -328,17 +328,16 @@ struct WaveSums {
 };
 
 // A workgroup takes 32 rows (tokens times the heads of a group, as the packed attention's) and
-// one of gridDim.z shares of their keys, its four waves in turn a tile of 32 keys each.  A tile
-// goes from memory to registers, the next one is on its way while one is multiplied; LDS is
+// one of gridDim.z shares of their keys, its W waves in turn a tile of 32 keys each.  A tile
+// goes from memory to registers, the next ones are on their way while one is multiplied; LDS is
 // used at the end only, where the waves' sums come together, two and two.
 // part, ml: see attn_join_kernel; m is in the exponent of 2, the values' scales with it.
-constexpr int CODE_WAVES = 4;
-template <typename T, int DP, bool STREAM>
-__global__ __launch_bounds__(64 * CODE_WAVES, (DP * sizeof(T) <= 256 ? 2 : 1)) void
+template <typename T, int DP, int W, bool STREAM>
+__global__ __launch_bounds__(64 * W, (DP * sizeof(T) <= 256 ? 2 : 1)) void
 cache_step_kernel(CacheAttnArgs a, const T* __restrict__ q, T* __restrict__ out,
                   float* __restrict__ part, float2* __restrict__ ml) {
-  constexpr int W = CODE_WAVES;
-  __shared__ WaveSums<T, DP> lds[2];
+  constexpr int N = 2;  // tiles in registers (three: no faster)
+  __shared__ WaveSums<T, DP> lds[W / 2];
   const int G = a.Hq / a.c.Hk, hk = blockIdx.y, shares = gridDim.z;
   const CacheRows p = cache_rows(a.sq, a.c, blockIdx.x, [G](int64_t start, int s) {
     return start * G / 32 + s;
@@ -358,41 +357,40 @@ cache_step_kernel(CacheAttnArgs a, const T* __restrict__ q, T* __restrict__ out,
   rows.clear();
   const float c = attn_count(a.scale);
   CodeRows<T, DP> x;
-  BlockPlaces pages;
-  if (t0 < t1) pages.load(a.c, p.b, hk, t0, W, t1);
+  const int mine = t0 < t1 ? (t1 - t0 + W - 1) / W : 0;  // the wave's tiles
+  // the places of 64 of them at a time: of those that are loaded, and of those multiplied
+  BlockPlaces ahead, now;
+  if (mine > 0) ahead.load(a.c, p.b, hk, t0, W, t1);
   x.load(q + (p.first + r / G) * a.q_row + (hk * G + r % G) * a.q_head, r < used, a.D,
          a.scale < 0.f);
-  auto load = [&](CodeTile<DP>& tile, int i) {  // the wave's tile i of those that `pages` has
-    tile.template load<STREAM>(a.c, pages.place(i));
+  CodeTile<DP> tile[N];
+  auto load = [&](CodeTile<DP>& to, int i) {
+    if (i >= mine) return;
+    if (i > 0 && (i & 63) == 0) ahead.load(a.c, p.b, hk, t0 + i * W, W, t1);
+    to.template load<STREAM>(a.c, ahead.place(i));
   };
-  auto add = [&](CodeTile<DP>& tile, int i) {
-    const int j0 = (t0 + i * W) * CACHE_BLOCK;
-    rows.add(tile, x, j0, n, j0 + 32 > least, length, c * pages.key_scale(i),
-             pages.value_log(i));
-  };
-  const int mine = t0 < t1 ? (t1 - t0 + W - 1) / W : 0;  // the wave's tiles
-  CodeTile<DP> one, two;
-  for (int i = 0; i < mine; i += 2) {
-    if ((i & 63) == 0) {
-      if (i > 0) pages.load(a.c, p.b, hk, t0 + i * W, W, t1);
-      load(one, i);
-    }
-    if (i + 1 < mine) load(two, i + 1);
-    add(one, i);
-    if (i + 1 < mine) {
-      if (i + 2 < mine && ((i + 2) & 63) != 0) load(one, i + 2);
-      add(two, i + 1);
+#pragma unroll
+  for (int y = 0; y < N - 1; ++y) load(tile[y], y);
+  for (int i = 0; i < mine; i += N) {
+#pragma unroll
+    for (int y = 0; y < N; ++y) {
+      const int at = i + y, j0 = (t0 + at * W) * CACHE_BLOCK;
+      if (at >= mine) break;
+      if ((at & 63) == 0) now = ahead;
+      load(tile[(y + N - 1) % N], at + N - 1);
+      rows.add(tile[y], x, j0, n, j0 + 32 > least, length, c * now.key_scale(at),
+               now.value_log(at));
     }
   }
 
-  if (w >= 2) lds[w - 2].put(rows);
-  __syncthreads();
-  if (w < 2) lds[w].add_to(rows);
-  __syncthreads();
-  if (w == 1) lds[0].put(rows);
-  __syncthreads();
+#pragma unroll
+  for (int half = W / 2; half > 0; half /= 2) {
+    if (w >= half && w < 2 * half) lds[w - half].put(rows);
+    __syncthreads();
+    if (w < half) lds[w].add_to(rows);
+    if (half > 1) __syncthreads();
+  }
   if (w != 0 || r >= all) return;
-  lds[0].add_to(rows);
   float total = rows.l + other_half(rows.l);
   if (r >= used) total = 0.f;
   const int64_t at = (p.first + r / G) * a.Hq + hk * G + r % G;
@@ -730,23 +728,29 @@ __global__ __launch_bounds__(256, (DP * sizeof(T) <= 256 ? 2 : 1)) void cache_pr
 // Past the caches: where a row tile is all that reads them in a call, and the next call finds
 // nothing left of a pool that is more than the 256 MB behind the L2s (the same case 141 us, past
 // them 129; 3 x 1500 tokens read by seven row tiles each 17.4, past them 19.1).
+// Waves: eight where a CU gets no more than one workgroup and each of four would have five tiles
+// or more (3 x 1500 tokens, 8 heads of 96, 200 new, float16: 15.6 us, by four waves 16.4; 7 x 2500,
+// 6 heads of 40, 5 new, float: 12.3, 13.2; 1 x 300, 8 heads of 64: 8.0, 7.5).
 struct CacheWay {
   bool prompt, stream;
-  int shares;
+  int shares, waves;
 };
 CacheWay cache_way(int dtype, int64_t B, int64_t T, int64_t room, int64_t Hq, int64_t Hk,
                    int64_t D, int64_t bytes) {
   const int64_t G = Hq / Hk, n = B < 1 ? 1 : B;
   const int64_t each = T < 1 ? 1 : (T * G + n - 1) / n;
   if (dtype != TPO_F32 && D > 64 && each > 32 && (each + 127) / 128 * n * Hk >= 512)
-    return CacheWay{true, false, 1};
+    return CacheWay{true, false, 1, 4};
   const int64_t blocks = (each + 31) / 32 * n * Hk;
   int64_t s = (128 + blocks - 1) / blocks, t = 1024 / blocks;
   if (s > room / 256) s = room / 256;
   if (t > room / 1024) t = room / 1024;
   if (s < t) s = t;
   if (room < 1024 || s < 1) s = 1;
-  return CacheWay{false, each <= 32 && bytes > (int64_t)256 << 20, s > 64 ? 64 : (int)s};
+  if (s > 64) s = 64;
+  const bool eight =
+      D * element_bytes(dtype) <= 256 && blocks * s <= 256 && room >= 20 * CACHE_BLOCK * s;
+  return CacheWay{false, each <= 32 && bytes > (int64_t)256 << 20, (int)s, eight ? 8 : 4};
 }
 
 int cache_attn_check(const char* op, int dtype, int64_t B, int64_t T, int64_t Hq, int64_t Hk,
@@ -835,15 +839,20 @@ extern "C" int tpo_cache_attention(int dtype, const void* q, const int64_t* offs
               <<<dim3((unsigned)(places * Hk)), 256, 0, s>>>(a, (const E*)q, (E*)out);
           return;
         }
-      auto step = [&](auto stream) {
-        cache_step_kernel<E, DP, decltype(stream)::value>
-            <<<dim3((unsigned)places, (unsigned)Hk, shares), 64 * CODE_WAVES, 0, s>>>(
+      auto step = [&](auto waves, auto stream) {
+        constexpr int W = decltype(waves)::value;
+        cache_step_kernel<E, DP, W, decltype(stream)::value>
+            <<<dim3((unsigned)places, (unsigned)Hk, shares), 64 * W, 0, s>>>(
                 a, (const E*)q, (E*)out, part, ml);
       };
-      if (way.stream)
-        step(std::true_type());
-      else
-        step(std::false_type());
+      const std::integral_constant<int, 4> four;
+      if constexpr (DP * sizeof(E) <= 256)
+        if (way.waves == 8) {
+          const std::integral_constant<int, 8> eight;
+          way.stream ? step(eight, std::true_type()) : step(eight, std::false_type());
+          return;
+        }
+      way.stream ? step(four, std::true_type()) : step(four, std::false_type());
     });
     if (shares > 1)
       attn_join_kernel<E><<<dim3((unsigned)(T * Hq)), 256, 0, s>>>(
