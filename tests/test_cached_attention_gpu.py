@@ -308,6 +308,23 @@ def test_prompts_nan(tpo, dev, dtype):
             assert torch.equal(got, clean)
 
 
+@pytest.mark.parametrize("dtype", HALVES)
+def test_prompts_nan_before_the_border(tpo, dev, dtype):
+    """A NaN that all rows see, in a tile that not all of them see the end of (the first row sees
+    places 0 .. 100), in either of its blocks."""
+    for place in (64, 70, 95, 96, 100):
+        cache = cache64.paged(tpo, dev, [140] * 16, 32, 80, 64, seed=24)
+        q = _q(640, 32, 80, dtype, 24).to(dev)
+        o = torch.tensor(_offsets(MANY), device=dev)
+        clean = tpo.cached_attention(q, cache, o)
+        p, s = int(cache.table[4, place // 64]), place % 64
+        cache.values.view(torch.uint8)[p, 3, s // 32, 5, s % 32] = 0x7f
+        got = tpo.cached_attention(q, cache, o)
+        bad = torch.zeros(got.shape, dtype=torch.bool, device=dev)
+        bad[160:200, 3, 5] = True
+        assert torch.equal(got.isnan(), bad) and torch.equal(got[~bad], clean[~bad])
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_large_pool(tpo, dev, dtype):
     """A pool of more than 256 MB, whose codes go past the caches."""

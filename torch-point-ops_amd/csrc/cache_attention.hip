@@ -694,7 +694,7 @@ __global__ __launch_bounds__(256, (DP * sizeof(T) <= 256 ? 2 : 1)) void cache_pr
   __syncthreads();
   if (r0 >= all) return;
   if (taken_out) {  // rare: the rows that see it get it, see CodeSums
-    const int first = all_see / CACHE_BLOCK, last = (end + 31) / CACHE_BLOCK;
+    const int first = all_see / 64 * 2, last = (end + 31) / CACHE_BLOCK;
     for (int i = first; i < last; ++i) {
       const int per = a.c.page / CACHE_BLOCK;
       const int page = __builtin_amdgcn_readfirstlane(a.c.page_of(p.b, i / per));
@@ -758,7 +758,8 @@ int cache_attn_check(const char* op, int dtype, int64_t B, int64_t T, int64_t Hq
   if (dtype != TPO_F32 && dtype != TPO_F16 && dtype != TPO_BF16)
     return set_error(TPO_ERR_DTYPE, "%s: unsupported dtype %d", op, dtype);
   if (int rc = cache_check(op, pages, Hk, page, Dr, B, M, D)) return rc;
-  if (T < 0 || Hq < 1 || Hq > 1024 || Hq % Hk != 0 || T * Hq >= ((int64_t)1 << 31))
+  if (T < 0 || T >= ((int64_t)1 << 31) || Hq < 1 || Hq > 1024 || Hq % Hk != 0 ||
+      T * Hq >= ((int64_t)1 << 31))
     return set_error(TPO_ERR_ARG,
                      "%s: bad sizes T=%lld Hq=%lld Hk=%lld (Hq a multiple of Hk, at most 1024)", op,
                      (long long)T, (long long)Hq, (long long)Hk);
