@@ -484,7 +484,7 @@ int tpo_rotary(int dtype, const void* x, int64_t tokens, int64_t heads, int64_t 
  *   [0, pages) is a page that is not there: nothing is written to it, and its
  *   places are not seen.  lengths (B) int64: the tokens of each sequence, those
  *   that a call brings included, clamped to M page.
- *   page is 32 to 256 in steps of 32, 1 <= D <= 128, M page < 2^31.
+ *   page is 32 to 256 in steps of 32, 1 <= D <= 128, M page <= 2^30.
  * The rows of a call (T) belong to the sequences as those of the packed
  * attention do: offsets (B + 1) int64, lengths_new or lengths_q (B) int64 or
  * NULL.  The n rows of a sequence that are in use are its last n tokens.

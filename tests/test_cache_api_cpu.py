@@ -218,7 +218,7 @@ def test_append_entry(lib):
     for bad in ({"_6": -1}, {"_7": -1}, {"_7": 1 << 31}, {"_8": 0}, {"_8": 2000}, {"_9": 0},
                 {"_9": 48}, {"_9": 129}, {"_20": 17}, {"_20": -1}, {"_29": -1}, {"_30": 0},
                 {"_30": 1025}, {"_31": 48}, {"_31": 0}, {"_31": 512}, {"_32": 48}, {"_33": -1},
-                {"_33": 1 << 26}):
+                {"_33": 1 << 26}, {"_33": (1 << 24) + 1}):
         assert call(**bad) == -1, bad
         assert b"bad sizes" in lib.tpo_last_error(), bad
     assert call(_0=1) == -2 and call(_16=P(4096), _17=2) == -2

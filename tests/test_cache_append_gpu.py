@@ -281,3 +281,25 @@ def test_versions_and_derivatives(tpo, dev):
         tpo.cache_append(cache, k.requires_grad_(True), k, o)
     with torch.no_grad():
         tpo.cache_append(cache, k, k, o)
+
+
+def test_scales_from_elsewhere(tpo, dev):
+    """Older codes of a page whose scale is above the largest: what does not fit is the largest
+    value, as of new tokens; in both kernels."""
+    for new in (1, 30):
+        cache = tpo.PagedCache.empty(1, 64, 1, 16, device=dev)
+        cache.lengths.fill_(20)
+        k = torch.ones(20, 1, 16, device=dev)
+        k[3], k[4], k[5, 0, 2] = -2.0, 0.0, float("nan")
+        tpo.cache_append(cache, k, k, torch.tensor([0, 20], device=dev))
+        old = cache.rows()[0][0, 0, :20].clone() / cache.key_scales[0, 0]
+        cache.key_scales.fill_(2.0 ** 44)
+        cache.value_scales.fill_(2.0 ** 44)
+        cache.lengths += new
+        z = torch.zeros(new, 1, 16, device=dev)
+        tpo.cache_append(cache, z, z, torch.tensor([0, new], device=dev))
+        assert (cache.key_scales == 2.0 ** 40).all() and (cache.value_scales == 2.0 ** 40).all()
+        want = (old * 16).clamp(-448, 448) * 2.0 ** 40
+        for rows in cache.rows():
+            assert torch.equal(rows[0, 0, :20].nan_to_num(1.0), want.nan_to_num(1.0))
+            assert rows[0, 0, 5, 2].isnan() and (rows[0, 0, 20:20 + new] == 0).all()

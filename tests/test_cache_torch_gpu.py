@@ -74,6 +74,31 @@ def test_compiled(tpo, dev, dtype):
         assert torch.equal(got, tpo.cached_attention(q, c, o) + 1)
 
 
+def test_compiled_step(tpo, dev):
+    """A step of generation as one graph: the cache is changed in place there too."""
+    one, _ = _cache(tpo, dev)
+    two, _ = _cache(tpo, dev)
+    o = torch.tensor([0, 1, 2], device=dev)
+    f = 4.0 ** -torch.arange(16, dtype=torch.float64, device=dev)
+
+    def step(cache, q, k, v):
+        cache.lengths += 1
+        q = tpo.cache_append(cache, k * 2, v, o, q + 1, f)
+        return tpo.cached_attention(q, cache, o) * 2
+
+    fn = torch.compile(step)
+    g = torch.Generator().manual_seed(4)
+    with torch.no_grad():
+        for _ in range(3):
+            q, k, v = (torch.randn(2, h, 32, generator=g).to(dev) for h in (4, 2, 2))
+            want, got = step(one, q, k, v), fn(two, q, k, v)
+            assert torch.equal(got, want)
+    for name in ("keys", "values"):
+        assert torch.equal(getattr(one, name).view(torch.uint8), getattr(two, name).view(torch.uint8))
+    for name in ("key_scales", "value_scales", "lengths"):
+        assert torch.equal(getattr(one, name), getattr(two, name))
+
+
 def test_vmap(tpo, dev):
     x, at, f = _rotary(dev, torch.float32)
     x = x.detach()

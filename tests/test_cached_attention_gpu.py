@@ -326,6 +326,21 @@ def test_prompts_nan_before_the_border(tpo, dev, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+def test_scale_of_nothing(tpo, dev, dtype):
+    """A scale of 0 over pages of the smallest scale, or of none: the mean of what a row sees."""
+    for smallest in (2.0 ** -40, 0.0):
+        for lengths, heads in ([70, 33], 2), ([140] * 16, 32):
+            n = 5 if heads == 2 else 40
+            cache = cache64.paged(tpo, dev, lengths, heads, 80, 64, seed=6)
+            q = _q(n * len(lengths), heads, 80, dtype, 6).to(dev)
+            o = torch.tensor(_offsets([n] * len(lengths)), device=dev)
+            want = tpo.cached_attention(q, cache, o, scale=0.0)
+            assert want.isfinite().all()
+            cache.key_scales.fill_(smallest)
+            assert torch.equal(tpo.cached_attention(q, cache, o, scale=0.0), want)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_large_pool(tpo, dev, dtype):
     """A pool of more than 256 MB, whose codes go past the caches."""
     small = cache64.paged(tpo, dev, [300, 70], 2, 64, 64, seed=23)

@@ -52,7 +52,7 @@ struct CacheRows {
 // The last sequence whose first place is at or before `place`; first(start, s): the first place
 // of sequence s (0 and B + 1 being the rows before and behind), not decreasing.  Up to 126
 // sequences: each lane has one or two of them, and one trip to memory brings all that is needed
-// (in four trips, a workgroup's beginning took 2 us of the 12 of 64 sequences' new tokens).
+// (64 sequences' new tokens: 11.0 us, by four trips 11.4).
 template <typename F>
 __device__ __forceinline__ CacheRows cache_rows(const Sequences& sq, const Cache& c, int64_t place,
                                                 const F& first) {

@@ -62,11 +62,12 @@ __device__ __forceinline__ uint32_t codes4(const float* v, float f, bool rare) {
     return codes4(for_code(v[0], f), for_code(v[1], f), for_code(v[2], f), for_code(v[3], f));
   return codes4(v[0] * f, v[1] * f, v[2] * f, v[3] * f);
 }
-// Four codes brought to another scale.
+// Four codes brought to another scale; f > 1 only where the old scale was above the largest.
 __device__ __forceinline__ uint32_t codes_times(uint32_t x, float f) {
   const auto a = __builtin_amdgcn_cvt_pk_f32_fp8((int)x, false);
   const auto b = __builtin_amdgcn_cvt_pk_f32_fp8((int)x, true);
-  return codes4(a[0] * f, a[1] * f, b[0] * f, b[1] * f);
+  const float v[4] = {a[0], a[1], b[0], b[1]};
+  return codes4(v, f, f > 1.f);
 }
 
 // The call's rows: strides in elements.
@@ -188,7 +189,8 @@ __device__ __forceinline__ void store_part(uint8_t* block, int token, int d, int
   } else {
 #pragma unroll
     for (int e = 0; e < 8; ++e)
-      if (e < n) to[(d + e) / 16 * 512 + (d + e) % 16] = (uint8_t)((e < 4 ? lo : hi) >> 8 * (e % 4));
+      if (e < n)
+        to[(d + e) / 16 * 512 + (d + e) % 16] = (uint8_t)((e < 4 ? lo : hi) >> 8 * (e % 4));
   }
 }
 
@@ -202,8 +204,8 @@ __device__ __forceinline__ void append_queries(const Cache& c, const Sequences& 
   float2* cs = (float2*)lds;
   int* at = (int*)(cs + block * angles.pitch);
   int* live = at + block;
-  TurnRows<T, THREADS, STREAM> rows(r.q, r.q_row, r.q_head, r.q_out, r.Hq, r.D, t0, n,
-                                           turn.pairs, turn.interleaved);
+  TurnRows<T, THREADS, STREAM> rows(r.q, r.q_row, r.q_head, r.q_out, r.Hq, r.D, t0, n, turn.pairs,
+                                    turn.interleaved);
   rows.load();
   for (int t = wave_id(); t < n; t += THREADS / 64) {
     const CacheRows s =
@@ -227,9 +229,10 @@ __device__ __forceinline__ void append_queries(const Cache& c, const Sequences& 
   rows.run(cs, live);
 }
 
-// The same in a launch of its own, 8 waves a SIMD, for more queries than the caches hold: their way
-// to and from memory is all that counts (20 thousand tokens, 16 heads of 128 in bfloat16: 33 us,
-// 5.2 TB/s; behind the pages' workgroups in one launch, 16 waves a CU, both take 83, apart 47 + 33).
+// The same in a launch of its own, 8 waves a SIMD, for more queries than the caches hold: their
+// way to and from memory is all that counts (21 thousand tokens, 16 heads of 128 in bfloat16: 33
+// us, 5.3 TB/s; behind the pages' workgroups in one launch, 16 waves a CU, both take 83, apart
+// 47 + 33).
 template <typename T>
 __global__ __launch_bounds__(256) void cache_queries_kernel(Cache c, Sequences sq, Turn turn,
                                                             AppendRows<T> r, int block) {
@@ -238,9 +241,9 @@ __global__ __launch_bounds__(256) void cache_queries_kernel(Cache c, Sequences s
 }
 
 // The page's older codes (slots below a) at a new scale, sixteen bytes at a time (a wave's lanes
-// with four of them under way): of keys sixteen values of a token, of values sixteen tokens.  A piece that
-// ends with new tokens gets its older bytes one by one, so that no byte is written twice and
-// the new ones need not wait.
+// with four of them under way): of keys sixteen values of a token, of values sixteen tokens.  A
+// piece that ends with new tokens gets its older bytes one by one, so that no byte is written
+// twice and the new ones need not wait.
 template <int TEAM>
 __device__ __forceinline__ void scale_older(const Cache& c, uint8_t* codes, int64_t number, int h,
                                             bool key, int a, float f, int lane) {
@@ -365,7 +368,8 @@ __device__ __forceinline__ uint32_t top16(const float (&x)[16], bool& rare) {
 // lanes, then over the four of them.
 __device__ __forceinline__ uint32_t wave_top(uint32_t v) {
   auto with = [&](auto move) {
-    const uint32_t o = (uint32_t)__builtin_amdgcn_mov_dpp((int)v, decltype(move)::value, 15, 15, true);
+    const uint32_t o =
+        (uint32_t)__builtin_amdgcn_mov_dpp((int)v, decltype(move)::value, 15, 15, true);
     v = o > v ? o : v;
   };
   with(std::integral_constant<int, 0xb1>());   // the neighbour
@@ -430,7 +434,7 @@ __device__ __forceinline__ void store_tile(const Cache& c, const char* tile, int
 // and the next head's are on their way meanwhile.  Two meetings a head: for the largest values,
 // and where the values have been turned over.
 // Bound by latency: 16 waves a CU, whose 128 registers angles and values take; 8 x 4096 tokens,
-// 4 heads of 128 in bfloat16: PAGEFIG.
+// 4 heads of 128 in bfloat16: 47 us, 66 MB read and written (1.4 TB/s).
 // Workgroups from kv on turn `block` tokens' queries each.
 template <typename T, int THREADS>
 __global__ __launch_bounds__(THREADS, 4) void cache_page_kernel(Cache c, Sequences sq, Turn turn,
@@ -590,8 +594,9 @@ __global__ __launch_bounds__(THREADS, 2) void cache_append_kernel(Cache c, Seque
 #pragma unroll 1
       for (int i = threadIdx.x; i < n * turn.pairs; i += THREADS) {
         const int t = t0 + i / turn.pairs, j = i % turn.pairs;
+        const double at = r.places ? turn.place(g.row0 + t, j) : (double)(g.base + t);
         double sn, co;
-        sine_cosine((r.places ? turn.place(g.row0 + t, j) : (double)(g.base + t)) * turn.f[j], sn, co);
+        sine_cosine(at * turn.f[j], sn, co);
         lds[i] = make_double2(co * turn.m, sn * turn.m);
       }
       __syncthreads();
@@ -720,11 +725,11 @@ int cache_check(const char* op, int64_t pages, int64_t Hk, int64_t page, int64_t
   if (pages < 0 || pages >= ((int64_t)1 << 31) || Hk < 1 || Hk > 1024 || page < CACHE_BLOCK ||
       page > CACHE_PAGE || page % CACHE_BLOCK != 0 || D < 1 || D > CACHE_DMAX ||
       Dr != round_up(D, 16) || B < 0 || B > (1 << 24) || M < 0 ||
-      M * page >= ((int64_t)1 << 31) || M >= ((int64_t)1 << 31))
+      M * page > ((int64_t)1 << 30) || M > ((int64_t)1 << 30))
     return set_error(TPO_ERR_ARG,
                      "%s: bad sizes pages=%lld Hk=%lld page=%lld Dr=%lld B=%lld M=%lld D=%lld "
                      "(pages of 32 to %d tokens in steps of 32, D at most %d and Dr the next "
-                     "multiple of 16, M page below 2^31)",
+                     "multiple of 16, M page at most 2^30)",
                      op, (long long)pages, (long long)Hk, (long long)page, (long long)Dr,
                      (long long)B, (long long)M, (long long)D, CACHE_PAGE, CACHE_DMAX);
   return TPO_OK;

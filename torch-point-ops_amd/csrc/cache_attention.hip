@@ -116,6 +116,10 @@ struct CodeTile {
 struct BlockPlaces {
   int lo, hi;    // bytes from the first block; hi < 0: the page is not there
   float ks, lv;  // the key's scale, log2 of the value's
+  // (scales are positive numbers)
+  static __device__ __forceinline__ float inside(float v) {
+    return fminf(fmaxf(v, 0x1p-100f), 0x1p100f);
+  }
   // blocks first, first + step, .. below end of sequence b
   __device__ __forceinline__ void load(const Cache& c, int b, int hk, int first, int step,
                                        int end) {
@@ -128,11 +132,11 @@ struct BlockPlaces {
     ks = 1.f;
     if (page >= 0) {
       const int64_t at = (int64_t)page * c.Hk + hk;
-      ks = c.key_scales[at];
-      vs = c.value_scales[at];
+      ks = inside(c.key_scales[at]);
+      vs = inside(c.value_scales[at]);
     }
-    // (what a page that is not there holds weighs nothing; scales are positive numbers)
-    lv = page < 0 ? NEG_INF : __builtin_amdgcn_logf(fminf(fmaxf(vs, 0x1p-100f), 0x1p100f));
+    // (what a page that is not there holds weighs nothing)
+    lv = page < 0 ? NEG_INF : __builtin_amdgcn_logf(vs);
   }
   // of block i, the same in all lanes
   __device__ __forceinline__ int64_t place(int i) const {
@@ -143,7 +147,11 @@ struct BlockPlaces {
     return __builtin_bit_cast(
         float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), i & 63));
   }
-  __device__ __forceinline__ float key_scale(int i) const { return lane(ks, i); }
+  // What a score of block i counts in the exponent of 2, count being that of a score of its
+  // own; never 0, as a masked score is -inf.
+  __device__ __forceinline__ float score(int i, float count) const {
+    return fmaxf(count * lane(ks, i), 1e-37f);
+  }
   __device__ __forceinline__ float value_log(int i) const { return lane(lv, i); }
 };
 
@@ -378,7 +386,7 @@ cache_step_kernel(CacheAttnArgs a, const T* __restrict__ q, T* __restrict__ out,
       if (at >= mine) break;
       if ((at & 63) == 0) now = ahead;
       load(tile[(y + N - 1) % N], at + N - 1);
-      rows.add(tile[y], x, j0, n, j0 + 32 > least, length, c * now.key_scale(at),
+      rows.add(tile[y], x, j0, n, j0 + 32 > least, length, now.score(at, c),
                now.value_log(at));
     }
   }
@@ -421,10 +429,10 @@ cache_step_kernel(CacheAttnArgs a, const T* __restrict__ q, T* __restrict__ out,
 // tiles of 64, which its waves load (a quarter each, two tiles ahead), turn into the products'
 // type and put into LDS for all four: a code is converted once for 128 rows, where the kernel
 // above does it for 32 (8 sequences of up to 8192, 1024 new tokens, 16 heads on 4, D = 128 in
-// bfloat16: PROMPTFIG).  Keys lie in LDS in the order of the product's rows in which a lane
-// receives the scores of sixteen tokens in a row; values by value, 64 tokens each, so that
-// sixteen bytes are what a product sums over.  Chunks of 16 bytes change places with the row, as
-// in HeadLds, so that a read touches all banks.
+// bfloat16: 386 us, the kernel above 425).  Keys lie in LDS in the order of the product's rows in
+// which a lane receives the scores of sixteen tokens in a row; values by value, 64 tokens each, so
+// that sixteen bytes are what a product sums over.  Chunks of 16 bytes change places with the row,
+// as in HeadLds, so that a read touches all banks.
 template <typename T, int DP>
 struct alignas(1024) CodeLds {
   typedef typename CodeType<T>::E E;
@@ -675,7 +683,7 @@ __global__ __launch_bounds__(256, (DP * sizeof(T) <= 256 ? 2 : 1)) void cache_pr
     float f[2], lv[2];
 #pragma unroll
     for (int y = 0; y < 2; ++y) {
-      f[y] = c * now.key_scale(2 * t + y);
+      f[y] = now.score(2 * t + y, c);
       lv[y] = now.value_log(2 * t + y);
     }
     bad |= code_step<T, DP>(lds.b + H * L::TILE, lds.b + (1 - H) * L::TILE, raw, t + 1 < tiles,

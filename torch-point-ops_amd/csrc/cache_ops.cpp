@@ -137,7 +137,8 @@ PagedCache cache_of(const Tensor& like, const Tensor& keys, const Tensor& values
   c.Dr = keys.size(3) * 16;
   TORCH_CHECK(values.scalar_type() == at::kFloat8_e4m3fn &&
                   values.sizes() == at::IntArrayRef({c.pages, c.Hk, keys.size(2), c.Dr, 32}),
-              op, ": values must be float8_e4m3fn (pages, Hk, page / 32, Dr, 32) as keys are, but got ",
+              op,
+              ": values must be float8_e4m3fn (pages, Hk, page / 32, Dr, 32) as keys are, but got ",
               values.scalar_type(), " ", values.sizes());
   for (const Tensor& t : {key_scales, value_scales})
     TORCH_CHECK(t.scalar_type() == at::kFloat && t.sizes() == at::IntArrayRef({c.pages, c.Hk}), op,

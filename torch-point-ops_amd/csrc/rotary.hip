@@ -75,8 +75,9 @@ extern "C" int tpo_rotary(int dtype, const void* x, int64_t tokens, int64_t head
   if (int rc = all_there("rotary", {x, y})) return rc;
   if (pairs > 0)
     if (int rc = all_there("rotary", {places, frequencies})) return rc;
-  // tokens of a workgroup: about 16 KB of them (32768 x 20 x 128 bfloat16: 2 to 4 tokens 81 us,
-  // 8 tokens 87, 32 91: a workgroup's angles come before its first store), and 2048 workgroups
+  // tokens of a workgroup: about 16 KB of them (32768 x 20 x 128 bfloat16, through the caches: 2
+  // to 4 tokens 81 us, 8 tokens 87, 32 91: a workgroup's angles come before its first store), and
+  // 2048 workgroups
   const int64_t pitch = dtype == TPO_F32 ? TurnAngles<float>(t.pairs, t.interleaved).pitch
                                          : TurnAngles<half_t>(t.pairs, t.interleaved).pitch;
   int64_t block = 16384 / (heads * D * element_bytes(dtype));
