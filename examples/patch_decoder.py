@@ -1,17 +1,21 @@
 """An autoregressive decoder of point patches, trained and sampled with this package.
 
     python examples/patch_decoder.py [--steps 50] [--clouds 8] [--width 256] [--dtype bf16]
+        [--positions none|places|centres] [--paged]
 
 Clouds are cut into patches: furthest point samples as centres, in the order of a curve
 through space, and the nearest points of each.  A transformer reads the patches of a cloud
 in order and predicts the next one; the loss is the Chamfer distance to it.  Clouds have
 different numbers of patches, and their tokens lie packed, one cloud after the other: layer
 norm, packed attention and the gated projection see no padding.  Afterwards the model
-continues clouds one patch at a time over a cache of keys and values.
+continues clouds one patch at a time over a cache of keys and values, with --paged one of
+8 bits in pages.  With --positions queries and keys are turned by the patches' places in their
+clouds, or by their centres' coordinates.
 """
 from __future__ import annotations
 
 import argparse
+import math
 import os
 import sys
 
@@ -34,50 +38,88 @@ class Block(torch.nn.Module):
         self.out = torch.nn.Linear(width, width, bias=False, **kw)
         self.ff = tpo.GatedFeedForward(width, 2 * width, **kw)
 
-    def project(self, x):
-        """q, k and v as slices of one product."""
+    def project(self, x, rotary=None, positions=None):
+        """q, k and v as slices of one product, queries and keys turned by their positions."""
         y = self.qkv(self.norm1(x)).view(len(x), -1, self.size)
-        return y.split([self.heads, self.key_heads, self.key_heads], 1)
+        if rotary is None:
+            return y.split([self.heads, self.key_heads, self.key_heads], 1)
+        qk, v = y.split([self.heads + self.key_heads, self.key_heads], 1)
+        return *rotary(qk, positions).split([self.heads, self.key_heads], 1), v
 
     def finish(self, x, attended):
         x = x + self.out(attended.flatten(1))
         return x + self.ff(self.norm2(x))
 
-    def forward(self, x, offsets):
-        return self.finish(x, tpo.packed_attention(*self.project(x), offsets))
+    def forward(self, x, offsets, rotary=None, positions=None):
+        return self.finish(x, tpo.packed_attention(*self.project(x, rotary, positions), offsets))
 
-    def step(self, x, keys, values, one, rooms, used):
+    def step(self, x, keys, values, one, rooms, used, rotary=None, positions=None):
         """One new token of every sequence; keys and values (B, room, heads, size) get its own."""
-        q, k, v = self.project(x)
+        q, k, v = self.project(x, rotary, positions)
         b = torch.arange(len(x), device=x.device)
         keys[b, used], values[b, used] = k, v
         a = tpo.packed_attention(q, keys.flatten(0, 1), values.flatten(0, 1), one, rooms,
                                  lengths_k=used + 1)
         return self.finish(x, a)
 
+    def step_paged(self, x, cache, one, rotary=None, positions=None):
+        """One new token of every sequence; the cache, whose lengths count it already, gets its
+        key and value."""
+        q, k, v = self.project(x)
+        if rotary is None:
+            tpo.cache_append(cache, k, v, one)
+        else:
+            q = tpo.cache_append(cache, k, v, one, q, rotary.frequencies, positions)
+        return self.finish(x, tpo.cached_attention(q, cache, one))
+
 
 class PatchDecoder(torch.nn.Module):
-    """Tokens (T, 3 + 3 K): a patch's centre and its points about it -> the next patch."""
+    """Tokens (T, 3 + 3 K): a patch's centre and its points about it -> the next patch.
 
-    def __init__(self, points, width=256, heads=8, key_heads=2, depth=4, **kw):
+    positions: "none", or what queries and keys are turned by: "places" of tokens in their
+    sequences, or the coordinates of patches' "centres".
+    """
+
+    def __init__(self, points, width=256, heads=8, key_heads=2, depth=4, positions="none", **kw):
         super().__init__()
+        size, dev = width // heads, kw.get("device")
+        self.positions, self.rotary = positions, None
+        if positions == "places":
+            self.rotary = tpo.RotaryPositions(size // 2 * 2, device=dev)
+        elif positions == "centres":  # (half a turn and more over [-1, 1], finer by octaves)
+            octaves = 2.0 ** torch.arange(size // 6, dtype=torch.float64)
+            self.rotary = tpo.RotaryPositions(
+                size // 6 * 6, frequencies=(math.pi / 2 * octaves).repeat(3), device=dev)
         self.embed = torch.nn.Linear(3 + 3 * points, width, **kw)
         self.blocks = torch.nn.ModuleList(Block(width, heads, key_heads, **kw)
                                           for _ in range(depth))
         self.norm = tpo.LayerNorm(width, **kw)
         self.head = torch.nn.Linear(width, 3 + 3 * points, **kw)
 
+    def positions_of(self, tokens, offsets):
+        """What the tokens of packed sequences are turned by."""
+        if self.positions == "centres":
+            return tokens[:, :3].float().contiguous()
+        if self.positions == "places":
+            at = torch.arange(len(tokens), device=tokens.device)
+            return at - offsets[torch.searchsorted(offsets, at, right=True) - 1]
+        return None
+
     def forward(self, tokens, offsets):
         x = self.embed(tokens.to(self.embed.weight.dtype))
+        positions = self.positions_of(tokens, offsets)
         for block in self.blocks:
-            x = block(x, offsets)
+            x = block(x, offsets, self.rotary, positions)
         return self.head(self.norm(x)).float()
 
     @torch.no_grad()
-    def generate(self, prompt, patches):
-        """Continues each of the prompts (B, 3 + 3 K), one patch each, to `patches` patches."""
+    def generate(self, prompt, patches, paged=False):
+        """Continues each of the prompts (B, 3 + 3 K), one patch each, to `patches` patches.
+        paged: over caches of 8 bits in pages."""
         B, dev, dt = len(prompt), prompt.device, self.embed.weight.dtype
         block = self.blocks[0]
+        if paged:
+            return self.generate_paged(prompt, patches)
         cache = [torch.empty(2, B, patches, block.key_heads, block.size, device=dev, dtype=dt)
                  for _ in self.blocks]
         one = torch.arange(B + 1, device=dev)
@@ -85,10 +127,27 @@ class PatchDecoder(torch.nn.Module):
         tokens = [prompt]
         for _ in range(patches - 1):
             x = self.embed(tokens[-1].to(dt))
+            at = used if self.positions == "places" else self.positions_of(tokens[-1], one)
             for b, (keys, values) in zip(self.blocks, cache):
-                x = b.step(x, keys, values, one, rooms, used)
+                x = b.step(x, keys, values, one, rooms, used, self.rotary, at)
             tokens.append(self.head(self.norm(x)).float())
             used = used + 1
+        return torch.stack(tokens, 1)
+
+    @torch.no_grad()
+    def generate_paged(self, prompt, patches):
+        B, dev, dt = len(prompt), prompt.device, self.embed.weight.dtype
+        caches = [tpo.PagedCache.empty(B, patches, b.key_heads, b.size, page=32, device=dev)
+                  for b in self.blocks]
+        one, tokens = torch.arange(B + 1, device=dev), [prompt]
+        for _ in range(patches - 1):
+            x = self.embed(tokens[-1].to(dt))
+            # (places are the cache's to know)
+            at = self.positions_of(tokens[-1], one) if self.positions == "centres" else None
+            for b, cache in zip(self.blocks, caches):
+                cache.lengths += 1
+                x = b.step_paged(x, cache, one, self.rotary, at)
+            tokens.append(self.head(self.norm(x)).float())
         return torch.stack(tokens, 1)
 
 
@@ -134,11 +193,13 @@ def main(argv=None):
     ap.add_argument("--points", type=int, default=16, help="points of a patch")
     ap.add_argument("--width", type=int, default=256)
     ap.add_argument("--dtype", choices=["f32", "f16", "bf16"], default="bf16")
+    ap.add_argument("--positions", choices=["none", "places", "centres"], default="none")
+    ap.add_argument("--paged", action="store_true", help="generate over an 8-bit cache in pages")
     a = ap.parse_args(argv)
     dtype = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}[a.dtype]
     torch.manual_seed(0)
     g = torch.Generator().manual_seed(0)
-    model = PatchDecoder(a.points, a.width, device="cuda", dtype=dtype)
+    model = PatchDecoder(a.points, a.width, positions=a.positions, device="cuda", dtype=dtype)
     # the optimiser's weights are float: half types lose small updates
     masters = [p.detach().float().requires_grad_(True) for p in model.parameters()]
     optimiser = torch.optim.AdamW(masters, lr=1e-3)
@@ -159,7 +220,7 @@ def main(argv=None):
         if step % 10 == 0 or step == a.steps - 1:
             print(f"step {step}: loss {losses[-1]:.4f}", flush=True)
     tokens, offsets = patches_of(shapes(g, 4, 2048, "cuda"), [32] * 4, a.points)
-    made = model.generate(tokens[offsets[:-1]], 32)
+    made = model.generate(tokens[offsets[:-1]], 32, a.paged)
     print(f"generated {tuple(made.shape)}: four clouds of 32 patches of {a.points} points")
     return losses
 
