@@ -122,38 +122,29 @@ struct Part {
 
 template <typename T>
 struct PartValues {
-  Piece<T, 8> a, b;
+  Loaded<T, 8> a, b;
   __device__ __forceinline__ void load(const T* row, const Part& p) {
     a = some<T, 8>(row + p.pa, p.load_a);
     b = some<T, 8>(row + p.pb, p.load_b);
   }
-  // sixteen values side by side to the first and the second of each pair
-  __device__ __forceinline__ void apart() {
-    PartValues o = *this;
+  // the sixteen as floats
+  __device__ __forceinline__ void to(float (&x)[16]) const {
+    const Piece<T, 8> p = a.values(), q = b.values();
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      a.v[e] = e < 4 ? o.a.v[2 * e & 7] : o.b.v[2 * e & 7];
-      b.v[e] = e < 4 ? o.a.v[(2 * e + 1) & 7] : o.b.v[(2 * e + 1) & 7];
+      x[e] = (float)p.v[e];
+      x[8 + e] = (float)q.v[e];
     }
-  }
-  // what was worked out of these is not kept
-  __device__ __forceinline__ void fresh() {
-    constexpr int N = sizeof(T) * 2;
-    struct Words { uint32_t w[N]; };
-    Words p = __builtin_bit_cast(Words, a), q = __builtin_bit_cast(Words, b);
-#pragma unroll
-    for (int i = 0; i < N; ++i) asm volatile("" : "+v"(p.w[i]), "+v"(q.w[i]));
-    a = __builtin_bit_cast(Piece<T, 8>, p);
-    b = __builtin_bit_cast(Piece<T, 8>, q);
   }
 };
 
-// Eight pairs turned, x[e] and x[8 + e] being pair e.  ODD: rounded to odd; else to the nearest
+// Eight pairs turned, x[e] and x[8 + e] being pair e; angle(e): its cosine and sine.  ODD: rounded to odd; else to the nearest
 // float, which has the same code but where it lies half-way between two of them, its last 19
 // bits 0 (e4m3 keeps 3 of 23): true where one may.
-template <bool ODD, typename T>
-__device__ __forceinline__ bool turn_pairs(const PartValues<T>& u, const double2 (&cs)[8],
-                                           float (&x)[16]) {
+template <bool ODD, typename T, typename F>
+__device__ __forceinline__ bool turn_pairs(const PartValues<T>& u, bool interleaved,
+                                           const F& angle, float (&x)[16]) {
+  const Piece<T, 8> p = u.a.values(), q = u.b.values();
   uint32_t least = ~0u;
   auto rounded = [&](double d) {
     const float f = ODD ? to_odd(d) : (float)d;
@@ -163,21 +154,21 @@ __device__ __forceinline__ bool turn_pairs(const PartValues<T>& u, const double2
   };
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
-    const double v0 = (float)u.a.v[e], v1 = (float)u.b.v[e];
-    x[e] = rounded(__builtin_fma(-v1, cs[e].y, v0 * cs[e].x));
-    x[8 + e] = rounded(__builtin_fma(v0, cs[e].y, v1 * cs[e].x));
+    const int i = 2 * e & 7;
+    const T s0 = e < 4 ? p.v[i] : q.v[i], s1 = e < 4 ? p.v[i + 1] : q.v[i + 1];  // side by side
+    const double v0 = (float)(interleaved ? s0 : p.v[e]);
+    const double v1 = (float)(interleaved ? s1 : q.v[e]);
+    const double2 cs = angle(e);
+    x[e] = rounded(__builtin_fma(-v1, cs.y, v0 * cs.x));
+    x[8 + e] = rounded(__builtin_fma(v0, cs.y, v1 * cs.x));
     if (e % 2) __builtin_amdgcn_sched_barrier(0);
   }
   return least == 0;
 }
-template <typename T>
-__device__ __forceinline__ void turn_part(PartValues<T> u, bool interleaved,
-                                          const double2 (&cs)[8], float (&x)[16]) {
-  if (interleaved) u.apart();
-  if (turn_pairs<false>(u, cs, x)) {
-    u.fresh();
-    turn_pairs<true>(u, cs, x);
-  }
+template <typename T, typename F>
+__device__ __forceinline__ void turn_part(const PartValues<T>& u, bool interleaved, const F& angle,
+                                          float (&x)[16]) {
+  if (turn_pairs<false>(u, interleaved, angle, x)) turn_pairs<true>(u, interleaved, angle, x);
 }
 
 // Eight codes to a key's place in a block: values d .. d + n - 1 of a token.
@@ -447,6 +438,7 @@ __global__ __launch_bounds__(THREADS, 4) void cache_page_kernel(Cache c, Sequenc
     return;
   }
   constexpr int WAVES = THREADS / 64;
+  __shared__ double2 angles[8][THREADS];
   AppendPage g(c, sq, blockIdx.x / groups);
   if (g.none()) return;
   const int NC = c.chunks, Dr = 16 * NC, pitch = c.page + 4;
@@ -466,8 +458,12 @@ __global__ __launch_bounds__(THREADS, 4) void cache_page_kernel(Cache c, Sequenc
   if (has_k) uk.load(kr + h0 * r.k_head, pk);
   if (has_v) uv.load(vr + h0 * r.v_head, pv);
   if (!g.there()) return;
-  double2 cs[8];
-  if (has_k && pk.pair >= 0) part_angles(pk, turn, r, g, t, cs);
+  if (has_k && pk.pair >= 0) {
+    double2 cs[8];
+    part_angles(pk, turn, r, g, t, cs);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) angles[e][threadIdx.x] = cs[e];
+  }
 #pragma unroll 1
   for (int h = h0; h < h1; ++h) {
     pk.fresh();
@@ -481,21 +477,15 @@ __global__ __launch_bounds__(THREADS, 4) void cache_page_kernel(Cache c, Sequenc
     uint32_t top_k = 0, top_v = 0;
     if (has_v) {
       float y[16];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        y[e] = (float)uv.a.v[e];
-        y[8 + e] = (float)uv.b.v[e];
-      }
+      uv.to(y);
       top_v = top16(y, rare_v);
     }
     __builtin_amdgcn_sched_barrier(0);
     if (has_k) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        x[e] = (float)uk.a.v[e];
-        x[8 + e] = (float)uk.b.v[e];
-      }
-      if (pk.pair >= 0) turn_part<T>(uk, turn.interleaved, cs, x);
+      if (pk.pair < 0)
+        uk.to(x);
+      else
+        turn_part<T>(uk, turn.interleaved, [&](int e) { return angles[e][threadIdx.x]; }, x);
       top_k = top16(x, rare_k);
       if (h + 1 < h1) uk.load(kr + (h + 1) * r.k_head, pk);
     }
@@ -526,11 +516,7 @@ __global__ __launch_bounds__(THREADS, 4) void cache_page_kernel(Cache c, Sequenc
       store_part(to, t % 32, pk.pb, pk.store_b, w[2], w[3]);
     }
     if (has_v) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        x[e] = (float)uv.a.v[e];
-        x[8 + e] = (float)uv.b.v[e];
-      }
+      uv.to(x);
       codes16(x, fv, rare_v, false, w);
       if (h + 1 < h1) uv.load(vr + (h + 1) * r.v_head, pv);
       char* at = tile + part * 16 * pitch + t;
@@ -646,12 +632,10 @@ __global__ __launch_bounds__(THREADS, 2) void cache_append_kernel(Cache c, Seque
     float x[16], f = 0.f;
     bool rare = false;
     auto take = [&](int t0) {  // what was loaded as the cache takes it
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        x[e] = (float)u.a.v[e];
-        x[8 + e] = (float)u.b.v[e];
-      }
-      if (has && in(t0) && key && pk.pair >= 0) turn_part<T>(u, turn.interleaved, cs, x);
+      if (!(has && in(t0) && key && pk.pair >= 0))
+        u.to(x);
+      else
+        turn_part<T>(u, turn.interleaved, [&](int e) { return cs[e]; }, x);
     };
     auto measure = [&](int t0) {
       if (!has || !in(t0)) return;

@@ -74,16 +74,46 @@ struct TurnPieces {
   }
 };
 
-// n values from p (at any element) and back; `n` of them, PER at once where there are as many.
+// PER values as they come from memory.  They stay words until they are used: taken apart into
+// values of two bytes where both ways of loading meet, they would be waited for right there.
 template <typename T, int PER>
-__device__ __forceinline__ Piece<T, PER> some(const T* p, int n) {
-  Piece<T, PER> v = {};
-  if (n >= PER)
-    v = *(const Piece<T, PER>*)p;
-  else
+struct Loaded {
+  static constexpr int N = PER * sizeof(T) / 4;
+  uint32_t w[N];
+
+  __device__ __forceinline__ void fresh() {  // what was worked out of them is not kept
+#pragma unroll
+    for (int i = 0; i < N; ++i) asm volatile("" : "+v"(w[i]));
+  }
+  __device__ __forceinline__ Piece<T, PER> values() const {
+    Loaded o = *this;
+    o.fresh();
+    return __builtin_bit_cast(Piece<T, PER>, o);
+  }
+};
+// n values from p (at any element), PER at once where there are as many; and back.
+template <typename T, int PER>
+__device__ __forceinline__ Loaded<T, PER> some(const T* p, int n) {
+  typedef uint32_t words __attribute__((ext_vector_type(4)));
+  typedef words anywhere __attribute__((aligned(2)));  // (of every type)
+  Loaded<T, PER> v = {};
+  if (n >= PER) {
+#pragma unroll
+    for (int i = 0; i < v.N; i += 4) {
+      const words x = ((const anywhere*)p)[i / 4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v.w[i + j] = x[j];
+    }
+  } else {
 #pragma unroll
     for (int e = 0; e < PER; ++e)
-      if (e < n) v.v[e] = p[e];
+      if (e < n) {
+        if constexpr (sizeof(T) == 4)
+          v.w[e] = __builtin_bit_cast(uint32_t, p[e]);
+        else
+          v.w[e / 2] |= (uint32_t)__builtin_bit_cast(uint16_t, p[e]) << 16 * (e % 2);
+      }
+  }
   return v;
 }
 // STREAM: past the caches.
@@ -136,7 +166,7 @@ struct TurnRows {
   int H, D, tokens, pairs, interleaved;
   int t, h, dt, dh, a, left;  // the piece at hand; the step to the next
   bool turned, on;
-  P u, v;
+  Loaded<T, PER> u, v;
 
   __device__ __forceinline__ TurnRows(const T* x, int64_t x_row, int64_t x_head, T* y, int H,
                                       int D, int64_t t0, int tokens, int pairs, int interleaved)
@@ -174,7 +204,7 @@ struct TurnRows {
     const TurnAngles<T> angles(pairs, interleaved);
     const int piece = a / PER;
     while (on) {
-      P p = u, q = v;
+      P p = u.values(), q = v.values();
       const int tp = t, hp = h;
       next();
       load();
