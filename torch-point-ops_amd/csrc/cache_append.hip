@@ -222,8 +222,8 @@ __device__ __forceinline__ void append_queries(const Cache& c, const Sequences& 
 
 // The same in a launch of its own, 8 waves a SIMD, for more queries than the caches hold: their
 // way to and from memory is all that counts (21 thousand tokens, 16 heads of 128 in bfloat16: 33
-// us, 5.3 TB/s; behind the pages' workgroups in one launch, 16 waves a CU, both take 83, apart
-// 47 + 33).
+// us, 5.3 TB/s; behind the pages' workgroups in one launch, 16 waves a CU, both took 83 where the
+// pages alone took 47).
 template <typename T>
 __global__ __launch_bounds__(256) void cache_queries_kernel(Cache c, Sequences sq, Turn turn,
                                                             AppendRows<T> r, int block) {
@@ -424,8 +424,10 @@ __device__ __forceinline__ void store_tile(const Cache& c, const char* tile, int
 // heads, and one of its value; both stay in registers between the largest value and the codes,
 // and the next head's are on their way meanwhile.  Two meetings a head: for the largest values,
 // and where the values have been turned over.
-// Bound by latency: 16 waves a CU, whose 128 registers angles and values take; 8 x 4096 tokens,
-// 4 heads of 128 in bfloat16: 47 us, 66 MB read and written (1.4 TB/s).
+// The angles lie in LDS, each read only by the lane that wrote it (in registers, of which 16 waves
+// a CU have 128 each, 17 were spilled: 21 MB more written, 46 us where it then took 40).
+// Bound by latency and instructions in turn (half of the time a vector instruction is issued): 8 x
+// 4096 tokens, 4 heads of 128 in bfloat16: 33 us, 66 MB read and written (2.0 TB/s).
 // Workgroups from kv on turn `block` tokens' queries each.
 template <typename T, int THREADS>
 __global__ __launch_bounds__(THREADS, 4) void cache_page_kernel(Cache c, Sequences sq, Turn turn,
@@ -789,7 +791,12 @@ extern "C" int tpo_cache_append(int dtype, const void* k, const void* v, const v
   const Sequences sq{offsets, lengths_new, T, (int)B};
   // a place for each page that a sequence's new tokens may lie in, see the kernel
   const int64_t slots = T / page + 2 * (B + 2);
+  // few tokens a sequence: a wave a head, where pages are many (64 sequences, 8 heads of 128 in
+  // bfloat16, a new token each 9.3 us, by whole workgroups 18.4; 8 new 10.3, 17.6; 16 new 25.3,
+  // 18.1; 8 sequences: 9 and 8; 16 new 19.9, 8.5)
   const bool few = T <= 8 * B;
+  // else 512 workgroups (5 x 300 tokens, 6 heads of 80, float16: by 52 workgroups 32 us, 156 14,
+  // 312 10; 8 x 4096, 4 heads of 128: 343 33, 686 33, 1372 40)
   const int64_t about = T / page + B + 1;  // pages
   int64_t groups = few ? (Hk + 3) / 4 : (512 + about - 1) / about;
   if (groups > Hk) groups = Hk;
