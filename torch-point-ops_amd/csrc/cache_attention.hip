@@ -737,8 +737,9 @@ __global__ __launch_bounds__(256, (DP * sizeof(T) <= 256 ? 2 : 1)) void cache_pr
 // nothing left of a pool that is more than the 256 MB behind the L2s (the same case 141 us, past
 // them 129; 3 x 1500 tokens read by seven row tiles each 17.4, past them 19.1).
 // Waves: eight where a CU gets no more than one workgroup and each of four would have five tiles
-// or more (3 x 1500 tokens, 8 heads of 96, 200 new, float16: 15.6 us, by four waves 16.4; 7 x 2500,
-// 6 heads of 40, 5 new, float: 12.3, 13.2; 1 x 300, 8 heads of 64: 8.0, 7.5).
+// or more (3 x 1500 tokens, 8 heads of 96, 200 new, float16: 15.6 us, by four waves 16.4; 7
+// sequences, 6 heads of 40, 5 new, float, with the join: 4096 tokens 15.4, 15.8; 2048 12.4, 12.1;
+// 1 x 300, 8 heads of 64: 8.0, 7.5).
 struct CacheWay {
   bool prompt, stream;
   int shares, waves;
