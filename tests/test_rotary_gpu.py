@@ -141,3 +141,20 @@ def test_captured(tpo, dev):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(y, tpo.rotary_positions(X, A, F))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_queries_of_append_are_the_same(tpo, dev, dtype, interleaved):
+    """Bit for bit, in each of the kernels that turn them, however often a rounding is close."""
+    g = torch.Generator().manual_seed(5)
+    for B, new, H in ((200, 3, 8), (2, 700, 8), (1, 3000, 96)):  # (the last past the caches)
+        T = B * new
+        q, k = (torch.randn(T, h, 128, generator=g).to(dev, dtype) for h in (H, 1))
+        f = tpo.rotary_frequencies(64, device=dev)
+        cache = tpo.PagedCache.empty(B, new, 1, 128, device=dev)
+        cache.lengths += new
+        o = torch.arange(B + 1, device=dev) * new
+        got = tpo.cache_append(cache, k, k, o, q, f, interleaved=interleaved)
+        at = torch.arange(T, device=dev) % new
+        assert torch.equal(got, tpo.rotary_positions(q, at, f, interleaved))

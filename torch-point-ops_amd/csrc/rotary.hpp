@@ -149,6 +149,15 @@ struct TurnAngles {
   }
 };
 
+// A float in T, rounded as a float first: to half also in one instruction with the product, which
+// rounds once; the compiler takes it in one kernel and not in another, whose results would
+// differ.
+template <typename T>
+__device__ __forceinline__ T result(float v) {
+  if constexpr (sizeof(T) == 2) asm("" : "+v"(v));
+  return (T)v;
+}
+
 // The rows of H heads of `tokens` tokens from t0 on, x strided, y (T, H, D): turned by cs (cosine
 // and sine of a token's pairs, m times each, in LDS).  THREADS of a workgroup go round (head,
 // piece): pieces lie side by side in memory, then heads.  A thread's next piece is on its way
@@ -216,8 +225,8 @@ struct TurnRows {
             const float4 z = c[e / 4 * angles.pieces];
             const float2 w = e & 2 ? make_float2(z.z, z.w) : make_float2(z.x, z.y);
             const float x0 = (float)p.v[e], x1 = (float)p.v[e + 1];
-            p.v[e] = (T)__builtin_fmaf(-x1, w.y, x0 * w.x);
-            p.v[e + 1] = (T)__builtin_fmaf(x0, w.y, x1 * w.x);
+            p.v[e] = result<T>(__builtin_fmaf(-x1, w.y, x0 * w.x));
+            p.v[e + 1] = result<T>(__builtin_fmaf(x0, w.y, x1 * w.x));
           }
         } else {
 #pragma unroll
@@ -225,8 +234,8 @@ struct TurnRows {
             const float4 z = c[e / 2 * angles.pieces];
             const float2 w = e & 1 ? make_float2(z.z, z.w) : make_float2(z.x, z.y);
             const float x0 = (float)p.v[e], x1 = (float)q.v[e];
-            p.v[e] = (T)__builtin_fmaf(-x1, w.y, x0 * w.x);
-            q.v[e] = (T)__builtin_fmaf(x0, w.y, x1 * w.x);
+            p.v[e] = result<T>(__builtin_fmaf(-x1, w.y, x0 * w.x));
+            q.v[e] = result<T>(__builtin_fmaf(x0, w.y, x1 * w.x));
           }
         }
       }
