@@ -127,6 +127,10 @@ struct PartValues {
     a = some<T, 8>(row + p.pa, p.load_a);
     b = some<T, 8>(row + p.pb, p.load_b);
   }
+  __device__ __forceinline__ void fresh() {
+    a.fresh();
+    b.fresh();
+  }
   // the sixteen as floats
   __device__ __forceinline__ void to(float (&x)[16]) const {
     const Piece<T, 8> p = a.values(), q = b.values();
@@ -426,8 +430,9 @@ __device__ __forceinline__ void store_tile(const Cache& c, const char* tile, int
 // and where the values have been turned over.
 // The angles lie in LDS, each read only by the lane that wrote it (in registers, of which 16 waves
 // a CU have 128 each, 17 were spilled: 21 MB more written, 46 us where it then took 40).
-// Bound by latency and instructions in turn (half of the time a vector instruction is issued): 8 x
-// 4096 tokens, 4 heads of 128 in bfloat16: 33 us, 66 MB read and written (2.0 TB/s).
+// Bound by its steps' latencies in turn (copies without the angles, the turn, the keys' stores or
+// the values' each took 30 to 33 of then 33 us; a vector instruction is issued in half of the
+// time): 8 x 4096 tokens, 4 heads of 128 in bfloat16: 31.5 us, 66 MB read and written (2.1 TB/s).
 // Workgroups from kv on turn `block` tokens' queries each.
 template <typename T, int THREADS>
 __global__ __launch_bounds__(THREADS, 4) void cache_page_kernel(Cache c, Sequences sq, Turn turn,
@@ -472,14 +477,15 @@ __global__ __launch_bounds__(THREADS, 4) void cache_page_kernel(Cache c, Sequenc
     pv.fresh();
     const int64_t scale_at = (int64_t)g.number * c.Hk + h;
     const bool older = g.a > 0;
-    const float old_k = older ? c.key_scales[scale_at] : 0.f;
-    const float old_v = older ? c.value_scales[scale_at] : 0.f;
+    float old_k = older ? c.key_scales[scale_at] : 0.f;
+    float old_v = older ? c.value_scales[scale_at] : 0.f;
     float x[16];
     bool rare_k = false, rare_v = false;
     uint32_t top_k = 0, top_v = 0;
+    PartValues<T> v = uv;
     if (has_v) {
       float y[16];
-      uv.to(y);
+      v.to(y);
       top_v = top16(y, rare_v);
     }
     __builtin_amdgcn_sched_barrier(0);
@@ -489,7 +495,14 @@ __global__ __launch_bounds__(THREADS, 4) void cache_page_kernel(Cache c, Sequenc
       else
         turn_part<T>(uk, turn.interleaved, [&](int e) { return angles[e][threadIdx.x]; }, x);
       top_k = top16(x, rare_k);
-      if (h + 1 < h1) uk.load(kr + (h + 1) * r.k_head, pk);
+    }
+    // Everything that was loaded is waited for here, and nothing that the rest of this head does:
+    // a wait further down would be one for the next head's rows as well.
+    asm volatile("" : "+v"(old_k), "+v"(old_v));
+    v.fresh();
+    if (h + 1 < h1) {
+      if (has_k) uk.load(kr + (h + 1) * r.k_head, pk);
+      if (has_v) uv.load(vr + (h + 1) * r.v_head, pv);
     }
     __builtin_amdgcn_sched_barrier(0);
     top_k = wave_top(top_k);
@@ -518,9 +531,8 @@ __global__ __launch_bounds__(THREADS, 4) void cache_page_kernel(Cache c, Sequenc
       store_part(to, t % 32, pk.pb, pk.store_b, w[2], w[3]);
     }
     if (has_v) {
-      uv.to(x);
+      v.to(x);
       codes16(x, fv, rare_v, false, w);
-      if (h + 1 < h1) uv.load(vr + (h + 1) * r.v_head, pv);
       char* at = tile + part * 16 * pitch + t;
 #pragma unroll
       for (int e = 0; e < 16; ++e) at[e * pitch] = (char)(w[e / 4] >> 8 * (e % 4));
@@ -796,7 +808,7 @@ extern "C" int tpo_cache_append(int dtype, const void* k, const void* v, const v
   // 18.1; 8 sequences: 9 and 8; 16 new 19.9, 8.5)
   const bool few = T <= 8 * B;
   // else 512 workgroups (5 x 300 tokens, 6 heads of 80, float16: by 52 workgroups 32 us, 156 14,
-  // 312 10; 8 x 4096, 4 heads of 128: 343 33, 686 33, 1372 40)
+  // 312 10; 8 x 4096, 4 heads of 128: 343 32, 686 31.5, 1372 38)
   const int64_t about = T / page + B + 1;  // pages
   int64_t groups = few ? (Hk + 3) / 4 : (512 + about - 1) / about;
   if (groups > Hk) groups = Hk;
