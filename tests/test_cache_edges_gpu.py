@@ -1,0 +1,48 @@
+"""cache_append and cached_attention where numbers end: keys next to nothing, the largest."""
+import math
+
+import pytest
+import torch
+
+from tests import cache64
+
+pytestmark = pytest.mark.gpu
+
+
+def _same(cache, want):
+    """The GPU's cache holds exactly what the definition gives."""
+    got = cache64.Cache(cache)
+    assert torch.equal(got.ks, want.ks) and torch.equal(got.vs, want.vs)
+    assert torch.equal(got.k.nan_to_num(999), want.k.nan_to_num(999))
+    assert torch.equal(got.v.nan_to_num(999), want.v.nan_to_num(999))
+
+
+def _append(tpo, dev, k, f, at, interleaved, amplitude=1.0):
+    """k (T, H, D) as keys and values of one sequence, against the definition; few tokens and many
+    take kernels of their own."""
+    T, H, D = k.shape
+    cache = cache64.paged(tpo, dev, [T + 3], H, D, 32, seed=T)
+    want = cache64.Cache(cache)
+    want.append(k, k, [0, T], f=f, at=at, interleaved=interleaved, amplitude=amplitude)
+    tpo.cache_append(cache, k.to(dev), k.to(dev), torch.tensor([0, T], device=dev), None, f.to(dev),
+                     at.to(dev), interleaved, amplitude)
+    _same(cache, want)
+    return want
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("T", [4, 40])
+def test_turned_keys_next_to_nothing(tpo, dev, dtype, interleaved, T):
+    """Finite keys whose turned values are under the least float, of either sign: their codes are
+    0, alone in a page and beside larger ones."""
+    tiny = torch.tensor([1e-30, 1e-40, 1.4e-45, 6e-8, 0.0, 1e-38])
+    f = torch.tensor([1e-9, 1e-7, 1e-20, 1e-40, math.pi / 2, 1.2, 3.0, 1e-300], dtype=torch.float64)
+    for larger in (False, True):
+        k = tiny.repeat(T * 6)[:T * 32].view(T, 2, 16) * torch.tensor([1.0, -1.0])[:, None]
+        k[:, :, 1::3] *= -1
+        if larger:
+            k[T // 2, 1] = torch.linspace(-3, 3, 16)
+        for at in (torch.ones(T, dtype=torch.int64), torch.arange(T) - T // 2):
+            want = _append(tpo, dev, k.to(dtype), f, at, interleaved)
+            assert want.k.isfinite().all()

@@ -10,42 +10,11 @@
 #include <type_traits>
 
 #include "cache.hpp"
+#include "cache_codes.hpp"
 #include "rotary.hpp"
 
 namespace tpo {
 
-constexpr int E_LEAST = -40, E_MOST = 40;
-constexpr float CODE_MOST = 448.f;
-
-// A double as a float whose last bit says that something was cut off (rounding to odd), so that
-// the next rounding, to a code, is that of the double itself.  Keys are turned in 64 bits and
-// rounded once in all: their codes are those of the exact products.
-__device__ __forceinline__ float to_odd(double d) {
-  const float f = (float)d;
-  const double rest = d - (double)f;
-  int b = __builtin_bit_cast(int, f);
-  if (rest != 0. && !(b & 1) && fabsf(f) < __builtin_inff()) b += (rest > 0.) == (f > 0.f) ? 1 : -1;
-  return __builtin_bit_cast(float, b);
-}
-__device__ __forceinline__ bool finite(float v) { return fabsf(v) < __builtin_inff(); }
-
-// The smallest e with top <= 448 2^e (448 = 0.875 2^9).
-__device__ __forceinline__ int exponent_for(float top) {
-  int e;
-  const float m = frexpf(top, &e);
-  e += m > 0.875f ? -8 : -9;
-  if (top == 0.f || e < E_LEAST) e = E_LEAST;
-  return e > E_MOST ? E_MOST : e;
-}
-// The smallest e with scale <= 2^e, for a scale from anywhere.
-__device__ __forceinline__ int exponent_of(float scale) {
-  if (!(scale > 0.f)) return E_LEAST;
-  if (!finite(scale)) return E_MOST;
-  int e;
-  const float m = frexpf(scale, &e);
-  if (m == 0.5f) --e;
-  return e < E_LEAST ? E_LEAST : (e > E_MOST ? E_MOST : e);
-}
 __device__ __forceinline__ float power(int e) { return __builtin_bit_cast(float, (e + 127) << 23); }
 
 __device__ __forceinline__ float for_code(float v, float f) {
