@@ -74,3 +74,10 @@ def test_exponents(host):
         top = float(np.float32(m * 2.0 ** e))
         assert host.exponent(top) == cache64.exponent(top), top
     assert host.exponent(0.0) == -40 and host.exponent(MOST) == 40
+
+
+def test_beyond_the_largest_float(host):
+    """A finite value is never taken for one that is not: the largest float, which is odd."""
+    d = np.array([s * x for x in (MOST * (1 + 2.0 ** -26), MOST * 1.0001, 4.2e38, 2.0 ** 128, 1e300)
+                  for s in (1, -1)])
+    assert (_odd(host, d) == np.sign(d) * MOST).all()

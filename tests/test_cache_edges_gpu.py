@@ -46,3 +46,22 @@ def test_turned_keys_next_to_nothing(tpo, dev, dtype, interleaved, T):
         for at in (torch.ones(T, dtype=torch.int64), torch.arange(T) - T // 2):
             want = _append(tpo, dev, k.to(dtype), f, at, interleaved)
             assert want.k.isfinite().all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("T", [4, 40])
+def test_turned_keys_beyond_the_largest_float(tpo, dev, dtype, interleaved, T):
+    """Finite keys whose turned values no float holds: the largest value that the cache has, and
+    only what is not finite is NaN."""
+    f = torch.tensor([math.pi / 4, 1.0, 3.0, 0.0], dtype=torch.float64)
+    k = torch.full((T, 1, 16), 3e38).to(dtype)
+    k[::2] *= -1
+    k[T // 2], k[T // 2 + 1] = 1.0, 1e30
+    at = torch.arange(T) % 3
+    for amplitude in (1.0, 8.0):
+        want = _append(tpo, dev, k, f, at, interleaved, amplitude)
+        assert want.k.isfinite().all() and (want.ks == 2.0 ** 40).any()
+    k[1, 0, 2], k[3, 0, 5], k[3, 0, 12] = float("inf"), float("nan"), float("-inf")
+    want = _append(tpo, dev, k, f, at, interleaved)
+    assert want.k.isnan().any()
