@@ -4,7 +4,7 @@ import math
 import pytest
 import torch
 
-from tests import cache64
+from tests import cache64, nn64
 
 pytestmark = pytest.mark.gpu
 
@@ -65,3 +65,27 @@ def test_turned_keys_beyond_the_largest_float(tpo, dev, dtype, interleaved, T):
     k[1, 0, 2], k[3, 0, 5], k[3, 0, 12] = float("inf"), float("nan"), float("-inf")
     want = _append(tpo, dev, k, f, at, interleaved)
     assert want.k.isnan().any()
+
+
+# Tables of an odd number of pages that are an odd number of blocks, the last sequence as long as
+# its table: the last two blocks of 32 tokens that go together are not both there.
+# (page, pages of a sequence); tests/test_cache_table_cpu.py looks up which kernel takes them.
+FULL = [(32, 1), (32, 7), (96, 1), (96, 3), (160, 1), (224, 3)]
+FULL_NEW, FULL_HEADS, FULL_D = 16 * [30], 32, 72
+
+
+@pytest.mark.parametrize("page,M", FULL)
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("causal", [True, False])
+def test_prompts_over_full_tables(tpo, dev, page, M, dtype, causal):
+    B, T = len(FULL_NEW), sum(FULL_NEW)
+    lengths = [max(30, page * M - 11 * b) for b in reversed(range(B))]
+    lengths[3] = page * M
+    cache = cache64.paged(tpo, dev, lengths, FULL_HEADS, FULL_D, page, seed=page)
+    assert cache.table.shape == (B, M) and lengths[-1] == page * M
+    g = torch.Generator().manual_seed(M)
+    q = torch.randn(T, 2 * FULL_HEADS, FULL_D, generator=g).to(dtype)
+    o = torch.arange(B + 1) * 30
+    got = tpo.cached_attention(q.to(dev), cache, o.to(dev), causal=causal)
+    want = cache64.Cache(cache).attention(q, o.tolist(), causal=causal)
+    nn64.near(got, want, roundings=2)  # probabilities and the result

@@ -36,7 +36,9 @@ struct Cache {
     const int64_t room = (int64_t)M * page;
     return n < 0 ? 0 : (int)(n > room ? room : n);
   }
-  __device__ __forceinline__ int page_of(int b, int i) const {
+  // the number of page i of sequence b; -1: none
+  __host__ __device__ __forceinline__ int page_of(int b, int i) const {
+    if (i < 0 || i >= M) return -1;
     const int p = table[(int64_t)b * M + i];
     return p >= 0 && p < pages ? p : -1;
   }

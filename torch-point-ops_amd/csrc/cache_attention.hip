@@ -659,9 +659,11 @@ __global__ __launch_bounds__(256, (DP * sizeof(T) <= 256 ? 2 : 1)) void cache_pr
   };
   const int n = keys(r), least = keys(r0), most = r0 < used ? keys(r0 + 31) : 0;
   const int all_see = keys(b0), end = b0 < used ? keys(b0 + 127) : 0, tiles = (end + 63) / 64;
+  // (the last tile's second block may be behind the sequence's pages)
+  const int blocks = (end + CACHE_BLOCK - 1) / CACHE_BLOCK;
   // 64 blocks' pages at a time: of the tiles that are loaded, and of those that are multiplied
   BlockPlaces ahead, now;
-  if (tiles > 0) ahead.load(a.c, p.b, hk, 0, 1, 2 * tiles);
+  if (tiles > 0) ahead.load(a.c, p.b, hk, 0, 1, blocks);
   CodeRows<T, DP, true> x;
   x.load(q + (p.first + r / G) * a.q_row + (hk * G + r % G) * a.q_head, r < used, a.D,
          a.scale < 0.f);
@@ -690,7 +692,7 @@ __global__ __launch_bounds__(256, (DP * sizeof(T) <= 256 ? 2 : 1)) void cache_pr
                             length - 64 * (t + 1), 64 * t + 128 > all_see,
                             rows, x, 64 * t < most, 64 * t, n, 64 * t + 64 > least, f, lv);
     if (t + 2 < tiles) {
-      if (((t + 2) & 31) == 0) ahead.load(a.c, p.b, hk, 2 * (t + 2), 1, 2 * tiles);
+      if (((t + 2) & 31) == 0) ahead.load(a.c, p.b, hk, 2 * (t + 2), 1, blocks);
       load(t + 2);
     }
   };
@@ -702,8 +704,7 @@ __global__ __launch_bounds__(256, (DP * sizeof(T) <= 256 ? 2 : 1)) void cache_pr
   __syncthreads();
   if (r0 >= all) return;
   if (taken_out) {  // rare: the rows that see it get it, see CodeSums
-    const int first = all_see / 64 * 2, last = (end + 31) / CACHE_BLOCK;
-    for (int i = first; i < last; ++i) {
+    for (int i = all_see / 64 * 2; i < blocks; ++i) {
       const int per = a.c.page / CACHE_BLOCK;
       const int page = __builtin_amdgcn_readfirstlane(a.c.page_of(p.b, i / per));
       if (page < 0) continue;
