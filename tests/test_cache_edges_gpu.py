@@ -89,3 +89,73 @@ def test_prompts_over_full_tables(tpo, dev, page, M, dtype, causal):
     got = tpo.cached_attention(q.to(dev), cache, o.to(dev), causal=causal)
     want = cache64.Cache(cache).attention(q, o.tolist(), causal=causal)
     nn64.near(got, want, roundings=2)  # probabilities and the result
+
+
+def _levels(tpo, dev, lengths, Hk, D, page, apart, order, seed):
+    """A cache whose pages are of two kinds: small values in all of a head's channels, and values
+    2^apart times as large in channel 3 and nothing in the others."""
+    cache = cache64.paged(tpo, dev, lengths, Hk, D, page, seed)
+    cache.value_scales.fill_(2.0 ** -19)
+    for row in cache.table.tolist():
+        for i, p in enumerate(row):
+            if p >= 0 and order(i):
+                codes = cache.values.view(torch.uint8)[p]
+                kept = codes[:, :, 3].clone()
+                codes.zero_()
+                codes[:, :, 3] = kept
+                cache.value_scales[p] = 2.0 ** (apart - 19)
+    return cache
+
+
+def _channels(cache, got, q, o, causal=True):
+    """Every value by itself: probabilities are off by a rounding each, and by 2^-24 of their sum,
+    which is 1; then the result is rounded (half's steps end at 2^-24)."""
+    model = cache64.Cache(cache)
+    want = model.attention(q, o, causal=causal)
+    model.v = model.v.abs()
+    sums = model.attention(q, o, causal=causal)
+    G = q.shape[1] // model.Hk
+    most = (model.v * model.vs[..., None, None]).amax((0, 2))[:, :q.shape[2]]
+    most = most.repeat_interleave(G, 0)
+    tol = (2 * nn64.U[q.dtype] + 1e-5) * sums
+    if q.dtype == torch.float16:
+        tol = tol + max(cache.lengths.tolist()) * 2.0 ** -24 * most + 2.0 ** -25
+    got = got.cpu().double()
+    there = want.abs() < 6e4  # (more is infinite in half, and no case of this test)
+    assert there[..., [c for c in range(q.shape[2]) if c != 3]].all()
+    off = ((got - want).abs() / tol.clamp(min=1e-300))[there]
+    assert off.max() <= 1, off.max().item()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("apart", [1, 3, 8, 16, 24, 40, 59, 80])
+def test_small_values_beside_large_ones(tpo, dev, dtype, apart):
+    """A page of large values in one channel leaves the others' small ones their bits, whatever
+    comes first and however many workgroups and waves have the keys."""
+    orders = (lambda i: i == 0, lambda i: i % 2 == 1, lambda i: i % 3 != 1, lambda i: i >= 3)
+    for n, order in enumerate(orders):
+        for lengths, new, page in (([500, 70, 1], [3, 40, 1], 32), ([3000], [2], 64)):
+            cache = _levels(tpo, dev, lengths, 2, 32, page, apart, order, 7 * n)
+            g = torch.Generator().manual_seed(n)
+            q = torch.randn(sum(new), 4, 32, generator=g).to(dtype)
+            o = [0]
+            for c in new:
+                o.append(o[-1] + c)
+            got = tpo.cached_attention(q.to(dev), cache, torch.tensor(o, device=dev))
+            _channels(cache, got, q, o)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("apart", [3, 16, 40, 80])
+@pytest.mark.parametrize("page", [32, 96])
+def test_small_values_beside_large_ones_in_prompts(tpo, dev, dtype, apart, page):
+    """The same by 128 rows, whose blocks of 32 go two at a time: of one page and of two."""
+    B = len(FULL_NEW)
+    for n, order in enumerate((lambda i: i == 0, lambda i: i % 2 == 1, lambda i: i % 3 != 1)):
+        lengths = [30 + 13 * b for b in range(B)]
+        cache = _levels(tpo, dev, lengths, FULL_HEADS, FULL_D, page, apart, order, n)
+        g = torch.Generator().manual_seed(n)
+        q = torch.randn(sum(FULL_NEW), 2 * FULL_HEADS, FULL_D, generator=g).to(dtype)
+        o = (torch.arange(B + 1) * 30).tolist()
+        got = tpo.cached_attention(q.to(dev), cache, torch.tensor(o, device=dev))
+        _channels(cache, got, q, o)

@@ -113,9 +113,14 @@ struct CodeTile {
 
 // Where a wave's next 64 blocks are, a lane each: what follows from a block's number is worked
 // out once for all of them.
+// NARROW: also which blocks are small, see CodeSums::follow: those whose value's scale is less than
+// 2^-HALF_LIFT of the largest so far (and no less than 2^-80, the most that cache_append's differ).
+constexpr float HALF_LIFT = 7.f;
+template <bool NARROW>
 struct BlockPlaces {
   int lo, hi;    // bytes from the first block; hi < 0: the page is not there
-  float ks, lv;  // the key's scale, log2 of the value's
+  float ks, lv;  // the key's scale (small ones': less than 0), log2 of the value's
+  float high = NEG_INF;  // the largest lv so far
   // (scales are positive numbers)
   static __device__ __forceinline__ float inside(float v) {
     return fminf(fmaxf(v, 0x1p-100f), 0x1p100f);
@@ -137,6 +142,13 @@ struct BlockPlaces {
     }
     // (what a page that is not there holds weighs nothing)
     lv = page < 0 ? NEG_INF : __builtin_amdgcn_logf(vs);
+    if constexpr (NARROW) {
+      high = fmaxf(high, wave_max(lv));
+      if (lv < high - HALF_LIFT && lv >= high - 80.f) ks = -ks;
+    }
+  }
+  __device__ __forceinline__ bool small(int i) const {
+    return NARROW && __builtin_amdgcn_readlane(__builtin_bit_cast(int, ks), i & 63) < 0;
   }
   // of block i, the same in all lanes
   __device__ __forceinline__ int64_t place(int i) const {
@@ -150,7 +162,7 @@ struct BlockPlaces {
   // What a score of block i counts in the exponent of 2, count being that of a score of its
   // own; never 0, as a masked score is -inf.
   __device__ __forceinline__ float score(int i, float count) const {
-    return fmaxf(count * lane(ks, i), 1e-37f);
+    return fmaxf(count * fabsf(lane(ks, i)), 1e-37f);
   }
   __device__ __forceinline__ float value_log(int i) const { return lane(lv, i); }
 };
@@ -160,6 +172,10 @@ template <typename T, int DP>
 struct CodeSums {
   typedef typename CodeType<T>::E E;
   static constexpr int PARTS = CodeType<T>::PARTS;
+  static constexpr bool NARROW = std::is_same_v<E, half_t>;
+  // Weights are 2^(s + lv - m), m being LIFT under the maximum and up to 8 more.  In half they go
+  // up to 2^15 and end at 2^-25, which is 2^-32 of the maximum's; the other type has float's range.
+  static constexpr float LIFT = NARROW ? HALF_LIFT : 0.f;
   f32x16 acc[DP / 32];
   float m, l;  // l: of the lane's own keys, half of the row's
 
@@ -171,9 +187,9 @@ struct CodeSums {
   }
   // The keys j0 .. j0 + 31, of which the lane's row sees those below n (masked: not all rows
   // see all), the sequence has those below length; f: what a score counts in the exponent of
-  // 2, with the keys' scale.
+  // 2, with the keys' scale; small: see follow.
   __device__ __forceinline__ void add(CodeTile<DP>& t, const CodeRows<T, DP>& q, int j0, int n,
-                                      bool masked, int length, float f, float lv) {
+                                      bool masked, int length, float f, float lv, bool small) {
     f32x16 s = {};
 #pragma unroll
     for (int i = 0; i < DP / 32; ++i)
@@ -195,7 +211,8 @@ struct CodeSums {
 #pragma unroll
     for (int e = 1; e < 16; ++e) top = fmaxf(top, s[e]);
     top = __builtin_fmaf(top, f, lv);
-    follow(fmaxf(top, other_half(top)));
+    top = fmaxf(top, other_half(top));
+    follow(top, lv, small);
     weigh(s, f, lv);
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
@@ -209,10 +226,23 @@ struct CodeSums {
       }
     }
   }
-  // The maximum follows where it grows by more than 2^8.
-  __device__ __forceinline__ void follow(float top) {
-    if (__builtin_amdgcn_ballot_w64(top - m > 8.f)) {
-      const float m2 = fmaxf(m, top);
+  // The maximum follows where it grows by more than 2^8.  And in half it goes down where it has
+  // to: the row's largest product of probability and value scale has set m, so that a page of
+  // small values could have most of the probability and weights of nothing.  Where the weights'
+  // last step, 2^(-25 - lv) in probability, is more than 2^-25 of the row's sum, m is set by the
+  // tile's largest weight, unless no key of the tile has 2^-24 of the sum.  So a key's weight is
+  // rounded by 2^-11 of itself and 2^-24 of the row's sum, whatever the scales; acc stays under
+  // 2^120 by that.  (8 sequences of up to 8192 tokens, 1024 new, 16 heads on 4, D = 128 in float16:
+  // 392 us, without it and LIFT 383; each is half of that.)
+  // small: whether it may be so.  The key that set m is 2^LIFT in the sum over its scale, so the
+  // scales have to be more than 2^LIFT apart, which those of values at common levels are not.
+  __device__ __forceinline__ void follow(float top, float lv, bool small) {
+    if (__builtin_amdgcn_ballot_w64(top - m > 8.f + LIFT) || small) {
+      float m2 = fmaxf(m, top - LIFT);
+      if (small) {
+        const float own = __builtin_amdgcn_exp2f(-lv), row = l + other_half(l);
+        if (own > row && __builtin_amdgcn_exp2f(top - m) * own > row * 0x1p-24f) m2 = top - LIFT;
+      }
       const float a = m2 == NEG_INF ? 1.f : __builtin_amdgcn_exp2f(m - m2);
       m = m2;
       l *= a;
@@ -367,7 +397,7 @@ cache_step_kernel(CacheAttnArgs a, const T* __restrict__ q, T* __restrict__ out,
   CodeRows<T, DP> x;
   const int mine = t0 < t1 ? (t1 - t0 + W - 1) / W : 0;  // the wave's tiles
   // the places of 64 of them at a time: of those that are loaded, and of those multiplied
-  BlockPlaces ahead, now;
+  BlockPlaces<CodeSums<T, DP>::NARROW> ahead, now;
   if (mine > 0) ahead.load(a.c, p.b, hk, t0, W, t1);
   x.load(q + (p.first + r / G) * a.q_row + (hk * G + r % G) * a.q_head, r < used, a.D,
          a.scale < 0.f);
@@ -386,8 +416,8 @@ cache_step_kernel(CacheAttnArgs a, const T* __restrict__ q, T* __restrict__ out,
       if (at >= mine) break;
       if ((at & 63) == 0) now = ahead;
       load(tile[(y + N - 1) % N], at + N - 1);
-      rows.add(tile[y], x, j0, n, j0 + 32 > least, length, now.score(at, c),
-               now.value_log(at));
+      rows.add(tile[y], x, j0, n, j0 + 32 > least, length, now.score(at, c), now.value_log(at),
+               now.small(at));
     }
   }
 
@@ -533,9 +563,10 @@ struct CodePrompt {
   }
   // Weights of the keys j0 .. j0 + 63 at lds, of which the lane's row sees those below n.  f, lv:
   // of the two blocks, see CodeSums.
+  // small: see CodeSums::follow.
   __device__ __forceinline__ void weigh(f32x16 (&s)[2], const char* lds,
                                         const CodeRows<T, DP, true>& q, int j0, int n, bool masked,
-                                        const float (&f)[2], const float (&lv)[2]) {
+                                        const float (&f)[2], const float (&lv)[2], bool small) {
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
       s[t] = f32x16{};
@@ -563,7 +594,7 @@ struct CodePrompt {
       for (int e = 1; e < 16; ++e) y = fmaxf(y, s[t][e]);
       top = fmaxf(top, __builtin_fmaf(y, f[t], lv[t]));
     }
-    sums.follow(fmaxf(top, other_half(top)));
+    sums.follow(fmaxf(top, other_half(top)), fmaxf(lv[0], lv[1]), small);
 #pragma unroll
     for (int t = 0; t < 2; ++t) sums.weigh(s[t], f[t], lv[t]);
   }
@@ -629,12 +660,18 @@ __device__ __forceinline__ bool code_step(const char* __restrict__ cur, char* __
                                           CodeLoads<T, DP>& raw, bool more, int left,
                                           bool next_masked, CodePrompt<T, DP>& rows,
                                           const CodeRows<T, DP, true>& q, bool any, int j0, int n,
-                                          bool masked, const float (&f)[2],
-                                          const float (&lv)[2]) {
+                                          bool masked, const float (&f)[2], const float (&lv)[2],
+                                          bool small) {
   const bool bad = more && raw.put(nxt, left, next_masked);
   if (any) {
     f32x16 s[2];
-    rows.weigh(s, cur, q, j0, n, masked, f, lv);
+    if (__builtin_expect(small, 0)) {  // a block at a time, as if the other's page were not there
+      const float one[2] = {lv[0], NEG_INF};
+      rows.weigh(s, cur, q, j0, n, masked, f, one, true);
+      rows.gather(s, cur);
+    }
+    const float rest[2] = {small ? NEG_INF : lv[0], lv[1]};
+    rows.weigh(s, cur, q, j0, n, masked, f, rest, small);
     rows.gather(s, cur);
   }
   return bad;
@@ -662,7 +699,7 @@ __global__ __launch_bounds__(256, (DP * sizeof(T) <= 256 ? 2 : 1)) void cache_pr
   // (the last tile's second block may be behind the sequence's pages)
   const int blocks = (end + CACHE_BLOCK - 1) / CACHE_BLOCK;
   // 64 blocks' pages at a time: of the tiles that are loaded, and of those that are multiplied
-  BlockPlaces ahead, now;
+  BlockPlaces<CodeSums<T, DP>::NARROW> ahead, now;
   if (tiles > 0) ahead.load(a.c, p.b, hk, 0, 1, blocks);
   CodeRows<T, DP, true> x;
   x.load(q + (p.first + r / G) * a.q_row + (hk * G + r % G) * a.q_head, r < used, a.D,
@@ -688,9 +725,10 @@ __global__ __launch_bounds__(256, (DP * sizeof(T) <= 256 ? 2 : 1)) void cache_pr
       f[y] = now.score(2 * t + y, c);
       lv[y] = now.value_log(2 * t + y);
     }
+    const bool small = now.small(2 * t) || now.small(2 * t + 1);
     bad |= code_step<T, DP>(lds.b + H * L::TILE, lds.b + (1 - H) * L::TILE, raw, t + 1 < tiles,
-                            length - 64 * (t + 1), 64 * t + 128 > all_see,
-                            rows, x, 64 * t < most, 64 * t, n, 64 * t + 64 > least, f, lv);
+                            length - 64 * (t + 1), 64 * t + 128 > all_see, rows, x, 64 * t < most,
+                            64 * t, n, 64 * t + 64 > least, f, lv, small);
     if (t + 2 < tiles) {
       if (((t + 2) & 31) == 0) ahead.load(a.c, p.b, hk, 2 * (t + 2), 1, blocks);
       load(t + 2);

@@ -63,7 +63,9 @@ def cached_attention(q, cache, offsets, lengths_q=None, causal=True, scale=None)
 
     Returns (T, Hq, D) of q's type; rows that are not in use or see no key are 0.  Scores, their
     statistics and all sums are float32; half and bfloat16 probabilities are rounded to the type
-    for the product.  Under torch.autocast q is taken in its type.  Without a derivative.
+    for the product, half ones by 2^-11 of themselves and 2^-24 of their sum, however far apart
+    the scales of pages that cache_append wrote.  Under torch.autocast q is taken in its type.
+    Without a derivative.
     """
     if scale is None:
         scale = q.shape[-1] ** -0.5
