@@ -14,15 +14,12 @@ constexpr float CODE_MOST = 448.f;
 // rounded once in all: their codes are those of the exact products.  Which way the float went off
 // is seen from d: the float of a small one is 0, and the least float of d's sign is then the odd
 // one.  What is finite but beyond the floats becomes the largest of them (an infinity's bits less
-// 1), which is odd: infinities are those of the inputs.
+// 1), which is odd; of an infinity nothing is cut off (the rest is NaN).
 __host__ __device__ __forceinline__ float to_odd(double d) {
   const float f = (float)d;
   const double rest = d - (double)f;
   int b = __builtin_bit_cast(int, f);
-  if (fabsf(f) == __builtin_inff())
-    b -= fabs(d) < __builtin_inf() ? 1 : 0;
-  else if (rest != 0. && !(b & 1))
-    b += (rest > 0.) == (d > 0.) ? 1 : -1;
+  if (fabs(rest) > 0. && !(b & 1)) b += (rest > 0.) == (d > 0.) ? 1 : -1;
   return __builtin_bit_cast(float, b);
 }
 __host__ __device__ __forceinline__ bool finite(float v) { return fabsf(v) < __builtin_inff(); }
