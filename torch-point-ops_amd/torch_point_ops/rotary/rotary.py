@@ -16,8 +16,10 @@ class RotaryPositions(torch.nn.Module):
         super().__init__()
         if size < 0 or size % 2 != 0:
             raise ValueError(f"size must be even and not negative, but got {size}")
+        self._made = None  # what makes the frequencies; those that were given are all there is
         if frequencies is None:
-            frequencies = rotary_frequencies(size // 2, base, stretch, trained, device)
+            self._made = (size // 2, base, stretch, trained)
+            frequencies = rotary_frequencies(*self._made, device)
         elif tuple(frequencies.shape) != (size // 2,):
             raise ValueError(f"frequencies must have shape ({size // 2},), but got "
                              f"{tuple(frequencies.shape)}")
@@ -32,7 +34,11 @@ class RotaryPositions(torch.nn.Module):
     def _apply(self, fn, recurse=True):
         # to(device) moves them, to(dtype) leaves them in 64 bits
         super()._apply(fn, recurse)
-        self._double = self._double.to(fn(torch.empty(0, device=self._double.device)).device)
+        device = fn(torch.empty(0, device=self._double.device)).device
+        if self._double.is_meta and device.type != "meta" and self._made is not None:
+            self._double = rotary_frequencies(*self._made, device)  # (to_empty)
+        else:
+            self._double = self._double.to(device)
         return self
 
     def forward(self, x, positions):
