@@ -111,9 +111,10 @@ struct PartValues {
   }
 };
 
-// Eight pairs turned, x[e] and x[8 + e] being pair e; angle(e): its cosine and sine.  ODD: rounded to odd; else to the nearest
-// float, which has the same code but where it lies half-way between two of them, its last 19
-// bits 0 (e4m3 keeps 3 of 23): true where one may.
+// Eight pairs turned, x[e] and x[8 + e] being pair e; angle(e): its cosine and sine.  ODD: rounded
+// to odd; else to the nearest float, which has the same code but where it lies half-way between
+// two of them, or is 0 or infinite: its last 19 bits are 0 then (e4m3 keeps 3 of 23): true where
+// one may.
 template <bool ODD, typename T, typename F>
 __device__ __forceinline__ bool turn_pairs(const PartValues<T>& u, bool interleaved,
                                            const F& angle, float (&x)[16]) {
@@ -774,7 +775,8 @@ extern "C" int tpo_cache_append(int dtype, const void* k, const void* v, const v
   const int64_t slots = T / page + 2 * (B + 2);
   // few tokens a sequence: a wave a head, where pages are many (64 sequences, 8 heads of 128 in
   // bfloat16, a new token each 9.3 us, by whole workgroups 18.4; 8 new 10.3, 17.6; 16 new 25.3,
-  // 18.1; 8 sequences: 9 and 8; 16 new 19.9, 8.5)
+  // 18.1; 8 sequences: 9 and 8; 16 new 19.9, 8.5).  The rule knows the average only: 63 sequences
+  // of one token and one of 400 take 66 us, in calls of their own 10 and 9.
   const bool few = T <= 8 * B;
   // else 512 workgroups (5 x 300 tokens, 6 heads of 80, float16: by 52 workgroups 32 us, 156 14,
   // 312 10; 8 x 4096, 4 heads of 128: 343 32, 686 31.5, 1372 38)

@@ -459,7 +459,8 @@ cache_step_kernel(CacheAttnArgs a, const T* __restrict__ q, T* __restrict__ out,
 // tiles of 64, which its waves load (a quarter each, two tiles ahead), turn into the products'
 // type and put into LDS for all four: a code is converted once for 128 rows, where the kernel
 // above does it for 32 (8 sequences of up to 8192, 1024 new tokens, 16 heads on 4, D = 128 in
-// bfloat16: 386 us, the kernel above 425).  Keys lie in LDS in the order of the product's rows in
+// bfloat16: 386 us by itself, the kernel above 425; among other calls 359 to 388, as the clock
+// goes).  Keys lie in LDS in the order of the product's rows in
 // which a lane receives the scores of sixteen tokens in a row; values by value, 64 tokens each, so
 // that sixteen bytes are what a product sums over.  Chunks of 16 bytes change places with the row,
 // as in HeadLds, so that a read touches all banks.
@@ -779,6 +780,11 @@ __global__ __launch_bounds__(256, (DP * sizeof(T) <= 256 ? 2 : 1)) void cache_pr
 // or more (3 x 1500 tokens, 8 heads of 96, 200 new, float16: 15.6 us, by four waves 16.4; 7
 // sequences, 6 heads of 40, 5 new, float, with the join: 4096 tokens 15.4, 15.8; 2048 12.4, 12.1;
 // 1 x 300, 8 heads of 64: 8.0, 7.5).
+// All this goes by the average of a call's rows and by the table's room, as the lengths are on the
+// GPU.  What it costs where they mislead: 63 single tokens over 16384 and a piece of 1024 rows,
+// groups of 4 in bfloat16: 189 us on 4 heads (apart 120 and 43), 435 on 8 (232 and 32); 1 x 300 as
+// above with room for 320 tokens 8.1, 4096 11.6, 32768 12.8; 16 x 1000, 8 heads of 64 in float16,
+// in a pool of 131 MB 10.7, of 2.6 GB 11.3.
 struct CacheWay {
   bool prompt, stream;
   int shares, waves;

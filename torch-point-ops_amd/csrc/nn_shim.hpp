@@ -30,15 +30,23 @@ typedef std::optional<Tensor> OptTensor;
   TORCH_CHECK(bytes >= 0, op, ": ", tpo_last_error());
   return bytes > 0 ? at::empty({bytes}, like.options().dtype(at::kByte)) : Tensor();
 }
-[[maybe_unused]] void* data_or_null(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+[[maybe_unused]] void* data_or_null(const Tensor& t) {
+  return t.defined() ? t.data_ptr() : nullptr;
+}
 [[maybe_unused]] Tensor get(const OptTensor& t) { return t.has_value() ? *t : Tensor(); }
-[[maybe_unused]] OptTensor opt(const Tensor& t) { return t.defined() ? OptTensor(t) : std::nullopt; }
+[[maybe_unused]] OptTensor opt(const Tensor& t) {
+  return t.defined() ? OptTensor(t) : std::nullopt;
+}
 // the place of a result that was not asked for
 [[maybe_unused]] Tensor nothing(const Tensor& like) { return at::empty({0}, like.options()); }
 
 // The distance of rows and of heads, also where there is one of them only.
-[[maybe_unused]] int64_t row_stride(const Tensor& t) { return t.size(0) > 1 ? t.stride(0) : t.size(1) * t.size(2); }
-[[maybe_unused]] int64_t head_stride(const Tensor& t) { return t.size(1) > 1 ? t.stride(1) : t.size(2); }
+[[maybe_unused]] int64_t row_stride(const Tensor& t) {
+  return t.size(0) > 1 ? t.stride(0) : t.size(1) * t.size(2);
+}
+[[maybe_unused]] int64_t head_stride(const Tensor& t) {
+  return t.size(1) > 1 ? t.stride(1) : t.size(2);
+}
 
 // q, k and v may be slices (of one projection, say) or broadcast over heads: a
 // head's values lie together, rows and heads at any distance that keeps 16-byte
@@ -46,8 +54,9 @@ typedef std::optional<Tensor> OptTensor;
 [[maybe_unused]] Tensor head_rows(const Tensor& t, int64_t D) {
   const int64_t z = t.element_size();
   if (t.size(2) != D) return at::constant_pad_nd(t, {0, D - t.size(2)}).contiguous();
-  const bool ok = (D == 1 || t.stride(2) == 1) && row_stride(t) > 0 && row_stride(t) * z % 16 == 0 &&
-                  row_stride(t) * z < (1 << 25) && head_stride(t) * z % 16 == 0;
+  const bool ok = (D == 1 || t.stride(2) == 1) && row_stride(t) > 0 &&
+                  row_stride(t) * z % 16 == 0 && row_stride(t) * z < (1 << 25) &&
+                  head_stride(t) * z % 16 == 0;
   return aligned16(ok ? t : t.contiguous());
 }
 
@@ -62,7 +71,9 @@ typedef std::optional<Tensor> OptTensor;
 }
 // The operators that autograd functions call have no formula of their own: a
 // gradient of a gradient, or a tangent, is refused instead of left out.
-[[maybe_unused]] torch::CppFunction no_formula() { return torch::autograd::autogradNotImplementedFallback(); }
+[[maybe_unused]] torch::CppFunction no_formula() {
+  return torch::autograd::autogradNotImplementedFallback();
+}
 
 }  // namespace
 }  // namespace torch_point_ops
