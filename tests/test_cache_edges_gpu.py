@@ -109,7 +109,11 @@ def _levels(tpo, dev, lengths, Hk, D, page, apart, order, seed):
 
 def _channels(cache, got, q, o, causal=True):
     """Every value by itself: probabilities are off by a rounding each, and by 2^-24 of their sum,
-    which is 1; then the result is rounded (half's steps end at 2^-24)."""
+    which is 1; then the result is rounded (half's steps end at 2^-24).  Floats end at 2^-126, and
+    bfloat16 with them: a result under that is 0, and so is a weight, the probability times the
+    page's scale against the row's largest such product.  With scales at most 2^80 apart that
+    probability is under 2^-126 2^80, so that a key's part of the result is off by 2^-46 of its
+    value at most."""
     model = cache64.Cache(cache)
     want = model.attention(q, o, causal=causal)
     model.v = model.v.abs()
@@ -117,13 +121,14 @@ def _channels(cache, got, q, o, causal=True):
     G = q.shape[1] // model.Hk
     most = (model.v * model.vs[..., None, None]).amax((0, 2))[:, :q.shape[2]]
     most = most.repeat_interleave(G, 0)
-    tol = (2 * nn64.U[q.dtype] + 1e-5) * sums
+    n = max(cache.lengths.tolist())
+    tol = (2 * nn64.U[q.dtype] + 1e-5) * sums + n * 2.0 ** -46 * most + 2.0 ** -126
     if q.dtype == torch.float16:
-        tol = tol + max(cache.lengths.tolist()) * 2.0 ** -24 * most + 2.0 ** -25
+        tol = tol + n * 2.0 ** -24 * most + 2.0 ** -25
     got = got.cpu().double()
     there = want.abs() < 6e4  # (more is infinite in half, and no case of this test)
     assert there[..., [c for c in range(q.shape[2]) if c != 3]].all()
-    off = ((got - want).abs() / tol.clamp(min=1e-300))[there]
+    off = ((got - want).abs() / tol)[there]
     assert off.max() <= 1, off.max().item()
 
 
@@ -159,3 +164,20 @@ def test_small_values_beside_large_ones_in_prompts(tpo, dev, dtype, apart, page)
         o = (torch.arange(B + 1) * 30).tolist()
         got = tpo.cached_attention(q.to(dev), cache, torch.tensor(o, device=dev))
         _channels(cache, got, q, o)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("gone", [0, 1, 2])
+def test_small_values_beside_a_page_that_is_not_there(tpo, dev, dtype, gone):
+    """A block of small values next to one whose page is not there, with scores beyond half's
+    range: what is not there weighs nothing, also before a row has seen a key."""
+    B = len(FULL_NEW)
+    lengths = [100 + 13 * b for b in range(B)]
+    cache = _levels(tpo, dev, lengths, FULL_HEADS, FULL_D, 32, 20, lambda i: i >= 2, gone)
+    cache.table[:, gone] = -1
+    g = torch.Generator().manual_seed(gone)
+    q = (4 * torch.randn(sum(FULL_NEW), 2 * FULL_HEADS, FULL_D, generator=g)).to(dtype)
+    o = (torch.arange(B + 1) * 30).tolist()
+    got = tpo.cached_attention(q.to(dev), cache, torch.tensor(o, device=dev))
+    assert got.isfinite()[..., [c for c in range(FULL_D) if c != 3]].all()
+    _channels(cache, got, q, o)

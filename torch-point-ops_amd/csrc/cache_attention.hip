@@ -254,7 +254,8 @@ struct CodeSums {
   }
   // Scores to weights, and their part of the row's sum.
   __device__ __forceinline__ void weigh(f32x16& s, float f, float lv) {
-    const float b = m == NEG_INF ? 0.f : lv - m;
+    // (a row that has seen nothing: its scores are -inf, or of a page that is not there)
+    const float b = m == NEG_INF ? NEG_INF : lv - m;
     float sum = 0.f;
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
