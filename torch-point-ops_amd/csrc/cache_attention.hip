@@ -114,7 +114,8 @@ struct CodeTile {
 // Where a wave's next 64 blocks are, a lane each: what follows from a block's number is worked
 // out once for all of them.
 // NARROW: also which blocks are small, see CodeSums::follow: those whose value's scale is less than
-// 2^-HALF_LIFT of the largest so far (and no less than 2^-80, the most that cache_append's differ).
+// 2^-HALF_LIFT of the largest so far (and no less than 2^-80, the most that cache_append's differ,
+// nor than 2^-80 itself, where sums over them would leave float's range).
 constexpr float HALF_LIFT = 7.f;
 template <bool NARROW>
 struct BlockPlaces {
@@ -144,7 +145,7 @@ struct BlockPlaces {
     lv = page < 0 ? NEG_INF : __builtin_amdgcn_logf(vs);
     if constexpr (NARROW) {
       high = fmaxf(high, wave_max(lv));
-      if (lv < high - HALF_LIFT && lv >= high - 80.f) ks = -ks;
+      if (lv < high - HALF_LIFT && lv >= fmaxf(high - 80.f, -80.f)) ks = -ks;
     }
   }
   __device__ __forceinline__ bool small(int i) const {

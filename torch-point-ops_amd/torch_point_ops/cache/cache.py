@@ -16,6 +16,8 @@ class PagedCache:
     Hk) float32: a value is its code times the scale of its page and head.  table (B, M) int32:
     the pages of each sequence in order, -1 where there is none.  lengths (B) int64: the tokens of
     each sequence, to which a program adds the new ones before cache_append and cached_attention.
+    More than the M pages of a sequence hold counts as what they hold: tokens appended beyond
+    would take the places of its last ones, so a program ends a sequence before that.
 
     All are plain tensors that the program owns: it hands out pages by writing to `table`, and
     frees a sequence by setting its length to 0 and its entries to -1.
